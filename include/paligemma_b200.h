@@ -507,6 +507,50 @@ int pg_attn_decode(const void* q, const void* k_pages, const void* v_pages, cons
                    int entries, int nsplit, int H, int G, int dim, int vdim, float scale, float softcap, int act_f32, long long krow,
                    long long vrow, int gate_per_head, const PgAttnScore* score, void* stream);
 
+/* pg_attn_prepare whose k and v rows are stored at cache row at[t] of the entry (NULL: pos[t]) while pos[t] still turns them: drafted tokens of one
+ * depth share a position and lie one behind another. */
+int pg_attn_prepare_at(const void* qkv, long long ld, const int* pos, const int* at, const int* row_entry, const int* page_table, int max_pages,
+                       int page, const double* freq, const float* q_norm, const float* k_norm, void* q_out, void* k_pages,
+                       void* v_pages, int rows, int H, int G, int dim, int vdim, int rot_dims, float eps, int norm_qk, int norm_v, int v_from_k,
+                       float rot_gain, const void* v_other, long long ld_v_other, float v_mix, int act_f32, void* stream);
+
+/* The 8-bit cache.  A row's elements are e4m3 codes (uint8 [pages, page, G * size]); every head of a row has one power of two, 2^(byte - 127)
+ * (uint8 [pages, G, page]): the least that takes the head's largest finite element to 448 or below (bytes 0 .. 247).  element = code * power, rounded to the
+ * nearest code, ties to even; infinities and NaN are stored as the NaN code.
+ * pg_attn_prepare_e4m3: pg_attn_prepare_at into such pages.  dim and vdim multiples of 16 up to 256; codes and q_out on 16-byte boundaries.
+ * pg_kv_read_e4m3: rows 0 .. ctx + n of every entry with entry_n > 1, in fp32 (out_f32) or bf16, to rows dense_row0[e] .. of k_out [.., G * dim] and
+ * v_out [.., G * vdim]; zeros behind the last row up to a multiple of 64 rows.  longest: at least the largest ctx + n among them (sizes the grid). */
+int pg_attn_prepare_e4m3(const void* qkv, long long ld, const int* pos, const int* at, const int* row_entry, const int* page_table, int max_pages, int page,
+                         const double* freq, const float* q_norm, const float* k_norm, void* q_out, void* k_codes, void* k_powers, void* v_codes,
+                         void* v_powers, int rows, int H, int G, int dim, int vdim, int rot_dims, float eps, int norm_qk, int norm_v, int v_from_k,
+                         float rot_gain, const void* v_other, long long ld_v_other, float v_mix, int act_f32, void* stream);
+int pg_kv_read_e4m3(const void* k_codes, const void* k_powers, const void* v_codes, const void* v_powers, const int* page_table, int max_pages, int page,
+                    const int* dense_row0, const int* entry_n, const int* entry_ctx, void* k_out, void* v_out, int entries, int longest, int G, int dim,
+                    int vdim, int out_f32, void* stream);
+
+/* A layer's pages: of the activations' type (f32 tells which; k_powers and v_powers unused) or 8-bit (e4m3 != 0). */
+typedef struct PgKvPages {
+  const void* k;
+  const void* v;
+  const void* k_powers;
+  const void* v_powers;
+  int e4m3;
+  int f32;
+} PgKvPages;
+
+/* Attention of a few rows an entry: every row of an entry sees the stored keys 0 .. ctx - 1 and, of the entry's own n rows (cache rows ctx ..), those whose bit
+ * is set in its mask: tree uint32 [rows, tree_words], bit m % 32 of word m / 32 (bits from n on are ignored; NULL: rows up to itself).  A row that sees nothing gets
+ * zeros (with a sink as well).  Score, gate and out as pg_attn_decode; windows and distances go by pos [rows] (required for them, at least ctx each).
+ * singles != 0: entries with one row only, others are left alone.  nsplit > 1: that many CTAs share an entry's keys through `partial`
+ * (pg_attn_rows_scratch bytes for `entries` rows with singles, all rows else), joined by a second launch.
+ * dim up to 128 in whole 16-byte pieces, vdim a multiple of 8 up to 128, page a multiple of 32, pages on 16-byte boundaries; anything else PG_ERR_ARG.
+ * max_n: the largest entry_n (rows past it are left out). */
+long long pg_attn_rows_scratch(int rows, int H, int vdim, int nsplit);
+int pg_attn_rows(const void* q, const PgKvPages* kv, const void* gate, long long ldg, void* out, float* partial, const int* entry_row0, const int* entry_n,
+                 const int* entry_ctx, const int* page_table, int max_pages, int page, const int* pos, const void* tree, int tree_words, int entries,
+                 int max_n, int singles, int nsplit, int H, int G, int dim, int vdim, float scale, float softcap, int act_f32, int gate_per_head,
+                 const PgAttnScore* score, void* stream);
+
 /* The merge launch of pg_attn_decode on its own: rows of single-token entries from `partial` (fp32 [entries, H, nsplit, vdim + 2]:
  * running max in natural-log units, sum, unnormalised accumulator), times the gate, to out [rows, H * vdim]. */
 int pg_attn_decode_merge(const float* partial, const void* gate, long long ldg, void* out, const int* entry_row0, const int* entry_n,
@@ -735,6 +779,12 @@ int pg_moe_combine(const float* expert_out, long long ldy, const int* pair_row, 
                    const float* shared_gate, long long ldsg, int accumulate, void* stream);
 int pg_moe_combine_norm_add(const float* expert_out, long long ldy, const int* pair_row, const float* weights, const float* norm_w, float* x,
                             void* out_act, int tokens, int D, int top, float eps, int act_f32, void* stream);
+
+/* One pass over fp32 logits rows: with z = logits / temperature, the log probability of tokens[row] under softmax(z), its rank (0: the largest; ties: the
+ * lower index is in front), the entropy in nats, and the `top` largest entries in order (ids, log probabilities), top 0 .. 32, at most V.  A token outside
+ * 0 .. V - 1: NaN and rank -1.  Masked entries are -inf; a row with a NaN, a +inf or nothing but -inf has NaN for every number (its ids: NaN behind -inf). */
+int pg_token_logprobs(const float* logits, long long ld, const int* tokens, float* logprob, float* entropy, int* rank, int* top_ids, float* top_logprob,
+                      int rows, int V, int top, float temperature, void* stream);
 
 #ifdef __cplusplus
 }

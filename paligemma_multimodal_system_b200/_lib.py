@@ -13,7 +13,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("PG_LIB_PATH") or os.path.join(_HERE, "libpaligemma_b200.so")  # PG_LIB_PATH: A/B builds (profiling)
 
 EPI_BF16, EPI_F32, EPI_ATOMIC_F32, EPI_GEGLU = 0, 1, 2, 3
-ABI_VERSION = 7  # pg_abi_version() of the library these signatures describe
+ABI_VERSION = 8  # pg_abi_version() of the library these signatures describe
 
 _ERRORS = {-1: "PG_ERR_ARG", -2: "PG_ERR_CUDA", -3: "PG_ERR_DRIVER", -4: "PG_ERR_TMAP", -5: "PG_ERR_ARCH"}
 
@@ -86,6 +86,12 @@ SIGNATURES = {
     "pg_token_side": [p, p, p, p, i64, i32, p, p, p, p, i32, i32, i32, i32, f32, i32, p],
     "pg_side_gate": [p, i64, p, p, i64, i32, p, i64, i32, i32, i32, i32, p],
     "pg_attn_prepare": [p, i64, p, p, p, i32, i32, p, p, p, p, p, p, i32, i32, i32, i32, i32, i32, f32, i32, i32, i32, f32, p, i64, f32, i32, p],
+    "pg_attn_prepare_at": [p, i64, p, p, p, p, i32, i32, p, p, p, p, p, p, i32, i32, i32, i32, i32, i32, f32, i32, i32, i32, f32, p, i64, f32, i32, p],
+    "pg_attn_prepare_e4m3": [p, i64, p, p, p, p, i32, i32, p, p, p, p, p, p, p, p, i32, i32, i32, i32, i32, i32, f32, i32, i32, i32, f32, p, i64, f32, i32, p],
+    "pg_kv_read_e4m3": [p, p, p, p, p, i32, i32, p, p, p, p, p, i32, i32, i32, i32, i32, i32, p],
+    "pg_attn_rows_scratch": [i32, i32, i32, i32],
+    "pg_attn_rows": [p, p, p, i64, p, p, p, p, p, p, i32, i32, p, p, i32, i32, i32, i32, i32, i32, i32, i32, i32, f32, f32, i32, i32, p, p],
+    "pg_token_logprobs": [p, i64, p, p, p, p, p, p, i32, i32, i32, f32, p],
     "pg_attn_ragged": [p, p, p, p, i64, p, p, p, p, p, i32, i32, i32, i32, i32, i32, i32, i32, f32, f32, i32, i32, i64, i64, i32, p, p],
     "pg_attn_ragged_mma": [p, p, p, p, i64, p, p, p, p, p, i32, i32, i32, i32, i32, i32, i32, i32, f32, f32, i32, i32, p, p],
     "pg_attn_ragged_mma_sized": [p, p, p, p, i64, p, p, p, p, p, i32, i32, i32, i32, i32, i32, i32, i32, f32, f32, i32, i32, i32, i32, p, p],
@@ -130,7 +136,7 @@ SIGNATURES = {
     "pg_gated_layernorm_add": [p, i64, p, i64, p, p, p, p, p, p, p, i32, i32, f32, i32, i32, p],
     "pg_glu": [p, i64, p, i64, i32, i32, i32, f32, f32, i32, p],
 }
-_RESTYPE = {"pg_launch_count": i64, "pg_gemm_fp32_scratch": i64, "pg_gemm_fp32_scratch_add": i64, "pg_routed_ff_scratch": i64}
+_RESTYPE = {"pg_launch_count": i64, "pg_gemm_fp32_scratch": i64, "pg_gemm_fp32_scratch_add": i64, "pg_routed_ff_scratch": i64, "pg_attn_rows_scratch": i64}
 
 
 
@@ -138,6 +144,11 @@ class AttnScore(C.Structure):
     """Mirror of PgAttnScore (include/paligemma_b200.h): the optional parts of an attention's score and mask."""
     _fields_ = [("window", i32), ("keep_first", i32), ("sink", p), ("dist_a", p), ("dist_b", p), ("head_scale", p), ("logistic", i32),
                 ("head_bias", p), ("out_scale", f32), ("out_ld", i64)]
+
+
+class KvPages(C.Structure):
+    """Mirror of PgKvPages."""
+    _fields_ = [("k", p), ("v", p), ("k_powers", p), ("v_powers", p), ("e4m3", i32), ("f32", i32)]
 
 
 class RoutedFf(C.Structure):

@@ -63,7 +63,7 @@ __device__ __forceinline__ float sigmoidf(float z) { return 1.0f / (1.0f + expf(
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename TA>
 __global__ void __launch_bounds__(128) attn_prepare_kernel(const TA* __restrict__ qkv, long long ld, const int* __restrict__ pos,
-                                                           const int* __restrict__ row_entry, const int* __restrict__ page_table, int max_pages,
+                                                           const int* __restrict__ at, const int* __restrict__ row_entry, const int* __restrict__ page_table, int max_pages,
                                                            int page, const double* __restrict__ freq, const float* __restrict__ qn,
                                                            const float* __restrict__ kn, TA* __restrict__ q_out, TA* __restrict__ k_pages,
                                                            TA* __restrict__ v_pages, int H, int G, int dim, int vdim, int rot, float eps,
@@ -81,7 +81,8 @@ __global__ void __launch_bounds__(128) attn_prepare_kernel(const TA* __restrict_
   }
   __syncthreads();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  const long long pg_row = (long long)page_table[(long long)row_entry[t] * max_pages + p / page] * page + p % page;
+  const int stored = at[t];
+  const long long pg_row = (long long)page_table[(long long)row_entry[t] * max_pages + stored / page] * page + stored % page;
   const TA* row = qkv + t * ld;
   const int nvec = k_pages != nullptr ? H + 2 * G : H;  // a layer that borrows another layer's keys / values prepares its queries only
   float inv_q = 1.0f, inv_k = 1.0f;
@@ -199,7 +200,7 @@ __device__ __forceinline__ void unraw(float (&v)[8], const Raw8<float>& r) {
 // ROT8: rot is a multiple of 8, so the four pairs of a lane are rotated or not as one
 template <typename TA, int TOK, bool ROT8>
 __global__ void __launch_bounds__(128) attn_prepare_vec_kernel(const TA* __restrict__ qkv, long long ld, const int* __restrict__ pos,
-                                                               const int* __restrict__ row_entry, const int* __restrict__ page_table, int max_pages,
+                                                               const int* __restrict__ at, const int* __restrict__ row_entry, const int* __restrict__ page_table, int max_pages,
                                                                int page, const double* __restrict__ freq, const float* __restrict__ qn,
                                                                const float* __restrict__ kn, TA* __restrict__ q_out, TA* __restrict__ k_pages,
                                                                TA* __restrict__ v_pages, int rows, int H, int G, int dim, int vdim, int rot, float eps,
@@ -213,7 +214,7 @@ __global__ void __launch_bounds__(128) attn_prepare_vec_kernel(const TA* __restr
   long long pg_row[TOK];
 #pragma unroll
   for (int k = 0; k < TOK; ++k) {
-    const int t = min(t0 + k, rows - 1), p = pos[t];
+    const int t = min(t0 + k, rows - 1), p = at[t];
     pg_row[k] = nk > 0 ? (long long)page_table[(long long)row_entry[t] * max_pages + p / page] * page + p % page : 0;
   }
   constexpr int DEEP = TOK == 1 ? 3 : 1;  // pieces of a row under way: one token has too few rows in flight otherwise
@@ -1206,10 +1207,11 @@ extern "C" int pg_rotary_table(const int* pos, const double* freq, float* out, i
   PG_RET();
 }
 
-extern "C" int pg_attn_prepare(const void* qkv, long long ld, const int* pos, const int* row_entry, const int* page_table, int max_pages,
+extern "C" int pg_attn_prepare_at(const void* qkv, long long ld, const int* pos, const int* at, const int* row_entry, const int* page_table, int max_pages,
                                int page, const double* freq, const float* q_norm, const float* k_norm, void* q_out, void* k_pages,
                                void* v_pages, int rows, int H, int G, int dim, int vdim, int rot_dims, float eps, int norm_qk, int norm_v,
                                int v_from_k, float rot_gain, const void* v_other, long long ld_v_other, float v_mix, int act_f32, void* stream) {
+  if (at == nullptr) at = pos;
   if (rows <= 0 || H <= 0 || G <= 0 || dim <= 0 || vdim <= 0 || rot_dims < 0 || rot_dims > dim || (rot_dims & 1) || page <= 0) return PG_ERR_ARG;
   if (v_from_k && vdim != dim) return PG_ERR_ARG;
   if (norm_qk < 0 || norm_qk > 2 || (v_other != nullptr && k_pages == nullptr)) return PG_ERR_ARG;
@@ -1226,7 +1228,7 @@ extern "C" int pg_attn_prepare(const void* qkv, long long ld, const int* pos, co
     auto go = [&](auto kernel, auto t, int tok) {
       using TA = decltype(t);
       pg::launch_dependent(kernel, (rows + tok - 1) / tok, 128, (size_t)(tok * rot_dims + 2) * sizeof(float), PG_ST(stream), 
-          static_cast<const TA*>(qkv), ld, pos, row_entry, page_table, max_pages, page, freq, q_norm, k_norm, static_cast<TA*>(q_out), static_cast<TA*>(k_pages),
+          static_cast<const TA*>(qkv), ld, pos, at, row_entry, page_table, max_pages, page, freq, q_norm, k_norm, static_cast<TA*>(q_out), static_cast<TA*>(k_pages),
           static_cast<TA*>(v_pages), rows, H, G, dim, vdim, rot_dims, eps, norm_qk, norm_v, v_from_k, rot_gain, static_cast<const TA*>(v_other), ld_v_other, v_mix,
           k_pages != nullptr ? 0 : pg::weights_follow());  // (pages may be read ahead of the wait of the kernel behind, whatever its products take)
     };
@@ -1242,16 +1244,24 @@ extern "C" int pg_attn_prepare(const void* qkv, long long ld, const int* pos, co
   }
   const size_t smem = (size_t)(rot_dims + 2) * sizeof(float);
   if (act_f32)
-    pg::launch_dependent(attn_prepare_kernel<float>, rows, 128, smem, PG_ST(stream), static_cast<const float*>(qkv), ld, pos, row_entry, page_table, max_pages, page, freq,
+    pg::launch_dependent(attn_prepare_kernel<float>, rows, 128, smem, PG_ST(stream), static_cast<const float*>(qkv), ld, pos, at, row_entry, page_table, max_pages, page, freq,
                                                                   q_norm, k_norm, static_cast<float*>(q_out), static_cast<float*>(k_pages),
                                                                   static_cast<float*>(v_pages), H, G, dim, vdim, rot_dims, eps, norm_qk, norm_v, v_from_k, rot_gain,
                                                                   static_cast<const float*>(v_other), ld_v_other, v_mix);
   else
-    pg::launch_dependent(attn_prepare_kernel<bf16>, rows, 128, smem, PG_ST(stream), static_cast<const bf16*>(qkv), ld, pos, row_entry, page_table, max_pages, page, freq,
+    pg::launch_dependent(attn_prepare_kernel<bf16>, rows, 128, smem, PG_ST(stream), static_cast<const bf16*>(qkv), ld, pos, at, row_entry, page_table, max_pages, page, freq,
                                                                  q_norm, k_norm, static_cast<bf16*>(q_out), static_cast<bf16*>(k_pages),
                                                                  static_cast<bf16*>(v_pages), H, G, dim, vdim, rot_dims, eps, norm_qk, norm_v, v_from_k, rot_gain,
                                                                  static_cast<const bf16*>(v_other), ld_v_other, v_mix);
   PG_RET();
+}
+
+extern "C" int pg_attn_prepare(const void* qkv, long long ld, const int* pos, const int* row_entry, const int* page_table, int max_pages,
+                               int page, const double* freq, const float* q_norm, const float* k_norm, void* q_out, void* k_pages,
+                               void* v_pages, int rows, int H, int G, int dim, int vdim, int rot_dims, float eps, int norm_qk, int norm_v,
+                               int v_from_k, float rot_gain, const void* v_other, long long ld_v_other, float v_mix, int act_f32, void* stream) {
+  return pg_attn_prepare_at(qkv, ld, pos, nullptr, row_entry, page_table, max_pages, page, freq, q_norm, k_norm, q_out, k_pages, v_pages, rows, H, G, dim, vdim, rot_dims, eps,
+                            norm_qk, norm_v, v_from_k, rot_gain, v_other, ld_v_other, v_mix, act_f32, stream);
 }
 
 template <typename TA, int VC>

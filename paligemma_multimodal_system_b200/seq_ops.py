@@ -55,6 +55,10 @@ class StepBatch:
     # with a fresh one (`step_scope`)
     shared: Optional[dict] = None
     min_n: int = 1            # the fewest new tokens of an entry (1 where that is not known)
+    # drafted trees: `pos` (which turns queries and keys) is then ctx + depth, rows are stored one behind another at cache rows `at`, and a row sees the
+    # drafted rows of its entry whose bit is set in its mask (bit m % 32 of word m / 32)
+    at: Optional[torch.Tensor] = None    # int32 [T]; None: pos
+    tree: Optional[torch.Tensor] = None  # int32 [T, words]; None: rows see every row in front of them
 
 
 def _single_rows(ns):
@@ -67,8 +71,26 @@ def _single_rows(ns):
     return None if first is None else (first, last)
 
 
+def _tree_masks(parents, ns):
+    """parents: per entry a list (parents[i] < i is the row that row i follows, -1 the stored tokens) or None for a chain.  Returns (mask words uint32 [T, words],
+    depth of every row)."""
+    words = (max(ns) + 31) // 32
+    masks, depth, r = np.zeros((sum(ns), words), dtype=np.uint32), np.zeros(sum(ns), dtype=np.int32), 0
+    for up, n in zip(parents, ns):
+        up = range(-1, n - 1) if up is None else [int(x) for x in up]
+        if len(up) != n or any(not -1 <= x < i for i, x in enumerate(up)):
+            raise ValueError("parents: one for every token, an earlier token of the entry or -1")
+        for i, x in enumerate(up):
+            if x >= 0:
+                masks[r + i], depth[r + i] = masks[r + x], depth[r + x] + 1
+            masks[r + i, i // 32] |= np.uint32(1 << (i % 32))
+        r += n
+    return masks, depth
+
+
 def make_step_batch(entries: Sequence[dict]) -> StepBatch:
-    """entries: dicts with tokens (list[int]), ctx (int), slot (int), pages (list[int]).  One host buffer, one copy."""
+    """entries: dicts with tokens (list[int]), ctx (int), slot (int), pages (list[int]); drafted trees: parents (list[int], see _tree_masks; entries without are
+    chains).  One host buffer, one copy."""
     E = len(entries)
     ns = [len(e["tokens"]) for e in entries]
     T = sum(ns)
@@ -78,13 +100,18 @@ def make_step_batch(entries: Sequence[dict]) -> StepBatch:
     lens = [e["ctx"] + k if k > 1 else 0 for e, k in zip(entries, ns)]
     dpages = [(l + 63) // 64 for l in lens]
     dmax = max(1, max(dpages))
-    buf = np.zeros(3 * T + 4 * E + E * max_pages + E + E * dmax, dtype=np.int32)
+    masks = depth = None
+    if any(e.get("parents") is not None for e in entries):
+        masks, depth = _tree_masks([e.get("parents") for e in entries], ns)
+    words = 0 if masks is None else masks.shape[1]
+    plain = 3 * T + 4 * E + E * max_pages + E + E * dmax
+    buf = np.zeros(plain + (0 if masks is None else T * (1 + words)), dtype=np.int32)
     tokens, pos, row_entry = buf[:T], buf[T:2 * T], buf[2 * T:3 * T]
     o = 3 * T
     row0, n, ctx, slot = buf[o:o + E], buf[o + E:o + 2 * E], buf[o + 2 * E:o + 3 * E], buf[o + 3 * E:o + 4 * E]
     pt = buf[o + 4 * E:o + 4 * E + E * max_pages].reshape(E, max_pages)
     o2 = o + 4 * E + E * max_pages
-    drow0, dpt = buf[o2:o2 + E], buf[o2 + E:].reshape(E, dmax)
+    drow0, dpt = buf[o2:o2 + E], buf[o2 + E:plain].reshape(E, dmax)
     page0 = 0
     for i in range(E):
         drow0[i] = page0 * 64
@@ -101,14 +128,19 @@ def make_step_batch(entries: Sequence[dict]) -> StepBatch:
         row0[i], n[i], ctx[i], slot[i] = r, k, e["ctx"], e["slot"]
         pt[i, :len(e["pages"])] = e["pages"]
         r += k
+    if masks is not None:
+        buf[plain:plain + T] = pos
+        buf[plain + T:] = masks.reshape(-1).view(np.int32)
+        pos[:] = ctx[row_entry] + depth
     dev = torch.from_numpy(buf).pin_memory().to("cuda", non_blocking=True)
     o = 3 * T
     return StepBatch(T=T, E=E, max_n=max(ns), min_n=min(ns), tokens=dev[:T], pos=dev[T:2 * T], row_entry=dev[2 * T:3 * T], row0=dev[o:o + E],
                      n=dev[o + E:o + 2 * E], ctx=dev[o + 2 * E:o + 3 * E], slot=dev[o + 3 * E:o + 4 * E],
                      page_table=dev[o + 4 * E:o2].view(E, max_pages), max_pages=max_pages, singles=sum(k == 1 for k in ns),
                      max_single_ctx=max([e["ctx"] for e, k in zip(entries, ns) if k == 1], default=0), single_rows=_single_rows(ns),
-                     dense_row0=dev[o2:o2 + E], dense_pages=dev[o2 + E:].view(E, dmax), dense_max_pages=dmax, dense_rows=page0 * 64,
-                     dense_max_len=max(lens))
+                     dense_row0=dev[o2:o2 + E], dense_pages=dev[o2 + E:plain].view(E, dmax), dense_max_pages=dmax, dense_rows=page0 * 64,
+                     dense_max_len=max(lens), at=None if masks is None else dev[plain:plain + T],
+                     tree=None if masks is None else dev[plain + T:].view(T, words))
 
 
 def step_scope(b: StepBatch) -> StepBatch:
@@ -372,17 +404,77 @@ def attn_prepare(qkv, b: StepBatch, freq, q_norm, k_norm, q_out, k_pages, v_page
     """q_norm / k_norm None: norms without a weight; norm_qk / norm_v False: no q/k norm / no value norm; k_pages and v_pages None: the
     rows hold queries only (the layer attends over another layer's cache); v_from_k: the rows have no value columns, the values are the
     keys as projected (before norm and rotation); norm_qk NORM_PROJECTION: the norms run over all heads at once (weights of that size);
-    rot_gain multiplies cosines and sines; v_other [T, G * vdim]: the values become (1 - v_mix) v + v_mix v_other."""
+    rot_gain multiplies cosines and sines; v_other [T, G * vdim]: the values become (1 - v_mix) v + v_mix v_other.
+    k_pages and v_pages may be QuantizedPages: the rows are quantised as they are written."""
     for w, heads in ((q_norm, H), (k_norm, G)):
         assert w is None or (w.dtype == torch.float32 and w.is_contiguous() and w.numel() == (heads * dim if norm_qk is NORM_PROJECTION else dim))
     assert v_other is None or (v_other.dtype == qkv.dtype and v_other.stride(1) == 1 and v_other.shape == (b.T, G * vdim))
     assert qkv.stride(1) == 1 and freq.dtype == torch.float64 and qkv.dtype == q_out.dtype and (k_pages is None) == (v_pages is None)
+    mode = 2 if norm_qk is NORM_PROJECTION else int(bool(norm_qk))
+    tail = (b.T, H, G, dim, vdim, rot_dims, float(eps), mode, int(bool(norm_v)), int(bool(v_from_k)), float(rot_gain), _lib.ptr(v_other),
+            0 if v_other is None else v_other.stride(0), float(v_mix), int(qkv.dtype == torch.float32), _lib.stream())
+    if isinstance(k_pages, QuantizedPages):
+        _check_quantized(k_pages, v_pages, G, dim, vdim, page)
+        assert q_out.is_contiguous()
+        _lib.check(_lib.lib().pg_attn_prepare_e4m3(qkv.data_ptr(), qkv.stride(0), b.pos.data_ptr(), _lib.ptr(b.at), b.row_entry.data_ptr(), b.page_table.data_ptr(),
+                                                   b.max_pages, page, freq.data_ptr(), _lib.ptr(q_norm), _lib.ptr(k_norm), q_out.data_ptr(), k_pages.codes.data_ptr(),
+                                                   k_pages.powers.data_ptr(), v_pages.codes.data_ptr(), v_pages.powers.data_ptr(), *tail), "pg_attn_prepare_e4m3")
+        return
     assert k_pages is None or k_pages.dtype == qkv.dtype
-    _lib.check(_lib.lib().pg_attn_prepare(qkv.data_ptr(), qkv.stride(0), b.pos.data_ptr(), b.row_entry.data_ptr(), b.page_table.data_ptr(),
-                                          b.max_pages, page, freq.data_ptr(), _lib.ptr(q_norm), _lib.ptr(k_norm), q_out.data_ptr(),
-                                          _lib.ptr(k_pages), _lib.ptr(v_pages), b.T, H, G, dim, vdim, rot_dims, float(eps), 2 if norm_qk is NORM_PROJECTION else int(bool(norm_qk)),
-                                          int(bool(norm_v)), int(bool(v_from_k)), float(rot_gain), _lib.ptr(v_other), 0 if v_other is None else v_other.stride(0),
-                                          float(v_mix), int(qkv.dtype == torch.float32), _lib.stream()), "pg_attn_prepare")
+    _lib.check(_lib.lib().pg_attn_prepare_at(qkv.data_ptr(), qkv.stride(0), b.pos.data_ptr(), _lib.ptr(b.at), b.row_entry.data_ptr(), b.page_table.data_ptr(),
+                                             b.max_pages, page, freq.data_ptr(), _lib.ptr(q_norm), _lib.ptr(k_norm), q_out.data_ptr(),
+                                             _lib.ptr(k_pages), _lib.ptr(v_pages), *tail), "pg_attn_prepare_at")
+
+
+# ---- the 8-bit cache -------------------------------------------------------------------------------------------------
+class QuantizedPages:
+    """One operand (keys or values) of a layer's paged cache in 8 bits: e4m3 codes uint8 [pages, page, heads * size] and one power of two per row and head,
+    2^(byte - 127), uint8 [pages, heads, page] -- the least that takes the head's largest finite element to 448 or below.  An element is code * power; what
+    is not finite is kept as NaN.  `attn_prepare` writes them, `attn_ragged` and `attn_tree` read them, `kv_read` gives rows back in an activation type."""
+
+    def __init__(self, codes: torch.Tensor, powers: torch.Tensor):
+        if codes.dtype != torch.uint8 or powers.dtype != torch.uint8 or codes.dim() != 3 or powers.dim() != 3:
+            raise ValueError("8-bit pages are uint8 codes [pages, page, heads * size] and uint8 powers [pages, heads, page]")
+        if powers.shape[0] != codes.shape[0] or powers.shape[2] != codes.shape[1] or codes.shape[2] % powers.shape[1] or not (codes.is_contiguous() and powers.is_contiguous()):
+            raise ValueError(f"8-bit pages that do not belong together: codes {tuple(codes.shape)}, powers {tuple(powers.shape)}")
+        self.codes, self.powers = codes, powers
+
+    @classmethod
+    def empty(cls, pages: int, page: int, heads: int, size: int, device="cuda"):
+        return cls(torch.zeros(pages, page, heads * size, device=device, dtype=torch.uint8), torch.zeros(pages, heads, page, device=device, dtype=torch.uint8))
+
+    @property
+    def heads(self):
+        return self.powers.shape[1]
+
+
+def _check_quantized(k: "QuantizedPages", v: "QuantizedPages", G, dim, vdim, page):
+    if not isinstance(k, QuantizedPages) or not isinstance(v, QuantizedPages):
+        raise ValueError("keys and values are kept in one form: both in 8 bits or neither")
+    if dim % 16 or vdim % 16 or dim > 256 or vdim > 256:
+        raise ValueError(f"the 8-bit cache keeps heads of a multiple of 16 elements up to 256: got {dim} and {vdim}")
+    for x, size in ((k, dim), (v, vdim)):
+        if x.heads != G or x.codes.shape[2] != G * size or x.codes.shape[1] != page:
+            raise ValueError(f"8-bit pages of {x.heads} heads, {x.codes.shape[2]} elements and {x.codes.shape[1]} rows for {G} heads of {size} and pages of {page}")
+
+
+def kv_read(k_pages: "QuantizedPages", v_pages: "QuantizedPages", b: StepBatch, dtype: torch.dtype):
+    """Keys and values of every entry with several new tokens, stored and new, in `dtype` (bf16 / fp32): [dense_rows, heads * size] each, in the dense scratch
+    layout of the batch (read through b.dense_pages); zeros behind an entry's last row."""
+    if not isinstance(k_pages, QuantizedPages) or not isinstance(v_pages, QuantizedPages):
+        raise ValueError("kv_read reads 8-bit pages")
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("rows come back as torch.bfloat16 or torch.float32")
+    G, page = k_pages.heads, k_pages.codes.shape[1]
+    dim, vdim = k_pages.codes.shape[2] // G, v_pages.codes.shape[2] // G
+    _check_quantized(k_pages, v_pages, G, dim, vdim, page)
+    k = torch.empty(b.dense_rows, G * dim, device=k_pages.codes.device, dtype=dtype)
+    v = torch.empty(b.dense_rows, G * vdim, device=k_pages.codes.device, dtype=dtype)
+    if b.dense_rows:
+        _lib.check(_lib.lib().pg_kv_read_e4m3(k_pages.codes.data_ptr(), k_pages.powers.data_ptr(), v_pages.codes.data_ptr(), v_pages.powers.data_ptr(), b.page_table.data_ptr(),
+                                              b.max_pages, page, b.dense_row0.data_ptr(), b.n.data_ptr(), b.ctx.data_ptr(), k.data_ptr(), v.data_ptr(), b.E, b.dense_max_len,
+                                              G, dim, vdim, int(dtype == torch.float32), _lib.stream()), "pg_kv_read_e4m3")
+    return k, v
 
 
 class ScoreOptions:
@@ -429,8 +521,25 @@ def attn_ragged(q, k_pages, v_pages, gate, out, b: StepBatch, H, G, dim, vdim, s
     order.  krow / vrow: elements per cache row when it is not G * dim / G * vdim (a latent cache: one row is key and value);
     gate_per_head: the gate holds one scalar per head instead of one per output element; only_singles / skip_singles: rows of
     entries with several new tokens / with one new token are left alone (another form computes them).  score: window, sink, distance
-    penalty and per-head multiplier (ScoreOptions; None: plain causal attention)."""
+    penalty and per-head multiplier (ScoreOptions; None: plain causal attention).
+    Pages in 8 bits (QuantizedPages): decoded tokens read the codes, entries with several new rows go over rows read back (kv_read).  A batch of drafted trees:
+    attn_tree."""
     import ctypes as C
+    if b.tree is not None:
+        if krow or vrow or only_singles or skip_singles:
+            raise ValueError("drafted trees go over a cache of one key row and one value row a token, all entries in one call")
+        return attn_tree(q, k_pages, v_pages, gate, out, b, H, G, dim, vdim, scale, softcap, page, gate_per_head=gate_per_head, score=score)
+    if isinstance(k_pages, QuantizedPages):
+        _check_quantized(k_pages, v_pages, G, dim, vdim, page)
+        if krow or vrow:
+            raise ValueError("8-bit pages have rows of their own width")
+        if b.singles < b.E and not only_singles:
+            k, v = kv_read(k_pages, v_pages, b, q.dtype)
+            attn_ragged(q, k, v, gate, out, dense_view(b), H, G, dim, vdim, scale, softcap, page, decode_kernel, tensor_cores, gate_per_head=gate_per_head, skip_singles=True,
+                        score=score)
+        if b.singles and not skip_singles:
+            _attn_rows(q, k_pages, v_pages, gate, out, b, H, G, dim, vdim, scale, softcap, page, gate_per_head, score, singles=True)
+        return
     L, f32 = _lib.lib(), int(q.dtype == torch.float32)
     sx = C.addressof(score.c) if score is not None else 0
     reach = score.visible_keys(b.max_single_ctx) if score is not None else b.max_single_ctx + 1  # keys a decoded token reads at most
@@ -479,6 +588,83 @@ def attn_ragged(q, k_pages, v_pages, gate, out, b: StepBatch, H, G, dim, vdim, s
                                     b.row0.data_ptr(), b.n.data_ptr(), b.ctx.data_ptr(), b.page_table.data_ptr(), b.max_pages, page, b.E, nsplit,
                                     H, G, dim, vdim, float(scale), float(softcap or 0.0), f32, int(krow), int(vrow), gph, sx, _lib.stream()),
                    "pg_attn_decode")
+
+
+def _rows_split(entries, G, rows, tiles, wide, row_tile):
+    """CTAs that share an entry's keys: what two CTAs an SM hold at once, and at least two key tiles for every warp."""
+    warps = 1  # of a CTA that hold rows; the others share the key walk
+    while warps < 4 and warps * row_tile < rows:
+        warps *= 2
+    ctas = entries * G * -(-rows // (warps * row_tile))
+    return max(1, min(2 * _lib.num_sms() // ctas, tiles // (2 * (4 // warps)), 64))
+
+
+def _attn_rows(q, k_pages, v_pages, gate, out, b: StepBatch, H, G, dim, vdim, scale, softcap, page, gate_per_head, score, singles):
+    import ctypes as C
+    quantized, f32 = isinstance(k_pages, QuantizedPages), int(q.dtype == torch.float32)
+    if dim > 128 or vdim > 128:
+        raise ValueError(f"attention of a few rows takes heads of up to 128 elements: got {dim} and {vdim}")
+    rows = (1 if singles else b.max_n) * (H // G)
+    row_tile = 32 if rows > 16 and not f32 else 16
+    wide = dim > 64 or vdim > 64
+    keys = 32 if quantized or not (f32 or wide) else 16
+    context = b.max_single_ctx + 1 if singles else max(b.max_single_ctx + 1, b.dense_max_len)
+    reach = context if score is None or not score.window else min(context, score.window + score.keep_first + b.max_n + 2 * keys)
+    nsplit = _rows_split(b.singles if singles else b.E, G, rows, -(-reach // keys), wide, row_tile)
+    L = _lib.lib()
+    need = L.pg_attn_rows_scratch(b.E if singles else b.T, H, vdim, nsplit)
+    partial = torch.empty(need // 4, device=q.device, dtype=torch.float32) if need else None
+    kv = _lib.KvPages(k_pages.codes.data_ptr(), v_pages.codes.data_ptr(), k_pages.powers.data_ptr(), v_pages.powers.data_ptr(), 1, 0) if quantized else \
+        _lib.KvPages(k_pages.data_ptr(), v_pages.data_ptr(), 0, 0, 0, f32)
+    tree = None if singles else b.tree
+    _lib.check(L.pg_attn_rows(q.data_ptr(), C.addressof(kv), _lib.ptr(gate), 0 if gate is None else gate.stride(0), out.data_ptr(), _lib.ptr(partial), b.row0.data_ptr(),
+                              b.n.data_ptr(), b.ctx.data_ptr(), b.page_table.data_ptr(), b.max_pages, page, b.pos.data_ptr(), _lib.ptr(tree),
+                              0 if tree is None else tree.shape[1], b.E, b.max_n, int(singles), nsplit, H, G, dim, vdim, float(scale), float(softcap or 0.0), f32,
+                              int(bool(gate_per_head)), C.addressof(score.c) if score is not None else 0, _lib.stream()), "pg_attn_rows")
+
+
+def attn_tree(q, k_pages, v_pages, gate, out, b: StepBatch, H, G, dim, vdim, scale, softcap, page, gate_per_head=False, score: Optional["ScoreOptions"] = None):
+    """Attention of drafted trees (b.tree; None: chains): every new row sees all stored keys of its entry and the drafted rows in its mask, softmax, gate and score
+    options as attn_ragged; windows and distances go by b.pos.  The drafted rows' keys and values are in the cache already (attn_prepare with b.at).  The cache:
+    pages of q's type or QuantizedPages.  Heads of up to 128 elements in whole 16-byte pieces, pages of a multiple of 32 rows.  A row whose mask is empty and
+    whose entry has nothing stored gets zeros."""
+    if isinstance(k_pages, QuantizedPages) or isinstance(v_pages, QuantizedPages):
+        _check_quantized(k_pages, v_pages, G, dim, vdim, page)
+    elif k_pages.dtype != q.dtype or v_pages.dtype != q.dtype:
+        raise ValueError("a cache that is not in 8 bits has the queries' type")
+    if q.dtype not in (torch.bfloat16, torch.float32) or out.dtype != q.dtype or (gate is not None and (gate.dtype != q.dtype or gate.stride(1) != 1)):
+        raise ValueError("queries, gate and output share a type, torch.bfloat16 or torch.float32")
+    if q.numel() != b.T * H * dim or not q.is_contiguous() or out.stride(-1) != 1 or H % G:
+        raise ValueError("queries are [rows, heads * size], heads a multiple of the key / value heads")
+    if b.tree is not None and (b.tree.dtype != torch.int32 or b.tree.dim() != 2 or b.tree.shape[0] != b.T or not b.tree.is_contiguous()):
+        raise ValueError("masks are int32 [rows, words]")
+    _attn_rows(q, k_pages, v_pages, gate, out, b, H, G, dim, vdim, scale, softcap, page, gate_per_head, score, singles=False)
+
+
+# ---- scored tokens ---------------------------------------------------------------------------------------------------
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, temperature: float = 1.0):
+    """logits fp32 [rows, vocab] (any row pitch), tokens int32 [rows]: under softmax(logits / temperature) the log probability of every row's token, the entropy in
+    nats, the token's rank (0: the most likely one; ties: the lower id is in front) and the `top` (0 .. 32) most likely ids with their log probabilities:
+    (fp32 [rows], fp32 [rows], int32 [rows], int32 [rows, top], fp32 [rows, top]).  A token outside the vocabulary: NaN and rank -1.  Masked entries are -inf; a row
+    with a NaN, a +inf or nothing but -inf has NaN for its numbers."""
+    if logits.dim() != 2 or logits.dtype != torch.float32 or logits.stride(1) != 1 or not logits.is_cuda:
+        raise ValueError("logits are fp32 [rows, vocab] on the device, entries of a row side by side")
+    rows, V = logits.shape
+    if tokens.dtype != torch.int32 or tokens.shape != (rows,) or not tokens.is_contiguous() or tokens.device != logits.device:
+        raise ValueError("one int32 token for every row of the logits, on their device")
+    if not 0 <= int(top) <= min(32, V):
+        raise ValueError(f"top is 0 .. 32 and at most the vocabulary: got {top}")
+    if not 0.0 < float(temperature) < float("inf"):
+        raise ValueError("the temperature is positive and finite")
+    top = int(top)
+    f = torch.empty(rows * (2 + top), device=logits.device, dtype=torch.float32)
+    i = torch.empty(rows * (1 + top), device=logits.device, dtype=torch.int32)
+    lp, entropy, top_lp = f[:rows], f[rows:2 * rows], f[2 * rows:].view(rows, top)
+    rank, ids = i[:rows], i[rows:].view(rows, top)
+    if rows:
+        _lib.check(_lib.lib().pg_token_logprobs(logits.data_ptr(), logits.stride(0) if rows > 1 else V, tokens.data_ptr(), lp.data_ptr(), entropy.data_ptr(), rank.data_ptr(), ids.data_ptr(),
+                                                top_lp.data_ptr(), rows, V, top, float(temperature), _lib.stream()), "pg_token_logprobs")
+    return lp, entropy, rank, ids, top_lp
 
 
 # ---- multi-stream residual -------------------------------------------------------------------------------------------
