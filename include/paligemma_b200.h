@@ -543,7 +543,7 @@ typedef struct PgKvPages {
  * zeros (with a sink as well).  Score, gate and out as pg_attn_decode; windows and distances go by pos [rows] (required for them, at least ctx each).
  * singles != 0: entries with one row only, others are left alone.  nsplit > 1: that many CTAs share an entry's keys through `partial`
  * (pg_attn_rows_scratch bytes for `entries` rows with singles, all rows else), joined by a second launch.
- * dim up to 128 in whole 16-byte pieces, vdim a multiple of 8 up to 128, page a multiple of 32, pages on 16-byte boundaries; anything else PG_ERR_ARG.
+ * dim up to 128 in whole 16-byte pieces, vdim a multiple of 8 up to 128, page a power of two from 32 on, pages on 16-byte boundaries; anything else PG_ERR_ARG.
  * max_n: the largest entry_n (rows past it are left out). */
 long long pg_attn_rows_scratch(int rows, int H, int vdim, int nsplit);
 int pg_attn_rows(const void* q, const PgKvPages* kv, const void* gate, long long ldg, void* out, float* partial, const int* entry_row0, const int* entry_n,

@@ -55,8 +55,16 @@ class StepBatch:
     # with a fresh one (`step_scope`)
     shared: Optional[dict] = None
     min_n: int = 1            # the fewest new tokens of an entry (1 where that is not known)
-    # drafted trees: `pos` (which turns queries and keys) is then ctx + depth, rows are stored one behind another at cache rows `at`, and a row sees the
-    # drafted rows of its entry whose bit is set in its mask (bit m % 32 of word m / 32)
+
+    # (no fields: TreeBatch)
+    at = None
+    tree = None
+
+
+@dataclasses.dataclass
+class TreeBatch(StepBatch):
+    """A step of drafted trees: `pos`, which turns queries and keys, is ctx + depth; rows are stored one behind another at cache rows `at`; a row sees the
+    drafted rows of its entry whose bit is set in its mask (bit m % 32 of word m / 32)."""
     at: Optional[torch.Tensor] = None    # int32 [T]; None: pos
     tree: Optional[torch.Tensor] = None  # int32 [T, words]; None: rows see every row in front of them
 
@@ -134,13 +142,15 @@ def make_step_batch(entries: Sequence[dict]) -> StepBatch:
         pos[:] = ctx[row_entry] + depth
     dev = torch.from_numpy(buf).pin_memory().to("cuda", non_blocking=True)
     o = 3 * T
-    return StepBatch(T=T, E=E, max_n=max(ns), min_n=min(ns), tokens=dev[:T], pos=dev[T:2 * T], row_entry=dev[2 * T:3 * T], row0=dev[o:o + E],
+    kind, more = StepBatch, {}
+    if masks is not None:
+        kind, more = TreeBatch, dict(at=dev[plain:plain + T], tree=dev[plain + T:].view(T, words))
+    return kind(T=T, E=E, max_n=max(ns), min_n=min(ns), tokens=dev[:T], pos=dev[T:2 * T], row_entry=dev[2 * T:3 * T], row0=dev[o:o + E],
                      n=dev[o + E:o + 2 * E], ctx=dev[o + 2 * E:o + 3 * E], slot=dev[o + 3 * E:o + 4 * E],
                      page_table=dev[o + 4 * E:o2].view(E, max_pages), max_pages=max_pages, singles=sum(k == 1 for k in ns),
                      max_single_ctx=max([e["ctx"] for e, k in zip(entries, ns) if k == 1], default=0), single_rows=_single_rows(ns),
                      dense_row0=dev[o2:o2 + E], dense_pages=dev[o2 + E:plain].view(E, dmax), dense_max_pages=dmax, dense_rows=page0 * 64,
-                     dense_max_len=max(lens), at=None if masks is None else dev[plain:plain + T],
-                     tree=None if masks is None else dev[plain + T:].view(T, words))
+                     dense_max_len=max(lens), **more)
 
 
 def step_scope(b: StepBatch) -> StepBatch:
@@ -596,7 +606,8 @@ def _rows_split(entries, G, rows, tiles, wide, row_tile):
     while warps < 4 and warps * row_tile < rows:
         warps *= 2
     ctas = entries * G * -(-rows // (warps * row_tile))
-    return max(1, min(2 * _lib.num_sms() // ctas, tiles // (2 * (4 // warps)), 64))
+    import os
+    return max(1, min(int(os.environ.get('TGT', 2)) * _lib.num_sms() // ctas, tiles // (int(os.environ.get('TPW', 2)) * (4 // warps)), 64))
 
 
 def _attn_rows(q, k_pages, v_pages, gate, out, b: StepBatch, H, G, dim, vdim, scale, softcap, page, gate_per_head, score, singles):
@@ -626,7 +637,7 @@ def _attn_rows(q, k_pages, v_pages, gate, out, b: StepBatch, H, G, dim, vdim, sc
 def attn_tree(q, k_pages, v_pages, gate, out, b: StepBatch, H, G, dim, vdim, scale, softcap, page, gate_per_head=False, score: Optional["ScoreOptions"] = None):
     """Attention of drafted trees (b.tree; None: chains): every new row sees all stored keys of its entry and the drafted rows in its mask, softmax, gate and score
     options as attn_ragged; windows and distances go by b.pos.  The drafted rows' keys and values are in the cache already (attn_prepare with b.at).  The cache:
-    pages of q's type or QuantizedPages.  Heads of up to 128 elements in whole 16-byte pieces, pages of a multiple of 32 rows.  A row whose mask is empty and
+    pages of q's type or QuantizedPages.  Heads of up to 128 elements in whole 16-byte pieces, pages of 32, 64, 128 .. rows.  A row whose mask is empty and
     whose entry has nothing stored gets zeros."""
     if isinstance(k_pages, QuantizedPages) or isinstance(v_pages, QuantizedPages):
         _check_quantized(k_pages, v_pages, G, dim, vdim, page)
