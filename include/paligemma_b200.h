@@ -528,28 +528,35 @@ int pg_kv_read_e4m3(const void* k_codes, const void* k_powers, const void* v_cod
                     const int* dense_row0, const int* entry_n, const int* entry_ctx, void* k_out, void* v_out, int entries, int longest, int G, int dim,
                     int vdim, int out_f32, void* stream);
 
-/* A layer's pages: of the activations' type (f32 tells which; k_powers and v_powers unused) or 8-bit (e4m3 != 0). */
-typedef struct PgKvPages {
+/* Attention of a few rows an entry: every row of an entry sees the stored keys 0 .. ctx - 1 and, of the entry's own n rows (cache rows ctx ..), those whose bit
+ * is set in its mask: tree uint32 [rows, tree_words], bit m % 32 of word m / 32 (bits from n on are ignored; NULL: rows up to itself).  A row that sees nothing gets
+ * zeros (with a sink as well).  Score, gate and out as pg_attn_decode; windows and distances go by pos [rows] (required for them, at least ctx each).
+ * The cache: pages of the activations' type, or 8-bit ones (e4m3 != 0, k_powers and v_powers).  singles != 0: entries with one row only, others are left alone.
+ * dim up to 128 in whole 16-byte pieces, vdim a multiple of 8 (8-bit: 16) up to 128, page a power of two from 32 on, pages and powers on 16-byte boundaries; anything
+ * else PG_ERR_ARG.  What the host knows of the step: rows, max_n the largest entry_n (rows past it are left out), busy the entries that have rows for this call and
+ * longest the longest ctx + n among them (these two only choose how many CTAs share an entry's keys).
+ * pg_attn_rows_scratch: the bytes of scratch (16-byte aligned) that the call needs, mostly 0; negative: the error that the call returns. */
+typedef struct PgAttnRows {
+  const void* q;
   const void* k;
   const void* v;
   const void* k_powers;
   const void* v_powers;
-  int e4m3;
-  int f32;
-} PgKvPages;
-
-/* Attention of a few rows an entry: every row of an entry sees the stored keys 0 .. ctx - 1 and, of the entry's own n rows (cache rows ctx ..), those whose bit
- * is set in its mask: tree uint32 [rows, tree_words], bit m % 32 of word m / 32 (bits from n on are ignored; NULL: rows up to itself).  A row that sees nothing gets
- * zeros (with a sink as well).  Score, gate and out as pg_attn_decode; windows and distances go by pos [rows] (required for them, at least ctx each).
- * singles != 0: entries with one row only, others are left alone.  nsplit > 1: that many CTAs share an entry's keys through `partial`
- * (pg_attn_rows_scratch bytes for `entries` rows with singles, all rows else), joined by a second launch.
- * dim up to 128 in whole 16-byte pieces, vdim a multiple of 8 up to 128, page a power of two from 32 on, pages on 16-byte boundaries; anything else PG_ERR_ARG.
- * max_n: the largest entry_n (rows past it are left out). */
-long long pg_attn_rows_scratch(int rows, int H, int vdim, int nsplit);
-int pg_attn_rows(const void* q, const PgKvPages* kv, const void* gate, long long ldg, void* out, float* partial, const int* entry_row0, const int* entry_n,
-                 const int* entry_ctx, const int* page_table, int max_pages, int page, const int* pos, const void* tree, int tree_words, int entries,
-                 int max_n, int singles, int nsplit, int H, int G, int dim, int vdim, float scale, float softcap, int act_f32, int gate_per_head,
-                 const PgAttnScore* score, void* stream);
+  const void* gate;
+  long long ldg;
+  void* out;
+  const int* entry_row0;
+  const int* entry_n;
+  const int* entry_ctx;
+  const int* page_table;
+  const int* pos;
+  const void* tree;
+  const PgAttnScore* score;
+  int max_pages, page, tree_words, entries, rows, max_n, busy, longest, singles, H, G, dim, vdim, act_f32, e4m3, gate_per_head;
+  float scale, softcap;
+} PgAttnRows;
+long long pg_attn_rows_scratch(const PgAttnRows* a);
+int pg_attn_rows(const PgAttnRows* a, void* scratch, long long scratch_bytes, void* stream);
 
 /* The merge launch of pg_attn_decode on its own: rows of single-token entries from `partial` (fp32 [entries, H, nsplit, vdim + 2]:
  * running max in natural-log units, sum, unnormalised accumulator), times the gate, to out [rows, H * vdim]. */

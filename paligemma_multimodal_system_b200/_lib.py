@@ -6,6 +6,7 @@ the stream.
 """
 import ctypes as C
 import os
+import struct
 
 import torch
 
@@ -89,8 +90,8 @@ SIGNATURES = {
     "pg_attn_prepare_at": [p, i64, p, p, p, p, i32, i32, p, p, p, p, p, p, i32, i32, i32, i32, i32, i32, f32, i32, i32, i32, f32, p, i64, f32, i32, p],
     "pg_attn_prepare_e4m3": [p, i64, p, p, p, p, i32, i32, p, p, p, p, p, p, p, p, i32, i32, i32, i32, i32, i32, f32, i32, i32, i32, f32, p, i64, f32, i32, p],
     "pg_kv_read_e4m3": [p, p, p, p, p, i32, i32, p, p, p, p, p, i32, i32, i32, i32, i32, i32, p],
-    "pg_attn_rows_scratch": [i32, i32, i32, i32],
-    "pg_attn_rows": [p, p, p, i64, p, p, p, p, p, p, i32, i32, p, p, i32, i32, i32, i32, i32, i32, i32, i32, i32, f32, f32, i32, i32, p, p],
+    "pg_attn_rows_scratch": [p],
+    "pg_attn_rows": [p, p, i64, p],
     "pg_token_logprobs": [p, i64, p, p, p, p, p, p, i32, i32, i32, f32, p],
     "pg_attn_ragged": [p, p, p, p, i64, p, p, p, p, p, i32, i32, i32, i32, i32, i32, i32, i32, f32, f32, i32, i32, i64, i64, i32, p, p],
     "pg_attn_ragged_mma": [p, p, p, p, i64, p, p, p, p, p, i32, i32, i32, i32, i32, i32, i32, i32, f32, f32, i32, i32, p, p],
@@ -146,9 +147,8 @@ class AttnScore(C.Structure):
                 ("head_bias", p), ("out_scale", f32), ("out_ld", i64)]
 
 
-class KvPages(C.Structure):
-    """Mirror of PgKvPages."""
-    _fields_ = [("k", p), ("v", p), ("k_powers", p), ("v_powers", p), ("e4m3", i32), ("f32", i32)]
+# Mirror of PgAttnRows, packed in one go (thirty-three conversions one by one: 2.6 us of a call, 0.3 this way)
+ATTN_ROWS = struct.Struct("@6Pq8P16i2f")
 
 
 class RoutedFf(C.Structure):

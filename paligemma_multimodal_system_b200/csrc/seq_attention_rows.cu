@@ -46,7 +46,7 @@ struct Args {
   float* partial;
   const int *row0, *n, *ctx, *pt, *pos;
   const uint32_t* tree;
-  int words, max_pages, page, tile_shift, singles, nsplit, blocks, H, G, dim, vdim, wr, mode;  // tile_shift: log2 of a page's tiles; mode: below
+  int words, max_pages, page, tile_shift, singles, nsplit, cluster, blocks, H, G, dim, vdim, wr, mode;  // tile_shift: log2 of a page's tiles
   float scale, softcap;
   int gate_per_head;
   PgAttnScore sx;
@@ -140,6 +140,42 @@ constexpr int ctas_per_sm() {
   return DC > 1 || VC > 1 ? OCCW : sizeof(TC) == 4 ? 2 : MT == 2 ? OCCM : sizeof(TC) == 1 ? OCC : 2;
 }
 
+// where a row of a k/v head's block goes
+struct Row {
+  long long t;
+  int head;
+  __device__ __forceinline__ Row(const Args& a, int rr, int gsz, int g, long long t0) {
+    const int i = rr / gsz;
+    t = t0 + i;
+    head = g * gsz + rr - i * gsz;
+  }
+};
+__device__ __forceinline__ void add(float4& acc, float f, float4 v) {
+  acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
+}
+template <typename TQ>
+__device__ __forceinline__ void gates(const Args& a, const Row& r, int col, float (&gv)[4]) {
+  if (a.gate == nullptr) return;
+  const TQ* g = static_cast<const TQ*>(a.gate) + r.t * a.ldg + (a.gate_per_head ? r.head : r.head * a.vdim + col);
+#pragma unroll
+  for (int y = 0; y < 4; ++y) gv[y] = ldf(g + (a.gate_per_head ? 0 : y));
+}
+// four columns of a row from its sums: sink, division, gate.  A row that sees nothing: zeros.
+template <typename TQ>
+__device__ __forceinline__ void finish(const Args& a, const Row& r, int col, float ref, float l, float4 acc, const float (&gv)[4]) {
+  float by = 1.f;
+  if (!a.sx.logistic && a.sx.sink != nullptr) {
+    const float sk = a.sx.sink[r.head] * kLog2e, mm = fmaxf(ref, sk);
+    by = ex2(ref - mm);
+    l = l * by + ex2(sk - mm);
+  }
+  by *= (a.sx.logistic ? 1.f : l == 0.f ? 0.f : 1.f / l) * (a.sx.out_scale != 0.f ? a.sx.out_scale : 1.f);
+  TQ* dst = static_cast<TQ*>(a.out) + r.t * (a.sx.out_ld > 0 ? a.sx.out_ld : (long long)a.H * a.vdim) + (long long)r.head * a.vdim + col;
+  const float v[4] = {acc.x, acc.y, acc.z, acc.w};
+#pragma unroll
+  for (int y = 0; y < 4; ++y) stf(dst + y, a.gate != nullptr ? v[y] * by / (1.0f + expf(-gv[y])) : v[y] * by);
+}
+
 // A 16-byte piece's place in a tile.  Keys: two neighbouring rows are read together, pieces 4 x .. 4 x + 3 of each: rows of 128 bytes and more turn the odd row's by four.  Values:
 // four rows KPL apart are read together: each takes other banks.
 template <int ROW>
@@ -153,8 +189,8 @@ __device__ __forceinline__ uint32_t value_place(int row, int piece) {
   return row * ROW + 16 * (piece ^ turn);
 }
 
-// DC, VC: 64-element pieces of a key / value row; MT: 16-row tiles of a warp; KT: keys of a tile
-template <typename TQ, typename TC, int DC, int VC, int MT, int KT>
+// DC, VC: 64-element pieces of a key / value row; MT: 16-row tiles of a warp; KT: keys of a tile; R8: a k/v head has at most eight rows, the tile's upper half is empty
+template <typename TQ, typename TC, int DC, int VC, int MT, int KT, bool R8>
 __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>())) attn_rows_kernel(const __grid_constant__ Args a) {
   using K = Kind<TQ, TC, DC, VC, MT, KT>;
   constexpr int NB = KT / 8, KPL = KT / 4;  // key fragments of a tile; keys of a lane
@@ -163,6 +199,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
   __shared__ float unscale[kWarps * 16 * MT];  // what a row's scores are multiplied by
   __shared__ float2 stat[kWarps][16 * MT];
   __shared__ float top_power[kWarps];
+  __shared__ float2 joined[kWarps * 16 * MT];
   // the step's descriptors are there before its first kernel
   const int split = blockIdx.x, g = blockIdx.y / a.blocks, block = blockIdx.y % a.blocks, e = blockIdx.z;
   const int n = a.n[e], ctx = a.ctx[e], gsz = a.H / a.G, len = ctx + n;
@@ -188,7 +225,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
     return w < nwalk ? pt[tile_of(w) >> a.tile_shift] : 0;
   };
   int pids = pages_from(walk0);
-  if (a.nsplit > 1) pg::griddep_begin<true>();  // (fp32 partials, read behind a wait)
+  if (a.nsplit > 1 && !a.cluster) pg::griddep_begin<true>();  // (fp32 partials, read behind a wait)
   else pg::griddep_begin_if(a.trigger);
   if (!mine) return;
 
@@ -287,9 +324,6 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
     node[x] = min((r0 + r) / gsz, n - 1);
     uns[x] = unscale[r];
   }
-  bool upper[MT];  // the second half of a tile holds rows
-#pragma unroll
-  for (int m = 0; m < MT; ++m) upper[m] = live > 16 * m + 8;
 
   float M[2 * MT], L[2 * MT], o[MT][8 * VC][4];
 #pragma unroll
@@ -421,9 +455,12 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
         grow = top - P >= 127 ? 0.f : __uint_as_float(static_cast<uint32_t>(127 - (top - P)) << 23);
         P = top;
       }
-      const int lift = 142 - P;  // 2^(15 + power - P): a weight of one is 2^15, halves reach down to 2^-24
+      // 2^(15 + power - P): a weight of one is 2^15, halves reach down to 2^-24; four bytes at a time, P - 142 <= byte <= P, so that none carries into the next
+      const uint32_t least = static_cast<uint32_t>(max(P - 142, 0)) * 0x01010101u, lift = static_cast<uint32_t>(142 - P) * 0x01010101u;
 #pragma unroll
-      for (int x = 0; x < KPL; ++x) vf[x] = __uint_as_float(static_cast<uint32_t>(max(static_cast<int>(vpw[x / 4] >> (8 * (x % 4)) & 0xffu) + lift, 0)) << 23);
+      for (int x = 0; x < KPL / 4; ++x) vpw[x] = __vmaxu4(vpw[x], least) + lift;
+#pragma unroll
+      for (int x = 0; x < KPL; ++x) vf[x] = __uint_as_float((vpw[x / 4] >> (8 * (x % 4)) & 0xffu) << 23);
     }
     uint4 pa[MT][NB / 2][K::PT];
 #pragma unroll
@@ -432,7 +469,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int x = 2 * m + h;
-        if (h == 1 && !upper[m]) {
+        if (h == 1 && R8) {
 #pragma unroll
           for (int f = 0; f < NB; ++f) s[m][f][2] = s[m][f][3] = 0.f;
           corr[1] = 1.f;
@@ -519,20 +556,25 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
           corr[h] *= grow;
         }
       }
-      if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
+      if (__any_sync(0xffffffffu, corr[0] != 1.f || (!R8 && corr[1] != 1.f))) {
 #pragma unroll
         for (int b = 0; b < 8 * VC; ++b) {
           o[m][b][0] *= corr[0], o[m][b][1] *= corr[0];
-          o[m][b][2] *= corr[1], o[m][b][3] *= corr[1];
+          if (!R8) o[m][b][2] *= corr[1], o[m][b][3] *= corr[1];
         }
       }
 #pragma unroll
       for (int q = 0; q < NB / 2; ++q) {
         uint32_t p0[K::PT], p1[K::PT], p2[K::PT], p3[K::PT];
         terms<K::HALF>(s[m][2 * q][0], s[m][2 * q][1], p0);
-        terms<K::HALF>(s[m][2 * q][2], s[m][2 * q][3], p1);
         terms<K::HALF>(s[m][2 * q + 1][0], s[m][2 * q + 1][1], p2);
-        terms<K::HALF>(s[m][2 * q + 1][2], s[m][2 * q + 1][3], p3);
+        if (R8) {
+#pragma unroll
+          for (int t = 0; t < K::PT; ++t) p1[t] = p3[t] = 0u;
+        } else {
+          terms<K::HALF>(s[m][2 * q][2], s[m][2 * q][3], p1);
+          terms<K::HALF>(s[m][2 * q + 1][2], s[m][2 * q + 1][3], p3);
+        }
 #pragma unroll
         for (int t = 0; t < K::PT; ++t) pa[m][q][t] = make_uint4(p0[t], p1[t], p2[t], p3[t]);
       }
@@ -670,7 +712,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     const int r = 16 * (x / 2) + 8 * (x % 2) + nn;
     if (c == 0) stat[warp][r] = make_float2(M[x], l);
-    if (x % 2 == 1 && !upper[x / 2]) continue;
+    if (R8 && x % 2 == 1) continue;
     float* dst = os + (warp * 16 * MT + r) * ldo_s;
 #pragma unroll
     for (int b = 0; b < VC; ++b)
@@ -688,22 +730,16 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
   if (K::C8 && lane == 0) top_power[warp] = static_cast<float>(P);
   __syncthreads();
   const int rows_here = min(rows_cta, R - r0);
-  const long long ldo = a.sx.out_ld > 0 ? a.sx.out_ld : (long long)a.H * a.vdim;
-  const float oscale = a.sx.out_scale != 0.f ? a.sx.out_scale : 1.f;
   const int quads = a.vdim / 4;  // four columns a thread
   for (int idx = tid; idx < rows_here * quads; idx += 32 * kWarps) {
     const int r = idx / quads, col = 4 * (idx - r * quads), tile = r / (16 * MT), in = r % (16 * MT);
-    const int rr = r0 + r, i = rr / gsz, head = g * gsz + rr - i * gsz;
-    const long long t = t0 + i;
-    const TQ* gt = static_cast<const TQ*>(a.gate) + t * a.ldg + (a.gate_per_head ? head : head * a.vdim + col);
+    const Row where(a, r0 + r, gsz, g, t0);
     float gv[4];
-    if (a.nsplit == 1 && a.gate != nullptr) {
-#pragma unroll
-      for (int y = 0; y < 4; ++y) gv[y] = ldf(gt + (a.gate_per_head ? 0 : y));
-    }
+    if (a.nsplit == 1) gates<TQ>(a, where, col, gv);
     float m = -INFINITY;
     for (int w = 0; w < wk; ++w) m = fmaxf(m, stat[w * wr + tile][in].x);
-    float acc[4] = {0.f, 0.f, 0.f, 0.f}, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
     const float ref = m == -INFINITY ? 0.f : m;
     for (int w = 0; w < wk; ++w) {
       const int ww = w * wr + tile;
@@ -711,33 +747,55 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
       float f = ex2(st.x - ref);
       l += f * st.y;  // (scores that are no numbers stay in the sum)
       if (K::C8) f *= exp2f(top_power[ww] - 142.f);  // the weights' power: 2^(P - 127 - 15)
-      if (f != 0.f) {
-        const float4 v = *reinterpret_cast<const float4*>(os + (ww * 16 * MT + in) * ldo_s + col);
-        acc[0] += f * v.x, acc[1] += f * v.y, acc[2] += f * v.z, acc[3] += f * v.w;
-      }
+      if (f != 0.f) add(acc, f, *reinterpret_cast<const float4*>(os + (ww * 16 * MT + in) * ldo_s + col));
     }
     if (a.nsplit == 1) {
-      if (!a.sx.logistic && a.sx.sink != nullptr) {
-        const float sk = a.sx.sink[head] * kLog2e, mm = fmaxf(ref, sk), f = ex2(ref - mm);
-#pragma unroll
-        for (int y = 0; y < 4; ++y) acc[y] *= f;
-        l = l * f + ex2(sk - mm);
-      }
-      TQ* dst = static_cast<TQ*>(a.out) + t * ldo + (long long)head * a.vdim + col;
-      const float inv = a.sx.logistic ? 1.f : l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: zeros
-#pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        float v = acc[y] * inv * oscale;
-        if (a.gate != nullptr) v /= 1.0f + expf(-gv[y]);
-        stf(dst + y, v);
-      }
+      finish<TQ>(a, where, col, ref, l, acc, gv);
+    } else if (a.cluster) {  // over the first warp's, whose columns only this thread reads
+      *reinterpret_cast<float4*>(os + (tile * 16 * MT + in) * ldo_s + col) = acc;
+      if (col == 0) joined[r] = make_float2(m, l);
     } else {
-      const long long row = (a.singles ? (long long)e : t) * a.H + head;
-      float* pp = a.partial + (row * a.nsplit + split) * (a.vdim + 4);
-      *reinterpret_cast<float4*>(pp + 4 + col) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      float* pp = a.partial + (((a.singles ? (long long)e : where.t) * a.H + where.head) * a.nsplit + split) * (a.vdim + 4);
+      *reinterpret_cast<float4*>(pp + 4 + col) = acc;
       if (col == 0) *reinterpret_cast<float2*>(pp) = make_float2(m, l);
     }
   }
+  if (!a.cluster) return;
+  // ---- the CTAs of a cluster share out the rows' columns and read one another's results
+  pg::cluster_sync_all();
+  for (int idx = tid + 32 * kWarps * split; idx < rows_here * quads; idx += 32 * kWarps * a.nsplit) {
+    const int r = idx / quads, col = 4 * (idx - r * quads), tile = r / (16 * MT), in = r % (16 * MT);
+    const Row where(a, r0 + r, gsz, g, t0);
+    float gv[4];
+    gates<TQ>(a, where, col, gv);
+    const uint32_t sa = pg::smem_u32(&joined[r]), oa = pg::smem_u32(os + (tile * 16 * MT + in) * ldo_s + col);
+    float2 st[8];
+    float4 v[8];
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      if (p >= a.nsplit) break;
+      uint32_t x, y;
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(x) : "r"(sa), "r"(p));
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(y) : "r"(oa), "r"(p));
+      asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(st[p].x), "=f"(st[p].y) : "r"(x) : "memory");
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[p].x), "=f"(v[p].y), "=f"(v[p].z), "=f"(v[p].w) : "r"(y) : "memory");
+    }
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int p = 0; p < 8; ++p)
+      if (p < a.nsplit) m = fmaxf(m, st[p].x);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      if (p >= a.nsplit) break;
+      const float f = ex2(st[p].x - ref);
+      l += f * st[p].y;
+      if (f != 0.f) add(acc, f, v[p]);
+    }
+    finish<TQ>(a, where, col, ref, l, acc, gv);
+  }
+  pg::cluster_sync_all();  // nobody leaves while its memory is read
 }
 
 // A CTA a row: its warps take every fourth split, four columns a lane (vdim <= 128), the first splits' values requested before their factors are known.
@@ -768,16 +826,9 @@ __global__ void __launch_bounds__(128) attn_rows_merge_kernel(const __grid_const
     float l = fx * x.y + fy * y.y;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    float fix = 1.f;
-    if (!a.sx.logistic && a.sx.sink != nullptr) {
-      const float sk = a.sx.sink[head] * kLog2e, mm = fmaxf(ref, sk);
-      fix = ex2(ref - mm);
-      l = l * fix + ex2(sk - mm);
-    }
-    const float oscale = a.sx.out_scale != 0.f ? a.sx.out_scale : 1.f;
     fs[lane] = fx;
     fs[lane + 32] = fy;
-    if (lane == 0) whole[0] = (a.sx.logistic ? 1.f : l == 0.f ? 0.f : fix / l) * oscale;
+    if (lane == 0) whole[0] = ref, whole[1] = l;
   }
   __syncthreads();
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -787,47 +838,73 @@ __global__ void __launch_bounds__(128) attn_rows_merge_kernel(const __grid_const
       const int s = warp + 4 * k;
       if (s >= a.nsplit) break;
       const float f = fs[s];
-      if (f == 0.f) continue;  // (a split without keys left zeros)
-      const float4 v = k < AHEAD ? ahead[k % AHEAD] : *reinterpret_cast<const float4*>(pp + s * ld + 4 + col);
-      acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
+      if (f != 0.f) add(acc, f, k < AHEAD ? ahead[k % AHEAD] : *reinterpret_cast<const float4*>(pp + s * ld + 4 + col));  // (a split without keys left zeros)
     }
   }
   sums[warp][lane] = acc;
   __syncthreads();
   if (warp == 0 && col < a.vdim) {
-    float v[4] = {acc.x, acc.y, acc.z, acc.w};
 #pragma unroll
-    for (int w = 1; w < 4; ++w) {
-      const float4 x = sums[w][lane];
-      v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
-    }
-    const long long ldo = a.sx.out_ld > 0 ? a.sx.out_ld : (long long)a.H * a.vdim;
-    TQ* dst = static_cast<TQ*>(a.out) + t * ldo + (long long)head * a.vdim + col;
-    const TQ* gt = static_cast<const TQ*>(a.gate) + t * a.ldg + (a.gate_per_head ? head : head * a.vdim + col);
-#pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      float z = v[y] * whole[0];
-      if (a.gate != nullptr) z /= 1.0f + expf(-ldf(gt + (a.gate_per_head ? 0 : y)));
-      stf(dst + y, z);
-    }
+    for (int w = 1; w < 4; ++w) add(acc, 1.f, sums[w][lane]);
+    Row where(a, 0, 1, 0, t);
+    where.head = head;
+    float gv[4];
+    gates<TQ>(a, where, col, gv);
+    finish<TQ>(a, where, col, whole[0], whole[1], acc, gv);
   }
 }
 
-template <typename TQ, typename TC, int DC, int VC, int MT, int KT>
-int launch(Args a, int entries, int max_n, cudaStream_t st) {
+// What the host decides: rows a warp, CTAs a walk.
+struct Plan {
+  int wr, blocks, nsplit, cluster;
+};
+Plan plan_of(const PgAttnRows& p, int rows, int row_tile, int keys, int per_sm) {
+  Plan x;
+  x.wr = 1;
+  while (x.wr < kWarps && x.wr * row_tile < rows) x.wr *= 2;
+  x.blocks = (rows + x.wr * row_tile - 1) / (x.wr * row_tile);
+  long long reach = p.longest;
+  if (p.score != nullptr && p.score->window > 0) {
+    const long long w = (long long)p.score->window + (p.score->keep_first > 0 ? p.score->keep_first : 0) + p.max_n + 2 * keys;
+    reach = reach < w ? reach : w;
+  }
+  const long long tiles = (reach + keys - 1) / keys, ctas = (long long)p.busy * p.G * x.blocks;
+  // CTAs that share a walk: what the SMs hold at once, and at least PG_ROWS_TILES tiles for a warp
+#ifndef PG_ROWS_TILES
+#define PG_ROWS_TILES 2
+#endif
+  long long n = (long long)per_sm * pg::num_sms() / (ctas > 0 ? ctas : 1);
+  const long long most = tiles * x.wr / (PG_ROWS_TILES * kWarps);
+  n = n < most ? n : most;
+  n = n > 64 ? 64 : n < 1 ? 1 : n;
+  // up to eight join through distributed shared memory in one launch; more, where that leaves warps with a long walk, through global memory and a second one
+  x.cluster = n <= 8 || most <= 12;
+  n = x.cluster && n > 8 ? 8 : n;
+  if (n == 1) x.cluster = 0;
+  x.nsplit = (int)n;
+  return x;
+}
+
+// need: the scratch that the call asks for, nothing is launched; NULL: launches
+template <typename TQ, typename TC, int DC, int VC, int MT, int KT, bool R8>
+int launch(const PgAttnRows& p, Args a, long long* need, long long scratch_bytes, cudaStream_t st) {
   using K = Kind<TQ, TC, DC, VC, MT, KT>;
-  const int rows = max_n * (a.H / a.G);
-  int wr = 1;
-  while (wr < kWarps && wr * 16 * MT < rows) wr *= 2;
-  a.wr = wr;
-  a.blocks = (rows + wr * 16 * MT - 1) / (wr * 16 * MT);
+  const int max_n = p.singles ? 1 : p.max_n;
+  const Plan plan = plan_of(p, max_n * (a.H / a.G), 16 * MT, KT, ctas_per_sm<TQ, TC, DC, VC, MT>());
+  const long long bytes = plan.nsplit > 1 && !plan.cluster ? 4LL * (p.singles ? p.entries : p.rows) * a.H * plan.nsplit * (a.vdim + 4) : 0;
+  if (need != nullptr) {
+    *need = bytes;
+    return PG_OK;
+  }
+  if (bytes > 0 && (a.partial == nullptr || scratch_bytes < bytes || (reinterpret_cast<uintptr_t>(a.partial) & 15) != 0)) return PG_ERR_ARG;
+  a.wr = plan.wr, a.blocks = plan.blocks, a.nsplit = plan.nsplit, a.cluster = plan.cluster;
   a.tile_shift = 0;
   while ((KT << a.tile_shift) < a.page) ++a.tile_shift;
   constexpr size_t kRing = (size_t)kWarps * K::STAGES * K::STAGE;
-  const size_t in = (size_t)wr * K::Q_BYTES + kRing, out = (size_t)kWarps * 16 * MT * (a.vdim + 4) * 4;
+  const size_t in = (size_t)a.wr * K::Q_BYTES + kRing, out = (size_t)kWarps * 16 * MT * (a.vdim + 4) * 4;
   const size_t smem = in > out ? in : out;
   if ((long long)a.blocks * a.G > 65535) return PG_ERR_ARG;
-  auto kern = attn_rows_kernel<TQ, TC, DC, VC, MT, KT>;
+  auto kern = attn_rows_kernel<TQ, TC, DC, VC, MT, KT, R8>;
   constexpr size_t kOut = (size_t)kWarps * 16 * MT * (64 * VC + 4) * 4, kIn = (size_t)kWarps * K::Q_BYTES + kRing, kMost = kIn > kOut ? kIn : kOut;
   static_assert(kMost <= 220 * 1024, "shared memory of a block");
   static bool configured[pg::kMaxDevices] = {};  // once a device, to the most that any call asks for
@@ -839,64 +916,84 @@ int launch(Args a, int entries, int max_n, cudaStream_t st) {
     }
     done = true;
   }
-  if (pg::launch_kernel(kern, dim3(a.nsplit, a.G * a.blocks, entries), dim3(32 * kWarps), smem, st, a) != cudaSuccess) return PG_ERR_CUDA;
-  if (a.nsplit > 1 && pg::launch_kernel(attn_rows_merge_kernel<TQ>, dim3(a.H, a.singles ? 1 : max_n, entries), dim3(128), 0, st, a) != cudaSuccess) return PG_ERR_CUDA;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(a.nsplit, a.G * a.blocks, p.entries);
+  cfg.blockDim = dim3(32 * kWarps);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (a.cluster) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = a.nsplit;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (pg_pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  pg_count_launch(1);
+  if (cudaLaunchKernelEx(&cfg, kern, a) != cudaSuccess) return PG_ERR_CUDA;
+  if (bytes > 0 && pg::launch_kernel(attn_rows_merge_kernel<TQ>, dim3(a.H, max_n, p.entries), dim3(128), 0, st, a) != cudaSuccess) return PG_ERR_CUDA;
   return PG_OK;
 }
 
-template <typename TQ, typename TC, int MT, int KT>
-int by_size(const Args& a, int entries, int max_n, cudaStream_t st) {
-  if (a.dim <= 64 && a.vdim <= 64) return launch<TQ, TC, 1, 1, MT, KT>(a, entries, max_n, st);
+template <typename TQ, typename TC, int MT, int KT, bool R8>
+int by_size(const PgAttnRows& p, const Args& a, long long* need, long long scratch_bytes, cudaStream_t st) {
+  if (a.dim <= 64 && a.vdim <= 64) return launch<TQ, TC, 1, 1, MT, KT, R8>(p, a, need, scratch_bytes, st);
   constexpr int kWide = sizeof(TC) == 1 && MT == 1 ? KT : 16;
-  return launch<TQ, TC, 2, 2, MT, kWide>(a, entries, max_n, st);
+  return launch<TQ, TC, 2, 2, MT, kWide, R8>(p, a, need, scratch_bytes, st);
+}
+template <typename TQ, typename TC, int KT>
+int by_rows(const PgAttnRows& p, const Args& a, long long* need, long long scratch_bytes, cudaStream_t st) {
+  const int rows = (p.singles ? 1 : p.max_n) * (p.H / p.G);
+  if (rows <= 8) return by_size<TQ, TC, 1, KT, true>(p, a, need, scratch_bytes, st);
+  // 32 rows a warp read a tile once where there are CTAs enough; else 16, for a shorter chain (one tree of 8 x 4 rows over 1100 keys: 20 / 16 us)
+  if (rows <= 16 || sizeof(TQ) == 4 || (long long)p.busy * p.G * 2 < pg::num_sms()) return by_size<TQ, TC, 1, KT, false>(p, a, need, scratch_bytes, st);
+  return by_size<TQ, TC, sizeof(TQ) == 4 ? 1 : 2, KT, false>(p, a, need, scratch_bytes, st);
 }
 
 bool aligned(const void* p, int n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-}  // namespace
-
-extern "C" long long pg_attn_rows_scratch(int rows, int H, int vdim, int nsplit) { return nsplit > 1 ? 4LL * rows * H * nsplit * (vdim + 4) : 0; }
-
-extern "C" int pg_attn_rows(const void* q, const PgKvPages* kv, const void* gate, long long ldg, void* out, float* partial, const int* entry_row0, const int* entry_n,
-                            const int* entry_ctx, const int* page_table, int max_pages, int page, const int* pos, const void* tree, int tree_words, int entries, int max_n,
-                            int singles, int nsplit, int H, int G, int dim, int vdim, float scale, float softcap, int act_f32, int gate_per_head, const PgAttnScore* score,
-                            void* stream) {
-  if (kv == nullptr || entries <= 0 || entries > 65535 || max_n <= 0 || nsplit <= 0 || nsplit > 64 || max_n > 65535 || H <= 0 || G <= 0 || H % G != 0 || dim <= 0 || vdim <= 0 || max_pages <= 0)
+int attn_rows(const PgAttnRows* q, long long* need, void* scratch, long long scratch_bytes, void* stream) {
+  if (q == nullptr) return PG_ERR_ARG;
+  const PgAttnRows& p = *q;
+  if (p.entries <= 0 || p.entries > 65535 || p.rows <= 0 || p.max_n <= 0 || p.max_n > 65535 || p.H <= 0 || p.G <= 0 || p.H % p.G != 0 || p.H > 65535 || p.dim <= 0 || p.vdim <= 0 ||
+      p.max_pages <= 0 || p.longest <= 0)
     return PG_ERR_ARG;
-  if (page < 32 || (page & (page - 1)) != 0 || dim > 128 || vdim > 128 || (tree != nullptr && tree_words <= 0) || (nsplit > 1 && partial == nullptr)) return PG_ERR_ARG;
-  const int unit = kv->e4m3 ? 16 : act_f32 ? 4 : 8;  // elements of a 16-byte piece
-  if (dim % unit != 0 || vdim % 8 != 0 || ((long long)G * dim) % unit != 0 || !aligned(kv->k, 16) || !aligned(kv->v, 16)) return PG_ERR_ARG;
-  if (kv->e4m3 && (kv->k_powers == nullptr || kv->v_powers == nullptr || !aligned(kv->k_powers, 16) || !aligned(kv->v_powers, 16))) return PG_ERR_ARG;
-  if (!kv->e4m3 && kv->f32 != act_f32) return PG_ERR_ARG;
-  if (nsplit > 1 && !aligned(partial, 16)) return PG_ERR_ARG;
-  if (score != nullptr && ((score->dist_a == nullptr) != (score->dist_b == nullptr))) return PG_ERR_ARG;
-  if (pos == nullptr && score != nullptr && (score->window > 0 || score->dist_a != nullptr)) return PG_ERR_ARG;
+  if (p.page < 32 || (p.page & (p.page - 1)) != 0 || p.dim > 128 || p.vdim > 128 || (p.tree != nullptr && p.tree_words <= 0)) return PG_ERR_ARG;
+  const int unit = p.e4m3 ? 16 : p.act_f32 ? 4 : 8;  // elements of a 16-byte piece
+  if (p.dim % unit != 0 || p.vdim % (p.e4m3 ? 16 : 8) != 0 || !aligned(p.k, 16) || !aligned(p.v, 16)) return PG_ERR_ARG;
+  if (p.e4m3 && (p.k_powers == nullptr || p.v_powers == nullptr || !aligned(p.k_powers, 16) || !aligned(p.v_powers, 16))) return PG_ERR_ARG;
+  const PgAttnScore* sx = p.score;
+  if (sx != nullptr && ((sx->dist_a == nullptr) != (sx->dist_b == nullptr))) return PG_ERR_ARG;
+  if (p.pos == nullptr && sx != nullptr && (sx->window > 0 || sx->dist_a != nullptr)) return PG_ERR_ARG;
   Args a{};
-  a.q = q;
-  a.kp = static_cast<const uint8_t*>(kv->k), a.vp = static_cast<const uint8_t*>(kv->v);
-  a.ke = static_cast<const uint8_t*>(kv->k_powers), a.ve = static_cast<const uint8_t*>(kv->v_powers);
-  a.gate = gate, a.ldg = ldg, a.out = out, a.partial = partial;
-  a.row0 = entry_row0, a.n = entry_n, a.ctx = entry_ctx, a.pt = page_table, a.pos = pos, a.tree = static_cast<const uint32_t*>(tree);
-  a.words = tree_words, a.max_pages = max_pages, a.page = page, a.singles = singles, a.nsplit = nsplit, a.H = H, a.G = G, a.dim = dim, a.vdim = vdim;
-  a.scale = scale, a.softcap = softcap, a.gate_per_head = gate_per_head;
-  a.sx = score != nullptr ? *score : PgAttnScore{};
-  a.mode = a.sx.dist_a != nullptr || a.sx.logistic ? kGeneral : softcap > 0.f ? kCapped : kPlain;
+  a.q = p.q;
+  a.kp = static_cast<const uint8_t*>(p.k), a.vp = static_cast<const uint8_t*>(p.v);
+  a.ke = static_cast<const uint8_t*>(p.k_powers), a.ve = static_cast<const uint8_t*>(p.v_powers);
+  a.gate = p.gate, a.ldg = p.ldg, a.out = p.out, a.partial = static_cast<float*>(scratch);
+  a.row0 = p.entry_row0, a.n = p.entry_n, a.ctx = p.entry_ctx, a.pt = p.page_table, a.pos = p.pos, a.tree = static_cast<const uint32_t*>(p.tree);
+  a.words = p.tree_words, a.max_pages = p.max_pages, a.page = p.page, a.singles = p.singles, a.H = p.H, a.G = p.G, a.dim = p.dim, a.vdim = p.vdim;
+  a.scale = p.scale, a.softcap = p.softcap, a.gate_per_head = p.gate_per_head;
+  a.sx = sx != nullptr ? *sx : PgAttnScore{};
+  a.mode = a.sx.dist_a != nullptr || a.sx.logistic ? kGeneral : p.softcap > 0.f ? kCapped : kPlain;
   a.trigger = pg::weights_follow();
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const int most = singles ? 1 : max_n, rows = most * (H / G);
-#ifndef KTE
-#define KTE 32
-#endif
-#ifdef ONLY8
-  if (kv->e4m3) {
-    return rows <= 16 ? by_size<bf16, e4m3, 1, KTE>(a, entries, most, st) : by_size<bf16, e4m3, 2, KTE>(a, entries, most, st);
-  }
-  return -1;
-#endif
-  if (kv->e4m3) {
-    if (act_f32) return by_size<float, e4m3, 1, 32>(a, entries, most, st);
-    return rows <= 16 ? by_size<bf16, e4m3, 1, 32>(a, entries, most, st) : by_size<bf16, e4m3, 2, 32>(a, entries, most, st);
-  }
-  if (act_f32) return by_size<float, float, 1, 16>(a, entries, most, st);
-  return rows <= 16 ? by_size<bf16, bf16, 1, 32>(a, entries, most, st) : by_size<bf16, bf16, 2, 32>(a, entries, most, st);
+  if (p.e4m3) return p.act_f32 ? by_rows<float, e4m3, 32>(p, a, need, scratch_bytes, st) : by_rows<bf16, e4m3, 32>(p, a, need, scratch_bytes, st);
+  return p.act_f32 ? by_rows<float, float, 16>(p, a, need, scratch_bytes, st) : by_rows<bf16, bf16, 32>(p, a, need, scratch_bytes, st);
 }
+
+}  // namespace
+
+extern "C" long long pg_attn_rows_scratch(const PgAttnRows* p) {
+  long long need = 0;
+  const int rc = attn_rows(p, &need, nullptr, 0, nullptr);
+  return rc == PG_OK ? need : rc;
+}
+
+extern "C" int pg_attn_rows(const PgAttnRows* p, void* scratch, long long scratch_bytes, void* stream) { return attn_rows(p, nullptr, scratch, scratch_bytes, stream); }

@@ -442,20 +442,20 @@ class QuantizedPages:
     2^(byte - 127), uint8 [pages, heads, page] -- the least that takes the head's largest finite element to 448 or below.  An element is code * power; what
     is not finite is kept as NaN.  `attn_prepare` writes them, `attn_ragged` and `attn_tree` read them, `kv_read` gives rows back in an activation type."""
 
+    __slots__ = ("codes", "powers", "pages", "page", "heads", "size")
+
     def __init__(self, codes: torch.Tensor, powers: torch.Tensor):
         if codes.dtype != torch.uint8 or powers.dtype != torch.uint8 or codes.dim() != 3 or powers.dim() != 3:
             raise ValueError("8-bit pages are uint8 codes [pages, page, heads * size] and uint8 powers [pages, heads, page]")
-        if powers.shape[0] != codes.shape[0] or powers.shape[2] != codes.shape[1] or codes.shape[2] % powers.shape[1] or not (codes.is_contiguous() and powers.is_contiguous()):
+        pages, page, width = codes.shape
+        pages2, heads, page2 = powers.shape
+        if pages != pages2 or page != page2 or heads < 1 or width % heads or not (codes.is_contiguous() and powers.is_contiguous()):
             raise ValueError(f"8-bit pages that do not belong together: codes {tuple(codes.shape)}, powers {tuple(powers.shape)}")
-        self.codes, self.powers = codes, powers
+        self.codes, self.powers, self.pages, self.page, self.heads, self.size = codes, powers, pages, page, heads, width // heads
 
     @classmethod
     def empty(cls, pages: int, page: int, heads: int, size: int, device="cuda"):
         return cls(torch.zeros(pages, page, heads * size, device=device, dtype=torch.uint8), torch.zeros(pages, heads, page, device=device, dtype=torch.uint8))
-
-    @property
-    def heads(self):
-        return self.powers.shape[1]
 
 
 def _check_quantized(k: "QuantizedPages", v: "QuantizedPages", G, dim, vdim, page):
@@ -463,9 +463,8 @@ def _check_quantized(k: "QuantizedPages", v: "QuantizedPages", G, dim, vdim, pag
         raise ValueError("keys and values are kept in one form: both in 8 bits or neither")
     if dim % 16 or vdim % 16 or dim > 256 or vdim > 256:
         raise ValueError(f"the 8-bit cache keeps heads of a multiple of 16 elements up to 256: got {dim} and {vdim}")
-    for x, size in ((k, dim), (v, vdim)):
-        if x.heads != G or x.codes.shape[2] != G * size or x.codes.shape[1] != page:
-            raise ValueError(f"8-bit pages of {x.heads} heads, {x.codes.shape[2]} elements and {x.codes.shape[1]} rows for {G} heads of {size} and pages of {page}")
+    if k.heads != G or v.heads != G or k.size != dim or v.size != vdim or k.page != page or v.page != page:
+        raise ValueError(f"8-bit pages of {k.heads} / {v.heads} heads of {k.size} / {v.size} and {k.page} / {v.page} rows for {G} heads of {dim} / {vdim} and pages of {page}")
 
 
 def kv_read(k_pages: "QuantizedPages", v_pages: "QuantizedPages", b: StepBatch, dtype: torch.dtype):
@@ -475,8 +474,7 @@ def kv_read(k_pages: "QuantizedPages", v_pages: "QuantizedPages", b: StepBatch, 
         raise ValueError("kv_read reads 8-bit pages")
     if dtype not in (torch.bfloat16, torch.float32):
         raise ValueError("rows come back as torch.bfloat16 or torch.float32")
-    G, page = k_pages.heads, k_pages.codes.shape[1]
-    dim, vdim = k_pages.codes.shape[2] // G, v_pages.codes.shape[2] // G
+    G, page, dim, vdim = k_pages.heads, k_pages.page, k_pages.size, v_pages.size
     _check_quantized(k_pages, v_pages, G, dim, vdim, page)
     k = torch.empty(b.dense_rows, G * dim, device=k_pages.codes.device, dtype=dtype)
     v = torch.empty(b.dense_rows, G * vdim, device=k_pages.codes.device, dtype=dtype)
@@ -600,38 +598,23 @@ def attn_ragged(q, k_pages, v_pages, gate, out, b: StepBatch, H, G, dim, vdim, s
                    "pg_attn_decode")
 
 
-def _rows_split(entries, G, rows, tiles, wide, row_tile):
-    """CTAs that share an entry's keys: what two CTAs an SM hold at once, and at least two key tiles for every warp."""
-    warps = 1  # of a CTA that hold rows; the others share the key walk
-    while warps < 4 and warps * row_tile < rows:
-        warps *= 2
-    ctas = entries * G * -(-rows // (warps * row_tile))
-    import os
-    return max(1, min(int(os.environ.get('TGT', 2)) * _lib.num_sms() // ctas, tiles // (int(os.environ.get('TPW', 2)) * (4 // warps)), 64))
-
-
 def _attn_rows(q, k_pages, v_pages, gate, out, b: StepBatch, H, G, dim, vdim, scale, softcap, page, gate_per_head, score, singles):
-    import ctypes as C
-    quantized, f32 = isinstance(k_pages, QuantizedPages), int(q.dtype == torch.float32)
     if dim > 128 or vdim > 128:
         raise ValueError(f"attention of a few rows takes heads of up to 128 elements: got {dim} and {vdim}")
-    rows = (1 if singles else b.max_n) * (H // G)
-    row_tile = 32 if rows > 16 and not f32 else 16
-    wide = dim > 64 or vdim > 64
-    keys = 32 if quantized or not (f32 or wide) else 16
-    context = b.max_single_ctx + 1 if singles else max(b.max_single_ctx + 1, b.dense_max_len)
-    reach = context if score is None or not score.window else min(context, score.window + score.keep_first + b.max_n + 2 * keys)
-    nsplit = _rows_split(b.singles if singles else b.E, G, rows, -(-reach // keys), wide, row_tile)
-    L = _lib.lib()
-    need = L.pg_attn_rows_scratch(b.E if singles else b.T, H, vdim, nsplit)
-    partial = torch.empty(need // 4, device=q.device, dtype=torch.float32) if need else None
-    kv = _lib.KvPages(k_pages.codes.data_ptr(), v_pages.codes.data_ptr(), k_pages.powers.data_ptr(), v_pages.powers.data_ptr(), 1, 0) if quantized else \
-        _lib.KvPages(k_pages.data_ptr(), v_pages.data_ptr(), 0, 0, 0, f32)
+    import ctypes as C
+    quantized = isinstance(k_pages, QuantizedPages)
     tree = None if singles else b.tree
-    _lib.check(L.pg_attn_rows(q.data_ptr(), C.addressof(kv), _lib.ptr(gate), 0 if gate is None else gate.stride(0), out.data_ptr(), _lib.ptr(partial), b.row0.data_ptr(),
-                              b.n.data_ptr(), b.ctx.data_ptr(), b.page_table.data_ptr(), b.max_pages, page, b.pos.data_ptr(), _lib.ptr(tree),
-                              0 if tree is None else tree.shape[1], b.E, b.max_n, int(singles), nsplit, H, G, dim, vdim, float(scale), float(softcap or 0.0), f32,
-                              int(bool(gate_per_head)), C.addressof(score.c) if score is not None else 0, _lib.stream()), "pg_attn_rows")
+    kv = ((k_pages.codes.data_ptr(), v_pages.codes.data_ptr(), k_pages.powers.data_ptr(), v_pages.powers.data_ptr()) if quantized else
+          (k_pages.data_ptr(), v_pages.data_ptr(), 0, 0))
+    a = _lib.ATTN_ROWS.pack(q.data_ptr(), *kv, 0 if gate is None else gate.data_ptr(), 0 if gate is None else gate.stride(0), out.data_ptr(), b.row0.data_ptr(), b.n.data_ptr(),
+                            b.ctx.data_ptr(), b.page_table.data_ptr(), b.pos.data_ptr(), 0 if tree is None else tree.data_ptr(), 0 if score is None else C.addressof(score.c),
+                            b.max_pages, page, 0 if tree is None else tree.shape[1], b.E, b.T, b.max_n, b.singles if singles else b.E,
+                            b.max_single_ctx + 1 if singles else max(b.max_single_ctx + 1, b.dense_max_len), singles, H, G, dim, vdim, q.dtype == torch.float32, quantized,
+                            bool(gate_per_head), scale, softcap or 0.0)
+    L = _lib.lib()
+    need = L.pg_attn_rows_scratch(a)
+    scratch = torch.empty(need, device=q.device, dtype=torch.uint8) if need > 0 else None
+    _lib.check(L.pg_attn_rows(a, 0 if scratch is None else scratch.data_ptr(), need, _lib.stream()), "pg_attn_rows")
 
 
 def attn_tree(q, k_pages, v_pages, gate, out, b: StepBatch, H, G, dim, vdim, scale, softcap, page, gate_per_head=False, score: Optional["ScoreOptions"] = None):
@@ -668,10 +651,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, tem
     if not 0.0 < float(temperature) < float("inf"):
         raise ValueError("the temperature is positive and finite")
     top = int(top)
-    f = torch.empty(rows * (2 + top), device=logits.device, dtype=torch.float32)
-    i = torch.empty(rows * (1 + top), device=logits.device, dtype=torch.int32)
-    lp, entropy, top_lp = f[:rows], f[rows:2 * rows], f[2 * rows:].view(rows, top)
-    rank, ids = i[:rows], i[rows:].view(rows, top)
+    lp, entropy, top_lp, rank, ids = logits.new_empty(rows), logits.new_empty(rows), logits.new_empty((rows, top)), tokens.new_empty(rows), tokens.new_empty((rows, top))
     if rows:
         _lib.check(_lib.lib().pg_token_logprobs(logits.data_ptr(), logits.stride(0) if rows > 1 else V, tokens.data_ptr(), lp.data_ptr(), entropy.data_ptr(), rank.data_ptr(), ids.data_ptr(),
                                                 top_lp.data_ptr(), rows, V, top, float(temperature), _lib.stream()), "pg_token_logprobs")
