@@ -19,10 +19,8 @@ __device__ __forceinline__ uint32_t finite_magnitude(float x) {
   const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
   return b < 0x7f800000u ? b : 0u;
 }
-// two codes, a in the low byte: to the nearest, ties to even
+// two codes, a in the low byte: to the nearest, ties to even; NaN is kept, infinities are not for this (they would become 448)
 __device__ __forceinline__ uint32_t codes_of(float a, float b) {
-  a = fabsf(a) < INFINITY ? a : __uint_as_float(0x7fffffffu);
-  b = fabsf(b) < INFINITY ? b : __uint_as_float(0x7fffffffu);
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
   return r;

@@ -69,32 +69,40 @@ struct Prepare {
   float v_mix;
 };
 
-// A group of LG lanes holds a head vector, eight elements a lane; its mean square and its largest element are butterflies inside the group.  A CTA takes TOK tokens: the cosines
-// and sines (angles in double) are made once for all heads behind the requests of the first vectors; DEEP vectors of a group are under way together.
-// What bounds it: for prompts the bytes (the row is read once, 8-bit rows are half of bf16 ones); for a few rows the chain row -> sum -> largest -> codes.
+// A group of LG lanes holds a head vector, eight elements a lane; its mean square and its largest element are butterflies inside the group.  A CTA takes TOK tokens, whose cosines
+// and sines (angles in double) are made once for all heads behind the first vectors' requests; four vectors of a group are under way together: one head of four tokens,
+// which share its weights, or four heads of one token.
+// What bounds it: for prompts instructions, then the bytes (a row is read once, 8-bit rows are half of bf16 ones); for a few rows the chain row -> sum -> largest -> codes.
 template <typename TA, int LG, int TOK, bool VEC>
 __global__ void __launch_bounds__(128) attn_prepare_e4m3_kernel(const __grid_constant__ Prepare a) {
-  constexpr int DEEP = sizeof(TA) == 2 ? 4 : 2, NG = 128 / LG;
+  constexpr int U = 4, NG = 128 / LG, HEADS = TOK == 1 ? U : 1;  // HEADS: head vectors of a round
   extern __shared__ __align__(16) float cs[];  // [TOK][cos rot / 2 | sin rot / 2]
   __shared__ float part[2][TOK][4];
-  pg::griddep_begin();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, l = tid % LG, group = tid / LG;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, l = tid % LG, group = tid / LG, d0 = 8 * l;
   const int t0 = blockIdx.x * TOK, nvec = a.H + 2 * a.G, half = a.rot / 2;
-  const int total = min(TOK, a.rows - t0) * nvec;
   const TA* qkv = static_cast<const TA*>(a.qkv);
-  auto offset = [&](int vec) {
-    return vec < a.H + a.G ? (long long)vec * a.dim : a.v_from_k ? (long long)(vec - a.G) * a.dim : (long long)(a.H + a.G) * a.dim + (long long)(vec - a.H - a.G) * a.vdim;
-  };
-  Eight<TA> raw[DEEP];
-  auto request = [&](Eight<TA>& r, int item) {
-    r.zero();
-    if (item < total) {
-      const int k = item / nvec, vec = item - k * nvec;
-      if (8 * l < (vec < a.H + a.G ? a.dim : a.vdim)) r.template load<VEC>(qkv + (t0 + k) * a.ld + offset(vec) + 8 * l);
+  long long kv_row[TOK], power_row[TOK];  // the token's row of codes, its byte of a page's first head
+#pragma unroll
+  for (int k = 0; k < TOK; ++k) {  // (positions and pages are the host's)
+    const int t = min(t0 + k, a.rows - 1), where = a.at[t], slot = where % a.page;
+    const long long page = a.page_table[(long long)a.row_entry[t] * a.max_pages + where / a.page];
+    kv_row[k] = page * a.page + slot;
+    power_row[k] = page * a.G * a.page + slot;
+  }
+  pg::griddep_begin();
+  Eight<TA> raw[U];
+  auto request = [&](int vec0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int vec = TOK == 1 ? vec0 + u * NG : vec0, t = min(t0 + (TOK == 1 ? 0 : u), a.rows - 1);
+      raw[u].zero();
+      if (vec < nvec && d0 < (vec < a.H + a.G ? a.dim : a.vdim)) {
+        const long long off = vec < a.H + a.G ? vec * a.dim : a.v_from_k ? (vec - a.G) * a.dim : (a.H + a.G) * a.dim + (vec - a.H - a.G) * a.vdim;
+        raw[u].template load<VEC>(qkv + t * a.ld + off + d0);
+      }
     }
   };
-#pragma unroll
-  for (int d = 0; d < DEEP; ++d) request(raw[d], group + d * NG);
+  request(group);
   for (int i = tid; i < TOK * half; i += 128) {
     const int k = i / half, j = i - k * half;
     double s, c;
@@ -116,77 +124,107 @@ __global__ void __launch_bounds__(128) attn_prepare_e4m3_kernel(const __grid_con
     }
   }
   __syncthreads();
-  const int rounds = (total + NG * DEEP - 1) / (NG * DEEP);
-#pragma unroll 1
-  for (int r = 0; r < rounds; ++r) {
+  const bool turn8 = a.rot % 8 == 0 && half % 4 == 0;  // a lane's four pairs turn or do not, and lie on 16 bytes
+  for (int vec0 = group; vec0 - group < nvec; vec0 += HEADS * NG) {
+    float v[U][8];
 #pragma unroll
-    for (int d = 0; d < DEEP; ++d) {
-      const int item = group + (r * DEEP + d) * NG;
-      const bool in = item < total;
-      const int k = in ? item / nvec : 0, vec = in ? item - k * nvec : 0;
+    for (int u = 0; u < U; ++u) raw[u].get(v[u]);
+    request(vec0 + HEADS * NG);
+#pragma unroll
+    for (int h = 0; h < HEADS; ++h) {
+      const int vec = vec0 + h * NG;
       const bool is_q = vec < a.H, is_k = !is_q && vec < a.H + a.G, is_v = !is_q && !is_k;
-      const int n = is_v ? a.vdim : a.dim, head = is_q ? vec : is_k ? vec - a.H : vec - a.H - a.G, d0 = 8 * l;
-      const bool mine = in && d0 < n;
-      const long long t = t0 + k;
-      float v[8];
-      raw[d].get(v);
-      request(raw[d], item + NG * DEEP);
-      float inv = 1.0f;
-      if (a.norm_qk == 1 || a.norm_v) {  // (uniform: every lane takes part in the exchange)
-        float s = 0.f;
+      const int n = is_v ? a.vdim : a.dim, head = is_q ? vec : is_k ? vec - a.H : vec - a.H - a.G;
+      const bool mine = vec < nvec && d0 < n;
+      float w[8];
+      const float* wp = is_v ? nullptr : is_q ? a.qn : a.kn;  // NULL: a norm without a weight
+      if (wp != nullptr && mine) {
+        wp += a.norm_qk == 2 ? head * a.dim + d0 : d0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s = fmaf(v[i], v[i], s);
-#pragma unroll
-        for (int o = LG / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (is_v ? a.norm_v != 0 : a.norm_qk == 1) inv = 1.0f / sqrtf(s / (float)n + a.eps);
-      }
-      if (a.norm_qk == 2 && !is_v) {
-        const float* p = part[is_q ? 0 : 1][k];
-        inv = 1.0f / sqrtf((p[0] + p[1] + p[2] + p[3]) / (float)((is_q ? a.H : a.G) * a.dim) + a.eps);
+        for (int i = 0; i < 8; ++i) w[i] = wp[i];
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] *= inv;
-      if (mine) {
-        const float* w = is_v ? nullptr : is_q ? a.qn : a.kn;  // NULL: a norm without a weight
-        if (w != nullptr) {
-          w += a.norm_qk == 2 ? head * a.dim + d0 : d0;
+      for (int k = 0; k < TOK; ++k) {
+        const int u = TOK == 1 ? h : k;
+        const long long t = t0 + k;
+        float(&x)[8] = v[u];
+        float inv = 1.0f;
+        if (a.norm_qk == 1 || a.norm_v) {  // (uniform: every lane takes part in the exchange)
+          float s = 0.f;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] *= w[i];
+          for (int i = 0; i < 8; ++i) s = fmaf(x[i], x[i], s);
+#pragma unroll
+          for (int o = LG / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+          if (is_v ? a.norm_v != 0 : a.norm_qk == 1) inv = rsqrtf(s * (1.0f / (float)n) + a.eps);
         }
-        if (!is_v && d0 < a.rot) {
-          const float* ck = cs + k * a.rot + d0 / 2;
+        if (a.norm_qk == 2 && !is_v) {
+          const float* p = part[is_q ? 0 : 1][k];
+          inv = rsqrtf((p[0] + p[1] + p[2] + p[3]) / (float)((is_q ? a.H : a.G) * a.dim) + a.eps);
+        }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (d0 + 2 * i >= a.rot) break;
-            const float c = ck[i], s = ck[half + i], x = v[2 * i], y = v[2 * i + 1];
-            v[2 * i] = x * c - y * s;
-            v[2 * i + 1] = y * c + x * s;
+        for (int i = 0; i < 8; ++i) x[i] *= inv;
+        if (mine) {
+          if (wp != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] *= w[i];
+          }
+          if (!is_v && d0 < a.rot) {
+            const float* ck = cs + k * a.rot + d0 / 2;
+            float cv[4], sv[4];
+            if (turn8) {
+              const float4 c4 = *reinterpret_cast<const float4*>(ck), s4 = *reinterpret_cast<const float4*>(ck + half);
+              cv[0] = c4.x, cv[1] = c4.y, cv[2] = c4.z, cv[3] = c4.w;
+              sv[0] = s4.x, sv[1] = s4.y, sv[2] = s4.z, sv[3] = s4.w;
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const bool turns = d0 + 2 * i < a.rot;
+                cv[i] = turns ? ck[i] : 1.f;
+                sv[i] = turns ? ck[half + i] : 0.f;
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float y = x[2 * i], z = x[2 * i + 1];
+              x[2 * i] = y * cv[i] - z * sv[i];
+              x[2 * i + 1] = z * cv[i] + y * sv[i];
+            }
+          }
+          if (is_v && a.v_other != nullptr && t < a.rows) {
+            const TA* o = static_cast<const TA*>(a.v_other) + t * a.ldvo + (long long)head * a.vdim + d0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = (1.0f - a.v_mix) * x[i] + a.v_mix * ldf(o + i);
           }
         }
-        if (is_v && a.v_other != nullptr) {
-          const TA* o = static_cast<const TA*>(a.v_other) + t * a.ldvo + (long long)head * a.vdim + d0;
+        float top = 0.f;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = (1.0f - a.v_mix) * v[i] + a.v_mix * ldf(o + i);
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));  // (passes over NaN)
+#pragma unroll
+        for (int o = LG / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (__any_sync(0xffffffffu, top == INFINITY)) {  // only finite elements count, infinities are kept as NaN
+          uint32_t most = 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) most = max(most, cache8::finite_magnitude(x[i]));
+#pragma unroll
+          for (int o = LG / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+          top = __uint_as_float(most);
+          if (!is_q) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = fabsf(x[i]) < INFINITY ? x[i] : __uint_as_float(0x7fffffffu);
+          }
         }
-      }
-      uint32_t top = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, cache8::finite_magnitude(v[i]));
-#pragma unroll
-      for (int o = LG / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      if (!mine) continue;
-      if (is_q) {
-        put8(static_cast<TA*>(a.q_out) + (t * a.H + head) * a.dim + d0, v);
-      } else {
-        const int where = a.at[t], slot = where % a.page;
-        const long long pg_id = a.page_table[(long long)a.row_entry[t] * a.max_pages + where / a.page];
-        const uint32_t byte = cache8::power_of(top);
-        const float up = cache8::inverse_of_power(byte);
-        uint2 codes;
-        codes.x = cache8::codes_of(v[0] * up, v[1] * up) | cache8::codes_of(v[2] * up, v[3] * up) << 16;
-        codes.y = cache8::codes_of(v[4] * up, v[5] * up) | cache8::codes_of(v[6] * up, v[7] * up) << 16;
-        *reinterpret_cast<uint2*>((is_k ? a.kc : a.vc) + ((pg_id * a.page + slot) * a.G + head) * n + d0) = codes;
-        if (l == 0) (is_k ? a.ke : a.ve)[(pg_id * a.G + head) * a.page + slot] = static_cast<uint8_t>(byte);
+        if (!mine || t >= a.rows) continue;
+        if (is_q) {
+          put8(static_cast<TA*>(a.q_out) + (t * a.H + head) * a.dim + d0, x);
+        } else {
+          const uint32_t byte = cache8::power_of(__float_as_uint(top));
+          const float up = cache8::inverse_of_power(byte);
+          uint2 codes;
+          codes.x = cache8::codes_of(x[0] * up, x[1] * up) | cache8::codes_of(x[2] * up, x[3] * up) << 16;
+          codes.y = cache8::codes_of(x[4] * up, x[5] * up) | cache8::codes_of(x[6] * up, x[7] * up) << 16;
+          *reinterpret_cast<uint2*>((is_k ? a.kc : a.vc) + (kv_row[k] * a.G + head) * n + d0) = codes;
+          if (l == 0) (is_k ? a.ke : a.ve)[power_row[k] + head * a.page] = static_cast<uint8_t>(byte);
+        }
       }
     }
   }
