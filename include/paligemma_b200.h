@@ -520,13 +520,26 @@ int pg_attn_prepare_at(const void* qkv, long long ld, const int* pos, const int*
  * pg_attn_prepare_e4m3: pg_attn_prepare_at into such pages.  dim and vdim multiples of 16 up to 256; codes and q_out on 16-byte boundaries.
  * pg_kv_read_e4m3: rows 0 .. ctx + n of every entry with entry_n > 1, in fp32 (out_f32) or bf16, to rows dense_row0[e] .. of k_out [.., G * dim] and
  * v_out [.., G * vdim]; zeros behind the last row up to a multiple of 64 rows.  longest: at least the largest ctx + n among them (sizes the grid). */
-int pg_attn_prepare_e4m3(const void* qkv, long long ld, const int* pos, const int* at, const int* row_entry, const int* page_table, int max_pages, int page,
-                         const double* freq, const float* q_norm, const float* k_norm, void* q_out, void* k_codes, void* k_powers, void* v_codes,
-                         void* v_powers, int rows, int H, int G, int dim, int vdim, int rot_dims, float eps, int norm_qk, int norm_v, int v_from_k,
-                         float rot_gain, const void* v_other, long long ld_v_other, float v_mix, int act_f32, void* stream);
-int pg_kv_read_e4m3(const void* k_codes, const void* k_powers, const void* v_codes, const void* v_powers, const int* page_table, int max_pages, int page,
-                    const int* dense_row0, const int* entry_n, const int* entry_ctx, void* k_out, void* v_out, int entries, int longest, int G, int dim,
-                    int vdim, int out_f32, void* stream);
+typedef struct PgPrepareE4m3 { /* as pg_attn_prepare_at's arguments */
+  const void* qkv;
+  long long ld;
+  const int *pos, *at, *row_entry, *page_table;
+  const double* freq;
+  const float *q_norm, *k_norm;
+  void *q_out, *k_codes, *k_powers, *v_codes, *v_powers;
+  const void* v_other;
+  long long ld_v_other;
+  int max_pages, page, rows, H, G, dim, vdim, rot, norm_qk, norm_v, v_from_k, act_f32;
+  float eps, rot_gain, v_mix;
+} PgPrepareE4m3;
+int pg_attn_prepare_e4m3(const PgPrepareE4m3* a, void* stream);
+typedef struct PgReadE4m3 {
+  const void *k_codes, *k_powers, *v_codes, *v_powers;
+  const int *page_table, *dense_row0, *entry_n, *entry_ctx;
+  void *k_out, *v_out;
+  int max_pages, page, entries, longest, G, dim, vdim, out_f32;
+} PgReadE4m3;
+int pg_kv_read_e4m3(const PgReadE4m3* a, void* stream);
 
 /* Attention of a few rows an entry: every row of an entry sees the stored keys 0 .. ctx - 1 and, of the entry's own n rows (cache rows ctx ..), those whose bit
  * is set in its mask: tree uint32 [rows, tree_words], bit m % 32 of word m / 32 (bits from n on are ignored; NULL: rows up to itself).  A row that sees nothing gets

@@ -88,8 +88,8 @@ SIGNATURES = {
     "pg_side_gate": [p, i64, p, p, i64, i32, p, i64, i32, i32, i32, i32, p],
     "pg_attn_prepare": [p, i64, p, p, p, i32, i32, p, p, p, p, p, p, i32, i32, i32, i32, i32, i32, f32, i32, i32, i32, f32, p, i64, f32, i32, p],
     "pg_attn_prepare_at": [p, i64, p, p, p, p, i32, i32, p, p, p, p, p, p, i32, i32, i32, i32, i32, i32, f32, i32, i32, i32, f32, p, i64, f32, i32, p],
-    "pg_attn_prepare_e4m3": [p, i64, p, p, p, p, i32, i32, p, p, p, p, p, p, p, p, i32, i32, i32, i32, i32, i32, f32, i32, i32, i32, f32, p, i64, f32, i32, p],
-    "pg_kv_read_e4m3": [p, p, p, p, p, i32, i32, p, p, p, p, p, i32, i32, i32, i32, i32, i32, p],
+    "pg_attn_prepare_e4m3": [p, p],
+    "pg_kv_read_e4m3": [p, p],
     "pg_attn_rows_scratch": [p],
     "pg_attn_rows": [p, p, i64, p],
     "pg_token_logprobs": [p, i64, p, p, p, p, p, p, i32, i32, i32, f32, p],
@@ -147,8 +147,10 @@ class AttnScore(C.Structure):
                 ("head_bias", p), ("out_scale", f32), ("out_ld", i64)]
 
 
-# Mirror of PgAttnRows, packed in one go (thirty-three conversions one by one: 2.6 us of a call, 0.3 this way)
+# Mirrors of PgAttnRows, PgPrepareE4m3 and PgReadE4m3, packed in one go (thirty conversions one by one: 2.6 us of a call, 0.3 this way)
 ATTN_ROWS = struct.Struct("@6Pq8P16i2f")
+PREPARE_E4M3 = struct.Struct("@Pq13Pq12i3f4x")
+READ_E4M3 = struct.Struct("@10P8i")
 
 
 class RoutedFf(C.Structure):

@@ -27,6 +27,8 @@ using bf16 = __nv_bfloat16;
 
 namespace {
 
+static_assert(sizeof(PgAttnRows) == 192, "callers pack this struct by its size");
+
 constexpr int kWarps = 4;
 constexpr float kLog2e = 1.4426950408889634f;
 struct e4m3 {

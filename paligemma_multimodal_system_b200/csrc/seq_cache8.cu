@@ -51,30 +51,26 @@ __device__ __forceinline__ void put8(bf16* p, const float (&v)[8]) {
   *reinterpret_cast<uint4*>(p) = make_uint4(pg::pack_bf16(v[0], v[1]), pg::pack_bf16(v[2], v[3]), pg::pack_bf16(v[4], v[5]), pg::pack_bf16(v[6], v[7]));
 }
 
-struct Prepare {
-  const void* qkv;
-  long long ld;
-  const int *pos, *at, *row_entry, *page_table;
-  int max_pages, page;
-  const double* freq;
-  const float *qn, *kn;
-  void* q_out;
-  uint8_t *kc, *ke, *vc, *ve;
-  int rows, H, G, dim, vdim, rot;
-  float eps;
-  int norm_qk, norm_v, v_from_k;
-  float rot_gain;
-  const void* v_other;
-  long long ldvo;
-  float v_mix;
-};
+// sine and cosine of an angle in double, to fp32: whole turns go in double, the rest as a sum of two floats (a library sincos in double took a third of the kernel's time)
+__device__ __forceinline__ void sine_of(double angle, float& s, float& c) {
+  const double turns = rint(angle * 0.15915494309189535);
+  const double rest = fma(-turns, 2.4492935982947064e-16, fma(-turns, 6.283185307179586, angle));
+  const float hi = (float)rest, lo = (float)(rest - (double)hi);
+  float s0, c0;
+  sincosf(hi, &s0, &c0);
+  s = fmaf(c0, lo, s0);
+  c = fmaf(-s0, lo, c0);
+}
+
+using Prepare = PgPrepareE4m3;
+static_assert(sizeof(PgPrepareE4m3) == 192 && sizeof(PgReadE4m3) == 112, "callers pack these structs by their sizes");
 
 // A group of LG lanes holds a head vector, eight elements a lane; its mean square and its largest element are butterflies inside the group.  A CTA takes TOK tokens, whose cosines
 // and sines (angles in double) are made once for all heads behind the first vectors' requests; four vectors of a group are under way together: one head of four tokens,
 // which share its weights, or four heads of one token.
 // What bounds it: for prompts instructions, then the bytes (a row is read once, 8-bit rows are half of bf16 ones); for a few rows the chain row -> sum -> largest -> codes.
 template <typename TA, int LG, int TOK, bool VEC>
-__global__ void __launch_bounds__(128) attn_prepare_e4m3_kernel(const __grid_constant__ Prepare a) {
+__global__ void __launch_bounds__(128, sizeof(TA) == 2 ? 8 : 5) attn_prepare_e4m3_kernel(const __grid_constant__ Prepare a) {
   constexpr int U = 4, NG = 128 / LG, HEADS = TOK == 1 ? U : 1;  // HEADS: head vectors of a round
   extern __shared__ __align__(16) float cs[];  // [TOK][cos rot / 2 | sin rot / 2]
   __shared__ float part[2][TOK][4];
@@ -105,10 +101,10 @@ __global__ void __launch_bounds__(128) attn_prepare_e4m3_kernel(const __grid_con
   request(group);
   for (int i = tid; i < TOK * half; i += 128) {
     const int k = i / half, j = i - k * half;
-    double s, c;
-    sincos((double)a.pos[min(t0 + k, a.rows - 1)] * a.freq[j], &s, &c);
-    cs[k * a.rot + j] = a.rot_gain * (float)c;
-    cs[k * a.rot + half + j] = a.rot_gain * (float)s;
+    float s, c;
+    sine_of((double)a.pos[min(t0 + k, a.rows - 1)] * a.freq[j], s, c);
+    cs[k * a.rot + j] = a.rot_gain * c;
+    cs[k * a.rot + half + j] = a.rot_gain * s;
   }
   if (a.norm_qk == 2) {  // one root mean square for all of q, one for all of k
     const int nq = a.H * a.dim, nk = a.G * a.dim;
@@ -126,18 +122,18 @@ __global__ void __launch_bounds__(128) attn_prepare_e4m3_kernel(const __grid_con
   __syncthreads();
   const bool turn8 = a.rot % 8 == 0 && half % 4 == 0;  // a lane's four pairs turn or do not, and lie on 16 bytes
   for (int vec0 = group; vec0 - group < nvec; vec0 += HEADS * NG) {
-    float v[U][8];
+    Eight<TA> now[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) raw[u].get(v[u]);
+    for (int u = 0; u < U; ++u) now[u] = raw[u];
     request(vec0 + HEADS * NG);
 #pragma unroll
     for (int h = 0; h < HEADS; ++h) {
       const int vec = vec0 + h * NG;
       const bool is_q = vec < a.H, is_k = !is_q && vec < a.H + a.G, is_v = !is_q && !is_k;
       const int n = is_v ? a.vdim : a.dim, head = is_q ? vec : is_k ? vec - a.H : vec - a.H - a.G;
-      const bool mine = vec < nvec && d0 < n;
+      const bool mine = vec < nvec && d0 < n, quantised = __any_sync(0xffffffffu, !is_q);  // a group of this warp has a key or a value
       float w[8];
-      const float* wp = is_v ? nullptr : is_q ? a.qn : a.kn;  // NULL: a norm without a weight
+      const float* wp = is_v ? nullptr : is_q ? a.q_norm : a.k_norm;  // NULL: a norm without a weight
       if (wp != nullptr && mine) {
         wp += a.norm_qk == 2 ? head * a.dim + d0 : d0;
 #pragma unroll
@@ -147,7 +143,8 @@ __global__ void __launch_bounds__(128) attn_prepare_e4m3_kernel(const __grid_con
       for (int k = 0; k < TOK; ++k) {
         const int u = TOK == 1 ? h : k;
         const long long t = t0 + k;
-        float(&x)[8] = v[u];
+        float x[8];
+        now[u].get(x);
         float inv = 1.0f;
         if (a.norm_qk == 1 || a.norm_v) {  // (uniform: every lane takes part in the exchange)
           float s = 0.f;
@@ -191,17 +188,19 @@ __global__ void __launch_bounds__(128) attn_prepare_e4m3_kernel(const __grid_con
             }
           }
           if (is_v && a.v_other != nullptr && t < a.rows) {
-            const TA* o = static_cast<const TA*>(a.v_other) + t * a.ldvo + (long long)head * a.vdim + d0;
+            const TA* o = static_cast<const TA*>(a.v_other) + t * a.ld_v_other + (long long)head * a.vdim + d0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = (1.0f - a.v_mix) * x[i] + a.v_mix * ldf(o + i);
           }
         }
         float top = 0.f;
+        if (quantised) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));  // (passes over NaN)
+          for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));  // (passes over NaN)
 #pragma unroll
-        for (int o = LG / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (__any_sync(0xffffffffu, top == INFINITY)) {  // only finite elements count, infinities are kept as NaN
+          for (int o = LG / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        }
+        if (quantised && __any_sync(0xffffffffu, top == INFINITY)) {  // only finite elements count, infinities are kept as NaN
           uint32_t most = 0;
 #pragma unroll
           for (int i = 0; i < 8; ++i) most = max(most, cache8::finite_magnitude(x[i]));
@@ -222,8 +221,8 @@ __global__ void __launch_bounds__(128) attn_prepare_e4m3_kernel(const __grid_con
           uint2 codes;
           codes.x = cache8::codes_of(x[0] * up, x[1] * up) | cache8::codes_of(x[2] * up, x[3] * up) << 16;
           codes.y = cache8::codes_of(x[4] * up, x[5] * up) | cache8::codes_of(x[6] * up, x[7] * up) << 16;
-          *reinterpret_cast<uint2*>((is_k ? a.kc : a.vc) + (kv_row[k] * a.G + head) * n + d0) = codes;
-          if (l == 0) (is_k ? a.ke : a.ve)[power_row[k] + head * a.page] = static_cast<uint8_t>(byte);
+          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(is_k ? a.k_codes : a.v_codes) + (kv_row[k] * a.G + head) * n + d0) = codes;
+          if (l == 0) static_cast<uint8_t*>(is_k ? a.k_powers : a.v_powers)[power_row[k] + head * a.page] = static_cast<uint8_t>(byte);
         }
       }
     }
@@ -233,34 +232,32 @@ __global__ void __launch_bounds__(128) attn_prepare_e4m3_kernel(const __grid_con
 // 16 codes a thread and step.  Rows behind an entry's last one up to the end of its last page are zeros: whoever walks whole tiles of the scratch reads numbers.
 constexpr int kReadRows = 16;
 template <typename TO>
-__global__ void __launch_bounds__(256) kv_read_e4m3_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ ke, const uint8_t* __restrict__ vc, const uint8_t* __restrict__ ve,
-                                                           const int* __restrict__ page_table, int max_pages, int page, const int* __restrict__ dense_row0,
-                                                           const int* __restrict__ entry_n, const int* __restrict__ entry_ctx, TO* __restrict__ k_out, TO* __restrict__ v_out,
-                                                           int G, int dim, int vdim) {
-  pg::griddep_begin();
-  const int e = blockIdx.y, n = entry_n[e], len = entry_ctx[e] + n, j0 = blockIdx.x * kReadRows;
+__global__ void __launch_bounds__(256) kv_read_e4m3_kernel(const __grid_constant__ PgReadE4m3 a) {
+  const int e = blockIdx.y, n = a.entry_n[e], len = a.entry_ctx[e] + n, j0 = blockIdx.x * kReadRows;
   const int end = (len + 63) / 64 * 64;  // the scratch has whole runs of 64 rows
   if (n <= 1 || j0 >= end) return;
   const bool is_k = blockIdx.z == 0;
-  const int size = is_k ? dim : vdim, pieces = G * size / 16, per_head = size / 16;
-  const uint8_t* codes = is_k ? kc : vc;
-  const uint8_t* powers = is_k ? ke : ve;
-  TO* out = (is_k ? k_out : v_out) + (dense_row0[e] + (long long)j0) * G * size;
+  const int size = is_k ? a.dim : a.vdim, pieces = a.G * size / 16, per_head = size / 16;
+  const uint8_t* codes = static_cast<const uint8_t*>(is_k ? a.k_codes : a.v_codes);
+  const uint8_t* powers = static_cast<const uint8_t*>(is_k ? a.k_powers : a.v_powers);
+  TO* out = static_cast<TO*>(is_k ? a.k_out : a.v_out) + (a.dense_row0[e] + (long long)j0) * a.G * size;
+  const int* pages = a.page_table + (long long)e * a.max_pages;
   const int rows = min(kReadRows, end - j0);
+  pg::griddep_begin();
 #pragma unroll 4
   for (int i = threadIdx.x; i < rows * pieces; i += 256) {
     const int r = i / pieces, p = i - r * pieces, j = j0 + r, head = p / per_head;
     uint4 c = make_uint4(0, 0, 0, 0);
     uint32_t byte = 127;
     if (j < len) {
-      const long long pg_id = page_table[(long long)e * max_pages + j / page];
-      const int slot = j % page;
-      c = *reinterpret_cast<const uint4*>(codes + (pg_id * page + slot) * G * size + 16 * p);
-      byte = powers[(pg_id * G + head) * page + slot];
+      const long long id = pages[j / a.page];
+      const int slot = j % a.page;
+      c = *reinterpret_cast<const uint4*>(codes + (id * a.page + slot) * a.G * size + 16 * p);
+      byte = powers[(id * a.G + head) * a.page + slot];
     }
     const float s = cache8::value_of_power(byte);
     const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-    TO* dst = out + (long long)r * G * size + 16 * p;
+    TO* dst = out + (long long)r * a.G * size + 16 * p;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float v[8];
@@ -280,18 +277,17 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 }  // namespace
 
-extern "C" int pg_attn_prepare_e4m3(const void* qkv, long long ld, const int* pos, const int* at, const int* row_entry, const int* page_table, int max_pages, int page,
-                                    const double* freq, const float* q_norm, const float* k_norm, void* q_out, void* k_codes, void* k_powers, void* v_codes, void* v_powers, int rows,
-                                    int H, int G, int dim, int vdim, int rot_dims, float eps, int norm_qk, int norm_v, int v_from_k, float rot_gain, const void* v_other,
-                                    long long ld_v_other, float v_mix, int act_f32, void* stream) {
-  if (rows <= 0 || H <= 0 || G <= 0 || dim <= 0 || vdim <= 0 || rot_dims < 0 || rot_dims > dim || (rot_dims & 1) || page <= 0 || max_pages <= 0) return PG_ERR_ARG;
-  if (dim % 16 != 0 || vdim % 16 != 0 || dim > 256 || vdim > 256 || (v_from_k && vdim != dim) || norm_qk < 0 || norm_qk > 2) return PG_ERR_ARG;
-  if (!aligned16(q_out) || !aligned16(k_codes) || !aligned16(v_codes) || k_codes == nullptr || v_codes == nullptr || k_powers == nullptr || v_powers == nullptr) return PG_ERR_ARG;
-  const Prepare a{qkv, ld, pos, at != nullptr ? at : pos, row_entry, page_table, max_pages, page, freq, q_norm, k_norm, q_out, static_cast<uint8_t*>(k_codes),
-                  static_cast<uint8_t*>(k_powers), static_cast<uint8_t*>(v_codes), static_cast<uint8_t*>(v_powers), rows, H, G, dim, vdim, rot_dims, eps, norm_qk, norm_v, v_from_k,
-                  rot_gain, v_other, ld_v_other, v_mix};
-  const int lanes = (dim > vdim ? dim : vdim) / 8;
-  const bool vec = aligned16(qkv) && ld % (act_f32 ? 4 : 8) == 0;
+extern "C" int pg_attn_prepare_e4m3(const PgPrepareE4m3* args, void* stream) {
+  if (args == nullptr) return PG_ERR_ARG;
+  Prepare a = *args;
+  if (a.rows <= 0 || a.H <= 0 || a.G <= 0 || a.dim <= 0 || a.vdim <= 0 || a.rot < 0 || a.rot > a.dim || (a.rot & 1) || a.page <= 0 || a.max_pages <= 0) return PG_ERR_ARG;
+  if (a.dim % 16 != 0 || a.vdim % 16 != 0 || a.dim > 256 || a.vdim > 256 || (a.v_from_k && a.vdim != a.dim) || a.norm_qk < 0 || a.norm_qk > 2) return PG_ERR_ARG;
+  if (!aligned16(a.q_out) || !aligned16(a.k_codes) || !aligned16(a.v_codes) || a.k_codes == nullptr || a.v_codes == nullptr || a.k_powers == nullptr || a.v_powers == nullptr)
+    return PG_ERR_ARG;
+  if (a.at == nullptr) a.at = a.pos;
+  const int rows = a.rows, rot_dims = a.rot, act_f32 = a.act_f32;
+  const int lanes = (a.dim > a.vdim ? a.dim : a.vdim) / 8;
+  const bool vec = aligned16(a.qkv) && a.ld % (act_f32 ? 4 : 8) == 0;
   const bool four = rows >= 16 * pg::num_sms();  // four tokens a CTA once that still fills the SMs
   pg_count_launch(1);
   cudaError_t rc;
@@ -313,18 +309,14 @@ extern "C" int pg_attn_prepare_e4m3(const void* qkv, long long ld, const int* po
   return rc == cudaSuccess ? PG_OK : PG_ERR_CUDA;
 }
 
-extern "C" int pg_kv_read_e4m3(const void* k_codes, const void* k_powers, const void* v_codes, const void* v_powers, const int* page_table, int max_pages, int page,
-                               const int* dense_row0, const int* entry_n, const int* entry_ctx, void* k_out, void* v_out, int entries, int longest, int G, int dim, int vdim,
-                               int out_f32, void* stream) {
-  if (entries <= 0 || entries > 65535 || longest <= 0 || G <= 0 || dim <= 0 || vdim <= 0 || dim % 16 != 0 || vdim % 16 != 0 || page <= 0 || max_pages <= 0) return PG_ERR_ARG;
-  if (!aligned16(k_codes) || !aligned16(v_codes) || !aligned16(k_out) || !aligned16(v_out)) return PG_ERR_ARG;
-  const dim3 grid(((longest + 63) / 64 * 64 + kReadRows - 1) / kReadRows, entries, 2);
-  auto go = [&](auto kern, auto t) {
-    using TO = decltype(t);
-    return pg::launch_kernel(kern, grid, dim3(256), 0, reinterpret_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(k_codes), static_cast<const uint8_t*>(k_powers),
-                             static_cast<const uint8_t*>(v_codes), static_cast<const uint8_t*>(v_powers), page_table, max_pages, page, dense_row0, entry_n, entry_ctx,
-                             static_cast<TO*>(k_out), static_cast<TO*>(v_out), G, dim, vdim);
-  };
-  const cudaError_t rc = out_f32 ? go(kv_read_e4m3_kernel<float>, float()) : go(kv_read_e4m3_kernel<bf16>, bf16());
+extern "C" int pg_kv_read_e4m3(const PgReadE4m3* args, void* stream) {
+  if (args == nullptr) return PG_ERR_ARG;
+  const PgReadE4m3& a = *args;
+  if (a.entries <= 0 || a.entries > 65535 || a.longest <= 0 || a.G <= 0 || a.dim <= 0 || a.vdim <= 0 || a.dim % 16 != 0 || a.vdim % 16 != 0 || a.page <= 0 || a.max_pages <= 0)
+    return PG_ERR_ARG;
+  if (!aligned16(a.k_codes) || !aligned16(a.v_codes) || !aligned16(a.k_out) || !aligned16(a.v_out)) return PG_ERR_ARG;
+  const dim3 grid(((a.longest + 63) / 64 * 64 + kReadRows - 1) / kReadRows, a.entries, 2);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const cudaError_t rc = a.out_f32 ? pg::launch_kernel(kv_read_e4m3_kernel<float>, grid, dim3(256), 0, st, a) : pg::launch_kernel(kv_read_e4m3_kernel<bf16>, grid, dim3(256), 0, st, a);
   return rc == cudaSuccess ? PG_OK : PG_ERR_CUDA;
 }

@@ -421,19 +421,20 @@ def attn_prepare(qkv, b: StepBatch, freq, q_norm, k_norm, q_out, k_pages, v_page
     assert v_other is None or (v_other.dtype == qkv.dtype and v_other.stride(1) == 1 and v_other.shape == (b.T, G * vdim))
     assert qkv.stride(1) == 1 and freq.dtype == torch.float64 and qkv.dtype == q_out.dtype and (k_pages is None) == (v_pages is None)
     mode = 2 if norm_qk is NORM_PROJECTION else int(bool(norm_qk))
-    tail = (b.T, H, G, dim, vdim, rot_dims, float(eps), mode, int(bool(norm_v)), int(bool(v_from_k)), float(rot_gain), _lib.ptr(v_other),
-            0 if v_other is None else v_other.stride(0), float(v_mix), int(qkv.dtype == torch.float32), _lib.stream())
     if isinstance(k_pages, QuantizedPages):
         _check_quantized(k_pages, v_pages, G, dim, vdim, page)
         assert q_out.is_contiguous()
-        _lib.check(_lib.lib().pg_attn_prepare_e4m3(qkv.data_ptr(), qkv.stride(0), b.pos.data_ptr(), _lib.ptr(b.at), b.row_entry.data_ptr(), b.page_table.data_ptr(),
-                                                   b.max_pages, page, freq.data_ptr(), _lib.ptr(q_norm), _lib.ptr(k_norm), q_out.data_ptr(), k_pages.codes.data_ptr(),
-                                                   k_pages.powers.data_ptr(), v_pages.codes.data_ptr(), v_pages.powers.data_ptr(), *tail), "pg_attn_prepare_e4m3")
+        a = _lib.PREPARE_E4M3.pack(qkv.data_ptr(), qkv.stride(0), b.pos.data_ptr(), _lib.ptr(b.at), b.row_entry.data_ptr(), b.page_table.data_ptr(), freq.data_ptr(),
+                                   _lib.ptr(q_norm), _lib.ptr(k_norm), q_out.data_ptr(), k_pages.codes.data_ptr(), k_pages.powers.data_ptr(), v_pages.codes.data_ptr(),
+                                   v_pages.powers.data_ptr(), _lib.ptr(v_other), 0 if v_other is None else v_other.stride(0), b.max_pages, page, b.T, H, G, dim, vdim, rot_dims,
+                                   mode, bool(norm_v), bool(v_from_k), qkv.dtype == torch.float32, eps, rot_gain, v_mix)
+        _lib.check(_lib.lib().pg_attn_prepare_e4m3(a, _lib.stream()), "pg_attn_prepare_e4m3")
         return
     assert k_pages is None or k_pages.dtype == qkv.dtype
     _lib.check(_lib.lib().pg_attn_prepare_at(qkv.data_ptr(), qkv.stride(0), b.pos.data_ptr(), _lib.ptr(b.at), b.row_entry.data_ptr(), b.page_table.data_ptr(),
-                                             b.max_pages, page, freq.data_ptr(), _lib.ptr(q_norm), _lib.ptr(k_norm), q_out.data_ptr(),
-                                             _lib.ptr(k_pages), _lib.ptr(v_pages), *tail), "pg_attn_prepare_at")
+                                             b.max_pages, page, freq.data_ptr(), _lib.ptr(q_norm), _lib.ptr(k_norm), q_out.data_ptr(), _lib.ptr(k_pages), _lib.ptr(v_pages),
+                                             b.T, H, G, dim, vdim, rot_dims, float(eps), mode, int(bool(norm_v)), int(bool(v_from_k)), float(rot_gain), _lib.ptr(v_other),
+                                             0 if v_other is None else v_other.stride(0), float(v_mix), int(qkv.dtype == torch.float32), _lib.stream()), "pg_attn_prepare_at")
 
 
 # ---- the 8-bit cache -------------------------------------------------------------------------------------------------
@@ -479,9 +480,10 @@ def kv_read(k_pages: "QuantizedPages", v_pages: "QuantizedPages", b: StepBatch, 
     k = torch.empty(b.dense_rows, G * dim, device=k_pages.codes.device, dtype=dtype)
     v = torch.empty(b.dense_rows, G * vdim, device=k_pages.codes.device, dtype=dtype)
     if b.dense_rows:
-        _lib.check(_lib.lib().pg_kv_read_e4m3(k_pages.codes.data_ptr(), k_pages.powers.data_ptr(), v_pages.codes.data_ptr(), v_pages.powers.data_ptr(), b.page_table.data_ptr(),
-                                              b.max_pages, page, b.dense_row0.data_ptr(), b.n.data_ptr(), b.ctx.data_ptr(), k.data_ptr(), v.data_ptr(), b.E, b.dense_max_len,
-                                              G, dim, vdim, int(dtype == torch.float32), _lib.stream()), "pg_kv_read_e4m3")
+        a = _lib.READ_E4M3.pack(k_pages.codes.data_ptr(), k_pages.powers.data_ptr(), v_pages.codes.data_ptr(), v_pages.powers.data_ptr(), b.page_table.data_ptr(),
+                                b.dense_row0.data_ptr(), b.n.data_ptr(), b.ctx.data_ptr(), k.data_ptr(), v.data_ptr(), b.max_pages, page, b.E, b.dense_max_len, G, dim, vdim,
+                                dtype == torch.float32)
+        _lib.check(_lib.lib().pg_kv_read_e4m3(a, _lib.stream()), "pg_kv_read_e4m3")
     return k, v
 
 
