@@ -50,7 +50,7 @@ struct Args {
   const uint32_t* tree;
   int words, max_pages, page, tile_shift, singles, nsplit, cluster, blocks, H, G, dim, vdim, wr, mode;  // tile_shift: log2 of a page's tiles
   float scale, softcap;
-  int gate_per_head;
+  int gate_per_head, vec_q, vec_gate, vec_out;  // vec_*: four elements in one piece
   PgAttnScore sx;
   int trigger;
 };
@@ -69,9 +69,43 @@ __device__ __forceinline__ float tanh_f32(float x) {
 }
 __device__ __forceinline__ float ldf(const float* p) { return *p; }
 __device__ __forceinline__ float ldf(const bf16* p) { return __bfloat162float(*p); }
-__device__ __forceinline__ void stf(float* p, float v) { *p = v; }
-__device__ __forceinline__ void stf(bf16* p, float v) { *p = __float2bfloat16_rn(v); }
 
+// four neighbouring elements; vec: they lie on a boundary of their own size
+__device__ __forceinline__ void ld4(float (&v)[4], const float* p, bool vec) {
+  if (vec) {
+    const float4 f = *reinterpret_cast<const float4*>(p);
+    v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = p[i];
+  }
+}
+__device__ __forceinline__ void ld4(float (&v)[4], const bf16* p, bool vec) {
+  uint2 u;
+  if (vec) {
+    u = *reinterpret_cast<const uint2*>(p);
+  } else {
+    const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
+    u = make_uint2(e[0] | static_cast<uint32_t>(e[1]) << 16, e[2] | static_cast<uint32_t>(e[3]) << 16);
+  }
+  v[0] = __uint_as_float(u.x << 16), v[1] = __uint_as_float(u.x & 0xffff0000u), v[2] = __uint_as_float(u.y << 16), v[3] = __uint_as_float(u.y & 0xffff0000u);
+}
+__device__ __forceinline__ void st4(float* p, const float (&v)[4], bool vec) {
+  if (vec) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = v[i];
+  }
+}
+__device__ __forceinline__ void st4(bf16* p, const float (&v)[4], bool vec) {
+  if (vec) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pg::pack_bf16(v[0], v[1]), pg::pack_bf16(v[2], v[3]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = __float2bfloat16_rn(v[i]);
+  }
+}
 __device__ __forceinline__ float rcp(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -110,8 +144,13 @@ __device__ __forceinline__ void terms(float lo, float hi, uint32_t (&t)[N]) {
   }
 }
 
-struct Yes { static constexpr bool value = true; };
-struct No { static constexpr bool value = false; };
+// the elements of a word that are infinite or NaN, as a mask
+template <int ES>
+__device__ __forceinline__ uint32_t no_numbers(uint32_t w) {
+  if (ES == 1) return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu);
+  if (ES == 2) return __vcmpeq2(w & 0x7f807f80u, 0x7f807f80u);
+  return (w & 0x7f800000u) == 0x7f800000u ? 0xffffffffu : 0u;
+}
 
 template <typename TQ, typename TC, int DC, int VC, int MT, int KT>
 struct Kind {
@@ -159,8 +198,8 @@ template <typename TQ>
 __device__ __forceinline__ void gates(const Args& a, const Row& r, int col, float (&gv)[4]) {
   if (a.gate == nullptr) return;
   const TQ* g = static_cast<const TQ*>(a.gate) + r.t * a.ldg + (a.gate_per_head ? r.head : r.head * a.vdim + col);
-#pragma unroll
-  for (int y = 0; y < 4; ++y) gv[y] = ldf(g + (a.gate_per_head ? 0 : y));
+  if (a.gate_per_head) gv[0] = gv[1] = gv[2] = gv[3] = ldf(g);
+  else ld4(gv, g, a.vec_gate);
 }
 // four columns of a row from its sums: sink, division, gate.  A row that sees nothing: zeros.
 template <typename TQ>
@@ -173,9 +212,41 @@ __device__ __forceinline__ void finish(const Args& a, const Row& r, int col, flo
   }
   by *= (a.sx.logistic ? 1.f : l == 0.f ? 0.f : 1.f / l) * (a.sx.out_scale != 0.f ? a.sx.out_scale : 1.f);
   TQ* dst = static_cast<TQ*>(a.out) + r.t * (a.sx.out_ld > 0 ? a.sx.out_ld : (long long)a.H * a.vdim) + (long long)r.head * a.vdim + col;
-  const float v[4] = {acc.x, acc.y, acc.z, acc.w};
+  float v[4] = {acc.x * by, acc.y * by, acc.z * by, acc.w * by};
+  if (a.gate != nullptr) {
 #pragma unroll
-  for (int y = 0; y < 4; ++y) stf(dst + y, a.gate != nullptr ? v[y] * by / (1.0f + expf(-gv[y])) : v[y] * by);
+    for (int y = 0; y < 4; ++y) v[y] = __fdividef(v[y], 1.0f + ex2(fminf(-kLog2e * gv[y], 125.f)));  // (the quotient wants a divisor below 2^126)
+  }
+  st4(dst, v, a.vec_out);
+}
+
+// Adds the values that are no numbers, among the keys with a mask that this CTA walks and the row sees.
+template <typename TC>
+__device__ __noinline__ void add_no_numbers(const Args& a, float4& acc, int e, int g, const Row r, int col, int split, int wk, int keys) {
+  const int n = a.n[e], ctx = a.ctx[e], len = ctx + n, window = a.sx.window > 0 ? a.sx.window : 0, keep = window ? max(a.sx.keep_first, 0) : 0;
+  const long long t0 = a.row0[e];
+  const int i = static_cast<int>(r.t - t0), mine = a.pos != nullptr ? a.pos[r.t] : ctx + i;
+  const int ntiles = (len + keys - 1) / keys, t_lo = window ? max(0, ctx - window + 1) / keys : 0, nkeep = min(min((keep + keys - 1) / keys, ntiles), t_lo);
+  float* out = &acc.x;
+  for (int walk = 0; walk < nkeep + ntiles - t_lo; ++walk) {
+    if (walk / wk % a.nsplit != split) continue;
+    const int j0 = (walk < nkeep ? walk : t_lo + walk - nkeep) * keys;
+    if (j0 + keys <= ctx && (window == 0 || j0 > len - 1 - window || j0 + keys <= keep)) continue;  // without a mask: in the sums
+    for (int j = j0; j < min(j0 + keys, len); ++j) {
+      const int m = j - ctx, pj = m < 0 ? j : a.pos != nullptr ? a.pos[t0 + m] : j;
+      const bool seen = m < 0 || (a.tree == nullptr ? m <= i : m / 32 < a.words && (a.tree[r.t * a.words + m / 32] >> (m % 32) & 1u));
+      if (!seen || (window && mine - pj >= window && pj >= keep)) continue;
+      const long long row = ((long long)a.pt[(long long)e * a.max_pages + j / a.page] * a.page + j % a.page) * a.G + g;
+      for (int y = 0; y < 4; ++y) {
+        const long long at = row * a.vdim + col + y;
+        float v;
+        if (sizeof(TC) == 1) v = (a.vp[at] & 0x7f) == 0x7f ? __uint_as_float(0x7fffffffu) : 0.f;
+        else if (sizeof(TC) == 2) v = __bfloat162float(reinterpret_cast<const bf16*>(a.vp)[at]);
+        else v = reinterpret_cast<const float*>(a.vp)[at];
+        if (!(fabsf(v) < INFINITY)) out[y] += v;
+      }
+    }
+  }
 }
 
 // A 16-byte piece's place in a tile.  Keys: two neighbouring rows are read together, pieces 4 x .. 4 x + 3 of each: rows of 128 bytes and more turn the odd row's by four.  Values:
@@ -202,6 +273,8 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
   __shared__ float2 stat[kWarps][16 * MT];
   __shared__ float top_power[kWarps];
   __shared__ float2 joined[kWarps * 16 * MT];
+  __shared__ int any_bad;
+  if (threadIdx.x == 0) any_bad = 0;
   // the step's descriptors are there before its first kernel
   const int split = blockIdx.x, g = blockIdx.y / a.blocks, block = blockIdx.y % a.blocks, e = blockIdx.z;
   const int n = a.n[e], ctx = a.ctx[e], gsz = a.H / a.G, len = ctx + n;
@@ -268,7 +341,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
       pg::cp_async16(dst + KT * (K::KROW + K::VROW) + 16 * lane, p, true);
     }
   };
-#pragma unroll
+#pragma unroll 1
   for (int k = 0; k < K::STAGES - 1; ++k) {
     const int w = walk0 + k * stride, pid = __shfl_sync(0xffffffffu, pids, k);
     if (w < nwalk) request(k, tile_of(w), pid);
@@ -280,7 +353,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
   const int tiles_m = wr * MT;
   constexpr int QL = DC == 1 ? 16 : 32;       // lanes of a row
   constexpr int RW = 32 / QL;                 // rows a warp and pass
-#pragma unroll 4
+#pragma unroll 2
   for (int rb = 0; rb < rows_cta; rb += kWarps * RW) {
     const int r = rb + warp * RW + lane / QL, w = lane % QL;
     const int rr = r0 + r;
@@ -291,7 +364,8 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
     const TQ* q = static_cast<const TQ*>(a.q) + (t0 + i) * (long long)a.H * a.dim + (long long)head * a.dim + d0;
     float v[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = in && d0 + k < a.dim ? ldf(q + k) : 0.f;
+    for (int k = 0; k < 4; ++k) v[k] = 0.f;
+    if (in && d0 < a.dim) ld4(v, q, a.vec_q);
     float s = a.scale * (a.sx.head_scale != nullptr ? a.sx.head_scale[head] : 1.f);
     if (K::C8) {
       float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
@@ -338,10 +412,19 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
       for (int k = 0; k < 4; ++k) o[m][b][k] = 0.f;
   int P = 0;  // largest power of a value row so far (byte)
 
-  // one tile; PLAIN: every row sees every key of it
-  auto step = [&](auto plain_tag, int it, const unsigned char* stage) {
-    constexpr bool PLAIN = decltype(plain_tag)::value;
-    const int j0 = it * KT;
+  bool bad = false;  // a value that is no number in a tile with a mask
+#pragma unroll 1
+  for (int k = 0, walk = walk0; walk < nwalk; ++k, walk += stride) {
+    pg::cp_async_wait<K::STAGES - 2>();
+    __syncwarp();  // tile k is here for all lanes, and all are done with the tile before
+    const int ahead = k + K::STAGES - 1;
+    if ((ahead & 31) == 0) pids = pages_from(walk0 + ahead * stride);
+    const int wa = walk0 + ahead * stride, pid = __shfl_sync(0xffffffffu, pids, ahead & 31);
+    if (wa < nwalk) request(ahead, tile_of(wa), pid);
+    pg::cp_async_commit();
+    const int it = tile_of(walk), j0 = it * KT;
+    const unsigned char* stage = ring + (k % K::STAGES) * K::STAGE;
+    const bool plain = j0 + KT <= ctx && (window == 0 || j0 > len - 1 - window || j0 + KT <= keep);  // every row sees every key of the tile
     // ---- S = Q K^T
     float s[MT][NB][4];
 #pragma unroll
@@ -391,29 +474,27 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
     }
     // ---- who sees what
     uint32_t vis[2 * MT];
-    if (!PLAIN) {
-      const int rel = j0 - ctx;
+    if (!plain) {
+      // 32 drafted tokens a word, in front of the first one stored keys; the tile's keys start inside word w
+      const int rel = j0 - ctx, w = rel >> 5;
+      uint32_t lo[2 * MT], hi[2 * MT];
 #pragma unroll
       for (int x = 0; x < 2 * MT; ++x) {
-        const uint32_t* mask = a.tree != nullptr ? a.tree + (t0 + node[x]) * a.words : nullptr;
-        auto word = [&](int w) -> uint32_t {  // drafted tokens 32 w .. 32 w + 31
-          if (w < 0 || 32 * w >= n) return 0u;
-          const int left = n - 32 * w;
-          const uint32_t have = left >= 32 ? 0xffffffffu : (1u << left) - 1u;
-          if (mask != nullptr) return w < a.words ? mask[w] & have : 0u;
-          const int upto = node[x] + 1 - 32 * w;
-          return upto >= 32 ? have : upto <= 0 ? 0u : have & ((1u << upto) - 1u);
-        };
-        uint32_t v;
-        if (rel >= 0) {
-          const int w = rel >> 5, sh = rel & 31;
-          v = word(w) >> sh;
-          if (sh) v |= word(w + 1) << (32 - sh);
-        } else if (rel > -32) {
-          v = word(0) << -rel | ((1u << -rel) - 1u);
+        if (a.tree != nullptr) {
+          const uint32_t* mask = a.tree + (t0 + node[x]) * a.words;
+          lo[x] = mask[min(max(w, 0), a.words - 1)];
+          hi[x] = mask[min(max(w + 1, 0), a.words - 1)];
         } else {
-          v = 0xffffffffu;
+          const int upto = node[x] + 1;  // a chain: rows up to itself
+          lo[x] = upto - 32 * w >= 32 ? 0xffffffffu : upto <= 32 * w ? 0u : (1u << (upto - 32 * w)) - 1u;
+          hi[x] = upto - 32 * w >= 64 ? 0xffffffffu : upto <= 32 * w + 32 ? 0u : (1u << (upto - 32 * w - 32)) - 1u;
         }
+      }
+      auto have = [&](int w) { return w < 0 || n - 32 * w >= 32 ? 0xffffffffu : n <= 32 * w || (a.tree != nullptr && w >= a.words) ? 0u : (1u << (n - 32 * w)) - 1u; };
+      const uint32_t all_lo = a.tree != nullptr && w >= a.words ? 0u : have(w), all_hi = a.tree != nullptr && w + 1 >= a.words ? 0u : have(w + 1);
+#pragma unroll
+      for (int x = 0; x < 2 * MT; ++x) {
+        uint32_t v = __funnelshift_r(w < 0 ? 0xffffffffu : lo[x] & all_lo, w + 1 < 0 ? 0xffffffffu : hi[x] & all_hi, rel & 31);
         if (window) {
           const int p = a.pos[t0 + node[x]];
           for (int k = 0; k < KT; ++k) {
@@ -441,7 +522,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
 #pragma unroll
       for (int x = 0; x < KPL / 4; ++x) {
         uint32_t w = vpw[x];
-        if (!PLAIN) {  // rows behind the last one hold anything
+        if (!plain) {  // rows behind the last one hold anything
           const int left = len - j0 - KPL * c - 4 * x;
           w = left >= 4 ? w : left <= 0 ? 0u : w & ((1u << (8 * left)) - 1u);
           vpw[x] = w;
@@ -520,7 +601,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
               if (y == f) s[m][y][2 * h] = two[0], s[m][y][2 * h + 1] = two[1];
           }
         }
-        if (!PLAIN) {
+        if (!plain) {
           const float nothing = a.sx.logistic ? 0.f : -INFINITY;
 #pragma unroll
           for (int f = 0; f < NB; ++f)
@@ -602,60 +683,18 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
             }
           }
         }
-      // a value that is not a number reaches only the rows that see its key: in a tile with a mask such rows are taken out and added one by one
-      if (!PLAIN) {
+      // a value that is not a number reaches only the rows that see its key (a weight of zero times it is none): taken out here, added to their outputs below
+      if (!plain) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          bool bad = false;
+        for (int x = 0; x < 4; ++x)
 #pragma unroll
           for (int b = 0; b < VC; ++b)
 #pragma unroll
             for (int y = 0; y < K::VW; ++y) {
-              const uint32_t w = vv[x][b][y];
-              if (K::F32) bad |= (w & 0x7f800000u) == 0x7f800000u;
-              else if (K::C8) bad |= (w & 0x7fu) == 0x7fu || (w & 0x7f00u) == 0x7f00u || (w & 0x7f0000u) == 0x7f0000u || (w & 0x7f000000u) == 0x7f000000u;
-              else bad |= (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+              const uint32_t no = no_numbers<K::ES>(vv[x][b][y]);
+              vv[x][b][y] &= ~no;
+              bad |= no != 0u;
             }
-          uint32_t lanes = __ballot_sync(0xffffffffu, bad);
-          lanes |= lanes >> 16;
-          lanes |= lanes >> 8;
-          lanes |= lanes >> 4;
-          lanes &= 15u;  // bit c: key KPL c + 4 q + x
-          if (lanes == 0) continue;
-          if (lanes >> c & 1u) {
-#pragma unroll
-            for (int b = 0; b < VC; ++b)
-#pragma unroll
-              for (int y = 0; y < K::VW; ++y) vv[x][b][y] = 0u;
-          }
-#pragma unroll 1
-          for (int cc = 0; cc < 4; ++cc) {
-            if (!(lanes >> cc & 1u)) continue;
-            const int row = KPL * cc + 4 * q + x;
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-              const float w0 = __shfl_sync(0xffffffffu, s[m][2 * q + x / 2][x % 2], 4 * nn + cc), w1 = __shfl_sync(0xffffffffu, s[m][2 * q + x / 2][2 + x % 2], 4 * nn + cc);
-#pragma unroll
-              for (int b = 0; b < 8 * VC; ++b)
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                  const int byte = (64 * (b / 8) + 16 * c + 8 * k + b % 8) * K::ES;  // my column's
-                  const unsigned char* at = vt + value_place<K::VROW, KPL, K::ES>(row, byte / 16) + byte % 16;
-                  float v;
-                  if (K::C8) {
-                    const uint32_t two = cache8::halves_of(*at);
-                    v = __low2float(*reinterpret_cast<const __half2*>(&two));
-                  } else if (K::F32) {
-                    v = *reinterpret_cast<const float*>(at);
-                  } else {
-                    v = __bfloat162float(*reinterpret_cast<const bf16*>(at));
-                  }
-                  if (w0 != 0.f) o[m][b][k] = fmaf(w0, v, o[m][b][k]);
-                  if (w1 != 0.f) o[m][b][2 + k] = fmaf(w1, v, o[m][b][2 + k]);
-                }
-            }
-          }
-        }
       }
 #pragma unroll
       for (int b = 0; b < VC; ++b) {
@@ -686,20 +725,6 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
         }
       }
     }
-  };
-#pragma unroll 1
-  for (int k = 0, walk = walk0; walk < nwalk; ++k, walk += stride) {
-    pg::cp_async_wait<K::STAGES - 2>();
-    __syncwarp();  // tile k is here for all lanes, and all are done with the tile before
-    const int ahead = k + K::STAGES - 1;
-    if ((ahead & 31) == 0) pids = pages_from(walk0 + ahead * stride);
-    const int wa = walk0 + ahead * stride, pid = __shfl_sync(0xffffffffu, pids, ahead & 31);
-    if (wa < nwalk) request(ahead, tile_of(wa), pid);
-    pg::cp_async_commit();
-    const int it = tile_of(walk), j0 = it * KT;
-    const unsigned char* stage = ring + (k % K::STAGES) * K::STAGE;
-    if (j0 + KT <= ctx && (window == 0 || j0 > len - 1 - window || j0 + KT <= keep)) step(Yes{}, it, stage);
-    else step(No{}, it, stage);
   }
 
   // ---- the warps' results into shared memory, then row by row
@@ -730,9 +755,11 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
       }
   }
   if (K::C8 && lane == 0) top_power[warp] = static_cast<float>(P);
+  if (bad) any_bad = 1;
   __syncthreads();
   const int rows_here = min(rows_cta, R - r0);
   const int quads = a.vdim / 4;  // four columns a thread
+#pragma unroll 2
   for (int idx = tid; idx < rows_here * quads; idx += 32 * kWarps) {
     const int r = idx / quads, col = 4 * (idx - r * quads), tile = r / (16 * MT), in = r % (16 * MT);
     const Row where(a, r0 + r, gsz, g, t0);
@@ -751,6 +778,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
       if (K::C8) f *= exp2f(top_power[ww] - 142.f);  // the weights' power: 2^(P - 127 - 15)
       if (f != 0.f) add(acc, f, *reinterpret_cast<const float4*>(os + (ww * 16 * MT + in) * ldo_s + col));
     }
+    if (any_bad) add_no_numbers<TC>(a, acc, e, g, where, col, split, wk, KT);
     if (a.nsplit == 1) {
       finish<TQ>(a, where, col, ref, l, acc, gv);
     } else if (a.cluster) {  // over the first warp's, whose columns only this thread reads
@@ -984,6 +1012,8 @@ int attn_rows(const PgAttnRows* q, long long* need, void* scratch, long long scr
   a.scale = p.scale, a.softcap = p.softcap, a.gate_per_head = p.gate_per_head;
   a.sx = sx != nullptr ? *sx : PgAttnScore{};
   a.mode = a.sx.dist_a != nullptr || a.sx.logistic ? kGeneral : p.softcap > 0.f ? kCapped : kPlain;
+  const int four = p.act_f32 ? 16 : 8;  // bytes of four elements
+  a.vec_q = aligned(p.q, four), a.vec_gate = aligned(p.gate, four) && p.ldg % 4 == 0, a.vec_out = aligned(p.out, four) && a.sx.out_ld % 4 == 0;
   a.trigger = pg::weights_follow();
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (p.e4m3) return p.act_f32 ? by_rows<float, e4m3, 32>(p, a, need, scratch_bytes, st) : by_rows<bf16, e4m3, 32>(p, a, need, scratch_bytes, st);
