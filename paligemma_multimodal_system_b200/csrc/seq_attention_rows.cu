@@ -106,6 +106,11 @@ __device__ __forceinline__ void st4(bf16* p, const float (&v)[4], bool vec) {
     for (int i = 0; i < 4; ++i) p[i] = __float2bfloat16_rn(v[i]);
   }
 }
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 __device__ __forceinline__ float rcp(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -185,11 +190,6 @@ constexpr int ctas_per_sm() {
 struct Row {
   long long t;
   int head;
-  __device__ __forceinline__ Row(const Args& a, int rr, int gsz, int g, long long t0) {
-    const int i = rr / gsz;
-    t = t0 + i;
-    head = g * gsz + rr - i * gsz;
-  }
 };
 __device__ __forceinline__ void add(float4& acc, float f, float4 v) {
   acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
@@ -273,6 +273,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
   __shared__ float2 stat[kWarps][16 * MT];
   __shared__ float top_power[kWarps];
   __shared__ float2 joined[kWarps * 16 * MT];
+  __shared__ int2 where_to[kWarps * 16 * MT];  // a row's token of the entry and its head; past the last row: the last one's
   __shared__ int any_bad;
   if (threadIdx.x == 0) any_bad = 0;
   // the step's descriptors are there before its first kernel
@@ -349,16 +350,20 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
   }
 
   // ---- queries: fragments in the order of the cache's pieces; four elements a lane, a warp takes every fourth row, one trip to memory
+  for (int r = tid; r < rows_cta; r += 32 * kWarps) {
+    const int rr = min(r0 + r, R - 1), i = rr / gsz;
+    where_to[r] = make_int2(i, g * gsz + rr - i * gsz);
+  }
+  __syncthreads();
   uint4* qs = reinterpret_cast<uint4*>(raw);  // [term][row tile][step][lane]
   const int tiles_m = wr * MT;
   constexpr int QL = DC == 1 ? 16 : 32;       // lanes of a row
   constexpr int RW = 32 / QL;                 // rows a warp and pass
-#pragma unroll 2
+#pragma unroll 4
   for (int rb = 0; rb < rows_cta; rb += kWarps * RW) {
     const int r = rb + warp * RW + lane / QL, w = lane % QL;
-    const int rr = r0 + r;
-    const bool in = rr < R;
-    const int i = in ? rr / gsz : 0, head = g * gsz + (in ? rr - i * gsz : 0);
+    const bool in = r0 + r < R;
+    const int i = where_to[r].x, head = where_to[r].y;
     const int st = w / 4, cc = w % 4;
     const int d0 = K::C8 ? 64 * (st / 4) + 16 * cc + 4 * (st % 4) : K::F32 ? 16 * st + 4 * cc : 32 * (st / 2) + 8 * cc + 4 * (st % 2);
     const TQ* q = static_cast<const TQ*>(a.q) + (t0 + i) * (long long)a.H * a.dim + (long long)head * a.dim + d0;
@@ -397,7 +402,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
 #pragma unroll
   for (int x = 0; x < 2 * MT; ++x) {
     const int r = 16 * (rg * MT + x / 2) + 8 * (x % 2) + nn;
-    node[x] = min((r0 + r) / gsz, n - 1);
+    node[x] = where_to[r].x;
     uns[x] = unscale[r];
   }
 
@@ -425,6 +430,53 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
     const int it = tile_of(walk), j0 = it * KT;
     const unsigned char* stage = ring + (k % K::STAGES) * K::STAGE;
     const bool plain = j0 + KT <= ctx && (window == 0 || j0 > len - 1 - window || j0 + KT <= keep);  // every row sees every key of the tile
+    // ---- who sees what
+    uint32_t vis[2 * MT];
+    if (!plain) {
+      // 32 drafted tokens a word, in front of the first one stored keys; the tile's keys start inside word w
+      const int rel = j0 - ctx, w = rel >> 5;
+      uint32_t lo[2 * MT], hi[2 * MT];
+#pragma unroll
+      for (int x = 0; x < 2 * MT; ++x) {
+        if (a.tree != nullptr) {
+          const uint32_t* mask = a.tree + (t0 + node[x]) * a.words;
+          lo[x] = mask[min(max(w, 0), a.words - 1)];
+          hi[x] = mask[min(max(w + 1, 0), a.words - 1)];
+        } else {
+          const int upto = node[x] + 1;  // a chain: rows up to itself
+          lo[x] = upto - 32 * w >= 32 ? 0xffffffffu : upto <= 32 * w ? 0u : (1u << (upto - 32 * w)) - 1u;
+          hi[x] = upto - 32 * w >= 64 ? 0xffffffffu : upto <= 32 * w + 32 ? 0u : (1u << (upto - 32 * w - 32)) - 1u;
+        }
+      }
+      auto have = [&](int w) { return w < 0 || n - 32 * w >= 32 ? 0xffffffffu : n <= 32 * w || (a.tree != nullptr && w >= a.words) ? 0u : (1u << (n - 32 * w)) - 1u; };
+      const uint32_t all_lo = a.tree != nullptr && w >= a.words ? 0u : have(w), all_hi = a.tree != nullptr && w + 1 >= a.words ? 0u : have(w + 1);
+#pragma unroll
+      for (int x = 0; x < 2 * MT; ++x) {
+        uint32_t v = __funnelshift_r(w < 0 ? 0xffffffffu : lo[x] & all_lo, w + 1 < 0 ? 0xffffffffu : hi[x] & all_hi, rel & 31);
+        if (window) {
+          const int p = a.pos[t0 + node[x]];
+          for (int k = 0; k < KT; ++k) {
+            const int j = j0 + k;
+            const int pj = j < ctx ? j : j < len ? a.pos[t0 + (j - ctx)] : 0;
+            if (!(p - pj < window || pj < keep)) v &= ~(1u << k);
+          }
+        }
+        vis[x] = v;
+      }
+      // a value that is not a number reaches only the rows that see its key (a weight of zero times it is none): taken out here, added to their outputs below
+      unsigned char* values = ring + (k % K::STAGES) * K::STAGE + KT * K::KROW;
+#pragma unroll 1
+      for (int at = 16 * lane; at < KT * K::VROW; at += 512) {
+        uint4 u = *reinterpret_cast<const uint4*>(values + at);
+        const uint4 no = make_uint4(no_numbers<K::ES>(u.x), no_numbers<K::ES>(u.y), no_numbers<K::ES>(u.z), no_numbers<K::ES>(u.w));
+        if (no.x | no.y | no.z | no.w) {
+          bad = true;
+          *reinterpret_cast<uint4*>(values + at) = make_uint4(u.x & ~no.x, u.y & ~no.y, u.z & ~no.z, u.w & ~no.w);
+        }
+      }
+      if (K::C8 && lane < KT && j0 + lane >= len) values[KT * K::VROW + KT + lane] = 0;  // (powers of rows behind the last one)
+      __syncwarp();
+    }
     // ---- S = Q K^T
     float s[MT][NB][4];
 #pragma unroll
@@ -472,43 +524,9 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
         }
       }
     }
-    // ---- who sees what
-    uint32_t vis[2 * MT];
-    if (!plain) {
-      // 32 drafted tokens a word, in front of the first one stored keys; the tile's keys start inside word w
-      const int rel = j0 - ctx, w = rel >> 5;
-      uint32_t lo[2 * MT], hi[2 * MT];
-#pragma unroll
-      for (int x = 0; x < 2 * MT; ++x) {
-        if (a.tree != nullptr) {
-          const uint32_t* mask = a.tree + (t0 + node[x]) * a.words;
-          lo[x] = mask[min(max(w, 0), a.words - 1)];
-          hi[x] = mask[min(max(w + 1, 0), a.words - 1)];
-        } else {
-          const int upto = node[x] + 1;  // a chain: rows up to itself
-          lo[x] = upto - 32 * w >= 32 ? 0xffffffffu : upto <= 32 * w ? 0u : (1u << (upto - 32 * w)) - 1u;
-          hi[x] = upto - 32 * w >= 64 ? 0xffffffffu : upto <= 32 * w + 32 ? 0u : (1u << (upto - 32 * w - 32)) - 1u;
-        }
-      }
-      auto have = [&](int w) { return w < 0 || n - 32 * w >= 32 ? 0xffffffffu : n <= 32 * w || (a.tree != nullptr && w >= a.words) ? 0u : (1u << (n - 32 * w)) - 1u; };
-      const uint32_t all_lo = a.tree != nullptr && w >= a.words ? 0u : have(w), all_hi = a.tree != nullptr && w + 1 >= a.words ? 0u : have(w + 1);
-#pragma unroll
-      for (int x = 0; x < 2 * MT; ++x) {
-        uint32_t v = __funnelshift_r(w < 0 ? 0xffffffffu : lo[x] & all_lo, w + 1 < 0 ? 0xffffffffu : hi[x] & all_hi, rel & 31);
-        if (window) {
-          const int p = a.pos[t0 + node[x]];
-          for (int k = 0; k < KT; ++k) {
-            const int j = j0 + k;
-            const int pj = j < ctx ? j : j < len ? a.pos[t0 + (j - ctx)] : 0;
-            if (!(p - pj < window || pj < keep)) v &= ~(1u << k);
-          }
-        }
-        vis[x] = v;
-      }
-    }
-    // ---- weights
-    float kf[KPL], vf[KPL];
-    float grow = 1.f;  // 2^(P - new P)
+    // ---- weights: one straight line but for options, masks and new maxima
+    uint64_t kf[NB], vf[NB];  // pairs of powers: keys 2 f, 2 f + 1 of this lane
+    float grow = 1.f;         // 2^(P - new P)
     if (K::C8) {
       uint32_t kpw[KPL / 4], vpw[KPL / 4];
 #pragma unroll
@@ -516,152 +534,140 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
         kpw[x] = *reinterpret_cast<const uint32_t*>(stage + KT * (K::KROW + K::VROW) + KPL * c + 4 * x);
         vpw[x] = *reinterpret_cast<const uint32_t*>(stage + KT * (K::KROW + K::VROW) + KT + KPL * c + 4 * x);
       }
+      uint32_t most = vpw[0];
 #pragma unroll
-      for (int x = 0; x < KPL; ++x) kf[x] = __uint_as_float((kpw[x / 4] >> (8 * (x % 4)) & 0xffu) << 23);  // (byte 0: what is below 2^-118 counts as zero)
-      uint32_t most = 0;
-#pragma unroll
-      for (int x = 0; x < KPL / 4; ++x) {
-        uint32_t w = vpw[x];
-        if (!plain) {  // rows behind the last one hold anything
-          const int left = len - j0 - KPL * c - 4 * x;
-          w = left >= 4 ? w : left <= 0 ? 0u : w & ((1u << (8 * left)) - 1u);
-          vpw[x] = w;
-        }
-        most = __vmaxu4(most, w);
-      }
+      for (int x = 1; x < KPL / 4; ++x) most = __vmaxu4(most, vpw[x]);
       most = __vmaxu4(most, most >> 16);
       most = max(most & 0xffu, most >> 8 & 0xffu);
-      int top = static_cast<int>(most);
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      if (top > P) {
-        grow = top - P >= 127 ? 0.f : __uint_as_float(static_cast<uint32_t>(127 - (top - P)) << 23);
-        P = top;
-      }
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      const int top = max(P, static_cast<int>(max(most, __shfl_xor_sync(0xffffffffu, most, 2))));
+      grow = __uint_as_float(static_cast<uint32_t>(max(127 - (top - P), 0)) << 23);
+      P = top;
       // 2^(15 + power - P): a weight of one is 2^15, halves reach down to 2^-24; four bytes at a time, P - 142 <= byte <= P, so that none carries into the next
       const uint32_t least = static_cast<uint32_t>(max(P - 142, 0)) * 0x01010101u, lift = static_cast<uint32_t>(142 - P) * 0x01010101u;
 #pragma unroll
       for (int x = 0; x < KPL / 4; ++x) vpw[x] = __vmaxu4(vpw[x], least) + lift;
 #pragma unroll
-      for (int x = 0; x < KPL; ++x) vf[x] = __uint_as_float((vpw[x / 4] >> (8 * (x % 4)) & 0xffu) << 23);
+      for (int f = 0; f < NB; ++f) {  // (a key's byte 0: what is below 2^-118 counts as zero)
+        const int sh = 8 * (2 * f % 4);
+        kf[f] = pg::pair_of((kpw[f / 2] >> sh & 0xffu) << 23, (kpw[f / 2] >> (sh + 8) & 0xffu) << 23);
+        vf[f] = pg::pair_of((vpw[f / 2] >> sh & 0xffu) << 23, (vpw[f / 2] >> (sh + 8) & 0xffu) << 23);
+      }
+    }
+    constexpr int HS = R8 ? 1 : 2;
+    uint64_t t[MT][HS][NB];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int h = 0; h < HS; ++h) {
+        const uint64_t u = pg::pair_of(uns[2 * m + h], uns[2 * m + h]);
+#pragma unroll
+        for (int f = 0; f < NB; ++f) t[m][h][f] = mul_pair(pg::pair_of(s[m][f][2 * h], s[m][f][2 * h + 1]), K::C8 ? mul_pair(u, kf[f]) : u);
+      }
+    if (a.mode == kCapped) {  // cap tanh(v / cap) in log2 units; v comes as 2 log2(e) v / cap
+      const float cap = a.softcap * kLog2e;
+      auto bend = [&](float v) {
+        if (sizeof(TQ) == 2) return fmaf(-2.f * cap, rcp(ex2(v) + 1.f), cap);  // off by 2^-22 cap: the output's rounding is 2^-9
+        return cap * tanh_f32(v * (0.5f / kLog2e));
+      };
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < HS; ++h)
+#pragma unroll
+          for (int f = 0; f < NB; ++f) t[m][h][f] = pg::pair_of(bend(pg::lo_f32(t[m][h][f])), bend(pg::hi_f32(t[m][h][f])));
+    } else if (a.mode == kGeneral) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < HS; ++h) {
+          const int head = where_to[16 * (rg * MT + m) + 8 * h + nn].y, mine = a.pos != nullptr ? a.pos[t0 + node[2 * m + h]] : 0;
+          auto bend = [&](float v, int j) {
+            if (a.softcap > 0.f) v = a.softcap * tanh_f32(v / a.softcap);
+            if (a.sx.dist_a != nullptr) v -= a.sx.dist_a[head] * log1pf(a.sx.dist_b[head] * (float)max(mine - (j < ctx || j >= len ? j : a.pos[t0 + (j - ctx)]), 0));
+            // a logistic weight as a power of two against a maximum of 0
+            if (a.sx.logistic) return -log2f(1.0f + expf(-(v + (a.sx.head_bias != nullptr ? a.sx.head_bias[head] : 0.f))));
+            return v * kLog2e;
+          };
+          uint64_t* row = t[m][h];
+#pragma unroll 1
+          for (int f = 0; f < NB; ++f) {
+            uint64_t two = 0;
+#pragma unroll
+            for (int y = 0; y < NB; ++y) two = y == f ? row[y] : two;
+            const int j = j0 + KPL * c + 2 * f;
+            two = pg::pair_of(bend(pg::lo_f32(two), j), bend(pg::hi_f32(two), j + 1));
+#pragma unroll
+            for (int y = 0; y < NB; ++y) row[y] = y == f ? two : row[y];
+          }
+        }
+    }
+    if (!plain) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < HS; ++h) {
+          const uint32_t v = vis[2 * m + h] >> (KPL * c);
+#pragma unroll
+          for (int f = 0; f < NB; ++f)
+            t[m][h][f] = pg::pair_of(v >> (2 * f) & 1u ? pg::lo_f32(t[m][h][f]) : -INFINITY, v >> (2 * f + 1) & 1u ? pg::hi_f32(t[m][h][f]) : -INFINITY);
+        }
+    }
+    float corr[2 * MT];
+    bool moved = false;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int h = 0; h < HS; ++h) {
+        const int x = 2 * m + h;
+        float mx = fmaxf(pg::lo_f32(t[m][h][0]), pg::hi_f32(t[m][h][0]));
+#pragma unroll
+        for (int f = 1; f < NB; ++f) mx = pg::max3(mx, pg::lo_f32(t[m][h][f]), pg::hi_f32(t[m][h][f]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float now = a.sx.logistic ? 0.f : fmaxf(M[x], mx), ref = now == -INFINITY ? 0.f : now;  // nothing seen so far: weights of zero
+        const float shrink = ex2(M[x] - ref);
+        corr[x] = shrink * grow;
+        M[x] = now;
+        const uint64_t minus = pg::pair_of(-ref, -ref);
+        uint64_t sum = 0;
+#pragma unroll
+        for (int f = 0; f < NB; ++f) {
+          const uint64_t d = pg::add_pair(t[m][h][f], minus);
+          const uint64_t p = pg::pair_of(ex2(pg::lo_f32(d)), ex2(pg::hi_f32(d)));
+          sum = f == 0 ? p : pg::add_pair(sum, p);
+          t[m][h][f] = K::C8 ? mul_pair(p, vf[f]) : p;
+        }
+        L[x] = fmaf(L[x], shrink, pg::lo_f32(sum) + pg::hi_f32(sum));
+        moved |= corr[x] != 1.f;
+      }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int b = 0; b < 8 * VC; ++b) {
+          o[m][b][0] *= corr[2 * m], o[m][b][1] *= corr[2 * m];
+          if (!R8) o[m][b][2] *= corr[2 * m + HS - 1], o[m][b][3] *= corr[2 * m + HS - 1];
+        }
     }
     uint4 pa[MT][NB / 2][K::PT];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      float corr[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int x = 2 * m + h;
-        if (h == 1 && R8) {
-#pragma unroll
-          for (int f = 0; f < NB; ++f) s[m][f][2] = s[m][f][3] = 0.f;
-          corr[1] = 1.f;
-          continue;
-        }
-#pragma unroll
-        for (int f = 0; f < NB; ++f)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float v = s[m][f][2 * h + i] * uns[x];
-            if (K::C8) v *= kf[2 * f + i];
-            s[m][f][2 * h + i] = v;
-          }
-        if (a.mode == kCapped) {  // cap tanh(v / cap) in log2 units; v comes as 2 log2(e) v / cap
-          const float cap = a.softcap * kLog2e;
-#pragma unroll
-          for (int f = 0; f < NB; ++f)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float v = s[m][f][2 * h + i];
-              if (sizeof(TQ) == 2) s[m][f][2 * h + i] = fmaf(-2.f * cap, rcp(ex2(v) + 1.f), cap);  // off by 2^-22 cap: the output's rounding is 2^-9
-              else s[m][f][2 * h + i] = cap * tanh_f32(v * (0.5f / kLog2e));
-            }
-        } else if (a.mode == kGeneral) {
-          const int head = g * gsz + min(r0 + 16 * (rg * MT + m) + 8 * h + nn, R - 1) % gsz;
-#pragma unroll 1
-          for (int f = 0; f < NB; ++f) {
-            float two[2];
-#pragma unroll
-            for (int y = 0; y < NB; ++y)
-              if (y == f) two[0] = s[m][y][2 * h], two[1] = s[m][y][2 * h + 1];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              float v = two[i];
-              if (a.softcap > 0.f) v = a.softcap * tanh_f32(v / a.softcap);
-              if (a.sx.dist_a != nullptr) {
-                const int j = j0 + KPL * c + 2 * f + i, pj = j < ctx || j >= len ? j : a.pos[t0 + (j - ctx)];
-                v -= a.sx.dist_a[head] * log1pf(a.sx.dist_b[head] * (float)max(a.pos[t0 + node[x]] - pj, 0));
-              }
-              if (a.sx.logistic) v = 1.0f / (1.0f + expf(-(v + (a.sx.head_bias != nullptr ? a.sx.head_bias[head] : 0.f))));
-              else v *= kLog2e;
-              two[i] = v;
-            }
-#pragma unroll
-            for (int y = 0; y < NB; ++y)
-              if (y == f) s[m][y][2 * h] = two[0], s[m][y][2 * h + 1] = two[1];
-          }
-        }
-        if (!plain) {
-          const float nothing = a.sx.logistic ? 0.f : -INFINITY;
-#pragma unroll
-          for (int f = 0; f < NB; ++f)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              if (!(vis[x] >> (KPL * c + 2 * f + i) & 1u)) s[m][f][2 * h + i] = nothing;
-        }
-        if (a.sx.logistic) {
-          corr[h] = 1.f;
-        } else {
-          float mx = s[m][0][2 * h];
-#pragma unroll
-          for (int f = 0; f < NB; ++f) mx = fmaxf(mx, fmaxf(s[m][f][2 * h], s[m][f][2 * h + 1]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          const float now = fmaxf(M[x], mx), ref = now == -INFINITY ? 0.f : now;  // nothing seen so far: weights of zero
-          corr[h] = ex2(M[x] - ref);
-          M[x] = now;
-          float sum = 0.f;
-#pragma unroll
-          for (int f = 0; f < NB; ++f)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float p = ex2(s[m][f][2 * h + i] - ref);
-              sum += p;
-              s[m][f][2 * h + i] = p;
-            }
-          L[x] = L[x] * corr[h] + sum;
-        }
-        if (K::C8) {
-#pragma unroll
-          for (int f = 0; f < NB; ++f)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) s[m][f][2 * h + i] *= vf[2 * f + i];
-          corr[h] *= grow;
-        }
-      }
-      if (__any_sync(0xffffffffu, corr[0] != 1.f || (!R8 && corr[1] != 1.f))) {
-#pragma unroll
-        for (int b = 0; b < 8 * VC; ++b) {
-          o[m][b][0] *= corr[0], o[m][b][1] *= corr[0];
-          if (!R8) o[m][b][2] *= corr[1], o[m][b][3] *= corr[1];
-        }
-      }
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int q = 0; q < NB / 2; ++q) {
         uint32_t p0[K::PT], p1[K::PT], p2[K::PT], p3[K::PT];
-        terms<K::HALF>(s[m][2 * q][0], s[m][2 * q][1], p0);
-        terms<K::HALF>(s[m][2 * q + 1][0], s[m][2 * q + 1][1], p2);
+        terms<K::HALF>(pg::lo_f32(t[m][0][2 * q]), pg::hi_f32(t[m][0][2 * q]), p0);
+        terms<K::HALF>(pg::lo_f32(t[m][0][2 * q + 1]), pg::hi_f32(t[m][0][2 * q + 1]), p2);
         if (R8) {
 #pragma unroll
-          for (int t = 0; t < K::PT; ++t) p1[t] = p3[t] = 0u;
+          for (int i = 0; i < K::PT; ++i) p1[i] = p3[i] = 0u;
         } else {
-          terms<K::HALF>(s[m][2 * q][2], s[m][2 * q][3], p1);
-          terms<K::HALF>(s[m][2 * q + 1][2], s[m][2 * q + 1][3], p3);
+          terms<K::HALF>(pg::lo_f32(t[m][HS - 1][2 * q]), pg::hi_f32(t[m][HS - 1][2 * q]), p1);
+          terms<K::HALF>(pg::lo_f32(t[m][HS - 1][2 * q + 1]), pg::hi_f32(t[m][HS - 1][2 * q + 1]), p3);
         }
 #pragma unroll
-        for (int t = 0; t < K::PT; ++t) pa[m][q][t] = make_uint4(p0[t], p1[t], p2[t], p3[t]);
+        for (int i = 0; i < K::PT; ++i) pa[m][q][i] = make_uint4(p0[i], p1[i], p2[i], p3[i]);
       }
-    }
     // ---- O += P V: rows KPL c + 4 q .. + 3 of the tile, columns 8 n .. 8 n + 7 of every 64
     const unsigned char* vt = stage + KT * K::KROW;
 #pragma unroll
@@ -683,19 +689,6 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
             }
           }
         }
-      // a value that is not a number reaches only the rows that see its key (a weight of zero times it is none): taken out here, added to their outputs below
-      if (!plain) {
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-#pragma unroll
-          for (int b = 0; b < VC; ++b)
-#pragma unroll
-            for (int y = 0; y < K::VW; ++y) {
-              const uint32_t no = no_numbers<K::ES>(vv[x][b][y]);
-              vv[x][b][y] &= ~no;
-              bad |= no != 0u;
-            }
-      }
 #pragma unroll
       for (int b = 0; b < VC; ++b) {
 #pragma unroll
@@ -758,32 +751,40 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
   if (bad) any_bad = 1;
   __syncthreads();
   const int rows_here = min(rows_cta, R - r0);
-  const int quads = a.vdim / 4;  // four columns a thread
-#pragma unroll 2
-  for (int idx = tid; idx < rows_here * quads; idx += 32 * kWarps) {
-    const int r = idx / quads, col = 4 * (idx - r * quads), tile = r / (16 * MT), in = r % (16 * MT);
-    const Row where(a, r0 + r, gsz, g, t0);
-    float gv[4];
-    if (a.nsplit == 1) gates<TQ>(a, where, col, gv);
-    float m = -INFINITY;
+  for (int r = tid; r < rows_here; r += 32 * kWarps) {  // a row's factors
+    const int tile = r / (16 * MT), in = r % (16 * MT);
+    float m = -INFINITY, l = 0.f;
     for (int w = 0; w < wk; ++w) m = fmaxf(m, stat[w * wr + tile][in].x);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f;
     const float ref = m == -INFINITY ? 0.f : m;
     for (int w = 0; w < wk; ++w) {
-      const int ww = w * wr + tile;
-      const float2 st = stat[ww][in];
-      float f = ex2(st.x - ref);
+      float2& st = stat[w * wr + tile][in];
+      const float f = ex2(st.x - ref);
       l += f * st.y;  // (scores that are no numbers stay in the sum)
-      if (K::C8) f *= exp2f(top_power[ww] - 142.f);  // the weights' power: 2^(P - 127 - 15)
+      st.x = K::C8 ? f * exp2f(top_power[w * wr + tile] - 142.f) : f;  // the weights' power: 2^(P - 127 - 15)
+    }
+    joined[r] = make_float2(m, l);
+  }
+  __syncthreads();
+  const int quads = a.vdim / 4, per_pass = 32 * kWarps / quads, row_of = tid / quads, col = 4 * (tid - row_of * quads);  // four columns a thread
+  auto row_at = [&](int r) { return Row{t0 + where_to[r].x, where_to[r].y}; };
+#pragma unroll 2
+  for (int r = row_of < per_pass ? row_of : rows_here; r < rows_here; r += per_pass) {
+    const int tile = r / (16 * MT), in = r % (16 * MT);
+    const Row where = row_at(r);
+    float gv[4];
+    if (a.nsplit == 1) gates<TQ>(a, where, col, gv);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = 0; w < wk; ++w) {
+      const int ww = w * wr + tile;
+      const float f = stat[ww][in].x;
       if (f != 0.f) add(acc, f, *reinterpret_cast<const float4*>(os + (ww * 16 * MT + in) * ldo_s + col));
     }
     if (any_bad) add_no_numbers<TC>(a, acc, e, g, where, col, split, wk, KT);
+    const float m = joined[r].x, l = joined[r].y;
     if (a.nsplit == 1) {
-      finish<TQ>(a, where, col, ref, l, acc, gv);
+      finish<TQ>(a, where, col, m == -INFINITY ? 0.f : m, l, acc, gv);
     } else if (a.cluster) {  // over the first warp's, whose columns only this thread reads
       *reinterpret_cast<float4*>(os + (tile * 16 * MT + in) * ldo_s + col) = acc;
-      if (col == 0) joined[r] = make_float2(m, l);
     } else {
       float* pp = a.partial + (((a.singles ? (long long)e : where.t) * a.H + where.head) * a.nsplit + split) * (a.vdim + 4);
       *reinterpret_cast<float4*>(pp + 4 + col) = acc;
@@ -793,9 +794,9 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
   if (!a.cluster) return;
   // ---- the CTAs of a cluster share out the rows' columns and read one another's results
   pg::cluster_sync_all();
-  for (int idx = tid + 32 * kWarps * split; idx < rows_here * quads; idx += 32 * kWarps * a.nsplit) {
-    const int r = idx / quads, col = 4 * (idx - r * quads), tile = r / (16 * MT), in = r % (16 * MT);
-    const Row where(a, r0 + r, gsz, g, t0);
+  for (int r = (row_of < per_pass ? row_of : rows_here) + per_pass * split; r < rows_here; r += per_pass * a.nsplit) {
+    const int tile = r / (16 * MT), in = r % (16 * MT);
+    const Row where = row_at(r);
     float gv[4];
     gates<TQ>(a, where, col, gv);
     const uint32_t sa = pg::smem_u32(&joined[r]), oa = pg::smem_u32(os + (tile * 16 * MT + in) * ldo_s + col);
@@ -876,8 +877,7 @@ __global__ void __launch_bounds__(128) attn_rows_merge_kernel(const __grid_const
   if (warp == 0 && col < a.vdim) {
 #pragma unroll
     for (int w = 1; w < 4; ++w) add(acc, 1.f, sums[w][lane]);
-    Row where(a, 0, 1, 0, t);
-    where.head = head;
+    const Row where{t, head};
     float gv[4];
     gates<TQ>(a, where, col, gv);
     finish<TQ>(a, where, col, whole[0], whole[1], acc, gv);
