@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
   const int split = blockIdx.x, g = blockIdx.y / a.blocks, block = blockIdx.y % a.blocks, e = blockIdx.z;
   const int n = a.n[e], ctx = a.ctx[e], gsz = a.H / a.G, len = ctx + n;
   const long long t0 = a.row0[e];
-  const int wr = a.wr, wk = kWarps / wr, rows_cta = wr * 16 * MT, r0 = block * rows_cta, R = n * gsz;
+  const int wr = R8 ? 1 : a.wr, wk = kWarps / wr, rows_cta = wr * 16 * MT, r0 = block * rows_cta, R = n * gsz;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nn = lane >> 2, c = lane & 3;
   const int rg = warp % wr, kgrp = warp / wr;
   const bool mine = !(a.singles && n != 1) && r0 < R;
@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
   const int ntiles = (len + KT - 1) / KT;
   const int t_lo = window ? max(0, ctx - window + 1) / KT : 0;
   const int nkeep = min(min((keep + KT - 1) / KT, ntiles), t_lo);
-  const int nwalk = live > 0 ? nkeep + ntiles - t_lo : 0;
+  const int nwalk = mine ? nkeep + ntiles - t_lo : 0;
   const int* pt = a.pt + (long long)e * a.max_pages;
   const int stride = a.nsplit * wk, tpp = 1 << a.tile_shift, walk0 = split * wk + kgrp;
   auto tile_of = [&](int walk) { return walk < nkeep ? walk : t_lo + (walk - nkeep); };
@@ -305,8 +305,13 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
   else pg::griddep_begin_if(a.trigger);
   if (!mine) return;
 
-  // ---- copies: a ring of tiles a warp, 16 bytes a lane and request
-  unsigned char* ring = raw + wr * K::Q_BYTES + warp * (K::STAGES * K::STAGE);
+  // ---- copies: a ring of tiles for the warps that walk together, 16 bytes a thread and request
+  unsigned char* ring = raw + wr * K::Q_BYTES + kgrp * (K::STAGES * K::STAGE);
+  const int tg = rg * 32 + lane, group = 32 * wr;
+  auto meet = [&] {
+    if (wr == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(1 + kgrp), "r"(group) : "memory");
+  };
   const long long kpitch = (long long)a.G * a.dim * K::ES, vpitch = (long long)a.G * a.vdim * K::ES;
   const int kbytes = a.dim * K::ES, vbytes = a.vdim * K::ES;
   auto request = [&](int k, int it, int pid) {  // tile `it` into stage k % STAGES
@@ -314,32 +319,24 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
     const long long first = (long long)pid * a.page + (it & (tpp - 1)) * KT;
     constexpr int KP = K::KROW / 16, VP = K::VROW / 16;
     {
-      const int row = lane / KP, piece = lane % KP;
-      const uint8_t* p = a.kp + (first + row) * kpitch + (long long)g * kbytes + 16 * piece;
+      const int piece = tg % KP;  // (a group is a multiple of a row's pieces)
+      const uint8_t* p = a.kp + first * kpitch + (long long)g * kbytes + 16 * piece;
       const bool in = 16 * piece < kbytes;
-#pragma unroll
-      for (int i = 0; i < KT * KP / 32; ++i) {
-        const int r = row + i * (32 / KP);
-        pg::cp_async16(dst + key_place<K::KROW>(r, piece), p, in);
-        p += (32 / KP) * kpitch;
-      }
+#pragma unroll (R8 ? KT * KP / 32 : 4)
+      for (int r = tg / KP; r < KT; r += group / KP) pg::cp_async16(dst + key_place<K::KROW>(r, piece), p + r * kpitch, in);
     }
     {
-      const int row = lane / VP, piece = lane % VP;
-      const uint8_t* p = a.vp + (first + row) * vpitch + (long long)g * vbytes + 16 * piece;
+      const int piece = tg % VP;
+      const uint8_t* p = a.vp + first * vpitch + (long long)g * vbytes + 16 * piece;
       const bool in = 16 * piece < vbytes;
       const int left = len - it * KT;  // rows behind the last one hold anything: zeros
-#pragma unroll
-      for (int i = 0; i < KT * VP / 32; ++i) {
-        const int r = row + i * (32 / VP);
-        pg::cp_async16(dst + KT * K::KROW + value_place<K::VROW, KPL, K::ES>(r, piece), p, in && r < left);
-        p += (32 / VP) * vpitch;
-      }
+#pragma unroll (R8 ? KT * VP / 32 : 4)
+      for (int r = tg / VP; r < KT; r += group / VP) pg::cp_async16(dst + KT * K::KROW + value_place<K::VROW, KPL, K::ES>(r, piece), p + r * vpitch, in && r < left);
     }
-    if (K::C8 && lane < KT / 8) {  // the powers: keys' in the first half of these lanes, values' in the second
-      const bool is_v = lane >= KT / 16;
-      const uint8_t* p = (is_v ? a.ve : a.ke) + ((long long)pid * a.G + g) * a.page + (it & (tpp - 1)) * KT + 16 * (lane % (KT / 16));
-      pg::cp_async16(dst + KT * (K::KROW + K::VROW) + 16 * lane, p, true);
+    if (K::C8 && tg < KT / 8) {  // the powers: keys' in the first half of these threads, values' in the second
+      const bool is_v = tg >= KT / 16;
+      const uint8_t* p = (is_v ? a.ve : a.ke) + ((long long)pid * a.G + g) * a.page + (it & (tpp - 1)) * KT + 16 * (tg % (KT / 16));
+      pg::cp_async16(dst + KT * (K::KROW + K::VROW) + 16 * tg, p, true);
     }
   };
 #pragma unroll 1
@@ -421,7 +418,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
 #pragma unroll 1
   for (int k = 0, walk = walk0; walk < nwalk; ++k, walk += stride) {
     pg::cp_async_wait<K::STAGES - 2>();
-    __syncwarp();  // tile k is here for all lanes, and all are done with the tile before
+    meet();  // tile k is here for all, and all are done with the tile before
     const int ahead = k + K::STAGES - 1;
     if ((ahead & 31) == 0) pids = pages_from(walk0 + ahead * stride);
     const int wa = walk0 + ahead * stride, pid = __shfl_sync(0xffffffffu, pids, ahead & 31);
@@ -466,7 +463,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
       // a value that is not a number reaches only the rows that see its key (a weight of zero times it is none): taken out here, added to their outputs below
       unsigned char* values = ring + (k % K::STAGES) * K::STAGE + KT * K::KROW;
 #pragma unroll 1
-      for (int at = 16 * lane; at < KT * K::VROW; at += 512) {
+      for (int at = 16 * tg; at < KT * K::VROW; at += 16 * group) {
         uint4 u = *reinterpret_cast<const uint4*>(values + at);
         const uint4 no = make_uint4(no_numbers<K::ES>(u.x), no_numbers<K::ES>(u.y), no_numbers<K::ES>(u.z), no_numbers<K::ES>(u.w));
         if (no.x | no.y | no.z | no.w) {
@@ -474,9 +471,10 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
           *reinterpret_cast<uint4*>(values + at) = make_uint4(u.x & ~no.x, u.y & ~no.y, u.z & ~no.z, u.w & ~no.w);
         }
       }
-      if (K::C8 && lane < KT && j0 + lane >= len) values[KT * K::VROW + KT + lane] = 0;  // (powers of rows behind the last one)
-      __syncwarp();
+      if (K::C8 && tg < KT && j0 + tg >= len) values[KT * K::VROW + KT + tg] = 0;  // (powers of rows behind the last one)
+      meet();
     }
+    if (live <= 0) continue;  // no rows for this warp
     // ---- S = Q K^T
     float s[MT][NB][4];
 #pragma unroll
@@ -930,12 +928,12 @@ int launch(const PgAttnRows& p, Args a, long long* need, long long scratch_bytes
   a.wr = plan.wr, a.blocks = plan.blocks, a.nsplit = plan.nsplit, a.cluster = plan.cluster;
   a.tile_shift = 0;
   while ((KT << a.tile_shift) < a.page) ++a.tile_shift;
-  constexpr size_t kRing = (size_t)kWarps * K::STAGES * K::STAGE;
-  const size_t in = (size_t)a.wr * K::Q_BYTES + kRing, out = (size_t)kWarps * 16 * MT * (a.vdim + 4) * 4;
+  constexpr size_t kRing = (size_t)K::STAGES * K::STAGE;  // of the warps that walk together
+  const size_t in = (size_t)a.wr * K::Q_BYTES + kWarps / a.wr * kRing, out = (size_t)kWarps * 16 * MT * (a.vdim + 4) * 4;
   const size_t smem = in > out ? in : out;
   if ((long long)a.blocks * a.G > 65535) return PG_ERR_ARG;
   auto kern = attn_rows_kernel<TQ, TC, DC, VC, MT, KT, R8>;
-  constexpr size_t kOut = (size_t)kWarps * 16 * MT * (64 * VC + 4) * 4, kIn = (size_t)kWarps * K::Q_BYTES + kRing, kMost = kIn > kOut ? kIn : kOut;
+  constexpr size_t kOut = (size_t)kWarps * 16 * MT * (64 * VC + 4) * 4, kIn = (size_t)kWarps * (K::Q_BYTES + kRing), kMost = kIn > kOut ? kIn : kOut;
   static_assert(kMost <= 220 * 1024, "shared memory of a block");
   static bool configured[pg::kMaxDevices] = {};  // once a device, to the most that any call asks for
   bool& done = configured[pg::current_device()];
