@@ -70,9 +70,10 @@ __device__ __forceinline__ float tanh_f32(float x) {
 __device__ __forceinline__ float ldf(const float* p) { return *p; }
 __device__ __forceinline__ float ldf(const bf16* p) { return __bfloat162float(*p); }
 
-// four neighbouring elements; vec: they lie on a boundary of their own size
-__device__ __forceinline__ void ld4(float (&v)[4], const float* p, bool vec) {
-  if (vec) {
+// four neighbouring elements; VEC: they lie on a boundary of their own size
+template <bool VEC>
+__device__ __forceinline__ void ld4(float (&v)[4], const float* p) {
+  if (VEC) {
     const float4 f = *reinterpret_cast<const float4*>(p);
     v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
   } else {
@@ -80,14 +81,10 @@ __device__ __forceinline__ void ld4(float (&v)[4], const float* p, bool vec) {
     for (int i = 0; i < 4; ++i) v[i] = p[i];
   }
 }
-__device__ __forceinline__ void ld4(float (&v)[4], const bf16* p, bool vec) {
-  uint2 u;
-  if (vec) {
-    u = *reinterpret_cast<const uint2*>(p);
-  } else {
-    const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
-    u = make_uint2(e[0] | static_cast<uint32_t>(e[1]) << 16, e[2] | static_cast<uint32_t>(e[3]) << 16);
-  }
+template <bool VEC>
+__device__ __forceinline__ void ld4(float (&v)[4], const bf16* p) {
+  const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
+  const uint2 u = VEC ? *reinterpret_cast<const uint2*>(p) : make_uint2(e[0] | static_cast<uint32_t>(e[1]) << 16, e[2] | static_cast<uint32_t>(e[3]) << 16);
   v[0] = __uint_as_float(u.x << 16), v[1] = __uint_as_float(u.x & 0xffff0000u), v[2] = __uint_as_float(u.y << 16), v[3] = __uint_as_float(u.y & 0xffff0000u);
 }
 __device__ __forceinline__ void st4(float* p, const float (&v)[4], bool vec) {
@@ -194,40 +191,44 @@ struct Row {
 __device__ __forceinline__ void add(float4& acc, float f, float4 v) {
   acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
 }
+// a row's four columns of the gate as factors
 template <typename TQ>
 __device__ __forceinline__ void gates(const Args& a, const Row& r, int col, float (&gv)[4]) {
+  gv[0] = gv[1] = gv[2] = gv[3] = 1.f;
   if (a.gate == nullptr) return;
   const TQ* g = static_cast<const TQ*>(a.gate) + r.t * a.ldg + (a.gate_per_head ? r.head : r.head * a.vdim + col);
   if (a.gate_per_head) gv[0] = gv[1] = gv[2] = gv[3] = ldf(g);
-  else ld4(gv, g, a.vec_gate);
-}
-// four columns of a row from its sums: sink, division, gate.  A row that sees nothing: zeros.
-template <typename TQ>
-__device__ __forceinline__ void finish(const Args& a, const Row& r, int col, float ref, float l, float4 acc, const float (&gv)[4]) {
-  float by = 1.f;
-  if (!a.sx.logistic && a.sx.sink != nullptr) {
-    const float sk = a.sx.sink[r.head] * kLog2e, mm = fmaxf(ref, sk);
-    by = ex2(ref - mm);
-    l = l * by + ex2(sk - mm);
-  }
-  by *= (a.sx.logistic ? 1.f : l == 0.f ? 0.f : 1.f / l) * (a.sx.out_scale != 0.f ? a.sx.out_scale : 1.f);
-  TQ* dst = static_cast<TQ*>(a.out) + r.t * (a.sx.out_ld > 0 ? a.sx.out_ld : (long long)a.H * a.vdim) + (long long)r.head * a.vdim + col;
-  float v[4] = {acc.x * by, acc.y * by, acc.z * by, acc.w * by};
-  if (a.gate != nullptr) {
+  else if (a.vec_gate) ld4<true>(gv, g);
+  else ld4<false>(gv, g);
 #pragma unroll
-    for (int y = 0; y < 4; ++y) v[y] = __fdividef(v[y], 1.0f + ex2(fminf(-kLog2e * gv[y], 125.f)));  // (the quotient wants a divisor below 2^126)
+  for (int y = 0; y < 4; ++y) gv[y] = rcp(1.0f + ex2(fminf(-kLog2e * gv[y], 125.f)));
+}
+// what a row's sum against the maximum `ref` is multiplied by: sink, division, scale.  A row that sees nothing: zeros.
+__device__ __forceinline__ float last_factor(const Args& a, int head, float ref, float l) {
+  float by = a.sx.out_scale != 0.f ? a.sx.out_scale : 1.f;
+  if (a.sx.logistic) return by;
+  if (a.sx.sink != nullptr) {
+    const float sk = a.sx.sink[head] * kLog2e, mm = fmaxf(ref, sk), f = ex2(ref - mm);
+    by *= f;
+    l = l * f + ex2(sk - mm);
   }
+  return l == 0.f ? 0.f : by / l;
+}
+template <typename TQ>
+__device__ __forceinline__ void put(const Args& a, const Row& r, int col, float4 acc, const float (&gv)[4]) {
+  TQ* dst = static_cast<TQ*>(a.out) + r.t * (a.sx.out_ld > 0 ? a.sx.out_ld : (long long)a.H * a.vdim) + (long long)r.head * a.vdim + col;
+  const float v[4] = {acc.x * gv[0], acc.y * gv[1], acc.z * gv[2], acc.w * gv[3]};
   st4(dst, v, a.vec_out);
 }
 
-// Adds the values that are no numbers, among the keys with a mask that this CTA walks and the row sees.
+// The sum of the values that are no numbers, among the keys with a mask that this CTA walks and the row sees.
 template <typename TC>
-__device__ __noinline__ void add_no_numbers(const Args& a, float4& acc, int e, int g, const Row r, int col, int split, int wk, int keys) {
+__device__ __noinline__ float4 no_number_values(const Args& a, int e, int g, const Row r, int col, int split, int wk, int keys) {
   const int n = a.n[e], ctx = a.ctx[e], len = ctx + n, window = a.sx.window > 0 ? a.sx.window : 0, keep = window ? max(a.sx.keep_first, 0) : 0;
   const long long t0 = a.row0[e];
   const int i = static_cast<int>(r.t - t0), mine = a.pos != nullptr ? a.pos[r.t] : ctx + i;
   const int ntiles = (len + keys - 1) / keys, t_lo = window ? max(0, ctx - window + 1) / keys : 0, nkeep = min(min((keep + keys - 1) / keys, ntiles), t_lo);
-  float* out = &acc.x;
+  float out[4] = {0.f, 0.f, 0.f, 0.f};
   for (int walk = 0; walk < nkeep + ntiles - t_lo; ++walk) {
     if (walk / wk % a.nsplit != split) continue;
     const int j0 = (walk < nkeep ? walk : t_lo + walk - nkeep) * keys;
@@ -247,6 +248,7 @@ __device__ __noinline__ void add_no_numbers(const Args& a, float4& acc, int e, i
       }
     }
   }
+  return make_float4(out[0], out[1], out[2], out[3]);
 }
 
 // A 16-byte piece's place in a tile.  Keys: two neighbouring rows are read together, pieces 4 x .. 4 x + 3 of each: rows of 128 bytes and more turn the odd row's by four.  Values:
@@ -274,6 +276,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
   __shared__ float top_power[kWarps];
   __shared__ float2 joined[kWarps * 16 * MT];
   __shared__ int2 where_to[kWarps * 16 * MT];  // a row's token of the entry and its head; past the last row: the last one's
+  __shared__ float share[8][kWarps * 16 * MT];
   __shared__ int any_bad;
   if (threadIdx.x == 0) any_bad = 0;
   // the step's descriptors are there before its first kernel
@@ -356,39 +359,55 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
   const int tiles_m = wr * MT;
   constexpr int QL = DC == 1 ? 16 : 32;       // lanes of a row
   constexpr int RW = 32 / QL;                 // rows a warp and pass
-#pragma unroll 4
-  for (int rb = 0; rb < rows_cta; rb += kWarps * RW) {
-    const int r = rb + warp * RW + lane / QL, w = lane % QL;
-    const bool in = r0 + r < R;
-    const int i = where_to[r].x, head = where_to[r].y;
-    const int st = w / 4, cc = w % 4;
-    const int d0 = K::C8 ? 64 * (st / 4) + 16 * cc + 4 * (st % 4) : K::F32 ? 16 * st + 4 * cc : 32 * (st / 2) + 8 * cc + 4 * (st % 2);
-    const TQ* q = static_cast<const TQ*>(a.q) + (t0 + i) * (long long)a.H * a.dim + (long long)head * a.dim + d0;
-    float v[4];
+  constexpr int PASS = R8 ? 1 : 4 * MT;            // passes whose loads are under way together
+  const int rows_staged = R8 ? 8 : rows_cta;  // (R8: what stands in the upper half's fragments reaches no output)
+  const int w = lane % QL, st = w / 4, cc = w % 4;
+  const int d0 = K::C8 ? 64 * (st / 4) + 16 * cc + 4 * (st % 4) : K::F32 ? 16 * st + 4 * cc : 32 * (st / 2) + 8 * cc + 4 * (st % 2);
+  const TQ* q0 = static_cast<const TQ*>(a.q) + t0 * a.H * a.dim + (d0 < a.dim ? d0 : 0);
+#pragma unroll 1
+  for (int rb = warp * RW + lane / QL; rb < rows_staged; rb += kWarps * RW * PASS) {  // (whole warps: rows are multiples of eight)
+    float v[PASS][4], by[PASS];
+    int2 to[PASS];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = 0.f;
-    if (in && d0 < a.dim) ld4(v, q, a.vec_q);
-    float s = a.scale * (a.sx.head_scale != nullptr ? a.sx.head_scale[head] : 1.f);
-    if (K::C8) {
-      float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+    for (int u = 0; u < PASS; ++u) to[u] = where_to[min(rb + u * kWarps * RW, rows_cta - 1)];
+    if (a.vec_q) {
 #pragma unroll
-      for (int o = QL / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      // largest element to [2^14, 2^15): a half keeps eleven bits down to 2^-14, and 2^-24 below
-      const int x = min(max(14 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), -100), 100);
-      const float up = __uint_as_float(static_cast<uint32_t>(x + 127) << 23);
-      s *= __uint_as_float(static_cast<uint32_t>(127 - x) << 23);
+      for (int u = 0; u < PASS; ++u) ld4<true>(v[u], q0 + ((long long)to[u].x * a.H + to[u].y) * a.dim);
+    } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] *= up;
+      for (int u = 0; u < PASS; ++u) ld4<false>(v[u], q0 + ((long long)to[u].x * a.H + to[u].y) * a.dim);
     }
-    if (w == 0) unscale[r] = a.mode == kGeneral ? s : a.mode == kCapped ? s * (2.f * kLog2e / a.softcap) : s * kLog2e;
-    uint32_t p[K::QT], s2[K::QT];
-    terms<K::HALF>(v[0], v[1], p);
-    terms<K::HALF>(v[2], v[3], s2);
 #pragma unroll
-    for (int t = 0; t < K::QT; ++t) {  // row r of its tile: lanes 4 (r % 8) + c, first or second half of the fragment's registers
-      uint32_t* f = reinterpret_cast<uint32_t*>(qs + ((t * tiles_m + r / 16) * Q16 + st) * 32 + 4 * (r % 8) + cc) + (r % 16 < 8 ? 0 : 1);
-      f[0] = p[t];
-      f[2] = s2[t];
+    for (int u = 0; u < PASS; ++u) by[u] = a.sx.head_scale != nullptr ? a.sx.head_scale[to[u].y] : 1.f;
+#pragma unroll
+    for (int u = 0; u < PASS; ++u) {
+      const int r = rb + u * kWarps * RW;
+      const bool in = r0 + r < R && d0 < a.dim;
+      float s = a.scale * by[u];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[u][k] = in ? v[u][k] : 0.f;
+      if (K::C8) {
+        float top = fmaxf(fmaxf(fabsf(v[u][0]), fabsf(v[u][1])), fmaxf(fabsf(v[u][2]), fabsf(v[u][3])));
+#pragma unroll
+        for (int o = QL / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        // largest element to [2^14, 2^15): a half keeps eleven bits down to 2^-14, and 2^-24 below
+        const int x = min(max(14 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), -100), 100);
+        const float up = __uint_as_float(static_cast<uint32_t>(x + 127) << 23);
+        s *= __uint_as_float(static_cast<uint32_t>(127 - x) << 23);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[u][k] *= up;
+      }
+      if (r >= rows_staged) break;
+      if (w == 0) unscale[r] = a.mode == kGeneral ? s : a.mode == kCapped ? s * (2.f * kLog2e / a.softcap) : s * kLog2e;
+      uint32_t p[K::QT], s2[K::QT];
+      terms<K::HALF>(v[u][0], v[u][1], p);
+      terms<K::HALF>(v[u][2], v[u][3], s2);
+#pragma unroll
+      for (int t = 0; t < K::QT; ++t) {  // row r of its tile: lanes 4 (r % 8) + c, first or second half of the fragment's registers
+        uint32_t* f = reinterpret_cast<uint32_t*>(qs + ((t * tiles_m + r / 16) * Q16 + st) * 32 + 4 * (r % 8) + cc) + (r % 16 < 8 ? 0 : 1);
+        f[0] = p[t];
+        f[2] = s2[t];
+      }
     }
   }
   __syncthreads();
@@ -754,18 +773,31 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
     float m = -INFINITY, l = 0.f;
     for (int w = 0; w < wk; ++w) m = fmaxf(m, stat[w * wr + tile][in].x);
     const float ref = m == -INFINITY ? 0.f : m;
+    for (int w = 0; w < wk; ++w) l += ex2(stat[w * wr + tile][in].x - ref) * stat[w * wr + tile][in].y;  // (scores that are no numbers stay in the sum)
+    const float by = a.nsplit == 1 ? last_factor(a, where_to[r].y, ref, l) : 1.f;
     for (int w = 0; w < wk; ++w) {
       float2& st = stat[w * wr + tile][in];
-      const float f = ex2(st.x - ref);
-      l += f * st.y;  // (scores that are no numbers stay in the sum)
-      st.x = K::C8 ? f * exp2f(top_power[w * wr + tile] - 142.f) : f;  // the weights' power: 2^(P - 127 - 15)
+      st.x = ex2(st.x - ref) * by * (K::C8 ? exp2f(top_power[w * wr + tile] - 142.f) : 1.f);  // the weights' power: 2^(P - 127 - 15)
     }
     joined[r] = make_float2(m, l);
   }
   __syncthreads();
   const int quads = a.vdim / 4, per_pass = 32 * kWarps / quads, row_of = tid / quads, col = 4 * (tid - row_of * quads);  // four columns a thread
   auto row_at = [&](int r) { return Row{t0 + where_to[r].x, where_to[r].y}; };
-#pragma unroll 2
+  if (any_bad) {  // values that are no numbers, into the first warp's sums
+    for (int r = row_of < per_pass ? row_of : rows_here; r < rows_here; r += per_pass) {
+      const int tile = r / (16 * MT), in = r % (16 * MT);
+      const float4 v = no_number_values<TC>(a, e, g, row_at(r), col, split, wk, KT);
+      add(*reinterpret_cast<float4*>(os + (tile * 16 * MT + in) * ldo_s + col), 1.f, v);
+    }
+    __syncthreads();
+    for (int r = tid; r < rows_here; r += 32 * kWarps) {
+      float2& st = stat[r / (16 * MT)][r % (16 * MT)];
+      if (st.x == 0.f) st.x = 1e-30f;  // (a factor of zero would leave them out)
+    }
+    __syncthreads();
+  }
+#pragma unroll 4
   for (int r = row_of < per_pass ? row_of : rows_here; r < rows_here; r += per_pass) {
     const int tile = r / (16 * MT), in = r % (16 * MT);
     const Row where = row_at(r);
@@ -777,52 +809,61 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
       const float f = stat[ww][in].x;
       if (f != 0.f) add(acc, f, *reinterpret_cast<const float4*>(os + (ww * 16 * MT + in) * ldo_s + col));
     }
-    if (any_bad) add_no_numbers<TC>(a, acc, e, g, where, col, split, wk, KT);
-    const float m = joined[r].x, l = joined[r].y;
     if (a.nsplit == 1) {
-      finish<TQ>(a, where, col, m == -INFINITY ? 0.f : m, l, acc, gv);
+      put<TQ>(a, where, col, acc, gv);
     } else if (a.cluster) {  // over the first warp's, whose columns only this thread reads
       *reinterpret_cast<float4*>(os + (tile * 16 * MT + in) * ldo_s + col) = acc;
     } else {
       float* pp = a.partial + (((a.singles ? (long long)e : where.t) * a.H + where.head) * a.nsplit + split) * (a.vdim + 4);
       *reinterpret_cast<float4*>(pp + 4 + col) = acc;
-      if (col == 0) *reinterpret_cast<float2*>(pp) = make_float2(m, l);
+      if (col == 0) *reinterpret_cast<float2*>(pp) = joined[r];
     }
   }
   if (!a.cluster) return;
   // ---- the CTAs of a cluster share out the rows' columns and read one another's results
   pg::cluster_sync_all();
+  auto of_cta = [&](const void* p, int cta) {
+    uint32_t x;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(x) : "r"(pg::smem_u32(p)), "r"(cta));
+    return x;
+  };
+  for (int r = tid; r < rows_here; r += 32 * kWarps) {
+    float2 st[8];
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      st[p] = make_float2(-INFINITY, 0.f);
+      if (p < a.nsplit) asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(st[p].x), "=f"(st[p].y) : "r"(of_cta(&joined[r], p)) : "memory");
+    }
+#pragma unroll
+    for (int p = 0; p < 8; ++p) m = fmaxf(m, st[p].x);
+    const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) l += ex2(st[p].x - ref) * st[p].y;
+    const float by = last_factor(a, where_to[r].y, ref, l);
+#pragma unroll
+    for (int p = 0; p < 8; ++p) share[p][r] = ex2(st[p].x - ref) * by;
+  }
+  __syncthreads();
   for (int r = (row_of < per_pass ? row_of : rows_here) + per_pass * split; r < rows_here; r += per_pass * a.nsplit) {
     const int tile = r / (16 * MT), in = r % (16 * MT);
     const Row where = row_at(r);
     float gv[4];
     gates<TQ>(a, where, col, gv);
-    const uint32_t sa = pg::smem_u32(&joined[r]), oa = pg::smem_u32(os + (tile * 16 * MT + in) * ldo_s + col);
-    float2 st[8];
-    float4 v[8];
+    const float* mine = os + (tile * 16 * MT + in) * ldo_s + col;
+    float4 v[8], acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
       if (p >= a.nsplit) break;
-      uint32_t x, y;
-      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(x) : "r"(sa), "r"(p));
-      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(y) : "r"(oa), "r"(p));
-      asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(st[p].x), "=f"(st[p].y) : "r"(x) : "memory");
-      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[p].x), "=f"(v[p].y), "=f"(v[p].z), "=f"(v[p].w) : "r"(y) : "memory");
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[p].x), "=f"(v[p].y), "=f"(v[p].z), "=f"(v[p].w) : "r"(of_cta(mine, p)) : "memory");
     }
-    float m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int p = 0; p < 8; ++p)
-      if (p < a.nsplit) m = fmaxf(m, st[p].x);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
       if (p >= a.nsplit) break;
-      const float f = ex2(st[p].x - ref);
-      l += f * st[p].y;
+      const float f = share[p][r];
       if (f != 0.f) add(acc, f, v[p]);
     }
-    finish<TQ>(a, where, col, ref, l, acc, gv);
+    put<TQ>(a, where, col, acc, gv);
   }
   pg::cluster_sync_all();  // nobody leaves while its memory is read
 }
@@ -878,7 +919,8 @@ __global__ void __launch_bounds__(128) attn_rows_merge_kernel(const __grid_const
     const Row where{t, head};
     float gv[4];
     gates<TQ>(a, where, col, gv);
-    finish<TQ>(a, where, col, whole[0], whole[1], acc, gv);
+    const float by = last_factor(a, head, whole[0], whole[1]);
+    put<TQ>(a, where, col, make_float4(acc.x * by, acc.y * by, acc.z * by, acc.w * by), gv);
   }
 }
 
