@@ -159,28 +159,20 @@ struct Kind {
   static constexpr int ES = sizeof(TC);
   static constexpr bool C8 = ES == 1, F32 = ES == 4, HALF = C8;
   static constexpr int QT = F32 ? 3 : (C8 && sizeof(TQ) == 4) ? 2 : 1;     // terms of a query
+  static constexpr int STEPS = 4 * DC;                                     // 16-deep steps of the first product
   static constexpr int CT = F32 ? 3 : 1;                                   // terms of a cached element
   static constexpr int PT = F32 ? 3 : C8 ? (sizeof(TQ) == 4 ? 2 : 1) : 2;  // terms of a weight
   static constexpr int VW = 2 * ES;                                        // words of eight value columns
   static constexpr int KROW = 64 * DC * ES, VROW = 64 * VC * ES;           // bytes of a row in shared memory
   static constexpr int STAGE = KT * (KROW + VROW) + (C8 ? 2 * KT : 0);
   static constexpr int STAGES = STAGE > 8 * 1024 + 256 ? 2 : 3;
-  static constexpr int Q_BYTES = QT * MT * 4 * DC * 512;  // of a warp's rows
+  static constexpr int Q_BYTES = QT * MT * STEPS * 512;  // of a warp's rows
 };
 
 // what registers and shared memory leave room for
 template <typename TQ, typename TC, int DC, int VC, int MT>
 constexpr int ctas_per_sm() {
-#ifndef OCC
-#define OCC 4
-#endif
-#ifndef OCCW
-#define OCCW 2
-#endif
-#ifndef OCCM
-#define OCCM 3
-#endif
-  return DC > 1 || VC > 1 ? OCCW : sizeof(TC) == 4 ? 2 : MT == 2 ? OCCM : sizeof(TC) == 1 ? OCC : 2;
+  return DC > 1 || VC > 1 || sizeof(TC) == 4 ? 2 : MT == 2 ? 3 : sizeof(TC) == 1 ? 4 : 2;
 }
 
 // where a row of a k/v head's block goes
@@ -269,7 +261,6 @@ template <typename TQ, typename TC, int DC, int VC, int MT, int KT, bool R8>
 __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>())) attn_rows_kernel(const __grid_constant__ Args a) {
   using K = Kind<TQ, TC, DC, VC, MT, KT>;
   constexpr int NB = KT / 8, KPL = KT / 4;  // key fragments of a tile; keys of a lane
-  constexpr int Q16 = 4 * DC;
   extern __shared__ __align__(128) unsigned char raw[];
   __shared__ float unscale[kWarps * 16 * MT];  // what a row's scores are multiplied by
   __shared__ float2 stat[kWarps][16 * MT];
@@ -399,14 +390,17 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
       }
       if (r >= rows_staged) break;
       if (w == 0) unscale[r] = a.mode == kGeneral ? s : a.mode == kCapped ? s * (2.f * kLog2e / a.softcap) : s * kLog2e;
-      uint32_t p[K::QT], s2[K::QT];
-      terms<K::HALF>(v[u][0], v[u][1], p);
-      terms<K::HALF>(v[u][2], v[u][3], s2);
+      // row r of its tile: lanes 4 (r % 8) + c, first or second half of the fragment's registers
+      {
+        uint32_t p[K::QT], s2[K::QT];
+        terms<K::HALF>(v[u][0], v[u][1], p);
+        terms<K::HALF>(v[u][2], v[u][3], s2);
 #pragma unroll
-      for (int t = 0; t < K::QT; ++t) {  // row r of its tile: lanes 4 (r % 8) + c, first or second half of the fragment's registers
-        uint32_t* f = reinterpret_cast<uint32_t*>(qs + ((t * tiles_m + r / 16) * Q16 + st) * 32 + 4 * (r % 8) + cc) + (r % 16 < 8 ? 0 : 1);
-        f[0] = p[t];
-        f[2] = s2[t];
+        for (int t = 0; t < K::QT; ++t) {
+          uint32_t* f = reinterpret_cast<uint32_t*>(qs + ((t * tiles_m + r / 16) * K::STEPS + st) * 32 + 4 * (r % 8) + cc) + (r % 16 < 8 ? 0 : 1);
+          f[0] = p[t];
+          f[2] = s2[t];
+        }
       }
     }
   }
@@ -422,13 +416,14 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
     uns[x] = unscale[r];
   }
 
-  float M[2 * MT], L[2 * MT], o[MT][8 * VC][4];
+  constexpr int OB = R8 ? 4 * VC : 8 * VC;  // R8: transposed, 16 columns x eight rows an instruction
+  float M[2 * MT], L[2 * MT], o[MT][OB][4];
 #pragma unroll
   for (int x = 0; x < 2 * MT; ++x) M[x] = a.sx.logistic ? 0.f : -INFINITY, L[x] = 0.f;
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int b = 0; b < 8 * VC; ++b)
+    for (int b = 0; b < OB; ++b)
 #pragma unroll
       for (int k = 0; k < 4; ++k) o[m][b][k] = 0.f;
   int P = 0;  // largest power of a value row so far (byte)
@@ -502,9 +497,9 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
       for (int f = 0; f < NB; ++f)
 #pragma unroll
         for (int k = 0; k < 4; ++k) s[m][f][k] = 0.f;
-    constexpr int SPL = K::C8 ? 4 : K::F32 ? 1 : 2;  // 16-deep steps of a piece
+    constexpr int SPL = K::C8 ? 4 : K::F32 ? 1 : 2;  // steps of a piece
 #pragma unroll
-    for (int x = 0; x < Q16 / SPL; ++x) {
+    for (int x = 0; x < K::STEPS / SPL; ++x) {
       uint4 kk[NB];
 #pragma unroll
       for (int f = 0; f < NB; ++f) kk[f] = *reinterpret_cast<const uint4*>(stage + key_place<K::KROW>(KPL * (nn >> 1) + 2 * f + (nn & 1), 4 * x + c));
@@ -515,7 +510,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int t = 0; t < K::QT; ++t) qa[m][t] = qs[((t * tiles_m + rg * MT + m) * Q16 + st) * 32 + lane];
+          for (int t = 0; t < K::QT; ++t) qa[m][t] = qs[((t * tiles_m + rg * MT + m) * K::STEPS + st) * 32 + lane];
 #pragma unroll
         for (int f = 0; f < NB; ++f) {
           uint32_t b0[K::CT], b1[K::CT];
@@ -659,13 +654,19 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
         moved |= corr[x] != 1.f;
       }
     if (__any_sync(0xffffffffu, moved)) {
+      if (R8) {  // my accumulators are rows 2 c and 2 c + 1
+        const float even = __shfl_sync(0xffffffffu, corr[0], 8 * c), odd = __shfl_sync(0xffffffffu, corr[0], 8 * c + 4);
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+        for (int b = 0; b < OB; ++b) o[0][b][0] *= even, o[0][b][1] *= odd, o[0][b][2] *= even, o[0][b][3] *= odd;
+      } else {
 #pragma unroll
-        for (int b = 0; b < 8 * VC; ++b) {
-          o[m][b][0] *= corr[2 * m], o[m][b][1] *= corr[2 * m];
-          if (!R8) o[m][b][2] *= corr[2 * m + HS - 1], o[m][b][3] *= corr[2 * m + HS - 1];
-        }
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int b = 0; b < OB; ++b) {
+            o[m][b][0] *= corr[2 * m], o[m][b][1] *= corr[2 * m];
+            o[m][b][2] *= corr[2 * m + HS - 1], o[m][b][3] *= corr[2 * m + HS - 1];
+          }
+      }
     }
     uint4 pa[MT][NB / 2][K::PT];
 #pragma unroll
@@ -708,9 +709,11 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
         }
 #pragma unroll
       for (int b = 0; b < VC; ++b) {
+        uint32_t w0[2][K::CT], w1[2][K::CT];  // two neighbouring columns: keys 4 q, 4 q + 1 and 4 q + 2, 4 q + 3
 #pragma unroll
         for (int y = 0; y < 8; ++y) {  // column 8 n + y of the piece
-          uint32_t b0[K::CT], b1[K::CT];
+          uint32_t(&b0)[K::CT] = w0[y % 2];
+          uint32_t(&b1)[K::CT] = w1[y % 2];
           if (K::C8) {
             const int w = y / 4, sel = y % 4;
             const uint32_t lo = __byte_perm(vv[0][b][w], vv[1][b][w], sel < 2 ? 0x5140 : 0x7362), hi = __byte_perm(vv[2][b][w], vv[3][b][w], sel < 2 ? 0x5140 : 0x7362);
@@ -725,13 +728,17 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
             b0[0] = __byte_perm(vv[0][b][w], vv[1][b][w], y % 2 ? 0x7632 : 0x5410);
             b1[0] = __byte_perm(vv[2][b][w], vv[3][b][w], y % 2 ? 0x7632 : 0x5410);
           }
+          if (R8 && y % 2 == 0) continue;
 #pragma unroll
           for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int t = K::PT - 1; t >= 0; --t)
 #pragma unroll
               for (int t2 = K::CT - 1; t2 >= 0; --t2)
-                if (t + t2 < 3) mma<K::HALF>(o[m][8 * b + y], pa[m][q][t], b0[t2], b1[t2]);
+                if (t + t2 < 3) {
+                  if (R8) mma<K::HALF>(o[0][(4 * b + y / 2) % OB], make_uint4(w0[0][t2], w0[1][t2], w1[0][t2], w1[1][t2]), pa[0][q][t].x, pa[0][q][t].z);
+                  else mma<K::HALF>(o[m][(8 * b + y) % OB], pa[m][q][t], b0[t2], b1[t2]);
+                }
         }
       }
     }
@@ -749,7 +756,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     const int r = 16 * (x / 2) + 8 * (x % 2) + nn;
     if (c == 0) stat[warp][r] = make_float2(M[x], l);
-    if (R8 && x % 2 == 1) continue;
+    if (R8) continue;
     float* dst = os + (warp * 16 * MT + r) * ldo_s;
 #pragma unroll
     for (int b = 0; b < VC; ++b)
@@ -759,10 +766,22 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
         if (col < a.vdim) {
 #pragma unroll
           for (int y = 0; y < 8; y += 4)
-            *reinterpret_cast<float4*>(dst + col + y) = make_float4(o[x / 2][8 * b + y][2 * (x % 2) + k], o[x / 2][8 * b + y + 1][2 * (x % 2) + k], o[x / 2][8 * b + y + 2][2 * (x % 2) + k],
-                                                                    o[x / 2][8 * b + y + 3][2 * (x % 2) + k]);
+            *reinterpret_cast<float4*>(dst + col + y) = make_float4(o[x / 2][(8 * b + y) % OB][2 * (x % 2) + k], o[x / 2][(8 * b + y + 1) % OB][2 * (x % 2) + k],
+                                                                    o[x / 2][(8 * b + y + 2) % OB][2 * (x % 2) + k], o[x / 2][(8 * b + y + 3) % OB][2 * (x % 2) + k]);
         }
       }
+  }
+  if (R8) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)  // rows 2 c and 2 c + 1, columns 8 n .. 8 n + 7 of every 64
+#pragma unroll
+      for (int b = 0; b < VC; ++b)
+        if (64 * b + 8 * nn < a.vdim) {
+          float* dst = os + (warp * 16 * MT + 2 * c + i) * ldo_s + 64 * b + 8 * nn;
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+            *reinterpret_cast<float4*>(dst + 4 * y) = make_float4(o[0][4 * b + 2 * y][i], o[0][4 * b + 2 * y][2 + i], o[0][4 * b + 2 * y + 1][i], o[0][4 * b + 2 * y + 1][2 + i]);
+        }
   }
   if (K::C8 && lane == 0) top_power[warp] = static_cast<float>(P);
   if (bad) any_bad = 1;
@@ -939,12 +958,9 @@ Plan plan_of(const PgAttnRows& p, int rows, int row_tile, int keys, int per_sm) 
     reach = reach < w ? reach : w;
   }
   const long long tiles = (reach + keys - 1) / keys, ctas = (long long)p.busy * p.G * x.blocks;
-  // CTAs that share a walk: what the SMs hold at once, and at least PG_ROWS_TILES tiles for a warp
-#ifndef PG_ROWS_TILES
-#define PG_ROWS_TILES 2
-#endif
+  // CTAs that share a walk: what the SMs hold at once, and at least two tiles for a warp
   long long n = (long long)per_sm * pg::num_sms() / (ctas > 0 ? ctas : 1);
-  const long long most = tiles * x.wr / (PG_ROWS_TILES * kWarps);
+  const long long most = tiles * x.wr / (2 * kWarps);
   n = n < most ? n : most;
   n = n > 64 ? 64 : n < 1 ? 1 : n;
   // up to eight join through distributed shared memory in one launch; more, where that leaves warps with a long walk, through global memory and a second one
