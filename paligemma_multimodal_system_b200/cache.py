@@ -9,6 +9,9 @@ A model describes what each of its layers keeps per sequence (`cache_layout()`):
     ("state", shape)                    one fp32 tensor per sequence             -> [num_slots, *shape]
     None                                nothing
 
+A "kv" layer that says how many heads its rows hold (`KvSpec`) can keep them in 8 bits (`kv_format="e4m3"`: seq_ops.QuantizedPages, an e4m3 code per element
+and a power of two per row and head, a little over half of bfloat16's bytes); latent rows and states keep their types.
+
 `SequenceStore` owns the device tensors and the host-side bookkeeping (free lists, per-request page lists and lengths).
 Pages and slots go back to the free lists when a request is released and are handed out again, lowest id first, so a
 second request really does land on memory a finished one used.  Nothing is cleared on reuse: a sequence's first step
@@ -19,6 +22,18 @@ from typing import Dict, List, Optional, Sequence
 import torch
 
 from .modeling_gemma import PAGE
+from .seq_ops import QuantizedPages
+
+KV_FORMATS = (None, "e4m3")
+
+
+class KvSpec(tuple):
+    """("kv", key_width, value_width) that also knows the number of key / value heads in a row."""
+
+    def __new__(cls, key_width: int, value_width: int, heads: int):
+        self = super().__new__(cls, ("kv", int(key_width), int(value_width)))
+        self.heads = int(heads)
+        return self
 
 
 class PagePool:
@@ -54,8 +69,12 @@ class SequenceRecord:
 class SequenceStore:
     """Pages + state slots of the live requests of one engine."""
 
-    def __init__(self, layout, max_tokens: int, num_slots: int, dtype: torch.dtype, device="cuda", allocate: bool = True):
+    def __init__(self, layout, max_tokens: int, num_slots: int, dtype: torch.dtype, device="cuda", allocate: bool = True,
+                 kv_format: Optional[str] = None):
+        if kv_format not in KV_FORMATS:
+            raise ValueError(f"unknown cache format {kv_format!r} (known: {KV_FORMATS})")
         self.page = PAGE
+        self.kv_format = kv_format
         self.num_slots = int(num_slots)
         num_pages = (int(max_tokens) + PAGE - 1) // PAGE
         self.pool = PagePool(num_pages)
@@ -67,7 +86,16 @@ class SequenceStore:
         self.state: List[Optional[torch.Tensor]] = []
         for spec in self.layout:
             k = v = s = None
-            if allocate and spec is not None and spec[0] == "kv":
+            if kv_format is not None and spec is not None and spec[0] == "kv":
+                heads = getattr(spec, "heads", None)
+                if heads is None:
+                    raise ValueError("a layer that does not say how many heads its rows hold cannot be kept in 8 bits")
+                sizes = (spec[1] // heads, spec[2] // heads)
+                if any(n % 16 or n > 128 for n in sizes):
+                    raise ValueError(f"the 8-bit cache serves heads of a multiple of 16 elements up to 128: got {sizes[0]} and {sizes[1]}")
+                if allocate:
+                    k, v = (QuantizedPages.empty(num_pages, PAGE, heads, n, device) for n in sizes)
+            elif allocate and spec is not None and spec[0] == "kv":
                 k = torch.zeros(num_pages, PAGE, spec[1], device=device, dtype=dtype)
                 v = torch.zeros(num_pages, PAGE, spec[2], device=device, dtype=dtype)
             elif allocate and spec is not None and spec[0] == "latent":

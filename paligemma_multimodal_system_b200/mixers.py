@@ -37,6 +37,7 @@ import math
 import torch
 
 from . import _lib, seq_ops
+from .cache import KvSpec
 from .modeling_gemma import PAGE
 
 
@@ -89,7 +90,7 @@ class GatedSoftmaxAttention:
         self.freq = rotary_frequencies(rot_base, rot_dims, rot_scaling) if rot_dims else torch.zeros(1, dtype=torch.float64)
 
     def cache_spec(self):
-        return ("kv", self.G * self.dim, self.G * self.vdim)
+        return KvSpec(self.G * self.dim, self.G * self.vdim, self.G)
 
     def load(self, take, pre):
         H, G, dim, vdim, D = self.H, self.G, self.dim, self.vdim, self.D
@@ -160,7 +161,7 @@ class WindowedSoftmaxAttention:
             self.freq = rotary_frequencies(rot_base, rot_dims) if rot_dims else torch.zeros(1, dtype=torch.float64)
 
     def cache_spec(self):
-        return None if self.kv_from is not None else ("kv", self.G * self.dim, self.G * self.vdim)
+        return None if self.kv_from is not None else KvSpec(self.G * self.dim, self.G * self.vdim, self.G)
 
     def cache_specs(self):
         return [self.cache_spec()]
@@ -818,7 +819,7 @@ class LogisticAttention(ProjectedMixer):
         self.freq = rotary_frequencies(rot_base, rot_dims) if rot_dims else torch.zeros(1, dtype=torch.float64)
 
     def cache_specs(self):
-        return [("kv", self.G * self.dim, self.G * self.vdim)]
+        return [KvSpec(self.G * self.dim, self.G * self.vdim, self.G)]
 
     def load(self, take, pre):
         H, G, dim, vdim, D = self.H, self.G, self.dim, self.vdim, self.D
