@@ -519,7 +519,7 @@ int pg_attn_prepare_at(const void* qkv, long long ld, const int* pos, const int*
  * nearest code, ties to even; infinities and NaN are stored as the NaN code.
  * pg_attn_prepare_e4m3: pg_attn_prepare_at into such pages.  dim and vdim multiples of 16 up to 256; codes and q_out on 16-byte boundaries.
  * pg_kv_read_e4m3: rows 0 .. ctx + n of every entry with entry_n > 1, in fp32 (out_f32) or bf16, to rows dense_row0[e] .. of k_out [.., G * dim] and
- * v_out [.., G * vdim]; zeros behind the last row up to a multiple of 64 rows.  longest: at least the largest ctx + n among them (sizes the grid). */
+ * v_out [.., G * vdim]; zeros behind the last row up to a multiple of 64 rows.  longest: at least the largest ctx + n among them (sizes the grid); page a multiple of 16. */
 typedef struct PgPrepareE4m3 { /* as pg_attn_prepare_at's arguments */
   const void* qkv;
   long long ld;

@@ -270,7 +270,9 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
   __shared__ float share[8][kWarps * 16 * MT];
   __shared__ int any_bad;
   if (threadIdx.x == 0) any_bad = 0;
-  // the step's descriptors are there before its first kernel
+  // (the step's descriptors, too, may come from the kernel in front)
+  if (a.nsplit > 1 && !a.cluster) pg::griddep_begin<true>();  // (fp32 partials, read behind a wait)
+  else pg::griddep_begin_if(a.trigger);
   const int split = blockIdx.x, g = blockIdx.y / a.blocks, block = blockIdx.y % a.blocks, e = blockIdx.z;
   const int n = a.n[e], ctx = a.ctx[e], gsz = a.H / a.G, len = ctx + n;
   const long long t0 = a.row0[e];
@@ -295,8 +297,6 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
     return w < nwalk ? pt[tile_of(w) >> a.tile_shift] : 0;
   };
   int pids = pages_from(walk0);
-  if (a.nsplit > 1 && !a.cluster) pg::griddep_begin<true>();  // (fp32 partials, read behind a wait)
-  else pg::griddep_begin_if(a.trigger);
   if (!mine) return;
 
   // ---- copies: a ring of tiles for the warps that walk together, 16 bytes a thread and request
@@ -895,9 +895,9 @@ __global__ void __launch_bounds__(128) attn_rows_merge_kernel(const __grid_const
   __shared__ float fs[64];
   __shared__ float whole[2];
   const int e = blockIdx.z, head = blockIdx.x, i = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pg::griddep_begin_if(a.trigger);
   const int n = a.n[e];
   const long long t = a.row0[e] + i;
-  pg::griddep_begin_if(a.trigger);
   if (i >= n || (a.singles && n != 1)) return;
   const int ld = a.vdim + 4, col = 4 * lane;
   const float* pp = a.partial + ((a.singles ? (long long)e : t) * a.H + head) * a.nsplit * ld;
@@ -1071,6 +1071,7 @@ int attn_rows(const PgAttnRows* q, long long* need, void* scratch, long long scr
   const int four = p.act_f32 ? 16 : 8;  // bytes of four elements
   a.vec_q = aligned(p.q, four), a.vec_gate = aligned(p.gate, four) && p.ldg % 4 == 0, a.vec_out = aligned(p.out, four) && a.sx.out_ld % 4 == 0;
   a.trigger = pg::weights_follow();
+  if ((long long)p.max_n * (p.H / p.G) > 1 << 24) return PG_ERR_ARG;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (p.e4m3) return p.act_f32 ? by_rows<float, e4m3, 32>(p, a, need, scratch_bytes, st) : by_rows<bf16, e4m3, 32>(p, a, need, scratch_bytes, st);
   return p.act_f32 ? by_rows<float, float, 16>(p, a, need, scratch_bytes, st) : by_rows<bf16, bf16, 32>(p, a, need, scratch_bytes, st);

@@ -70,31 +70,33 @@ static_assert(sizeof(PgPrepareE4m3) == 192 && sizeof(PgReadE4m3) == 112, "caller
 // which share its weights, or four heads of one token.
 // What bounds it: for prompts instructions, then the bytes (a row is read once, 8-bit rows are half of bf16 ones); for a few rows the chain row -> sum -> largest -> codes.
 template <typename TA, int LG, int TOK, bool VEC>
-__global__ void __launch_bounds__(128, sizeof(TA) == 2 ? 8 : 5) attn_prepare_e4m3_kernel(const __grid_constant__ Prepare a) {
+__global__ void __launch_bounds__(128, sizeof(TA) == 2 ? 7 : 5) attn_prepare_e4m3_kernel(const __grid_constant__ Prepare a) {
   constexpr int U = 4, NG = 128 / LG, HEADS = TOK == 1 ? U : 1;  // HEADS: head vectors of a round
   extern __shared__ __align__(16) float cs[];  // [TOK][cos rot / 2 | sin rot / 2]
   __shared__ float part[2][TOK][4];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, l = tid % LG, group = tid / LG, d0 = 8 * l;
   const int t0 = blockIdx.x * TOK, nvec = a.H + 2 * a.G, half = a.rot / 2;
   const TA* qkv = static_cast<const TA*>(a.qkv);
-  long long kv_row[TOK], power_row[TOK];  // the token's row of codes, its byte of a page's first head
-#pragma unroll
-  for (int k = 0; k < TOK; ++k) {  // (positions and pages are the host's)
-    const int t = min(t0 + k, a.rows - 1), where = a.at[t], slot = where % a.page;
-    const long long page = a.page_table[(long long)a.row_entry[t] * a.max_pages + where / a.page];
-    kv_row[k] = page * a.page + slot;
-    power_row[k] = page * a.G * a.page + slot;
-  }
+  __shared__ long long kv_row[TOK], power_row[TOK];  // a token's row of codes, its byte of a page's first head
   pg::griddep_begin();
+  if (tid < TOK) {
+    const int t = min(t0 + tid, a.rows - 1), where = a.at[t], slot = where % a.page;
+    const long long page = a.page_table[(long long)a.row_entry[t] * a.max_pages + where / a.page];
+    kv_row[tid] = page * a.page + slot;
+    power_row[tid] = page * a.G * a.page + slot;
+  }
   Eight<TA> raw[U];
+  const TA* rows[TOK];
+#pragma unroll
+  for (int k = 0; k < TOK; ++k) rows[k] = qkv + min(t0 + k, a.rows - 1) * a.ld + d0;
   auto request = [&](int vec0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int vec = TOK == 1 ? vec0 + u * NG : vec0, t = min(t0 + (TOK == 1 ? 0 : u), a.rows - 1);
+      const int vec = TOK == 1 ? vec0 + u * NG : vec0;
       raw[u].zero();
       if (vec < nvec && d0 < (vec < a.H + a.G ? a.dim : a.vdim)) {
-        const long long off = vec < a.H + a.G ? vec * a.dim : a.v_from_k ? (vec - a.G) * a.dim : (a.H + a.G) * a.dim + (vec - a.H - a.G) * a.vdim;
-        raw[u].template load<VEC>(qkv + t * a.ld + off + d0);
+        const int off = vec < a.H + a.G ? vec * a.dim : a.v_from_k ? (vec - a.G) * a.dim : (a.H + a.G) * a.dim + (vec - a.H - a.G) * a.vdim;
+        raw[u].template load<VEC>(rows[TOK == 1 ? 0 : u] + off);
       }
     }
   };
@@ -131,13 +133,19 @@ __global__ void __launch_bounds__(128, sizeof(TA) == 2 ? 8 : 5) attn_prepare_e4m
       const int vec = vec0 + h * NG;
       const bool is_q = vec < a.H, is_k = !is_q && vec < a.H + a.G, is_v = !is_q && !is_k;
       const int n = is_v ? a.vdim : a.dim, head = is_q ? vec : is_k ? vec - a.H : vec - a.H - a.G;
+      const float mean = 1.0f / (float)n;
       const bool mine = vec < nvec && d0 < n, quantised = __any_sync(0xffffffffu, !is_q);  // a group of this warp has a key or a value
       float w[8];
       const float* wp = is_v ? nullptr : is_q ? a.q_norm : a.k_norm;  // NULL: a norm without a weight
       if (wp != nullptr && mine) {
         wp += a.norm_qk == 2 ? head * a.dim + d0 : d0;
+        if (VEC) {
+          const float4 lo = reinterpret_cast<const float4*>(wp)[0], hi = reinterpret_cast<const float4*>(wp)[1];
+          w[0] = lo.x, w[1] = lo.y, w[2] = lo.z, w[3] = lo.w, w[4] = hi.x, w[5] = hi.y, w[6] = hi.z, w[7] = hi.w;
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = wp[i];
+          for (int i = 0; i < 8; ++i) w[i] = wp[i];
+        }
       }
 #pragma unroll
       for (int k = 0; k < TOK; ++k) {
@@ -152,7 +160,7 @@ __global__ void __launch_bounds__(128, sizeof(TA) == 2 ? 8 : 5) attn_prepare_e4m
           for (int i = 0; i < 8; ++i) s = fmaf(x[i], x[i], s);
 #pragma unroll
           for (int o = LG / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-          if (is_v ? a.norm_v != 0 : a.norm_qk == 1) inv = rsqrtf(s * (1.0f / (float)n) + a.eps);
+          if (is_v ? a.norm_v != 0 : a.norm_qk == 1) inv = rsqrtf(s * mean + a.eps);
         }
         if (a.norm_qk == 2 && !is_v) {
           const float* p = part[is_q ? 0 : 1][k];
@@ -214,14 +222,14 @@ __global__ void __launch_bounds__(128, sizeof(TA) == 2 ? 8 : 5) attn_prepare_e4m
         }
         if (!mine || t >= a.rows) continue;
         if (is_q) {
-          put8(static_cast<TA*>(a.q_out) + (t * a.H + head) * a.dim + d0, x);
+          put8(static_cast<TA*>(a.q_out) + t * (a.H * a.dim) + (head * a.dim + d0), x);
         } else {
           const uint32_t byte = cache8::power_of(__float_as_uint(top));
           const float up = cache8::inverse_of_power(byte);
           uint2 codes;
           codes.x = cache8::codes_of(x[0] * up, x[1] * up) | cache8::codes_of(x[2] * up, x[3] * up) << 16;
           codes.y = cache8::codes_of(x[4] * up, x[5] * up) | cache8::codes_of(x[6] * up, x[7] * up) << 16;
-          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(is_k ? a.k_codes : a.v_codes) + (kv_row[k] * a.G + head) * n + d0) = codes;
+          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(is_k ? a.k_codes : a.v_codes) + kv_row[k] * (a.G * n) + (head * n + d0)) = codes;
           if (l == 0) static_cast<uint8_t*>(is_k ? a.k_powers : a.v_powers)[power_row[k] + head * a.page] = static_cast<uint8_t>(byte);
         }
       }
@@ -229,46 +237,63 @@ __global__ void __launch_bounds__(128, sizeof(TA) == 2 ? 8 : 5) attn_prepare_e4m
   }
 }
 
-// 16 codes a thread and step.  Rows behind an entry's last one up to the end of its last page are zeros: whoever walks whole tiles of the scratch reads numbers.
+// 16 codes (bf16: two 16-byte pieces of output) or four (fp32: one) a thread and step, fp32 four steps under way together; a CTA's 16 rows lie in one page.  Rows behind an entry's last one up to the end of its last run of 64
+// are zeros: whoever walks whole tiles of the scratch reads numbers.  What bounds it: the bytes, half again as many as it writes in bf16.
 constexpr int kReadRows = 16;
 template <typename TO>
 __global__ void __launch_bounds__(256) kv_read_e4m3_kernel(const __grid_constant__ PgReadE4m3 a) {
+  constexpr int E = sizeof(TO) == 2 ? 16 : 4, U = sizeof(TO) == 2 ? 1 : 4;  // codes of a piece; pieces of a thread and round
+  pg::griddep_begin();
   const int e = blockIdx.y, n = a.entry_n[e], len = a.entry_ctx[e] + n, j0 = blockIdx.x * kReadRows;
   const int end = (len + 63) / 64 * 64;  // the scratch has whole runs of 64 rows
   if (n <= 1 || j0 >= end) return;
   const bool is_k = blockIdx.z == 0;
-  const int size = is_k ? a.dim : a.vdim, pieces = a.G * size / 16, per_head = size / 16;
-  const uint8_t* codes = static_cast<const uint8_t*>(is_k ? a.k_codes : a.v_codes);
-  const uint8_t* powers = static_cast<const uint8_t*>(is_k ? a.k_powers : a.v_powers);
-  TO* out = static_cast<TO*>(is_k ? a.k_out : a.v_out) + (a.dense_row0[e] + (long long)j0) * a.G * size;
-  const int* pages = a.page_table + (long long)e * a.max_pages;
-  const int rows = min(kReadRows, end - j0);
-  pg::griddep_begin();
-#pragma unroll 4
-  for (int i = threadIdx.x; i < rows * pieces; i += 256) {
-    const int r = i / pieces, p = i - r * pieces, j = j0 + r, head = p / per_head;
-    uint4 c = make_uint4(0, 0, 0, 0);
-    uint32_t byte = 127;
-    if (j < len) {
-      const long long id = pages[j / a.page];
-      const int slot = j % a.page;
-      c = *reinterpret_cast<const uint4*>(codes + (id * a.page + slot) * a.G * size + 16 * p);
-      byte = powers[(id * a.G + head) * a.page + slot];
-    }
-    const float s = cache8::value_of_power(byte);
-    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-    TO* dst = out + (long long)r * a.G * size + 16 * p;
+  const int size = is_k ? a.dim : a.vdim, width = a.G * size, pieces = width / E;
+  const long long id = j0 < len ? a.page_table[(long long)e * a.max_pages + j0 / a.page] : 0;
+  const int slot0 = j0 % a.page, rows = min(kReadRows, end - j0), held = len - j0;
+  const uint8_t* codes = static_cast<const uint8_t*>(is_k ? a.k_codes : a.v_codes) + (id * a.page + slot0) * width;
+  const uint8_t* powers = static_cast<const uint8_t*>(is_k ? a.k_powers : a.v_powers) + id * a.G * a.page + slot0;
+  TO* out = static_cast<TO*>(is_k ? a.k_out : a.v_out) + (a.dense_row0[e] + (long long)j0) * width;
+  for (int i0 = threadIdx.x; i0 < rows * pieces; i0 += 256 * U) {
+    uint32_t c[U][E / 4], byte[U];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float v[8];
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + 256 * u, r = i / pieces, at = (i - r * pieces) * E;
+      byte[u] = 0;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const uint32_t two = cache8::halves_of(w[2 * h + q / 2] >> (16 * (q & 1)));
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&two));
-        v[2 * q] = f.x * s;
-        v[2 * q + 1] = f.y * s;
+      for (int y = 0; y < E / 4; ++y) c[u][y] = 0u;
+      if (r < rows && r < held) {
+        const uint8_t* p = codes + r * width + at;
+        if constexpr (E == 16) {
+          const uint4 w = *reinterpret_cast<const uint4*>(p);
+          c[u][0] = w.x, c[u][1] = w.y, c[u][2] = w.z, c[u][3] = w.w;
+        } else {
+          c[u][0] = *reinterpret_cast<const uint32_t*>(p);
+        }
+        byte[u] = powers[at / size * a.page + r];
       }
-      put8(dst + 8 * h, v);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + 256 * u;
+      if (i >= rows * pieces) break;
+      const float s = cache8::value_of_power(byte[u]);
+      float v[E];
+#pragma unroll
+      for (int y = 0; y < E / 2; ++y) {
+        const uint32_t two = cache8::halves_of(c[u][y / 2] >> (16 * (y % 2)));
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&two));
+        v[2 * y] = f.x * s;
+        v[2 * y + 1] = f.y * s;
+      }
+      uint4* dst = reinterpret_cast<uint4*>(out + (long long)i * E);
+      if constexpr (E == 16) {
+#pragma unroll
+        for (int y = 0; y < 16; y += 8)
+          dst[y / 8] = make_uint4(pg::pack_bf16(v[y], v[y + 1]), pg::pack_bf16(v[y + 2], v[y + 3]), pg::pack_bf16(v[y + 4], v[y + 5]), pg::pack_bf16(v[y + 6], v[y + 7]));
+      } else {
+        dst[0] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+      }
     }
   }
 }
@@ -287,7 +312,7 @@ extern "C" int pg_attn_prepare_e4m3(const PgPrepareE4m3* args, void* stream) {
   if (a.at == nullptr) a.at = a.pos;
   const int rows = a.rows, rot_dims = a.rot, act_f32 = a.act_f32;
   const int lanes = (a.dim > a.vdim ? a.dim : a.vdim) / 8;
-  const bool vec = aligned16(a.qkv) && a.ld % (act_f32 ? 4 : 8) == 0;
+  const bool vec = aligned16(a.qkv) && a.ld % (act_f32 ? 4 : 8) == 0 && aligned16(a.q_norm) && aligned16(a.k_norm);
   const bool four = rows >= 16 * pg::num_sms();  // four tokens a CTA once that still fills the SMs
   pg_count_launch(1);
   cudaError_t rc;
@@ -312,7 +337,7 @@ extern "C" int pg_attn_prepare_e4m3(const PgPrepareE4m3* args, void* stream) {
 extern "C" int pg_kv_read_e4m3(const PgReadE4m3* args, void* stream) {
   if (args == nullptr) return PG_ERR_ARG;
   const PgReadE4m3& a = *args;
-  if (a.entries <= 0 || a.entries > 65535 || a.longest <= 0 || a.G <= 0 || a.dim <= 0 || a.vdim <= 0 || a.dim % 16 != 0 || a.vdim % 16 != 0 || a.page <= 0 || a.max_pages <= 0)
+  if (a.entries <= 0 || a.entries > 65535 || a.longest <= 0 || a.G <= 0 || a.dim <= 0 || a.vdim <= 0 || a.dim % 16 != 0 || a.vdim % 16 != 0 || a.page <= 0 || a.page % kReadRows != 0 || a.max_pages <= 0)
     return PG_ERR_ARG;
   if (!aligned16(a.k_codes) || !aligned16(a.v_codes) || !aligned16(a.k_out) || !aligned16(a.v_out)) return PG_ERR_ARG;
   const dim3 grid(((a.longest + 63) / 64 * 64 + kReadRows - 1) / kReadRows, a.entries, 2);

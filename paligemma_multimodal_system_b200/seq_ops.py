@@ -195,6 +195,12 @@ def _aligned(t, n=16):
     return t.data_ptr() % n == 0
 
 
+def _on_current_device(t):
+    """Launches go to the current device's current stream: its kernels read and write its own memory."""
+    if t.device.index != torch._C._cuda_getDevice():
+        raise ValueError(f"the tensors lie on {t.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+
+
 # ACT_SILU_GLU: grouped products only (gate / up rows alternate); ACT_GELU is the tanh form, ACT_GELU_ERF the exact one
 ACT_NONE, ACT_GELU, ACT_RELU2, ACT_SILU_GLU, ACT_GELU_ERF = 0, 1, 2, 3, 6
 
@@ -423,6 +429,7 @@ def attn_prepare(qkv, b: StepBatch, freq, q_norm, k_norm, q_out, k_pages, v_page
     mode = 2 if norm_qk is NORM_PROJECTION else int(bool(norm_qk))
     if isinstance(k_pages, QuantizedPages):
         _check_quantized(k_pages, v_pages, G, dim, vdim, page)
+        _on_current_device(qkv)
         assert q_out.is_contiguous()
         a = _lib.PREPARE_E4M3.pack(qkv.data_ptr(), qkv.stride(0), b.pos.data_ptr(), _lib.ptr(b.at), b.row_entry.data_ptr(), b.page_table.data_ptr(), freq.data_ptr(),
                                    _lib.ptr(q_norm), _lib.ptr(k_norm), q_out.data_ptr(), k_pages.codes.data_ptr(), k_pages.powers.data_ptr(), v_pages.codes.data_ptr(),
@@ -477,6 +484,7 @@ def kv_read(k_pages: "QuantizedPages", v_pages: "QuantizedPages", b: StepBatch, 
         raise ValueError("rows come back as torch.bfloat16 or torch.float32")
     G, page, dim, vdim = k_pages.heads, k_pages.page, k_pages.size, v_pages.size
     _check_quantized(k_pages, v_pages, G, dim, vdim, page)
+    _on_current_device(k_pages.codes)
     k = torch.empty(b.dense_rows, G * dim, device=k_pages.codes.device, dtype=dtype)
     v = torch.empty(b.dense_rows, G * vdim, device=k_pages.codes.device, dtype=dtype)
     if b.dense_rows:
@@ -604,6 +612,7 @@ def _attn_rows(q, k_pages, v_pages, gate, out, b: StepBatch, H, G, dim, vdim, sc
     if dim > 128 or vdim > 128:
         raise ValueError(f"attention of a few rows takes heads of up to 128 elements: got {dim} and {vdim}")
     import ctypes as C
+    _on_current_device(q)
     quantized = isinstance(k_pages, QuantizedPages)
     tree = None if singles else b.tree
     kv = ((k_pages.codes.data_ptr(), v_pages.codes.data_ptr(), k_pages.powers.data_ptr(), v_pages.powers.data_ptr()) if quantized else
@@ -652,6 +661,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, tem
         raise ValueError(f"top is 0 .. 32 and at most the vocabulary: got {top}")
     if not 0.0 < float(temperature) < float("inf"):
         raise ValueError("the temperature is positive and finite")
+    _on_current_device(logits)
     top = int(top)
     lp, entropy, top_lp, rank, ids = logits.new_empty(rows), logits.new_empty(rows), logits.new_empty((rows, top)), tokens.new_empty(rows), tokens.new_empty((rows, top))
     if rows:
