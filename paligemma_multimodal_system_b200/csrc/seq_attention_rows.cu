@@ -3,20 +3,30 @@
 //   out_i = sum_j w_ij v_j / sum_j w_ij,  w_ij = exp(s_ij),  s_ij = cap(scale q_i . k_j) - penalty,  j over the keys that row i sees:
 //   every stored key j < ctx, and drafted key m (cache row ctx + m) where bit m of the row's mask is set (no mask: m <= i); windows go by positions.
 //
-// A warp owns 16 MT rows (token x query head of one k/v head) and walks key tiles of its own straight from the pages: no shared memory, no barrier in
-// the loop.  Both products run on mma.sync m16n8k16 with fp32 accumulation, and the operands' k indexes are permuted so that a lane's 16-byte pieces of
-// the cache ARE its fragments:
+// A warp owns 16 MT rows (token x query head of one k/v head) and walks key tiles through a ring in shared memory that asynchronous copies fill two tiles ahead (one where a tile
+// is 16 KB).  Both products run on mma.sync m16n8k16 with fp32 accumulation, and the operands' k indexes are permuted so that a lane's 16-byte pieces of the cache ARE its
+// fragments:
 //   * keys: lane (n, c) reads piece c of key n's row; the elements of a piece are k indexes of ITS lane in consecutive 16-deep steps, and the
 //     queries are stored in that order once.  Key n of fragment f is key (KT / 4)(n / 2) + 2 f + n % 2 of the tile, so lane c's scores belong to KT / 4
 //     neighbouring keys, and those are the keys whose value rows it reads for the second product, columns 8 n .. 8 n + 7 of every 64.
 //   * no transposition, no conversion but codes -> halves (exact) and, for fp32, the cut into three bf16 terms.
+//   * at most eight rows a k/v head (decoded tokens): the second product is transposed, O^T = V^T P^T, sixteen columns x eight rows an instruction; the weights are its second
+//     operand as they stand, and no half of the instruction is empty.
+// Few rows: the CTA's four warps walk tiles of their own and join in shared memory.  More: warps that hold rows of one head share a ring (a barrier a tile), since four private
+// copies of every tile cost shared memory and L2 (24 trees of 31 x 4 rows over 1500 keys, bf16 pages: 154 -> 90 us).  CTAs split the keys further; up to eight join in a
+// cluster, more through scratch and a second launch.
+//
 // Precision: bf16 operands as they are; codes as halves, exact, against queries scaled by a power of two per row into half range (fp32 queries: two
 // halves, 22 bits); fp32 as three bf16 terms, six products.  Weights: two bf16 terms over bf16 values (16 bits); one half over codes for bf16
 // rows (11 bits: an eighth of the output's own rounding), two for fp32 rows; three bf16 terms over fp32 values.  The values' powers of two
 // go into the weights relative to the largest one so far.  Scores, maxima, sums and outputs are fp32.
 //
-// What bounds it: the bytes of keys and values while a k/v head has few rows; the tensor instructions for large trees.  Warps of a CTA share a key walk
-// (few rows) or the rows (trees); CTAs split the keys further, and a merge launch joins their (maximum, sum, accumulator).
+// What bounds it: while a k/v head has few rows, the bytes of keys and values where walks are long (6 x 32000 keys of 4 x 128 over codes 41 us, 4.7 TB/s), the unequal lengths of a
+// batch (64 x 1125 .. 2250 of 8 x 64 with soft cap and gate 38 us: the loop runs at the memory's rate, then short entries leave SMs empty), else a chain of trips
+// (descriptors, pages, tiles, join: one x 3000 10 us).  Large trees: instructions -- conversions, exponentials and a tensor rate of 550 TFLOP/s (one m16n8k16 in 2.1 clocks an SM) --
+// at ten warps an SM (24 trees of 31 x 4 rows over codes 78 us).
+// The loop body is one straight line but for masks, options and new maxima: branches between the row halves cost a quarter (98 -> 84 us); a second body for masked tiles cost
+// as much in instruction fetch as it saved.
 #include <cuda_fp16.h>
 
 #include "cache8.cuh"
@@ -958,10 +968,13 @@ Plan plan_of(const PgAttnRows& p, int rows, int row_tile, int keys, int per_sm) 
     reach = reach < w ? reach : w;
   }
   const long long tiles = (reach + keys - 1) / keys, ctas = (long long)p.busy * p.G * x.blocks;
-  // CTAs that share a walk: what the SMs hold at once, and at least two tiles for a warp
-  long long n = (long long)per_sm * pg::num_sms() / (ctas > 0 ? ctas : 1);
-  const long long most = tiles * x.wr / (2 * kWarps);
+  // CTAs that share a walk: what the SMs hold at once, with two tiles for a warp at least, and four where there are two CTAs an SM already (24 x 1500 keys of 8 heads in three / two
+  // parts 20.6 / 16.8 us; one x 3000 in eight parts of three tiles 10.3, in four 12.3)
+  const long long sms = pg::num_sms(), most = tiles * x.wr / (2 * kWarps);
+  long long n = per_sm * sms / (ctas > 0 ? ctas : 1);
+  const long long filled = 2 * sms / (ctas > 0 ? ctas : 1), calm = most / 2 > filled ? most / 2 : filled;
   n = n < most ? n : most;
+  n = n < calm ? n : calm;
   n = n > 64 ? 64 : n < 1 ? 1 : n;
   // up to eight join through distributed shared memory in one launch; more, where that leaves warps with a long walk, through global memory and a second one
   x.cluster = n <= 8 || most <= 12;
@@ -1038,8 +1051,9 @@ template <typename TQ, typename TC, int KT>
 int by_rows(const PgAttnRows& p, const Args& a, long long* need, long long scratch_bytes, cudaStream_t st) {
   const int rows = (p.singles ? 1 : p.max_n) * (p.H / p.G);
   if (rows <= 8) return by_size<TQ, TC, 1, KT, true>(p, a, need, scratch_bytes, st);
-  // 32 rows a warp read a tile once where there are CTAs enough; else 16, for a shorter chain (one tree of 8 x 4 rows over 1100 keys: 20 / 16 us)
-  if (rows <= 16 || sizeof(TQ) == 4 || (long long)p.busy * p.G * 2 < pg::num_sms()) return by_size<TQ, TC, 1, KT, false>(p, a, need, scratch_bytes, st);
+  // 32 rows a warp read and convert a tile once where there are CTAs enough (24 trees of 8 x 4 rows over codes, 16 / 32 rows a warp 39 / 30 us; 16 x 4 rows 62 / 47); else, and where
+  // nothing is converted, 16 for a shorter chain (one tree of 8 x 4 rows 14 / 20; 24 over bf16 pages 41 / 48)
+  if (rows <= 16 || sizeof(TQ) == 4 || (sizeof(TC) == 2 && rows <= 32) || (long long)p.busy * p.G * 2 < pg::num_sms()) return by_size<TQ, TC, 1, KT, false>(p, a, need, scratch_bytes, st);
   return by_size<TQ, TC, sizeof(TQ) == 4 ? 1 : 2, KT, false>(p, a, need, scratch_bytes, st);
 }
 

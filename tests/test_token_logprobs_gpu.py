@@ -135,3 +135,17 @@ def test_no_rows():
     from paligemma_multimodal_system_b200 import seq_ops
     out = seq_ops.token_logprobs(torch.empty(0, 10, device="cuda"), torch.empty(0, dtype=torch.int32, device="cuda"), top=2)
     assert [tuple(o.shape) for o in out] == [(0,), (0,), (0,), (0, 2), (0, 2)]
+
+
+@pytest.mark.parametrize("first,pitch,V", [(0, 3001, 3001), (3, 9007, 9001), (1, 2050, 2049)])
+def test_more_rows_than_blocks(first, pitch, V):
+    """Blocks that take several rows in turn, on all alignments; some rows need the careful way (masked, equal, rising) between others that do not."""
+    rows = 1000
+    x = _logits(rows, pitch, pitch)[:, first:first + V]
+    x[5::50, 20:] = -math.inf
+    x[6::50] = 1.0
+    x[7::50] = torch.arange(V, device="cuda").float()
+    x[8::50, 1::2] = x[8::50, 0::2][:, :x[8::50, 1::2].shape[1]]
+    _check(x, [(i * 37) % V for i in range(rows)], 25)
+    _check(x, [(i * 31) % V for i in range(rows)], 0)
+    _check(x, [0] * rows, 1)
