@@ -10,7 +10,7 @@ using bf16 = __nv_bfloat16;
 
 namespace {
 
-__device__ __forceinline__ float wsum(float v) {
+__device__ __forceinline__ double wsum(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
@@ -51,15 +51,15 @@ __device__ __forceinline__ void put8(bf16* p, const float (&v)[8]) {
   *reinterpret_cast<uint4*>(p) = make_uint4(pg::pack_bf16(v[0], v[1]), pg::pack_bf16(v[2], v[3]), pg::pack_bf16(v[4], v[5]), pg::pack_bf16(v[6], v[7]));
 }
 
-// sine and cosine of an angle in double, to fp32: whole turns go in double, the rest as a sum of two floats (a library sincos in double took a third of the kernel's time)
-__device__ __forceinline__ void sine_of(double angle, float& s, float& c) {
-  const double turns = rint(angle * 0.15915494309189535);
-  const double rest = fma(-turns, 2.4492935982947064e-16, fma(-turns, 6.283185307179586, angle));
-  const float hi = (float)rest, lo = (float)(rest - (double)hi);
-  float s0, c0;
-  sincosf(hi, &s0, &c0);
-  s = fmaf(c0, lo, s0);
-  c = fmaf(-s0, lo, c0);
+constexpr float kDoubt = 0x1p-20f;  // no further are fp32 elements from the exact ones, relative to their size (12 half steps of 2^-24 without a turn, which cancels more in a few)
+__device__ __forceinline__ uint2 codes8(const float (&x)[8], float up) {
+  return make_uint2(cache8::codes_of(x[0] * up, x[1] * up) | cache8::codes_of(x[2] * up, x[3] * up) << 16,
+                    cache8::codes_of(x[4] * up, x[5] * up) | cache8::codes_of(x[6] * up, x[7] * up) << 16);
+}
+// to fp32 towards zero, the last bit set where something was cut off: what is rounded to fewer bits from here is rounded once
+__device__ __forceinline__ float to_odd(double y) {
+  const float f = __double2float_rz(y);
+  return static_cast<double>(f) != y ? __uint_as_float(__float_as_uint(f) | 1u) : f;  // (NaN stays NaN)
 }
 
 using Prepare = PgPrepareE4m3;
@@ -68,12 +68,19 @@ static_assert(sizeof(PgPrepareE4m3) == 192 && sizeof(PgReadE4m3) == 112, "caller
 // A group of LG lanes holds a head vector, eight elements a lane; its mean square and its largest element are butterflies inside the group.  A CTA takes TOK tokens, whose cosines
 // and sines (angles in double) are made once for all heads behind the first vectors' requests; four vectors of a group are under way together: one head of four tokens,
 // which share its weights, or four heads of one token.
+// Elements that a norm or a rotation computes are fp32; where that could choose the code beside the nearest (one in a million would be), the head's vector is marked and made again
+// in double behind the loop, so that the codes are those of the exact elements.  Inside the loop the same work costs twice as much (its registers are live beside four vectors'):
+// 36.9 us against 34.4 for the first size below, 30.8 without it.
 // What bounds it: for prompts instructions, then the bytes (a row is read once, 8-bit rows are half of bf16 ones); for a few rows the chain row -> sum -> largest -> codes.
+// 7,796 bf16 rows of 32 + 8 + 8 heads of 64, normed and turned, in 34.4 us (2.6 of 6.6 TB/s; 28.8 into pages of bf16); 1,363 fp32 rows of 16 + 4 + 4 heads of 128 as they come in 12.4;
+// 23 rows in 6.2.
 template <typename TA, int LG, int TOK, bool VEC>
 __global__ void __launch_bounds__(128, sizeof(TA) == 2 ? 7 : 5) attn_prepare_e4m3_kernel(const __grid_constant__ Prepare a) {
   constexpr int U = 4, NG = 128 / LG, HEADS = TOK == 1 ? U : 1;  // HEADS: head vectors of a round
-  extern __shared__ __align__(16) float cs[];  // [TOK][cos rot / 2 | sin rot / 2]
-  __shared__ float part[2][TOK][4];
+  extern __shared__ __align__(16) double cs64[];  // [TOK][cos rot / 2 | sin rot / 2], behind them the same in fp32 and a bit per key or value head and token
+  float* cs = reinterpret_cast<float*>(cs64 + (TOK * a.rot + 1) / 2 * 2);
+  uint32_t* doubtful = reinterpret_cast<uint32_t*>(cs + TOK * a.rot);
+  __shared__ double part[2][TOK][4];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, l = tid % LG, group = tid / LG, d0 = 8 * l;
   const int t0 = blockIdx.x * TOK, nvec = a.H + 2 * a.G, half = a.rot / 2;
   const TA* qkv = static_cast<const TA*>(a.qkv);
@@ -101,21 +108,22 @@ __global__ void __launch_bounds__(128, sizeof(TA) == 2 ? 7 : 5) attn_prepare_e4m
     }
   };
   request(group);
+  for (int i = tid; i < (2 * a.G * TOK + 31) / 32; i += 128) doubtful[i] = 0u;
   for (int i = tid; i < TOK * half; i += 128) {
     const int k = i / half, j = i - k * half;
-    float s, c;
-    sine_of((double)a.pos[min(t0 + k, a.rows - 1)] * a.freq[j], s, c);
-    cs[k * a.rot + j] = a.rot_gain * c;
-    cs[k * a.rot + half + j] = a.rot_gain * s;
+    double s, c;
+    sincos((double)a.pos[min(t0 + k, a.rows - 1)] * a.freq[j], &s, &c);
+    cs[k * a.rot + j] = static_cast<float>(cs64[k * a.rot + j] = a.rot_gain * c);
+    cs[k * a.rot + half + j] = static_cast<float>(cs64[k * a.rot + half + j] = a.rot_gain * s);
   }
   if (a.norm_qk == 2) {  // one root mean square for all of q, one for all of k
     const int nq = a.H * a.dim, nk = a.G * a.dim;
 #pragma unroll 1
     for (int k = 0; k < TOK; ++k) {
       const TA* row = qkv + (long long)min(t0 + k, a.rows - 1) * a.ld;
-      float sq = 0.f, sk = 0.f;
-      for (int d = tid; d < nq; d += 128) { const float x = ldf(row + d); sq = fmaf(x, x, sq); }
-      for (int d = tid; d < nk; d += 128) { const float x = ldf(row + nq + d); sk = fmaf(x, x, sk); }
+      double sq = 0.0, sk = 0.0;
+      for (int d = tid; d < nq; d += 128) { const double x = ldf(row + d); sq = fma(x, x, sq); }
+      for (int d = tid; d < nk; d += 128) { const double x = ldf(row + nq + d); sk = fma(x, x, sk); }
       sq = wsum(sq);
       sk = wsum(sk);
       if (lane == 0) { part[0][k][warp] = sq; part[1][k][warp] = sk; }
@@ -163,8 +171,8 @@ __global__ void __launch_bounds__(128, sizeof(TA) == 2 ? 7 : 5) attn_prepare_e4m
           if (is_v ? a.norm_v != 0 : a.norm_qk == 1) inv = rsqrtf(s * mean + a.eps);
         }
         if (a.norm_qk == 2 && !is_v) {
-          const float* p = part[is_q ? 0 : 1][k];
-          inv = rsqrtf((p[0] + p[1] + p[2] + p[3]) / (float)((is_q ? a.H : a.G) * a.dim) + a.eps);
+          const double* p = part[is_q ? 0 : 1][k];
+          inv = rsqrtf(static_cast<float>(p[0] + p[1] + p[2] + p[3]) / (float)((is_q ? a.H : a.G) * a.dim) + a.eps);
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] *= inv;
@@ -226,19 +234,85 @@ __global__ void __launch_bounds__(128, sizeof(TA) == 2 ? 7 : 5) attn_prepare_e4m
         } else {
           const uint32_t byte = cache8::power_of(__float_as_uint(top));
           const float up = cache8::inverse_of_power(byte);
-          uint2 codes;
-          codes.x = cache8::codes_of(x[0] * up, x[1] * up) | cache8::codes_of(x[2] * up, x[3] * up) << 16;
-          codes.y = cache8::codes_of(x[4] * up, x[5] * up) | cache8::codes_of(x[6] * up, x[7] * up) << 16;
-          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(is_k ? a.k_codes : a.v_codes) + kv_row[k] * (a.G * n) + (head * n + d0)) = codes;
+          if (is_k ? a.norm_qk != 0 || d0 < a.rot : a.norm_v != 0 || a.v_other != nullptr) {  // (else it is what came)
+            const uint2 more = codes8(x, up * (1.f + kDoubt)), less = codes8(x, up * (1.f - kDoubt));
+            if (more.x != less.x || more.y != less.y ||
+                cache8::power_of(__float_as_uint(top * (1.f + kDoubt))) != cache8::power_of(__float_as_uint(top * (1.f - kDoubt))))
+              atomicOr(&doubtful[((vec - a.H) * TOK + k) / 32], 1u << ((vec - a.H) * TOK + k) % 32);
+          }
+          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(is_k ? a.k_codes : a.v_codes) + kv_row[k] * (a.G * n) + (head * n + d0)) = codes8(x, up);
           if (l == 0) static_cast<uint8_t*>(is_k ? a.k_powers : a.v_powers)[power_row[k] + head * a.page] = static_cast<uint8_t>(byte);
         }
       }
+    }
+  }
+  // Codes that a little more or less would change, by elements in double.  The groups of a warp make the same vector, the first one writes it.
+  __syncthreads();
+  for (int word = warp; word < (2 * a.G * TOK + 31) / 32; word += 4) {
+    for (uint32_t left = doubtful[word]; left != 0; left &= left - 1) {
+      const int bit = 32 * word + __ffs(left) - 1, k = bit % TOK, vec = bit / TOK;
+      const bool is_v = vec >= a.G;
+      const int n = is_v ? a.vdim : a.dim, head = is_v ? vec - a.G : vec;
+      const bool mine = d0 < n;
+      Eight<TA> again;
+      float x[8];
+      double y[8], scale = 1.0;
+      again.zero();
+      if (mine) again.template load<VEC>(rows[k] + (is_v && !a.v_from_k ? (a.H + a.G) * a.dim + head * a.vdim : (a.H + head) * a.dim));
+      again.get(x);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = x[i];
+      if (is_v ? a.norm_v != 0 : a.norm_qk == 1) {
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum = fma(y[i], y[i], sum);
+#pragma unroll
+        for (int o = LG / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        scale = 1.0 / sqrt(sum / n + static_cast<double>(a.eps));
+      } else if (!is_v && a.norm_qk == 2) {
+        const double* p = part[1][k];
+        scale = 1.0 / sqrt((p[0] + p[1] + p[2] + p[3]) / (a.G * a.dim) + static_cast<double>(a.eps));
+      }
+      float top = 0.f;
+      if (mine) {
+        const float* wp = is_v || a.k_norm == nullptr ? nullptr : a.k_norm + (a.norm_qk == 2 ? head * a.dim + d0 : d0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] *= wp != nullptr ? scale * wp[i] : scale;
+        if (!is_v && d0 < a.rot) {
+          const double* ck = cs64 + k * a.rot + d0 / 2;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (d0 + 2 * i >= a.rot) break;
+            const double p = y[2 * i], r = y[2 * i + 1];
+            y[2 * i] = p * ck[i] - r * ck[half + i];
+            y[2 * i + 1] = r * ck[i] + p * ck[half + i];
+          }
+        }
+        if (is_v && a.v_other != nullptr) {
+          const TA* o = static_cast<const TA*>(a.v_other) + static_cast<long long>(t0 + k) * a.ld_v_other + (long long)head * a.vdim + d0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = (1.0 - static_cast<double>(a.v_mix)) * y[i] + static_cast<double>(a.v_mix) * static_cast<double>(ldf(o + i));
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[i] = to_odd(y[i]);
+          if (fabsf(x[i]) < INFINITY) top = fmaxf(top, fabsf(x[i]));
+          else x[i] = __uint_as_float(0x7fffffffu);
+        }
+      }
+#pragma unroll
+      for (int o = LG / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (!mine || lane >= LG) continue;
+      const uint32_t byte = cache8::power_of(__float_as_uint(top));
+      *reinterpret_cast<uint2*>(static_cast<uint8_t*>(is_v ? a.v_codes : a.k_codes) + kv_row[k] * (a.G * n) + (head * n + d0)) = codes8(x, cache8::inverse_of_power(byte));
+      if (l == 0) static_cast<uint8_t*>(is_v ? a.v_powers : a.k_powers)[power_row[k] + head * a.page] = static_cast<uint8_t>(byte);
     }
   }
 }
 
 // 16 codes (bf16: two 16-byte pieces of output) or four (fp32: one) a thread and step, fp32 four steps under way together; a CTA's 16 rows lie in one page.  Rows behind an entry's last one up to the end of its last run of 64
 // are zeros: whoever walks whole tiles of the scratch reads numbers.  What bounds it: the bytes, half again as many as it writes in bf16.
+// 7,796 rows of 2 x 8 heads of 64 to bf16 in 8.3 us (2.9 of 6.6 TB/s).
 constexpr int kReadRows = 16;
 template <typename TO>
 __global__ void __launch_bounds__(256) kv_read_e4m3_kernel(const __grid_constant__ PgReadE4m3 a) {
@@ -311,16 +385,17 @@ extern "C" int pg_attn_prepare_e4m3(const PgPrepareE4m3* args, void* stream) {
     return PG_ERR_ARG;
   if (a.at == nullptr) a.at = a.pos;
   const int rows = a.rows, rot_dims = a.rot, act_f32 = a.act_f32;
+  const auto smem = [&](int tokens) { return static_cast<size_t>(tokens * rot_dims + 4) * 12 + static_cast<size_t>(2ll * a.G * tokens + 31) / 32 * 4; };
   const int lanes = (a.dim > a.vdim ? a.dim : a.vdim) / 8;
   const bool vec = aligned16(a.qkv) && a.ld % (act_f32 ? 4 : 8) == 0 && aligned16(a.q_norm) && aligned16(a.k_norm);
   const bool four = rows >= 16 * pg::num_sms();  // four tokens a CTA once that still fills the SMs
   pg_count_launch(1);
   cudaError_t rc;
 #define PG_P8(TA, LG)                                                                                                                                       \
-  rc = four ? (vec ? pg::launch_dependent(attn_prepare_e4m3_kernel<TA, LG, 4, true>, dim3((rows + 3) / 4), dim3(128), (size_t)(4 * rot_dims + 4) * 4, st, a)   \
-                   : pg::launch_dependent(attn_prepare_e4m3_kernel<TA, LG, 4, false>, dim3((rows + 3) / 4), dim3(128), (size_t)(4 * rot_dims + 4) * 4, st, a)) \
-            : (vec ? pg::launch_dependent(attn_prepare_e4m3_kernel<TA, LG, 1, true>, dim3(rows), dim3(128), (size_t)(rot_dims + 4) * 4, st, a)                 \
-                   : pg::launch_dependent(attn_prepare_e4m3_kernel<TA, LG, 1, false>, dim3(rows), dim3(128), (size_t)(rot_dims + 4) * 4, st, a))
+  rc = four ? (vec ? pg::launch_dependent(attn_prepare_e4m3_kernel<TA, LG, 4, true>, dim3((rows + 3) / 4), dim3(128), smem(4), st, a)   \
+                   : pg::launch_dependent(attn_prepare_e4m3_kernel<TA, LG, 4, false>, dim3((rows + 3) / 4), dim3(128), smem(4), st, a)) \
+            : (vec ? pg::launch_dependent(attn_prepare_e4m3_kernel<TA, LG, 1, true>, dim3(rows), dim3(128), smem(1), st, a)                 \
+                   : pg::launch_dependent(attn_prepare_e4m3_kernel<TA, LG, 1, false>, dim3(rows), dim3(128), smem(1), st, a))
 #define PG_P8T(TA)               \
   if (lanes <= 4) PG_P8(TA, 4);       \
   else if (lanes <= 8) PG_P8(TA, 8);  \

@@ -228,3 +228,33 @@ def test_many_rows_take_four_tokens_a_block():
         r += n
     for x, y in zip(all_at_once, [torch.cat(parts), kq.codes, kq.powers, vq.codes, vq.powers]):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,G,dim,mode", [(1, 1, 16, True), (37, 3, 96, "projection"), (3001, 2, 256, True), (6000, 8, 128, True), (6001, 3, 64, "projection")])
+def test_codes_of_computed_elements_are_the_nearest(dtype, rows, G, dim, mode):
+    """Without a rotation an fp32 element is within 2^-20 of the exact one: a sum of squares of 8 products a lane and 5 exchanges (13 half steps of 2^-24, halved by the root), the
+    mean, the root to 2 steps, two products.  What that could move to another code is made in double (off by 2^-48 or so), so that bytes are determined here too."""
+    from paligemma_multimodal_system_b200 import seq_ops
+    H, eps = 1, 2.0 ** -20
+    b, entries, pool = batch_of([(rows, 5)], rows)
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    proj = torch.randn(b.T, (H + 2 * G) * dim, generator=g, device="cuda").to(dtype)
+    n = dim if mode is True else G * dim
+    wk = 1 + 0.2 * torch.randn(n, generator=g, device="cuda")
+    wq = torch.ones(dim if mode is True else H * dim, device="cuda")
+    kq, vq, q = fresh(pool, G, dim), fresh(pool, G, dim), torch.empty(b.T, H * dim, device="cuda", dtype=dtype)
+    seq_ops.attn_prepare(proj, b, torch.zeros(1, device="cuda", dtype=torch.float64), wq, wk, q, kq, vq, H, G, dim, dim, 0, eps, PAGE,
+                         norm_qk=True if mode is True else seq_ops.NORM_PROJECTION, norm_v=True)
+    x = proj.double().cpu().numpy()
+    for pages, lo, w in ((kq, H * dim, wk.double().cpu().numpy()), (vq, (H + G) * dim, None)):
+        y = x[:, lo:lo + G * dim].reshape(rows, G, dim)
+        whole = w is not None and mode is not True
+        y = y / np.sqrt((y ** 2).mean((-2, -1) if whole else -1, keepdims=True) + eps)
+        y = y if w is None else y * (w.reshape(1, G, dim) if whole else w)
+        codes, powers = stored(pages, entries[0], 5 + rows, G)
+        want = powers_of(y)
+        assert np.array_equal(powers[5:], want)
+        code, sign = codes_of(y, want)
+        assert np.array_equal(codes[5:] & 0x7f, code)
+        assert np.array_equal(codes[5:] >> 7 == 1, sign)
