@@ -7,13 +7,15 @@
 // The largest `top` entries without sorting: the order is by value, then by the lower index, as one 64-bit key.  A thread leaves the largest entry of every
 // tile (or of a run of tiles) in shared memory.  Behind the pass, 64 groups of threads know their largest entries; the top-th of those 64 is reached by
 // `top` entries at least, so only entries that reach it can be among the first `top`.  The few tiles whose largest entry does are read once more, and
-// their entries that reach it go to a list (some dozens), whose order is counted.  Where that fails -- more entries than the list holds: many equal
-// ones; fewer than `top`: masked rows -- the part is read again by keys, tile by tile, and the list cut to its first `top` as often as it fills.
+// their entries that reach it go to a list (some dozens), whose order is counted.  Masked rows (fewer than `top` entries left, or the least of them shared
+// by more than the list holds) take the equal ones from the front.  Where that fails -- large entries that lie in few threads' tiles -- the part is read
+// again by keys, tile by tile, and the list cut to its first `top` as often as it fills.
 //
 // What bounds it: the bytes of the row (one read) where rows are many; for few rows the trip to memory and the joins, so up to eight CTAs of a
 // cluster share a row and the first of them joins what they found through distributed shared memory: one launch, no scratch, no atomics on
 // global memory (the list's order does not change results: keys are distinct and counted).  Many rows: CTAs that stay walk them, the next row's first tile under way while one is
 // joined.  64 x 257216 with 20 alternatives 26 us (2.5 TB/s; without alternatives 21), 1500 x 32000 with one 51 (3.7 TB/s; 43), one x 257216 with five 14.
+// Rows of masked entries or of one number take 28 to 36 us for the first of these (read again by keys 340 to 610).
 // Lists kept while the row goes by (a floor in shared memory, raised tile by tile) cost the loop its registers and took 33 to 97 us for the first of these.
 #include "common.cuh"
 #include "paligemma_b200.h"
@@ -129,6 +131,70 @@ struct Part {
     }
   }
 };
+
+// The entries that reach `least`, from the runs of tiles whose largest one does, into the list.
+__device__ __forceinline__ void list_hits(Shared& sh, const Part& p, int V, float least, int slots, int run) {
+  const int tid = threadIdx.x;
+  for (int k = 0; k < slots; ++k)
+    if (sh.slot[k][tid] >= least) {
+      const int at = atomicAdd(&sh.hits, 1);
+      if (at < kHits) sh.hit[at] = k << 16 | tid;
+    }
+  __syncthreads();
+  // four lanes a run, all of them under way together
+  const int hits = min(sh.hits, kHits);
+  for (int i = tid / 4; i < hits; i += kThreads / 4) {
+    const int k = sh.hit[i] >> 16, who = sh.hit[i] & 0xffff;
+    for (int v = p.v0 + k * run + (tid % 4) * kThreads + who; v < min(p.v0 + (k + 1) * run, p.v1); v += 4 * kThreads) {
+      const int e = 4 * v - p.lead;
+      float z[4];
+#pragma unroll
+      for (int y = 0; y < 4; ++y) z[y] = e + y >= 0 && e + y < V ? p.x[e + y] : -INFINITY;
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+        if (z[y] >= least) list_key(sh, key_of(z[y], e + y));
+    }
+  }
+  __syncthreads();
+}
+
+// the number behind x: what is larger than x reaches it.  Behind +inf and NaN: NaN, which nothing reaches.
+__device__ __forceinline__ float number_above(float x) {
+  const uint32_t b = __float_as_uint(x + 0.0f);
+  return __uint_as_float(x + 0.0f < 0.f ? b - 1u : b + 1u);
+}
+
+// Masked rows: fewer than `top` entries are left (the others -inf), or more share the least value that counts (a mask of the lowest value) than the list holds.  What is larger is
+// listed; of the equal ones only those in front matter, and they are met after few entries.
+__device__ __noinline__ void list_ties(Shared& sh, const Part p, int V, int top, float least, int slots, int run) {
+  const int tid = threadIdx.x;
+  float tie = -INFINITY;
+  if (sh.hits > kHits || sh.over) {
+    tie = least;
+    __syncthreads();
+    if (tid == 0) { sh.count = 0; sh.over = 0; sh.hits = 0; }
+    __syncthreads();
+    list_hits(sh, p, V, number_above(least), slots, run);
+    if (sh.hits > kHits || sh.over) return;  // (the careful way)
+  }
+  const int larger = sh.count;
+  for (int v0 = p.v0; v0 < p.v1; v0 += kThreads) {
+    const int v = v0 + tid, e = 4 * v - p.lead;
+    __syncthreads();  // the count is read
+    bool is[4];
+    int front = 0;  // equal ones in front of this lane's in its warp, whose first `top` are enough
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      is[y] = v < p.v1 && e + y >= 0 && e + y < V && p.x[e + y] == tie;
+      front += __popc(__ballot_sync(0xffffffffu, is[y]) & ((1u << (tid & 31)) - 1u));
+    }
+#pragma unroll
+    for (int y = 0; y < 4; ++y)
+      if (is[y] && front++ < top) list_key(sh, key_of(tie, e + y));
+    __syncthreads();
+    if (sh.count - larger >= top || sh.over) break;
+  }
+}
 
 // The careful way: tiles by keys, with barriers.
 __device__ __noinline__ void list_by_keys(Shared& sh, const Part p, int V, int top) {
@@ -249,9 +315,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) token_logprobs_kernel(const 
     const bool more = row + stride < rows, known = t >= 0 && t < V;
     if (more) t_next = tokens[row + stride];
     const float xt = known ? p.x[t] : INFINITY;
-    // x > x_t as x >= the next number (of +inf and NaN: NaN, which nothing reaches)
-    const uint32_t bt = __float_as_uint(xt + 0.0f);
-    const float above = __uint_as_float(xt + 0.0f < 0.f ? bt - 1u : bt + 1u);
+    const float above = number_above(xt);
     const int run = ((p.v1 - p.v0 + step - 1) / step + kSlots - 1) / kSlots * step;  // vectors of a slot
     Stats st{-INFINITY, 0.f, 0.f};
     uint64_t sums = 0, weighted = 0, front = 0;  // pairs: sum of e^d, sum of d e^d, entries in front of t
@@ -332,28 +396,9 @@ __global__ void __launch_bounds__(kThreads, kPerSm) token_logprobs_kernel(const 
       }
       __syncthreads();
       const float least = fmaxf(unordered(sh.least), -3.402823466e38f);  // (masked entries are not listed)
-      for (int k = 0; k < slot; ++k)
-        if (sh.slot[k][tid] >= least) {
-          const int at = atomicAdd(&sh.hits, 1);
-          if (at < kHits) sh.hit[at] = k << 16 | tid;
-        }
-      __syncthreads();
-      // four lanes a run, all of them under way together
-      const int hits = sh.hits;
-      for (int i = tid / 4; i < min(hits, kHits); i += kThreads / 4) {
-        const int k = sh.hit[i] >> 16, who = sh.hit[i] & 0xffff;
-        for (int v = p.v0 + k * run + (tid % 4) * kThreads + who; v < min(p.v0 + (k + 1) * run, p.v1); v += 4 * kThreads) {
-          const int e = 4 * v - p.lead;
-          float z[4];
-#pragma unroll
-          for (int y = 0; y < 4; ++y) z[y] = e + y >= 0 && e + y < V ? p.x[e + y] : -INFINITY;
-#pragma unroll
-          for (int y = 0; y < 4; ++y)
-            if (z[y] >= least) list_key(sh, key_of(z[y], e + y));
-        }
-      }
-      __syncthreads();
-      if (tid == 0) sh.fails = hits > kHits || sh.over || (sh.count < top && p.v0 < p.v1);  // (fewer entries than `top`: the careful way lists them all)
+      list_hits(sh, p, V, least, slot, run);
+      if (sh.hits > kHits || sh.over || sh.count < top) list_ties(sh, p, V, top, least, slot, run);
+      if (tid == 0) sh.fails = sh.hits > kHits || sh.over || (sh.count < top && p.v0 < p.v1);  // (fewer entries than `top`: the careful way lists them all)
     }
     if (warp == kWarps - 1) {
       const Stats a = join_warp(lane < kWarps ? sh.warp[lane % kWarps] : Stats{-INFINITY, 0.f, 0.f}, c);
@@ -463,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) token_logprobs_kernel(const 
 
 extern "C" int pg_token_logprobs(const float* logits, long long ld, const int* tokens, float* logprob, float* entropy, int* rank, int* top_ids, float* top_logprob,
                                  int rows, int V, int top, float temperature, void* stream) {
-  if (rows <= 0 || V <= 0 || top < 0 || top > kTop || top > V || ld < V || !(temperature > 0.f) || !(temperature < INFINITY)) return PG_ERR_ARG;
+  if (rows <= 0 || V <= 0 || top < 0 || top > kTop || top > V || ld < V || !(temperature > 0.f) || !(temperature < INFINITY) || !(1.0f / temperature < INFINITY)) return PG_ERR_ARG;
   if (logits == nullptr || tokens == nullptr || logprob == nullptr || entropy == nullptr || rank == nullptr || (top > 0 && (top_ids == nullptr || top_logprob == nullptr))) return PG_ERR_ARG;
   if (V > 0x7fffff00 / 2 || (reinterpret_cast<uintptr_t>(logits) & 3) != 0) return PG_ERR_ARG;
   // CTAs that share a row: as many as fit the GPU at two an SM, no share below a tile's half

@@ -20,7 +20,7 @@ def _want(x, t, top, temperature):
     z = x.double().cpu() / temperature
     logs = torch.log_softmax(z, -1)
     p = logs.exp()
-    entropy = -torch.where(p > 0, p * logs, torch.zeros_like(p)).sum(-1)
+    entropy = -torch.where(p == 0, torch.zeros_like(p), p * logs).sum(-1)
     ids = torch.sort(x.cpu(), dim=-1, descending=True, stable=True).indices
     t = torch.as_tensor(t).long()
     lp = logs.gather(1, t[:, None])[:, 0]
@@ -149,3 +149,27 @@ def test_more_rows_than_blocks(first, pitch, V):
     _check(x, [(i * 37) % V for i in range(rows)], 25)
     _check(x, [(i * 31) % V for i in range(rows)], 0)
     _check(x, [0] * rows, 1)
+
+
+@pytest.mark.parametrize("mask", [-math.inf, -1e9, torch.finfo(torch.float32).min])
+@pytest.mark.parametrize("rows,V", [(1, 257216), (40, 70001), (500, 5003)])
+def test_masks_that_leave_fewer_than_asked_for(mask, rows, V):
+    """The rest of the alternatives are masked entries, the lowest ids first, wherever those that are left lie: in front, behind, in one thread's tiles, among the first masked ones."""
+    x = torch.full((rows, V), mask, device="cuda")
+    some = torch.randn(rows, 12, generator=torch.Generator(device="cuda").manual_seed(V), device="cuda")
+    for r in range(rows):
+        at = [torch.arange(12), V - 12 + torch.arange(12), 1024 * torch.arange(4), 3 * torch.arange(12) + 1, torch.arange(1) + V // 2][r % 5]
+        x[r, at.cuda()] = some[r, :len(at)]
+    for top in (1, 4, 13, 32):
+        _check(x, [(i * 37) % V for i in range(rows)], top)
+    x[:, :V - 40] = 3.0 * mask if mask == -1e9 else -math.inf  # the equal ones that count lie behind
+    _check(x, [V - 1] * rows, 32)
+
+
+@pytest.mark.parametrize("rows,V", [(1, 257216), (70, 65536), (500, 32000)])
+def test_large_entries_in_few_threads_tiles(rows, V):
+    """More than the list holds, all of them above the rest: the row is read again by keys."""
+    x = _logits(rows, V, 5 * V)
+    x[:, torch.arange(V, device="cuda") // 4 % 256 < 12] += 100.0
+    _check(x, [(i * 37) % V for i in range(rows)], 32)
+    _check(x, [0] * rows, 5)
