@@ -822,7 +822,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
     __syncthreads();
     for (int r = tid; r < rows_here; r += 32 * kWarps) {
       float2& st = stat[r / (16 * MT)][r % (16 * MT)];
-      if (st.x == 0.f) st.x = 1e-30f;  // (a factor of zero would leave them out)
+      if (st.x == 0.f) st.x = __uint_as_float(1u);  // (a factor of zero would leave them out)
     }
     __syncthreads();
   }

@@ -128,6 +128,7 @@ class SequenceEngine:
         for rid, toks, parents in batch:
             rec = store.reserve(rid, len(toks))
             rows.append(dict(tokens=toks, ctx=rec.length, slot=rec.slot, pages=rec.pages, parents=parents))
+            self._drafted.pop(rid, None)  # (written over; nothing to accept should the step fail)
         b = make_step_batch(rows)
         with _weights_follow():
             logits = self.model.step(b, store, torch.arange(b.T, device="cuda"))
@@ -221,6 +222,8 @@ class SequenceEngine:
         and pages as earlier ones finish.  Returns the new tokens per prompt (EOS included when it was emitted): List[List[int]].
         logprobs = k (0 .. 32): (tokens, records), records per prompt and token a dict with its logprob, rank and entropy and the k most likely (id, logprob)
         pairs in `top`, under softmax(logits / temperature) where tokens are sampled and softmax(logits) else."""
+        if logprobs is not None and not 0 <= logprobs <= min(32, self.model.vocab_size):
+            raise ValueError(f"logprobs is 0 .. 32 and at most the vocabulary: got {logprobs}")
         records = {}
         sched = StepScheduler(self.store.num_slots, self.store.pool.num_pages, self.store.page, step_tokens, eos_token_id)
         for i, pr in enumerate(prompts):
@@ -252,6 +255,8 @@ class SequenceEngine:
         after another in portions of up to `step_tokens` tokens, whose logits are held at once."""
         if step_tokens < 1:
             raise ValueError("a portion has at least one token")
+        if not 0 <= top <= min(32, self.model.vocab_size):
+            raise ValueError(f"top is 0 .. 32 and at most the vocabulary: got {top}")
         prompts = [self._checked(("score", i), pr) for i, pr in enumerate(prompts)]
         scored = []
         for i, pr in enumerate(prompts):

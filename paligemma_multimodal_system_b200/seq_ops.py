@@ -427,7 +427,7 @@ def attn_prepare(qkv, b: StepBatch, freq, q_norm, k_norm, q_out, k_pages, v_page
     assert v_other is None or (v_other.dtype == qkv.dtype and v_other.stride(1) == 1 and v_other.shape == (b.T, G * vdim))
     assert qkv.stride(1) == 1 and freq.dtype == torch.float64 and qkv.dtype == q_out.dtype and (k_pages is None) == (v_pages is None)
     mode = 2 if norm_qk is NORM_PROJECTION else int(bool(norm_qk))
-    if isinstance(k_pages, QuantizedPages):
+    if isinstance(k_pages, QuantizedPages) or isinstance(v_pages, QuantizedPages):
         _check_quantized(k_pages, v_pages, G, dim, vdim, page)
         _on_current_device(qkv)
         assert q_out.is_contiguous()
@@ -547,7 +547,7 @@ def attn_ragged(q, k_pages, v_pages, gate, out, b: StepBatch, H, G, dim, vdim, s
         if krow or vrow or only_singles or skip_singles:
             raise ValueError("drafted trees go over a cache of one key row and one value row a token, all entries in one call")
         return attn_tree(q, k_pages, v_pages, gate, out, b, H, G, dim, vdim, scale, softcap, page, gate_per_head=gate_per_head, score=score)
-    if isinstance(k_pages, QuantizedPages):
+    if isinstance(k_pages, QuantizedPages) or isinstance(v_pages, QuantizedPages):
         _check_quantized(k_pages, v_pages, G, dim, vdim, page)
         if krow or vrow:
             raise ValueError("8-bit pages have rows of their own width")
@@ -611,6 +611,10 @@ def attn_ragged(q, k_pages, v_pages, gate, out, b: StepBatch, H, G, dim, vdim, s
 def _attn_rows(q, k_pages, v_pages, gate, out, b: StepBatch, H, G, dim, vdim, scale, softcap, page, gate_per_head, score, singles):
     if dim > 128 or vdim > 128:
         raise ValueError(f"attention of a few rows takes heads of up to 128 elements: got {dim} and {vdim}")
+    if q.dtype not in (torch.bfloat16, torch.float32) or out.dtype != q.dtype or (gate is not None and (gate.dtype != q.dtype or gate.stride(1) != 1)):
+        raise ValueError("queries, gate and output share a type, torch.bfloat16 or torch.float32")
+    if q.numel() != b.T * H * dim or not q.is_contiguous() or out.stride(-1) != 1 or H % G:
+        raise ValueError("queries are [rows, heads * size], heads a multiple of the key / value heads")
     import ctypes as C
     _on_current_device(q)
     quantized = isinstance(k_pages, QuantizedPages)
@@ -637,10 +641,8 @@ def attn_tree(q, k_pages, v_pages, gate, out, b: StepBatch, H, G, dim, vdim, sca
         _check_quantized(k_pages, v_pages, G, dim, vdim, page)
     elif k_pages.dtype != q.dtype or v_pages.dtype != q.dtype:
         raise ValueError("a cache that is not in 8 bits has the queries' type")
-    if q.dtype not in (torch.bfloat16, torch.float32) or out.dtype != q.dtype or (gate is not None and (gate.dtype != q.dtype or gate.stride(1) != 1)):
-        raise ValueError("queries, gate and output share a type, torch.bfloat16 or torch.float32")
-    if q.numel() != b.T * H * dim or not q.is_contiguous() or out.stride(-1) != 1 or H % G:
-        raise ValueError("queries are [rows, heads * size], heads a multiple of the key / value heads")
+    elif k_pages.shape[1:] != (page, G * dim) or v_pages.shape[1:] != (page, G * vdim) or not k_pages.is_contiguous() or not v_pages.is_contiguous():
+        raise ValueError(f"pages of {tuple(k_pages.shape)} and {tuple(v_pages.shape)} for {G} heads of {dim} / {vdim} and pages of {page} rows")
     if b.tree is not None and (b.tree.dtype != torch.int32 or b.tree.dim() != 2 or b.tree.shape[0] != b.T or not b.tree.is_contiguous()):
         raise ValueError("masks are int32 [rows, words]")
     _attn_rows(q, k_pages, v_pages, gate, out, b, H, G, dim, vdim, scale, softcap, page, gate_per_head, score, singles=False)

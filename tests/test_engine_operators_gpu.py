@@ -237,3 +237,26 @@ def test_the_command_prints_them(tmp_path, capsys):
     text = capsys.readouterr().out
     assert [len(t) for t in tokens] == [4, 4] and text.count("logprob") == 8 and len(said[0][0]["top"]) == 2
     assert generate_token_ids(str(tmp_path), "5 17 3; 8 9", 4, 0.8, 0.9, False, dtype="float32", kv_format="e4m3") == tokens
+
+
+def test_a_step_that_fails_leaves_no_drafts(monkeypatch):
+    eng = engine(ATTENTION, torch.float32)
+    eng.step([("a", toks(70, 80, 1), [])])
+    first = eng.step_drafts([("a", [3, 4], [-1, 0])])
+    with monkeypatch.context() as m:
+        m.setattr(eng.model, "step", lambda *a: (_ for _ in ()).throw(RuntimeError("no step")))
+        with pytest.raises(RuntimeError):
+            eng.step_drafts([("a", [5, 6, 7], [-1, 0, 1])])
+    with pytest.raises(KeyError):  # (the first drafts' rows may be written over)
+        eng.accept("a", [0])
+    assert torch.equal(eng.step_drafts([("a", [3, 4], [-1, 0])]), first)
+
+
+@pytest.mark.parametrize("count", [-1, 33, 81])
+def test_counts_of_alternatives_are_refused_before_anything_runs(count):
+    eng = engine(ATTENTION, torch.float32)
+    with pytest.raises(ValueError):
+        eng.generate([[1, 2, 3]], 4, logprobs=count)
+    with pytest.raises(ValueError):
+        eng.score([[1, 2, 3]], top=count)
+    assert not eng.store.live
