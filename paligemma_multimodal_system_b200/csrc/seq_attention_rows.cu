@@ -20,6 +20,8 @@
 // halves, 22 bits); fp32 as three bf16 terms, six products.  Weights: two bf16 terms over bf16 values (16 bits); one half over codes for bf16
 // rows (11 bits: an eighth of the output's own rounding), two for fp32 rows; three bf16 terms over fp32 values.  The values' powers of two
 // go into the weights relative to the largest one so far.  Scores, maxima, sums and outputs are fp32.
+// The matrix instruction cuts off what it adds to a larger sum; over many it adds up (fp32, 4700 keys: 1.0e-5 off).  For fp32 queries the small terms' products and every tile's
+// outputs have sums of their own, added with a rounding (1.2e-6, as fp32 operators have); for bf16 ones it is a hundredth of the output's rounding.
 //
 // What bounds it: while a k/v head has few rows, the bytes of keys and values where walks are long (6 x 32000 keys of 4 x 128 over codes 41 us, 4.7 TB/s), the unequal lengths of a
 // batch (64 x 1125 .. 2250 of 8 x 64 with soft cap and gate 38 us: the loop runs at the memory's rate, then short entries leave SMs empty), else a chain of trips
@@ -70,12 +72,12 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// tanh to fp32 accuracy: odd series near zero, else 1 - 2 / (e^(2 |x|) + 1)
+// tanh to fp32 accuracy: an odd polynomial below 0.625 (least squares on tanh(x) / x, 6e-9 off) -- scores are small against their cap --, else 1 - 2 / (e^(2 |x|) + 1)
 __device__ __forceinline__ float tanh_f32(float x) {
-  const float ax = fabsf(x), x2 = x * x;
-  const float small = x * fmaf(x2, fmaf(x2, 0.13333333f, -0.33333334f), 1.0f);
+  const float ax = fabsf(x), z = x * x;
+  const float p = fmaf(z, fmaf(z, fmaf(z, fmaf(z, -0.0057040425f, 0.020637862f), -0.053739157f), 0.13331431f), -0.33333281f);
   const float big = copysignf(1.0f - __fdividef(2.0f, ex2(ax * (2.f * kLog2e)) + 1.0f), x);
-  return ax < 0.1f ? small : big;
+  return ax < 0.625f ? fmaf(x * z, p, x) : big;
 }
 __device__ __forceinline__ float ldf(const float* p) { return *p; }
 __device__ __forceinline__ float ldf(const bf16* p) { return __bfloat162float(*p); }
@@ -168,6 +170,7 @@ template <typename TQ, typename TC, int DC, int VC, int MT, int KT>
 struct Kind {
   static constexpr int ES = sizeof(TC);
   static constexpr bool C8 = ES == 1, F32 = ES == 4, HALF = C8;
+  static constexpr bool APART = sizeof(TQ) == 4;
   static constexpr int QT = F32 ? 3 : (C8 && sizeof(TQ) == 4) ? 2 : 1;     // terms of a query
   static constexpr int STEPS = 4 * DC;                                     // 16-deep steps of the first product
   static constexpr int CT = F32 ? 3 : 1;                                   // terms of a cached element
@@ -399,7 +402,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
         for (int k = 0; k < 4; ++k) v[u][k] *= up;
       }
       if (r >= rows_staged) break;
-      if (w == 0) unscale[r] = a.mode == kGeneral ? s : a.mode == kCapped ? s * (2.f * kLog2e / a.softcap) : s * kLog2e;
+      if (w == 0) unscale[r] = a.mode == kGeneral ? s : a.mode == kCapped ? s * ((sizeof(TQ) == 2 ? 2.f * kLog2e : 1.f) / a.softcap) : s * kLog2e;
       // row r of its tile: lanes 4 (r % 8) + c, first or second half of the fragment's registers
       {
         uint32_t p[K::QT], s2[K::QT];
@@ -500,13 +503,13 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
     }
     if (live <= 0) continue;  // no rows for this warp
     // ---- S = Q K^T
-    float s[MT][NB][4];
+    float s[MT][NB][4], small[MT][NB][4];  // small: products of all but the first terms (fp32 queries)
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int f = 0; f < NB; ++f)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s[m][f][k] = 0.f;
+        for (int k = 0; k < 4; ++k) s[m][f][k] = small[m][f][k] = 0.f;
     constexpr int SPL = K::C8 ? 4 : K::F32 ? 1 : 2;  // steps of a piece
 #pragma unroll
     for (int x = 0; x < K::STEPS / SPL; ++x) {
@@ -542,9 +545,17 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
             for (int t = K::QT - 1; t >= 0; --t)  // small terms first
 #pragma unroll
               for (int t2 = K::CT - 1; t2 >= 0; --t2)
-                if (t + t2 < 3) mma<K::HALF>(s[m][f], qa[m][t], b0[t2], b1[t2]);
+                if (t + t2 < 3) mma<K::HALF>(K::APART && t + t2 > 0 ? small[m][f] : s[m][f], qa[m][t], b0[t2], b1[t2]);
         }
       }
+    }
+    if (K::APART) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int f = 0; f < NB; ++f)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) s[m][f][k] += small[m][f][k];
     }
     // ---- weights: one straight line but for options, masks and new maxima
     uint64_t kf[NB], vf[NB];  // pairs of powers: keys 2 f, 2 f + 1 of this lane
@@ -586,11 +597,11 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
 #pragma unroll
         for (int f = 0; f < NB; ++f) t[m][h][f] = mul_pair(pg::pair_of(s[m][f][2 * h], s[m][f][2 * h + 1]), K::C8 ? mul_pair(u, kf[f]) : u);
       }
-    if (a.mode == kCapped) {  // cap tanh(v / cap) in log2 units; v comes as 2 log2(e) v / cap
+    if (a.mode == kCapped) {  // cap tanh(v / cap) in log2 units; v comes as v / cap, for bf16 queries times 2 log2(e)
       const float cap = a.softcap * kLog2e;
       auto bend = [&](float v) {
         if (sizeof(TQ) == 2) return fmaf(-2.f * cap, rcp(ex2(v) + 1.f), cap);  // off by 2^-22 cap: the output's rounding is 2^-9
-        return cap * tanh_f32(v * (0.5f / kLog2e));
+        return cap * tanh_f32(v);
       };
 #pragma unroll
       for (int m = 0; m < MT; ++m)
@@ -740,15 +751,23 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
           }
           if (R8 && y % 2 == 0) continue;
 #pragma unroll
-          for (int m = 0; m < MT; ++m)
+          for (int m = 0; m < MT; ++m) {
+            float(&acc)[4] = o[m][R8 ? (4 * b + y / 2) % OB : (8 * b + y) % OB];
+            float own[4] = {0.f, 0.f, 0.f, 0.f};  // fp32 queries: a tile's products apart, added with a rounding
+            float(&sum)[4] = K::APART ? own : acc;
 #pragma unroll
             for (int t = K::PT - 1; t >= 0; --t)
 #pragma unroll
               for (int t2 = K::CT - 1; t2 >= 0; --t2)
                 if (t + t2 < 3) {
-                  if (R8) mma<K::HALF>(o[0][(4 * b + y / 2) % OB], make_uint4(w0[0][t2], w0[1][t2], w1[0][t2], w1[1][t2]), pa[0][q][t].x, pa[0][q][t].z);
-                  else mma<K::HALF>(o[m][(8 * b + y) % OB], pa[m][q][t], b0[t2], b1[t2]);
+                  if (R8) mma<K::HALF>(sum, make_uint4(w0[0][t2], w0[1][t2], w1[0][t2], w1[1][t2]), pa[0][q][t].x, pa[0][q][t].z);
+                  else mma<K::HALF>(sum, pa[m][q][t], b0[t2], b1[t2]);
                 }
+            if (K::APART) {
+#pragma unroll
+              for (int x = 0; x < 4; ++x) acc[x] += own[x];
+            }
+          }
         }
       }
     }
