@@ -313,3 +313,23 @@ def test_the_same_call_gives_the_same_bits():
         seq_ops.attn_tree(c.q, *c.kv, None, c.out, c.b, 8, 2, 64, 64, 0.125, 0.0, PAGE)
         seen.append(c.out.clone())
     assert all(torch.equal(x, seen[0]) for x in seen)
+
+
+@pytest.mark.parametrize("dtype,cache", [(torch.float32, "same"), (torch.float32, "e4m3")])
+@pytest.mark.parametrize("nodes", [1, 13])
+def test_long_sums_are_rounded_and_not_cut(dtype, cache, nodes):
+    """Values of one sign under nearly equal weights, walks that nobody shares (24 entries x 8 heads): about 90 tiles are added to a growing sum.  Rounded to nearest they are off by
+    half a step of 2^-24 each with random signs, sqrt(90) 2^-24 = 2^-20.8 together and a sixth of 2^-18; cut off, by half a step with one sign an instruction, six of them a tile:
+    90 * 6 * 2^-25 = 2^-16.  Weights: three bf16 terms (2^-24) or two halves (2^-22 at random); what a score or the exponential is off has the same sign for all keys of a row and cancels."""
+    c = Case(dtype, cache, [(nodes, 3000 - 9 * i) for i in range(24)], 16, 8, 64, 64, None if nodes == 1 else [random_tree(nodes, i) for i in range(24)], seed=30, spread=1e-3)
+    v = c.kv[1]
+    if cache == "e4m3":
+        v.codes.bitwise_and_(0x7f)
+        v.codes.copy_(torch.where(v.codes == 0x7f, v.codes, 0x38 + v.codes % 8))  # 1 .. 1.875
+        v.powers.fill_(120)
+        c.kv[0].powers.fill_(110)  # (small scores)
+    else:
+        v.abs_().add_(0.5)
+    got = c.check()
+    want, _ = c.want(c.dim ** -0.5)
+    assert float(((got - want) / want).abs().max()) < 2.0 ** -18
