@@ -69,9 +69,9 @@ static_assert(sizeof(PgPrepareE4m3) == 192 && sizeof(PgReadE4m3) == 112, "caller
 // and sines (angles in double) are made once for all heads behind the first vectors' requests; four vectors of a group are under way together: one head of four tokens,
 // which share its weights, or four heads of one token.
 // Elements that a norm or a rotation computes are fp32; where that could choose the code beside the nearest (one in a million would be), the head's vector is marked and made again
-// in double behind the loop, so that the codes are those of the exact elements -- but for
-// one in some ten million that a rotation or a blend leaves small beside its parts, whose errors count by those: doubting by the parts took 37.7 us for the first size below.  Inside the loop the same work costs twice as much (its registers are live beside four vectors'):
-// 36.9 us against 34.4 for the first size below, 30.8 without it.
+// in double behind the loop, so that the codes are those of the exact elements -- but for one in some ten million that a rotation or a blend leaves small beside its parts, whose
+// errors count by those (doubting by the parts: 37.7 us for the first size below against 34.4; 30.8 without any of it).  Inside the loop the second making cost 36.9: its registers
+// are live beside four vectors'.
 // What bounds it: for prompts instructions, then the bytes (a row is read once, 8-bit rows are half of bf16 ones); for a few rows the chain row -> sum -> largest -> codes.
 // 7,796 bf16 rows of 32 + 8 + 8 heads of 64, normed and turned, in 34.4 us (2.6 of 6.6 TB/s; 28.8 into pages of bf16); 1,363 fp32 rows of 16 + 4 + 4 heads of 128 as they come in 12.4;
 // 23 rows in 6.2.
