@@ -56,17 +56,17 @@ class StepBatch:
     shared: Optional[dict] = None
     min_n: int = 1            # the fewest new tokens of an entry (1 where that is not known)
 
-    # (no fields: TreeBatch)
-    at = None
-    tree = None
+    # drafted trees: `pos`, which turns queries and keys, is then ctx + depth; rows are stored one behind another at cache rows `at`, and a row sees the
+    # drafted rows of its entry whose bit is set in its mask (bit m % 32 of word m / 32)
+    # (taken by name, or behind the others; `dataclasses.replace` keeps them)
+    at: dataclasses.InitVar[Optional[torch.Tensor]] = None    # int32 [T]; None: pos
+    tree: dataclasses.InitVar[Optional[torch.Tensor]] = None  # int32 [T, words]; None: rows see every row in front of them
+
+    def __post_init__(self, at, tree):
+        self.at, self.tree = at, tree
 
 
-@dataclasses.dataclass
-class TreeBatch(StepBatch):
-    """A step of drafted trees: `pos`, which turns queries and keys, is ctx + depth; rows are stored one behind another at cache rows `at`; a row sees the
-    drafted rows of its entry whose bit is set in its mask (bit m % 32 of word m / 32)."""
-    at: Optional[torch.Tensor] = None    # int32 [T]; None: pos
-    tree: Optional[torch.Tensor] = None  # int32 [T, words]; None: rows see every row in front of them
+TreeBatch = StepBatch  # (another name for a step that has these two)
 
 
 def _single_rows(ns):
@@ -142,15 +142,13 @@ def make_step_batch(entries: Sequence[dict]) -> StepBatch:
         pos[:] = ctx[row_entry] + depth
     dev = torch.from_numpy(buf).pin_memory().to("cuda", non_blocking=True)
     o = 3 * T
-    kind, more = StepBatch, {}
-    if masks is not None:
-        kind, more = TreeBatch, dict(at=dev[plain:plain + T], tree=dev[plain + T:].view(T, words))
-    return kind(T=T, E=E, max_n=max(ns), min_n=min(ns), tokens=dev[:T], pos=dev[T:2 * T], row_entry=dev[2 * T:3 * T], row0=dev[o:o + E],
+    drafted = {} if masks is None else dict(at=dev[plain:plain + T], tree=dev[plain + T:].view(T, words))
+    return StepBatch(T=T, E=E, max_n=max(ns), min_n=min(ns), tokens=dev[:T], pos=dev[T:2 * T], row_entry=dev[2 * T:3 * T], row0=dev[o:o + E],
                      n=dev[o + E:o + 2 * E], ctx=dev[o + 2 * E:o + 3 * E], slot=dev[o + 3 * E:o + 4 * E],
                      page_table=dev[o + 4 * E:o2].view(E, max_pages), max_pages=max_pages, singles=sum(k == 1 for k in ns),
                      max_single_ctx=max([e["ctx"] for e, k in zip(entries, ns) if k == 1], default=0), single_rows=_single_rows(ns),
                      dense_row0=dev[o2:o2 + E], dense_pages=dev[o2 + E:plain].view(E, dmax), dense_max_pages=dmax, dense_rows=page0 * 64,
-                     dense_max_len=max(lens), **more)
+                     dense_max_len=max(lens), **drafted)
 
 
 def step_scope(b: StepBatch) -> StepBatch:
