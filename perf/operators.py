@@ -292,7 +292,7 @@ def run(state):
     from paligemma_multimodal_system_b200 import seq_ops
     if kind == "score":
         return list(seq_ops.token_logprobs(s["logits"], s["tokens"], top=s["top"], temperature=s["temperature"]))
-    b, H, G, dim = (seq_ops.TreeBatch if kind == "tree" else seq_ops.StepBatch)(**s["plan"]), s["heads"], s["kv_heads"], s["dim"]
+    b, H, G, dim = seq_ops.StepBatch(**s["plan"]), s["heads"], s["kv_heads"], s["dim"]
     k, v = (seq_ops.QuantizedPages(*s[x]) if isinstance(s[x], tuple) else s[x] for x in "kv")
     if kind == "store":
         q = torch.empty(b.T, H * dim, device="cuda", dtype=s["type"])
