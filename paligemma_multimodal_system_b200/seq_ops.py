@@ -551,8 +551,8 @@ def attn_ragged(q, k_pages, v_pages, gate, out, b: StepBatch, H, G, dim, vdim, s
             raise ValueError("8-bit pages have rows of their own width")
         if b.singles < b.E and not only_singles:
             k, v = kv_read(k_pages, v_pages, b, q.dtype)
-            attn_ragged(q, k, v, gate, out, dense_view(b), H, G, dim, vdim, scale, softcap, page, decode_kernel, tensor_cores, gate_per_head=gate_per_head, skip_singles=True,
-                        score=score)
+            attn_ragged(q, k, v, gate, out, dense_view(b), H, G, dim, vdim, scale, softcap, 64, decode_kernel, tensor_cores, gate_per_head=gate_per_head, skip_singles=True,
+                        score=score)  # (the scratch's pages hold 64 rows, whatever the cache's do)
         if b.singles and not skip_singles:
             _attn_rows(q, k_pages, v_pages, gate, out, b, H, G, dim, vdim, scale, softcap, page, gate_per_head, score, singles=True)
         return
