@@ -1,5 +1,7 @@
 """8-bit caches whose pages hold 32 or 128 rows: a mixed step gives what it gives over pages of 64 (whose results are tested against the formula), bit by bit -- the same tiles of
 keys are walked in the same order, wherever they lie."""
+import dataclasses
+
 import numpy as np
 import pytest
 import torch
@@ -8,12 +10,14 @@ pytestmark = pytest.mark.gpu
 
 
 def _step(page, lens, seed):
-    """(batch, pages of every entry, pages in all): pages in any order."""
+    """(batch, pages of every entry, pages in all): pages in any order.  The engine's pages hold 64 rows: the table of others takes the place of its own."""
     from paligemma_multimodal_system_b200 import seq_ops
     need = [-(-(n + c) // page) for n, c in lens]
     order = np.random.RandomState(seed).permutation(sum(need) + 2).tolist()
-    entries = [dict(tokens=[1] * n, ctx=c, slot=i, pages=[order.pop() for _ in range(k)]) for i, ((n, c), k) in enumerate(zip(lens, need))]
-    return seq_ops.make_step_batch(entries), [e["pages"] for e in entries], sum(need) + 2
+    pages = [[order.pop() for _ in range(k)] for k in need]
+    b = seq_ops.make_step_batch([dict(tokens=[1] * n, ctx=c, slot=i, pages=range(-(-(n + c) // 64))) for i, (n, c) in enumerate(lens)])
+    table = torch.tensor([own + [0] * (max(need) - len(own)) for own in pages], dtype=torch.int32, device="cuda")
+    return dataclasses.replace(b, page_table=table, max_pages=max(need)), pages, sum(need) + 2
 
 
 def _paged(codes, powers, page, pages, pool):
