@@ -19,7 +19,9 @@
 // Precision: bf16 operands as they are; codes as halves, exact, against queries scaled by a power of two per row into half range (fp32 queries: two
 // halves, 22 bits); fp32 as three bf16 terms, six products.  Weights: two bf16 terms over bf16 values (16 bits); one half over codes for bf16
 // rows (11 bits: an eighth of the output's own rounding), two for fp32 rows; three bf16 terms over fp32 values.  The values' powers of two
-// go into the weights relative to the largest one so far.  Scores, maxima, sums and outputs are fp32.
+// go into the weights, which are taken relative to the row's largest product of weight and power so far: what falls 2^-38 below it counts as zero (the head with that product keeps its
+// own elements no finer than 2^-10 of its power).  Relative to the largest power met, a row that a query does not see or one of no weight took the others' values away.  24 trees of
+// 31 x 4 rows over codes 75 -> 80 us, decoded tokens as before.  Weights below 2^-126 of a row's largest are zero.  Scores, maxima, sums and outputs are fp32.
 // The matrix instruction cuts off what it adds to a larger sum; over many it adds up (fp32, 4700 keys: 1.0e-5 off).  For fp32 queries the small terms' products and every tile's
 // outputs have sums of their own, added with a rounding (1.2e-6, as fp32 operators have); for bf16 ones it is a hundredth of the output's rounding.
 //
@@ -166,6 +168,9 @@ __device__ __forceinline__ uint32_t no_numbers(uint32_t w) {
   return (w & 0x7f800000u) == 0x7f800000u ? 0xffffffffu : 0u;
 }
 
+// The power (as an exponent's byte) that takes a row's largest product of weight and power to [2^14, 2^15): halves reach 38 bits below.
+__device__ __forceinline__ int lift_of(float largest) { return min(14 + 2 * 127 - static_cast<int>(__float_as_uint(largest) >> 23), 254); }
+
 template <typename TQ, typename TC, int DC, int VC, int MT, int KT>
 struct Kind {
   static constexpr int ES = sizeof(TC);
@@ -277,7 +282,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
   extern __shared__ __align__(128) unsigned char raw[];
   __shared__ float unscale[kWarps * 16 * MT];  // what a row's scores are multiplied by
   __shared__ float2 stat[kWarps][16 * MT];
-  __shared__ float top_power[kWarps];
+  __shared__ float power[kWarps][16 * MT];  // what a warp's sums of a row are multiplied by (8-bit cache)
   __shared__ float2 joined[kWarps * 16 * MT];
   __shared__ int2 where_to[kWarps * 16 * MT];  // a row's token of the entry and its head; past the last row: the last one's
   __shared__ float share[8][kWarps * 16 * MT];
@@ -439,7 +444,9 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
     for (int b = 0; b < OB; ++b)
 #pragma unroll
       for (int k = 0; k < 4; ++k) o[m][b][k] = 0.f;
-  int P = 0;  // largest power of a value row so far (byte)
+  float top[2 * MT];  // 8-bit cache: a row's largest weight times power so far, against its maximum
+#pragma unroll
+  for (int x = 0; x < 2 * MT; ++x) top[x] = 0.f;
 
   bool bad = false;  // a value that is no number in a tile with a mask
 #pragma unroll 1
@@ -559,32 +566,17 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
     }
     // ---- weights: one straight line but for options, masks and new maxima
     uint64_t kf[NB], vf[NB];  // pairs of powers: keys 2 f, 2 f + 1 of this lane
-    float grow = 1.f;         // 2^(P - new P)
     if (K::C8) {
-      uint32_t kpw[KPL / 4], vpw[KPL / 4];
 #pragma unroll
       for (int x = 0; x < KPL / 4; ++x) {
-        kpw[x] = *reinterpret_cast<const uint32_t*>(stage + KT * (K::KROW + K::VROW) + KPL * c + 4 * x);
-        vpw[x] = *reinterpret_cast<const uint32_t*>(stage + KT * (K::KROW + K::VROW) + KT + KPL * c + 4 * x);
-      }
-      uint32_t most = vpw[0];
+        const uint32_t kp = *reinterpret_cast<const uint32_t*>(stage + KT * (K::KROW + K::VROW) + KPL * c + 4 * x);
+        const uint32_t vp = *reinterpret_cast<const uint32_t*>(stage + KT * (K::KROW + K::VROW) + KT + KPL * c + 4 * x);
 #pragma unroll
-      for (int x = 1; x < KPL / 4; ++x) most = __vmaxu4(most, vpw[x]);
-      most = __vmaxu4(most, most >> 16);
-      most = max(most & 0xffu, most >> 8 & 0xffu);
-      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-      const int top = max(P, static_cast<int>(max(most, __shfl_xor_sync(0xffffffffu, most, 2))));
-      grow = __uint_as_float(static_cast<uint32_t>(max(127 - (top - P), 0)) << 23);
-      P = top;
-      // 2^(15 + power - P): a weight of one is 2^15, halves reach down to 2^-24; four bytes at a time, P - 142 <= byte <= P, so that none carries into the next
-      const uint32_t least = static_cast<uint32_t>(max(P - 142, 0)) * 0x01010101u, lift = static_cast<uint32_t>(142 - P) * 0x01010101u;
-#pragma unroll
-      for (int x = 0; x < KPL / 4; ++x) vpw[x] = __vmaxu4(vpw[x], least) + lift;
-#pragma unroll
-      for (int f = 0; f < NB; ++f) {  // (a key's byte 0: what is below 2^-118 counts as zero)
-        const int sh = 8 * (2 * f % 4);
-        kf[f] = pg::pair_of((kpw[f / 2] >> sh & 0xffu) << 23, (kpw[f / 2] >> (sh + 8) & 0xffu) << 23);
-        vf[f] = pg::pair_of((vpw[f / 2] >> sh & 0xffu) << 23, (vpw[f / 2] >> (sh + 8) & 0xffu) << 23);
+        for (int y = 0; y < 2; ++y) {  // (a key's byte 0: what is below 2^-118 counts as zero)
+          const int sh = 16 * y;
+          kf[2 * x + y] = pg::pair_of((kp >> sh & 0xffu) << 23, (kp >> (sh + 8) & 0xffu) << 23);
+          vf[2 * x + y] = pg::pair_of(cache8::value_of_power(vp >> sh & 0xffu), cache8::value_of_power(vp >> (sh + 8) & 0xffu));
+        }
       }
     }
     constexpr int HS = R8 ? 1 : 2;
@@ -660,7 +652,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         const float now = a.sx.logistic ? 0.f : fmaxf(M[x], mx), ref = now == -INFINITY ? 0.f : now;  // nothing seen so far: weights of zero
         const float shrink = ex2(M[x] - ref);
-        corr[x] = shrink * grow;
+        corr[x] = shrink;
         M[x] = now;
         const uint64_t minus = pg::pair_of(-ref, -ref);
         uint64_t sum = 0;
@@ -672,6 +664,20 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
           t[m][h][f] = K::C8 ? mul_pair(p, vf[f]) : p;
         }
         L[x] = fmaf(L[x], shrink, pg::lo_f32(sum) + pg::hi_f32(sum));
+        if (K::C8) {
+          float most = fmaxf(pg::lo_f32(t[m][h][0]), pg::hi_f32(t[m][h][0]));
+#pragma unroll
+          for (int f = 1; f < NB; ++f) most = pg::max3(most, pg::lo_f32(t[m][h][f]), pg::hi_f32(t[m][h][f]));
+          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+          const int was = lift_of(top[x]);
+          top[x] = fmaxf(top[x] * shrink, most);
+          const int lift = lift_of(top[x]);
+          corr[x] *= __uint_as_float(static_cast<uint32_t>(min(max(127 + lift - was, 0), 254)) << 23);
+          const float by = __uint_as_float(static_cast<uint32_t>(lift) << 23);
+#pragma unroll
+          for (int f = 0; f < NB; ++f) t[m][h][f] = mul_pair(t[m][h][f], pg::pair_of(by, by));
+        }
         moved |= corr[x] != 1.f;
       }
     if (__any_sync(0xffffffffu, moved)) {
@@ -785,6 +791,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     const int r = 16 * (x / 2) + 8 * (x % 2) + nn;
     if (c == 0) stat[warp][r] = make_float2(M[x], l);
+    if (K::C8 && c == 0) power[warp][r] = cache8::value_of_power(254 - lift_of(top[x]));
     if (R8) continue;
     float* dst = os + (warp * 16 * MT + r) * ldo_s;
 #pragma unroll
@@ -812,7 +819,6 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
             *reinterpret_cast<float4*>(dst + 4 * y) = make_float4(o[0][4 * b + 2 * y][i], o[0][4 * b + 2 * y][2 + i], o[0][4 * b + 2 * y + 1][i], o[0][4 * b + 2 * y + 1][2 + i]);
         }
   }
-  if (K::C8 && lane == 0) top_power[warp] = static_cast<float>(P);
   if (bad) any_bad = 1;
   __syncthreads();
   const int rows_here = min(rows_cta, R - r0);
@@ -825,7 +831,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
     const float by = a.nsplit == 1 ? last_factor(a, where_to[r].y, ref, l) : 1.f;
     for (int w = 0; w < wk; ++w) {
       float2& st = stat[w * wr + tile][in];
-      st.x = ex2(st.x - ref) * by * (K::C8 ? exp2f(top_power[w * wr + tile] - 142.f) : 1.f);  // the weights' power: 2^(P - 127 - 15)
+      st.x = ex2(st.x - ref) * by * (K::C8 ? power[w * wr + tile][in] : 1.f);
     }
     joined[r] = make_float2(m, l);
   }
