@@ -17,11 +17,12 @@
 // cluster, more through scratch and a second launch.
 //
 // Precision: bf16 operands as they are; codes as halves, exact, against queries scaled by a power of two per row into half range (fp32 queries: two
-// halves, 22 bits); fp32 as three bf16 terms, six products.  Weights: two bf16 terms over bf16 values (16 bits); one half over codes for bf16
-// rows (11 bits: an eighth of the output's own rounding), two for fp32 rows; three bf16 terms over fp32 values.  The values' powers of two
+// halves, 22 bits); fp32 as three bf16 terms, six products.  Weights: two halves over codes (22 bits; one half, 11 bits, left
+// one output of bf16 rows in forty beside the one that fp32 weights give, two one in 1,700: 24 trees of 31 x 4 rows 80 -> 90 us, decoded tokens 6 %); two bf16 terms over bf16 values
+// (16 bits: one output in 1,000 beside it, three terms one in 1,400 at 12 % of the time); three over fp32 values.  The values' powers of two
 // go into the weights, which are taken relative to the row's largest product of weight and power so far: what falls 2^-38 below it counts as zero (the head with that product keeps its
 // own elements no finer than 2^-10 of its power).  Relative to the largest power met, a row that a query does not see or one of no weight took the others' values away.  24 trees of
-// 31 x 4 rows over codes 75 -> 80 us, decoded tokens as before.  Weights below 2^-126 of a row's largest are zero.  Scores, maxima, sums and outputs are fp32.
+// 31 x 4 rows over codes 76 -> 80 us, decoded tokens as before.  Weights below 2^-126 of a row's largest are zero.  Scores, maxima, sums and outputs are fp32.
 // The matrix instruction cuts off what it adds to a larger sum; over many it adds up (fp32, 4700 keys: 1.0e-5 off).  For fp32 queries the small terms' products and every tile's
 // outputs have sums of their own, added with a rounding (1.2e-6, as fp32 operators have); for bf16 ones it is a hundredth of the output's rounding.
 //
@@ -179,7 +180,7 @@ struct Kind {
   static constexpr int QT = F32 ? 3 : (C8 && sizeof(TQ) == 4) ? 2 : 1;     // terms of a query
   static constexpr int STEPS = 4 * DC;                                     // 16-deep steps of the first product
   static constexpr int CT = F32 ? 3 : 1;                                   // terms of a cached element
-  static constexpr int PT = F32 ? 3 : C8 ? (sizeof(TQ) == 4 ? 2 : 1) : 2;  // terms of a weight
+  static constexpr int PT = F32 ? 3 : 2;  // terms of a weight
   static constexpr int VW = 2 * ES;                                        // words of eight value columns
   static constexpr int KROW = 64 * DC * ES, VROW = 64 * VC * ES;           // bytes of a row in shared memory
   static constexpr int STAGE = KT * (KROW + VROW) + (C8 ? 2 * KT : 0);
