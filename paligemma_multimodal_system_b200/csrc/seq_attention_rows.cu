@@ -76,11 +76,13 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 // tanh to fp32 accuracy: an odd polynomial below 0.625 (least squares on tanh(x) / x, 6e-9 off) -- scores are small against their cap --, else 1 - 2 / (e^(2 |x|) + 1)
+constexpr float kSmall = 0.625f;
+constexpr float kTanh0 = -0.33333281f, kTanh1 = 0.13331431f, kTanh2 = -0.053739157f, kTanh3 = 0.020637862f, kTanh4 = -0.0057040425f;
 __device__ __forceinline__ float tanh_f32(float x) {
   const float ax = fabsf(x), z = x * x;
-  const float p = fmaf(z, fmaf(z, fmaf(z, fmaf(z, -0.0057040425f, 0.020637862f), -0.053739157f), 0.13331431f), -0.33333281f);
+  const float p = fmaf(z, fmaf(z, fmaf(z, fmaf(z, kTanh4, kTanh3), kTanh2), kTanh1), kTanh0);
   const float big = copysignf(1.0f - __fdividef(2.0f, ex2(ax * (2.f * kLog2e)) + 1.0f), x);
-  return ax < 0.625f ? fmaf(x * z, p, x) : big;
+  return ax < kSmall ? fmaf(x * z, p, x) : big;
 }
 __device__ __forceinline__ float ldf(const float* p) { return *p; }
 __device__ __forceinline__ float ldf(const bf16* p) { return __bfloat162float(*p); }
@@ -409,7 +411,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
         for (int k = 0; k < 4; ++k) v[u][k] *= up;
       }
       if (r >= rows_staged) break;
-      if (w == 0) unscale[r] = a.mode == kGeneral ? s : a.mode == kCapped ? s * ((sizeof(TQ) == 2 ? 2.f * kLog2e : 1.f) / a.softcap) : s * kLog2e;
+      if (w == 0) unscale[r] = a.mode == kGeneral ? s : a.mode == kCapped ? s / a.softcap : s * kLog2e;
       // row r of its tile: lanes 4 (r % 8) + c, first or second half of the fragment's registers
       {
         uint32_t p[K::QT], s2[K::QT];
@@ -591,18 +593,36 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
 #pragma unroll
         for (int f = 0; f < NB; ++f) t[m][h][f] = mul_pair(pg::pair_of(s[m][f][2 * h], s[m][f][2 * h + 1]), K::C8 ? mul_pair(u, kf[f]) : u);
       }
-    if (a.mode == kCapped) {  // cap tanh(v / cap) in log2 units; v comes as v / cap, for bf16 queries times 2 log2(e)
+    if (a.mode == kCapped) {  // cap tanh(v / cap) in log2 units; v comes as v / cap
       const float cap = a.softcap * kLog2e;
-      auto bend = [&](float v) {
-        if (sizeof(TQ) == 2) return fmaf(-2.f * cap, rcp(ex2(v) + 1.f), cap);  // off by 2^-22 cap: the output's rounding is 2^-9
-        return cap * tanh_f32(v);
-      };
+      float far = 0.f;
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int h = 0; h < HS; ++h)
 #pragma unroll
-          for (int f = 0; f < NB; ++f) t[m][h][f] = pg::pair_of(bend(pg::lo_f32(t[m][h][f])), bend(pg::hi_f32(t[m][h][f])));
+          for (int f = 0; f < NB; ++f) far = pg::max3(far, fabsf(pg::lo_f32(t[m][h][f])), fabsf(pg::hi_f32(t[m][h][f])));
+      // (fp32 rows of several tokens over codes have no registers for both: 24 trees of 31 x 4 without a cap 109 -> 114 us, with one 131 -> 125)
+      if ((K::C8 && K::APART && !R8) || __any_sync(0xffffffffu, far >= kSmall)) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int h = 0; h < HS; ++h)
+#pragma unroll
+            for (int f = 0; f < NB; ++f) t[m][h][f] = pg::pair_of(cap * tanh_f32(pg::lo_f32(t[m][h][f])), cap * tanh_f32(pg::hi_f32(t[m][h][f])));
+      } else {  // scores are small against their cap: two at a time
+        auto both = [](float x) { return pg::pair_of(x, x); };
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int h = 0; h < HS; ++h)
+#pragma unroll
+            for (int f = 0; f < NB; ++f) {
+              const uint64_t x = t[m][h][f], z = mul_pair(x, x);
+              const uint64_t p = pg::fma_pair(z, pg::fma_pair(z, pg::fma_pair(z, pg::fma_pair(z, both(kTanh4), both(kTanh3)), both(kTanh2)), both(kTanh1)), both(kTanh0));
+              t[m][h][f] = mul_pair(pg::fma_pair(mul_pair(x, z), p, x), both(cap));
+            }
+      }
     } else if (a.mode == kGeneral) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)

@@ -63,3 +63,11 @@ def _off(cache, lens, kind, cap, H=16, G=4):
 def test_weights(cache, lens, kind):
     if cache == "e4m3" or kind:
         assert _off(cache, lens, kind, 0.0) <= 0
+
+
+@pytest.mark.parametrize("cache", ["e4m3", "same"])
+@pytest.mark.parametrize("lens,kind", SHAPES)
+@pytest.mark.parametrize("cap", [2.0, 30.0, 500.0, 2000.0])
+def test_capped_scores(cache, lens, kind, cap):
+    if cache == "e4m3" or kind:
+        assert _off(cache, lens, kind, cap) <= 0
