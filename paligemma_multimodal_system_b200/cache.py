@@ -35,6 +35,9 @@ class KvSpec(tuple):
         self.heads = int(heads)
         return self
 
+    def __getnewargs__(self):  # (copies and pickles make it anew)
+        return self[1], self[2], self.heads
+
 
 class PagePool:
     """Host-side free list of page ids (no tensors; CPU-testable)."""
