@@ -802,7 +802,7 @@ int pg_moe_combine_norm_add(const float* expert_out, long long ldy, const int* p
 
 /* One pass over fp32 logits rows: with z = logits / temperature, the log probability of tokens[row] under softmax(z), its rank (0: the largest; ties: the
  * lower index is in front), the entropy in nats, and the `top` largest entries in order (ids, log probabilities), top 0 .. 32, at most V.  A token outside
- * 0 .. V - 1: NaN and rank -1.  Masked entries are -inf; a row with a NaN, a +inf or nothing but -inf has NaN for every number (its ids: NaN behind -inf). */
+ * 0 .. V - 1, or whose own logit is a NaN: NaN and rank -1.  Masked entries are -inf; a row with a NaN, a +inf or nothing but -inf has NaN for every number (its ids: NaN behind -inf). */
 int pg_token_logprobs(const float* logits, long long ld, const int* tokens, float* logprob, float* entropy, int* rank, int* top_ids, float* top_logprob,
                       int rows, int V, int top, float temperature, void* stream);
 

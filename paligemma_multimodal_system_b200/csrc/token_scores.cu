@@ -160,6 +160,7 @@ __device__ __forceinline__ void list_hits(Shared& sh, const Part& p, int V, floa
 
 // the number behind x: what is larger than x reaches it.  Behind +inf and NaN: NaN, which nothing reaches.
 __device__ __forceinline__ float number_above(float x) {
+  if (x != x) return x;
   const uint32_t b = __float_as_uint(x + 0.0f);
   return __uint_as_float(x + 0.0f < 0.f ? b - 1u : b + 1u);
 }
@@ -452,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) token_logprobs_kernel(const 
       if (lane == 0) {
         logprob[row] = known ? (xt - a.m) * inv_t - ln_s : __uint_as_float(0x7fc00000u);
         entropy[row] = ln_s - kLn2 * (a.u / a.s);
-        rank[row] = known ? sh.rank : -1;
+        rank[row] = known && xt == xt ? sh.rank : -1;  // (a NaN has no place among numbers)
       }
       if (TOP && lane < top) {
         const unsigned long long k = sh.best[lane];

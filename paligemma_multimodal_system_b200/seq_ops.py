@@ -650,7 +650,7 @@ def attn_tree(q, k_pages, v_pages, gate, out, b: StepBatch, H, G, dim, vdim, sca
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, temperature: float = 1.0):
     """logits fp32 [rows, vocab] (any row pitch), tokens int32 [rows]: under softmax(logits / temperature) the log probability of every row's token, the entropy in
     nats, the token's rank (0: the most likely one; ties: the lower id is in front) and the `top` (0 .. 32) most likely ids with their log probabilities:
-    (fp32 [rows], fp32 [rows], int32 [rows], int32 [rows, top], fp32 [rows, top]).  A token outside the vocabulary: NaN and rank -1.  Masked entries are -inf; a row
+    (fp32 [rows], fp32 [rows], int32 [rows], int32 [rows, top], fp32 [rows, top]).  A token outside the vocabulary, or whose own logit is a NaN: NaN and rank -1.  Masked entries are -inf; a row
     with a NaN, a +inf or nothing but -inf has NaN for its numbers."""
     if logits.dim() != 2 or logits.dtype != torch.float32 or logits.stride(1) != 1 or not logits.is_cuda:
         raise ValueError("logits are fp32 [rows, vocab] on the device, entries of a row side by side")
