@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) token_logprobs_kernel(const 
 
 extern "C" int pg_token_logprobs(const float* logits, long long ld, const int* tokens, float* logprob, float* entropy, int* rank, int* top_ids, float* top_logprob,
                                  int rows, int V, int top, float temperature, void* stream) {
-  if (rows <= 0 || V <= 0 || top < 0 || top > kTop || top > V || ld < V || !(temperature > 0.f) || !(temperature < INFINITY) || !(1.0f / temperature < INFINITY)) return PG_ERR_ARG;
+  if (rows <= 0 || V <= 0 || top < 0 || top > kTop || top > V || ld < V || !(temperature > 0.f) || !(temperature < INFINITY) || !(1.0f / temperature * kLog2e < INFINITY)) return PG_ERR_ARG;
   if (logits == nullptr || tokens == nullptr || logprob == nullptr || entropy == nullptr || rank == nullptr || (top > 0 && (top_ids == nullptr || top_logprob == nullptr))) return PG_ERR_ARG;
   if (V > 0x7fffff00 / 2 || (reinterpret_cast<uintptr_t>(logits) & 3) != 0) return PG_ERR_ARG;
   // CTAs that share a row: as many as fit the GPU at two an SM, no share below a tile's half
