@@ -63,7 +63,7 @@ struct Args {
   float* partial;
   const int *row0, *n, *ctx, *pt, *pos;
   const uint32_t* tree;
-  int words, max_pages, page, tile_shift, singles, nsplit, cluster, blocks, H, G, dim, vdim, wr, mode;  // tile_shift: log2 of a page's tiles
+  int words, max_pages, page, max_n, tile_shift, singles, nsplit, cluster, blocks, H, G, dim, vdim, wr, mode;  // tile_shift: log2 of a page's tiles
   float scale, softcap;
   int gate_per_head, vec_q, vec_gate, vec_out;  // vec_*: four elements in one piece
   PgAttnScore sx;
@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
   const int split = blockIdx.x, g = blockIdx.y / a.blocks, block = blockIdx.y % a.blocks, e = blockIdx.z;
   const int n = a.n[e], ctx = a.ctx[e], gsz = a.H / a.G, len = ctx + n;
   const long long t0 = a.row0[e];
-  const int wr = R8 ? 1 : a.wr, wk = kWarps / wr, rows_cta = wr * 16 * MT, r0 = block * rows_cta, R = n * gsz;
+  const int wr = R8 ? 1 : a.wr, wk = kWarps / wr, rows_cta = wr * 16 * MT, r0 = block * rows_cta, R = min(n, a.max_n) * gsz;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nn = lane >> 2, c = lane & 3;
   const int rg = warp % wr, kgrp = warp / wr;
   const bool mine = !(a.singles && n != 1) && r0 < R;
@@ -1125,7 +1125,7 @@ int attn_rows(const PgAttnRows* q, long long* need, void* scratch, long long scr
   a.ke = static_cast<const uint8_t*>(p.k_powers), a.ve = static_cast<const uint8_t*>(p.v_powers);
   a.gate = p.gate, a.ldg = p.ldg, a.out = p.out, a.partial = static_cast<float*>(scratch);
   a.row0 = p.entry_row0, a.n = p.entry_n, a.ctx = p.entry_ctx, a.pt = p.page_table, a.pos = p.pos, a.tree = static_cast<const uint32_t*>(p.tree);
-  a.words = p.tree_words, a.max_pages = p.max_pages, a.page = p.page, a.singles = p.singles, a.H = p.H, a.G = p.G, a.dim = p.dim, a.vdim = p.vdim;
+  a.words = p.tree_words, a.max_pages = p.max_pages, a.page = p.page, a.max_n = p.max_n, a.singles = p.singles, a.H = p.H, a.G = p.G, a.dim = p.dim, a.vdim = p.vdim;
   a.scale = p.scale, a.softcap = p.softcap, a.gate_per_head = p.gate_per_head;
   a.sx = sx != nullptr ? *sx : PgAttnScore{};
   a.mode = a.sx.dist_a != nullptr || a.sx.logistic ? kGeneral : p.softcap > 0.f ? kCapped : kPlain;
