@@ -237,7 +237,7 @@ __device__ __forceinline__ void put(const Args& a, const Row& r, int col, float4
 
 // The sum of the values that are no numbers, among the keys with a mask that this CTA walks and the row sees.
 template <typename TC>
-__device__ __noinline__ float4 no_number_values(const Args& a, int e, int g, const Row r, int col, int split, int wk, int keys) {
+__device__ __noinline__ float4 no_number_values(const Args& a, int e, int g, const Row r, int col, int split, int wk, int keys, int newest) {
   const int n = a.n[e], ctx = a.ctx[e], len = ctx + n, window = a.sx.window > 0 ? a.sx.window : 0, keep = window ? max(a.sx.keep_first, 0) : 0;
   const long long t0 = a.row0[e];
   const int i = static_cast<int>(r.t - t0), mine = a.pos != nullptr ? a.pos[r.t] : ctx + i;
@@ -246,7 +246,7 @@ __device__ __noinline__ float4 no_number_values(const Args& a, int e, int g, con
   for (int walk = 0; walk < nkeep + ntiles - t_lo; ++walk) {
     if (walk / wk % a.nsplit != split) continue;
     const int j0 = (walk < nkeep ? walk : t_lo + walk - nkeep) * keys;
-    if (j0 + keys <= ctx && (window == 0 || j0 > len - 1 - window || j0 + keys <= keep)) continue;  // without a mask: in the sums
+    if (j0 + keys <= ctx && (window == 0 || j0 > newest - window || j0 + keys <= keep)) continue;  // without a mask: in the sums
     for (int j = j0; j < min(j0 + keys, len); ++j) {
       const int m = j - ctx, pj = m < 0 ? j : a.pos != nullptr ? a.pos[t0 + m] : j;
       const bool seen = m < 0 || (a.tree == nullptr ? m <= i : m / 32 < a.words && (a.tree[r.t * a.words + m / 32] >> (m % 32) & 1u));
@@ -291,7 +291,8 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
   __shared__ int2 where_to[kWarps * 16 * MT];  // a row's token of the entry and its head; past the last row: the last one's
   __shared__ float share[8][kWarps * 16 * MT];
   __shared__ int any_bad;
-  if (threadIdx.x == 0) any_bad = 0;
+  __shared__ int last_pos;  // windows: the farthest position of the CTA's rows
+  if (threadIdx.x == 0) any_bad = 0, last_pos = 0;
   // (the step's descriptors, too, may come from the kernel in front)
   if (a.nsplit > 1 && !a.cluster) pg::griddep_begin<true>();  // (fp32 partials, read behind a wait)
   else pg::griddep_begin_if(a.trigger);
@@ -368,6 +369,8 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
     where_to[r] = make_int2(i, g * gsz + rr - i * gsz);
   }
   __syncthreads();
+  if (window)
+    for (int r = tid; r < min(rows_cta, R - r0); r += 32 * kWarps) atomicMax(&last_pos, a.pos[t0 + where_to[r].x]);
   uint4* qs = reinterpret_cast<uint4*>(raw);  // [term][row tile][step][lane]
   const int tiles_m = wr * MT;
   constexpr int QL = DC == 1 ? 16 : 32;       // lanes of a row
@@ -464,7 +467,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
     pg::cp_async_commit();
     const int it = tile_of(walk), j0 = it * KT;
     const unsigned char* stage = ring + (k % K::STAGES) * K::STAGE;
-    const bool plain = j0 + KT <= ctx && (window == 0 || j0 > len - 1 - window || j0 + KT <= keep);  // every row sees every key of the tile
+    const bool plain = j0 + KT <= ctx && (window == 0 || j0 > last_pos - window || j0 + KT <= keep);  // every row sees every key of the tile
     // ---- who sees what
     uint32_t vis[2 * MT];
     if (!plain) {
@@ -863,7 +866,7 @@ __global__ void __launch_bounds__(32 * kWarps, (ctas_per_sm<TQ, TC, DC, VC, MT>(
   if (any_bad) {  // values that are no numbers, into the first warp's sums
     for (int r = row_of < per_pass ? row_of : rows_here; r < rows_here; r += per_pass) {
       const int tile = r / (16 * MT), in = r % (16 * MT);
-      const float4 v = no_number_values<TC>(a, e, g, row_at(r), col, split, wk, KT);
+      const float4 v = no_number_values<TC>(a, e, g, row_at(r), col, split, wk, KT, last_pos);
       add(*reinterpret_cast<float4*>(os + (tile * 16 * MT + in) * ldo_s + col), 1.f, v);
     }
     __syncthreads();
