@@ -259,8 +259,8 @@ class SequenceEngine:
             raise ValueError(f"top is 0 .. 32 and at most the vocabulary: got {top}")
         prompts = [self._checked(("score", i), pr) for i, pr in enumerate(prompts)]
         scored = []
-        for i, pr in enumerate(prompts):
-            rid, got = ("score", i), []
+        for pr in prompts:
+            rid, got = object(), []  # (a name that no live request has)
             try:
                 for lo in range(0, len(pr) - 1, step_tokens):
                     part = pr[lo:min(lo + step_tokens, len(pr) - 1)]  # (nothing follows the last token)
