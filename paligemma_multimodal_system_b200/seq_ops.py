@@ -609,10 +609,17 @@ def attn_ragged(q, k_pages, v_pages, gate, out, b: StepBatch, H, G, dim, vdim, s
 def _attn_rows(q, k_pages, v_pages, gate, out, b: StepBatch, H, G, dim, vdim, scale, softcap, page, gate_per_head, score, singles):
     if dim > 128 or vdim > 128:
         raise ValueError(f"attention of a few rows takes heads of up to 128 elements: got {dim} and {vdim}")
-    if q.dtype not in (torch.bfloat16, torch.float32) or out.dtype != q.dtype or (gate is not None and (gate.dtype != q.dtype or gate.stride(1) != 1)):
+    if q.dtype not in (torch.bfloat16, torch.float32) or out.dtype != q.dtype or (gate is not None and (gate.dtype != q.dtype or gate.stride(-1) != 1)):
         raise ValueError("queries, gate and output share a type, torch.bfloat16 or torch.float32")
     if q.numel() != b.T * H * dim or not q.is_contiguous() or out.stride(-1) != 1 or H % G:
         raise ValueError("queries are [rows, heads * size], heads a multiple of the key / value heads")
+    wide = H * vdim
+    pitch = score.out_ld if score is not None and score.out_ld else wide
+    if not (out.is_contiguous() and out.numel() == b.T * wide and pitch == wide) and (
+            out.dim() != 2 or out.shape[0] != b.T or out.shape[1] < wide or (b.T > 1 and out.stride(0) != pitch)):
+        raise ValueError(f"the output's rows are {wide} elements, {pitch} apart: got {tuple(out.shape)} with strides {out.stride()}")
+    if gate is not None and (gate.dim() != 2 or gate.shape[0] < b.T or gate.shape[1] < (H if gate_per_head else wide)):
+        raise ValueError(f"the gate has one number for every {'head' if gate_per_head else 'output'} of every row: got {tuple(gate.shape)}")
     import ctypes as C
     _on_current_device(q)
     quantized = isinstance(k_pages, QuantizedPages)
