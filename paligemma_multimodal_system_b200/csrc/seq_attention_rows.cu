@@ -26,10 +26,10 @@
 // The matrix instruction cuts off what it adds to a larger sum; over many it adds up (fp32, 4700 keys: 1.0e-5 off).  For fp32 queries the small terms' products and every tile's
 // outputs have sums of their own, added with a rounding (1.2e-6, as fp32 operators have); for bf16 ones it is a hundredth of the output's rounding.
 //
-// What bounds it: while a k/v head has few rows, the bytes of keys and values where walks are long (6 x 32000 keys of 4 x 128 over codes 41 us, 4.7 TB/s), the unequal lengths of a
-// batch (64 x 1125 .. 2250 of 8 x 64 with soft cap and gate 38 us: the loop runs at the memory's rate, then short entries leave SMs empty), else a chain of trips
+// What bounds it: while a k/v head has few rows, the bytes of keys and values where walks are long (6 x 32000 keys of 4 x 128 over codes 45 us, 4.4 TB/s), the unequal lengths of a
+// batch (64 x 1125 .. 2250 of 8 x 64 with soft cap and gate 39 us: the loop runs at the memory's rate, then short entries leave SMs empty), else a chain of trips
 // (descriptors, pages, tiles, join: one x 3000 10 us).  Large trees: instructions -- conversions, exponentials and a tensor rate of 550 TFLOP/s (one m16n8k16 in 2.1 clocks an SM) --
-// at ten warps an SM (24 trees of 31 x 4 rows over codes 78 us).
+// at ten warps an SM (24 trees of 31 x 4 rows over codes 90 us).
 // The loop body is one straight line but for masks, options and new maxima: branches between the row halves cost a quarter (98 -> 84 us); a second body for masked tiles cost
 // as much in instruction fetch as it saved.
 #include <cuda_fp16.h>
@@ -1101,8 +1101,8 @@ template <typename TQ, typename TC, int KT>
 int by_rows(const PgAttnRows& p, const Args& a, long long* need, long long scratch_bytes, cudaStream_t st) {
   const int rows = (p.singles ? 1 : p.max_n) * (p.H / p.G);
   if (rows <= 8) return by_size<TQ, TC, 1, KT, true>(p, a, need, scratch_bytes, st);
-  // 32 rows a warp read and convert a tile once where there are CTAs enough (24 trees of 8 x 4 rows over codes, 16 / 32 rows a warp 39 / 30 us; 16 x 4 rows 62 / 47); else, and where
-  // nothing is converted, 16 for a shorter chain (one tree of 8 x 4 rows 14 / 20; 24 over bf16 pages 41 / 48)
+  // 32 rows a warp read and convert a tile once where there are CTAs enough (24 trees of 8 x 4 rows over codes, 16 / 32 rows a warp 40 / 34 us; 16 x 4 rows 67 / 53); else, and where
+  // nothing is converted, 16 for a shorter chain (one tree of 8 x 4 rows 14 / 18; 24 over bf16 pages 41 / 46)
   if (rows <= 16 || sizeof(TQ) == 4 || (sizeof(TC) == 2 && rows <= 32) || (long long)p.busy * p.G * 2 < pg::num_sms()) return by_size<TQ, TC, 1, KT, false>(p, a, need, scratch_bytes, st);
   return by_size<TQ, TC, sizeof(TQ) == 4 ? 1 : 2, KT, false>(p, a, need, scratch_bytes, st);
 }

@@ -512,7 +512,7 @@ extern "C" int pg_token_logprobs(const float* logits, long long ld, const int* t
   if (rows <= 0 || V <= 0 || top < 0 || top > kTop || top > V || ld < V || !(temperature > 0.f) || !(temperature < INFINITY) || !(1.0f / temperature * kLog2e < INFINITY)) return PG_ERR_ARG;
   if (logits == nullptr || tokens == nullptr || logprob == nullptr || entropy == nullptr || rank == nullptr || (top > 0 && (top_ids == nullptr || top_logprob == nullptr))) return PG_ERR_ARG;
   if (V > 0x7fffff00 / 2 || (reinterpret_cast<uintptr_t>(logits) & 3) != 0) return PG_ERR_ARG;
-  // CTAs that share a row: as many as fit the GPU at two an SM, no share below a tile's half
+  // CTAs that share a row: as many as fit the GPU at three an SM, no share below a tile's half
   int split = 1;
   while (split < 8 && (long long)rows * split * 2 <= (long long)kPerSm * pg::num_sms() && V / (split * 2) >= kThreads * kVecs * 4 / 2) split *= 2;
   auto kern = top > 0 ? token_logprobs_kernel<true> : token_logprobs_kernel<false>;
@@ -526,7 +526,7 @@ extern "C" int pg_token_logprobs(const float* logits, long long ld, const int* t
     }
     done = true;
   }
-  // (clusters share rows only while all of them are there at once; else two CTAs an SM walk the rows)
+  // (clusters share rows only while all of them are there at once; else three CTAs an SM walk the rows)
   const int sms = pg::num_sms();
   const long long grid = split > 1 ? (long long)rows * split : rows < kPerSm * sms ? rows : kPerSm * sms;
   cudaLaunchConfig_t cfg = {};
