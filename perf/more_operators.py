@@ -317,7 +317,7 @@ def run(state):
         return {"verify": _verify, "fork": _fork, "keep": _keep, "adapt": _adapt}[kind](s)
     from paligemma_multimodal_system_b200 import seq_ops
     if kind == "verify":
-        return list(seq_ops.verify_drafts(s["logits"], seq_ops.StepBatch(**s["plan"]), s["uniforms"], draft_logits=s["draft"], temperature=s["temperature"], top_p=s["top_p"]))
+        return list(seq_ops.verify_drafts(s["logits"], seq_ops.RequestBatch(**s["plan"]), s["uniforms"], draft_logits=s["draft"], temperature=s["temperature"], top_p=s["top_p"]))
     if kind == "fork":
         seq_ops.copy_pages(s["cache"], s["moves"])
         return s["pool"]
