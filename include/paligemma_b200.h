@@ -806,6 +806,57 @@ int pg_moe_combine_norm_add(const float* expert_out, long long ldy, const int* p
 int pg_token_logprobs(const float* logits, long long ld, const int* tokens, float* logprob, float* entropy, int* rank, int* top_ids, float* top_logprob,
                       int rows, int V, int top, float temperature, void* stream);
 
+/* Rows of paged caches from one place to another, every operand of a cache in one launch.  An operand is `pages` pages of `page` rows: rows of row_bytes bytes one
+ * after another (heads 0; unit: 16, 4, 2 or 1, the widest piece that its base and rows are multiples of), or a byte per row and head, [pages, heads, page] (heads > 0).
+ * operands: a table on the device.
+ * pg_copy_pages: for each of `moves` triples (source page, destination page, rows; host memory, read before the call returns) the first rows of the source; no
+ *   destination is another triple's source or destination.  most_page_bytes: the largest page_bytes.
+ * pg_keep_rows: cache row ctx + i of entry e <- row ctx + path[e, i], i < kept[e], for ascending paths with path[e, i] >= i (others within 0 .. n - 1 leave rows of
+ *   that entry undefined; what lies outside is skipped).  most_columns: the largest number of units (heads) in a row. */
+typedef struct {
+  void* base;
+  long long page_bytes;
+  int row_bytes, heads, unit, pages;
+} PgPageOperand;
+int pg_copy_pages(const PgPageOperand* operands, int count, int page, long long most_page_bytes, const int* moves_host, int moves, void* stream);
+int pg_keep_rows(const PgPageOperand* operands, int count, int page, int most_columns, const int* page_table, int max_pages, const int* entry_n, const int* entry_ctx,
+                 const int* path, int path_ld, const int* kept, int entries, void* stream);
+
+/* Drafted trees against the target's distributions, from given random numbers.  Entry e owns rows row0[e] .. + n[e] of everything; row 0 of an entry is its pending
+ * token, which stays; parents[row] is an earlier row of the entry (others, and rows below -1, are never reached).  A row's distribution: softmax(x / temperature)
+ * cut to the entries above which a mass of top_p at most lies, and renormalised.  A row decides by itself:
+ *   uniforms NULL: t = the first largest entry; the walk goes on at the first child that carries t and else ends with t
+ *   draft NULL: t drawn from the row with uniforms[row, 1], the first id whose running sum is above u times the whole; then as above
+ *   draft (row v: the distribution q that v's children were drawn from): c = 0, S = 1; children in order: x stays if uniforms[child, 0] q(x) S < max(p(x) - c q(x), 0),
+ *     else c += S, S = sum max(p - c q, 0).  Where none stays the walk ends with a draw from max(p - c q, 0), from p where that is nothing
+ * path[e, 0 .. kept[e]) = the rows of the walk (-1 behind), next[e] = the token behind it.  A row without a distribution (a NaN, a +inf, nothing but -inf; of the
+ * draft's only those with children count) ends the walk with -1.  outcome: rows + 1 words of scratch. */
+typedef struct {
+  const float *logits, *draft, *uniforms;
+  const int *tokens, *parents, *row0, *n;
+  int *path, *kept, *next, *outcome;
+  long long ld, draft_ld, path_ld;
+  double temperature, top_p, draft_temperature, draft_top_p;
+  int entries, rows, max_n, V;
+} PgVerify;
+int pg_verify_drafts(const PgVerify* a, void* stream);
+
+/* Low-rank adapters of a step's rows beside a shared projection: out[t, f] = y[t, f] + gain * scale[s] * sum_r b[s][f, r] (sum_k a[s][part(f) * rank + r, k] x[t, k])
+ * for rows of adapter s.  The columns are `parts` runs of part_cols; each has rank rows of a for itself.  a: [slots, parts * rank, K8], b: [slots, F, rank], dense, in x's
+ * type, rank a multiple of 8 up to 128, K8 = K rounded up to 8 (zeros behind K).  rows / tiles: the plan, tiles of up to tile_rows (16 or 64) rows
+ * (adapter, first, count) of one adapter, rows[first ..] their numbers; adapter -1: rows without one, which are copied where out is not y. */
+typedef struct {
+  const void *x, *y, *a, *b;
+  void* out;
+  const float* scale;
+  const int *rows, *tiles;
+  long long ldx, ldy, ldo;
+  int part_cols[8];
+  int parts, K, F, rank, slots, tile_count, tile_rows, T, in_f32, out_f32;
+  float gain;
+} PgAdapter;
+int pg_adapter_add(const PgAdapter* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

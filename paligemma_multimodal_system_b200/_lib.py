@@ -14,7 +14,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("PG_LIB_PATH") or os.path.join(_HERE, "libpaligemma_b200.so")  # PG_LIB_PATH: A/B builds (profiling)
 
 EPI_BF16, EPI_F32, EPI_ATOMIC_F32, EPI_GEGLU = 0, 1, 2, 3
-ABI_VERSION = 8  # pg_abi_version() of the library these signatures describe
+ABI_VERSION = 9  # pg_abi_version() of the library these signatures describe
 
 _ERRORS = {-1: "PG_ERR_ARG", -2: "PG_ERR_CUDA", -3: "PG_ERR_DRIVER", -4: "PG_ERR_TMAP", -5: "PG_ERR_ARCH"}
 
@@ -92,6 +92,10 @@ SIGNATURES = {
     "pg_kv_read_e4m3": [p, p],
     "pg_attn_rows_scratch": [p],
     "pg_attn_rows": [p, p, i64, p],
+    "pg_copy_pages": [p, i32, i32, i64, p, i32, p],
+    "pg_keep_rows": [p, i32, i32, i32, p, i32, p, p, p, i32, p, i32, p],
+    "pg_verify_drafts": [p, p],
+    "pg_adapter_add": [p, p],
     "pg_token_logprobs": [p, i64, p, p, p, p, p, p, i32, i32, i32, f32, p],
     "pg_attn_ragged": [p, p, p, p, i64, p, p, p, p, p, i32, i32, i32, i32, i32, i32, i32, i32, f32, f32, i32, i32, i64, i64, i32, p, p],
     "pg_attn_ragged_mma": [p, p, p, p, i64, p, p, p, p, p, i32, i32, i32, i32, i32, i32, i32, i32, f32, f32, i32, i32, p, p],
@@ -151,6 +155,9 @@ class AttnScore(C.Structure):
 ATTN_ROWS = struct.Struct("@6Pq8P16i2f")
 PREPARE_E4M3 = struct.Struct("@Pq13Pq12i3f4x")
 READ_E4M3 = struct.Struct("@10P8i")
+VERIFY = struct.Struct("@11P3q4d4i")
+ADAPTER = struct.Struct("@8P3q18if4x")
+PAGE_OPERAND = struct.Struct("@Pq4i")  # PgPageOperand
 
 
 class RoutedFf(C.Structure):

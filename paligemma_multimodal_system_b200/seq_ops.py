@@ -67,6 +67,17 @@ class StepBatch:
 
 
 TreeBatch = StepBatch  # (another name for a step that has these two)
+StepBatch.parents = StepBatch.adapters = None
+
+
+@dataclasses.dataclass
+class RequestBatch(StepBatch):
+    """A step whose requests have something of their own (`dataclasses.replace` keeps both)."""
+    parents: dataclasses.InitVar[Optional[torch.Tensor]] = None  # int32 [T], drafted trees: the row of its entry that a row follows, -1 the stored tokens
+    adapters: dataclasses.InitVar[Optional["StepAdapters"]] = None  # low-rank adapters of the entries
+
+    def __post_init__(self, at, tree, parents, adapters):
+        self.at, self.tree, self.parents, self.adapters = at, tree, parents, adapters
 
 
 def _single_rows(ns):
@@ -113,7 +124,7 @@ def make_step_batch(entries: Sequence[dict]) -> StepBatch:
         masks, depth = _tree_masks([e.get("parents") for e in entries], ns)
     words = 0 if masks is None else masks.shape[1]
     plain = 3 * T + 4 * E + E * max_pages + E + E * dmax
-    buf = np.zeros(plain + (0 if masks is None else T * (1 + words)), dtype=np.int32)
+    buf = np.zeros(plain + (0 if masks is None else T * (2 + words)), dtype=np.int32)
     tokens, pos, row_entry = buf[:T], buf[T:2 * T], buf[2 * T:3 * T]
     o = 3 * T
     row0, n, ctx, slot = buf[o:o + E], buf[o + E:o + 2 * E], buf[o + 2 * E:o + 3 * E], buf[o + 3 * E:o + 4 * E]
@@ -138,12 +149,13 @@ def make_step_batch(entries: Sequence[dict]) -> StepBatch:
         r += k
     if masks is not None:
         buf[plain:plain + T] = pos
-        buf[plain + T:] = masks.reshape(-1).view(np.int32)
+        buf[plain + T:plain + 2 * T] = np.concatenate([np.arange(-1, k - 1) if e.get("parents") is None else np.asarray(e["parents"]) for e, k in zip(entries, ns)])
+        buf[plain + 2 * T:] = masks.reshape(-1).view(np.int32)
         pos[:] = ctx[row_entry] + depth
     dev = torch.from_numpy(buf).pin_memory().to("cuda", non_blocking=True)
     o = 3 * T
-    drafted = {} if masks is None else dict(at=dev[plain:plain + T], tree=dev[plain + T:].view(T, words))
-    return StepBatch(T=T, E=E, max_n=max(ns), min_n=min(ns), tokens=dev[:T], pos=dev[T:2 * T], row_entry=dev[2 * T:3 * T], row0=dev[o:o + E],
+    drafted = {} if masks is None else dict(at=dev[plain:plain + T], parents=dev[plain + T:plain + 2 * T], tree=dev[plain + 2 * T:].view(T, words))
+    return (StepBatch if masks is None else RequestBatch)(T=T, E=E, max_n=max(ns), min_n=min(ns), tokens=dev[:T], pos=dev[T:2 * T], row_entry=dev[2 * T:3 * T], row0=dev[o:o + E],
                      n=dev[o + E:o + 2 * E], ctx=dev[o + 2 * E:o + 3 * E], slot=dev[o + 3 * E:o + 4 * E],
                      page_table=dev[o + 4 * E:o2].view(E, max_pages), max_pages=max_pages, singles=sum(k == 1 for k in ns),
                      max_single_ctx=max([e["ctx"] for e, k in zip(entries, ns) if k == 1], default=0), single_rows=_single_rows(ns),
@@ -651,6 +663,286 @@ def attn_tree(q, k_pages, v_pages, gate, out, b: StepBatch, H, G, dim, vdim, sca
     if b.tree is not None and (b.tree.dtype != torch.int32 or b.tree.dim() != 2 or b.tree.shape[0] != b.T or not b.tree.is_contiguous()):
         raise ValueError("masks are int32 [rows, words]")
     _attn_rows(q, k_pages, v_pages, gate, out, b, H, G, dim, vdim, scale, softcap, page, gate_per_head, score, singles=False)
+
+
+# ---- rows of the cache from one place to another -----------------------------------------------------------------------
+class CachePages:
+    """The paged operands of a cache, all layers together, as `copy_pages` and `keep_rows` take them: tensors [pages, page, width] of any type and QuantizedPages.
+    Made once for a cache: a table of where they lie is kept on the device."""
+
+    def __init__(self, operands: Sequence, page: int):
+        flat = []
+        for o in operands:
+            flat += [(o.codes, 0), (o.powers, o.heads)] if isinstance(o, QuantizedPages) else [(o, 0)]
+        if not flat:
+            raise ValueError("a cache has at least one operand")
+        if len(flat) > 65535:
+            raise ValueError(f"at most 65535 operands: got {len(flat)}")
+        self.operands, self.page, self.pages, self.device = list(operands), int(page), flat[0][0].shape[0], flat[0][0].device
+        table, self.most_page_bytes, self.most_columns = b"", 0, 0
+        for t, heads in flat:
+            if t.dim() != 3 or not t.is_contiguous() or t.shape[0] != self.pages or t.shape[2 if heads else 1] != page or t.numel() == 0:
+                raise ValueError(f"operands are dense [pages, {page}, width] of {self.pages} pages: got {tuple(t.shape)}")
+            if not t.is_cuda or t.device != self.device:
+                raise ValueError("the operands of a cache lie on one device")
+            row = t.shape[2] * t.element_size()
+            unit = next(u for u in (16, 4, 2, 1) if (row | t.data_ptr()) % u == 0)
+            if row * page >= 1 << 31:
+                raise ValueError("a page has less than 2 GB")
+            self.most_page_bytes = max(self.most_page_bytes, t.stride(0) * t.element_size())
+            self.most_columns = max(self.most_columns, heads or row // unit)
+            table += _lib.PAGE_OPERAND.pack(t.data_ptr(), t.stride(0) * t.element_size(), row, heads, unit, self.pages)
+        self.count = len(flat)
+        self.table = torch.frombuffer(bytearray(table), dtype=torch.uint8).to(self.device)
+
+    def __reduce__(self):  # (a copy's table says where the copies lie)
+        return type(self), (self.operands, self.page)
+
+
+def copy_pages(cache: CachePages, moves):
+    """moves: whole numbers [n, 3] on the host, (source page, destination page, rows): the first `rows` rows of the source page go to the destination page, in every
+    operand.  No destination is another move's source or destination."""
+    moves = np.asarray(moves)
+    if moves.size == 0:
+        return
+    if moves.ndim != 2 or moves.shape[1] != 3 or moves.dtype.kind not in "iu":
+        raise ValueError("moves are (source page, destination page, rows)")
+    if moves.min() < 0 or moves[:, :2].max() >= cache.pages or moves[:, 2].max() > cache.page:
+        raise IndexError(f"moves go between pages 0 .. {cache.pages - 1} and take up to {cache.page} rows")
+    if np.unique(moves[:, 1]).size != len(moves) or np.isin(moves[:, 1], moves[:, 0]).any():
+        raise ValueError("a page that is copied to is no other move's source or destination")
+    _on_current_device(cache.table)
+    moves = np.ascontiguousarray(moves, dtype=np.int32)
+    _lib.check(_lib.lib().pg_copy_pages(cache.table.data_ptr(), cache.count, cache.page, cache.most_page_bytes, moves.ctypes.data, len(moves), _lib.stream()), "pg_copy_pages")
+
+
+def keep_rows(cache: CachePages, b: StepBatch, path: torch.Tensor, kept: torch.Tensor):
+    """The drafted rows path[e, :kept[e]] of every entry (int32 [entries, width] and [entries] on the device, `verify_drafts`' outputs) move together behind the entry's stored
+    rows, in every operand: cache row ctx + i takes row ctx + path[e, i].  Paths ascend (a token stands behind the one it follows); numbers outside the entry's rows are
+    skipped."""
+    if path.dtype != torch.int32 or path.dim() != 2 or path.shape[0] != b.E or not path.is_contiguous() or path.shape[1] < 1:
+        raise ValueError("paths are int32 [entries, width]")
+    if kept.dtype != torch.int32 or kept.shape != (b.E,) or not kept.is_contiguous():
+        raise ValueError("kept is int32 [entries]")
+    if path.device != cache.device or kept.device != cache.device or b.page_table.device != cache.device:
+        raise ValueError(f"paths, counts and page table lie on the cache's device, {cache.device}")
+    _on_current_device(cache.table)
+    _lib.check(_lib.lib().pg_keep_rows(cache.table.data_ptr(), cache.count, cache.page, cache.most_columns, b.page_table.data_ptr(), b.max_pages, b.n.data_ptr(), b.ctx.data_ptr(),
+                                       path.data_ptr(), path.shape[1], kept.data_ptr(), b.E, _lib.stream()), "pg_keep_rows")
+
+
+# ---- low-rank adapters of the step's requests -----------------------------------------------------------------------
+ADAPTER_MOST_RANK, ADAPTER_MOST_PARTS = 128, 8
+
+
+class AdapterBank:
+    """The low-rank adapters that stand beside one shared projection [columns, K]: adapter s adds scale[s] * b[s] (a[s] x).  The projection's columns are `parts` runs
+    (a joint query, key and value projection has three); each run has `rank` rows of a[s] for itself: a [slots, len(parts) * rank, K], b [slots, sum(parts), rank], both
+    bf16 or fp32 on the device, scale fp32 [slots].  They are laid out anew, once; `put` replaces one."""
+
+    def __init__(self, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor, parts: Sequence[int]):
+        parts = [int(n) for n in parts]
+        if not 1 <= len(parts) <= ADAPTER_MOST_PARTS or min(parts) < 1:
+            raise ValueError(f"1 .. {ADAPTER_MOST_PARTS} runs of at least one column: got {parts}")
+        if a.dim() != 3 or b.dim() != 3 or a.dtype != b.dtype or a.dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError("a is [slots, parts * rank, K] and b [slots, columns, rank], both torch.bfloat16 or torch.float32")
+        slots, rows, K = a.shape
+        rank = b.shape[2]
+        if slots < 1 or K < 1 or b.shape[0] != slots or b.shape[1] != sum(parts) or rows != len(parts) * rank or not 1 <= rank <= ADAPTER_MOST_RANK:
+            raise ValueError(f"a {tuple(a.shape)} and b {tuple(b.shape)} for runs of {parts} columns and a rank of 1 .. {ADAPTER_MOST_RANK}")
+        if scale.dtype != torch.float32 or scale.shape != (slots,):
+            raise ValueError("one fp32 factor for every adapter")
+        if not a.is_cuda or b.device != a.device or scale.device != a.device:
+            raise ValueError("adapters lie on one device")
+        self.parts, self.slots, self.rank, self.K, self.F, self.dtype, self.device = tuple(parts), slots, rank, K, sum(parts), a.dtype, a.device
+        r8, K8 = -(-rank // 8) * 8, -(-K // 8) * 8  # (ranks and depths in whole 16-byte pieces; zeros behind)
+        self.rank8 = r8
+        self.a, self.b, self.scale = a.new_zeros(slots, len(parts) * r8, K8), b.new_zeros(slots, self.F, r8), scale.clone()
+        self.a.view(slots, len(parts), r8, K8)[:, :, :rank, :K] = a.view(slots, len(parts), rank, K) if a.is_contiguous() else a.reshape(slots, len(parts), rank, K)
+        self.b[:, :, :rank] = b
+
+    @classmethod
+    def empty(cls, slots: int, rank: int, K: int, parts: Sequence[int], dtype: torch.dtype, device="cuda"):
+        return cls(torch.zeros(slots, len(parts) * rank, K, device=device, dtype=dtype), torch.zeros(slots, sum(parts), rank, device=device, dtype=dtype),
+                   torch.zeros(slots, device=device), parts)
+
+    def put(self, slot: int, part: int, a: torch.Tensor, b: torch.Tensor):
+        """One run's matrices of one adapter: a [r, K], b [columns of the run, r], r up to the bank's rank (the rest becomes zero)."""
+        r = a.shape[0]
+        if not 0 <= slot < self.slots or not 0 <= part < len(self.parts):
+            raise IndexError(f"adapter {slot}, run {part} of {self.slots} adapters with {len(self.parts)} runs")
+        if a.dim() != 2 or b.dim() != 2 or r > self.rank or a.shape[1] != self.K or tuple(b.shape) != (self.parts[part], r):
+            raise ValueError(f"a {tuple(a.shape)} and b {tuple(b.shape)} for {self.parts[part]} columns of a depth of {self.K} and a rank up to {self.rank}")
+        col = sum(self.parts[:part])
+        here = self.a[slot, part * self.rank8:(part + 1) * self.rank8]
+        here.zero_()
+        here[:r, :self.K] = a.to(self.device, self.dtype)
+        there = self.b[slot, col:col + self.parts[part]]
+        there.zero_()
+        there[:, :r] = b.to(self.device, self.dtype)
+
+    def clear(self, slot: int):
+        self.a[slot].zero_()
+        self.b[slot].zero_()
+        self.scale[slot] = 0
+
+
+class AdapterPlan:
+    """Which rows of a step go through which adapter: entries of ns[e] rows, one behind the other, with adapters[e] (-1: none).  Rows of one adapter stand together in
+    tiles, whichever entries they belong to.  tiles: a fixed number of them (a plan that is `fill`ed again, for a step that is captured)."""
+
+    def __init__(self, ns: Sequence[int], adapters: Sequence[int], device="cuda", tiles: Optional[int] = None):
+        self.T, self.fixed, self._copied, self.host = 0, tiles, None, None
+        self._make(ns, adapters, device)
+
+    def _order(self, ns, adapters):
+        ns, who = np.asarray(ns, dtype=np.int64), np.asarray(adapters, dtype=np.int64)
+        if ns.ndim != 1 or ns.shape != who.shape or ns.size == 0 or ns.min() < 1:
+            raise ValueError("one adapter (-1: none) for every entry, and entries of at least one row")
+        if who.min() < -1:
+            raise IndexError("adapters are 0 .. slots - 1, -1 for none")
+        rows = np.repeat(who, ns)
+        order = np.argsort(rows, kind="stable")
+        ids, first, count = np.unique(rows[order], return_index=True, return_counts=True)
+        return order, ids, first, count
+
+    def _make(self, ns, adapters, device):
+        order, ids, first, count = self._order(ns, adapters)
+        # rows of an adapter on average: tiles of 64 read it once for four of 16, tiles of 16 are four times the CTAs (decoded tokens)
+        size = 64 if self.fixed is None and len(order) >= 32 * len(ids) else 16
+        tiles = [(a, f + o, min(size, c - o)) for a, f, c in zip(ids.tolist(), first.tolist(), count.tolist()) for o in range(0, c, size)]
+        n = len(tiles) if self.fixed is None else self.fixed
+        if len(tiles) > n:
+            raise ValueError(f"{len(tiles)} tiles, room for {n}")
+        T = len(order)
+        if self.host is None:
+            self.T, self.tile_rows, self.tile_count = T, size, n
+            self.host = torch.zeros(T + 3 * n, dtype=torch.int32)
+            if torch.device(device).type == "cuda":
+                self.host = self.host.pin_memory()
+            self.dev = torch.empty_like(self.host, device=device)
+            self.rows, self.tiles = self.dev[:T], self.dev[T:]
+        elif T != self.T:
+            raise ValueError(f"a plan of {self.T} rows is filled with {T}")
+        h = self.host.numpy()
+        h[:T] = order
+        h[T:] = 0
+        h[T:T + 3 * len(tiles)] = np.asarray(tiles).reshape(-1)
+        self.most, self.used = int(ids[-1]), sum(int(a) >= 0 for a in ids)
+        self.dev.copy_(self.host, non_blocking=True)
+
+    def fill(self, ns: Sequence[int], adapters: Sequence[int]):
+        """Other adapters for as many rows, at the same addresses."""
+        if self.fixed is None:
+            raise ValueError("only a plan with a fixed number of tiles is filled again")
+        if self._copied is not None:
+            self._copied.synchronize()  # the image before must have left the pinned buffer
+        self._make(ns, adapters, self.dev.device)
+        self._copied = torch.cuda.Event()
+        self._copied.record()
+
+
+def _rows_overlap(s, s_pitch, t, t_pitch):
+    """Whether two row matrices have bytes in common; column slices that stand side by side in one matrix have none."""
+    def span(m, pitch):
+        return m.data_ptr(), ((m.shape[0] - 1) * pitch + m.shape[1]) * m.element_size(), pitch * m.element_size(), m.shape[1] * m.element_size()
+
+    (a, a_len, a_pitch, a_row), (b, b_len, b_pitch, b_row) = span(s, s_pitch), span(t, t_pitch)
+    if a + a_len <= b or b + b_len <= a:
+        return False
+    d = (b - a) % a_pitch
+    return a_pitch != b_pitch or d < a_row or a_pitch - d < b_row
+
+
+def adapter_add(x: torch.Tensor, y: torch.Tensor, bank: AdapterBank, plan: AdapterPlan, out: Optional[torch.Tensor] = None, gain: float = 1.0):
+    """out[t] = y[t] + gain * scale[s] * b[s] (a[s] x[t]) for the rows of adapter s, y[t] for those without (out None: y, in place).  x [rows, K] of the bank's type, y and
+    out [rows, columns] bf16 or fp32 (fp32 beside fp32 adapters), unit last strides, any row pitch.  The sum over K and over the rank is fp32; y is added to it and rounded once.  A row of x that is not
+    finite makes its own row of out NaN."""
+    out = y if out is None else out
+    T, K = x.shape if x.dim() == 2 else (0, 0)
+    if x.dtype != bank.dtype or K != bank.K or T != plan.T:
+        raise ValueError(f"x is [{plan.T}, {bank.K}] of {bank.dtype}: got {tuple(x.shape)} of {x.dtype}")
+    if y.dtype not in (torch.bfloat16, torch.float32) or out.dtype != y.dtype or (bank.dtype == torch.float32 and y.dtype != torch.float32):
+        raise ValueError("y and out share a type, torch.bfloat16 or torch.float32; torch.float32 beside fp32 adapters")
+    if tuple(y.shape) != (T, bank.F) or tuple(out.shape) != (T, bank.F):
+        raise ValueError(f"y and out are [{T}, {bank.F}]: got {tuple(y.shape)} and {tuple(out.shape)}")
+    pitches = []
+    for t, n in ((x, K), (y, bank.F), (out, bank.F)):
+        pitch = n if T == 1 else t.stride(0)
+        if (t.stride(1) != 1 and n > 1) or pitch < n:
+            raise ValueError("elements of a row stand side by side, rows do not overlap")
+        if t.device != bank.device:
+            raise ValueError(f"rows and adapters lie on one device: got {t.device} and {bank.device}")
+        pitches.append(pitch)
+    same = out.data_ptr() == y.data_ptr() and pitches[1] == pitches[2]
+    if _rows_overlap(out, pitches[2], x, pitches[0]) or (not same and _rows_overlap(out, pitches[2], y, pitches[1])):
+        raise ValueError("out is y or lies apart from it, and apart from x")
+    if plan.most >= bank.slots:
+        raise IndexError(f"adapter {plan.most} of {bank.slots}")
+    if plan.dev.device != bank.device:
+        raise ValueError(f"the plan lies on {plan.dev.device}, the adapters on {bank.device}")
+    _on_current_device(bank.a)
+    a = _lib.ADAPTER.pack(x.data_ptr(), y.data_ptr(), bank.a.data_ptr(), bank.b.data_ptr(), out.data_ptr(), bank.scale.data_ptr(), plan.rows.data_ptr(), plan.tiles.data_ptr(),
+                          *pitches, *bank.parts, *(0,) * (8 - len(bank.parts)), len(bank.parts), K, bank.F, bank.rank8, bank.slots, plan.tile_count, plan.tile_rows, T,
+                          bank.dtype == torch.float32, y.dtype == torch.float32, gain)
+    _lib.check(_lib.lib().pg_adapter_add(a, _lib.stream()), "pg_adapter_add")
+    return out
+
+
+# ---- verified drafts -------------------------------------------------------------------------------------------------
+VERIFY_MOST_VOCAB = 16 * 49152  # entries of a row that a cluster of CTAs holds at once
+
+
+def _check_rows_of_logits(logits, b: StepBatch, what):
+    if logits.dim() != 2 or logits.dtype != torch.float32 or logits.stride(1) != 1 or not logits.is_cuda or logits.shape[0] != b.T:
+        raise ValueError(f"{what} are fp32 [rows of the step, vocab] on the device, entries of a row side by side: got {tuple(logits.shape)} of {logits.dtype} for {b.T} rows")
+
+
+def verify_drafts(logits: torch.Tensor, b: StepBatch, uniforms: Optional[torch.Tensor] = None, draft_logits: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                  top_p: float = 1.0, draft_temperature: Optional[float] = None, draft_top_p: Optional[float] = None):
+    """Which tokens of every entry's drafted tree (b.tokens, b.parents) stay, and the token behind them: (path int32 [entries, max_n], kept int32 [entries], next int32 [entries]).
+    logits fp32 [rows, vocab] (any row pitch): row v of an entry says what follows token v.  The first row of an entry is its pending token, which stays: path[e, 0] = 0; rows below
+    -1 are never reached.  path[e, :kept[e]] are the rows of the walk, -1 behind them.
+
+    uniforms None: greedy -- the walk goes on at the first child that carries the row's first largest entry.  Else fp32 [rows, 2] from [0, 1), and a row's distribution is
+    softmax(logits / temperature) cut to the tokens above which at most top_p of the mass lies (equal logits stay together).  Without draft_logits a token is drawn from it
+    with uniforms[v, 1], the first id whose running sum is above that part of the whole, and the walk goes on at the first child that carries it.  draft_logits (as logits; row v:
+    what v's children were drawn from, one after another, with draft_temperature and draft_top_p, the target's where they are None): child i stays with probability
+    min(1, r / q) under uniforms[i, 0], r = p at first and the normalised max(r - q, 0) after each rejected one; where none stays the token is drawn from r.  Either way the
+    kept tokens and the next one are distributed as the target's own.  Rows without a distribution (a NaN, a +inf, nothing but -inf; the draft's where there are children) end
+    the walk with next -1."""
+    _check_rows_of_logits(logits, b, "logits")
+    V = logits.shape[1]
+    if not 0 < V <= VERIFY_MOST_VOCAB:
+        raise ValueError(f"rows of 1 .. {VERIFY_MOST_VOCAB} entries: got {V}")
+    if b.parents is None or b.parents.dtype != torch.int32 or b.parents.shape != (b.T,) or not b.parents.is_contiguous():
+        raise ValueError("the step's parents (RequestBatch) are int32 [rows]")
+    if uniforms is not None and (uniforms.dtype != torch.float32 or uniforms.shape != (b.T, 2) or not uniforms.is_contiguous()):
+        raise ValueError("random numbers are fp32 [rows, 2]")
+    if draft_logits is not None:
+        if uniforms is None:
+            raise ValueError("drafted distributions need random numbers: a greedy walk takes none")
+        _check_rows_of_logits(draft_logits, b, "draft_logits")
+        if draft_logits.shape != logits.shape:
+            raise ValueError(f"draft_logits are as wide as logits: got {tuple(draft_logits.shape)} and {tuple(logits.shape)}")
+    draft_temperature, draft_top_p = temperature if draft_temperature is None else draft_temperature, top_p if draft_top_p is None else draft_top_p
+    for t, p in ((temperature, top_p), (draft_temperature, draft_top_p)):
+        if not 1e-30 < float(t) < float("inf"):
+            raise ValueError("a temperature is above 1e-30 and finite")
+        if not 0.0 <= float(p) <= 1.0:
+            raise ValueError("top_p is 0 .. 1")
+    for t in (uniforms, draft_logits, b.parents, b.tokens):
+        if t is not None and t.device != logits.device:
+            raise ValueError(f"logits, random numbers and the step lie on one device: got {t.device} and {logits.device}")
+    _on_current_device(logits)
+    i32 = dict(dtype=torch.int32, device=logits.device)
+    path, ends, outcome = torch.empty(b.E, b.max_n, **i32), torch.empty(2, b.E, **i32), torch.empty(b.T + 1, **i32)
+    pitch = V if b.T == 1 else logits.stride(0)
+    dpitch = 0 if draft_logits is None else V if b.T == 1 else draft_logits.stride(0)
+    a = _lib.VERIFY.pack(logits.data_ptr(), _lib.ptr(draft_logits), _lib.ptr(uniforms), b.tokens.data_ptr(), b.parents.data_ptr(), b.row0.data_ptr(), b.n.data_ptr(), path.data_ptr(),
+                         ends.data_ptr(), ends.data_ptr() + 4 * b.E, outcome.data_ptr(), pitch, dpitch, b.max_n, temperature, top_p, draft_temperature, draft_top_p, b.E, b.T, b.max_n, V)
+    _lib.check(_lib.lib().pg_verify_drafts(a, _lib.stream()), "pg_verify_drafts")
+    return path, ends[0], ends[1]
 
 
 # ---- scored tokens ---------------------------------------------------------------------------------------------------

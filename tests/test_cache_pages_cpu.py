@@ -1,0 +1,65 @@
+"""Moves of cache pages that are refused before anything runs."""
+import copy
+
+import numpy as np
+import pytest
+import torch
+
+from paligemma_multimodal_system_b200 import seq_ops
+
+
+class _OnDevice(torch.Tensor):
+    is_cuda = True
+
+    def __deepcopy__(self, memo):
+        return self.clone().as_subclass(_OnDevice)
+
+
+def pages(*shape, dtype=torch.bfloat16):
+    return torch.zeros(*shape, dtype=dtype).as_subclass(_OnDevice)
+
+
+def cache(n=6):
+    return seq_ops.CachePages([pages(n, 64, 32), pages(n, 64, 16, dtype=torch.float32)], 64)
+
+
+@pytest.mark.parametrize("operands,page", [([], 64), ([torch.zeros(4, 64, 8)], 64), ([pages(4, 64, 8), pages(5, 64, 8)], 64), ([pages(4, 64, 8)], 32), ([pages(4, 64)], 64),
+                                           ([pages(4, 64, 8)[:, :, :4]], 64), ([pages(4, 64, 0)], 64)])
+def test_operands_that_are_no_cache(operands, page):
+    with pytest.raises(ValueError):
+        seq_ops.CachePages(operands, page)
+
+
+@pytest.mark.parametrize("moves,error", [([[0, 1]], ValueError), ([0, 1, 2], ValueError), ([[0.0, 1.0, 2.0]], ValueError), ([[0, 6, 3]], IndexError), ([[6, 0, 3]], IndexError),
+                                         ([[-1, 0, 3]], IndexError), ([[0, 1, 65]], IndexError), ([[0, 1, -1]], IndexError), ([[0, 1, 2], [3, 1, 2]], ValueError),
+                                         ([[0, 1, 2], [1, 2, 2]], ValueError), ([[2, 2, 4]], ValueError)])
+def test_moves_that_are_refused(moves, error):
+    with pytest.raises(error):
+        seq_ops.copy_pages(cache(), moves)
+
+
+def test_nothing_to_move_is_no_call():
+    seq_ops.copy_pages(cache(), [])
+    seq_ops.copy_pages(cache(), np.zeros((0, 3), np.int32))
+
+
+@pytest.mark.parametrize("path,kept", [(torch.zeros(2, 3), torch.zeros(2, dtype=torch.int32)), (torch.zeros(3, 3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)),
+                                       (torch.zeros(2, 0, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)), (torch.zeros(2, 3, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)),
+                                       (torch.zeros(2, 3, dtype=torch.int32), torch.zeros(2)), (torch.zeros(3, 2, dtype=torch.int32).t(), torch.zeros(2, dtype=torch.int32))])
+def test_paths_that_are_refused(path, kept):
+    z = torch.zeros(2, dtype=torch.int32)
+    b = seq_ops.StepBatch(T=2, E=2, max_n=1, tokens=z, pos=z, row_entry=z, row0=z, n=z, ctx=z, slot=z, page_table=z.view(2, 1), max_pages=1)
+    with pytest.raises(ValueError):
+        seq_ops.keep_rows(cache(), b, path, kept)
+
+
+def test_a_copy_says_where_the_copies_lie():
+    c = cache()
+    d = copy.deepcopy(c)
+    assert d.operands[0].data_ptr() != c.operands[0].data_ptr() and bytes(d.table.numpy().tobytes())[:8] == int(d.operands[0].data_ptr()).to_bytes(8, "little")
+
+
+def test_every_operand_is_in_the_table():
+    q = seq_ops.QuantizedPages(torch.zeros(6, 64, 48, dtype=torch.uint8).as_subclass(_OnDevice), torch.zeros(6, 3, 64, dtype=torch.uint8).as_subclass(_OnDevice))
+    c = seq_ops.CachePages([pages(6, 64, 33), q], 64)
+    assert c.count == 3 and c.table.numel() == 32 * 3 and c.most_page_bytes == 64 * 66 and c.most_columns == 33
