@@ -13,6 +13,7 @@ A "kv" layer that says how many heads its rows hold (`KvSpec`) can keep them in 
 and a power of two per row and head, a little over half of bfloat16's bytes); latent rows and states keep their types.
 
 `SequenceStore` owns the device tensors and the host-side bookkeeping (free lists, per-request page lists and lengths).
+Requests that fork (`fork`) share their full pages, which have as many owners, and have copies of the last, partly filled one and of the states.
 Pages and slots go back to the free lists when a request is released and are handed out again, lowest id first, so a
 second request really does land on memory a finished one used.  Nothing is cleared on reuse: a sequence's first step
 starts from length zero (attention reads no stale key; recurrent layers start from a zero state when their context is empty).
@@ -22,7 +23,7 @@ from typing import Dict, List, Optional, Sequence
 import torch
 
 from .modeling_gemma import PAGE
-from .seq_ops import QuantizedPages
+from .seq_ops import CachePages, QuantizedPages, copy_pages
 
 KV_FORMATS = (None, "e4m3")
 
@@ -47,6 +48,7 @@ class PagePool:
             raise ValueError("a page pool needs at least one page")
         self.num_pages = int(num_pages)
         self.free: List[int] = list(range(self.num_pages))
+        self.shared: Dict[int, int] = {}  # page -> owners, of pages with more than one
 
     def take(self, n: int) -> List[int]:
         if n > len(self.free):
@@ -55,11 +57,23 @@ class PagePool:
         got, self.free = self.free[:n], self.free[n:]
         return got
 
+    def share(self, pages: Sequence[int]):
+        """One more owner for each page: it is free again when all have given it back."""
+        for p in pages:
+            self.shared[p] = self.shared.get(p, 1) + 1
+
     def give(self, pages: Sequence[int]):
         dup = set(pages) & set(self.free)
         if dup:
             raise RuntimeError(f"pages freed twice: {sorted(dup)[:4]}")
-        self.free.extend(pages)
+        for p in pages:
+            owners = self.shared.get(p, 1)
+            if owners == 1:
+                self.free.append(p)
+            elif owners == 2:
+                del self.shared[p]
+            else:
+                self.shared[p] = owners - 1
 
 
 class SequenceRecord:
@@ -110,6 +124,15 @@ class SequenceStore:
             self.k_pages.append(k)
             self.v_pages.append(v)
             self.state.append(s)
+        self._operands = None
+
+    def operands(self):
+        """(CachePages of the layers' pages, CachePages of the states as pages of one row): what moves with a request; None where there is none."""
+        if self._operands is None:
+            pages = [p for p in self.k_pages + self.v_pages if p is not None]
+            states = [s.view(self.num_slots, 1, -1) for s in self.state if s is not None]
+            self._operands = (CachePages(pages, self.page) if pages else None, CachePages(states, 1) if states else None)
+        return self._operands
 
     # -- bookkeeping ---------------------------------------------------------------------------------------------------
     def admit(self, rid) -> SequenceRecord:
@@ -132,6 +155,39 @@ class SequenceStore:
 
     def commit(self, rid, new_tokens: int):
         self.live[rid].length += int(new_tokens)
+
+    def fork(self, rid, new: Sequence, length: Optional[int] = None) -> List[SequenceRecord]:
+        """New requests that go on where the first `length` (None: all) stored tokens of `rid` end.  They share its full pages, which nobody writes again, and have copies of the
+        rest of the last one and of its states: one launch for all of them."""
+        if rid not in self.live:
+            raise KeyError(f"request {rid!r} is not live")
+        rec, new = self.live[rid], list(new)
+        length = rec.length if length is None else int(length)
+        if not 0 < length <= rec.length:
+            raise ValueError(f"request {rid!r} has {rec.length} stored tokens: no fork behind {length}")
+        if length != rec.length and any(spec is not None and spec[0] == "state" for spec in self.layout):
+            raise ValueError("a model that keeps states forks behind its last token: there is no state of an earlier one")
+        if len(set(new)) != len(new) or any(n in self.live for n in new):
+            raise KeyError("a fork needs names that no live request has, each once")
+        full, rest = divmod(length, self.page)
+        if len(new) > len(self.free_slots):
+            raise MemoryError(f"{len(new)} forks wanted, {len(self.free_slots)} of {self.num_slots} sequence slots free")
+        mine = self.pool.take(len(new)) if rest else []
+        made = [self.admit(n) for n in new]
+        for i, r in enumerate(made):
+            r.pages, r.length = rec.pages[:full] + mine[i:i + 1], length
+            self.pool.share(rec.pages[:full])
+        pages, states = self.operands()
+        try:
+            if pages is not None and mine:
+                copy_pages(pages, [(rec.pages[full], p, rest) for p in mine])
+            if states is not None and made:
+                copy_pages(states, [(rec.slot, r.slot, 1) for r in made])
+        except BaseException:
+            for n in new:
+                self.release(n)
+            raise
+        return made
 
     def release(self, rid):
         rec = self.live.pop(rid)

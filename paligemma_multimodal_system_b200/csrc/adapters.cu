@@ -99,13 +99,13 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const PgAdapter a, co
   const int* tile = a.tiles + 3 * (item / subs);
   const int who = tile[0], skip = item % subs * M, first = tile[1] + skip, count = min(tile[2] - skip, M);
   const bool none = who < 0 || who >= a.slots;
+  pg::griddep_wait();  // (CTAs without work as well: the kernel behind counts on this one's end; the plan comes from the host, ahead of the step)
   if (count <= 0 || (none && a.out == a.y)) return;  // (the whole cluster)
   if (tid < M) {
     const int t = tid < count ? a.rows[first + tid] : -1;
     row_of[tid] = t < a.T ? t : -1;
   }
   __syncthreads();
-  pg::griddep_wait();
   constexpr int kOut = OUT32 ? 4 : 2;
   if (none) {
     for (int i = 0; i < count; ++i) {

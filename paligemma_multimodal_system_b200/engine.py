@@ -10,15 +10,19 @@ that has some -- whole prompts, portions of prompts and single decoded tokens si
   SequenceEngine.score(prompts)       log probabilities of the prompts' own tokens (pg_token_logprobs)
   SequenceEngine.step_drafts(entries) drafted trees: logits of every drafted token in one step, nothing committed;
   SequenceEngine.accept(rid, path)    keeps the drafted tokens of one path and drops the others
+  SequenceEngine.step_verify(entries) both at once: drafted tokens are judged against the model's own distributions and the accepted ones kept
+  SequenceEngine.fork(rid, new)       new requests that go on where a live one stands (or stood), over shared pages
+  adapters.AdapterSet                 low-rank adapters: every request may have one of its own
 
 The model supplies `cache_layout()`, `step(batch, store, want_rows)`, `prec` and `vocab_size` (modeling_mapedra.py).
 """
 import contextlib
-from typing import Dict, List, Optional, Sequence, Tuple
+from typing import Callable, Dict, List, Optional, Sequence, Tuple
 
 import torch
 
 from . import _lib, seq_ops
+from .adapters import AdapterSet, StepAdapters
 from .cache import SequenceStore
 from .seq_ops import StaticDecodeBatch, make_step_batch
 from .serving import StepScheduler, TokenRequest
@@ -41,11 +45,31 @@ def _records(scores):
     return [dict(logprob=a, rank=r, entropy=h, top=list(zip(i, t))) for a, h, r, i, t in zip(lp, entropy, rank, ids, top)]
 
 
+class LookupDrafter:
+    """Drafts from a request's own text: what followed the last earlier place that reads as its newest `match` tokens (or fewer, down to one) does."""
+
+    def __init__(self, most: int = 4, match: int = 3):
+        if most < 1 or match < 1:
+            raise ValueError("at least one drafted token, found by at least one")
+        self.most, self.match = int(most), int(match)
+
+    def __call__(self, history: List[int]):
+        for n in range(min(self.match, len(history) - 1), 0, -1):
+            tail = history[-n:]
+            for at in range(len(history) - n - 1, -1, -1):
+                if history[at:at + n] == tail:
+                    tokens = history[at + n:at + n + self.most]
+                    return tokens, list(range(-1, len(tokens) - 1))
+        return [], []
+
+
 class SequenceEngine:
-    def __init__(self, model, max_tokens: int, num_slots: int = 4, use_cuda_graph: bool = True, kv_format: Optional[str] = None):
-        """kv_format "e4m3": keys and values are cached in 8 bits (cache.py)."""
+    def __init__(self, model, max_tokens: int, num_slots: int = 4, use_cuda_graph: bool = True, kv_format: Optional[str] = None, adapters: Optional[AdapterSet] = None):
+        """kv_format "e4m3": keys and values are cached in 8 bits (cache.py).  adapters: the model's low-rank adapters, which requests name when they are admitted."""
         _lib.require_device()
         self.model = model
+        self.adapters = adapters
+        self._adapter_of: Dict[object, str] = {}
         self.store = SequenceStore(model.cache_layout(), max_tokens, num_slots, model.prec.dtype, kv_format=kv_format)
         self._drafted: Dict[object, List[int]] = {}  # request -> parents of the drafted tokens whose rows stand behind its own
         self._step_no = torch.zeros(1, device="cuda", dtype=torch.int32)
@@ -55,11 +79,17 @@ class SequenceEngine:
         self._decode_graphs = {}
 
     @torch.no_grad()
-    def step(self, entries: Sequence[Tuple[object, Sequence[int], Sequence[int]]], end: Sequence[object] = (), trace=None):
+    def step(self, entries: Sequence[Tuple[object, Sequence[int], Sequence[int]]], end: Sequence[object] = (), trace=None, adapters: Optional[Dict[object, str]] = None):
         """Runs the new tokens of every entry; returns fp32 logits [sum(len(want)), vocab] in entry / want order (None when
-        nothing is wanted).  A request id seen for the first time is admitted; ids in `end` are released after the step."""
+        nothing is wanted).  A request id seen for the first time is admitted, with the adapter that `adapters` names for it, and keeps that one; ids in `end` are released
+        after the step."""
         store = self.store
         batch, want, row = [], [], 0
+        for rid, name in (adapters or {}).items():
+            if name is not None and (self.adapters is None or name not in self.adapters.names):
+                raise KeyError(f"request {rid!r}: no adapter {name!r} is loaded")
+            if rid in store.live and self._adapter_of.get(rid) != name:
+                raise ValueError(f"request {rid!r} is live: it keeps the adapter that it was admitted with")
         seen = set()
         for rid, toks, w in entries:
             if rid in seen:
@@ -68,6 +98,8 @@ class SequenceEngine:
             toks = self._checked(rid, toks)
             if rid not in store.live:
                 store.admit(rid)
+                if adapters and adapters.get(rid) is not None:
+                    self._adapter_of[rid] = adapters[rid]
             rec = store.reserve(rid, len(toks))
             batch.append(dict(tokens=toks, ctx=rec.length, slot=rec.slot, pages=rec.pages))
             for k in w:
@@ -79,11 +111,11 @@ class SequenceEngine:
             self._drafted.pop(rid, None)  # (rows of drafts that were not accepted are written over)
         logits = None
         if batch and trace is None and self.use_cuda_graph and all(len(e["tokens"]) == 1 for e in batch):
-            logits = self._decode_step(batch, want)
+            logits = self._decode_step(batch, want, self._slots_of([rid for rid, _, _ in entries]))
             for (rid, toks, _w) in entries:
                 store.commit(rid, len(toks))
         elif batch:
-            b = make_step_batch(batch)
+            b = self._adapted(make_step_batch(batch), [rid for rid, _, _ in entries], [len(e["tokens"]) for e in batch])
             rows = torch.tensor(want, dtype=torch.int64).to("cuda", non_blocking=True) if want else None
             with _weights_follow():
                 logits = self.model.step(b, store, rows, trace=trace)
@@ -110,6 +142,23 @@ class SequenceEngine:
         drafted rows stand behind them until `accept`, or until the request's next step writes over them.  Models whose layers keep nothing but keys
         and values."""
         store = self.store
+        b, logits, batch = self._draft_step(entries)
+        for rid, _, parents in batch:
+            self._drafted[rid] = parents
+        return logits
+
+    def _slots_of(self, rids):
+        """Adapters of requests by their places, None where no request has one."""
+        names = [self._adapter_of.get(rid) for rid in rids]
+        return self.adapters.slots_of(names) if any(n is not None for n in names) else None
+
+    def _adapted(self, b, rids, ns):
+        slots = self._slots_of(rids)
+        return b if slots is None else seq_ops.with_adapters(b, StepAdapters(self.adapters.banks, seq_ops.AdapterPlan(ns, slots)))
+
+    def _draft_step(self, entries):
+        """Runs drafted trees; the requests' lengths stay.  (step, logits of every row, [(request, tokens, parents)])."""
+        store = self.store
         if any(spec is not None and spec[0] != "kv" for spec in store.layout):
             raise ValueError("drafted trees need a model whose layers keep nothing but keys and values: a state has no branches")
         if not entries:
@@ -129,12 +178,10 @@ class SequenceEngine:
             rec = store.reserve(rid, len(toks))
             rows.append(dict(tokens=toks, ctx=rec.length, slot=rec.slot, pages=rec.pages, parents=parents))
             self._drafted.pop(rid, None)  # (written over; nothing to accept should the step fail)
-        b = make_step_batch(rows)
+        b = self._adapted(make_step_batch(rows), [rid for rid, _, _ in batch], [len(toks) for _, toks, _ in batch])
         with _weights_follow():
             logits = self.model.step(b, store, torch.arange(b.T, device="cuda"))
-        for rid, _, parents in batch:
-            self._drafted[rid] = parents
-        return logits
+        return b, logits, batch
 
     @torch.no_grad()
     def accept(self, rid, path: Sequence[int]):
@@ -147,37 +194,80 @@ class SequenceEngine:
         if any(not 0 <= p < len(parents) for p in path) or any(parents[p] != up for p, up in zip(path, [-1] + path)):
             raise ValueError("a path runs from a root of the drafted tree, every token the parent of the next")
         store, rec = self.store, self.store.live[rid]
-        moved = [(i, p) for i, p in enumerate(path) if i != p]
-        if moved:
-            page = store.page
-            at = torch.tensor([[rec.length + x for x in m] for m in moved], dtype=torch.int64)
-            pages = torch.tensor(rec.pages, dtype=torch.int64)
-            idx = torch.cat([pages[at // page], at % page], 1).to("cuda", non_blocking=True)
-            (dst, src), (dslot, sslot) = (idx[:, 0], idx[:, 1]), (idx[:, 2], idx[:, 3])
-            for kind in (store.k_pages, store.v_pages):
-                for p in kind:
-                    if isinstance(p, seq_ops.QuantizedPages):
-                        p.codes[dst, dslot] = p.codes[src, sslot]
-                        p.powers[dst, :, dslot] = p.powers[src, :, sslot]
-                    elif p is not None:
-                        p[dst, dslot] = p[src, sslot]
+        if any(i != p for i, p in enumerate(path)):
+            n = len(parents)
+            b = make_step_batch([dict(tokens=[0] * n, ctx=rec.length, slot=rec.slot, pages=rec.pages)])  # (says where the rows lie)
+            where = torch.tensor([path + [len(path)]], dtype=torch.int32).to("cuda", non_blocking=True)
+            seq_ops.keep_rows(store.operands()[0], b, where, where[:, -1])
         store.commit(rid, len(path))
         del self._drafted[rid]
 
-    def _decode_step(self, batch, want):
-        """A step of single-token entries through a captured graph (eagerly the first time a geometry is seen)."""
+    @torch.no_grad()
+    def step_verify(self, entries: Sequence[Tuple[object, Sequence[int], Sequence[int]]], do_sample: bool = False, temperature: float = 0.8, top_p: float = 0.9,
+                    uniforms: Optional[torch.Tensor] = None, draft_logits: Optional[torch.Tensor] = None, draft_temperature: Optional[float] = None,
+                    draft_top_p: Optional[float] = None):
+        """Runs drafted trees and keeps what the model itself would have said (seq_ops.verify_drafts): entries as step_drafts', the first token of each the request's pending
+        one (chosen, not yet run), from which the others descend.  Returns per entry (path, next token): the rows that were kept, 0 in front, which the request has stored
+        now, and the token behind them (-1: the logits there are no distribution).  Greedy, or with do_sample at `temperature` and `top_p`; uniforms: fp32 [rows, 2] (None: drawn here); draft_logits
+        fp32 [rows, vocab]: what the children of every row were drawn from (None: guessed)."""
+        out, _, _ = self._verified(entries, do_sample, temperature, top_p, uniforms, draft_logits, draft_temperature, draft_top_p)
+        return out
+
+    def _verified(self, entries, do_sample, temperature, top_p, uniforms=None, draft_logits=None, draft_temperature=None, draft_top_p=None):
+        if not do_sample and (uniforms is not None or draft_logits is not None):
+            raise ValueError("a greedy walk takes no random numbers and no drafted distributions")
+        for rid, toks, parents in entries:
+            if len(parents) == 0 or parents[0] != -1 or any(p < 0 for p in parents[1:]):
+                raise ValueError(f"request {rid!r}: the first token is the pending one, the others descend from it")
+        b, logits, batch = self._draft_step(entries)
+        if do_sample and uniforms is None:
+            uniforms = torch.rand(b.T, 2, device="cuda")
+        how = dict(temperature=temperature, top_p=top_p) if do_sample else {}
+        path, kept, last = seq_ops.verify_drafts(logits, b, uniforms, draft_logits, draft_temperature=draft_temperature, draft_top_p=draft_top_p, **how)
+        seq_ops.keep_rows(self.store.operands()[0], b, path, kept)
+        said = torch.cat([path, kept[:, None], last[:, None]], 1).tolist()
+        out = []
+        for (rid, _, _), (*row, n, token) in zip(batch, said):
+            self.store.commit(rid, n)
+            out.append((row[:n], token))
+        return out, b, logits
+
+    @torch.no_grad()
+    def fork(self, rid, new: Sequence[object], length: Optional[int] = None):
+        """New requests, admitted under the names `new`, that go on where the first `length` stored tokens (None: all) of `rid` end, with its adapter.  Full pages are
+        shared; what each owns is a copy of the last, partly filled page and of the states.  Models with states fork behind the last token only."""
+        self.store.fork(rid, new, length)
+        if rid in self._adapter_of:
+            self._adapter_of.update((n, self._adapter_of[rid]) for n in new)
+
+    def remove_adapter(self, name: str):
+        users = [rid for rid, n in self._adapter_of.items() if n == name]
+        if users:
+            raise ValueError(f"adapter {name!r} is in use by {users[:4]}")
+        self.adapters.remove(name)
+
+    def _decode_step(self, batch, want, adapters=None):
+        """A step of single-token entries through a captured graph (eagerly the first time a geometry is seen).  adapters: their places, or None."""
         E = len(batch)
         pages = max(len(e["pages"]) for e in batch)
         pages_cap = 4
         while pages_cap < pages:
             pages_cap *= 2
         ctx_cap = pages_cap * self.store.page  # every context of this page-table width; fixes the key split of the attention
-        key = (E, pages_cap)
+        version = None if adapters is None else self.adapters.version
+        key = (E, pages_cap) if adapters is None else (E, pages_cap, version)
         slot = self._decode_graphs.get(key)
         if slot is None:
+            if adapters is not None:  # (steps that hold banks of before are not replayed again)
+                self._decode_graphs = {k: v for k, v in self._decode_graphs.items() if len(k) == 2 or k[2] == version}
             slot = self._decode_graphs[key] = dict(static=StaticDecodeBatch(E, pages_cap, ctx_cap), graph=None, logits=None, seen=0)
+            if adapters is not None:
+                slot["plan"] = seq_ops.AdapterPlan([1] * E, adapters, tiles=E)
+                slot["static"].batch = seq_ops.with_adapters(slot["static"].batch, StepAdapters(dict(self.adapters.banks), slot["plan"]))
         st = slot["static"]
         st.fill(batch)
+        if adapters is not None:
+            slot["plan"].fill([1] * E, adapters)
         slot["seen"] += 1
         if slot["graph"] is None and slot["seen"] >= 2:
             side = torch.cuda.Stream()
@@ -200,6 +290,7 @@ class SequenceEngine:
 
     def release(self, rid):
         self._drafted.pop(rid, None)
+        self._adapter_of.pop(rid, None)
         self.store.release(rid)
 
     # -- generation ------------------------------------------------------------------------------------------------
@@ -217,23 +308,39 @@ class SequenceEngine:
 
     @torch.no_grad()
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int, do_sample: bool = False, temperature: float = 0.8,
-                 top_p: float = 0.9, eos_token_id: Optional[int] = None, seed: int = 0, step_tokens: int = 512, logprobs: Optional[int] = None):
+                 top_p: float = 0.9, eos_token_id: Optional[int] = None, seed: int = 0, step_tokens: int = 512, logprobs: Optional[int] = None,
+                 draft: Optional[Callable[[List[int]], Tuple[List[int], List[int]]]] = None, adapters: Optional[Sequence[Optional[str]]] = None):
         """Greedy (or temperature / top-p) continuation of every prompt; more prompts than slots queue up and take over slots
         and pages as earlier ones finish.  Returns the new tokens per prompt (EOS included when it was emitted): List[List[int]].
         logprobs = k (0 .. 32): (tokens, records), records per prompt and token a dict with its logprob, rank and entropy and the k most likely (id, logprob)
-        pairs in `top`, under softmax(logits / temperature) where tokens are sampled and softmax(logits) else."""
+        pairs in `top`, under softmax(logits / temperature) where tokens are sampled and softmax(logits) else.
+        draft: guesses how a request goes on -- its tokens so far -> (drafted tokens, parents), parents[i] the drafted token that token i follows or -1 the newest one
+        (LookupDrafter) -- and steps of decoded tokens run the guesses along and keep those that the model says as well: the tokens of a greedy run are the same, those of a
+        sampled one have the same distribution.  adapters: one name or None for every prompt."""
+        if draft is not None and any(spec is not None and spec[0] != "kv" for spec in self.store.layout):
+            raise ValueError("drafted trees need a model whose layers keep nothing but keys and values: a state has no branches")
+        if adapters is not None and len(adapters) != len(prompts):
+            raise ValueError("one adapter (or None) for every prompt")
+        named = {("gen", i): n for i, n in enumerate(adapters or ())}
+        rng = torch.Generator(device="cuda").manual_seed(int(seed)) if draft is not None and do_sample else None
         if logprobs is not None and not 0 <= logprobs <= min(32, self.model.vocab_size):
             raise ValueError(f"logprobs is 0 .. 32 and at most the vocabulary: got {logprobs}")
         records = {}
-        sched = StepScheduler(self.store.num_slots, self.store.pool.num_pages, self.store.page, step_tokens, eos_token_id)
+        # (what live requests hold stays theirs)
+        sched = StepScheduler(len(self.store.free_slots), len(self.store.pool.free), self.store.page, step_tokens, eos_token_id)
         for i, pr in enumerate(prompts):
             sched.submit(TokenRequest(("gen", i), [int(t) for t in pr], int(max_new_tokens)))
         while not sched.idle():
             plan = sched.plan()
             if not plan:
                 raise RuntimeError("scheduler made no progress")
+            if draft is not None and all(req.fed == len(req.prompt) for req, _, _ in plan):
+                guessed = self._guesses(plan, draft)
+                if any(len(toks) > 1 for _, toks, _ in guessed):
+                    self._drafted_turn(plan, guessed, sched, do_sample, temperature, top_p, rng, logprobs, records)
+                    continue
             entries = [(req.rid, toks, [len(toks) - 1] if sample else []) for req, toks, sample in plan]
-            logits = self.step(entries)
+            logits = self.step(entries, adapters={rid: named.get(rid) for rid, _, _ in entries} if named else None)
             picked, said = [], None
             if logits is not None:
                 out = self._sample(logits, do_sample, temperature, top_p, seed)
@@ -248,6 +355,40 @@ class SequenceEngine:
                     self.release(req.rid)
         tokens = [sched.finished[("gen", i)] for i in range(len(prompts))]
         return tokens if logprobs is None else (tokens, [records.get(("gen", i), []) for i in range(len(prompts))])
+
+    def _guesses(self, plan, draft):
+        """Entries of a drafted step: every decoding request's newest token and what is guessed behind it."""
+        entries = []
+        for req, toks, _ in plan:
+            tokens, parents = draft(req.prompt + req.tokens)
+            room = req.max_new_tokens - len(req.tokens) - 1  # (rows that the request's pages have room for beside the newest token's)
+            tokens, parents = list(tokens)[:room], list(parents)[:room]
+            entries.append((req.rid, toks + tokens, [-1] + [int(p) + 1 for p in parents]))
+        return entries
+
+    def _drafted_turn(self, plan, entries, sched, do_sample, temperature, top_p, rng, logprobs, records):
+        """One step of `generate` in which every request decodes, with its guesses."""
+        T = sum(len(toks) for _, toks, _ in entries)
+        uniforms = torch.rand(T, 2, device="cuda", generator=rng) if do_sample else None
+        out, b, logits = self._verified(entries, do_sample, temperature, top_p, uniforms)
+        if any(token < 0 for _, token in out):
+            raise RuntimeError("a row of logits is no distribution")
+        said, rows, row0 = [], [], 0
+        for (_, toks, _), (path, token) in zip(entries, out):
+            said.append([toks[i] for i in path[1:]] + [token])
+            rows += [row0 + i for i in path]
+            row0 += len(toks)
+        if logprobs is not None:
+            idx = torch.tensor(rows + [t for ts in said for t in ts], dtype=torch.int64).to("cuda", non_blocking=True)
+            told = iter(_records(seq_ops.token_logprobs(logits.index_select(0, idx[:len(rows)]), idx[len(rows):].int(), top=logprobs, temperature=temperature if do_sample else 1.0)))
+        for (req, _, _), tokens in zip(plan, said):
+            told_here = [next(told) for _ in tokens] if logprobs is not None else []
+            for i, t in enumerate(tokens):
+                if logprobs is not None:
+                    records.setdefault(req.rid, []).append(told_here[i])
+                if sched.advance(req, 1, t):
+                    self.release(req.rid)
+                    break
 
     @torch.no_grad()
     def score(self, prompts: Sequence[Sequence[int]], top: int = 0, step_tokens: int = 512):

@@ -58,18 +58,19 @@ def test_inference(model: PaliGemmaForConditionalGeneration, processor, device: 
 
 def generate_token_ids(model_path: str, prompt_ids, max_tokens_to_generate: int, temperature: float, top_p: float, do_sample: bool,
                        dtype: str = "bfloat16", max_tokens: int = 0, slots: int = 4, eos_token_id: int = None,
-                       logprobs: int = None, kv_format: str = None):
+                       logprobs: int = None, kv_format: str = None, draft: int = 0):
     """Text-only checkpoints of the registry (config.json `architecture`, e.g. Mapedra) carry no tokenizer: prompts are lists of
     token ids (several prompts separated by ';'), served by the ragged-step engine; prints and returns the new ids per prompt.
     kv_format "e4m3": keys and values are cached in 8 bits; logprobs k: every new token's log probability, rank and entropy and the k likeliest
-    alternatives are printed below, and (ids, records) are returned."""
-    from .engine import SequenceEngine
+    alternatives are printed below, and (ids, records) are returned; draft n: up to n tokens a step are guessed from the request's own text and kept where the model agrees."""
+    from .engine import LookupDrafter, SequenceEngine
     from .registry import load_model
     prompts = [[int(t) for t in part.replace(",", " ").split()] for part in str(prompt_ids).split(";") if part.strip()]
     model = load_model(model_path, dtype=getattr(torch, dtype))
     need = sum((len(p) + max_tokens_to_generate + 63) // 64 * 64 for p in prompts[:slots])
     engine = SequenceEngine(model, max(max_tokens, need), slots, kv_format=kv_format)
-    out = engine.generate(prompts, max_tokens_to_generate, do_sample=do_sample, temperature=temperature, top_p=top_p, eos_token_id=eos_token_id, logprobs=logprobs)
+    out = engine.generate(prompts, max_tokens_to_generate, do_sample=do_sample, temperature=temperature, top_p=top_p, eos_token_id=eos_token_id, logprobs=logprobs,
+                          draft=LookupDrafter(draft) if draft else None)
     tokens, records = out if logprobs is not None else (out, [[]] * len(out))
     for p, o, said in zip(prompts, tokens, records):
         print(" ".join(map(str, p)), "->", " ".join(map(str, o)))
@@ -81,7 +82,7 @@ def generate_token_ids(model_path: str, prompt_ids, max_tokens_to_generate: int,
 def main(model_path: str = None, prompt: str = None, image_file_path: str = None, max_tokens_to_generate: int = 100,
          temperature: float = 0.8, top_p: float = 0.9, do_sample: bool = False, only_cpu: bool = False, prompt_ids: str = None,
          dtype: str = "bfloat16", max_tokens: int = 0, slots: int = 4, eos_token_id: int = None,
-         logprobs: int = None, kv_format: str = None):
+         logprobs: int = None, kv_format: str = None, draft: int = 0):
     if only_cpu:
         raise RuntimeError("this build has no CPU path: it needs a B200 (sm_100a)")
     import json
@@ -93,7 +94,7 @@ def main(model_path: str = None, prompt: str = None, image_file_path: str = None
         if prompt_ids is None:
             raise SystemExit(f"{arch} is a text-only model without a tokenizer: pass --prompt_ids \"1 2 3\"")
         return generate_token_ids(model_path, prompt_ids, max_tokens_to_generate, temperature, top_p, do_sample, dtype, max_tokens, slots,
-                                  eos_token_id, logprobs, kv_format)
+                                  eos_token_id, logprobs, kv_format, draft)
     from .processing_paligemma import PaliGemmaProcessor
     from .utils import load_hf_model
     device = "cuda"
@@ -130,4 +131,5 @@ if __name__ == "__main__":
     ap.add_argument("--eos_token_id", type=int, default=None)
     ap.add_argument("--logprobs", type=int, default=None, help="text-only models: print every new token's log probability and this many alternatives (0 .. 32)")
     ap.add_argument("--kv_format", default=None, choices=["e4m3"], help="text-only models: keep keys and values in 8 bits")
+    ap.add_argument("--draft", type=int, default=0, help="text-only models: guess up to this many tokens a step from the request's own text")
     main(**vars(ap.parse_args()))

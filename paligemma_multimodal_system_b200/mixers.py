@@ -28,7 +28,8 @@
 
 Every sub-layer gets its weights from a name -> tensor dict (`take(name)` pops and checks the shape), packs them once for a
 `Precision`, says what it keeps per sequence (`cache_spec`), and maps the step's rows h [T, D] (activation type) to
-y [T, D] fp32; the block around it owns norms and the residual stream.  The newer sub-layers take `resid=` (the fp32 residual
+y [T, D] fp32; the block around it owns norms and the residual stream.  Sub-layers that say `adapter_sites` add the step's low-rank adapters behind those
+projections.  The newer sub-layers take `resid=` (the fp32 residual
 rows): their last projection then adds into it in the GEMM epilogue instead of returning y.
 """
 import ctypes as C
@@ -79,6 +80,11 @@ def half_to_pair_order(n: int, rot_dims: int):
     return [i // 2 + (i % 2) * half if i < rot_dims else i for i in range(n)]
 
 
+def _attention_sites(pre, width, parts, inner):
+    """Projections beside which low-rank adapters may stand (adapters.AdapterSet): name -> (depth, [(weight, columns)])."""
+    return {pre + "in": (width, [(pre + n, c) for n, c in parts]), pre + "out": (inner, [(pre + "o", width)])}
+
+
 class GatedSoftmaxAttention:
     def __init__(self, width, heads, kv_heads, dim, vdim, scale, softcap, rot_dims, rot_base, rot_scaling, eps):
         if heads % kv_heads:
@@ -94,9 +100,13 @@ class GatedSoftmaxAttention:
 
     def load(self, take, pre):
         H, G, dim, vdim, D = self.H, self.G, self.dim, self.vdim, self.D
+        self.pre = pre
         self.w = dict(q=take(pre + "q", (H * dim, D)), k=take(pre + "k", (G * dim, D)), v=take(pre + "v", (G * vdim, D)),
                       g=take(pre + "g", (H * vdim, D)), o=take(pre + "o", (D, H * vdim)),
                       qn=take(pre + "q.norm", (dim,)), kn=take(pre + "k.norm", (dim,)))
+
+    def adapter_sites(self):
+        return _attention_sites(self.pre, self.D, [("q", self.H * self.dim), ("k", self.G * self.dim), ("v", self.G * self.vdim), ("g", self.H * self.vdim)], self.H * self.vdim)
 
     def pack(self, prec):
         w = self.w
@@ -108,13 +118,16 @@ class GatedSoftmaxAttention:
     def __call__(self, h, b, store, li, prec):
         H, G, dim, vdim = self.H, self.G, self.dim, self.vdim
         proj = seq_ops.linear(h, self.w_in, prec.empty(b.T, self.w_in.shape[0]))
+        seq_ops.adapt(b, self.pre + "in", h, proj)
         q = prec.empty(b.T, H * dim)
         kp, vp = store.k_pages[li], store.v_pages[li]
         seq_ops.attn_prepare(proj, b, self.freq_d, self.qn, self.kn, q, kp, vp, H, G, dim, vdim, self.rot_dims, self.eps, PAGE)
         att = prec.empty(b.T, H * vdim)
         gate = proj[:, (H + G) * dim + G * vdim:]
         seq_ops.attn_ragged(q, kp, vp, gate, att, b, H, G, dim, vdim, self.scale, self.softcap, PAGE)
-        return seq_ops.linear(att, self.w_o, torch.empty(b.T, self.D, device="cuda", dtype=torch.float32))
+        y = seq_ops.linear(att, self.w_o, torch.empty(b.T, self.D, device="cuda", dtype=torch.float32))
+        seq_ops.adapt(b, self.pre + "out", att, y)
+        return y
 
 
 class WindowedSoftmaxAttention:
@@ -168,6 +181,7 @@ class WindowedSoftmaxAttention:
 
     def load(self, take, pre):
         H, G, dim, vdim, D = self.H, self.G, self.dim, self.vdim, self.D
+        self.pre = pre
         w = dict(q=take(pre + "q", (H * dim, D)))
         if self.bias:
             w["qb"] = take(pre + "q.b", (H * dim,))
@@ -195,6 +209,10 @@ class WindowedSoftmaxAttention:
             w["g"] = take(pre + "g", (H, D))
         w["o"] = take(pre + "o", (D, H * vdim))
         self.w = w
+
+    def adapter_sites(self):
+        kv = [] if self.kv_from is not None else [("k", self.G * self.dim)] + ([] if self.value_is_key else [("v", self.G * self.vdim)])
+        return _attention_sites(self.pre, self.D, [("q", self.H * self.dim)] + kv + ([("g", self.H)] if self.head_gate else []), self.H * self.vdim)
 
     def pack(self, prec):
         w, H = self.w, self.H
@@ -225,6 +243,7 @@ class WindowedSoftmaxAttention:
     def __call__(self, h, b, store, li, prec, resid=None, resid_scale=1.0):
         H, G, dim, vdim = self.H, self.G, self.dim, self.vdim
         proj = seq_ops.linear(h, self.w_in, prec.empty(b.T, self.w_in.shape[0]), bias=self.b_in)
+        seq_ops.adapt(b, self.pre + "in", h, proj)
         q = prec.empty(b.T, H * dim)
         own = self.kv_from is None
         src = li if own else self.kv_from
@@ -240,8 +259,11 @@ class WindowedSoftmaxAttention:
         gate = proj[:, self.gate_col:] if self.head_gate else None
         seq_ops.attn_ragged(q, kp, vp, gate, att, b, H, G, dim, vdim, self.scale, 0.0, PAGE, gate_per_head=True, score=self.score)
         if resid is not None:
-            return seq_ops.linear_add(att, self.w_o, resid, scale=resid_scale)
-        return seq_ops.linear(att, self.w_o, torch.empty(b.T, self.D, device="cuda", dtype=torch.float32))
+            y = seq_ops.linear_add(att, self.w_o, resid, scale=resid_scale)
+        else:
+            y = seq_ops.linear(att, self.w_o, torch.empty(b.T, self.D, device="cuda", dtype=torch.float32))
+        seq_ops.adapt(b, self.pre + "out", att, y, resid_scale if resid is not None else 1.0)
+        return y
 
 
 class LightningAttention:
@@ -256,8 +278,13 @@ class LightningAttention:
 
     def load(self, take, pre):
         H, dim, vdim, D = self.H, self.dim, self.vdim, self.D
+        self.pre = pre
         self.w = dict(q=take(pre + "q", (H * dim, D)), k=take(pre + "k", (H * dim, D)), v=take(pre + "v", (H * vdim, D)),
                       g=take(pre + "g", (H * vdim, D)), o=take(pre + "o", (D, H * vdim)), norm=take(pre + "norm", (H * vdim,)))
+
+    def adapter_sites(self):
+        H, dim, vdim = self.H, self.dim, self.vdim
+        return _attention_sites(self.pre, self.D, [("q", H * dim), ("k", H * dim), ("v", H * vdim), ("g", H * vdim)], H * vdim)
 
     def pack(self, prec):
         w = self.w
@@ -269,11 +296,14 @@ class LightningAttention:
     def __call__(self, h, b, store, li, prec):
         H, dim, vdim = self.H, self.dim, self.vdim
         proj = seq_ops.linear(h, self.w_in, prec.empty(b.T, self.w_in.shape[0]))
+        seq_ops.adapt(b, self.pre + "in", h, proj)
         o = torch.empty(b.T, H * vdim, device="cuda", dtype=torch.float32)
         seq_ops.linear_attn(proj, store.state[li], self.decay_d, o, b, H, dim, vdim)
         att = prec.empty(b.T, H * vdim)
         seq_ops.rmsnorm_gate(o, self.norm, proj[:, 2 * H * dim + H * vdim:], att, self.eps)
-        return seq_ops.linear(att, self.w_o, torch.empty(b.T, self.D, device="cuda", dtype=torch.float32))
+        y = seq_ops.linear(att, self.w_o, torch.empty(b.T, self.D, device="cuda", dtype=torch.float32))
+        seq_ops.adapt(b, self.pre + "out", att, y)
+        return y
 
 
 class GegluFeedForward:
@@ -281,7 +311,11 @@ class GegluFeedForward:
         self.D, self.F = width, ff
 
     def load(self, take, pre):
+        self.pre = pre
         self.w = dict(gate=take(pre + "gate", (self.F, self.D)), up=take(pre + "up", (self.F, self.D)), down=take(pre + "down", (self.D, self.F)))
+
+    def adapter_sites(self):
+        return {self.pre + "down": (self.F, [(self.pre + "down", self.D)])}
 
     def pack(self, prec):
         w, F, D = self.w, self.F, self.D
@@ -314,13 +348,16 @@ class GegluFeedForward:
         if self.fused:
             mid = prec.empty(T, self.Fp)
             _lib.gemm(h, self.w_gu, mid, mode=_lib.EPI_GEGLU, swap=1 if T <= 128 else 0)
-            if zeros is not None:
-                return seq_ops.linear(mid, self.w_down, zeros, zeros=True)
         else:
             gu = seq_ops.linear(h, self.w_gu, prec.empty(T, 2 * self.F))
             mid = prec.empty(T, self.F)
             seq_ops.geglu(gu, mid)
-        return seq_ops.linear(mid, self.w_down, torch.empty(T, self.D, device="cuda", dtype=torch.float32))
+        if self.fused and zeros is not None:
+            y = seq_ops.linear(mid, self.w_down, zeros, zeros=True)
+        else:
+            y = seq_ops.linear(mid, self.w_down, torch.empty(T, self.D, device="cuda", dtype=torch.float32))
+        seq_ops.adapt(b, self.pre + "down", mid, y)
+        return y
 
 
 class GluFeedForward:
@@ -337,9 +374,13 @@ class GluFeedForward:
 
     def load(self, take, pre):
         F, D = self.F, self.D
+        self.pre = pre
         self.w = dict(gate=take(pre + "gate", (F, D)), up=take(pre + "up", (F, D)), down=take(pre + "down", (D, F)))
         if self.bias:
             self.w.update(gate_b=take(pre + "gate.b", (F,)), up_b=take(pre + "up.b", (F,)), down_b=take(pre + "down.b", (D,)))
+
+    def adapter_sites(self):
+        return {self.pre + "down": (self.F, [(self.pre + "down", self.D)])}
 
     def pack(self, prec):
         w, F, D = self.w, self.F, self.D
@@ -379,8 +420,11 @@ class GluFeedForward:
             gu = seq_ops.linear(h, self.w_gu, prec.empty(T, 2 * self.F), bias=self.b_gu)
             mid = seq_ops.glu(gu, prec.empty(T, self.F), self.kind, self.limit, self.alpha)
         if resid is not None:
-            return seq_ops.linear_add(mid, self.w_down, resid, bias=self.b_down)
-        return seq_ops.linear(mid, self.w_down, torch.empty(T, self.D, device="cuda", dtype=torch.float32), bias=self.b_down)
+            y = seq_ops.linear_add(mid, self.w_down, resid, bias=self.b_down)
+        else:
+            y = seq_ops.linear(mid, self.w_down, torch.empty(T, self.D, device="cuda", dtype=torch.float32), bias=self.b_down)
+        seq_ops.adapt(b, self.pre + "down", mid, y)
+        return y
 
 
 class TokenSideInput:
@@ -464,11 +508,15 @@ class LatentAttention:
 
     def load(self, take, pre):
         H, dim, rot, vdim, Q, R, D = self.H, self.dim, self.rot, self.vdim, self.Q, self.R, self.D
+        self.pre = pre
         self.w = dict(dq=take(pre + "dq", (Q, D)), qn=take(pre + "dq.norm", (Q,)), uq=take(pre + "uq", (H * (dim + rot), Q)))
         if self.kv_from is None:
             self.w.update(dkv=take(pre + "dkv", (R + rot, D)), cn=take(pre + "dkv.norm", (R,)))
         self.w.update(uk=take(pre + "uk", (H * dim, R)), uv=take(pre + "uv", (H * vdim, R)),
                       g=take(pre + "g", (H * vdim if self.gate_kind == "element" else H, D)), o=take(pre + "o", (D, H * vdim)))
+
+    def adapter_sites(self):
+        return {self.pre + "out": (self.H * self.vdim, [(self.pre + "o", self.D)])}
 
     def pack(self, prec):
         w, H, dim, rot, vdim, R = self.w, self.H, self.dim, self.rot, self.vdim, self.R
@@ -532,9 +580,13 @@ class LatentAttention:
             seq_ops.rotate_heads(qr, qr, b.pos, self.freq_d, self.rot_dims, self.rot_gain)
             seq_ops.attn_ragged(q.view(T, H * (dim + rot)), kx, vx, gate, att.view(T, H * vdim), seq_ops.dense_view(b), H, H, dim + rot, vdim,
                                 self.scale, 0.0, PAGE, gate_per_head=per_head, skip_singles=True, score=self.score)
+        att = att.view(T, H * vdim)
         if resid is not None:
-            return seq_ops.linear_add(att.view(T, H * vdim), self.w_o, resid, scale=resid_scale)
-        return seq_ops.linear(att.view(T, H * vdim), self.w_o, torch.empty(T, self.D, device="cuda", dtype=torch.float32))
+            y = seq_ops.linear_add(att, self.w_o, resid, scale=resid_scale)
+        else:
+            y = seq_ops.linear(att, self.w_o, torch.empty(T, self.D, device="cuda", dtype=torch.float32))
+        seq_ops.adapt(b, self.pre + "out", att, y, resid_scale if resid is not None else 1.0)
+        return y
 
 
 class PolyNormFeedForward:
@@ -547,9 +599,13 @@ class PolyNormFeedForward:
 
     def load(self, take, pre):
         F, D = self.F, self.D
+        self.pre = pre
         self.w = dict(up=take(pre + "up", (F, D)), down=take(pre + "down", (D, F)), act=take(pre + "act", (4,)))
         if self.bias:
             self.w.update(up_b=take(pre + "up.b", (F,)), down_b=take(pre + "down.b", (D,)))
+
+    def adapter_sites(self):
+        return {self.pre + "up": (self.D, [(self.pre + "up", self.F)]), self.pre + "down": (self.F, [(self.pre + "down", self.D)])}
 
     def pack(self, prec):
         w = self.w
@@ -563,10 +619,14 @@ class PolyNormFeedForward:
     def __call__(self, h, b, prec, resid=None, resid_scale=1.0):
         T = h.shape[0]
         z = seq_ops.linear(h, self.w_up, prec.empty(T, self.F), bias=self.b_up)
+        seq_ops.adapt(b, self.pre + "up", h, z)
         mid = seq_ops.polynorm(z, self.coef, z, self.eps)
         if resid is not None:
-            return seq_ops.linear_add(mid, self.w_down, resid, bias=self.b_down, scale=resid_scale)
-        return seq_ops.linear(mid, self.w_down, torch.empty(T, self.D, device="cuda", dtype=torch.float32), bias=self.b_down)
+            y = seq_ops.linear_add(mid, self.w_down, resid, bias=self.b_down, scale=resid_scale)
+        else:
+            y = seq_ops.linear(mid, self.w_down, torch.empty(T, self.D, device="cuda", dtype=torch.float32), bias=self.b_down)
+        seq_ops.adapt(b, self.pre + "down", mid, y, resid_scale if resid is not None else 1.0)
+        return y
 
 
 class SquaredReluFeedForward:

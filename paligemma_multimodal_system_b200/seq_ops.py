@@ -74,7 +74,7 @@ StepBatch.parents = StepBatch.adapters = None
 class RequestBatch(StepBatch):
     """A step whose requests have something of their own (`dataclasses.replace` keeps both)."""
     parents: dataclasses.InitVar[Optional[torch.Tensor]] = None  # int32 [T], drafted trees: the row of its entry that a row follows, -1 the stored tokens
-    adapters: dataclasses.InitVar[Optional["StepAdapters"]] = None  # low-rank adapters of the entries
+    adapters: dataclasses.InitVar[Optional[object]] = None  # low-rank adapters of the entries (adapters.StepAdapters)
 
     def __post_init__(self, at, tree, parents, adapters):
         self.at, self.tree, self.parents, self.adapters = at, tree, parents, adapters
@@ -161,6 +161,17 @@ def make_step_batch(entries: Sequence[dict]) -> StepBatch:
                      max_single_ctx=max([e["ctx"] for e, k in zip(entries, ns) if k == 1], default=0), single_rows=_single_rows(ns),
                      dense_row0=dev[o2:o2 + E], dense_pages=dev[o2 + E:plain].view(E, dmax), dense_max_pages=dmax, dense_rows=page0 * 64,
                      dense_max_len=max(lens), **drafted)
+
+
+def with_adapters(b: StepBatch, adapters) -> RequestBatch:
+    """The same step whose entries have adapters (adapters.StepAdapters)."""
+    return RequestBatch(**{f.name: getattr(b, f.name) for f in dataclasses.fields(b)}, at=b.at, tree=b.tree, parents=b.parents, adapters=adapters)
+
+
+def adapt(b: Optional[StepBatch], site: str, x, y, gain=1.0):
+    """Adds what the step's adapters have beside the projection `site` of x to y; nothing in a step without adapters."""
+    if b is not None and b.adapters is not None:
+        b.adapters.add(site, x, y, gain)
 
 
 def step_scope(b: StepBatch) -> StepBatch:
@@ -830,6 +841,9 @@ class AdapterPlan:
         h[T:T + 3 * len(tiles)] = np.asarray(tiles).reshape(-1)
         self.most, self.used = int(ids[-1]), sum(int(a) >= 0 for a in ids)
         self.dev.copy_(self.host, non_blocking=True)
+        if self.fixed is not None and self.dev.is_cuda:
+            self._copied = torch.cuda.Event()
+            self._copied.record()
 
     def fill(self, ns: Sequence[int], adapters: Sequence[int]):
         """Other adapters for as many rows, at the same addresses."""
@@ -838,8 +852,6 @@ class AdapterPlan:
         if self._copied is not None:
             self._copied.synchronize()  # the image before must have left the pinned buffer
         self._make(ns, adapters, self.dev.device)
-        self._copied = torch.cuda.Event()
-        self._copied.record()
 
 
 def _rows_overlap(s, s_pitch, t, t_pitch):
