@@ -7,44 +7,67 @@
 // After rejections the rest is r_j = (p - c_j q)+ / S_j: from r_j q is taken again, (p - c_j q)+ - S_j q = p - (c_j + S_j) q where that is positive, so c and S are
 // two numbers and a rejection is one pass over the row, whatever came before it.
 //
-// The results are whole numbers that hang on running sums: a draw is wrong once a sum is off by the distance of u from a token's border.  Weights are therefore
-// e^((x - m) / T) in double, 2^(j / 64) from a table times a polynomial of degree 4 (error below 1e-13), nine operations of the double pipe, half of fp32's rate.
+// The results are whole numbers that hang on running sums: a draw is wrong once a sum is off by the distance of u from a token's border.  Weights e^((x - m) / T) from
+// 2^-16 on are therefore made in double, 2^(j / 256) from a table times a polynomial of degree 3 (error below 1e-13); smaller ones in fp32, where a run of 128 holds no other.
 //
 // The nucleus is a threshold on the logit: the entries above which at most top_p Z lies.  Entries below (1 - top_p) Z / V cannot belong to it.  The others are
-// counted by mass into 1024 runs of the ordered bit patterns, in fixed point (sums do not hang on their order), and the run that holds the border is divided
-// again until a run is one pattern: at most three rounds of one cluster barrier, and few entries take part.
+// counted by mass into 1024 runs of the ordered bit patterns, in fixed point (sums do not hang on their order).  The entries of the run that holds the border go to
+// all CTAs and are compared one by one; where they are many the run is divided again, until it is one pattern.
 //
-// A CTA keeps its share of the row in shared memory: one read of global memory, whatever follows.
+// Two passes over a row, one for its maximum and one, from L2, for its sum; the second leaves the entries that may belong to the nucleus in shared memory, in the
+// order of their places, and everything behind it goes over those (over the row where they are too many).
 #include "common.cuh"
 #include "paligemma_b200.h"
 
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kRanks = 16, kBins = 1024, kCoarse = kBins / 32, kTable = 64;
-constexpr int kShare = 16384;      // entries of a row that a CTA keeps where that many CTAs do (64 KB: three CTAs an SM)
-constexpr int kMostShare = 49152;  // and at most (192 KB)
+constexpr int kThreads = 512, kPerSm = 2, kWarps = kThreads / 32, kRanks = 16, kBins = 1024, kCoarse = kBins / 32, kTable = 256, kList = 32;
+constexpr int kRun = 128, kRuns = 4;  // entries that a warp takes at once, a float4 a lane; runs under way
+constexpr int kHeld = 512;            // entries of a row that a warp can hold as candidates of the nucleus
 constexpr int kDead = -2147483647 - 1;
 constexpr double kLog2e = 1.4426950408889634;
 
-struct __align__(16) Shared {
-  double table[kTable];                    // 2^(j / 64)
-  double warp[kWarps];
-  double all[2][kRanks];                   // one double of every CTA, by turns
-  unsigned long long key[2][kRanks];
-  unsigned long long hist[2][kBins];       // mass of runs of bit patterns, by turns
-  unsigned long long coarse[2][kCoarse];
-  unsigned long long gather[kRanks][32];
-  unsigned long long found_base;
-  int found, pick, state, last;
+struct Entry {
+  unsigned long long mass;
+  uint32_t key;
 };
-
-static_assert(sizeof(Shared) % 16 == 0, "a share of a row starts on a 16-byte boundary");
-
+struct Candidate {
+  float x;
+  int at;  // place in the CTA's share
+};
+struct __align__(16) Shared {
+  double table[kTable];                    // 2^(j / 256)
+  double warp[kWarps];
+  double all[2][kRanks], part[2][kRanks];  // doubles of every CTA, by turns
+  double warp_part[kWarps];
+  unsigned long long key[2][kRanks];
+  unsigned long long hist[kBins];          // mass of runs of bit patterns
+  unsigned long long coarse[kRanks][kCoarse], fine[kRanks][32];
+  Entry own[kList], list[kRanks][kList];   // entries of the run that holds the border
+  Candidate held[kWarps][kHeld];
+  int held_count[kWarps], listed[kRanks], over[2][kRanks];
+  unsigned long long found_base;
+  float largest[kWarps], whole[2][kRanks]; // what the threads' largest entries sum up to, relative to the CTA's
+  int found, pick, state, last, own_listed;
+  uint32_t least;
+};
 PG_DEVINL uint32_t ordered(float x) {  // larger numbers have larger ones; both zeros alike, NaN above all
   const uint32_t b = __float_as_uint(x + 0.0f);
   return x != x ? 0xffffffffu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 PG_DEVINL float unordered(uint32_t o) { return __uint_as_float((o & 0x80000000u) ? o & 0x7fffffffu : ~o); }
+PG_DEVINL float max_nan(float a, float b) {  // a NaN stays one
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+PG_DEVINL float max_nan(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+using pg::max3;
 
 PG_DEVINL uint32_t remote(const void* p, int rank) {
   uint32_t there;
@@ -64,60 +87,172 @@ PG_DEVINL int load_relaxed(const int* p) {
   return v;
 }
 
+// e^((x - m) / T) = 2^(x a + shift) with a = log2(e) / T and shift = -m a.  (The rounding of m a is in every weight alike.)  Entries below `cut` weigh nothing: they are 2^-1000 of
+// the largest or outside the nucleus.
 struct Scale {
-  double m, a;  // maximum, log2(e) / T
+  double a, shift;
+  float cut;
+  // for fp32: a and shift in two parts, shift's first a multiple of 2^-8; runs with an entry of `fine` or more are weighed in double
+  float a0, a1, s0, s1, fine;
 };
-// e^((x - m) / T) for x <= m (the difference of two floats first: it stays right for the smallest temperatures)
-PG_DEVINL double weight(const double* table, Scale s, float x) {
-  const double t = (static_cast<double>(x) - s.m) * s.a;
-  if (!(t > -1000.0)) return 0.0;  // (-inf too)
-  constexpr double kRound = 6755399441055744.0 / kTable;  // 1.5 2^52 / 64: its last place is 1 / 64
-  const double rounded = t + kRound, f = t - (rounded - kRound);  // |f| <= 1 / 128
+PG_DEVINL Scale scale_of(float m, double temperature) {
+  Scale s;
+  s.a = kLog2e / temperature;
+  s.shift = -static_cast<double>(m) * s.a;
+  s.cut = nextafterf(__double2float_rd(static_cast<double>(m) - 1000.0 / s.a), INFINITY);
+  if (!(fabs(s.shift) < 0x1p40)) s.a = s.shift = 0.0, s.cut = m;  // the float in front of m weighs less than 2^-1000 here: what equals m shares the mass
+  s.a0 = static_cast<float>(s.a);
+  s.a1 = static_cast<float>(s.a - s.a0);
+  s.s0 = static_cast<float>(rint(s.shift * 256.0) / 256.0);
+  s.s1 = static_cast<float>(s.shift - s.s0);
+  s.fine = fabs(s.shift) < 0x1p15 ? static_cast<float>(static_cast<double>(m) - 16.0 / s.a) : -INFINITY;
+  return s;
+}
+PG_DEVINL double weight(const double* table, const Scale& s, float x) {
+  const double t = fma(static_cast<double>(x), s.a, s.shift);
+  constexpr double kRound = 6755399441055744.0 / kTable;  // 1.5 2^52 / 256: its last place is 1 / 256
+  const double rounded = t + kRound, f = t - (rounded - kRound);  // |f| <= 1 / 512
   const int k = __double2loint(rounded);
-  constexpr double c1 = 0.6931471805599453, c2 = c1 * c1 / 2, c3 = c1 * c1 * c1 / 6, c4 = c1 * c1 * c1 * c1 / 24;
-  const double p = fma(f, fma(f, fma(f, fma(f, c4, c3), c2), c1), 1.0) * table[k & (kTable - 1)];
-  return __hiloint2double(__double2hiint(p) + ((k >> 6) << 20), __double2loint(p));
+  const double power = table[k & (kTable - 1)];
+  constexpr double c1 = 0.6931471805599453, c2 = c1 * c1 / 2, c3 = c1 * c1 * c1 / 6;
+  const double w = fma(f, fma(f, fma(f, c3, c2), c1), 1.0) * __hiloint2double(__double2hiint(power) + ((k >> 8) << 20), __double2loint(power));
+  return x >= s.cut ? w : 0.0;
+}
+// The same for weights below 2^-16 in fp32, each off by 2^-23 and without a bias: together by 2^-23 sqrt(2^-16) of the whole at most.  The argument is divided exactly: s0 - k is, x a0 is
+// inside the instruction.  Taylor's polynomial of degree 7, |f| <= 1 / 2 (error 5e-9 at the ends, 6e-10 on average).  Entries below `low` count as 2^-100.  Two at a time: issue slots
+// are what bounds the pass.
+struct Pairs {
+  uint64_t a0, a1, s0, s1;
+  float low;
+  PG_DEVINL explicit Pairs(const Scale& s) : a0(pg::pair_of(s.a0, s.a0)), a1(pg::pair_of(s.a1, s.a1)), s0(pg::pair_of(s.s0, s.s0)), s1(pg::pair_of(s.s1, s.s1)) {
+    low = static_cast<float>((-100.0 - s.shift) / s.a);
+  }
+  PG_DEVINL float2 operator()(float x, float y) const {
+    constexpr double c1 = 0.6931471805599453, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4, c5 = c4 * c1 / 5, c6 = c5 * c1 / 6, c7 = c6 * c1 / 7;
+    constexpr float kRound = 12582912.0f;  // 1.5 2^23
+    auto both = [](double c) { return pg::pair_of(static_cast<float>(c), static_cast<float>(c)); };
+    const uint64_t z = pg::pair_of(fmaxf(x, low), fmaxf(y, low));
+    const uint64_t rounded = pg::add_pair(pg::fma_pair(z, a0, s0), both(kRound)), k = pg::add_pair(rounded, both(-kRound));
+    const uint64_t f = pg::add_pair(pg::fma_pair(z, a0, pg::fma_pair(k, both(-1.0), s0)), pg::fma_pair(z, a1, s1));
+    uint64_t p = pg::fma_pair(f, both(c7), both(c6));
+    p = pg::fma_pair(f, p, both(c5)), p = pg::fma_pair(f, p, both(c4)), p = pg::fma_pair(f, p, both(c3));
+    p = pg::fma_pair(f, p, both(c2)), p = pg::fma_pair(f, p, both(c1)), p = pg::fma_pair(f, p, both(1.0));
+    return make_float2(__uint_as_float(pg::lo_of(p) + (pg::lo_of(rounded) << 23)), __uint_as_float(pg::hi_of(p) + (pg::hi_of(rounded) << 23)));
+  }
+};
+
+PG_DEVINL bool is_fine(const Scale& s, float4 x) { return __any_sync(0xffffffffu, fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)) >= s.fine); }
+// the sum of four entries of a run (whole warps); the run alone says in which form
+PG_DEVINL double weights_sum(const double* table, const Scale& s, const Pairs& small, float4 x) {
+  if (is_fine(s, x)) return (weight(table, s, x.x) + weight(table, s, x.y)) + (weight(table, s, x.z) + weight(table, s, x.w));
+  const float2 u = small(x.x, x.y), v = small(x.z, x.w);
+  return static_cast<double>(((x.x >= s.cut ? u.x : 0.0f) + (x.y >= s.cut ? u.y : 0.0f)) + ((x.z >= s.cut ? v.x : 0.0f) + (x.w >= s.cut ? v.y : 0.0f)));
 }
 
-struct Part {  // a CTA's share of a row: entries lo .. lo + n of it in xs; warp w has seg from w seg on
-  float* xs;
+struct Part {  // a CTA's share of a row: entries lo .. lo + n of it; warp w has seg from w seg on
   int lo, n, seg, rank, ranks;
 };
+struct Source {  // a share in global memory (behind the first pass: in L2)
+  const float* x;
+  bool aligned;
+  PG_DEVINL Source(const float* row, int lo) : x(row + lo), aligned((reinterpret_cast<uintptr_t>(row + lo) & 15) == 0) {}
+  PG_DEVINL float4 four(int i, int n) const {  // entries i .. i + 3 of n, -inf behind
+    if (aligned && i + 4 <= n) return __ldg(reinterpret_cast<const float4*>(x + i));
+    return make_float4(i < n ? x[i] : -INFINITY, i + 1 < n ? x[i + 1] : -INFINITY, i + 2 < n ? x[i + 2] : -INFINITY, i + 3 < n ? x[i + 3] : -INFINITY);
+  }
+};
 
-PG_DEVINL void load_share(const Part& p, const float* row) {
-  const float* src = row + p.lo;
-  const uint32_t dst = pg::smem_u32(p.xs);
-  const int whole = (reinterpret_cast<uintptr_t>(src) & 15) == 0 ? p.n / 4 * 4 : 0;
-  for (int i = 4 * threadIdx.x; i < whole; i += 4 * kThreads) pg::cp_async16(dst + 4 * i, src + i, true);
-  for (int i = whole + threadIdx.x; i < p.n; i += kThreads)
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + 4 * i), "l"(src + i) : "memory");
-  pg::cp_async_commit();
+// f(first place, four entries) over entries begin .. end of the share, a warp's runs; whole warps
+template <typename F>
+PG_DEVINL void each4(const Part& p, const Source& s, int begin, int end, F f) {
+  const int lane = threadIdx.x % 32;
+  int i = begin;
+  if (s.aligned)
+    for (; i + kRun * kRuns <= end; i += kRun * kRuns) {
+      const float4* from = reinterpret_cast<const float4*>(s.x + i) + lane;
+      float4 x[kRuns];
+#pragma unroll
+      for (int k = 0; k < kRuns; ++k) x[k] = __ldg(from + k * (kRun / 4));
+#pragma unroll
+      for (int k = 0; k < kRuns; ++k) f(i + k * kRun + 4 * lane, x[k]);
+    }
+#pragma unroll 1
+  for (; i < end; i += kRun) f(i + 4 * lane, s.four(i + 4 * lane, end));
+}
+template <typename F>
+PG_DEVINL void each4(const Part& p, const Source& s, F f) {
+  const int warp = threadIdx.x / 32;
+  each4(p, s, warp * p.seg, min((warp + 1) * p.seg, p.n), f);
 }
 
-// (largest entry, lowest place) of the row as one number, known to all CTAs
-PG_DEVINL unsigned long long row_top(Shared& sh, const Part& p, int& turn) {
-  uint32_t best = 0;
+PG_DEVINL float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// (largest entry, lowest place) of the row as one number, known to all CTAs.  PLACE false: the entry alone, and in `whole` the sum of the largest entries' weights of all threads,
+// a being log2(e) / T: less than the row's.
+template <bool PLACE>
+PG_DEVINL unsigned long long row_top(Shared& sh, const Part& p, const Source& s, int& turn, float a, float& whole) {
+  float best = -INFINITY;  // this thread's largest
+  int run = 0;
+  each4(p, s, [&](int i, float4 x) {
+    if (PLACE) {
+      const float four = max_nan(max_nan(x.x, x.y), x.z, x.w);
+      if (four > best) run = i;
+      best = max_nan(best, four);  // (where that is a NaN the place does not matter)
+    } else {
+      best = max_nan(max_nan(best, x.x, x.y), x.z, x.w);
+    }
+  });
   int at = 0;
-  for (int i = threadIdx.x; i < p.n; i += kThreads) {
-    const uint32_t k = ordered(p.xs[i]);
-    if (k > best) best = k, at = i;
+  if (PLACE && run < p.n) {  // the first of the four that were the first to hold it
+    const float4 x = s.four(run, p.n);
+    at = p.lo + run + (x.x == best ? 0 : x.y == best ? 1 : x.z == best ? 2 : 3);
   }
-  unsigned long long key = p.n > 0 ? static_cast<unsigned long long>(best) << 32 | static_cast<uint32_t>(~(p.lo + at)) : 0ull;
+  unsigned long long key = static_cast<unsigned long long>(ordered(best)) << 32 | static_cast<uint32_t>(~at);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, o);
     key = other > key ? other : key;
   }
   unsigned long long* mine = reinterpret_cast<unsigned long long*>(sh.warp);
+  __syncthreads();  // (the sums before have been read)
   if (threadIdx.x % 32 == 0) mine[threadIdx.x / 32] = key;
   __syncthreads();
-  if (static_cast<int>(threadIdx.x) < p.ranks) {
-    for (int w = 0; w < kWarps; ++w) key = mine[w] > key ? mine[w] : key;
-    put64(&sh.key[turn][p.rank], threadIdx.x, key);
+  if (threadIdx.x < 32) {
+    key = threadIdx.x < kWarps ? mine[threadIdx.x] : 0ull;
+#pragma unroll
+    for (int o = kWarps / 2; o > 0; o >>= 1) {
+      const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, o);
+      key = other > key ? other : key;
+    }
+    key = __shfl_sync(0xffffffffu, key, 0);
+    if (static_cast<int>(threadIdx.x) < p.ranks) put64(&sh.key[turn][p.rank], threadIdx.x, key);
+  }
+  if (!PLACE) {
+    unsigned long long here = 0;
+    for (int w = 0; w < kWarps; ++w) here = mine[w] > here ? mine[w] : here;
+    float some = ex2((best - unordered(static_cast<uint32_t>(here >> 32))) * a);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) some += __shfl_xor_sync(0xffffffffu, some, o);
+    if (threadIdx.x % 32 == 0) sh.largest[threadIdx.x / 32] = some;
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) < p.ranks) {
+      some = 0.0f;
+      for (int w = 0; w < kWarps; ++w) some += sh.largest[w];
+      put32(&sh.whole[turn][p.rank], threadIdx.x, __float_as_int(some));
+    }
   }
   pg::cluster_sync_all();
   unsigned long long top = 0;
   for (int r = 0; r < p.ranks; ++r) top = sh.key[turn][r] > top ? sh.key[turn][r] : top;
+  if (!PLACE) {
+    whole = 0.0f;
+    const float m = unordered(static_cast<uint32_t>(top >> 32));
+    for (int r = 0; r < p.ranks; ++r) whole += sh.whole[turn][r] * ex2((unordered(static_cast<uint32_t>(sh.key[turn][r] >> 32)) - m) * a);
+  }
   turn ^= 1;
   return top;
 }
@@ -126,114 +261,217 @@ PG_DEVINL bool is_distribution(unsigned long long top) {
   return k > ordered(-INFINITY) && k < ordered(INFINITY);
 }
 
-// Sums of f over the row: the warps' in sh.warp, the CTAs' in sh.all[turn] (until the next but one), the whole as the result.  The order of additions is fixed.
-template <typename F>
-PG_DEVINL double row_mass(Shared& sh, const Part& p, int& turn, F f) {
+// What the warps have summed: theirs in sh.warp, the CTAs' in sh.all[turn] (until the next but one), the whole as the result.  The order of additions is fixed.  `over` of any
+// thread becomes all CTAs'; `part`: a second sum.
+PG_DEVINL double share_sums(Shared& sh, const Part& p, int& turn, double sum, bool over = false, double* part = nullptr) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int lo = min(warp * p.seg, p.n), hi = min(lo + p.seg, p.n);
-  double sum = 0.0;
-  for (int i = lo + lane; i < hi; i += 32) sum += f(i);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  __syncthreads();  // (the sums before have been read)
-  if (lane == 0) sh.warp[warp] = sum;
+  for (int o = 16; o > 0; o >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (part != nullptr) *part += __shfl_xor_sync(0xffffffffu, *part, o);
+  }
+  over = __syncthreads_or(over);  // (and the sums before have been read)
+  if (lane == 0) {
+    sh.warp[warp] = sum;
+    if (part != nullptr) sh.warp_part[warp] = *part;
+  }
   __syncthreads();
-  if (static_cast<int>(threadIdx.x) < p.ranks) {
-    double all = 0.0;
-    for (int w = 0; w < kWarps; ++w) all += sh.warp[w];
-    put64(&sh.all[turn][p.rank], threadIdx.x, __double_as_longlong(all));
+  if (warp == 0) {
+    double all = lane < kWarps ? sh.warp[lane] : 0.0, all_part = part != nullptr && lane < kWarps ? sh.warp_part[lane] : 0.0;
+#pragma unroll
+    for (int o = kWarps / 2; o > 0; o >>= 1) {
+      all += __shfl_xor_sync(0xffffffffu, all, o);
+      if (part != nullptr) all_part += __shfl_xor_sync(0xffffffffu, all_part, o);
+    }
+    all = __shfl_sync(0xffffffffu, all, 0);
+    all_part = __shfl_sync(0xffffffffu, all_part, 0);
+    if (lane < p.ranks) {
+      put64(&sh.all[turn][p.rank], lane, __double_as_longlong(all));
+      if (part != nullptr) {
+        put64(&sh.part[turn][p.rank], lane, __double_as_longlong(all_part));
+        put32(&sh.over[turn][p.rank], lane, over);
+      }
+    }
   }
   pg::cluster_sync_all();
   double total = 0.0;
   for (int r = 0; r < p.ranks; ++r) total += sh.all[turn][r];
+  if (part != nullptr) {
+    *part = 0.0;
+    for (int r = 0; r < p.ranks; ++r) *part += sh.over[turn][r] ? NAN : sh.part[turn][r];
+  }
   turn ^= 1;
   return total;
 }
 
-// The token at u times the whole of f, whose sums row_mass has left (`turn` behind it): the first place whose running sum is above that.  Known to all CTAs.
+// Sums over the row: f(place, four entries) is their sum
 template <typename F>
-PG_DEVINL int row_draw(Shared& sh, const Part& p, int turn, double total, float u, F f) {
+PG_DEVINL double row_mass(Shared& sh, const Part& p, const Source& s, int& turn, F f) {
+  double sum = 0.0;
+  each4(p, s, [&](int i, float4 x) { sum += f(i, x); });
+  return share_sums(sh, p, turn, sum);
+}
+// and over the candidates: f(candidate)
+template <typename F>
+PG_DEVINL double held_mass(Shared& sh, const Part& p, int& turn, F f) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  double rest = static_cast<double>(u) * total, run = 0.0;
-  int owner = -1, behind = -1;
-  for (int r = 0; r < p.ranks; ++r) {  // (where rounding leaves no border behind u: the last one with any mass)
-    const double m = sh.all[turn ^ 1][r];
-    if (m > 0.0) behind = r;
-    if (owner < 0 && run + m > rest) owner = r;
-    if (owner < 0) run += m;
-  }
-  if (owner < 0) owner = behind;
-  if (owner == p.rank) {
-    int mine = -1, other = -1;
-    for (int w = 0; w < kWarps; ++w) {
-      const double m = sh.warp[w];
-      if (m > 0.0) other = w;
-      if (mine < 0 && run + m > rest) mine = w;
-      if (mine < 0) run += m;
-    }
-    if (mine < 0) mine = other;
-    if (warp == mine) {
-      const int lo = min(warp * p.seg, p.n), hi = min(lo + p.seg, p.n);
-      int place = -1, last = -1;
-      for (int i0 = lo; i0 < hi && place < 0; i0 += 32) {
-        const double w = i0 + lane < hi ? f(i0 + lane) : 0.0;
-        double incl = w;
+  double sum = 0.0;
+  for (int i = lane; i < sh.held_count[warp]; i += 32) sum += f(sh.held[warp][i]);
+  return share_sums(sh, p, turn, sum);
+}
+
+// Where u times the whole lies among n sums (n <= 32, one a lane): the first whose running sum is above `rest`, else the last with any mass; `run` becomes what lies in
+// front of it.  Whole warps; every lane has the result.
+PG_DEVINL int place_among(double mine, int n, double rest, double& run) {
+  const int lane = threadIdx.x % 32;
+  double incl = lane < n ? mine : 0.0;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double before = __shfl_up_sync(0xffffffffu, incl, o);
-          if (lane >= o) incl += before;
-        }
-        const uint32_t some = __ballot_sync(0xffffffffu, w > 0.0), past = __ballot_sync(0xffffffffu, run + incl > rest) & some;
-        if (some) last = i0 + 31 - __clz(some);
-        if (past) place = i0 + __ffs(past) - 1;
-        run += __shfl_sync(0xffffffffu, incl, 31);
-      }
-      if (place < 0) place = last;
-      if (lane < p.ranks) put32(&sh.pick, lane, p.lo + place);
-    }
+  for (int o = 1; o < 32; o <<= 1) {
+    const double before = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += before;
+  }
+  const uint32_t some = __ballot_sync(0xffffffffu, lane < n && mine > 0.0), past = __ballot_sync(0xffffffffu, run + incl > rest) & some;
+  const int at = past ? __ffs(past) - 1 : 31 - __clz(some);
+  run += __shfl_sync(0xffffffffu, incl - (lane < n ? mine : 0.0), at & 31);
+  return at;
+}
+
+// The token at u times the whole, whose sums are in sh.warp and sh.all (`turn` behind them): the first place whose running sum is above that.  Known to all CTAs.  (Where
+// rounding leaves no border behind u: the last place with any mass.)  find(warp, rest, run) gives the place in the share, within that warp's part.
+template <typename F>
+PG_DEVINL int share_draw(Shared& sh, const Part& p, int turn, double total, float u, F find) {
+  const int lane = threadIdx.x % 32;
+  double rest = static_cast<double>(u) * total, run = 0.0;
+  const int owner = place_among(lane < p.ranks ? sh.all[turn ^ 1][lane] : 0.0, p.ranks, rest, run);
+  if (owner == p.rank) {
+    const int mine = place_among(lane < kWarps ? sh.warp[lane] : 0.0, kWarps, rest, run);
+    __syncthreads();  // (the warps' sums have been read)
+    const int place = find(mine, rest, run);
+    if (static_cast<int>(threadIdx.x) / 32 == mine && lane < p.ranks) put32(&sh.pick, lane, p.lo + place);
   }
   pg::cluster_sync_all();
   return sh.pick;
 }
+template <typename F>
+PG_DEVINL int row_draw(Shared& sh, const Part& p, const Source& s, int turn, double total, float u, F f) {
+  return share_draw(sh, p, turn, total, u, [&](int mine, double rest, double run) {
+    // all warps sum pieces of that warp's part, which then looks for the piece, the lane and the entry
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, begin = mine * p.seg, end = min(begin + p.seg, p.n);
+    const int piece = (end - begin + kWarps * kRun - 1) / (kWarps * kRun) * kRun, from = min(begin + warp * piece, end), to = min(from + piece, end);
+    double sum = 0.0;
+    for (int i = from; i < to; i += kRun) {
+      double w[4];
+      f(i + 4 * lane, s.four(i + 4 * lane, to), w);
+      sum += (w[0] + w[1]) + (w[2] + w[3]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) sh.warp[warp] = sum;
+    __syncthreads();
+    int place = -1, last = 0;
+    if (warp == mine) {
+      const int at = place_among(lane < kWarps ? sh.warp[lane] : 0.0, kWarps, rest, run);
+      const int begin2 = min(begin + at * piece, end), end2 = min(begin2 + piece, end);
+      for (int i = begin2; i < end2 && place < 0; i += kRun) {
+        double w[4];
+        f(i + 4 * lane, s.four(i + 4 * lane, end2), w);
+        const double four = (w[0] + w[1]) + (w[2] + w[3]);
+        double all = four;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+        const uint32_t some = __ballot_sync(0xffffffffu, four > 0.0);
+        if (some == 0) continue;
+        const int l0 = 31 - __clz(some), k0 = w[3] > 0.0 ? 3 : w[2] > 0.0 ? 2 : w[1] > 0.0 ? 1 : 0;
+        last = i + 4 * l0 + __shfl_sync(0xffffffffu, k0, l0);
+        if (run + all > rest) {
+          double before = run;
+          const int l = place_among(four, 32, rest, before);
+          int k = -1, behind = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            before += w[j];
+            if (w[j] > 0.0) {
+              behind = j;
+              if (k < 0 && before > rest) k = j;
+            }
+          }
+          place = i + 4 * l + __shfl_sync(0xffffffffu, k < 0 ? behind : k, l);
+        }
+        run += all;
+      }
+    }
+    return place < 0 ? last : place;
+  });
+}
+template <typename F>
+PG_DEVINL int held_draw(Shared& sh, const Part& p, int turn, double total, float u, F f) {
+  return share_draw(sh, p, turn, total, u, [&](int mine, double rest, double run) {
+    const int lane = threadIdx.x % 32;
+    int place = -1, last = 0;
+    if (static_cast<int>(threadIdx.x) / 32 == mine)
+      for (int i = 0; i < sh.held_count[mine] && place < 0; i += 32) {
+        const bool there = i + lane < sh.held_count[mine];
+        const double w = there ? f(sh.held[mine][i + lane]) : 0.0;
+        const uint32_t some = __ballot_sync(0xffffffffu, w > 0.0);
+        if (some == 0) continue;
+        double all = w;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+        double before = run;
+        const int l = run + all > rest ? place_among(w, 32, rest, before) : 31 - __clz(some);
+        if (run + all > rest) place = sh.held[mine][i + l].at;
+        last = sh.held[mine][i + l].at;
+        run += all;
+      }
+    return place < 0 ? last : place;
+  });
+}
 
-// Least ordered pattern of the nucleus.  z: the whole mass, `bits`: of the fixed point.
-PG_DEVINL uint32_t nucleus(Shared& sh, const Part& p, Scale s, uint32_t top, double z, double top_p, double temperature, int V, int bits, int& turn) {
-  const double least = static_cast<double>(unordered(top)) + log((1.0 - top_p) * z / V) * temperature;
-  float floor_x = __double2float_rd(least);
-  floor_x -= fabsf(floor_x) * 3e-7f + 1e-37f;
-  uint32_t hi = top, lo = floor_x == floor_x ? min(ordered(floor_x), top) : 0u;
+// An entry below this has (1 - top_p) z / V at most: even all of them together are not what the nucleus leaves out.
+PG_DEVINL float least_of(float m, double z, double top_p, double temperature, int V) {
+  const float x = __double2float_rd(static_cast<double>(m) + log((1.0 - top_p) * z / V) * temperature);
+  return x - (fabsf(x) * 3e-7f + 1e-37f);
+}
+
+// Least entry of the nucleus.  z: the whole mass, `bits`: of the fixed point.
+// each(f): f of every entry that may belong
+template <typename E>
+PG_DEVINL float nucleus(Shared& sh, const Part& p, const Scale& s, uint32_t top, double z, double top_p, double temperature, int V, int bits, E each) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const float floor_x = least_of(unordered(top), z, top_p, temperature, V);
+  uint32_t hi = top, lo = floor_x == floor_x ? min(ordered(fmaxf(floor_x, s.cut)), top) : ordered(s.cut);
   const double one = static_cast<double>(1ull << bits), border = top_p * z * one;
   unsigned long long base = 0;  // mass above hi
   for (;;) {
     const uint32_t range = hi - lo;
     const int shift = range < kBins ? 0 : 32 - __clz(range) - 10;
-    unsigned long long* hist = sh.hist[turn];
     __syncthreads();
-    for (int i = threadIdx.x; i < kBins; i += kThreads) hist[i] = 0;
+    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.hist[i] = 0;
+    if (threadIdx.x == 0) sh.own_listed = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < p.n; i += kThreads) {
-      const float x = p.xs[i];
-      const uint32_t k = ordered(x);
-      if (k >= lo && k <= hi) atomicAdd(&hist[(hi - k) >> shift], static_cast<unsigned long long>(weight(sh.table, s, x) * one));
-    }
+    const float least = unordered(lo), most = unordered(hi);
+    auto count = [&](float x) {
+      if (x >= least && x <= most) atomicAdd(&sh.hist[(hi - ordered(x)) >> shift], static_cast<unsigned long long>(weight(sh.table, s, x) * one));
+    };
+    each(count);
     __syncthreads();
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     for (int c = warp; c < kCoarse; c += kWarps) {
-      unsigned long long v = hist[c * 32 + lane];
+      unsigned long long v = sh.hist[c * 32 + lane];
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (lane == 0) sh.coarse[turn][c] = v;
+      if (lane < p.ranks) put64(&sh.coarse[p.rank][c], lane, v);
     }
     pg::cluster_sync_all();
     int bin = 0;
 #pragma unroll
     for (int step = 0; step < 2; ++step) {  // 32 runs of 32, then one of them
-      const unsigned long long* from = step == 0 ? sh.coarse[turn] : hist + bin * 32;
-      if (warp < p.ranks) sh.gather[warp][lane] = get64(from + lane, warp);
-      __syncthreads();
+      if (step == 1) {
+        for (int r = warp; r < p.ranks; r += kWarps) sh.fine[r][lane] = get64(sh.hist + bin * 32 + lane, r);
+        __syncthreads();
+      }
       if (warp == 0) {
         unsigned long long v = 0;
-        for (int r = 0; r < p.ranks; ++r) v += sh.gather[r][lane];
+        for (int r = 0; r < p.ranks; ++r) v += step == 0 ? sh.coarse[r][lane] : sh.fine[r][lane];
         unsigned long long incl = v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -249,159 +487,307 @@ PG_DEVINL uint32_t nucleus(Shared& sh, const Part& p, Scale s, uint32_t top, dou
       base = sh.found_base;
       bin = bin * 32 + sh.found;
     }
-    const int found = sh.found;
-    turn ^= 1;
-    if (found < 0) return lo;
+    if (sh.found < 0) return unordered(lo);
     hi -= static_cast<uint32_t>(bin) << shift;
-    if (shift == 0) return hi;
+    if (shift == 0) return unordered(hi);
     const uint32_t width = (1u << shift) - 1;
     lo = hi - lo > width ? hi - width : lo;
+    // the run's entries to all CTAs; where they are few it is decided at once
+    const float run_least = unordered(lo), run_most = unordered(hi);
+    each([&](float x) {
+      if (x >= run_least && x <= run_most) {
+        const int at = atomicAdd(&sh.own_listed, 1);
+        if (at < kList) {
+          sh.own[at].mass = static_cast<unsigned long long>(weight(sh.table, s, x) * one);
+          sh.own[at].key = ordered(x);
+        }
+      }
+    });
+    __syncthreads();
+    const int own = sh.own_listed;
+    for (int r = warp; r < p.ranks; r += kWarps) {
+      if (lane < min(own, kList)) {
+        put64(&sh.list[p.rank][lane].mass, r, sh.own[lane].mass);
+        put32(&sh.list[p.rank][lane].key, r, static_cast<int>(sh.own[lane].key));
+      }
+      if (lane == 0) put32(&sh.listed[p.rank], r, own);
+    }
+    if (threadIdx.x == 0) sh.least = hi;
+    pg::cluster_sync_all();
+    bool few = true;
+    for (int r = 0; r < p.ranks; ++r) few = few && sh.listed[r] <= kList;
+    if (few) {  // an entry belongs if what is above it does not pass the border
+      for (int mine = warp; mine < p.ranks; mine += kWarps) {
+        if (lane >= sh.listed[mine]) continue;
+        const uint32_t key = sh.list[mine][lane].key;
+        unsigned long long above = base;
+        for (int r = 0; r < p.ranks; ++r)
+          for (int i = 0; i < sh.listed[r]; ++i)
+            if (sh.list[r][i].key > key) above += sh.list[r][i].mass;
+        if (static_cast<double>(above) <= border) atomicMin(&sh.least, key);
+      }
+      __syncthreads();
+      return unordered(sh.least);
+    }
   }
 }
 
-struct Row {  // a row's distribution: weight / mass where the pattern is `least` or above
+struct Row {  // a row's distribution: weights / mass
   Scale s;
-  uint32_t least;
   double mass;
+  float bound;  // entries from here on are the candidates in shared memory (listed)
+  bool good, listed, held;  // held: nothing else weighs anything
+  int turn;
 };
 
-PG_DEVINL double kept_weight(const double* table, const Row& r, float x) { return ordered(x) >= r.least ? weight(table, r.s, x) : 0.0; }
-
-// max(p - c q, 0) of one entry; both products rounded alike, so that equal ones leave nothing
-PG_DEVINL double rest_weight(const double* table, const Row& t, double pf, float x, const Row& q, double qf, float y) {
-  return fmax(__dsub_rn(__dmul_rn(pf, kept_weight(table, t, x)), __dmul_rn(qf, kept_weight(table, q, y))), 0.0);
-}
-
-// The distribution of the row in xs; its sums of the kept weights are left behind for a draw.
-PG_DEVINL bool distribution(Shared& sh, const Part& p, double temperature, double top_p, int V, int bits, Row& r, int& turn) {
-  const unsigned long long top = row_top(sh, p, turn);
-  if (!is_distribution(top)) return false;
-  r.s.a = kLog2e / temperature;
-  r.s.m = unordered(static_cast<uint32_t>(top >> 32));
-  r.least = 0;
-  r.mass = row_mass(sh, p, turn, [&](int i) { return weight(sh.table, r.s, p.xs[i]); });
+// The distribution of a row; its sums of the kept weights are left behind for a draw.  (Once in the program: its loops are long.  All by value: what has an address is loaded anew
+// for every entry.)
+__device__ __noinline__ Row distribution(Shared& sh, const Part p, const Source s, const double temperature, const double top_p, const int V, const int bits, int turn) {
+  Row r;
+  r.good = false;
+  float some;
+  const unsigned long long top = row_top<false>(sh, p, s, turn, static_cast<float>(kLog2e / temperature), some);
+  r.turn = turn;
+  if (!is_distribution(top)) return r;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const float m = unordered(static_cast<uint32_t>(top >> 32));
+  Scale sc = scale_of(m, temperature);
+  const bool in_fp32 = sc.fine > -INFINITY;
+  const double whole = fmax(1.0, 0.99 * some);  // small is what is below 2^-16 of that
+  if (in_fp32) sc.fine += static_cast<float>(log(whole) * temperature);
+  // Candidates, in the order of their places: what is not small, and what probably belongs to the nucleus (an entry at its border weighs many times the mean of those outside;
+  // sixteen times in most rows).
+  float bound = sc.fine;
+  if (top_p < 1.0) bound = fminf(bound, static_cast<float>(static_cast<double>(m) + log((1.0 - top_p) * whole * 16.0 / V) * temperature));
+  bound = fmaxf(bound, sc.cut);  // (the same number in all CTAs)
+  int held = 0;
+  double sum = 0.0;
+  const Pairs small(sc);
+  if (in_fp32)
+    each4(p, s, [&](int i, float4 x) {
+      float2 u = small(x.x, x.y), v = small(x.z, x.w);
+      if (__any_sync(0xffffffffu, max3(fmaxf(x.x, x.y), x.z, x.w) >= bound)) {
+        const float xs[4] = {x.x, x.y, x.z, x.w};
+        u.x = x.x >= bound ? 0.0f : u.x, u.y = x.y >= bound ? 0.0f : u.y, v.x = x.z >= bound ? 0.0f : v.x, v.y = x.w >= bound ? 0.0f : v.y;
+        int is = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) is |= xs[k] >= bound ? 1 << k : 0;
+        const uint32_t front = (1u << lane) - 1, any = __ballot_sync(0xffffffffu, is != 0);
+        int at = held + __popc(any & front), all = __popc(any);
+        if (__any_sync(0xffffffffu, (is & (is - 1)) != 0)) {  // (a lane with several)
+          const int count = __popc(is);
+          const uint32_t b0 = __ballot_sync(0xffffffffu, count & 1), b1 = __ballot_sync(0xffffffffu, count & 2), b2 = __ballot_sync(0xffffffffu, count & 4);
+          at = held + __popc(b0 & front) + 2 * __popc(b1 & front) + 4 * __popc(b2 & front);
+          all = __popc(b0) + 2 * __popc(b1) + 4 * __popc(b2);
+        }
+        for (; is != 0; is &= is - 1, ++at) {
+          const int k = __ffs(is) - 1;
+          if (at < kHeld) sh.held[warp][at] = Candidate{k == 0 ? x.x : k == 1 ? x.y : k == 2 ? x.z : x.w, i + k};
+        }
+        held += all;
+      }
+      sum += static_cast<double>((u.x + u.y) + (v.x + v.y));
+    });
+  const bool over = !in_fp32 || held > kHeld;
+  held = min(held, kHeld);
+  if (lane == 0) sh.held_count[warp] = held;
+  __syncwarp();
+  double part = 0.0;
+  for (int i = lane; i < held; i += 32) part += weight(sh.table, sc, sh.held[warp][i].x);
+  r.mass = share_sums(sh, p, turn, sum + part, over, &part);
+  r.listed = part == part;  // (NaN: some warp had no room)
+  r.held = false;
+  r.bound = bound;
+  auto sum_of = [&](int, float4 x) { return weights_sum(sh.table, sc, small, x); };
+  if (!r.listed) r.mass = row_mass(sh, p, s, turn, sum_of);
   if (top_p < 1.0) {
-    r.least = nucleus(sh, p, r.s, static_cast<uint32_t>(top >> 32), r.mass, top_p, temperature, V, bits, turn);
-    r.mass = row_mass(sh, p, turn, [&](int i) { return kept_weight(sh.table, r, p.xs[i]); });
+    const uint32_t top_key = static_cast<uint32_t>(top >> 32);
+    r.held = r.listed && part > top_p * r.mass * (1.0 + 1e-9);  // the border lies among the candidates
+    if (r.held) {
+      sc.cut = nucleus(sh, p, sc, top_key, r.mass, top_p, temperature, V, bits, [&](auto f) {
+        for (int i = lane; i < sh.held_count[warp]; i += 32) f(sh.held[warp][i].x);
+      });
+      r.mass = held_mass(sh, p, turn, [&](const Candidate& c) { return weight(sh.table, sc, c.x); });
+    } else {
+      r.listed = false;
+      sc.cut = nucleus(sh, p, sc, top_key, r.mass, top_p, temperature, V, bits, [&](auto f) { each4(p, s, [&](int, float4 x) { f(x.x), f(x.y), f(x.z), f(x.w); }); });
+      r.mass = row_mass(sh, p, s, turn, sum_of);
+    }
   }
-  return true;
+  r.s = sc;
+  r.good = true;
+  r.turn = turn;
+  return r;
 }
 
 PG_DEVINL float unit_number(float u) { return fminf(fmaxf(u, 0.0f), 1.0f - 0x1p-24f); }  // (a NaN is 0)
 
-// first row behind `v` (exclusive) from `i` on whose parent is v; n where there is none.  Whole warps.
-PG_DEVINL int next_child(const int* parents, int v, int i, int n) {
-  for (int i0 = i; i0 < n; i0 += 32) {
-    const int j = i0 + threadIdx.x % 32;
-    const uint32_t is = __ballot_sync(0xffffffffu, j < n && parents[j] == v);
-    if (is) return i0 + __ffs(is) - 1;
+struct Family {  // parents and tokens of an entry; those of the 32 rows behind v lie in the lanes
+  const int *parents, *tokens;
+  int v, n, up, token;
+  PG_DEVINL void look() {
+    const int j = v + 1 + threadIdx.x % 32;
+    up = j < n ? parents[j] : -1;
+    token = j < n ? tokens[j] : 0;
   }
-  return n;
-}
+  // first row from `i` on (i > v) whose parent is v, n where there is none; x: its token.  Whole warps.
+  PG_DEVINL int child(int i, int& x) const {
+    for (int i0 = i; i0 < n;) {
+      const int base = i0 <= v + 32 ? v + 1 : i0, j = base + threadIdx.x % 32;
+      const bool near = base == v + 1;
+      const uint32_t is = __ballot_sync(0xffffffffu, j >= i0 && j < n && (near ? up : parents[j]) == v);
+      if (is) {
+        const int l = __ffs(is) - 1;
+        x = near ? __shfl_sync(0xffffffffu, token, l) : tokens[base + l];
+        return base + l;
+      }
+      i0 = base + 32;
+    }
+    return n;
+  }
+  PG_DEVINL int with(int t) const {  // first child that carries t, or n
+    int x = 0;
+    for (int i = child(v + 1, x); i < n; i = child(i + 1, x))
+      if (x == t) return i;
+    return n;
+  }
+};
 
-// first child of v that carries `token`, or n
-PG_DEVINL int child_with(const int* parents, const int* tokens, int v, int n, int token) {
-  for (int i = next_child(parents, v, v + 1, n); i < n; i = next_child(parents, v, i + 1, n))
-    if (tokens[i] == token) return i;
-  return n;
-}
-
-__global__ void __launch_bounds__(kThreads) verify_kernel(const PgVerify a, int share, int bits) {
+__global__ void __launch_bounds__(kThreads, kPerSm) verify_kernel(const PgVerify a, int share, int bits, int look) {
   extern __shared__ __align__(16) char raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw);
-  float* xs = reinterpret_cast<float*>(raw + sizeof(Shared));
   uint32_t ranks;
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ranks));
   const int rank = pg::cluster_ctarank(), item = blockIdx.x / ranks, tid = threadIdx.x;
-  if (tid < kTable) sh.table[tid] = exp2(static_cast<double>(tid) / kTable);
   const int v = item / a.entries, e = item % a.entries;  // the entries' first rows come first
   const int n = a.n[e];
   const long long row0 = a.row0[e], row = row0 + v;
   bool live = v < n && row0 >= 0 && row0 + n <= a.rows;
   int* outcome = a.outcome + row0;
-  const int* parents = a.parents + row0;
-  const int* tokens = a.tokens + row0;
+  Family fam;
+  fam.parents = a.parents + row0, fam.tokens = a.tokens + row0, fam.v = v, fam.n = n;
   if (live && v > 0) {
-    if (rank == 0 && tid < 32) {  // one look for all: what the parent decides may come in between
-      int said = 0;
-      if (tid == 0) {
-        const int up = parents[v];
-        said = up >= 0 && up < v ? load_relaxed(outcome + up) : kDead;
+    if (look) {
+      if (rank == 0 && tid < 32) {  // one look for all: what the parent decides may come in between
+        int said = 0;
+        if (tid == 0) {
+          const int up = fam.parents[v];
+          said = up >= 0 && up < v ? load_relaxed(outcome + up) : kDead;
+        }
+        said = __shfl_sync(0xffffffffu, said, 0);
+        if (tid < static_cast<int>(ranks)) put32(&sh.state, tid, said == 0 || said == v);
       }
-      said = __shfl_sync(0xffffffffu, said, 0);
-      if (tid < static_cast<int>(ranks)) put32(&sh.state, tid, said == 0 || said == v);
+      pg::cluster_sync_all();
+      live = sh.state != 0;
+      if (!live && rank == 0 && tid == 0) outcome[v] = kDead;
+    } else {
+      const int up = fam.parents[v];
+      live = up >= 0 && up < v;
     }
-    pg::cluster_sync_all();
-    live = sh.state != 0;
-    if (!live && rank == 0 && tid == 0) outcome[v] = kDead;
   }
   if (live) {
     Part p;
-    p.xs = xs, p.rank = rank, p.ranks = ranks;
+    p.rank = rank, p.ranks = ranks;
     p.lo = min(rank * share, a.V);
     p.n = min(share, a.V - p.lo);
-    p.seg = (share + kThreads - 1) / kThreads * 32;
-    int turn = 0, to = 0;  // to: the child, or -2 - token where the walk ends
-    const float* logits = a.logits + row * a.ld;
-    auto wait = [&]() {
-      pg::cp_async_wait<0>();
-      __syncthreads();
-    };
+    p.seg = (share + kWarps * kRun - 1) / (kWarps * kRun) * kRun;
+    int turn = 0, to = 0, x = 0;  // to: the child, or -2 - token where the walk ends
+    const float *logits = a.logits + row * a.ld, *draft = a.draft + row * a.draft_ld;
+    const Source target(logits, p.lo);
+    fam.look();
+    if (tid < kTable) sh.table[tid] = exp2(static_cast<double>(tid) / kTable);
+    __syncthreads();
     if (a.uniforms == nullptr) {
-      load_share(p, logits);
-      wait();
-      const unsigned long long top = row_top(sh, p, turn);
+      float whole;
+      const unsigned long long top = row_top<true>(sh, p, target, turn, 0.0f, whole);
       const int token = is_distribution(top) ? static_cast<int>(~static_cast<uint32_t>(top)) : -1;
-      const int child = token >= 0 ? child_with(parents, tokens, v, n, token) : n;
-      to = child < n ? child : -2 - token;
+      const int next = token >= 0 ? fam.with(token) : n;
+      to = next < n ? next : -2 - token;
     } else {
       const float u = unit_number(a.uniforms[2 * row + 1]);
-      int child = a.draft != nullptr ? next_child(parents, v, v + 1, n) : n;
+      const Source other(draft, p.lo);
+      int child = a.draft != nullptr ? fam.child(v + 1, x) : n;
       Row t, q;
       bool good = true;
-      const float* draft = a.draft + row * a.draft_ld;
       if (child < n) {
-        load_share(p, draft);
-        wait();
-        good = distribution(sh, p, a.draft_temperature, a.draft_top_p, a.V, bits, q, turn);
-        __syncthreads();  // (xs has been read)
+        q = distribution(sh, p, other, a.draft_temperature, a.draft_top_p, a.V, bits, turn);
+        good = q.good;
+        turn = q.turn;
       }
       if (good) {
-        load_share(p, logits);
-        wait();
-        good = distribution(sh, p, a.temperature, a.top_p, a.V, bits, t, turn);
+        t = distribution(sh, p, target, a.temperature, a.top_p, a.V, bits, turn);
+        good = t.good;
+        turn = t.turn;
       }
       if (!good) {
         to = -1;
       } else {
-        double c = 0.0, left = 1.0;
+        double c = 0.0, left = 1.0, pf = 0.0, qf = 0.0;
+        // max(p - c q, 0); both products rounded alike, so that equal ones leave nothing
+        auto rest_of = [&](double wt, double wq) { return fmax(__dsub_rn(__dmul_rn(pf, wt), __dmul_rn(qf, wq)), 0.0); };
+        auto rest4 = [&](int i, float4 y, double (&w)[4]) {
+          const float4 z = other.four(i, p.n);
+          w[0] = rest_of(weight(sh.table, t.s, y.x), weight(sh.table, q.s, z.x)), w[1] = rest_of(weight(sh.table, t.s, y.y), weight(sh.table, q.s, z.y));
+          w[2] = rest_of(weight(sh.table, t.s, y.z), weight(sh.table, q.s, z.z)), w[3] = rest_of(weight(sh.table, t.s, y.w), weight(sh.table, q.s, z.w));
+        };
+        const bool quick = child < n && t.listed && q.s.fine > -INFINITY;
+        const Pairs small_t(t.s), small_q(child < n ? q.s : t.s);
+        float pf0 = 0.0f, pf1 = 0.0f, qf0 = 0.0f, qf1 = 0.0f;  // the factors in two parts
+        auto rest_sum = [&](int i, float4 y) {
+          if (!quick) {
+            double w[4];
+            rest4(i, y, w);
+            return (w[0] + w[1]) + (w[2] + w[3]);
+          }
+          const float4 z = other.four(i, p.n);  // (what is not small is added from the candidates; what p has not is not there, whatever q has)
+          const float2 t0 = small_t(y.x, y.y), t1 = small_t(y.z, y.w), q0 = small_q(z.x, z.y), q1 = small_q(z.z, z.w);
+          const float ys[4] = {y.x, y.y, y.z, y.w}, zs[4] = {z.x, z.y, z.z, z.w}, wt[4] = {t0.x, t0.y, t1.x, t1.y}, wq[4] = {q0.x, q0.y, q1.x, q1.y};
+          float w = 0.0f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float b = zs[k] >= q.s.cut ? wq[k] : 0.0f;
+            const float left_over = __fsub_rn(fmaf(wt[k], pf0, __fmul_rn(wt[k], pf1)), fmaf(b, qf0, __fmul_rn(b, qf1)));
+            w += ys[k] < t.bound && ys[k] >= t.s.cut ? fmaxf(left_over, 0.0f) : 0.0f;
+          }
+          return static_cast<double>(w);
+        };
+        auto rest1 = [&](const Candidate& k) { return k.x >= t.s.cut ? rest_of(weight(sh.table, t.s, k.x), weight(sh.table, q.s, other.x[k.at])) : 0.0; };
+        auto rest_mass = [&]() {
+          double sum = 0.0;
+          each4(p, target, [&](int i, float4 y) { sum += rest_sum(i, y); });
+          if (quick)
+            for (int i = tid % 32; i < sh.held_count[tid / 32]; i += 32) sum += rest1(sh.held[tid / 32][i]);
+          return share_sums(sh, p, turn, sum);
+        };
         while (child < n) {
-          const int x = tokens[child];
           if (x >= 0 && x < a.V) {  // (what is no token was drawn from nothing: it takes nothing away)
-            const double pt = kept_weight(sh.table, t, logits[x]) / t.mass, qt = kept_weight(sh.table, q, draft[x]) / q.mass;
+            const double pt = weight(sh.table, t.s, logits[x]) / t.mass, qt = weight(sh.table, q.s, draft[x]) / q.mass;
             const bool stays = static_cast<double>(unit_number(a.uniforms[2 * (row0 + child)])) * qt * left < __dsub_rn(pt, __dmul_rn(c, qt));
             if (stays) break;
             c += left;
-            const double pf = 1.0 / t.mass, qf = c / q.mass;
-            left = row_mass(sh, p, turn, [&](int i) { return rest_weight(sh.table, t, pf, xs[i], q, qf, draft[p.lo + i]); });
+            pf = 1.0 / t.mass, qf = c / q.mass;
+            pf0 = static_cast<float>(pf), pf1 = static_cast<float>(pf - pf0), qf0 = static_cast<float>(qf), qf1 = static_cast<float>(qf - qf0);
+            left = t.held ? held_mass(sh, p, turn, rest1) : rest_mass();
             if (!(left > 0.0)) break;
           }
-          child = next_child(parents, v, child + 1, n);
+          child = fam.child(child + 1, x);
         }
         if (child < n && left > 0.0) {
           to = child;
         } else {
           int token;
           if (c > 0.0 && left > 0.0) {
-            const double pf = 1.0 / t.mass, qf = c / q.mass;
-            token = row_draw(sh, p, turn, left, u, [&](int i) { return rest_weight(sh.table, t, pf, xs[i], q, qf, draft[p.lo + i]); });
+            token = t.held ? held_draw(sh, p, turn, left, u, rest1) : row_draw(sh, p, target, turn, left, u, rest4);
           } else {
-            auto f = [&](int i) { return kept_weight(sh.table, t, xs[i]); };
-            if (c > 0.0) t.mass = row_mass(sh, p, turn, f);
-            token = row_draw(sh, p, turn, t.mass, u, f);
+            auto one = [&](const Candidate& k) { return weight(sh.table, t.s, k.x); };
+            auto four = [&](int, float4 y, double (&w)[4]) {
+              w[0] = weight(sh.table, t.s, y.x), w[1] = weight(sh.table, t.s, y.y), w[2] = weight(sh.table, t.s, y.z), w[3] = weight(sh.table, t.s, y.w);
+            };
+            if (c > 0.0) t.mass = t.held ? held_mass(sh, p, turn, one) : row_mass(sh, p, target, turn, [&](int, float4 y) { return weights_sum(sh.table, t.s, small_t, y); });
+            token = t.held ? held_draw(sh, p, turn, t.mass, u, one) : row_draw(sh, p, target, turn, t.mass, u, four);
           }
-          child = a.draft == nullptr ? child_with(parents, tokens, v, n, token) : n;
-          to = child < n ? child : -2 - token;
+          const int next = a.draft == nullptr ? fam.with(token) : n;
+          to = next < n ? next : -2 - token;
         }
       }
     }
@@ -416,8 +802,9 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const PgVerify a, int 
     }
     __syncthreads();
     if (sh.last) {
-      const bool fits = a.rows <= share;
-      int* held = reinterpret_cast<int*>(xs);
+      constexpr int kMost = sizeof(sh.held) / sizeof(int);  // (the candidates are not needed any more)
+      const bool fits = a.rows <= kMost;
+      int* held = reinterpret_cast<int*>(sh.held);
       if (fits)
         for (int i = tid; i < a.rows; i += kThreads) held[i] = load_relaxed(a.outcome + i);
       __syncthreads();
@@ -453,21 +840,23 @@ extern "C" int pg_verify_drafts(const PgVerify* args, void* stream) {
   auto sound = [](double temperature, double top_p) { return temperature > 0.0 && temperature < INFINITY && kLog2e / temperature < 1e30 && top_p >= 0.0 && top_p <= 1.0; };
   if (a.logits == nullptr || a.tokens == nullptr || a.parents == nullptr || a.row0 == nullptr || a.n == nullptr || a.path == nullptr || a.kept == nullptr || a.next == nullptr ||
       a.outcome == nullptr || a.entries <= 0 || a.rows <= 0 || a.max_n <= 0 || a.V <= 0 || a.ld < a.V || a.path_ld < a.max_n || (a.draft != nullptr && (a.draft_ld < a.V || a.uniforms == nullptr)) ||
-      !sound(a.temperature, a.top_p) || (a.draft != nullptr && !sound(a.draft_temperature, a.draft_top_p)) || a.V > kRanks * kMostShare)
+      !sound(a.temperature, a.top_p) || (a.draft != nullptr && !sound(a.draft_temperature, a.draft_top_p)) || a.V > 0x7fffff00 / 2)
     return PG_ERR_ARG;
   const long long items = static_cast<long long>(a.entries) * a.max_n;
+  // CTAs that share a row: so many that a warp's candidates have room, and more while all of them stay within nine an SM (5 rows of 257216 with 4, 8, 16 CTAs: 46, 37, 35 us; 240 of them
+  // beside a draft 298, 384, 542; 48 trees of 32000 with 1, 2, 4: 132, 118, 140).
   int ranks = 1;
-  while (ranks < kRanks && (a.V + ranks - 1) / ranks > kShare) ranks *= 2;
-  while (ranks < kRanks && items * ranks * 2 <= pg::num_sms() && a.V / (ranks * 2) >= 4 * kThreads) ranks *= 2;  // few rows: more CTAs for each
+  while (ranks < kRanks && a.V / ranks > 65536) ranks *= 2;
+  while (ranks < kRanks && items * ranks * 2 <= 9LL * pg::num_sms() && a.V / (ranks * 2) >= 4 * kThreads) ranks *= 2;
   if (items * ranks > 0x7fffffff) return PG_ERR_ARG;
   const int share = ((a.V + ranks - 1) / ranks + 3) / 4 * 4;
   int bits = 62;
   while ((1ll << (62 - bits)) < a.V) --bits;  // V weights of at most 1 stay below 2^62
-  const size_t smem = sizeof(Shared) + sizeof(float) * share;
+  const int look = items * ranks > 2 * pg::num_sms();  // (all rows at once: nothing is decided when they begin)
   static bool configured[pg::kMaxDevices] = {};
   bool& done = configured[pg::current_device()];
   if (!done) {
-    if (cudaFuncSetAttribute(verify_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared) + 4 * kMostShare) != cudaSuccess ||
+    if (cudaFuncSetAttribute(verify_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared)) != cudaSuccess ||
         cudaFuncSetAttribute(verify_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
       cudaGetLastError();
       return PG_ERR_CUDA;
@@ -479,7 +868,7 @@ extern "C" int pg_verify_drafts(const PgVerify* args, void* stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(items * ranks));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = sizeof(Shared);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -488,5 +877,5 @@ extern "C" int pg_verify_drafts(const PgVerify* args, void* stream) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   pg_count_launch(1);
-  return cudaLaunchKernelEx(&cfg, verify_kernel, a, share, bits) == cudaSuccess ? PG_OK : PG_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, verify_kernel, a, share, bits, look) == cudaSuccess ? PG_OK : PG_ERR_CUDA;
 }

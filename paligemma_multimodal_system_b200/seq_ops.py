@@ -902,9 +902,6 @@ def adapter_add(x: torch.Tensor, y: torch.Tensor, bank: AdapterBank, plan: Adapt
 
 
 # ---- verified drafts -------------------------------------------------------------------------------------------------
-VERIFY_MOST_VOCAB = 16 * 49152  # entries of a row that a cluster of CTAs holds at once
-
-
 def _check_rows_of_logits(logits, b: StepBatch, what):
     if logits.dim() != 2 or logits.dtype != torch.float32 or logits.stride(1) != 1 or not logits.is_cuda or logits.shape[0] != b.T:
         raise ValueError(f"{what} are fp32 [rows of the step, vocab] on the device, entries of a row side by side: got {tuple(logits.shape)} of {logits.dtype} for {b.T} rows")
@@ -925,8 +922,8 @@ def verify_drafts(logits: torch.Tensor, b: StepBatch, uniforms: Optional[torch.T
     the walk with next -1."""
     _check_rows_of_logits(logits, b, "logits")
     V = logits.shape[1]
-    if not 0 < V <= VERIFY_MOST_VOCAB:
-        raise ValueError(f"rows of 1 .. {VERIFY_MOST_VOCAB} entries: got {V}")
+    if not 0 < V < 1 << 30:
+        raise ValueError(f"rows of 1 .. 2^30 - 1 entries: got {V}")
     if b.parents is None or b.parents.dtype != torch.int32 or b.parents.shape != (b.T,) or not b.parents.is_contiguous():
         raise ValueError("the step's parents (RequestBatch) are int32 [rows]")
     if uniforms is not None and (uniforms.dtype != torch.float32 or uniforms.shape != (b.T, 2) or not uniforms.is_contiguous()):

@@ -51,12 +51,6 @@ def test_what_is_refused(call):
         seq_ops.verify_drafts(*call())
 
 
-def test_rows_wider_than_a_cluster_holds_are_refused():
-    wide = torch.zeros(1, 1).expand(3, seq_ops.VERIFY_MOST_VOCAB + 1).as_subclass(_OnDevice)
-    with pytest.raises(ValueError):
-        seq_ops.verify_drafts(wide, step())
-
-
 def test_a_step_of_drafts_keeps_what_requests_have_of_their_own():
     import dataclasses
     b = step()
