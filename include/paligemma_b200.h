@@ -842,8 +842,9 @@ typedef struct {
 int pg_verify_drafts(const PgVerify* a, void* stream);
 
 /* Low-rank adapters of a step's rows beside a shared projection: out[t, f] = y[t, f] + gain * scale[s] * sum_r b[s][f, r] (sum_k a[s][part(f) * rank + r, k] x[t, k])
- * for rows of adapter s.  The columns are `parts` runs of part_cols; each has rank rows of a for itself.  a: [slots, parts * rank, K8], b: [slots, F, rank], dense, in x's
- * type, rank a multiple of 8 up to 128, K8 = K rounded up to 8 (zeros behind K).  rows / tiles: the plan, tiles of up to tile_rows (16 or 64) rows
+ * for rows of adapter s.  The columns are `parts` runs of part_cols; each has rank rows of a for itself.  rank: a multiple of 8 up to
+ * 128.  b: [slots, F, rank] in x's type.  a, fp32: [slots, parts * rank, K8], K8 = K rounded up to 8; bf16: [slots, ceil(K / 64), parts * rank rounded up to 16, 8, 8], element (n, k) at
+ * [k / 64, n, (k / 8 % 8) ^ (n % 8), k % 8].  Zeros where there is no k or no row.  rows / tiles: the plan, tiles of up to tile_rows (16 or 128) rows
  * (adapter, first, count) of one adapter, rows[first ..] their numbers; adapter -1: rows without one, which are copied where out is not y. */
 typedef struct {
   const void *x, *y, *a, *b;

@@ -1,6 +1,6 @@
 // Low-rank adapters of many requests beside a shared projection: out[t] = y[t] + gain scale[s] B_s (A_s x[t]) for the rows t of adapter s.
 //
-// A tile is up to 16 or 64 rows of one adapter, gathered by number, so decoded tokens of requests that share an adapter and the rows of a prompt are one thing.  A
+// A tile is up to 16 or 128 rows of one adapter, gathered by number, so decoded tokens of requests that share an adapter and the rows of a prompt are one thing.  A
 // cluster of CTAs takes a tile in one launch: each CTA multiplies a share of K (v = A x, rank columns), the shares are added through distributed shared memory in
 // a fixed order, and each CTA then makes a share of the columns (B v) and adds it to y.  v stays in shared memory.
 //
@@ -39,31 +39,58 @@ PG_DEVINL void split8(const float (&f)[8], uint4 (&t)[TERMS]) {
   }
 }
 
-// Eight elements k .. k + 7 of a row as bf16 terms; zeros from `end` on.  vec: 16-byte pieces start on 16-byte boundaries and `end` is a multiple of 8.
+// 16 bytes where `there`, zeros else, without a branch: what is merged behind a branch is waited for there, and the loads come one after another
+PG_DEVINL uint4 ld16(const void* p, bool there) {
+  uint4 v;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.u32 q, %5, 0;\n\t"
+      "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+      "@q ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}\n"
+      : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+      : "l"(p), "r"(static_cast<uint32_t>(there)));
+  return v;
+}
+
+// Eight elements k .. k + 7 of a row as they are; zeros from `end` on.  vec: rows start on 16-byte boundaries.
 template <bool F32>
-PG_DEVINL void load8(const void* row, int k, int end, bool vec, uint4 (&t)[F32 ? 3 : 1]) {
-  if constexpr (F32) {
-    const float* p = static_cast<const float*>(row) + k;
-    float f[8];
-    if (vec && k + 8 <= end) {
-      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-      f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = k + i < end ? p[i] : 0.f;
-    }
-    split8<3>(f, t);
-  } else {
-    const uint16_t* p = static_cast<const uint16_t*>(row) + k;
-    if (vec && k + 8 <= end) {
-      t[0] = *reinterpret_cast<const uint4*>(p);
-    } else {
+struct Raw8 {
+  uint4 v[F32 ? 2 : 1];
+  PG_DEVINL void load(const void* row, int k, int end, bool vec) {
+    constexpr int kSize = F32 ? 4 : 2;
+    const char* p = static_cast<const char*>(row) + static_cast<long long>(k) * kSize;
+    const bool whole = vec && k + 8 <= end;
+    v[0] = ld16(p, whole);
+    if constexpr (F32) v[1] = ld16(p + 16, whole);
+    if (!whole && k < end) {
       uint32_t h[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) h[i] = k + i < end ? p[i] : 0u;
-      t[0] = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+      for (int i = 0; i < 8; ++i) h[i] = k + i >= end ? 0u : F32 ? reinterpret_cast<const uint32_t*>(p)[i] : reinterpret_cast<const uint16_t*>(p)[i];
+      if constexpr (F32) v[0] = make_uint4(h[0], h[1], h[2], h[3]), v[1] = make_uint4(h[4], h[5], h[6], h[7]);
+      else v[0] = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
     }
   }
+  PG_DEVINL void terms(uint4 (&t)[F32 ? 3 : 1]) const {
+    if constexpr (F32) {
+      const float f[8] = {__uint_as_float(v[0].x), __uint_as_float(v[0].y), __uint_as_float(v[0].z), __uint_as_float(v[0].w),
+                          __uint_as_float(v[1].x), __uint_as_float(v[1].y), __uint_as_float(v[1].z), __uint_as_float(v[1].w)};
+      split8<3>(f, t);
+    } else {
+      t[0] = v[0];
+    }
+  }
+};
+
+// Where elements k .. k + 7 of row n of an adapter's a lie: bf16 in blocks of 64 k's, 128-byte rows whose 16-byte pieces are exchanged by the row's last bits (the matrix unit's operand
+// layout: a block is copied as it is); fp32 row by row.
+template <bool F32>
+PG_DEVINL const char* down_at(const char* a, int rows16, int K8, int n, int k) {
+  if constexpr (F32) return a + (static_cast<long long>(n) * K8 + k) * 4;
+  else return a + (static_cast<long long>(k / 64) * rows16 + n) * 128 + ((k / 8 % 8 ^ (n & 7)) * 16);
+}
+template <bool F32>
+PG_DEVINL long long down_bytes(int R, int K) {
+  return F32 ? static_cast<long long>(R) * ((K + 7) / 8 * 8) * 4 : static_cast<long long>((R + 15) / 16 * 16) * ((K + 63) / 64) * 128;
 }
 
 // d += (rows g and g + 8: 32 k's) x (column g: 32 k's)
@@ -82,7 +109,7 @@ PG_DEVINL float4 get_f4(const float* p, int rank) {
   uint32_t there;
   float4 v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(pg::smem_u32(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(there) : "memory");
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(there));
   return v;
 }
 
@@ -111,28 +138,59 @@ PG_DEVINL Tile tile_of(const PgAdapter& a, int item, int subs, int (&row_of)[M])
   return t;
 }
 
-// Rows without an adapter
+// Rows without an adapter: pieces of 16 bytes (or one element), four under way
+template <typename U>
+PG_DEVINL void copy_pieces(const PgAdapter& a, const int* row_of, int count, int rank, int ranks, int bytes, int element) {
+  const int per_row = bytes / static_cast<int>(sizeof(U)), all = count * per_row;
+  for (int i0 = rank * kThreads + threadIdx.x; i0 < all; i0 += 4 * ranks * kThreads) {
+    U v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = i0 + k * ranks * kThreads, t = i < all ? row_of[i / per_row] : -1;
+      if (t >= 0) v[k] = reinterpret_cast<const U*>(static_cast<const char*>(a.y) + t * a.ldy * element)[i % per_row];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = i0 + k * ranks * kThreads, t = i < all ? row_of[i / per_row] : -1;
+      if (t >= 0) reinterpret_cast<U*>(static_cast<char*>(a.out) + t * a.ldo * element)[i % per_row] = v[k];
+    }
+  }
+}
 template <bool OUT32>
 PG_DEVINL void copy_rows(const PgAdapter& a, const int* row_of, int count, int rank, int ranks, bool vec) {
   constexpr int kOut = OUT32 ? 4 : 2;
-  const int tid = threadIdx.x, bytes = a.F * kOut;
-  for (int i = 0; i < count; ++i) {
-    const int t = row_of[i];
-    if (t < 0) continue;
-    const char* from = static_cast<const char*>(a.y) + t * a.ldy * kOut;
-    char* to = static_cast<char*>(a.out) + t * a.ldo * kOut;
-    const int step = vec ? 16 : 2, whole = bytes / step * step;
-    for (int c = (rank * kThreads + tid) * step; c < whole; c += ranks * kThreads * step) {
-      if (vec) *reinterpret_cast<uint4*>(to + c) = *reinterpret_cast<const uint4*>(from + c);
-      else *reinterpret_cast<uint16_t*>(to + c) = *reinterpret_cast<const uint16_t*>(from + c);
-    }
-    for (int c = whole + 2 * tid; rank == 0 && c < bytes; c += 2 * kThreads) *reinterpret_cast<uint16_t*>(to + c) = *reinterpret_cast<const uint16_t*>(from + c);
+  if (vec && a.F * kOut % 16 == 0) copy_pieces<uint4>(a, row_of, count, rank, ranks, a.F * kOut, kOut);
+  else copy_pieces<uint16_t>(a, row_of, count, rank, ranks, a.F * kOut, kOut);
+}
+
+// Eight numbers of v, the CTAs' shares added in their order; N of them at once, all CTAs' asked for together
+template <int N>
+PG_DEVINL void joined8(const float* (&from)[N], int ranks, float (&f)[N][8]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[n][i] = 0.0f;
+  for (int p = 0; p < ranks; p += 2) {
+    float4 v[2][N][2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) v[k][n][h] = get_f4(from[n] + 4 * h, min(p + k, ranks - 1));
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (p + k < ranks)
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) f[n][4 * h] += v[k][n][h].x, f[n][4 * h + 1] += v[k][n][h].y, f[n][4 * h + 2] += v[k][n][h].z, f[n][4 * h + 3] += v[k][n][h].w;
   }
 }
 
-// The CTAs' shares of v (partial, [SHARES] one behind another in each) together, in a fixed order; v as bf16 terms, every part's ranks rounded up to 32
+// v as bf16 terms, every part's ranks rounded up to 32
 template <int M, int VT>
-PG_DEVINL void join_shares(const PgAdapter& a, const Layout& lay, const float* partial, int shares, uint16_t* vt, int count, int ranks) {
+PG_DEVINL void join_shares(const PgAdapter& a, const Layout& lay, const float* partial, uint16_t* vt, int count, int ranks) {
   const int per_row = a.parts * lay.rank32 / 8;
   for (int i = threadIdx.x; i < M * per_row; i += kThreads) {
     const int m = i / per_row, c = i % per_row * 8, part = c / lay.rank32, r = c % lay.rank32;
@@ -140,16 +198,10 @@ PG_DEVINL void join_shares(const PgAdapter& a, const Layout& lay, const float* p
 #pragma unroll
     for (int k = 0; k < VT; ++k) t[k] = zero4();
     if (m < count && r < a.rank) {
-      float f[8] = {};
-      for (int w = 0; w < shares; ++w) {
-        const float* from = partial + (w * M + m) * lay.partial_ld + part * a.rank + r;
-#pragma unroll 4
-        for (int p = 0; p < ranks; ++p) {
-          const float4 lo = get_f4(from, p), hi = get_f4(from + 4, p);
-          f[0] += lo.x, f[1] += lo.y, f[2] += lo.z, f[3] += lo.w, f[4] += hi.x, f[5] += hi.y, f[6] += hi.z, f[7] += hi.w;
-        }
-      }
-      split8<VT>(f, t);
+      const float* from[1] = {partial + m * lay.partial_ld + part * a.rank + r};
+      float f[1][8];
+      joined8(from, ranks, f);
+      split8<VT>(f[0], t);
     }
 #pragma unroll
     for (int k = 0; k < VT; ++k) *reinterpret_cast<uint4*>(vt + (k * M + m) * lay.v_ld + c) = t[k];
@@ -160,27 +212,17 @@ PG_DEVINL void join_shares(const PgAdapter& a, const Layout& lay, const float* p
 template <bool OUT32>
 struct Eight {
   uint4 y[OUT32 ? 2 : 1];
-  PG_DEVINL void load(const void* base, long long at, int n, bool vec) {
-    if constexpr (OUT32) {
-      const float* p = static_cast<const float*>(base) + at;
-      if (vec && n >= 8) {
-        y[0] = reinterpret_cast<const uint4*>(p)[0], y[1] = reinterpret_cast<const uint4*>(p)[1];
-      } else {
-        uint32_t w[8];
+  PG_DEVINL void load(const void* base, long long at, int n, bool vec, bool there) {
+    const char* p = static_cast<const char*>(base) + at * (OUT32 ? 4 : 2);
+    const bool whole = there && vec && n >= 8;
+    y[0] = ld16(p, whole);
+    if constexpr (OUT32) y[1] = ld16(p + 16, whole);
+    if (there && !whole) {
+      uint32_t w[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) w[k] = k < n ? __float_as_uint(p[k]) : 0u;
-        y[0] = make_uint4(w[0], w[1], w[2], w[3]), y[1] = make_uint4(w[4], w[5], w[6], w[7]);
-      }
-    } else {
-      const uint16_t* p = static_cast<const uint16_t*>(base) + at;
-      if (vec && n >= 8) {
-        y[0] = *reinterpret_cast<const uint4*>(p);
-      } else {
-        uint32_t w[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) w[k] = k < n ? p[k] : 0u;
-        y[0] = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
-      }
+      for (int k = 0; k < 8; ++k) w[k] = k >= n ? 0u : OUT32 ? reinterpret_cast<const uint32_t*>(p)[k] : reinterpret_cast<const uint16_t*>(p)[k];
+      if constexpr (OUT32) y[0] = make_uint4(w[0], w[1], w[2], w[3]), y[1] = make_uint4(w[4], w[5], w[6], w[7]);
+      else y[0] = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
     }
   }
   PG_DEVINL void store(void* base, long long at, int n, bool vec, float factor, const float (&v)[8]) const {
@@ -215,18 +257,18 @@ struct Eight {
   }
 };
 
-// out = y + B v: units of 32 columns, a warp each.  A unit's part of B and of y are asked for before they are needed: the first unit's while v is still made (`start`), and two runs of
-// 32 ranks at once.
-template <int MT, bool IN32, bool OUT32>
+// out = y + B v of 16 rows: units of 32 columns, a warp each.  A unit's part of B (two runs of 32 ranks at once) and of y are asked for before they are needed, the first unit's while v
+// is still made (`start`).
+template <bool IN32, bool OUT32>
 struct Columns {
-  static constexpr int M = 16 * MT, XT = IN32 ? 3 : 1, VT = IN32 || OUT32 ? 3 : 2, H = MT < 2 ? MT : 2, KC = IN32 ? 1 : 2;  // H: row tiles at once
+  static constexpr int M = 16, XT = IN32 ? 3 : 1, VT = IN32 || OUT32 ? 3 : 2, KC = IN32 ? 1 : 2;
   const PgAdapter& a;
   const Layout& lay;
   const int* row_of;
   int who, stride, u, part = 0, col = 0, unit0 = 0, f0 = 0, wide = 0, g, q;
   bool vec;
-  uint4 bf[KC][4][XT];
-  Eight<OUT32> y[H][2];
+  Raw8<IN32> bf[KC][4];
+  Eight<OUT32> y[2];
 
   PG_DEVINL Columns(const PgAdapter& a_, const Layout& lay_, const int* row_of_, int who_, int rank, int ranks, bool vec_)
       : a(a_), lay(lay_), row_of(row_of_), who(who_), stride(ranks * kWarps), u(rank * kWarps + threadIdx.x / 32), g(threadIdx.x % 32 / 4), q(threadIdx.x % 4), vec(vec_) {}
@@ -248,64 +290,55 @@ struct Columns {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int f = g / 2 * 8 + 2 * j + g % 2, r = r0 + 32 * c + 8 * q;
-#pragma unroll
-        for (int i = 0; i < XT; ++i) bf[c][j][i] = zero4();
-        if (f < wide && r < a.rank) load8<IN32>(B + static_cast<long long>(f0 + f) * a.rank * kIn, r, a.rank, true, bf[c][j]);
+        bf[c][j].load(B + static_cast<long long>(f0 + f) * a.rank * kIn, r, f < wide ? a.rank : 0, true);
       }
   }
-  PG_DEVINL void ask_y(int m0) {
+  PG_DEVINL void ask_y() {
 #pragma unroll
-    for (int m = 0; m < H; ++m)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int t = row_of[16 * (m0 + m) + 8 * h + g];
-        if (t >= 0 && 8 * q < wide) y[m][h].load(a.y, t * a.ldy + f0 + 8 * q, wide - 8 * q, vec);
-      }
+    for (int h = 0; h < 2; ++h) {
+      const int t = row_of[8 * h + g];
+      y[h].load(a.y, t * a.ldy + f0 + 8 * q, wide - 8 * q, vec, t >= 0 && 8 * q < wide);
+    }
   }
   PG_DEVINL void start() {
-    if (find()) ask_b(0), ask_y(0);
+    if (find()) ask_b(0), ask_y();
   }
   PG_DEVINL void run(const uint16_t* vt) {
     const float factor = a.gain * a.scale[who];
     for (bool first = true; find(); u += stride, first = false) {
-      if (!first) ask_b(0);
-      for (int m0 = 0; m0 < MT; m0 += H) {
-        if (!first || m0 > 0) ask_y(m0);
-        float acc[H][4][4] = {};
-        for (int r0 = 0; r0 < lay.rank32; r0 += 32 * KC) {
-          if (r0 > 0 || (m0 > 0 && lay.rank32 > 32 * KC)) ask_b(r0);
+      if (!first) ask_b(0), ask_y();
+      float acc[4][4] = {};
+      for (int r0 = 0; r0 < lay.rank32; r0 += 32 * KC) {
+        if (r0 > 0) ask_b(r0);
 #pragma unroll
-          for (int c = 0; c < KC; ++c) {
-            if (r0 + 32 * c >= lay.rank32) break;
+        for (int c = 0; c < KC; ++c) {
+          if (r0 + 32 * c >= lay.rank32) break;
+          const uint16_t* from = vt + g * lay.v_ld + part * lay.rank32 + r0 + 32 * c + 8 * q;
+          uint4 lo[VT], hi[VT];
 #pragma unroll
-            for (int m = 0; m < H; ++m) {
-              const uint16_t* from = vt + (16 * (m0 + m) + g) * lay.v_ld + part * lay.rank32 + r0 + 32 * c + 8 * q;
-              uint4 lo[VT], hi[VT];
+          for (int k = 0; k < VT; ++k) {
+            lo[k] = *reinterpret_cast<const uint4*>(from + k * M * lay.v_ld);
+            hi[k] = *reinterpret_cast<const uint4*>(from + (k * M + 8) * lay.v_ld);
+          }
 #pragma unroll
-              for (int k = 0; k < VT; ++k) {
-                lo[k] = *reinterpret_cast<const uint4*>(from + k * M * lay.v_ld);
-                hi[k] = *reinterpret_cast<const uint4*>(from + (k * M + 8) * lay.v_ld);
-              }
+          for (int j = 0; j < 4; ++j) {
+            uint4 b[XT];
+            bf[c][j].terms(b);
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
+            for (int k = VT - 1; k >= 0; --k)
 #pragma unroll
-                for (int k = VT - 1; k >= 0; --k)
-#pragma unroll
-                  for (int i = (IN32 ? VT - 1 - k : 0); i >= 0; --i) mma32(acc[m][j], lo[k], hi[k], bf[c][j][i]);
-            }
+              for (int i = (IN32 ? VT - 1 - k : 0); i >= 0; --i) mma32(acc[j], lo[k], hi[k], b[i]);
           }
         }
+      }
 #pragma unroll
-        for (int m = 0; m < H; ++m)
+      for (int h = 0; h < 2; ++h) {
+        const int t = row_of[8 * h + g];
+        if (t < 0 || 8 * q >= wide) continue;
+        float v[8];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int t = row_of[16 * (m0 + m) + 8 * h + g];
-            if (t < 0 || 8 * q >= wide) continue;
-            float v[8];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[2 * j] = acc[m][j][2 * h], v[2 * j + 1] = acc[m][j][2 * h + 1];
-            y[m][h].store(a.out, t * a.ldo + f0 + 8 * q, wide - 8 * q, vec, factor, v);
-          }
+        for (int j = 0; j < 4; ++j) v[2 * j] = acc[j][2 * h], v[2 * j + 1] = acc[j][2 * h + 1];
+        y[h].store(a.out, t * a.ldo + f0 + 8 * q, wide - 8 * q, vec, factor, v);
       }
     }
   }
@@ -328,39 +361,41 @@ __global__ void __launch_bounds__(kThreads, 2) adapter_rows_kernel(const PgAdapt
   const int wk = kWarps / wn, kg = warp / wn;
   float* partial = reinterpret_cast<float*>(raw);                                                // [wk][M][partial_ld]
   uint16_t* vt = reinterpret_cast<uint16_t*>(raw + sizeof(float) * wk * M * lay.partial_ld);     // [VT][M][v_ld]
-  Columns<1, IN32, OUT32> columns(a, lay, row_of, tile.who, rank, ranks, y_vec);
+  Columns<IN32, OUT32> columns(a, lay, row_of, tile.who, rank, ranks, y_vec);
   columns.start();
   {
     const int steps = (a.K + 31) / 32, per = (steps + ranks - 1) / ranks, s0 = min(rank * per, steps), s1 = min(s0 + per, steps);
-    const char* A = static_cast<const char*>(a.a) + static_cast<long long>(tile.who) * R * K8 * kIn;
+    const char* A = static_cast<const char*>(a.a) + tile.who * down_bytes<IN32>(R, a.K);
+    const int rows16 = (R + 15) / 16 * 16;
     const char* xrow[2];
+    int x_end[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) xrow[h] = row_of[8 * h + g] >= 0 ? static_cast<const char*>(a.x) + row_of[8 * h + g] * a.ldx * kIn : nullptr;
+    for (int h = 0; h < 2; ++h) {
+      const int t = row_of[8 * h + g];
+      xrow[h] = static_cast<const char*>(a.x) + max(t, 0) * a.ldx * kIn;
+      x_end[h] = t >= 0 ? a.K : 0;
+    }
     for (int base = 0; base < tiles8; base += wn * NW) {
       const int n0 = base + warp % wn * NW;
       float sum[NW][4] = {};
       for (int s = s0 + kg; s < s1; s += wk) {
         const int k = 32 * s + 8 * q;
-        uint4 xf[2][XT], af[NW][XT];
+        Raw8<IN32> xr[2], ar[NW];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 2; ++h) xr[h].load(xrow[h], k, x_end[h], x_vec);
 #pragma unroll
-          for (int i = 0; i < XT; ++i) xf[h][i] = zero4();
-          if (xrow[h] != nullptr && k < a.K) load8<IN32>(xrow[h], k, a.K, x_vec, xf[h]);
-        }
-#pragma unroll
-        for (int j = 0; j < NW; ++j) {
-#pragma unroll
-          for (int i = 0; i < XT; ++i) af[j][i] = zero4();
-          if (n0 + j < tiles8 && k < K8) load8<IN32>(A + static_cast<long long>((n0 + j) * 8 + g) * K8 * kIn, k, K8, true, af[j]);
-        }
+        for (int j = 0; j < NW; ++j) ar[j].load(down_at<IN32>(A, rows16, K8, (n0 + j) * 8 + g, k), 0, n0 + j < tiles8 && k < K8 ? 8 : 0, true);
+        uint4 xf[2][XT];
+        xr[0].terms(xf[0]), xr[1].terms(xf[1]);
 #pragma unroll
         for (int j = 0; j < NW; ++j) {
+          uint4 af[XT];
+          ar[j].terms(af);
           float d[4] = {};
 #pragma unroll
           for (int o = XT - 1; o >= 0; --o)  // the smallest products first
 #pragma unroll
-            for (int i = 0; i <= o; ++i) mma32(d, xf[0][i], xf[1][i], af[j][o - i]);
+            for (int i = 0; i <= o; ++i) mma32(d, xf[0][i], xf[1][i], af[o - i]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) sum[j][i] += d[i];
         }
@@ -386,116 +421,252 @@ __global__ void __launch_bounds__(kThreads, 2) adapter_rows_kernel(const PgAdapt
     }
   }
   pg::cluster_sync_all();
-  join_shares<M, VT>(a, lay, partial, 1, vt, tile.count, ranks);
+  join_shares<M, VT>(a, lay, partial, vt, tile.count, ranks);
   __syncthreads();
   columns.run(vt);
   pg::cluster_sync_all();  // nobody leaves while its share is read
 }
 
-// Tiles of 64 bf16 rows: x and A go through shared memory, three stages of 64 k's, 128-byte rows whose 16-byte pieces are exchanged by the row's last bits; warps two by four.
-constexpr int kStages = 3;
+// Tiles of 128 bf16 rows, both products on the tensor cores with their sums in tensor memory.
+//   v = x A^T        x and A come in stages of 64 k's by asynchronous copies, 128-byte rows whose 16-byte pieces are exchanged by the row's last bits; N = ranks of all parts, up to 256
+//   shares of K      from tensor memory to shared memory, added over the cluster, as bf16 terms into shared memory again (operand layout, 64 ranks a block of 16 KB)
+//   B v              blocks of 128 columns: every term times the same rows of B; y of the next block is under way meanwhile; sums leave through shared memory so that a warp reads and
+//                    writes whole lines of y and out
+// 256 columns of tensor memory for v, two times 128 for the blocks: one CTA an SM.
+constexpr int kStages = 3, kRows = 128, kBlock = 128, kStageLd = 68;  // (68: lanes' rows of 64 numbers lie in different banks)
+struct Plan {                                                       // of shared memory
+  int R16, stage_bytes, v_bytes, v_at, blocks64;                    // v: [parts][blocks of 64 ranks][terms] operands of 16 KB
+};
 template <bool OUT32>
-__global__ void __launch_bounds__(kThreads, OUT32 ? 1 : 2) adapter_tiles_kernel(const PgAdapter a, const Layout lay, int y_vec) {
-  constexpr int M = 64, VT = OUT32 ? 3 : 2;
-  extern __shared__ __align__(16) char raw[];
-  __shared__ int row_of[M];
+__global__ void __launch_bounds__(kThreads, 1) adapter_tensor_kernel(const PgAdapter a, const Layout lay, const Plan plan, int y_vec) {
+  constexpr int VT = OUT32 ? 3 : 2;
+  extern __shared__ char raw_unaligned[];
+  __shared__ int row_of[kRows];
+  __shared__ __align__(8) uint64_t bars[2 * kStages + 2];  // stages read, stages' A there, blocks done
+  __shared__ uint32_t tmem_at;
+  char* raw = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw_unaligned) + 1023) & ~static_cast<uintptr_t>(1023));  // (the same place in every CTA)
   const int ranks = cluster_size(), rank = pg::cluster_ctarank(), item = blockIdx.x / ranks, tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  const Tile tile = tile_of<M>(a, item, 1, row_of);
+  const Tile tile = tile_of<kRows>(a, item, 1, row_of);
   pg::griddep_wait();
   if (tile.count <= 0 || (tile.none && a.out == a.y)) return;  // (the whole cluster)
   if (tile.none) return copy_rows<OUT32>(a, row_of, tile.count, rank, ranks, y_vec);
-  const int R = lay.R, K8 = (a.K + 7) / 8 * 8, blocks = (R + 15) / 16, per_warp = (blocks + 3) / 4, wm = warp % 2, n0 = warp / 2 * per_warp;
-  const int stage_bytes = (M + blocks * 16) * 128;
-  float* partial = reinterpret_cast<float*>(raw);  // (in the stages' place behind the product)
-  uint16_t* vt = reinterpret_cast<uint16_t*>(raw + sizeof(float) * M * lay.partial_ld);
+  const uint32_t base = pg::smem_u32(raw), bar0 = pg::smem_u32(bars);
+  if (warp == 0) {
+    pg::tmem_alloc(pg::smem_u32(&tmem_at), 512);
+    pg::tmem_relinquish();
+  }
+  if (tid == 32) {
+    for (int i = 0; i < 2 * kStages + 2; ++i) pg::mbar_init(bar0 + 8 * i, 1);
+    pg::mbar_fence_init();
+  }
+  pg::tc_fence_before();
+  __syncthreads();
+  pg::tc_fence_after();
+  const uint32_t tmem = tmem_at;
+  const int R = lay.R;
+
+  // ---- this CTA's share of v, into columns 0 .. R of tensor memory --------------------------------------------------------
+  const int chunks = (a.K + 63) / 64, per = (chunks + ranks - 1) / ranks, c0 = min(rank * per, chunks), c1 = min(c0 + per, chunks);
   {
-    const int chunks = (a.K + 63) / 64, per = (chunks + ranks - 1) / ranks, c0 = min(rank * per, chunks), c1 = min(c0 + per, chunks);
-    const char* A = static_cast<const char*>(a.a) + static_cast<long long>(tile.who) * R * K8 * 2;
-    const uint32_t base = pg::smem_u32(raw);
+    const char* A = static_cast<const char*>(a.a) + tile.who * down_bytes<false>(R, a.K);
+    const int down_block = plan.R16 * 128, row0 = tid / 8, piece = tid % 8;  // a thread's piece of rows row0, row0 + 32 ..
+    const char* from[kRows / 32];
+#pragma unroll
+    for (int i = 0; i < kRows / 32; ++i) {
+      const int t = row_of[row0 + 32 * i];
+      from[i] = t >= 0 ? static_cast<const char*>(a.x) + (t * a.ldx + 8 * piece) * 2 : nullptr;
+    }
     auto ask = [&](int c) {
       if (c < c1) {
-        const uint32_t to = base + (c - c0) % kStages * stage_bytes;
-        for (int i = tid; i < (M + blocks * 16) * 8; i += kThreads) {
-          const int row = i / 8, piece = i % 8, k = 64 * c + 8 * piece;
-          const char* from;
-          bool there;
-          if (row < M) {
-            there = row_of[row] >= 0 && k < a.K;
-            from = static_cast<const char*>(a.x) + ((there ? row_of[row] : 0) * a.ldx + (there ? k : 0)) * 2;
-          } else {
-            there = row - M < R && k < K8;
-            from = A + (there ? static_cast<long long>(row - M) * K8 + k : 0) * 2;
-          }
-          pg::cp_async16(to + row * 128 + ((piece ^ (row & 7)) * 16), from, there);
+        const int stage = (c - c0) % kStages;
+        const uint32_t to = base + stage * plan.stage_bytes;
+        if (tid == 0) {
+          pg::mbar_expect_tx(bar0 + 8 * (kStages + stage), down_block);
+          pg::bulk_copy_g2s(to + kRows * 128, A + static_cast<long long>(c) * down_block, down_block, bar0 + 8 * (kStages + stage));
+        }
+        const bool in = 64 * c + 8 * piece < a.K;
+#pragma unroll
+        for (int i = 0; i < kRows / 32; ++i) {
+          const int row = row0 + 32 * i;
+          const bool there = in && from[i] != nullptr;
+          pg::cp_async16(to + row * 128 + ((piece ^ (row & 7)) * 16), there ? from[i] + 128LL * c : static_cast<const char*>(a.x), there);
         }
       }
       pg::cp_async_commit();
     };
+    const uint32_t idesc = pg::make_idesc_bf16(kRows, plan.R16);
     for (int i = 0; i < kStages - 1; ++i) ask(c0 + i);
-    float sum[2][4][2][4] = {};
     for (int c = c0; c < c1; ++c) {
+      const int i = c - c0;
       pg::cp_async_wait<kStages - 2>();
+      pg::fence_proxy_async_smem();
       __syncthreads();
+      if (tid == 0) {
+        pg::mbar_wait(bar0 + 8 * (kStages + i % kStages), i / kStages % 2);
+        pg::tc_fence_after();
+        const uint32_t at = base + i % kStages * plan.stage_bytes;
+        const uint64_t x = pg::make_sdesc_k_sw128(at), w = pg::make_sdesc_k_sw128(at + kRows * 128);
+        for (int k = 0; k < 4; ++k) pg::umma_f16(tmem, x + 2 * k, w + 2 * k, idesc, i > 0 || k > 0);
+        pg::umma_commit(bar0 + 8 * (i % kStages));
+      }
+      if (i > 0) pg::mbar_wait(bar0 + 8 * ((i - 1) % kStages), (i - 1) / kStages % 2);  // (the stage that is filled next has been read)
       ask(c + kStages - 1);
-      const uint32_t at = base + (c - c0) % kStages * stage_bytes;
-      float d[OUT32 ? 2 : 1][OUT32 ? 4 : 1][2][4] = {};
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        uint32_t xf[2][4];
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          const int row = 32 * wm + 16 * m + lane % 16, piece = 2 * kk + lane / 16;
-          pg::ldmatrix_x4(at + row * 128 + ((piece ^ (row & 7)) * 16), xf[m][0], xf[m][1], xf[m][2], xf[m][3]);
-        }
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          if (b >= per_warp || n0 + b >= blocks) continue;
-          const int row = M + 16 * (n0 + b) + lane % 8 + lane / 16 * 8, piece = 2 * kk + lane / 8 % 2;
-          uint32_t w0, w1, w2, w3;
-          pg::ldmatrix_x4(at + row * 128 + ((piece ^ (row & 7)) * 16), w0, w1, w2, w3);
-#pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            if constexpr (OUT32) {
-              pg::mma_bf16_16816(d[m][b][0], xf[m], w0, w1);
-              pg::mma_bf16_16816(d[m][b][1], xf[m], w2, w3);
-            } else {
-              pg::mma_bf16_16816(sum[m][b][0], xf[m], w0, w1);
-              pg::mma_bf16_16816(sum[m][b][1], xf[m], w2, w3);
-            }
-          }
-        }
-      }
-      if constexpr (OUT32) {
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-          for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sum[m][b][i / 4][i % 4] += d[m][b][i / 4][i % 4];
-      }
     }
+    const int last = c1 - c0 - 1;
+    if (last >= 0) pg::mbar_wait(bar0 + 8 * (last % kStages), last / kStages % 2);
+    pg::tc_fence_after();
     pg::cp_async_wait<0>();
     __syncthreads();
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-      for (int b = 0; b < 4; ++b)
-        if (b < per_warp && n0 + b < blocks)
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int row = 32 * wm + 16 * m + 8 * h + lane / 4, n = 16 * (n0 + b) + 8 * i + lane % 4 * 2;
-              if (n < R) *reinterpret_cast<float2*>(partial + row * lay.partial_ld + n) = make_float2(sum[m][b][i][2 * h], sum[m][b][i][2 * h + 1]);
-            }
   }
-  Columns<4, false, OUT32> columns(a, lay, row_of, tile.who, rank, ranks, y_vec);
-  columns.start();
+  float* partial = reinterpret_cast<float*>(raw);  // [rows][partial_ld], in the stages' place
+  const int quarter = warp % 4, half = warp / 4;   // a warp reads 32 lanes of tensor memory; two warps share them
+  {
+    float* to = partial + (32 * quarter + lane) * lay.partial_ld;
+    for (int c = 16 * half; c < plan.R16; c += 32) {
+      uint32_t v[16];
+      if (c1 > c0) {
+        pg::tmem_ld16(tmem + (static_cast<uint32_t>(32 * quarter) << 16) + c, v);
+        pg::tmem_ld_wait();
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = 0u;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c + 4 * i < R) *reinterpret_cast<uint4*>(to + c + 4 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    }
+  }
   pg::cluster_sync_all();
-  join_shares<M, VT>(a, lay, partial, 1, vt, tile.count, ranks);
+  {
+    // a thread has every second piece of one row; two pieces at once
+    const int per_row = a.parts * plan.blocks64 * 8, m = tid % kRows;
+    for (int c0 = tid / kRows; c0 < per_row; c0 += 4) {
+      const float* from[2];
+      bool in[2];
+      char* to[2];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int c = min(c0 + 2 * n, per_row - 1), part = c / (plan.blocks64 * 8), r = c % (plan.blocks64 * 8) * 8;
+        in[n] = m < tile.count && r < a.rank;
+        from[n] = partial + m * lay.partial_ld + (in[n] ? part * a.rank + r : 0);
+        to[n] = raw + plan.v_at + (part * plan.blocks64 + r / 64) * VT * (kRows * 128) + m * 128 + ((r / 8 % 8 ^ (m & 7)) * 16);
+      }
+      float f[2][8];
+      joined8(from, ranks, f);
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        uint4 t[VT];
+        split8<VT>(f[n], t);
+        if (c0 + 2 * n < per_row)
+#pragma unroll
+          for (int k = 0; k < VT; ++k) *reinterpret_cast<uint4*>(to[n] + k * (kRows * 128)) = in[n] ? t[k] : zero4();
+      }
+    }
+  }
+  pg::fence_proxy_async_smem();
+  pg::tc_fence_before();
+  pg::cluster_sync_all();  // all shares have been read: their place is free
+  pg::tc_fence_after();
+
+  // ---- out = y + B v: blocks of 128 columns ------------------------------------------------------------------------------
+  {
+    const char* B = static_cast<const char*>(a.b) + static_cast<long long>(tile.who) * a.F * a.rank * 2;
+    const float factor = a.gain * a.scale[tile.who];
+    const int b_bytes = plan.blocks64 * kBlock * 128, k16 = (a.rank + 15) / 16;
+    float* stage = reinterpret_cast<float*>(raw + 2 * b_bytes) + warp * 32 * kStageLd;
+    constexpr uint32_t idesc = pg::make_idesc_bf16(kRows, kBlock);
+    struct Block {
+      int part, f0, wide;
+    };
+    auto block = [&](int u) {  // the u-th block of all parts
+      Block b{0, 0, 0};
+      while (b.part < a.parts && u >= (a.part_cols[b.part] + kBlock - 1) / kBlock) {
+        u -= (a.part_cols[b.part] + kBlock - 1) / kBlock;
+        b.f0 += a.part_cols[b.part];
+        ++b.part;
+      }
+      if (b.part < a.parts) b.wide = min(kBlock, a.part_cols[b.part] - kBlock * u), b.f0 += kBlock * u;
+      return b;
+    };
+    const int pieces = min(2 * k16, 8);  // of a row of 64 ranks
+    auto ask_b = [&](const Block& b, int turn) {
+      if (b.wide > 0)
+        for (int i = tid; i < plan.blocks64 * kBlock * pieces; i += kThreads) {
+          const int row = i / pieces % kBlock, piece = i % pieces, q = i / pieces / kBlock, r = q * 64 + 8 * piece;
+          const bool there = row < b.wide && r < a.rank;
+          pg::cp_async16(base + turn * b_bytes + q * (kBlock * 128) + row * 128 + ((piece ^ (row & 7)) * 16), B + (there ? static_cast<long long>(b.f0 + row) * a.rank + r : 0) * 2, there);
+        }
+      pg::cp_async_commit();
+    };
+    // a warp's 32 rows and 64 of the block's columns: eight lanes a row
+    Eight<OUT32> y[8];
+    auto ask_y = [&](const Block& b) {
+      const int c = 64 * half + lane % 8 * 8;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int t = row_of[32 * quarter + 4 * i + lane / 8];
+        y[i].load(a.y, t * a.ldy + b.f0 + c, b.wide - c, y_vec, t >= 0 && c < b.wide);
+      }
+    };
+    int u = rank, turn = 0;
+    Block now = block(u);
+    ask_b(now, 0);
+    ask_y(now);
+    for (; now.wide > 0; turn ^= 1) {
+      u += ranks;
+      const Block next = block(u);
+      pg::cp_async_wait<0>();
+      pg::fence_proxy_async_smem();
+      __syncthreads();
+      if (tid == 0) {
+        pg::tc_fence_after();
+        const uint32_t to = tmem + 256 + kBlock * turn;
+        bool more = false;
+        for (int k = VT - 1; k >= 0; --k)  // the smallest term first
+          for (int s = 0; s < k16; ++s) {
+            const uint64_t v = pg::make_sdesc_k_sw128(base + plan.v_at + ((now.part * plan.blocks64 + s / 4) * VT + k) * (kRows * 128));
+            const uint64_t w = pg::make_sdesc_k_sw128(base + turn * b_bytes + s / 4 * (kBlock * 128));
+            pg::umma_f16(to, v + 2 * (s % 4), w + 2 * (s % 4), idesc, more);
+            more = true;
+          }
+        pg::umma_commit(bar0 + 8 * (2 * kStages + turn));
+      }
+      ask_b(next, turn ^ 1);
+      const int at = (u - ranks - rank) / ranks;  // the block's number here
+      pg::mbar_wait(bar0 + 8 * (2 * kStages + turn), at / 2 % 2);
+      __syncwarp();
+      pg::tc_fence_after();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t v[16];
+        pg::tmem_ld16(tmem + (static_cast<uint32_t>(32 * quarter) << 16) + 256 + kBlock * turn + 64 * half + 16 * i, v);
+        pg::tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(stage + lane * kStageLd + 16 * i + 4 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+      }
+      pg::tc_fence_before();
+      __syncwarp();
+      const int c = 64 * half + lane % 8 * 8;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = 4 * i + lane / 8, t = row_of[32 * quarter + row];
+        const float4 lo = *reinterpret_cast<const float4*>(stage + row * kStageLd + lane % 8 * 8), hi = *reinterpret_cast<const float4*>(stage + row * kStageLd + lane % 8 * 8 + 4);
+        const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        if (t >= 0 && c < now.wide) y[i].store(a.out, t * a.ldo + now.f0 + c, now.wide - c, y_vec, factor, v);
+      }
+      __syncwarp();
+      now = next;
+      ask_y(now);
+    }
+  }
+  pg::cp_async_wait<0>();
+  pg::tc_fence_before();
   __syncthreads();
-  columns.run(vt);
-  pg::cluster_sync_all();  // nobody leaves while its share is read
+  if (warp == 0) {
+    __syncwarp();
+    pg::tc_fence_after();
+    pg::tmem_dealloc(tmem, 512);
+  }
 }
 
 template <typename Kern, typename... Args>
@@ -536,15 +707,22 @@ int pick(const PgAdapter& a, cudaStream_t st, int x_vec, int y_vec) {
   lay.v_ld = a.parts * lay.rank32;
   lay.v_ld += (lay.v_ld % 64 == 32) ? 0 : 32;  // eight lanes' 16-byte pieces of two rows lie in different banks
   if constexpr (!IN32) {
-    // many rows of an adapter (up to 256 columns of v in a warp's registers)
-    if (a.tile_rows == 64 && lay.R <= 256 && x_vec && a.K % 8 == 0) {
-      const size_t stages = static_cast<size_t>(kStages) * (64 + (lay.R + 15) / 16 * 16) * 128, behind = sizeof(float) * 64 * lay.partial_ld + sizeof(uint16_t) * VT * 64 * lay.v_ld;
-      const int room = (OUT32 ? 1 : 2) * pg::num_sms();
-      int ranks = room / a.tile_count;  // shares of K: all CTAs at once
+    // many rows of an adapter, up to 256 columns of v, and room for its terms
+    Plan plan;
+    plan.R16 = (lay.R + 15) / 16 * 16;
+    plan.stage_bytes = (kRows + plan.R16) * 128;
+    plan.blocks64 = (a.rank + 63) / 64;
+    plan.v_bytes = a.parts * plan.blocks64 * VT * kRows * 128;
+    // v's terms stand behind the shares of v, in whose place B's blocks and the sums that leave come later
+    const int shares = static_cast<int>(sizeof(float)) * kRows * lay.partial_ld, leave = 2 * plan.blocks64 * kBlock * 128 + static_cast<int>(sizeof(float)) * kWarps * 32 * kStageLd;
+    plan.v_at = ((shares > leave ? shares : leave) + 1023) / 1024 * 1024;
+    const int stages = kStages * plan.stage_bytes, behind = plan.v_at + plan.v_bytes, smem = (stages > behind ? stages : behind) + 1024;
+    if (a.tile_rows == kRows && plan.R16 <= 256 && x_vec && a.K % 8 == 0 && smem <= kMostShared) {
+      int ranks = pg::num_sms() / a.tile_count;  // shares of K and of the columns: all CTAs at once
       ranks = ranks < 1 ? 1 : ranks > kMostRanks ? kMostRanks : ranks;
       while (ranks > 1 && a.K / ranks < 128) --ranks;
       static bool configured[pg::kMaxDevices] = {};
-      return launch(adapter_tiles_kernel<OUT32>, configured, a.tile_count, ranks, stages > behind ? stages : behind, st, a, lay, y_vec);
+      return launch(adapter_tensor_kernel<OUT32>, configured, a.tile_count, ranks, smem, st, a, lay, plan, y_vec);
     }
   }
   const int subs = a.tile_rows / 16;
@@ -563,7 +741,7 @@ extern "C" int pg_adapter_add(const PgAdapter* args, void* stream) {
   if (args == nullptr) return PG_ERR_ARG;
   const PgAdapter& a = *args;
   if (a.x == nullptr || a.y == nullptr || a.out == nullptr || a.a == nullptr || a.b == nullptr || a.scale == nullptr || a.rows == nullptr || a.tiles == nullptr || a.parts < 1 ||
-      a.parts > 8 || a.K < 1 || a.rank < 8 || a.rank > 128 || a.rank % 8 || a.slots < 1 || a.tile_count < 1 || (a.tile_rows != 16 && a.tile_rows != 64) || a.T < 1 || a.ldx < a.K ||
+      a.parts > 8 || a.K < 1 || a.rank < 8 || a.rank > 128 || a.rank % 8 || a.slots < 1 || a.tile_count < 1 || (a.tile_rows != 16 && a.tile_rows != 128) || a.T < 1 || a.ldx < a.K ||
       a.ldy < a.F || a.ldo < a.F || (a.in_f32 && !a.out_f32) || ((reinterpret_cast<uintptr_t>(a.a) | reinterpret_cast<uintptr_t>(a.b)) & 15))
     return PG_ERR_ARG;
   long long cols = 0;

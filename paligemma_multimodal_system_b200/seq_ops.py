@@ -766,11 +766,29 @@ class AdapterBank:
         if not a.is_cuda or b.device != a.device or scale.device != a.device:
             raise ValueError("adapters lie on one device")
         self.parts, self.slots, self.rank, self.K, self.F, self.dtype, self.device = tuple(parts), slots, rank, K, sum(parts), a.dtype, a.device
-        r8, K8 = -(-rank // 8) * 8, -(-K // 8) * 8  # (ranks and depths in whole 16-byte pieces; zeros behind)
-        self.rank8 = r8
-        self.a, self.b, self.scale = a.new_zeros(slots, len(parts) * r8, K8), b.new_zeros(slots, self.F, r8), scale.clone()
-        self.a.view(slots, len(parts), r8, K8)[:, :, :rank, :K] = a.view(slots, len(parts), rank, K) if a.is_contiguous() else a.reshape(slots, len(parts), rank, K)
+        r8 = -(-rank // 8) * 8  # (ranks and depths in whole 16-byte pieces; zeros behind)
+        self.rank8, self.scale = r8, scale.clone()
+        if self.dtype == torch.bfloat16:  # blocks of 64 k's, see _pieces
+            self.a = a.new_zeros(slots, -(-K // 64), -(-len(parts) * r8 // 16) * 16, 8, 8)
+        else:
+            self.a = a.new_zeros(slots, len(parts) * r8, -(-K // 8) * 8)
+        self.b = b.new_zeros(slots, self.F, r8)
+        for p in range(len(parts)):
+            self._put_a(slice(None), p, a[:, p * rank:(p + 1) * rank])
         self.b[:, :, :rank] = b
+
+    def _put_a(self, slot, part, a):
+        """a [.., r, K] into rows of the run; bf16: [K / 64, rows, 8, 8], in row n the eight pieces of eight k's exchanged by n % 8, the matrix unit's operand layout."""
+        r, here = a.shape[-2], slice(part * self.rank8, part * self.rank8 + a.shape[-2])
+        if self.dtype != torch.bfloat16:
+            self.a[slot, here, :self.K] = a
+            return
+        blocks = self.a.shape[1]
+        wide = a.new_zeros(*a.shape[:-1], 64 * blocks)
+        wide[..., :self.K] = a
+        pieces = wide.unflatten(-1, (blocks, 8, 8)).movedim(-4, -3)  # [.., blocks, r, 8, 8]
+        order = torch.arange(8, device=a.device) ^ (torch.arange(here.start, here.start + r, device=a.device) % 8)[:, None]
+        self.a[slot, :, here] = pieces.gather(-2, order[..., None].expand(pieces.shape))
 
     @classmethod
     def empty(cls, slots: int, rank: int, K: int, parts: Sequence[int], dtype: torch.dtype, device="cuda"):
@@ -785,9 +803,9 @@ class AdapterBank:
         if a.dim() != 2 or b.dim() != 2 or r > self.rank or a.shape[1] != self.K or tuple(b.shape) != (self.parts[part], r):
             raise ValueError(f"a {tuple(a.shape)} and b {tuple(b.shape)} for {self.parts[part]} columns of a depth of {self.K} and a rank up to {self.rank}")
         col = sum(self.parts[:part])
-        here = self.a[slot, part * self.rank8:(part + 1) * self.rank8]
-        here.zero_()
-        here[:r, :self.K] = a.to(self.device, self.dtype)
+        full = torch.zeros(self.rank8, self.K, device=self.device, dtype=self.dtype)
+        full[:r] = a.to(self.device, self.dtype)
+        self._put_a(slot, part, full)
         there = self.b[slot, col:col + self.parts[part]]
         there.zero_()
         there[:, :r] = b.to(self.device, self.dtype)
@@ -819,8 +837,8 @@ class AdapterPlan:
 
     def _make(self, ns, adapters, device):
         order, ids, first, count = self._order(ns, adapters)
-        # rows of an adapter on average: tiles of 64 read it once for four of 16, tiles of 16 are four times the CTAs (decoded tokens)
-        size = 64 if self.fixed is None and len(order) >= 32 * len(ids) else 16
+        # by the rows of an adapter on average: tiles of 128 go over the tensor memory, tiles of 16 are more CTAs (decoded tokens)
+        size = 128 if self.fixed is None and len(order) >= 64 * len(ids) else 16
         tiles = [(a, f + o, min(size, c - o)) for a, f, c in zip(ids.tolist(), first.tolist(), count.tolist()) for o in range(0, c, size)]
         n = len(tiles) if self.fixed is None else self.fixed
         if len(tiles) > n:
