@@ -845,17 +845,20 @@ int pg_verify_drafts(const PgVerify* a, void* stream);
  * for rows of adapter s.  The columns are `parts` runs of part_cols; each has rank rows of a for itself.  rank: a multiple of 8 up to
  * 128.  b: [slots, F, rank] in x's type.  a, fp32: [slots, parts * rank, K8], K8 = K rounded up to 8; bf16: [slots, ceil(K / 64), parts * rank rounded up to 16, 8, 8], element (n, k) at
  * [k / 64, n, (k / 8 % 8) ^ (n % 8), k % 8].  Zeros where there is no k or no row.  rows / tiles: the plan, tiles of up to tile_rows (16 or 128) rows
- * (adapter, first, count) of one adapter, rows[first ..] their numbers; adapter -1: rows without one, which are copied where out is not y. */
+ * (adapter, first, count) of one adapter, rows[first ..] their numbers; adapter -1: rows without one, which are copied where out is not y.
+ * shares: pg_adapter_scratch bytes of scratch (0: none is read). */
 typedef struct {
   const void *x, *y, *a, *b;
   void* out;
   const float* scale;
   const int *rows, *tiles;
+  float* shares;
   long long ldx, ldy, ldo;
   int part_cols[8];
   int parts, K, F, rank, slots, tile_count, tile_rows, T, in_f32, out_f32;
   float gain;
 } PgAdapter;
+long long pg_adapter_scratch(const PgAdapter* a);
 int pg_adapter_add(const PgAdapter* a, void* stream);
 
 #ifdef __cplusplus

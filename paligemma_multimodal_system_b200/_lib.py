@@ -95,6 +95,7 @@ SIGNATURES = {
     "pg_copy_pages": [p, i32, i32, i64, p, i32, p],
     "pg_keep_rows": [p, i32, i32, i32, p, i32, p, p, p, i32, p, i32, p],
     "pg_verify_drafts": [p, p],
+    "pg_adapter_scratch": [p],
     "pg_adapter_add": [p, p],
     "pg_token_logprobs": [p, i64, p, p, p, p, p, p, i32, i32, i32, f32, p],
     "pg_attn_ragged": [p, p, p, p, i64, p, p, p, p, p, i32, i32, i32, i32, i32, i32, i32, i32, f32, f32, i32, i32, i64, i64, i32, p, p],
@@ -141,7 +142,7 @@ SIGNATURES = {
     "pg_gated_layernorm_add": [p, i64, p, i64, p, p, p, p, p, p, p, i32, i32, f32, i32, i32, p],
     "pg_glu": [p, i64, p, i64, i32, i32, i32, f32, f32, i32, p],
 }
-_RESTYPE = {"pg_launch_count": i64, "pg_gemm_fp32_scratch": i64, "pg_gemm_fp32_scratch_add": i64, "pg_routed_ff_scratch": i64, "pg_attn_rows_scratch": i64}
+_RESTYPE = {"pg_launch_count": i64, "pg_gemm_fp32_scratch": i64, "pg_gemm_fp32_scratch_add": i64, "pg_routed_ff_scratch": i64, "pg_attn_rows_scratch": i64, "pg_adapter_scratch": i64}
 
 
 
@@ -156,7 +157,7 @@ ATTN_ROWS = struct.Struct("@6Pq8P16i2f")
 PREPARE_E4M3 = struct.Struct("@Pq13Pq12i3f4x")
 READ_E4M3 = struct.Struct("@10P8i")
 VERIFY = struct.Struct("@11P3q4d4i")
-ADAPTER = struct.Struct("@8P3q18if4x")
+ADAPTER = struct.Struct("@9P3q18if4x")
 PAGE_OPERAND = struct.Struct("@Pq4i")  # PgPageOperand
 
 

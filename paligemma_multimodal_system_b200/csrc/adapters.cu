@@ -105,10 +105,11 @@ PG_DEVINL int cluster_size() {
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
   return static_cast<int>(n);
 }
-PG_DEVINL float4 get_f4(const float* p, int rank) {
+PG_DEVINL float4 get_f4(const float* p, int rank, int own) {  // (its own memory a CTA reads by the address that it has there)
   uint32_t there;
   float4 v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(pg::smem_u32(p)), "r"(rank));
+  there = rank == own ? pg::smem_u32(p) : there;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(there));
   return v;
 }
@@ -142,16 +143,17 @@ PG_DEVINL Tile tile_of(const PgAdapter& a, int item, int subs, int (&row_of)[M])
 template <typename U>
 PG_DEVINL void copy_pieces(const PgAdapter& a, const int* row_of, int count, int rank, int ranks, int bytes, int element) {
   const int per_row = bytes / static_cast<int>(sizeof(U)), all = count * per_row;
-  for (int i0 = rank * kThreads + threadIdx.x; i0 < all; i0 += 4 * ranks * kThreads) {
+  const int step = ranks * blockDim.x;
+  for (int i0 = rank * blockDim.x + threadIdx.x; i0 < all; i0 += 4 * step) {
     U v[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int i = i0 + k * ranks * kThreads, t = i < all ? row_of[i / per_row] : -1;
+      const int i = i0 + k * step, t = i < all ? row_of[i / per_row] : -1;
       if (t >= 0) v[k] = reinterpret_cast<const U*>(static_cast<const char*>(a.y) + t * a.ldy * element)[i % per_row];
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int i = i0 + k * ranks * kThreads, t = i < all ? row_of[i / per_row] : -1;
+      const int i = i0 + k * step, t = i < all ? row_of[i / per_row] : -1;
       if (t >= 0) reinterpret_cast<U*>(static_cast<char*>(a.out) + t * a.ldo * element)[i % per_row] = v[k];
     }
   }
@@ -166,6 +168,7 @@ PG_DEVINL void copy_rows(const PgAdapter& a, const int* row_of, int count, int r
 // Eight numbers of v, the CTAs' shares added in their order; N of them at once, all CTAs' asked for together
 template <int N>
 PG_DEVINL void joined8(const float* (&from)[N], int ranks, float (&f)[N][8]) {
+  const int own = pg::cluster_ctarank();
 #pragma unroll
   for (int n = 0; n < N; ++n)
 #pragma unroll
@@ -177,7 +180,7 @@ PG_DEVINL void joined8(const float* (&from)[N], int ranks, float (&f)[N][8]) {
 #pragma unroll
       for (int n = 0; n < N; ++n)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) v[k][n][h] = get_f4(from[n] + 4 * h, min(p + k, ranks - 1));
+        for (int h = 0; h < 2; ++h) v[k][n][h] = get_f4(from[n] + 4 * h, min(p + k, ranks - 1), own);
 #pragma unroll
     for (int k = 0; k < 2; ++k)
       if (p + k < ranks)
@@ -429,248 +432,338 @@ __global__ void __launch_bounds__(kThreads, 2) adapter_rows_kernel(const PgAdapt
 
 // Tiles of 128 bf16 rows, both products on the tensor cores with their sums in tensor memory.
 //   v = x A^T        x and A come in stages of 64 k's by asynchronous copies, 128-byte rows whose 16-byte pieces are exchanged by the row's last bits; N = ranks of all parts, up to 256
-//   shares of K      from tensor memory to shared memory, added over the cluster, as bf16 terms into shared memory again (operand layout, 64 ranks a block of 16 KB)
-//   B v              blocks of 128 columns: every term times the same rows of B; y of the next block is under way meanwhile; sums leave through shared memory so that a warp reads and
-//                    writes whole lines of y and out
+//   shares of K      added over the cluster by way of L2 (through distributed shared memory a CTA read 6 bytes a clock: 18,000 clocks for 192 columns of v, 4,000 this way), as bf16 terms
+//                    into shared memory (operand layout, 64 ranks a block of 16 KB)
+//   B v              blocks of 128 columns: every term times the same rows of B, a block ahead of the one whose sums leave; y is asked for a block ahead as well; sums leave through
+//                    shared memory so that lanes read and write neighbouring pieces of y and out
 // 256 columns of tensor memory for v, two times 128 for the blocks: one CTA an SM.
-constexpr int kStages = 3, kRows = 128, kBlock = 128, kStageLd = 68;  // (68: lanes' rows of 64 numbers lie in different banks)
+// A warp of its own issues the products: it waits where operands are not there yet, the others do not wait for it.  Stages are asked for three chunks ahead of five, so that the one
+// that is filled was read two products ago.
+constexpr int kWorkers = 512, kWorkerWarps = kWorkers / 32, kTensorThreads = kWorkers + 32, kCols = 32;  // columns of a block that a warp takes, beside three others with the same rows
+constexpr int kStages = 5, kRows = 128, kBlock = 128, kStageLd = kCols + 4;                          // (+ 4: lanes' rows lie in different banks)
+constexpr int kFull = 0, kEmpty = kStages, kShare = 2 * kStages, kThere = kShare + 1, kDone = kThere + 2, kLeft = kDone + 2, kBars = kLeft + 2;  // barriers: stages, v, blocks
 struct Plan {                                                       // of shared memory
-  int R16, stage_bytes, v_bytes, v_at, blocks64;                    // v: [parts][blocks of 64 ranks][terms] operands of 16 KB
+  int R16, stages, stage_bytes, v_at, blocks64, smem;               // v: [parts][blocks of 64 ranks][terms] operands of 16 KB
 };
+
+struct Blocks {  // of 128 columns, of all parts
+  const PgAdapter& a;
+  struct Block {
+    int part, f0, wide, left;  // left: of the part, this block among them
+  };
+  PG_DEVINL Block at(int u) const { return next(Block{0, 0, 1, a.part_cols[0]}, u); }
+  PG_DEVINL Block next(Block b, int u) const {  // u blocks on; wide 0: there is none
+    if (b.wide == 0) return b;
+    for (;;) {
+      const int here = (b.left + kBlock - 1) / kBlock;
+      if (u < here) break;
+      u -= here;
+      b.f0 += b.left;
+      if (++b.part >= a.parts) {
+        b.wide = 0;
+        return b;
+      }
+      b.left = a.part_cols[b.part];
+    }
+    b.f0 += kBlock * u, b.left -= kBlock * u;
+    b.wide = min(kBlock, b.left);
+    return b;
+  }
+};
+
 template <bool OUT32>
-__global__ void __launch_bounds__(kThreads, 1) adapter_tensor_kernel(const PgAdapter a, const Layout lay, const Plan plan, int y_vec) {
+__global__ void __launch_bounds__(kTensorThreads, 1) adapter_tensor_kernel(const PgAdapter a, const Layout lay, const Plan plan, int y_vec) {
   constexpr int VT = OUT32 ? 3 : 2;
   extern __shared__ char raw_unaligned[];
   __shared__ int row_of[kRows];
-  __shared__ __align__(8) uint64_t bars[2 * kStages + 2];  // stages read, stages' A there, blocks done
+  __shared__ __align__(8) uint64_t bars[kBars];
   __shared__ uint32_t tmem_at;
-  char* raw = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw_unaligned) + 1023) & ~static_cast<uintptr_t>(1023));  // (the same place in every CTA)
+  char* raw = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw_unaligned) + 1023) & ~static_cast<uintptr_t>(1023));
   const int ranks = cluster_size(), rank = pg::cluster_ctarank(), item = blockIdx.x / ranks, tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const Tile tile = tile_of<kRows>(a, item, 1, row_of);
   pg::griddep_wait();
   if (tile.count <= 0 || (tile.none && a.out == a.y)) return;  // (the whole cluster)
   if (tile.none) return copy_rows<OUT32>(a, row_of, tile.count, rank, ranks, y_vec);
   const uint32_t base = pg::smem_u32(raw), bar0 = pg::smem_u32(bars);
+  auto bar = [&](int i) { return bar0 + 8 * i; };
   if (warp == 0) {
     pg::tmem_alloc(pg::smem_u32(&tmem_at), 512);
     pg::tmem_relinquish();
   }
-  if (tid == 32) {
-    for (int i = 0; i < 2 * kStages + 2; ++i) pg::mbar_init(bar0 + 8 * i, 1);
+  if (tid == kWorkers) {
+    for (int i = 0; i < kStages; ++i) pg::mbar_init(bar(kFull + i), kWorkerWarps + 1), pg::mbar_init(bar(kEmpty + i), 1);
+    pg::mbar_init(bar(kShare), 1);
+    for (int i = 0; i < 2; ++i) pg::mbar_init(bar(kThere + i), kWorkerWarps), pg::mbar_init(bar(kDone + i), 1), pg::mbar_init(bar(kLeft + i), kWorkerWarps);
     pg::mbar_fence_init();
   }
   pg::tc_fence_before();
   __syncthreads();
   pg::tc_fence_after();
   const uint32_t tmem = tmem_at;
-  const int R = lay.R;
+  const int R = lay.R, k16 = (a.rank + 15) / 16, b_bytes = plan.blocks64 * kBlock * 128;
+  const int all = (a.K + 63) / 64, per = (all + ranks - 1) / ranks, c0 = min(rank * per, all), chunks = min(per, all - c0);  // this CTA's share of K
+  const Blocks blocks{a};
 
-  // ---- this CTA's share of v, into columns 0 .. R of tensor memory --------------------------------------------------------
-  const int chunks = (a.K + 63) / 64, per = (chunks + ranks - 1) / ranks, c0 = min(rank * per, chunks), c1 = min(c0 + per, chunks);
-  {
-    const char* A = static_cast<const char*>(a.a) + tile.who * down_bytes<false>(R, a.K);
-    const int down_block = plan.R16 * 128, row0 = tid / 8, piece = tid % 8;  // a thread's piece of rows row0, row0 + 32 ..
-    const char* from[kRows / 32];
-#pragma unroll
-    for (int i = 0; i < kRows / 32; ++i) {
-      const int t = row_of[row0 + 32 * i];
-      from[i] = t >= 0 ? static_cast<const char*>(a.x) + (t * a.ldx + 8 * piece) * 2 : nullptr;
-    }
-    auto ask = [&](int c) {
-      if (c < c1) {
-        const int stage = (c - c0) % kStages;
-        const uint32_t to = base + stage * plan.stage_bytes;
-        if (tid == 0) {
-          pg::mbar_expect_tx(bar0 + 8 * (kStages + stage), down_block);
-          pg::bulk_copy_g2s(to + kRows * 128, A + static_cast<long long>(c) * down_block, down_block, bar0 + 8 * (kStages + stage));
-        }
-        const bool in = 64 * c + 8 * piece < a.K;
-#pragma unroll
-        for (int i = 0; i < kRows / 32; ++i) {
-          const int row = row0 + 32 * i;
-          const bool there = in && from[i] != nullptr;
-          pg::cp_async16(to + row * 128 + ((piece ^ (row & 7)) * 16), there ? from[i] + 128LL * c : static_cast<const char*>(a.x), there);
-        }
-      }
-      pg::cp_async_commit();
-    };
-    const uint32_t idesc = pg::make_idesc_bf16(kRows, plan.R16);
-    for (int i = 0; i < kStages - 1; ++i) ask(c0 + i);
-    for (int c = c0; c < c1; ++c) {
-      const int i = c - c0;
-      pg::cp_async_wait<kStages - 2>();
-      pg::fence_proxy_async_smem();
-      __syncthreads();
-      if (tid == 0) {
-        pg::mbar_wait(bar0 + 8 * (kStages + i % kStages), i / kStages % 2);
+  if (warp == kWorkerWarps) {
+    // ---- products: v = x A^T into columns 0 .. R of tensor memory, then B v by blocks into 256 .. 383 and 384 .. 511 ----------
+    const uint32_t down = pg::make_idesc_bf16(kRows, plan.R16);
+    constexpr uint32_t up = pg::make_idesc_bf16(kRows, kBlock);
+    if (lane == 0) {
+      // (one thread's instructions come one after another, ten clocks each: no divisions here)
+      const uint64_t x0 = pg::make_sdesc_k_sw128(base);
+      uint64_t x = x0;
+      uint32_t phase = 0;
+      for (int i = 0, stage = 0; i < chunks; ++i) {
+        pg::mbar_wait(bar(kFull + stage), phase);
         pg::tc_fence_after();
-        const uint32_t at = base + i % kStages * plan.stage_bytes;
-        const uint64_t x = pg::make_sdesc_k_sw128(at), w = pg::make_sdesc_k_sw128(at + kRows * 128);
-        for (int k = 0; k < 4; ++k) pg::umma_f16(tmem, x + 2 * k, w + 2 * k, idesc, i > 0 || k > 0);
-        pg::umma_commit(bar0 + 8 * (i % kStages));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) pg::umma_f16(tmem, x + 2 * k, x + (kRows * 128 >> 4) + 2 * k, down, i > 0 || k > 0);
+        pg::umma_commit(bar(kEmpty + stage));
+        x += plan.stage_bytes >> 4;
+        if (++stage == plan.stages) stage = 0, phase ^= 1, x = x0;
       }
-      if (i > 0) pg::mbar_wait(bar0 + 8 * ((i - 1) % kStages), (i - 1) / kStages % 2);  // (the stage that is filled next has been read)
-      ask(c + kStages - 1);
+      if (chunks > 0) pg::umma_commit(bar(kShare));
     }
-    const int last = c1 - c0 - 1;
-    if (last >= 0) pg::mbar_wait(bar0 + 8 * (last % kStages), last / kStages % 2);
-    pg::tc_fence_after();
-    pg::cp_async_wait<0>();
-    __syncthreads();
-  }
-  float* partial = reinterpret_cast<float*>(raw);  // [rows][partial_ld], in the stages' place
-  const int quarter = warp % 4, half = warp / 4;   // a warp reads 32 lanes of tensor memory; two warps share them
-  {
-    float* to = partial + (32 * quarter + lane) * lay.partial_ld;
-    for (int c = 16 * half; c < plan.R16; c += 32) {
-      uint32_t v[16];
-      if (c1 > c0) {
-        pg::tmem_ld16(tmem + (static_cast<uint32_t>(32 * quarter) << 16) + c, v);
-        pg::tmem_ld_wait();
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = 0u;
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (c + 4 * i < R) *reinterpret_cast<uint4*>(to + c + 4 * i) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-    }
-  }
-  pg::cluster_sync_all();
-  {
-    // a thread has every second piece of one row; two pieces at once
-    const int per_row = a.parts * plan.blocks64 * 8, m = tid % kRows;
-    for (int c0 = tid / kRows; c0 < per_row; c0 += 4) {
-      const float* from[2];
-      bool in[2];
-      char* to[2];
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const int c = min(c0 + 2 * n, per_row - 1), part = c / (plan.blocks64 * 8), r = c % (plan.blocks64 * 8) * 8;
-        in[n] = m < tile.count && r < a.rank;
-        from[n] = partial + m * lay.partial_ld + (in[n] ? part * a.rank + r : 0);
-        to[n] = raw + plan.v_at + (part * plan.blocks64 + r / 64) * VT * (kRows * 128) + m * 128 + ((r / 8 % 8 ^ (m & 7)) * 16);
-      }
-      float f[2][8];
-      joined8(from, ranks, f);
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        uint4 t[VT];
-        split8<VT>(f[n], t);
-        if (c0 + 2 * n < per_row)
-#pragma unroll
-          for (int k = 0; k < VT; ++k) *reinterpret_cast<uint4*>(to[n] + k * (kRows * 128)) = in[n] ? t[k] : zero4();
-      }
-    }
-  }
-  pg::fence_proxy_async_smem();
-  pg::tc_fence_before();
-  pg::cluster_sync_all();  // all shares have been read: their place is free
-  pg::tc_fence_after();
-
-  // ---- out = y + B v: blocks of 128 columns ------------------------------------------------------------------------------
-  {
-    const char* B = static_cast<const char*>(a.b) + static_cast<long long>(tile.who) * a.F * a.rank * 2;
-    const float factor = a.gain * a.scale[tile.who];
-    const int b_bytes = plan.blocks64 * kBlock * 128, k16 = (a.rank + 15) / 16;
-    float* stage = reinterpret_cast<float*>(raw + 2 * b_bytes) + warp * 32 * kStageLd;
-    constexpr uint32_t idesc = pg::make_idesc_bf16(kRows, kBlock);
-    struct Block {
-      int part, f0, wide;
-    };
-    auto block = [&](int u) {  // the u-th block of all parts
-      Block b{0, 0, 0};
-      while (b.part < a.parts && u >= (a.part_cols[b.part] + kBlock - 1) / kBlock) {
-        u -= (a.part_cols[b.part] + kBlock - 1) / kBlock;
-        b.f0 += a.part_cols[b.part];
-        ++b.part;
-      }
-      if (b.part < a.parts) b.wide = min(kBlock, a.part_cols[b.part] - kBlock * u), b.f0 += kBlock * u;
-      return b;
-    };
-    const int pieces = min(2 * k16, 8);  // of a row of 64 ranks
-    auto ask_b = [&](const Block& b, int turn) {
-      if (b.wide > 0)
-        for (int i = tid; i < plan.blocks64 * kBlock * pieces; i += kThreads) {
-          const int row = i / pieces % kBlock, piece = i % pieces, q = i / pieces / kBlock, r = q * 64 + 8 * piece;
-          const bool there = row < b.wide && r < a.rank;
-          pg::cp_async16(base + turn * b_bytes + q * (kBlock * 128) + row * 128 + ((piece ^ (row & 7)) * 16), B + (there ? static_cast<long long>(b.f0 + row) * a.rank + r : 0) * 2, there);
-        }
-      pg::cp_async_commit();
-    };
-    // a warp's 32 rows and 64 of the block's columns: eight lanes a row
-    Eight<OUT32> y[8];
-    auto ask_y = [&](const Block& b) {
-      const int c = 64 * half + lane % 8 * 8;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int t = row_of[32 * quarter + 4 * i + lane / 8];
-        y[i].load(a.y, t * a.ldy + b.f0 + c, b.wide - c, y_vec, t >= 0 && c < b.wide);
-      }
-    };
-    int u = rank, turn = 0;
-    Block now = block(u);
-    ask_b(now, 0);
-    ask_y(now);
-    for (; now.wide > 0; turn ^= 1) {
-      u += ranks;
-      const Block next = block(u);
-      pg::cp_async_wait<0>();
-      pg::fence_proxy_async_smem();
-      __syncthreads();
-      if (tid == 0) {
-        pg::tc_fence_after();
+    __syncwarp();
+    if (ranks > 1) pg::cluster_sync_all();
+    __syncthreads();  // (v's terms are there)
+    if (lane == 0) {
+      pg::tc_fence_after();
+      const uint64_t v0 = pg::make_sdesc_k_sw128(base + plan.v_at), w0 = pg::make_sdesc_k_sw128(base);
+      const int v_part = plan.blocks64 * VT * (kRows * 128 >> 4);
+      Blocks::Block b = blocks.at(rank);
+      for (int at = 0; b.wide > 0; ++at) {
+        const int turn = at & 1, phase = at >> 1 & 1;
         const uint32_t to = tmem + 256 + kBlock * turn;
+        uint64_t v = v0 + b.part * v_part, w = w0 + turn * (b_bytes >> 4);
+        b = blocks.next(b, ranks);
+        pg::mbar_wait(bar(kThere + turn), phase);
+        if (at >= 2) pg::mbar_wait(bar(kLeft + turn), phase ^ 1);  // (what stood there has been read)
+        pg::tc_fence_after();
         bool more = false;
-        for (int k = VT - 1; k >= 0; --k)  // the smallest term first
-          for (int s = 0; s < k16; ++s) {
-            const uint64_t v = pg::make_sdesc_k_sw128(base + plan.v_at + ((now.part * plan.blocks64 + s / 4) * VT + k) * (kRows * 128));
-            const uint64_t w = pg::make_sdesc_k_sw128(base + turn * b_bytes + s / 4 * (kBlock * 128));
-            pg::umma_f16(to, v + 2 * (s % 4), w + 2 * (s % 4), idesc, more);
-            more = true;
-          }
-        pg::umma_commit(bar0 + 8 * (2 * kStages + turn));
+        for (int left = k16; left > 0; left -= 4) {  // 64 ranks; the smallest term first within them
+#pragma unroll
+          for (int k = VT - 1; k >= 0; --k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (i < left) {
+                pg::umma_f16(to, v + k * (kRows * 128 >> 4) + 2 * i, w + 2 * i, up, more);
+                more = true;
+              }
+          v += VT * (kRows * 128 >> 4), w += kBlock * 128 >> 4;
+        }
+        pg::umma_commit(bar(kDone + turn));
       }
-      ask_b(next, turn ^ 1);
-      const int at = (u - ranks - rank) / ranks;  // the block's number here
-      pg::mbar_wait(bar0 + 8 * (2 * kStages + turn), at / 2 % 2);
+    }
+    __syncwarp();
+  } else {
+    auto arrive = [&](int i) {  // of a warp
+      __syncwarp();
+      if (lane == 0) pg::mbar_arrive(bar(i));
+    };
+    {
+      const char* A = static_cast<const char*>(a.a) + tile.who * down_bytes<false>(R, a.K);
+      const int down_block = plan.R16 * 128, row0 = tid / 8, piece = tid % 8;  // a thread's piece of rows row0 and row0 + 64
+      const char* from[2];
+      uint32_t to[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = row0 + 64 * i, t = row_of[row];
+        from[i] = t >= 0 ? static_cast<const char*>(a.x) + (t * a.ldx + 64LL * c0 + 8 * piece) * 2 : nullptr;
+        to[i] = base + row * 128 + ((piece ^ (row & 7)) * 16);
+      }
+      int asked = 0, stage = 0;  // the next chunk and its stage
+      uint32_t phase = 1;        // (of the round before: the first passes)
+      auto ask = [&]() {
+        if (asked < chunks) {
+          const uint32_t at = stage * plan.stage_bytes;
+          if (asked >= plan.stages) pg::mbar_wait(bar(kEmpty + stage), phase);
+          if (tid == 0) {
+            pg::mbar_expect_tx(bar(kFull + stage), down_block);
+            pg::bulk_copy_g2s(base + at + kRows * 128, A + static_cast<long long>(c0 + asked) * down_block, down_block, bar(kFull + stage));
+          }
+          const bool in = 64 * (c0 + asked) + 8 * piece < a.K;
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const bool there = in && from[r] != nullptr;
+            pg::cp_async16(to[r] + at, there ? from[r] : static_cast<const char*>(a.x), there);
+            if (from[r] != nullptr) from[r] += 128;
+          }
+          ++asked;
+          if (++stage == plan.stages) stage = 0, phase ^= 1;
+        }
+        pg::cp_async_commit();
+      };
+      const int ahead = plan.stages - 2;
+      for (int i = 0; i < ahead; ++i) ask();
+      for (int i = 0, full = 0; i < chunks; ++i) {
+        ask();
+        if (ahead == 3) pg::cp_async_wait<3>();
+        else if (ahead == 2) pg::cp_async_wait<2>();
+        else pg::cp_async_wait<1>();
+        pg::fence_proxy_async_smem();
+        arrive(kFull + full);
+        if (++full == plan.stages) full = 0;
+      }
+      if (chunks > 0) pg::mbar_wait(bar(kShare), 0);
       __syncwarp();
       pg::tc_fence_after();
+      pg::cp_async_wait<0>();
+    }
+    // ---- the shares of v together ------------------------------------------------------------------------------------------
+    const int quarter = warp % 4, group = warp / 4, m = 32 * quarter + lane;  // a warp reads 32 lanes of tensor memory; four warps share them
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
+    const long long share = static_cast<long long>(R) * kRows;
+    float* shares = a.shares + item * share * ranks;  // [ranks][R / 4][rows][4]
+    if (ranks > 1) {
+      for (int c = 16 * group; c < R; c += 64) {
+        uint32_t v[16] = {};
+        if (chunks > 0) {
+          pg::tmem_ld16(lanes + c, v);
+          pg::tmem_ld_wait();
+        }
+        uint4* to = reinterpret_cast<uint4*>(shares + rank * share) + c / 4 * kRows + m;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t v[16];
-        pg::tmem_ld16(tmem + (static_cast<uint32_t>(32 * quarter) << 16) + 256 + kBlock * turn + 64 * half + 16 * i, v);
-        pg::tmem_ld_wait();
-#pragma unroll
-        for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(stage + lane * kStageLd + 16 * i + 4 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        for (int i = 0; i < 4; ++i)
+          if (c + 4 * i < R) to[i * kRows] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
       }
-      pg::tc_fence_before();
-      __syncwarp();
-      const int c = 64 * half + lane % 8 * 8;
+      pg::cluster_sync_all();
+    } else {
+      asm volatile("bar.sync 1, %0;" ::"n"(kWorkers) : "memory");  // (nobody writes v's terms while a stage is still read)
+    }
+    const int per_row = a.parts * plan.blocks64 * 8;
+    constexpr int N = 3;  // pieces at once
+    for (int first = group; first < per_row; first += 4 * N) {
+      float f[N][8], own[N][8];
+      int at[N];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int row = 4 * i + lane / 8, t = row_of[32 * quarter + row];
-        const float4 lo = *reinterpret_cast<const float4*>(stage + row * kStageLd + lane % 8 * 8), hi = *reinterpret_cast<const float4*>(stage + row * kStageLd + lane % 8 * 8 + 4);
-        const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-        if (t >= 0 && c < now.wide) y[i].store(a.out, t * a.ldo + now.f0 + c, now.wide - c, y_vec, factor, v);
+      for (int n = 0; n < N; ++n) {
+        const int q = (first + 4 * n) >> 3, part = plan.blocks64 == 1 ? q : q >> 1, r = (plan.blocks64 == 1 ? 0 : (q & 1) * 64) + ((first + 4 * n) & 7) * 8;
+        at[n] = first + 4 * n < per_row && r < a.rank ? part * a.rank + r : -1;  // (the same in a whole warp)
+        uint32_t v[16] = {};
+        if (chunks > 0 && at[n] >= 0) {
+          pg::tmem_ld8(lanes + at[n], v);
+          pg::tmem_ld_wait();
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[n][i] = 0.0f, own[n][i] = __uint_as_float(v[i]);
       }
-      __syncwarp();
-      now = next;
-      ask_y(now);
+      for (int p = 0; p < ranks; ++p) {  // (the ranks' order, whoever adds)
+        float4 v[N][2];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          const float* from = shares + p * share + (static_cast<long long>(max(at[n], 0)) / 4 * kRows + m) * 4;
+          const bool there = p != rank && at[n] >= 0;
+          const uint4 lo = ld16(from, there), hi = ld16(from + 4 * kRows, there);
+          v[n][0] = make_float4(__uint_as_float(lo.x), __uint_as_float(lo.y), __uint_as_float(lo.z), __uint_as_float(lo.w));
+          v[n][1] = make_float4(__uint_as_float(hi.x), __uint_as_float(hi.y), __uint_as_float(hi.z), __uint_as_float(hi.w));
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          if (p == rank) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[n][i] += own[n][i];
+          } else {
+            f[n][0] += v[n][0].x, f[n][1] += v[n][0].y, f[n][2] += v[n][0].z, f[n][3] += v[n][0].w, f[n][4] += v[n][1].x, f[n][5] += v[n][1].y, f[n][6] += v[n][1].z, f[n][7] += v[n][1].w;
+          }
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const int c = first + 4 * n;
+        if (c >= per_row) break;
+        uint4 terms[VT];
+        split8<VT>(f[n], terms);
+        char* to = raw + plan.v_at + (c >> 3) * VT * (kRows * 128) + m * 128 + (((c & 7) ^ (m & 7)) * 16);
+#pragma unroll
+        for (int k = 0; k < VT; ++k) *reinterpret_cast<uint4*>(to + k * (kRows * 128)) = m < tile.count && at[n] >= 0 ? terms[k] : zero4();
+      }
+    }
+    pg::fence_proxy_async_smem();
+    pg::tc_fence_before();
+    __syncthreads();
+    pg::tc_fence_after();
+
+    // ---- out = y + B v: blocks of 128 columns ------------------------------------------------------------------------------
+    const char* B = static_cast<const char*>(a.b) + static_cast<long long>(tile.who) * a.F * a.rank * 2;
+    const float factor = a.gain * a.scale[tile.who];
+    float* stage = reinterpret_cast<float*>(raw + 2 * b_bytes) + warp * 32 * kStageLd;
+    const int c = kCols * group + lane % 4 * 8;  // the first of a lane's columns of a block; four lanes a row
+    int row[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) row[i] = row_of[32 * quarter + 8 * i + lane / 4];
+    auto ask_b = [&](const Blocks::Block& b, int turn) {
+      if (b.wide > 0)
+        for (int q = 0; q < plan.blocks64; ++q)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int n = tid / 8 + 64 * i, piece = tid % 8, r = 64 * q + 8 * piece;
+            const bool there = n < b.wide && r < a.rank;
+            if (piece < 2 * k16 - 8 * q)  // (what the product reads)
+              pg::cp_async16(base + turn * b_bytes + q * (kBlock * 128) + n * 128 + ((piece ^ (n & 7)) * 16), B + (there ? static_cast<long long>(b.f0 + n) * a.rank + r : 0) * 2, there);
+          }
+      pg::cp_async_commit();
+    };
+    auto ask_y = [&](const Blocks::Block& b, Eight<OUT32> (&y)[4]) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i].load(a.y, row[i] * a.ldy + b.f0 + c, b.wide - c, y_vec, row[i] >= 0 && c < b.wide);
+    };
+    Eight<OUT32> y[2][4];
+    Blocks::Block b[2];
+    b[0] = blocks.at(rank), b[1] = blocks.next(b[0], ranks);
+    ask_b(b[0], 0);
+    ask_b(b[1], 1);
+    ask_y(b[0], y[0]);
+    pg::cp_async_wait<1>();
+    pg::fence_proxy_async_smem();
+    arrive(kThere);
+    pg::cp_async_wait<0>();
+    pg::fence_proxy_async_smem();
+    arrive(kThere + 1);
+    for (int at = 0; b[0].wide > 0; at += 2) {
+#pragma unroll
+      for (int turn = 0; turn < 2; ++turn) {
+        if (b[turn].wide <= 0) break;
+        const Blocks::Block now = b[turn];
+        ask_y(b[turn ^ 1], y[turn ^ 1]);
+        b[turn] = blocks.next(b[turn ^ 1], ranks);
+        pg::mbar_wait(bar(kDone + turn), at / 2 % 2);
+        __syncwarp();
+        pg::tc_fence_after();
+        ask_b(b[turn], turn);
+#pragma unroll
+        for (int i = 0; i < kCols / 16; ++i) {
+          uint32_t v[16];
+          pg::tmem_ld16(lanes + 256 + kBlock * turn + kCols * group + 16 * i, v);
+          pg::tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(stage + lane * kStageLd + 16 * i + 4 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        }
+        pg::tc_fence_before();
+        arrive(kLeft + turn);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float* from = stage + (8 * i + lane / 4) * kStageLd + lane % 4 * 8;
+          const float4 lo = *reinterpret_cast<const float4*>(from), hi = *reinterpret_cast<const float4*>(from + 4);
+          const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+          if (row[i] >= 0 && c < now.wide) y[turn][i].store(a.out, row[i] * a.ldo + now.f0 + c, now.wide - c, y_vec, factor, v);
+        }
+        pg::cp_async_wait<0>();
+        pg::fence_proxy_async_smem();
+        arrive(kThere + turn);
+      }
     }
   }
-  pg::cp_async_wait<0>();
   pg::tc_fence_before();
   __syncthreads();
   if (warp == 0) {
-    __syncwarp();
     pg::tc_fence_after();
     pg::tmem_dealloc(tmem, 512);
   }
 }
 
 template <typename Kern, typename... Args>
-int launch(Kern kern, bool (&configured)[pg::kMaxDevices], long long items, int ranks, size_t smem, cudaStream_t st, Args... args) {
+int launch(Kern kern, bool (&configured)[pg::kMaxDevices], long long items, int ranks, int threads, size_t smem, cudaStream_t st, Args... args) {
   bool& done = configured[pg::current_device()];
   if (!done) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared) != cudaSuccess) {
@@ -682,7 +775,7 @@ int launch(Kern kern, bool (&configured)[pg::kMaxDevices], long long items, int 
   if (smem > kMostShared || items * ranks > 0x7fffffff) return PG_ERR_ARG;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(items * ranks));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -697,32 +790,49 @@ int launch(Kern kern, bool (&configured)[pg::kMaxDevices], long long items, int 
   return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? PG_OK : PG_ERR_CUDA;
 }
 
-template <bool IN32, bool OUT32>
-int pick(const PgAdapter& a, cudaStream_t st, int x_vec, int y_vec) {
-  constexpr int VT = IN32 || OUT32 ? 3 : 2, NW = IN32 ? 2 : 6;  // (fp32: three terms of every fragment)
+Layout layout_of(const PgAdapter& a) {
   Layout lay;
   lay.R = a.parts * a.rank;
   lay.partial_ld = lay.R + 4;
   lay.rank32 = (a.rank + 31) / 32 * 32;
   lay.v_ld = a.parts * lay.rank32;
   lay.v_ld += (lay.v_ld % 64 == 32) ? 0 : 32;  // eight lanes' 16-byte pieces of two rows lie in different banks
+  return lay;
+}
+// Shared memory of a tile of 128 rows; no stages: it does not go over the tensor memory (few rows of an adapter, more than 256 columns of v, no room for its terms)
+template <int VT>
+void plan_of(const PgAdapter& a, const Layout& lay, Plan& plan) {
+  plan.R16 = (lay.R + 15) / 16 * 16;
+  plan.stage_bytes = (kRows + plan.R16) * 128;
+  plan.blocks64 = (a.rank + 63) / 64;
+  const int v_bytes = a.parts * plan.blocks64 * VT * kRows * 128;
+  const int leave = 2 * plan.blocks64 * kBlock * 128 + static_cast<int>(sizeof(float)) * kWorkerWarps * 32 * kStageLd;  // B's blocks and the sums that leave, in front of v's terms
+  plan.v_at = (leave + 1023) / 1024 * 1024;
+  plan.stages = kStages;
+  while (plan.stages * plan.stage_bytes + 1024 > kMostShared) --plan.stages;
+  const int behind = plan.v_at + v_bytes, stages = plan.stages * plan.stage_bytes;
+  plan.smem = (stages > behind ? stages : behind) + 1024;
+  if (a.tile_rows != kRows || a.in_f32 || plan.R16 > 256 || plan.smem > kMostShared) plan.stages = 0;
+}
+int shares_of(const PgAdapter& a) {  // of K and of the columns, a CTA each: all CTAs at once
+  int ranks = pg::num_sms() / a.tile_count;
+  ranks = ranks < 1 ? 1 : ranks > kMostRanks ? kMostRanks : ranks;
+  while (ranks > 1 && a.K / ranks < 128) --ranks;
+  return ranks;
+}
+
+template <bool IN32, bool OUT32>
+int pick(const PgAdapter& a, cudaStream_t st, int x_vec, int y_vec) {
+  constexpr int VT = IN32 || OUT32 ? 3 : 2, NW = IN32 ? 2 : 6;  // (fp32: three terms of every fragment)
+  const Layout lay = layout_of(a);
   if constexpr (!IN32) {
-    // many rows of an adapter, up to 256 columns of v, and room for its terms
     Plan plan;
-    plan.R16 = (lay.R + 15) / 16 * 16;
-    plan.stage_bytes = (kRows + plan.R16) * 128;
-    plan.blocks64 = (a.rank + 63) / 64;
-    plan.v_bytes = a.parts * plan.blocks64 * VT * kRows * 128;
-    // v's terms stand behind the shares of v, in whose place B's blocks and the sums that leave come later
-    const int shares = static_cast<int>(sizeof(float)) * kRows * lay.partial_ld, leave = 2 * plan.blocks64 * kBlock * 128 + static_cast<int>(sizeof(float)) * kWarps * 32 * kStageLd;
-    plan.v_at = ((shares > leave ? shares : leave) + 1023) / 1024 * 1024;
-    const int stages = kStages * plan.stage_bytes, behind = plan.v_at + plan.v_bytes, smem = (stages > behind ? stages : behind) + 1024;
-    if (a.tile_rows == kRows && plan.R16 <= 256 && x_vec && a.K % 8 == 0 && smem <= kMostShared) {
-      int ranks = pg::num_sms() / a.tile_count;  // shares of K and of the columns: all CTAs at once
-      ranks = ranks < 1 ? 1 : ranks > kMostRanks ? kMostRanks : ranks;
-      while (ranks > 1 && a.K / ranks < 128) --ranks;
+    plan_of<VT>(a, lay, plan);
+    if (plan.stages > 0 && x_vec && a.K % 8 == 0) {
+      const int ranks = shares_of(a);
+      if (ranks > 1 && a.shares == nullptr) return PG_ERR_ARG;
       static bool configured[pg::kMaxDevices] = {};
-      return launch(adapter_tensor_kernel<OUT32>, configured, a.tile_count, ranks, smem, st, a, lay, plan, y_vec);
+      return launch(adapter_tensor_kernel<OUT32>, configured, a.tile_count, ranks, kTensorThreads, plan.smem, st, a, lay, plan, y_vec);
     }
   }
   const int subs = a.tile_rows / 16;
@@ -732,10 +842,19 @@ int pick(const PgAdapter& a, cudaStream_t st, int x_vec, int y_vec) {
   while (wn < kWarps && wn * NW < lay.R / 8) wn *= 2;
   const size_t smem = sizeof(float) * (kWarps / wn) * 16 * lay.partial_ld + sizeof(uint16_t) * VT * 16 * lay.v_ld;
   static bool configured[pg::kMaxDevices] = {};
-  return launch(adapter_rows_kernel<NW, IN32, OUT32>, configured, items, ranks, smem, st, a, lay, subs, x_vec, y_vec);
+  return launch(adapter_rows_kernel<NW, IN32, OUT32>, configured, items, ranks, kThreads, smem, st, a, lay, subs, x_vec, y_vec);
 }
 
 }  // namespace
+
+extern "C" long long pg_adapter_scratch(const PgAdapter* args) {
+  if (args == nullptr || args->parts < 1 || args->parts > 8 || args->rank < 8 || args->rank > 128 || args->tile_count < 1 || args->K < 1) return 0;
+  Plan plan;
+  if (args->out_f32) plan_of<3>(*args, layout_of(*args), plan);
+  else plan_of<2>(*args, layout_of(*args), plan);
+  const int ranks = plan.stages > 0 ? shares_of(*args) : 1;
+  return ranks > 1 ? static_cast<long long>(sizeof(float)) * args->tile_count * ranks * kRows * args->parts * args->rank : 0;
+}
 
 extern "C" int pg_adapter_add(const PgAdapter* args, void* stream) {
   if (args == nullptr) return PG_ERR_ARG;

@@ -765,6 +765,7 @@ class AdapterBank:
             raise ValueError("one fp32 factor for every adapter")
         if not a.is_cuda or b.device != a.device or scale.device != a.device:
             raise ValueError("adapters lie on one device")
+        self.columns = (*parts, *(0,) * (ADAPTER_MOST_PARTS - len(parts)))
         self.parts, self.slots, self.rank, self.K, self.F, self.dtype, self.device = tuple(parts), slots, rank, K, sum(parts), a.dtype, a.device
         r8 = -(-rank // 8) * 8  # (ranks and depths in whole 16-byte pieces; zeros behind)
         self.rank8, self.scale = r8, scale.clone()
@@ -912,10 +913,20 @@ def adapter_add(x: torch.Tensor, y: torch.Tensor, bank: AdapterBank, plan: Adapt
     if plan.dev.device != bank.device:
         raise ValueError(f"the plan lies on {plan.dev.device}, the adapters on {bank.device}")
     _on_current_device(bank.a)
-    a = _lib.ADAPTER.pack(x.data_ptr(), y.data_ptr(), bank.a.data_ptr(), bank.b.data_ptr(), out.data_ptr(), bank.scale.data_ptr(), plan.rows.data_ptr(), plan.tiles.data_ptr(),
-                          *pitches, *bank.parts, *(0,) * (8 - len(bank.parts)), len(bank.parts), K, bank.F, bank.rank8, bank.slots, plan.tile_count, plan.tile_rows, T,
-                          bank.dtype == torch.float32, y.dtype == torch.float32, gain)
-    _lib.check(_lib.lib().pg_adapter_add(a, _lib.stream()), "pg_adapter_add")
+    L, shares = _lib.lib(), None
+
+    def packed():
+        return _lib.ADAPTER.pack(x.data_ptr(), y.data_ptr(), bank.a.data_ptr(), bank.b.data_ptr(), out.data_ptr(), bank.scale.data_ptr(), plan.rows.data_ptr(), plan.tiles.data_ptr(),
+                                 _lib.ptr(shares), *pitches, *bank.columns, len(bank.parts), K, bank.F, bank.rank8, bank.slots, plan.tile_count, plan.tile_rows, T,
+                                 bank.dtype == torch.float32, y.dtype == torch.float32, gain)
+
+    a = packed()
+    if plan.tile_rows > 16:
+        need = L.pg_adapter_scratch(a)
+        if need:
+            shares = torch.empty(need // 4, device=x.device, dtype=torch.float32)
+            a = packed()
+    _lib.check(L.pg_adapter_add(a, _lib.stream()), "pg_adapter_add")
     return out
 
 
