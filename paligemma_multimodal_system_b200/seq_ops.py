@@ -714,17 +714,28 @@ def copy_pages(cache: CachePages, moves):
     """moves: whole numbers [n, 3] on the host, (source page, destination page, rows): the first `rows` rows of the source page go to the destination page, in every
     operand.  No destination is another move's source or destination."""
     moves = np.asarray(moves)
+    n = len(moves)
     if moves.size == 0:
         return
     if moves.ndim != 2 or moves.shape[1] != 3 or moves.dtype.kind not in "iu":
         raise ValueError("moves are (source page, destination page, rows)")
-    if moves.min() < 0 or moves[:, :2].max() >= cache.pages or moves[:, 2].max() > cache.page:
+    if n <= 16:  # (a few numbers are looked over faster one by one)
+        rows = moves.tolist()
+        inside = all(0 <= a < cache.pages and 0 <= b < cache.pages and 0 <= r <= cache.page for a, b, r in rows)
+        to = {b for _, b, _ in rows}
+        apart = len(to) == n and not any(a in to for a, _, _ in rows)
+    else:
+        most = moves.max(0)
+        inside = moves.min() >= 0 and most[0] < cache.pages and most[1] < cache.pages and most[2] <= cache.page
+        count = np.bincount(moves[:, 1], minlength=cache.pages) if inside else None
+        apart = inside and count.max() == 1 and not count[moves[:, 0]].any()
+    if not inside:
         raise IndexError(f"moves go between pages 0 .. {cache.pages - 1} and take up to {cache.page} rows")
-    if np.unique(moves[:, 1]).size != len(moves) or np.isin(moves[:, 1], moves[:, 0]).any():
+    if not apart:
         raise ValueError("a page that is copied to is no other move's source or destination")
     _on_current_device(cache.table)
     moves = np.ascontiguousarray(moves, dtype=np.int32)
-    _lib.check(_lib.lib().pg_copy_pages(cache.table.data_ptr(), cache.count, cache.page, cache.most_page_bytes, moves.ctypes.data, len(moves), _lib.stream()), "pg_copy_pages")
+    _lib.check(_lib.lib().pg_copy_pages(cache.table.data_ptr(), cache.count, cache.page, cache.most_page_bytes, moves.ctypes.data, n, _lib.stream()), "pg_copy_pages")
 
 
 def keep_rows(cache: CachePages, b: StepBatch, path: torch.Tensor, kept: torch.Tensor):
@@ -767,6 +778,7 @@ class AdapterBank:
             raise ValueError("adapters lie on one device")
         self.columns = (*parts, *(0,) * (ADAPTER_MOST_PARTS - len(parts)))
         self.parts, self.slots, self.rank, self.K, self.F, self.dtype, self.device = tuple(parts), slots, rank, K, sum(parts), a.dtype, a.device
+        self.index = a.get_device()
         r8 = -(-rank // 8) * 8  # (ranks and depths in whole 16-byte pieces; zeros behind)
         self.rank8, self.scale = r8, scale.clone()
         if self.dtype == torch.bfloat16:  # blocks of 64 k's, see _pieces
@@ -875,14 +887,12 @@ class AdapterPlan:
 
 def _rows_overlap(s, s_pitch, t, t_pitch):
     """Whether two row matrices have bytes in common; column slices that stand side by side in one matrix have none."""
-    def span(m, pitch):
-        return m.data_ptr(), ((m.shape[0] - 1) * pitch + m.shape[1]) * m.element_size(), pitch * m.element_size(), m.shape[1] * m.element_size()
-
-    (a, a_len, a_pitch, a_row), (b, b_len, b_pitch, b_row) = span(s, s_pitch), span(t, t_pitch)
-    if a + a_len <= b or b + b_len <= a:
+    (rows, n), (more, m), a, b, i, j = s.shape, t.shape, s.data_ptr(), t.data_ptr(), s.element_size(), t.element_size()
+    if a + ((rows - 1) * s_pitch + n) * i <= b or b + ((more - 1) * t_pitch + m) * j <= a:
         return False
-    d = (b - a) % a_pitch
-    return a_pitch != b_pitch or d < a_row or a_pitch - d < b_row
+    pitch = s_pitch * i
+    d = (b - a) % pitch
+    return pitch != t_pitch * j or d < n * i or pitch - d < m * j
 
 
 def adapter_add(x: torch.Tensor, y: torch.Tensor, bank: AdapterBank, plan: AdapterPlan, out: Optional[torch.Tensor] = None, gain: float = 1.0):
@@ -890,35 +900,34 @@ def adapter_add(x: torch.Tensor, y: torch.Tensor, bank: AdapterBank, plan: Adapt
     out [rows, columns] bf16 or fp32 (fp32 beside fp32 adapters), unit last strides, any row pitch.  The sum over K and over the rank is fp32; y is added to it and rounded once.  A row of x that is not
     finite makes its own row of out NaN."""
     out = y if out is None else out
-    T, K = x.shape if x.dim() == 2 else (0, 0)
-    if x.dtype != bank.dtype or K != bank.K or T != plan.T:
-        raise ValueError(f"x is [{plan.T}, {bank.K}] of {bank.dtype}: got {tuple(x.shape)} of {x.dtype}")
-    if y.dtype not in (torch.bfloat16, torch.float32) or out.dtype != y.dtype or (bank.dtype == torch.float32 and y.dtype != torch.float32):
+    T, K, F, dtype, index = plan.T, bank.K, bank.F, bank.dtype, bank.index
+    if x.dtype != dtype or x.shape != (T, K):
+        raise ValueError(f"x is [{T}, {K}] of {dtype}: got {tuple(x.shape)} of {x.dtype}")
+    wide = y.dtype == torch.float32
+    if not (wide or y.dtype == torch.bfloat16) or out.dtype != y.dtype or (dtype == torch.float32 and not wide):
         raise ValueError("y and out share a type, torch.bfloat16 or torch.float32; torch.float32 beside fp32 adapters")
-    if tuple(y.shape) != (T, bank.F) or tuple(out.shape) != (T, bank.F):
-        raise ValueError(f"y and out are [{T}, {bank.F}]: got {tuple(y.shape)} and {tuple(out.shape)}")
-    pitches = []
-    for t, n in ((x, K), (y, bank.F), (out, bank.F)):
-        pitch = n if T == 1 else t.stride(0)
-        if (t.stride(1) != 1 and n > 1) or pitch < n:
-            raise ValueError("elements of a row stand side by side, rows do not overlap")
-        if t.device != bank.device:
-            raise ValueError(f"rows and adapters lie on one device: got {t.device} and {bank.device}")
-        pitches.append(pitch)
-    same = out.data_ptr() == y.data_ptr() and pitches[1] == pitches[2]
-    if _rows_overlap(out, pitches[2], x, pitches[0]) or (not same and _rows_overlap(out, pitches[2], y, pitches[1])):
+    if y.shape != (T, F) or out.shape != (T, F):
+        raise ValueError(f"y and out are [{T}, {F}]: got {tuple(y.shape)} and {tuple(out.shape)}")
+    (lx, ux), (ly, uy), (lo, uo) = x.stride(), y.stride(), out.stride()
+    if T == 1:
+        lx, ly, lo = K, F, F
+    if (ux != 1 and K > 1) or ((uy != 1 or uo != 1) and F > 1) or lx < K or ly < F or lo < F:
+        raise ValueError("elements of a row stand side by side, rows do not overlap")
+    if x.get_device() != index or y.get_device() != index or out.get_device() != index:
+        raise ValueError(f"rows and adapters lie on one device: got {x.device}, {y.device}, {out.device} and {bank.device}")
+    if _rows_overlap(out, lo, x, lx) or (not (lo == ly and out.data_ptr() == y.data_ptr()) and _rows_overlap(out, lo, y, ly)):
         raise ValueError("out is y or lies apart from it, and apart from x")
     if plan.most >= bank.slots:
         raise IndexError(f"adapter {plan.most} of {bank.slots}")
-    if plan.dev.device != bank.device:
+    if plan.dev.get_device() != index:
         raise ValueError(f"the plan lies on {plan.dev.device}, the adapters on {bank.device}")
     _on_current_device(bank.a)
     L, shares = _lib.lib(), None
 
     def packed():
         return _lib.ADAPTER.pack(x.data_ptr(), y.data_ptr(), bank.a.data_ptr(), bank.b.data_ptr(), out.data_ptr(), bank.scale.data_ptr(), plan.rows.data_ptr(), plan.tiles.data_ptr(),
-                                 _lib.ptr(shares), *pitches, *bank.columns, len(bank.parts), K, bank.F, bank.rank8, bank.slots, plan.tile_count, plan.tile_rows, T,
-                                 bank.dtype == torch.float32, y.dtype == torch.float32, gain)
+                                 _lib.ptr(shares), lx, ly, lo, *bank.columns, len(bank.parts), K, F, bank.rank8, bank.slots, plan.tile_count, plan.tile_rows, T,
+                                 dtype == torch.float32, wide, gain)
 
     a = packed()
     if plan.tile_rows > 16:
