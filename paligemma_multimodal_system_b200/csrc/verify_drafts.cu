@@ -653,6 +653,23 @@ struct Family {  // parents and tokens of an entry; those of the 32 rows behind 
   }
 };
 
+// Whether nothing that is decided yet leads past row v: all the way up, since rows that nothing leads to are judged as well while that is not known.  A warp; the parents and outcomes
+// of the 32 rows in front of v lie in its lanes.
+PG_DEVINL bool may_be_reached(const int* parents, const int* outcome, int v) {
+  const int j = v - 1 - static_cast<int>(threadIdx.x % 32);
+  const int ups = j >= 0 ? parents[j] : -1, saids = j >= 0 ? load_relaxed(outcome + j) : 0;
+  int row = v, up = parents[v];
+  for (;;) {
+    if (up < 0 || up >= row) return false;
+    const int l = v - 1 - up;
+    const int said = l < 32 ? __shfl_sync(0xffffffffu, saids, l) : load_relaxed(outcome + up);
+    if (said != 0 && said != row) return false;
+    if (up == 0) return true;
+    row = up;
+    up = l < 32 ? __shfl_sync(0xffffffffu, ups, l) : parents[up];
+  }
+}
+
 __global__ void __launch_bounds__(kThreads, kPerSm) verify_kernel(const PgVerify a, int share, int bits, int look) {
   extern __shared__ __align__(16) char raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw);
@@ -669,13 +686,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm) verify_kernel(const PgVerify
   if (live && v > 0) {
     if (look) {
       if (rank == 0 && tid < 32) {  // one look for all: what the parent decides may come in between
-        int said = 0;
-        if (tid == 0) {
-          const int up = fam.parents[v];
-          said = up >= 0 && up < v ? load_relaxed(outcome + up) : kDead;
-        }
-        said = __shfl_sync(0xffffffffu, said, 0);
-        if (tid < static_cast<int>(ranks)) put32(&sh.state, tid, said == 0 || said == v);
+        const bool reached = may_be_reached(fam.parents, outcome, v);
+        if (tid < static_cast<int>(ranks)) put32(&sh.state, tid, reached);
       }
       pg::cluster_sync_all();
       live = sh.state != 0;
