@@ -10,7 +10,7 @@
 
 namespace {
 
-constexpr int kThreads = 256, kLoads = 4, kPiece = kThreads * kLoads * 16, kMoves = 256, kCols = 64, kRowLanes = kThreads / kCols;
+constexpr int kThreads = 256, kLoads = 4, kPiece = kThreads * kLoads * 16, kMoves = 256, kCols = 64, kRowLanes = kThreads / kCols, kParts = 4;
 
 struct Moves {
   int n;
@@ -61,42 +61,47 @@ __global__ void __launch_bounds__(kThreads) copy_pages_kernel(const PgPageOperan
   }
 }
 
-// The columns [c0, c0 + kCols) of the path's rows: kRowLanes x kLoads rows are read, then written.  Paths ascend with path[i] >= i, so what a batch writes lies in
+// The columns [c0, c0 + kParts kCols) of the path's rows: kRowLanes x kLoads rows are read, then written.  Paths ascend with path[i] >= i, so what a batch writes lies in
 // front of every row that is still to be read.
 template <typename U>
 __device__ __forceinline__ void keep_columns(const PgPageOperand& op, const int* __restrict__ table, int max_pages, const int* __restrict__ path, int kept, int ctx, int n, int page,
                                              int c0) {
   const int c = c0 + threadIdx.x % kCols, lane = threadIdx.x / kCols;
   const int cols = op.heads > 0 ? op.heads : op.row_bytes / static_cast<int>(sizeof(U));
-  auto place = [&](int row) -> U* {
+  const long long step = kCols * (op.heads > 0 ? static_cast<long long>(page) : static_cast<long long>(sizeof(U)));  // bytes between a thread's columns
+  auto place = [&](int row) -> char* {
     const int slot = row / page;
     const int id = slot < max_pages ? table[slot] : -1;
     if (id < 0 || id >= op.pages) return nullptr;
     char* p = static_cast<char*>(op.base) + id * op.page_bytes;
-    return op.heads > 0 ? reinterpret_cast<U*>(p + static_cast<long long>(c) * page + row % page)
-                        : reinterpret_cast<U*>(p + static_cast<long long>(row % page) * op.row_bytes) + c;
+    return op.heads > 0 ? p + static_cast<long long>(c) * page + row % page : p + static_cast<long long>(row % page) * op.row_bytes + c * static_cast<long long>(sizeof(U));
   };
   for (int i0 = 0; i0 < kept; i0 += kRowLanes * kLoads) {
-    U v[kLoads];
-    U* to[kLoads];
+    U v[kLoads][kParts];
+    char* to[kLoads];
 #pragma unroll
     for (int k = 0; k < kLoads; ++k) {
       const int i = i0 + k * kRowLanes + lane;
       to[k] = nullptr;
-      if (i < kept && c < cols) {
+      if (i < kept) {
         const int p = path[i];
         if (p > i && p < n) {  // (rows that stay where they are need no move)
-          const U* from = place(ctx + p);
-          to[k] = place(ctx + i);
-          if (from != nullptr && to[k] != nullptr) v[k] = *from;
-          else to[k] = nullptr;
+          const char* from = place(ctx + p);
+          to[k] = from != nullptr ? place(ctx + i) : nullptr;
+          if (to[k] != nullptr)
+#pragma unroll
+            for (int j = 0; j < kParts; ++j)
+              if (c + j * kCols < cols) v[k][j] = *reinterpret_cast<const U*>(from + j * step);
         }
       }
     }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kLoads; ++k)
-      if (to[k] != nullptr) *to[k] = v[k];
+      if (to[k] != nullptr)
+#pragma unroll
+        for (int j = 0; j < kParts; ++j)
+          if (c + j * kCols < cols) *reinterpret_cast<U*>(to[k] + j * step) = v[k][j];
     __syncthreads();
   }
 }
@@ -105,7 +110,7 @@ __global__ void __launch_bounds__(kThreads) keep_rows_kernel(const PgPageOperand
                                                              const int* __restrict__ entry_n, const int* __restrict__ entry_ctx, const int* __restrict__ path, int path_ld,
                                                              const int* __restrict__ kept, int pieces) {
   pg::griddep_begin();
-  const int e = blockIdx.x / pieces, c0 = blockIdx.x % pieces * kCols;
+  const int e = blockIdx.x / pieces, c0 = blockIdx.x % pieces * (kCols * kParts);
   const PgPageOperand op = ops[blockIdx.y];
   if (c0 >= (op.heads > 0 ? op.heads : op.row_bytes / op.unit)) return;
   const int n = entry_n[e], ctx = entry_ctx[e], count = min(min(kept[e], path_ld), n);
@@ -143,7 +148,7 @@ extern "C" int pg_keep_rows(const PgPageOperand* operands, int count, int page, 
   if (operands == nullptr || count <= 0 || count > 65535 || page <= 0 || most_columns <= 0 || page_table == nullptr || max_pages <= 0 || entry_n == nullptr || entry_ctx == nullptr ||
       path == nullptr || path_ld <= 0 || kept == nullptr || entries <= 0)
     return PG_ERR_ARG;
-  const long long pieces = (most_columns + kCols - 1) / kCols;
+  const long long pieces = (most_columns + kCols * kParts - 1) / (kCols * kParts);
   if (pieces * entries > 0x7fffffff) return PG_ERR_ARG;
   return pg::launch_kernel(keep_rows_kernel, dim3(static_cast<unsigned>(entries * pieces), count), dim3(kThreads), 0, static_cast<cudaStream_t>(stream), operands, page, page_table,
                            max_pages, entry_n, entry_ctx, path, path_ld, kept, static_cast<int>(pieces)) == cudaSuccess
