@@ -689,6 +689,8 @@ class CachePages:
             raise ValueError("a cache has at least one operand")
         if len(flat) > 65535:
             raise ValueError(f"at most 65535 operands: got {len(flat)}")
+        if len({t.data_ptr() for t, _ in flat}) != len(flat):
+            raise ValueError("an operand is named twice: its rows would move twice")
         self.operands, self.page, self.pages, self.device = list(operands), int(page), flat[0][0].shape[0], flat[0][0].device
         table, self.most_page_bytes, self.most_columns = b"", 0, 0
         for t, heads in flat:
@@ -714,11 +716,11 @@ def copy_pages(cache: CachePages, moves):
     """moves: whole numbers [n, 3] on the host, (source page, destination page, rows): the first `rows` rows of the source page go to the destination page, in every
     operand.  No destination is another move's source or destination."""
     moves = np.asarray(moves)
-    n = len(moves)
     if moves.size == 0:
         return
     if moves.ndim != 2 or moves.shape[1] != 3 or moves.dtype.kind not in "iu":
         raise ValueError("moves are (source page, destination page, rows)")
+    n = len(moves)
     if n <= 16:  # (a few numbers are looked over faster one by one)
         rows = moves.tolist()
         inside = all(0 <= a < cache.pages and 0 <= b < cache.pages and 0 <= r <= cache.page for a, b, r in rows)
@@ -941,7 +943,8 @@ def adapter_add(x: torch.Tensor, y: torch.Tensor, bank: AdapterBank, plan: Adapt
 
 # ---- verified drafts -------------------------------------------------------------------------------------------------
 def _check_rows_of_logits(logits, b: StepBatch, what):
-    if logits.dim() != 2 or logits.dtype != torch.float32 or logits.stride(1) != 1 or not logits.is_cuda or logits.shape[0] != b.T:
+    if (logits.dim() != 2 or logits.dtype != torch.float32 or logits.stride(1) != 1 or not logits.is_cuda or logits.shape[0] != b.T
+            or (b.T > 1 and logits.stride(0) < logits.shape[1])):
         raise ValueError(f"{what} are fp32 [rows of the step, vocab] on the device, entries of a row side by side: got {tuple(logits.shape)} of {logits.dtype} for {b.T} rows")
 
 
@@ -964,6 +967,8 @@ def verify_drafts(logits: torch.Tensor, b: StepBatch, uniforms: Optional[torch.T
         raise ValueError(f"rows of 1 .. 2^30 - 1 entries: got {V}")
     if b.parents is None or b.parents.dtype != torch.int32 or b.parents.shape != (b.T,) or not b.parents.is_contiguous():
         raise ValueError("the step's parents (RequestBatch) are int32 [rows]")
+    if b.tokens.dtype != torch.int32 or b.tokens.shape != (b.T,) or not b.tokens.is_contiguous():
+        raise ValueError("the step's tokens are int32 [rows]")
     if uniforms is not None and (uniforms.dtype != torch.float32 or uniforms.shape != (b.T, 2) or not uniforms.is_contiguous()):
         raise ValueError("random numbers are fp32 [rows, 2]")
     if draft_logits is not None:

@@ -141,3 +141,73 @@ def test_a_plan_that_is_filled_again_under_a_graph():
         g.replay()
         value, bound = expected(x, y, a, b, scale, [1] * E, who, parts, 8)
         compare(Z, value, bound)
+
+
+@pytest.mark.parametrize("rank,parts", [(100, [320, 200]), (128, [264]), (8, [16, 130, 8, 300, 24, 128, 129, 40]), (64, [128, 640, 72]), (72, [1000]), (16, [3])])
+@pytest.mark.parametrize("dtype,out", FORMS[:2])
+@pytest.mark.parametrize("ns,who,slots", [([300], [0], 1), ([150, 1, 260, 128, 1], [1, 0, -1, 1, 1], 2)])
+def test_tiles_of_many_rows(rank, parts, dtype, out, ns, who, slots):
+    """Blocks of 64 ranks and 128 columns that are not full, several parts, shares of K that differ, rows without an adapter beside."""
+    K = 1096
+    x, y, a, b, scale = make(ns, who, K, parts, rank, slots, dtype, out, seed=rank)
+    bank, plan = seq_ops.AdapterBank(a.cuda(), b.cuda(), scale.cuda(), parts), seq_ops.AdapterPlan(ns, who)
+    assert plan.tile_rows == 128
+    value, bound = expected(x, y, a, b, scale, ns, who, parts, rank)
+    z = y.cuda()
+    apart = seq_ops.adapter_add(x.cuda(), z, bank, plan, out=torch.full_like(z, float("nan")))
+    compare(apart, value, bound)
+    assert torch.equal(seq_ops.adapter_add(x.cuda(), z, bank, plan), apart)
+    assert torch.equal(seq_ops.adapter_add(x.cuda(), y.cuda(), bank, plan), apart)  # the same sums every time
+
+
+@pytest.mark.parametrize("dtype,out", FORMS[:2])
+@pytest.mark.parametrize("K", [64, 200, 8])
+def test_more_tiles_than_processors(dtype, out, K):
+    ns, who, parts, rank = [20100, 300], [0, 1], [40, 136], 24
+    x, y, a, b, scale = make(ns, who, K, parts, rank, 2, dtype, out)
+    bank, plan = seq_ops.AdapterBank(a.cuda(), b.cuda(), scale.cuda(), parts), seq_ops.AdapterPlan(ns, who)
+    value, bound = expected(x, y, a, b, scale, ns, who, parts, rank)
+    compare(seq_ops.adapter_add(x.cuda(), y.cuda(), bank, plan), value, bound)
+
+
+@pytest.mark.parametrize("pitch,off", [(1104, 8), (1101, 3)])
+def test_tiles_of_many_rows_at_any_pitch(pitch, off):
+    ns, who, parts, K, rank = [270], [0], [1000, 20], 1000, 32
+    x, y, a, b, scale = make(ns, who, K, parts, rank, 1, torch.bfloat16, torch.bfloat16)
+    X, Y = torch.full((270, pitch), float("nan"), dtype=torch.bfloat16, device="cuda"), torch.full((270, pitch), float("nan"), dtype=torch.bfloat16, device="cuda")
+    X[:, off:off + K], Y[:, off:off + 1020] = x.cuda(), y.cuda()
+    before = Y.clone()
+    bank, plan = seq_ops.AdapterBank(a.cuda(), b.cuda(), scale.cuda(), parts), seq_ops.AdapterPlan(ns, who)
+    seq_ops.adapter_add(X[:, off:off + K], Y[:, off:off + 1020], bank, plan)
+    value, bound = expected(x, y, a, b, scale, ns, who, parts, rank)
+    compare(Y[:, off:off + 1020], value, bound)
+    Y[:, off:off + 1020] = before[:, off:off + 1020]
+    assert torch.equal(Y.view(torch.uint8), before.view(torch.uint8))
+
+
+def test_two_streams_and_a_captured_call():
+    """Calls that run at the same time have scratch of their own."""
+    ns, who, parts, K, rank = [700], [0], [512, 256], 1024, 64
+    x, y, a, b, scale = make(ns, who, K, parts, rank, 1, torch.bfloat16, torch.float32)
+    bank, plan = seq_ops.AdapterBank(a.cuda(), b.cuda(), scale.cuda(), parts), seq_ops.AdapterPlan(ns, who)
+    X, Y = x.cuda(), y.cuda()
+    want = seq_ops.adapter_add(X, Y, bank, plan, out=torch.empty_like(Y))
+    value, bound = expected(x, y, a, b, scale, ns, who, parts, rank)
+    compare(want, value, bound)
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(3)], []
+    for s in streams * 4:
+        with torch.cuda.stream(s):
+            outs.append(seq_ops.adapter_add(X, Y, bank, plan, out=torch.empty_like(Y)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+    with torch.cuda.stream(streams[0]):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=streams[0]):
+            o = seq_ops.adapter_add(X, Y, bank, plan, out=torch.empty_like(Y))
+    torch.cuda.synchronize()
+    for _ in range(2):
+        o.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, want)

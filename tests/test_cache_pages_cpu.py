@@ -32,10 +32,24 @@ def test_operands_that_are_no_cache(operands, page):
 
 @pytest.mark.parametrize("moves,error", [([[0, 1]], ValueError), ([0, 1, 2], ValueError), ([[0.0, 1.0, 2.0]], ValueError), ([[0, 6, 3]], IndexError), ([[6, 0, 3]], IndexError),
                                          ([[-1, 0, 3]], IndexError), ([[0, 1, 65]], IndexError), ([[0, 1, -1]], IndexError), ([[0, 1, 2], [3, 1, 2]], ValueError),
-                                         ([[0, 1, 2], [1, 2, 2]], ValueError), ([[2, 2, 4]], ValueError)])
+                                         ([[0, 1, 2], [1, 2, 2]], ValueError), ([[2, 2, 4]], ValueError), (5, ValueError), ([[True, False, True]], ValueError)])
 def test_moves_that_are_refused(moves, error):
     with pytest.raises(error):
         seq_ops.copy_pages(cache(), moves)
+
+
+def test_more_moves_are_looked_over_alike():
+    c = cache(100)
+    good = [[i, 50 + i, 3] for i in range(40)]
+    for at, bad, error in ((7, [7, 49, 65], IndexError), (7, [100, 57, 3], IndexError), (39, [39, 57, 3], ValueError), (3, [60, 53, 3], ValueError), (3, [3, -1, 3], IndexError)):
+        with pytest.raises(error):
+            seq_ops.copy_pages(c, good[:at] + [bad] + good[at + 1:])
+
+
+def test_an_operand_that_is_named_twice():
+    p = pages(4, 64, 8)
+    with pytest.raises(ValueError, match="twice"):
+        seq_ops.CachePages([p, p], 64)
 
 
 def test_nothing_to_move_is_no_call():

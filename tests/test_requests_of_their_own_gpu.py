@@ -315,3 +315,28 @@ def test_the_command_guesses(tmp_path, capsys):
     save_file({k: v.to(torch.bfloat16).contiguous() for k, v in w.items()}, str(tmp_path / "model.safetensors"))
     plain = generate_token_ids(str(tmp_path), "5 17 3 5 17 3 5; 8 9", 12, 0.8, 0.9, False, dtype="float32")
     assert generate_token_ids(str(tmp_path), "5 17 3 5 17 3 5; 8 9", 12, 0.8, 0.9, False, dtype="float32", draft=3) == plain
+
+
+def test_forks_beside_drafts_that_wait_and_of_latent_rows():
+    eng, ref = engine(ATTENTION, torch.float32), engine(ATTENTION, torch.float32)
+    prompt, drafts, later = toks(70, 80, 1), toks(4, 80, 2), toks(9, 80, 3)
+    eng.step([("a", prompt, [])])
+    eng.step_drafts([("a", drafts, [-1, 0, 0, 2])])
+    eng.fork("a", ["b"])  # what is not accepted is not the fork's
+    with pytest.raises(KeyError):
+        eng.accept("b", [0])
+    eng.accept("a", [0, 2, 3])
+    assert (eng.store.live["a"].length, eng.store.live["b"].length) == (73, 70)
+    for rid, full in (("a", prompt + [drafts[i] for i in (0, 2, 3)]), ("b", prompt)):
+        assert rel_err(run_cut_live(eng, rid, later, [1, 8]), run_cut(ref, "x", full + later, [len(full), 1, 8])[len(full):]) < TOL[torch.float32]
+    # one cached row a token, borrowed by another layer
+    from test_pukerax_gpu import BASE_CFG, engine_for
+    from oracle import pukerax_oracle as PO
+    w = PO.random_weights(BASE_CFG, seed=3)
+    V = BASE_CFG["vocab"]
+    eng, ref = engine_for(BASE_CFG, w, torch.float32), engine_for(BASE_CFG, w, torch.float32)
+    prompt, later = toks(90, V, 4), toks(6, V, 5)
+    eng.step([("a", prompt, [])])
+    eng.fork("a", ["b"], length=77)
+    for rid, full in (("a", prompt), ("b", prompt[:77])):
+        assert rel_err(run_cut_live(eng, rid, later, [1, 5]), run_cut(ref, "x", full + later, [len(full), 1, 5])[len(full):]) < TOL[torch.float32]

@@ -31,6 +31,8 @@ def logits(rows=3, V=40, dtype=torch.float32):
     lambda: (torch.zeros(3, 40), step()),
     lambda: (logits().t().contiguous().t(), step()),
     lambda: (logits()[0], step()),
+    lambda: (logits(1).expand(3, 40), step()),
+    lambda: (logits(), step(), torch.zeros(3, 2), logits(1).expand(3, 40)),
     lambda: (logits(V=0), step()),
     lambda: (logits(), step(), torch.zeros(3)),
     lambda: (logits(), step(), torch.zeros(3, 2, dtype=torch.float64)),

@@ -205,3 +205,56 @@ def test_captured_and_replayed_and_on_another_stream():
         fill(s)
         g.replay()
         check(out, ns, s[0], s[2], s[3], s[4], s[1], 0.8, 0.9)
+
+
+@pytest.mark.parametrize("spread,top_p", [(0.05, 0.9), (1.0, 0.99), (1.0, 0.999999), (6.0, 0.9)])
+@pytest.mark.parametrize("V", [9000, 150000])
+def test_flat_and_steep_rows(V, spread, top_p):
+    """More entries that may belong to the nucleus than are kept in shared memory, a border far down, and one among the first entries."""
+    ns = [3, 4]
+    logits, draft, parents, tokens, u = make(ns, V, 2, 31, spread=spread, top_p=top_p, agree=0.5)
+    for d in (draft, None):
+        got = seq_ops.verify_drafts(logits.cuda(), batch(ns, parents, tokens), u.cuda(), None if d is None else d.cuda(), 1.0, top_p)
+        check(got, ns, logits, parents, tokens, u, d, 1.0, top_p)
+
+
+@pytest.mark.parametrize("temperature", [1e-29, 1e-6, 0.01, 30.0, 1e6, 1e300])
+@pytest.mark.parametrize("offset", [0.0, -500.0, 3e4, 1e30])
+def test_temperatures_and_sizes_of_logits(temperature, offset):
+    ns = [3]
+    logits, draft, parents, tokens, u = make(ns, 5000, 1, 77, agree=0.0)
+    logits, draft = logits + offset, draft + offset
+    got = seq_ops.verify_drafts(logits.cuda(), batch(ns, parents, tokens), u.cuda(), draft.cuda(), temperature, 0.9)
+    check(got, ns, logits, parents, tokens, u, draft, temperature, 0.9)
+
+
+def test_two_streams_at_once():
+    ns = [7, 3, 9, 1]
+    logits, draft, parents, tokens, u = make(ns, 60000, 2, 5, temperature=0.8, top_p=0.9)
+    dev = (logits.cuda(), batch(ns, parents, tokens), u.cuda(), draft.cuda(), 0.8, 0.9)
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(3)], []
+    for s in streams * 4:
+        with torch.cuda.stream(s):
+            outs.append(seq_ops.verify_drafts(*dev))
+    torch.cuda.synchronize()
+    for o in outs:
+        check(o, ns, logits, parents, tokens, u, draft, 0.8, 0.9)
+
+
+def test_a_long_chain():
+    """More rows in front of one than a warp has lanes."""
+    n, V = 90, 400
+    g = torch.Generator().manual_seed(3)
+    logits = torch.randn(n, V, generator=g)
+    tokens = [0] + logits.argmax(-1).tolist()[:-1]
+    parents = list(range(-1, n - 1))
+    for wrong in (None, 40, 85):
+        t = list(tokens)
+        if wrong is not None:
+            t[wrong] = (t[wrong] + 1) % V
+        for copies in (1, 40):
+            got = seq_ops.verify_drafts(logits.repeat(copies, 1).cuda(), batch([n] * copies, parents * copies, t * copies))
+            stop = n if wrong is None else wrong
+            assert got[1].tolist() == [stop] * copies and got[0][-1].tolist() == list(range(stop)) + [-1] * (n - stop)
+            assert got[2].tolist() == [int(logits[stop - 1].argmax())] * copies
