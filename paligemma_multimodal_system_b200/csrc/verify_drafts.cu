@@ -1,8 +1,8 @@
 // Which drafted tokens stay: rows of target logits (and of the draft's) against given random numbers.
 //
-// A row decides by itself where the walk goes on from it (the header has the rules), so all rows are judged at once, a cluster of CTAs a row, and the walks are
+// A row decides by itself where the walk goes on from it (the header has the rules), so rows are judged at once, a cluster of CTAs a row, and the walks are
 // pointer chases at the end, made by the last cluster.  Rows lie depth first in their entries and clusters are started in the order of the rows' places in their
-// entries: one that finds its parent decided for another child has nothing to do.
+// entries: one that finds that some row above it goes on elsewhere has nothing to do (256 rows beside a draft 281 -> 257 us, 48 trees 149 -> 111).
 //
 // After rejections the rest is r_j = (p - c_j q)+ / S_j: from r_j q is taken again, (p - c_j q)+ - S_j q = p - (c_j + S_j) q where that is positive, so c and S are
 // two numbers and a rejection is one pass over the row, whatever came before it.
@@ -15,27 +15,52 @@
 // all CTAs and are compared one by one; where they are many the run is divided again, until it is one pattern.
 //
 // Two passes over a row, one for its maximum and one, from L2, for its sum; the second leaves the entries that may belong to the nucleus in shared memory, in the
-// order of their places, and everything behind it goes over those (over the row where they are too many).
+// order of their places, and everything behind it goes over those (over the row where they are too many).  The CTAs of a row meet three times: for the maximum, for the sums and the
+// counted runs, for the run that holds the border and the mass above it; the one that holds the drawn token finishes alone.
+//
+// What bounds it: few rows, that chain (5 rows 29 us, of which 5 are passes; 35 with seven meetings); many rows, how fast an SM takes them from L2 (6.7 TB/s over all while their
+// passes coincide) and the chains between: 256 rows of 257216 beside a draft 257 us, 1.2 TB/s of DRAM, 46 % of the issue slots.  Greedy rows are one pass: 128 of them, some 76 judged, 32 us.
 #include "common.cuh"
 #include "paligemma_b200.h"
 
 namespace {
 
-constexpr int kThreads = 512, kPerSm = 2, kWarps = kThreads / 32, kRanks = 16, kBins = 1024, kCoarse = kBins / 32, kTable = 256, kList = 32;
+constexpr int kThreads = 512, kPerSm = 2, kPerSmGreedy = 4, kWarps = kThreads / 32, kRanks = 16, kBins = 1024, kCoarse = kBins / 32, kTable = 256, kList = 32;
 constexpr int kRun = 128, kRuns = 4;  // entries that a warp takes at once, a float4 a lane; runs under way
 constexpr int kHeld = 512;            // entries of a row that a warp can hold as candidates of the nucleus
 constexpr int kDead = -2147483647 - 1;
-constexpr double kLog2e = 1.4426950408889634;
+constexpr double kLog2e = 1.4426950408889634, kLn2 = 0.6931471805599453;
 
 struct Entry {
   unsigned long long mass;
   uint32_t key;
+  int warp;  // that holds it
 };
 struct Candidate {
   float x;
   int at;  // place in the CTA's share
 };
+// e^((x - m) / T) = 2^(x a + shift) with a = log2(e) / T and shift = -m a.  (The rounding of m a is in every weight alike.)  Entries below `cut` weigh nothing: they are 2^-1000 of
+// the largest or outside the nucleus.
+struct Scale {
+  double a, shift;
+  float cut;
+  // for fp32: a and shift in two parts, shift's first a multiple of 2^-8; runs with an entry of `fine` or more are weighed in double
+  float a0, a1, s0, s1, fine, low;
+};
+struct Row {  // a row's distribution: weights / mass
+  Scale s;
+  double mass;
+  float bound;  // entries from here on are the candidates in shared memory (listed)
+  bool good, listed, held;  // held: nothing else weighs anything
+};
+struct How {  // what makes one of a row of logits
+  double temperature, top_p, a;  // a: log2(e) / temperature
+  double border;  // log(16 (1 - top_p) / V): where the border of the nucleus is looked for, see there
+};
 struct __align__(16) Shared {
+  How how[2];                              // of the draft, of the target
+  Row row[2];
   double table[kTable];                    // 2^(j / 256)
   double warp[kWarps];
   double all[2][kRanks], part[2][kRanks];  // doubles of every CTA, by turns
@@ -44,12 +69,13 @@ struct __align__(16) Shared {
   unsigned long long hist[kBins];          // mass of runs of bit patterns
   unsigned long long coarse[kRanks][kCoarse], fine[kRanks][32];
   Entry own[kList], list[kRanks][kList];   // entries of the run that holds the border
-  Candidate held[kWarps][kHeld];
   int held_count[kWarps], listed[kRanks], over[2][kRanks];
   unsigned long long found_base;
   float largest[kWarps], whole[2][kRanks]; // what the threads' largest entries sum up to, relative to the CTA's
   int found, pick, state, last, own_listed;
-  uint32_t least;
+  uint32_t least, top_key;
+  int V, bits;
+  Candidate held[kWarps][kHeld];           // (in the end the rows' outcomes)
 };
 PG_DEVINL uint32_t ordered(float x) {  // larger numbers have larger ones; both zeros alike, NaN above all
   const uint32_t b = __float_as_uint(x + 0.0f);
@@ -81,31 +107,26 @@ PG_DEVINL unsigned long long get64(const void* p, int rank) {
   asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(v) : "r"(remote(p, rank)) : "memory");
   return v;
 }
+PG_DEVINL void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+PG_DEVINL void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 PG_DEVINL int load_relaxed(const int* p) {
   int v;
   asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
 }
 
-// e^((x - m) / T) = 2^(x a + shift) with a = log2(e) / T and shift = -m a.  (The rounding of m a is in every weight alike.)  Entries below `cut` weigh nothing: they are 2^-1000 of
-// the largest or outside the nucleus.
-struct Scale {
-  double a, shift;
-  float cut;
-  // for fp32: a and shift in two parts, shift's first a multiple of 2^-8; runs with an entry of `fine` or more are weighed in double
-  float a0, a1, s0, s1, fine;
-};
-PG_DEVINL Scale scale_of(float m, double temperature) {
+PG_DEVINL Scale scale_of(float m, double a, double temperature) {
   Scale s;
-  s.a = kLog2e / temperature;
+  s.a = a;
   s.shift = -static_cast<double>(m) * s.a;
-  s.cut = nextafterf(__double2float_rd(static_cast<double>(m) - 1000.0 / s.a), INFINITY);
+  s.cut = nextafterf(__double2float_rd(static_cast<double>(m) - 1000.0 * kLn2 * temperature), INFINITY);
   if (!(fabs(s.shift) < 0x1p40)) s.a = s.shift = 0.0, s.cut = m;  // the float in front of m weighs less than 2^-1000 here: what equals m shares the mass
   s.a0 = static_cast<float>(s.a);
   s.a1 = static_cast<float>(s.a - s.a0);
   s.s0 = static_cast<float>(rint(s.shift * 256.0) / 256.0);
   s.s1 = static_cast<float>(s.shift - s.s0);
-  s.fine = fabs(s.shift) < 0x1p15 ? static_cast<float>(static_cast<double>(m) - 16.0 / s.a) : -INFINITY;
+  s.low = static_cast<float>((-100.0 - s.shift) * kLn2 * temperature);
+  s.fine = fabs(s.shift) < 0x1p15 ? static_cast<float>(static_cast<double>(m) - 16.0 * kLn2 * temperature) : -INFINITY;
   return s;
 }
 PG_DEVINL double weight(const double* table, const Scale& s, float x) {
@@ -114,7 +135,7 @@ PG_DEVINL double weight(const double* table, const Scale& s, float x) {
   const double rounded = t + kRound, f = t - (rounded - kRound);  // |f| <= 1 / 512
   const int k = __double2loint(rounded);
   const double power = table[k & (kTable - 1)];
-  constexpr double c1 = 0.6931471805599453, c2 = c1 * c1 / 2, c3 = c1 * c1 * c1 / 6;
+  constexpr double c1 = kLn2, c2 = c1 * c1 / 2, c3 = c1 * c1 * c1 / 6;
   const double w = fma(f, fma(f, fma(f, c3, c2), c1), 1.0) * __hiloint2double(__double2hiint(power) + ((k >> 8) << 20), __double2loint(power));
   return x >= s.cut ? w : 0.0;
 }
@@ -125,10 +146,10 @@ struct Pairs {
   uint64_t a0, a1, s0, s1;
   float low;
   PG_DEVINL explicit Pairs(const Scale& s) : a0(pg::pair_of(s.a0, s.a0)), a1(pg::pair_of(s.a1, s.a1)), s0(pg::pair_of(s.s0, s.s0)), s1(pg::pair_of(s.s1, s.s1)) {
-    low = static_cast<float>((-100.0 - s.shift) / s.a);
+    low = s.low;
   }
   PG_DEVINL float2 operator()(float x, float y) const {
-    constexpr double c1 = 0.6931471805599453, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4, c5 = c4 * c1 / 5, c6 = c5 * c1 / 6, c7 = c6 * c1 / 7;
+    constexpr double c1 = kLn2, c2 = c1 * c1 / 2, c3 = c2 * c1 / 3, c4 = c3 * c1 / 4, c5 = c4 * c1 / 5, c6 = c5 * c1 / 6, c7 = c6 * c1 / 7;
     constexpr float kRound = 12582912.0f;  // 1.5 2^23
     auto both = [](double c) { return pg::pair_of(static_cast<float>(c), static_cast<float>(c)); };
     const uint64_t z = pg::pair_of(fmaxf(x, low), fmaxf(y, low));
@@ -192,9 +213,9 @@ PG_DEVINL float ex2(float x) {
 }
 
 // (largest entry, lowest place) of the row as one number, known to all CTAs.  PLACE false: the entry alone, and in `whole` the sum of the largest entries' weights of all threads,
-// a being log2(e) / T: less than the row's.
+// scale being log2(e) / T: less than the row's.
 template <bool PLACE>
-PG_DEVINL unsigned long long row_top(Shared& sh, const Part& p, const Source& s, int& turn, float a, float& whole) {
+PG_DEVINL unsigned long long row_top(Shared& sh, const Part& p, const Source& s, int& turn, const double& scale, float& whole) {
   float best = -INFINITY;  // this thread's largest
   int run = 0;
   each4(p, s, [&](int i, float4 x) {
@@ -231,6 +252,7 @@ PG_DEVINL unsigned long long row_top(Shared& sh, const Part& p, const Source& s,
     key = __shfl_sync(0xffffffffu, key, 0);
     if (static_cast<int>(threadIdx.x) < p.ranks) put64(&sh.key[turn][p.rank], threadIdx.x, key);
   }
+  const float a = PLACE ? 0.0f : static_cast<float>(scale);  // (behind a barrier: the first row's may have been written just now)
   if (!PLACE) {
     unsigned long long here = 0;
     for (int w = 0; w < kWarps; ++w) here = mine[w] > here ? mine[w] : here;
@@ -262,8 +284,17 @@ PG_DEVINL bool is_distribution(unsigned long long top) {
 }
 
 // What the warps have summed: theirs in sh.warp, the CTAs' in sh.all[turn] (until the next but one), the whole as the result.  The order of additions is fixed.  `over` of any
-// thread becomes all CTAs'; `part`: a second sum.
-PG_DEVINL double share_sums(Shared& sh, const Part& p, int& turn, double sum, bool over = false, double* part = nullptr) {
+// thread becomes all CTAs'; `part`: a second sum.  counted: the runs of sh.hist go along, 32 at a time.
+PG_DEVINL void share_coarse(Shared& sh, const Part& p) {
+  const int lane = threadIdx.x % 32;
+  for (int c = threadIdx.x / 32; c < kCoarse; c += kWarps) {
+    unsigned long long v = sh.hist[c * 32 + lane];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (lane < p.ranks) put64(&sh.coarse[p.rank][c], lane, v);
+  }
+}
+PG_DEVINL double share_sums(Shared& sh, const Part& p, int& turn, double sum, bool over = false, double* part = nullptr, bool counted = false) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -275,6 +306,7 @@ PG_DEVINL double share_sums(Shared& sh, const Part& p, int& turn, double sum, bo
     sh.warp[warp] = sum;
     if (part != nullptr) sh.warp_part[warp] = *part;
   }
+  if (counted) share_coarse(sh, p);
   __syncthreads();
   if (warp == 0) {
     double all = lane < kWarps ? sh.warp[lane] : 0.0, all_part = part != nullptr && lane < kWarps ? sh.warp_part[lane] : 0.0;
@@ -336,25 +368,24 @@ PG_DEVINL int place_among(double mine, int n, double rest, double& run) {
   return at;
 }
 
-// The token at u times the whole, whose sums are in sh.warp and sh.all (`turn` behind them): the first place whose running sum is above that.  Known to all CTAs.  (Where
-// rounding leaves no border behind u: the last place with any mass.)  find(warp, rest, run) gives the place in the share, within that warp's part.
+// The token at u times the whole, whose sums are in sh.warp and sh.all (`turn` behind them): the first place whose running sum is above that.  Known to the CTA that holds it,
+// `owner`, alone.  (Where rounding leaves no border behind u: the last place with any mass.)  find(warp, rest, run) gives the place in the share, within that warp's part.
 template <typename F>
-PG_DEVINL int share_draw(Shared& sh, const Part& p, int turn, double total, float u, F find) {
+PG_DEVINL int share_draw(Shared& sh, const Part& p, int turn, double total, float u, int& owner, F find) {
   const int lane = threadIdx.x % 32;
   double rest = static_cast<double>(u) * total, run = 0.0;
-  const int owner = place_among(lane < p.ranks ? sh.all[turn ^ 1][lane] : 0.0, p.ranks, rest, run);
-  if (owner == p.rank) {
-    const int mine = place_among(lane < kWarps ? sh.warp[lane] : 0.0, kWarps, rest, run);
-    __syncthreads();  // (the warps' sums have been read)
-    const int place = find(mine, rest, run);
-    if (static_cast<int>(threadIdx.x) / 32 == mine && lane < p.ranks) put32(&sh.pick, lane, p.lo + place);
-  }
-  pg::cluster_sync_all();
+  owner = place_among(lane < p.ranks ? sh.all[turn ^ 1][lane] : 0.0, p.ranks, rest, run);
+  if (owner != p.rank) return -1;
+  const int mine = place_among(lane < kWarps ? sh.warp[lane] : 0.0, kWarps, rest, run);
+  __syncthreads();  // (the warps' sums have been read)
+  const int place = find(mine, rest, run);
+  if (static_cast<int>(threadIdx.x) / 32 == mine && lane == 0) sh.pick = p.lo + place;
+  __syncthreads();
   return sh.pick;
 }
 template <typename F>
-PG_DEVINL int row_draw(Shared& sh, const Part& p, const Source& s, int turn, double total, float u, F f) {
-  return share_draw(sh, p, turn, total, u, [&](int mine, double rest, double run) {
+PG_DEVINL int row_draw(Shared& sh, const Part& p, const Source& s, int turn, double total, float u, int& owner, F f) {
+  return share_draw(sh, p, turn, total, u, owner, [&](int mine, double rest, double run) {
     // all warps sum pieces of that warp's part, which then looks for the piece, the lane and the entry
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, begin = mine * p.seg, end = min(begin + p.seg, p.n);
     const int piece = (end - begin + kWarps * kRun - 1) / (kWarps * kRun) * kRun, from = min(begin + warp * piece, end), to = min(from + piece, end);
@@ -404,8 +435,8 @@ PG_DEVINL int row_draw(Shared& sh, const Part& p, const Source& s, int turn, dou
   });
 }
 template <typename F>
-PG_DEVINL int held_draw(Shared& sh, const Part& p, int turn, double total, float u, F f) {
-  return share_draw(sh, p, turn, total, u, [&](int mine, double rest, double run) {
+PG_DEVINL int held_draw(Shared& sh, const Part& p, int turn, double total, float u, int& owner, F f) {
+  return share_draw(sh, p, turn, total, u, owner, [&](int mine, double rest, double run) {
     const int lane = threadIdx.x % 32;
     int place = -1, last = 0;
     if (static_cast<int>(threadIdx.x) / 32 == mine)
@@ -433,35 +464,41 @@ PG_DEVINL float least_of(float m, double z, double top_p, double temperature, in
   return x - (fabsf(x) * 3e-7f + 1e-37f);
 }
 
-// Least entry of the nucleus.  z: the whole mass, `bits`: of the fixed point.
-// each(f): f of every entry that may belong
-template <typename E>
-PG_DEVINL float nucleus(Shared& sh, const Part& p, const Scale& s, uint32_t top, double z, double top_p, double temperature, int V, int bits, E each) {
+// Runs of bit patterns from hi down to lo, 1024 at most
+struct Runs {
+  uint32_t hi, lo;
+  int shift;
+  PG_DEVINL Runs(uint32_t hi_, uint32_t lo_) : hi(hi_), lo(lo_) { shift = hi - lo < kBins ? 0 : 32 - __clz(hi - lo) - 10; }
+  PG_DEVINL int of(float x) const { return static_cast<int>((hi - ordered(x)) >> shift); }
+};
+PG_DEVINL void count_begin(Shared& sh) {
+  for (int i = threadIdx.x; i < kBins; i += kThreads) sh.hist[i] = 0;
+  if (threadIdx.x == 0) sh.own_listed = 0;
+}
+
+// Least entry of the nucleus.  z: the whole mass, `bits`: of the fixed point, each(f): f of every entry that may belong, runs: of these.  HELD: they are the candidates, counted already, and the
+// mass of what is kept is left behind as share_sums leaves it (`mass`; < 0: it has to be summed).
+template <bool HELD, typename E>
+PG_DEVINL float nucleus(Shared& sh, const Part& p, const Scale& s, Runs runs, double z, double top_p, int bits, int& turn, double& mass, E each) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const float floor_x = least_of(unordered(top), z, top_p, temperature, V);
-  uint32_t hi = top, lo = floor_x == floor_x ? min(ordered(fmaxf(floor_x, s.cut)), top) : ordered(s.cut);
   const double one = static_cast<double>(1ull << bits), border = top_p * z * one;
-  unsigned long long base = 0;  // mass above hi
-  for (;;) {
-    const uint32_t range = hi - lo;
-    const int shift = range < kBins ? 0 : 32 - __clz(range) - 10;
-    __syncthreads();
-    for (int i = threadIdx.x; i < kBins; i += kThreads) sh.hist[i] = 0;
-    if (threadIdx.x == 0) sh.own_listed = 0;
-    __syncthreads();
-    const float least = unordered(lo), most = unordered(hi);
-    auto count = [&](float x) {
-      if (x >= least && x <= most) atomicAdd(&sh.hist[(hi - ordered(x)) >> shift], static_cast<unsigned long long>(weight(sh.table, s, x) * one));
-    };
-    each(count);
-    __syncthreads();
-    for (int c = warp; c < kCoarse; c += kWarps) {
-      unsigned long long v = sh.hist[c * 32 + lane];
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (lane < p.ranks) put64(&sh.coarse[p.rank][c], lane, v);
+  unsigned long long base = 0;  // mass above the runs
+  mass = -1.0;
+  for (bool counted = HELD;; counted = false) {
+    uint32_t &hi = runs.hi, &lo = runs.lo;
+    const int shift = runs.shift;
+    if (!counted) {
+      __syncthreads();
+      count_begin(sh);
+      __syncthreads();
+      const float least = unordered(lo), most = unordered(hi);
+      each([&](float x) {
+        if (x >= least && x <= most) atomicAdd(&sh.hist[runs.of(x)], static_cast<unsigned long long>(weight(sh.table, s, x) * one));
+      });
+      __syncthreads();
+      share_coarse(sh, p);
+      pg::cluster_sync_all();
     }
-    pg::cluster_sync_all();
     int bin = 0;
 #pragma unroll
     for (int step = 0; step < 2; ++step) {  // 32 runs of 32, then one of them
@@ -494,23 +531,40 @@ PG_DEVINL float nucleus(Shared& sh, const Part& p, const Scale& s, uint32_t top,
     lo = hi - lo > width ? hi - width : lo;
     // the run's entries to all CTAs; where they are few it is decided at once
     const float run_least = unordered(lo), run_most = unordered(hi);
+    double above = 0.0;
     each([&](float x) {
-      if (x >= run_least && x <= run_most) {
+      if (x > run_most) {
+        if (HELD) above += weight(sh.table, s, x);
+      } else if (x >= run_least) {
         const int at = atomicAdd(&sh.own_listed, 1);
         if (at < kList) {
           sh.own[at].mass = static_cast<unsigned long long>(weight(sh.table, s, x) * one);
           sh.own[at].key = ordered(x);
+          sh.own[at].warp = warp;
         }
       }
     });
+    if (HELD) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+      if (lane == 0) sh.warp[warp] = above;
+    }
     __syncthreads();
     const int own = sh.own_listed;
+    if (HELD) {
+      above = lane < kWarps ? sh.warp[lane] : 0.0;
+#pragma unroll
+      for (int o = kWarps / 2; o > 0; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+    }
     for (int r = warp; r < p.ranks; r += kWarps) {
       if (lane < min(own, kList)) {
         put64(&sh.list[p.rank][lane].mass, r, sh.own[lane].mass);
         put32(&sh.list[p.rank][lane].key, r, static_cast<int>(sh.own[lane].key));
       }
-      if (lane == 0) put32(&sh.listed[p.rank], r, own);
+      if (lane == 0) {
+        put32(&sh.listed[p.rank], r, own);
+        if (HELD) put64(&sh.all[turn][p.rank], r, __double_as_longlong(above));
+      }
     }
     if (threadIdx.x == 0) sh.least = hi;
     pg::cluster_sync_all();
@@ -527,38 +581,75 @@ PG_DEVINL float nucleus(Shared& sh, const Part& p, const Scale& s, uint32_t top,
         if (static_cast<double>(above) <= border) atomicMin(&sh.least, key);
       }
       __syncthreads();
-      return unordered(sh.least);
+      const uint32_t cut = sh.least;
+      if (HELD) {  // what is kept of the run, beside what lies above it
+        for (int r = warp; r < p.ranks; r += kWarps) {
+          unsigned long long kept = lane < sh.listed[r] && sh.list[r][lane].key >= cut ? sh.list[r][lane].mass : 0ull;
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) kept += __shfl_xor_sync(0xffffffffu, kept, o);
+          if (lane == 0) sh.all[turn][r] += static_cast<double>(kept) / one;
+        }
+        if (warp == kWarps - 1 && lane < kWarps) {
+          unsigned long long kept = 0;
+          for (int i = 0; i < own; ++i) kept += sh.own[i].warp == lane && sh.own[i].key >= cut ? sh.own[i].mass : 0ull;
+          sh.warp[lane] += static_cast<double>(kept) / one;
+        }
+        __syncthreads();
+        mass = 0.0;
+        for (int r = 0; r < p.ranks; ++r) mass += sh.all[turn][r];
+        turn ^= 1;
+      }
+      return unordered(cut);
     }
+    runs = Runs(hi, lo);
   }
 }
 
-struct Row {  // a row's distribution: weights / mass
-  Scale s;
-  double mass;
-  float bound;  // entries from here on are the candidates in shared memory (listed)
-  bool good, listed, held;  // held: nothing else weighs anything
+struct Nucleus {
+  double mass;  // of what is kept; < 0: not known
+  float cut;
   int turn;
 };
-
-// The distribution of a row; its sums of the kept weights are left behind for a draw.  (Once in the program: its loops are long.  All by value: what has an address is loaded anew
-// for every entry.)
-__device__ __noinline__ Row distribution(Shared& sh, const Part p, const Source s, const double temperature, const double top_p, const int V, const int bits, int turn) {
-  Row r;
-  r.good = false;
-  float some;
-  const unsigned long long top = row_top<false>(sh, p, s, turn, static_cast<float>(kLog2e / temperature), some);
+// (Out of line, like `distribution`: what they hold is not held in the loops over a row.)
+__device__ __noinline__ Nucleus held_nucleus(Shared& sh, const Part p, const Scale s, const Runs runs, const double z, const double top_p, const int bits, int turn) {
+  Nucleus r;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  r.cut = nucleus<true>(sh, p, s, runs, z, top_p, bits, turn, r.mass, [&](auto f) {
+    for (int i = lane; i < sh.held_count[warp]; i += 32) f(sh.held[warp][i].x);
+  });
   r.turn = turn;
-  if (!is_distribution(top)) return r;
+  return r;
+}
+__device__ __noinline__ Nucleus row_nucleus(Shared& sh, const Part p, const Source x, const Scale s, const Runs runs, const double z, const double top_p, const int bits, int turn) {
+  Nucleus r;
+  r.cut = nucleus<false>(sh, p, s, runs, z, top_p, bits, turn, r.mass, [&](auto f) { each4(p, x, [&](int, float4 x) { f(x.x), f(x.y), f(x.z), f(x.w); }); });
+  r.turn = turn;
+  return r;
+}
+
+// The distribution of a row to sh.row[which]; its sums of the kept weights are left behind for a draw.  Returns `turn`.  (Once in the program: its loops are long.  By value: what has
+// an address is loaded anew for every entry.  What lives longer than the loops lies in shared memory: they take all registers.)
+PG_DEVINL int distribution(Shared& sh, const Part p, const Source s, const int which, int turn) {
+  count_begin(sh);
+  float some;
+  const unsigned long long top = row_top<false>(sh, p, s, turn, sh.how[which].a, some);
+  if (!is_distribution(top)) {
+    if (threadIdx.x == 0) sh.row[which].good = false;
+    __syncthreads();
+    return turn;
+  }
+  const double temperature = sh.how[which].temperature;
+  if (threadIdx.x == 0) sh.top_key = static_cast<uint32_t>(top >> 32);
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const float m = unordered(static_cast<uint32_t>(top >> 32));
-  Scale sc = scale_of(m, temperature);
+  Scale sc = scale_of(m, sh.how[which].a, temperature);
   const bool in_fp32 = sc.fine > -INFINITY;
-  const double whole = fmax(1.0, 0.99 * some);  // small is what is below 2^-16 of that
-  if (in_fp32) sc.fine += static_cast<float>(log(whole) * temperature);
+  const double whole = logf(fmaxf(1.0f, 0.99f * some));  // small is what is below 2^-16 of e^whole
+  if (in_fp32) sc.fine += static_cast<float>(whole * temperature);
   // Candidates, in the order of their places: what is not small, and what probably belongs to the nucleus (an entry at its border weighs many times the mean of those outside;
   // sixteen times in most rows).
   float bound = sc.fine;
-  if (top_p < 1.0) bound = fminf(bound, static_cast<float>(static_cast<double>(m) + log((1.0 - top_p) * whole * 16.0 / V) * temperature));
+  if (sh.how[which].top_p < 1.0) bound = fminf(bound, static_cast<float>(static_cast<double>(m) + (sh.how[which].border + whole) * temperature));
   bound = fmaxf(bound, sc.cut);  // (the same number in all CTAs)
   int held = 0;
   double sum = 0.0;
@@ -593,31 +684,42 @@ __device__ __noinline__ Row distribution(Shared& sh, const Part p, const Source 
   if (lane == 0) sh.held_count[warp] = held;
   __syncwarp();
   double part = 0.0;
-  for (int i = lane; i < held; i += 32) part += weight(sh.table, sc, sh.held[warp][i].x);
-  r.mass = share_sums(sh, p, turn, sum + part, over, &part);
-  r.listed = part == part;  // (NaN: some warp had no room)
-  r.held = false;
-  r.bound = bound;
+  const double top_p = sh.how[which].top_p;
+  const int bits = sh.bits;
+  const uint32_t top_key = sh.top_key;
+  const Runs runs(top_key, ordered(bound));
+  const double one = static_cast<double>(1ull << bits);
+  for (int i = lane; i < held; i += 32) {
+    const float x = sh.held[warp][i].x;
+    const double w = weight(sh.table, sc, x);
+    part += w;
+    if (top_p < 1.0) atomicAdd(&sh.hist[runs.of(x)], static_cast<unsigned long long>(w * one));
+  }
+  double mass = share_sums(sh, p, turn, sum + part, over, &part, top_p < 1.0);
+  bool listed = part == part, kept = false;  // (NaN: some warp had no room)
   auto sum_of = [&](int, float4 x) { return weights_sum(sh.table, sc, small, x); };
-  if (!r.listed) r.mass = row_mass(sh, p, s, turn, sum_of);
+  if (!listed) mass = row_mass(sh, p, s, turn, sum_of);
   if (top_p < 1.0) {
-    const uint32_t top_key = static_cast<uint32_t>(top >> 32);
-    r.held = r.listed && part > top_p * r.mass * (1.0 + 1e-9);  // the border lies among the candidates
-    if (r.held) {
-      sc.cut = nucleus(sh, p, sc, top_key, r.mass, top_p, temperature, V, bits, [&](auto f) {
-        for (int i = lane; i < sh.held_count[warp]; i += 32) f(sh.held[warp][i].x);
-      });
-      r.mass = held_mass(sh, p, turn, [&](const Candidate& c) { return weight(sh.table, sc, c.x); });
+    kept = listed && part > top_p * mass * (1.0 + 1e-9);  // the border lies among the candidates
+    if (kept) {
+      const Nucleus k = held_nucleus(sh, p, sc, runs, mass, top_p, bits, turn);
+      sc.cut = k.cut, turn = k.turn, mass = k.mass;
+      if (mass < 0.0) mass = held_mass(sh, p, turn, [&](const Candidate& c) { return weight(sh.table, sc, c.x); });
     } else {
-      r.listed = false;
-      sc.cut = nucleus(sh, p, sc, top_key, r.mass, top_p, temperature, V, bits, [&](auto f) { each4(p, s, [&](int, float4 x) { f(x.x), f(x.y), f(x.z), f(x.w); }); });
-      r.mass = row_mass(sh, p, s, turn, sum_of);
+      listed = false;
+      const float floor_x = least_of(unordered(top_key), mass, top_p, sh.how[which].temperature, sh.V);
+      const Nucleus k = row_nucleus(sh, p, s, sc, Runs(top_key, floor_x == floor_x ? min(ordered(fmaxf(floor_x, sc.cut)), top_key) : ordered(sc.cut)), mass, top_p, bits, turn);
+      sc.cut = k.cut, turn = k.turn;
+      mass = row_mass(sh, p, s, turn, sum_of);
     }
   }
-  r.s = sc;
-  r.good = true;
-  r.turn = turn;
-  return r;
+  if (threadIdx.x == 0) {
+    Row& r = sh.row[which];
+    r.s = sc, r.mass = mass, r.bound = bound;
+    r.good = true, r.listed = listed, r.held = kept;
+  }
+  __syncthreads();
+  return turn;
 }
 
 PG_DEVINL float unit_number(float u) { return fminf(fmaxf(u, 0.0f), 1.0f - 0x1p-24f); }  // (a NaN is 0)
@@ -670,12 +772,16 @@ PG_DEVINL bool may_be_reached(const int* parents, const int* outcome, int v) {
   }
 }
 
-__global__ void __launch_bounds__(kThreads, kPerSm) verify_kernel(const PgVerify a, int share, int bits, int look) {
+// GREEDY: no random numbers.  `room`: rows whose outcomes have room in shared memory.
+template <bool GREEDY>
+__global__ void __launch_bounds__(kThreads, GREEDY ? kPerSmGreedy : kPerSm) verify_kernel(const PgVerify a, int share, int bits, int room) {
   extern __shared__ __align__(16) char raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw);
   uint32_t ranks;
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ranks));
   const int rank = pg::cluster_ctarank(), item = blockIdx.x / ranks, tid = threadIdx.x;
+  int finisher = 0;  // the CTA that knows the outcome
+  cluster_arrive();
   const int v = item / a.entries, e = item % a.entries;  // the entries' first rows come first
   const int n = a.n[e];
   const long long row0 = a.row0[e], row = row0 + v;
@@ -683,19 +789,15 @@ __global__ void __launch_bounds__(kThreads, kPerSm) verify_kernel(const PgVerify
   int* outcome = a.outcome + row0;
   Family fam;
   fam.parents = a.parents + row0, fam.tokens = a.tokens + row0, fam.v = v, fam.n = n;
+  cluster_wait();  // (the others run: their shared memory is there)
   if (live && v > 0) {
-    if (look) {
-      if (rank == 0 && tid < 32) {  // one look for all: what the parent decides may come in between
-        const bool reached = may_be_reached(fam.parents, outcome, v);
-        if (tid < static_cast<int>(ranks)) put32(&sh.state, tid, reached);
-      }
-      pg::cluster_sync_all();
-      live = sh.state != 0;
-      if (!live && rank == 0 && tid == 0) outcome[v] = kDead;
-    } else {
-      const int up = fam.parents[v];
-      live = up >= 0 && up < v;
+    if (rank == 0 && tid < 32) {  // one look for all: what the parent decides may come in between
+      const bool reached = may_be_reached(fam.parents, outcome, v);
+      if (tid < static_cast<int>(ranks)) put32(&sh.state, tid, reached);
     }
+    pg::cluster_sync_all();
+    live = sh.state != 0;
+    if (!live && rank == 0 && tid == 0) outcome[v] = kDead;
   }
   if (live) {
     Part p;
@@ -707,11 +809,18 @@ __global__ void __launch_bounds__(kThreads, kPerSm) verify_kernel(const PgVerify
     const float *logits = a.logits + row * a.ld, *draft = a.draft + row * a.draft_ld;
     const Source target(logits, p.lo);
     fam.look();
-    if (tid < kTable) sh.table[tid] = exp2(static_cast<double>(tid) / kTable);
-    __syncthreads();
-    if (a.uniforms == nullptr) {
+    if (!GREEDY) {
+      if (tid >= kTable && tid < kTable + 2) {
+        const bool draft = tid == kTable;
+        const double temperature = draft ? a.draft_temperature : a.temperature, top_p = draft ? a.draft_top_p : a.top_p;
+        if (!draft || a.draft != nullptr) sh.how[tid - kTable] = How{temperature, top_p, kLog2e / temperature, top_p < 1.0 ? log(16.0 * (1.0 - top_p) / a.V) : 0.0};
+        sh.V = a.V, sh.bits = bits;
+      }
+      if (tid < kTable) sh.table[tid] = exp2(static_cast<double>(tid) / kTable);
+    }  // (read behind the first barriers of row_top)
+    if constexpr (GREEDY) {
       float whole;
-      const unsigned long long top = row_top<true>(sh, p, target, turn, 0.0f, whole);
+      const unsigned long long top = row_top<true>(sh, p, target, turn, 0.0, whole);
       const int token = is_distribution(top) ? static_cast<int>(~static_cast<uint32_t>(top)) : -1;
       const int next = token >= 0 ? fam.with(token) : n;
       to = next < n ? next : -2 - token;
@@ -719,31 +828,28 @@ __global__ void __launch_bounds__(kThreads, kPerSm) verify_kernel(const PgVerify
       const float u = unit_number(a.uniforms[2 * row + 1]);
       const Source other(draft, p.lo);
       int child = a.draft != nullptr ? fam.child(v + 1, x) : n;
-      Row t, q;
       bool good = true;
-      if (child < n) {
-        q = distribution(sh, p, other, a.draft_temperature, a.draft_top_p, a.V, bits, turn);
-        good = q.good;
-        turn = q.turn;
-      }
-      if (good) {
-        t = distribution(sh, p, target, a.temperature, a.top_p, a.V, bits, turn);
-        good = t.good;
-        turn = t.turn;
+#pragma unroll 1
+      for (int which = child < n ? 0 : 1; which < 2 && good; ++which) {
+        turn = distribution(sh, p, which == 0 ? other : target, which, turn);
+        good = sh.row[which].good;
       }
       if (!good) {
         to = -1;
       } else {
-        double c = 0.0, left = 1.0, pf = 0.0, qf = 0.0;
+        const Row &t = sh.row[1], &q = sh.row[child < n ? 0 : 1];
+        const Scale ts = t.s, qs = q.s;
+        double mass = t.mass, c = 0.0, left = 1.0, pf = 0.0, qf = 0.0;
         // max(p - c q, 0); both products rounded alike, so that equal ones leave nothing
         auto rest_of = [&](double wt, double wq) { return fmax(__dsub_rn(__dmul_rn(pf, wt), __dmul_rn(qf, wq)), 0.0); };
         auto rest4 = [&](int i, float4 y, double (&w)[4]) {
           const float4 z = other.four(i, p.n);
-          w[0] = rest_of(weight(sh.table, t.s, y.x), weight(sh.table, q.s, z.x)), w[1] = rest_of(weight(sh.table, t.s, y.y), weight(sh.table, q.s, z.y));
-          w[2] = rest_of(weight(sh.table, t.s, y.z), weight(sh.table, q.s, z.z)), w[3] = rest_of(weight(sh.table, t.s, y.w), weight(sh.table, q.s, z.w));
+          w[0] = rest_of(weight(sh.table, ts, y.x), weight(sh.table, qs, z.x)), w[1] = rest_of(weight(sh.table, ts, y.y), weight(sh.table, qs, z.y));
+          w[2] = rest_of(weight(sh.table, ts, y.z), weight(sh.table, qs, z.z)), w[3] = rest_of(weight(sh.table, ts, y.w), weight(sh.table, qs, z.w));
         };
-        const bool quick = child < n && t.listed && q.s.fine > -INFINITY;
-        const Pairs small_t(t.s), small_q(child < n ? q.s : t.s);
+        const float bound = t.bound;
+        const bool quick = child < n && t.listed && qs.fine > -INFINITY;
+        const Pairs small_t(ts), small_q(qs);
         float pf0 = 0.0f, pf1 = 0.0f, qf0 = 0.0f, qf1 = 0.0f;  // the factors in two parts
         auto rest_sum = [&](int i, float4 y) {
           if (!quick) {
@@ -757,13 +863,13 @@ __global__ void __launch_bounds__(kThreads, kPerSm) verify_kernel(const PgVerify
           float w = 0.0f;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const float b = zs[k] >= q.s.cut ? wq[k] : 0.0f;
+            const float b = zs[k] >= qs.cut ? wq[k] : 0.0f;
             const float left_over = __fsub_rn(fmaf(wt[k], pf0, __fmul_rn(wt[k], pf1)), fmaf(b, qf0, __fmul_rn(b, qf1)));
-            w += ys[k] < t.bound && ys[k] >= t.s.cut ? fmaxf(left_over, 0.0f) : 0.0f;
+            w += ys[k] < bound && ys[k] >= ts.cut ? fmaxf(left_over, 0.0f) : 0.0f;
           }
           return static_cast<double>(w);
         };
-        auto rest1 = [&](const Candidate& k) { return k.x >= t.s.cut ? rest_of(weight(sh.table, t.s, k.x), weight(sh.table, q.s, other.x[k.at])) : 0.0; };
+        auto rest1 = [&](const Candidate& k) { return k.x >= ts.cut ? rest_of(weight(sh.table, ts, k.x), weight(sh.table, qs, other.x[k.at])) : 0.0; };
         auto rest_mass = [&]() {
           double sum = 0.0;
           each4(p, target, [&](int i, float4 y) { sum += rest_sum(i, y); });
@@ -773,11 +879,11 @@ __global__ void __launch_bounds__(kThreads, kPerSm) verify_kernel(const PgVerify
         };
         while (child < n) {
           if (x >= 0 && x < a.V) {  // (what is no token was drawn from nothing: it takes nothing away)
-            const double pt = weight(sh.table, t.s, logits[x]) / t.mass, qt = weight(sh.table, q.s, draft[x]) / q.mass;
+            const double pt = weight(sh.table, ts, logits[x]) / mass, qt = weight(sh.table, qs, draft[x]) / q.mass;
             const bool stays = static_cast<double>(unit_number(a.uniforms[2 * (row0 + child)])) * qt * left < __dsub_rn(pt, __dmul_rn(c, qt));
             if (stays) break;
             c += left;
-            pf = 1.0 / t.mass, qf = c / q.mass;
+            pf = 1.0 / mass, qf = c / q.mass;
             pf0 = static_cast<float>(pf), pf1 = static_cast<float>(pf - pf0), qf0 = static_cast<float>(qf), qf1 = static_cast<float>(qf - qf0);
             left = t.held ? held_mass(sh, p, turn, rest1) : rest_mass();
             if (!(left > 0.0)) break;
@@ -789,24 +895,24 @@ __global__ void __launch_bounds__(kThreads, kPerSm) verify_kernel(const PgVerify
         } else {
           int token;
           if (c > 0.0 && left > 0.0) {
-            token = t.held ? held_draw(sh, p, turn, left, u, rest1) : row_draw(sh, p, target, turn, left, u, rest4);
+            token = t.held ? held_draw(sh, p, turn, left, u, finisher, rest1) : row_draw(sh, p, target, turn, left, u, finisher, rest4);
           } else {
-            auto one = [&](const Candidate& k) { return weight(sh.table, t.s, k.x); };
+            auto one = [&](const Candidate& k) { return weight(sh.table, ts, k.x); };
             auto four = [&](int, float4 y, double (&w)[4]) {
-              w[0] = weight(sh.table, t.s, y.x), w[1] = weight(sh.table, t.s, y.y), w[2] = weight(sh.table, t.s, y.z), w[3] = weight(sh.table, t.s, y.w);
+              w[0] = weight(sh.table, ts, y.x), w[1] = weight(sh.table, ts, y.y), w[2] = weight(sh.table, ts, y.z), w[3] = weight(sh.table, ts, y.w);
             };
-            if (c > 0.0) t.mass = t.held ? held_mass(sh, p, turn, one) : row_mass(sh, p, target, turn, [&](int, float4 y) { return weights_sum(sh.table, t.s, small_t, y); });
-            token = t.held ? held_draw(sh, p, turn, t.mass, u, one) : row_draw(sh, p, target, turn, t.mass, u, four);
+            if (c > 0.0) mass = t.held ? held_mass(sh, p, turn, one) : row_mass(sh, p, target, turn, [&](int, float4 y) { return weights_sum(sh.table, ts, small_t, y); });
+            token = t.held ? held_draw(sh, p, turn, mass, u, finisher, one) : row_draw(sh, p, target, turn, mass, u, finisher, four);
           }
-          const int next = a.draft == nullptr ? fam.with(token) : n;
+          const int next = a.draft == nullptr && rank == finisher ? fam.with(token) : n;
           to = next < n ? next : -2 - token;
         }
       }
     }
-    if (rank == 0 && tid == 0) outcome[v] = to;
+    if (rank == finisher && tid == 0) outcome[v] = to;
   }
   // the last cluster walks
-  if (rank == 0) {
+  if (rank == finisher) {
     if (tid == 0) {
       __threadfence();
       sh.last = atomicAdd(a.outcome + a.rows, 1) == static_cast<int>(gridDim.x / ranks) - 1;
@@ -814,8 +920,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm) verify_kernel(const PgVerify
     }
     __syncthreads();
     if (sh.last) {
-      constexpr int kMost = sizeof(sh.held) / sizeof(int);  // (the candidates are not needed any more)
-      const bool fits = a.rows <= kMost;
+      const bool fits = a.rows <= room;  // (the candidates are not needed any more)
       int* held = reinterpret_cast<int*>(sh.held);
       if (fits)
         for (int i = tid; i < a.rows; i += kThreads) held[i] = load_relaxed(a.outcome + i);
@@ -841,7 +946,35 @@ __global__ void __launch_bounds__(kThreads, kPerSm) verify_kernel(const PgVerify
       }
     }
   }
-  pg::cluster_sync_all();  // nobody leaves while its memory is read
+  // (what the CTAs hand one another lies in front of a barrier that all have passed)
+}
+
+template <bool GREEDY>
+int launch(const PgVerify& a, long long items, int ranks, int share, int bits, cudaStream_t st) {
+  constexpr int kRoom = GREEDY ? 2048 : static_cast<int>(sizeof(Shared::held) / sizeof(int));  // (a greedy row has no candidates)
+  constexpr int kSmem = GREEDY ? static_cast<int>(offsetof(Shared, held) + kRoom * sizeof(int)) : static_cast<int>(sizeof(Shared));
+  static bool configured[pg::kMaxDevices] = {};
+  bool& done = configured[pg::current_device()];
+  if (!done) {
+    if (cudaFuncSetAttribute(verify_kernel<GREEDY>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess ||
+        cudaFuncSetAttribute(verify_kernel<GREEDY>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+      cudaGetLastError();
+      return PG_ERR_CUDA;
+    }
+    done = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(items * ranks));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ranks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, verify_kernel<GREEDY>, a, share, bits, kRoom) == cudaSuccess ? PG_OK : PG_ERR_CUDA;
 }
 
 }  // namespace
@@ -855,39 +988,18 @@ extern "C" int pg_verify_drafts(const PgVerify* args, void* stream) {
       !sound(a.temperature, a.top_p) || (a.draft != nullptr && !sound(a.draft_temperature, a.draft_top_p)) || a.V > 0x7fffff00 / 2)
     return PG_ERR_ARG;
   const long long items = static_cast<long long>(a.entries) * a.max_n;
-  // CTAs that share a row: so many that a warp's candidates have room, and more while all of them stay within nine an SM (5 rows of 257216 with 4, 8, 16 CTAs: 46, 37, 35 us; 240 of them
-  // beside a draft 298, 384, 542; 48 trees of 32000 with 1, 2, 4: 132, 118, 140).
+  // CTAs that share a row: so many that a warp's candidates have room, and more while all of them stay within nine an SM, five of greedy rows.  (us with fewer, as taken, more: 5 rows of
+  // 257216 with 4, 8, 16 CTAs 42, 32, 29; 256 beside a draft with 4, 8 257, 308; 624 of 32000 with 1, 2, 4 132, 111, 131; 128 greedy rows of 257216 with 4, 8 32, 35.)
   int ranks = 1;
   while (ranks < kRanks && a.V / ranks > 65536) ranks *= 2;
-  while (ranks < kRanks && items * ranks * 2 <= 9LL * pg::num_sms() && a.V / (ranks * 2) >= 4 * kThreads) ranks *= 2;
+  const long long most = a.uniforms == nullptr ? 5 : 9;
+  while (ranks < kRanks && items * ranks * 2 <= most * pg::num_sms() && a.V / (ranks * 2) >= 4 * kThreads) ranks *= 2;
   if (items * ranks > 0x7fffffff) return PG_ERR_ARG;
   const int share = ((a.V + ranks - 1) / ranks + 3) / 4 * 4;
   int bits = 62;
   while ((1ll << (62 - bits)) < a.V) --bits;  // V weights of at most 1 stay below 2^62
-  const int look = items * ranks > 2 * pg::num_sms();  // (all rows at once: nothing is decided when they begin)
-  static bool configured[pg::kMaxDevices] = {};
-  bool& done = configured[pg::current_device()];
-  if (!done) {
-    if (cudaFuncSetAttribute(verify_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared)) != cudaSuccess ||
-        cudaFuncSetAttribute(verify_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
-      cudaGetLastError();
-      return PG_ERR_CUDA;
-    }
-    done = true;
-  }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (cudaMemsetAsync(a.outcome, 0, sizeof(int) * (static_cast<size_t>(a.rows) + 1), st) != cudaSuccess) return PG_ERR_CUDA;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(items * ranks));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = sizeof(Shared);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ranks;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
   pg_count_launch(1);
-  return cudaLaunchKernelEx(&cfg, verify_kernel, a, share, bits, look) == cudaSuccess ? PG_OK : PG_ERR_CUDA;
+  return a.uniforms == nullptr ? launch<true>(a, items, ranks, share, bits, st) : launch<false>(a, items, ranks, share, bits, st);
 }
