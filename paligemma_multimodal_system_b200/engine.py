@@ -54,11 +54,13 @@ class LookupDrafter:
         self.most, self.match = int(most), int(match)
 
     def __call__(self, history: List[int]):
-        for n in range(min(self.match, len(history) - 1), 0, -1):
-            tail = history[-n:]
-            for at in range(len(history) - n - 1, -1, -1):
-                if history[at:at + n] == tail:
-                    tokens = history[at + n:at + n + self.most]
+        back = history[::-1]  # (newest first)
+        for n in range(min(self.match, len(back) - 1), 0, -1):
+            at = 0
+            for _ in range(back.count(back[0]) - 1):
+                at = back.index(back[0], at + 1)
+                if back[at:at + n] == back[:n]:
+                    tokens = back[max(0, at - self.most):at][::-1]
                     return tokens, list(range(-1, len(tokens) - 1))
         return [], []
 

@@ -77,3 +77,46 @@ def test_every_operand_is_in_the_table():
     q = seq_ops.QuantizedPages(torch.zeros(6, 64, 48, dtype=torch.uint8).as_subclass(_OnDevice), torch.zeros(6, 3, 64, dtype=torch.uint8).as_subclass(_OnDevice))
     c = seq_ops.CachePages([pages(6, 64, 33), q], 64)
     assert c.count == 3 and c.table.numel() == 32 * 3 and c.most_page_bytes == 64 * 66 and c.most_columns == 33
+
+
+def test_shared_pages_are_free_when_all_owners_have_given_them_back():
+    from paligemma_multimodal_system_b200.cache import PagePool, SequenceStore
+    pool = PagePool(6)
+    mine = pool.take(3)
+    pool.share(mine[:2])
+    pool.share(mine[:1])
+    pool.give(mine)
+    assert sorted(pool.free) == [2, 3, 4, 5]
+    pool.give(mine[:2])
+    assert sorted(pool.free) == [1, 2, 3, 4, 5]
+    pool.give(mine[:1])
+    assert sorted(pool.free) == list(range(6)) and not pool.shared
+    with pytest.raises(RuntimeError):
+        pool.give(mine[:1])
+    store = SequenceStore([("kv", 8, 8)], 64 * 10, 4, torch.float32, allocate=False)
+    store.admit("a")
+    store.reserve("a", 150)
+    store.commit("a", 150)
+    b, c = store.fork("a", ["b", "c"])
+    assert b.pages[:2] == c.pages[:2] == store.live["a"].pages[:2] and len({*store.live["a"].pages, *b.pages, *c.pages}) == 5 and b.length == c.length == 150
+    (d,) = store.fork("b", ["d"], length=128)
+    assert d.pages == b.pages[:2] and d.length == 128 and store.pool.shared == {p: 4 for p in d.pages}
+    for rid in ("a", "d", "b"):
+        store.release(rid)
+    assert len(store.pool.free) == 7
+    store.release("c")
+    assert len(store.pool.free) == 10 and not store.pool.shared and len(store.free_slots) == 4
+
+
+@pytest.mark.parametrize("history,most,match,tokens", [([], 4, 3, []), ([5], 4, 3, []), ([5, 5], 4, 3, [5]), ([1, 2, 3, 9, 1, 2, 3], 2, 3, [9, 1]), ([1, 2, 8, 7, 2], 4, 3, [8, 7, 2]),
+                                                       ([4, 1, 2, 7, 3, 2, 6, 1, 2], 3, 2, [7, 3, 2]), ([1, 2, 3, 4], 4, 3, []), ([6, 6, 6, 6], 4, 2, [6])])
+def test_guesses_from_the_text(history, most, match, tokens):
+    from paligemma_multimodal_system_b200.engine import LookupDrafter
+    assert LookupDrafter(most, match)(history) == (tokens, list(range(-1, len(tokens) - 1)))
+
+
+def test_guesses_need_something_to_go_by():
+    from paligemma_multimodal_system_b200.engine import LookupDrafter
+    for bad in ((0, 3), (4, 0), (-1, 3)):
+        with pytest.raises(ValueError):
+            LookupDrafter(*bad)
