@@ -165,29 +165,22 @@ PG_DEVINL void copy_rows(const PgAdapter& a, const int* row_of, int count, int r
   else copy_pieces<uint16_t>(a, row_of, count, rank, ranks, a.F * kOut, kOut);
 }
 
-// Eight numbers of v, the CTAs' shares added in their order; N of them at once, all CTAs' asked for together
-template <int N>
-PG_DEVINL void joined8(const float* (&from)[N], int ranks, float (&f)[N][8]) {
+// Eight numbers of v, the CTAs' shares added in their order, two asked for at once
+PG_DEVINL void joined8(const float* from, int ranks, float (&f)[8]) {
   const int own = pg::cluster_ctarank();
 #pragma unroll
-  for (int n = 0; n < N; ++n)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[n][i] = 0.0f;
+  for (int i = 0; i < 8; ++i) f[i] = 0.0f;
   for (int p = 0; p < ranks; p += 2) {
-    float4 v[2][N][2];
+    float4 v[2][2];
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
-      for (int n = 0; n < N; ++n)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) v[k][n][h] = get_f4(from[n] + 4 * h, min(p + k, ranks - 1), own);
+      for (int h = 0; h < 2; ++h) v[k][h] = get_f4(from + 4 * h, min(p + k, ranks - 1), own);
 #pragma unroll
     for (int k = 0; k < 2; ++k)
       if (p + k < ranks)
 #pragma unroll
-        for (int n = 0; n < N; ++n)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) f[n][4 * h] += v[k][n][h].x, f[n][4 * h + 1] += v[k][n][h].y, f[n][4 * h + 2] += v[k][n][h].z, f[n][4 * h + 3] += v[k][n][h].w;
+        for (int h = 0; h < 2; ++h) f[4 * h] += v[k][h].x, f[4 * h + 1] += v[k][h].y, f[4 * h + 2] += v[k][h].z, f[4 * h + 3] += v[k][h].w;
   }
 }
 
@@ -201,10 +194,9 @@ PG_DEVINL void join_shares(const PgAdapter& a, const Layout& lay, const float* p
 #pragma unroll
     for (int k = 0; k < VT; ++k) t[k] = zero4();
     if (m < count && r < a.rank) {
-      const float* from[1] = {partial + m * lay.partial_ld + part * a.rank + r};
-      float f[1][8];
-      joined8(from, ranks, f);
-      split8<VT>(f[0], t);
+      float f[8];
+      joined8(partial + m * lay.partial_ld + part * a.rank + r, ranks, f);
+      split8<VT>(f, t);
     }
 #pragma unroll
     for (int k = 0; k < VT; ++k) *reinterpret_cast<uint4*>(vt + (k * M + m) * lay.v_ld + c) = t[k];

@@ -983,7 +983,7 @@ def verify_drafts(logits: torch.Tensor, b: StepBatch, uniforms: Optional[torch.T
             raise ValueError("a temperature is above 1e-30 and finite")
         if not 0.0 <= float(p) <= 1.0:
             raise ValueError("top_p is 0 .. 1")
-    for t in (uniforms, draft_logits, b.parents, b.tokens):
+    for t in (uniforms, draft_logits, b.parents, b.tokens, b.row0, b.n):
         if t is not None and t.device != logits.device:
             raise ValueError(f"logits, random numbers and the step lie on one device: got {t.device} and {logits.device}")
     _on_current_device(logits)

@@ -143,7 +143,7 @@ def test_a_plan_that_is_filled_again_under_a_graph():
         compare(Z, value, bound)
 
 
-@pytest.mark.parametrize("rank,parts", [(100, [320, 200]), (128, [264]), (8, [16, 130, 8, 300, 24, 128, 129, 40]), (64, [128, 640, 72]), (72, [1000]), (16, [3])])
+@pytest.mark.parametrize("rank,parts", [(100, [320, 200]), (128, [264]), (8, [16, 130, 8, 300, 24, 128, 129, 40]), (64, [128, 640, 72]), (72, [1000]), (16, [3]), (128, [64, 40, 24]), (128, [24] * 8)])
 @pytest.mark.parametrize("dtype,out", FORMS[:2])
 @pytest.mark.parametrize("ns,who,slots", [([300], [0], 1), ([150, 1, 260, 128, 1], [1, 0, -1, 1, 1], 2)])
 def test_tiles_of_many_rows(rank, parts, dtype, out, ns, who, slots):
