@@ -417,9 +417,10 @@ __global__ void __launch_bounds__(kThreads, 2) adapter_rows_kernel(const PgAdapt
   }
   pg::cluster_sync_all();
   join_shares<M, VT>(a, lay, partial, vt, tile.count, ranks);
+  pg::cluster_arrive();
   __syncthreads();
   columns.run(vt);
-  pg::cluster_sync_all();  // nobody leaves while its share is read
+  pg::cluster_wait();  // nobody leaves while its share is read
 }
 
 // Tiles of 128 bf16 rows, both products on the tensor cores with their sums in tensor memory.

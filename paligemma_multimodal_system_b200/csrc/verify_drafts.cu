@@ -107,8 +107,6 @@ PG_DEVINL unsigned long long get64(const void* p, int rank) {
   asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(v) : "r"(remote(p, rank)) : "memory");
   return v;
 }
-PG_DEVINL void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-PG_DEVINL void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 PG_DEVINL int load_relaxed(const int* p) {
   int v;
   asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
@@ -781,7 +779,7 @@ __global__ void __launch_bounds__(kThreads, GREEDY ? kPerSmGreedy : kPerSm) veri
   asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ranks));
   const int rank = pg::cluster_ctarank(), item = blockIdx.x / ranks, tid = threadIdx.x;
   int finisher = 0;  // the CTA that knows the outcome
-  cluster_arrive();
+  pg::cluster_arrive();
   const int v = item / a.entries, e = item % a.entries;  // the entries' first rows come first
   const int n = a.n[e];
   const long long row0 = a.row0[e], row = row0 + v;
@@ -789,7 +787,7 @@ __global__ void __launch_bounds__(kThreads, GREEDY ? kPerSmGreedy : kPerSm) veri
   int* outcome = a.outcome + row0;
   Family fam;
   fam.parents = a.parents + row0, fam.tokens = a.tokens + row0, fam.v = v, fam.n = n;
-  cluster_wait();  // (the others run: their shared memory is there)
+  pg::cluster_wait();  // (the others run: their shared memory is there)
   if (live && v > 0) {
     if (rank == 0 && tid < 32) {  // one look for all: what the parent decides may come in between
       const bool reached = may_be_reached(fam.parents, outcome, v);
