@@ -865,7 +865,7 @@ class AdapterPlan:
             if torch.device(device).type == "cuda":
                 self.host = self.host.pin_memory()
             self.dev = torch.empty_like(self.host, device=device)
-            self.rows, self.tiles = self.dev[:T], self.dev[T:]
+            self.rows, self.tiles, self.index = self.dev[:T], self.dev[T:], self.dev.get_device()
         elif T != self.T:
             raise ValueError(f"a plan of {self.T} rows is filled with {T}")
         h = self.host.numpy()
@@ -887,14 +887,12 @@ class AdapterPlan:
         self._make(ns, adapters, self.dev.device)
 
 
-def _rows_overlap(s, s_pitch, t, t_pitch):
-    """Whether two row matrices have bytes in common; column slices that stand side by side in one matrix have none."""
-    (rows, n), (more, m), a, b, i, j = s.shape, t.shape, s.data_ptr(), t.data_ptr(), s.element_size(), t.element_size()
-    if a + ((rows - 1) * s_pitch + n) * i <= b or b + ((more - 1) * t_pitch + m) * j <= a:
+def _rows_overlap(a, a_pitch, a_bytes, b, b_pitch, b_bytes, rows):
+    """Whether two row matrices (where they begin, bytes from row to row, bytes of a row) have bytes in common; column slices that stand side by side in one matrix have none."""
+    if a + (rows - 1) * a_pitch + a_bytes <= b or b + (rows - 1) * b_pitch + b_bytes <= a:
         return False
-    pitch = s_pitch * i
-    d = (b - a) % pitch
-    return pitch != t_pitch * j or d < n * i or pitch - d < m * j
+    d = (b - a) % a_pitch
+    return a_pitch != b_pitch or d < a_bytes or a_pitch - d < b_bytes
 
 
 def adapter_add(x: torch.Tensor, y: torch.Tensor, bank: AdapterBank, plan: AdapterPlan, out: Optional[torch.Tensor] = None, gain: float = 1.0):
@@ -917,26 +915,26 @@ def adapter_add(x: torch.Tensor, y: torch.Tensor, bank: AdapterBank, plan: Adapt
         raise ValueError("elements of a row stand side by side, rows do not overlap")
     if x.get_device() != index or y.get_device() != index or out.get_device() != index:
         raise ValueError(f"rows and adapters lie on one device: got {x.device}, {y.device}, {out.device} and {bank.device}")
-    if _rows_overlap(out, lo, x, lx) or (not (lo == ly and out.data_ptr() == y.data_ptr()) and _rows_overlap(out, lo, y, ly)):
+    px, py, po, ex, ey = x.data_ptr(), y.data_ptr(), out.data_ptr(), 4 if dtype == torch.float32 else 2, 4 if wide else 2
+    if _rows_overlap(po, lo * ey, F * ey, px, lx * ex, K * ex, T) or (not (lo == ly and po == py) and _rows_overlap(po, lo * ey, F * ey, py, ly * ey, F * ey, T)):
         raise ValueError("out is y or lies apart from it, and apart from x")
     if plan.most >= bank.slots:
         raise IndexError(f"adapter {plan.most} of {bank.slots}")
-    if plan.dev.get_device() != index:
+    if plan.index != index:
         raise ValueError(f"the plan lies on {plan.dev.device}, the adapters on {bank.device}")
     _on_current_device(bank.a)
-    L, shares = _lib.lib(), None
+    L = _lib.lib()
 
-    def packed():
-        return _lib.ADAPTER.pack(x.data_ptr(), y.data_ptr(), bank.a.data_ptr(), bank.b.data_ptr(), out.data_ptr(), bank.scale.data_ptr(), plan.rows.data_ptr(), plan.tiles.data_ptr(),
-                                 _lib.ptr(shares), lx, ly, lo, *bank.columns, len(bank.parts), K, F, bank.rank8, bank.slots, plan.tile_count, plan.tile_rows, T,
-                                 dtype == torch.float32, wide, gain)
+    def packed(shares):
+        return _lib.ADAPTER.pack(px, py, bank.a.data_ptr(), bank.b.data_ptr(), po, bank.scale.data_ptr(), plan.rows.data_ptr(), plan.tiles.data_ptr(), shares, lx, ly, lo, *bank.columns,
+                                 len(bank.parts), K, F, bank.rank8, bank.slots, plan.tile_count, plan.tile_rows, T, dtype == torch.float32, wide, gain)
 
-    a = packed()
+    a, scratch = packed(0), None
     if plan.tile_rows > 16:
         need = L.pg_adapter_scratch(a)
         if need:
-            shares = torch.empty(need // 4, device=x.device, dtype=torch.float32)
-            a = packed()
+            scratch = torch.empty(need // 4, device=x.device, dtype=torch.float32)
+            a = packed(scratch.data_ptr())
     _lib.check(L.pg_adapter_add(a, _lib.stream()), "pg_adapter_add")
     return out
 

@@ -94,5 +94,10 @@ def test_outputs_that_lie_in_their_inputs_are_refused():
     for out in (both[1:], both[:3, 3:27], both[:3, 40:64]):
         with pytest.raises(ValueError):
             seq_ops.adapter_add(both[:3, 24:48], both[:3, :24], bank(), plan, out=out[:, :24])
-    assert not seq_ops._rows_overlap(both[:3, :24], 100, both[:3, 24:48], 100) and not seq_ops._rows_overlap(both[:2], 100, both[2:], 100)
-    assert seq_ops._rows_overlap(both[:3, 76:], 100, both[:3, :25], 100) is False and seq_ops._rows_overlap(both[:3, :25], 100, both[:3, 24:48], 100)
+
+    def overlap(a, b):
+        size = a.element_size()
+        return seq_ops._rows_overlap(a.data_ptr(), 100 * size, a.shape[1] * size, b.data_ptr(), 100 * size, b.shape[1] * size, len(a))
+
+    assert not overlap(both[:3, :24], both[:3, 24:48]) and not overlap(both[:2], both[2:])
+    assert overlap(both[:3, 76:], both[:3, :25]) is False and overlap(both[:3, :25], both[:3, 24:48])
