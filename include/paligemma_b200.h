@@ -819,8 +819,12 @@ typedef struct {
   int row_bytes, heads, unit, pages;
 } PgPageOperand;
 int pg_copy_pages(const PgPageOperand* operands, int count, int page, long long most_page_bytes, const int* moves_host, int moves, void* stream);
-int pg_keep_rows(const PgPageOperand* operands, int count, int page, int most_columns, const int* page_table, int max_pages, const int* entry_n, const int* entry_ctx,
-                 const int* path, int path_ld, const int* kept, int entries, void* stream);
+typedef struct {
+  const PgPageOperand* operands;
+  const int *page_table, *n, *ctx, *path, *kept; /* of the step's entries: [entries, max_pages], [entries] twice, [entries, path_ld], [entries] */
+  int count, page, most_columns, max_pages, path_ld, entries;
+} PgKeepRows;
+int pg_keep_rows(const PgKeepRows* a, void* stream);
 
 /* Drafted trees against the target's distributions, from given random numbers.  Entry e owns rows row0[e] .. + n[e] of everything; row 0 of an entry is its pending
  * token, which stays; parents[row] is an earlier row of the entry (others, and rows below -1, are never reached).  A row's distribution: softmax(x / temperature)

@@ -93,7 +93,7 @@ SIGNATURES = {
     "pg_attn_rows_scratch": [p],
     "pg_attn_rows": [p, p, i64, p],
     "pg_copy_pages": [p, i32, i32, i64, p, i32, p],
-    "pg_keep_rows": [p, i32, i32, i32, p, i32, p, p, p, i32, p, i32, p],
+    "pg_keep_rows": [p, p],
     "pg_verify_drafts": [p, p],
     "pg_adapter_scratch": [p],
     "pg_adapter_add": [p, p],
@@ -158,6 +158,7 @@ PREPARE_E4M3 = struct.Struct("@Pq13Pq12i3f4x")
 READ_E4M3 = struct.Struct("@10P8i")
 VERIFY = struct.Struct("@11P3q4d4i")
 ADAPTER = struct.Struct("@9P3q18if4x")
+KEEP_ROWS = struct.Struct("@6P6i")
 PAGE_OPERAND = struct.Struct("@Pq4i")  # PgPageOperand
 
 

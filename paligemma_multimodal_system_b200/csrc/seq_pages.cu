@@ -109,17 +109,15 @@ __device__ __forceinline__ void keep_columns(const PgPageOperand& op, const int*
   }
 }
 
-__global__ void __launch_bounds__(kThreads) keep_rows_kernel(const PgPageOperand* __restrict__ ops, int page, const int* __restrict__ page_table, int max_pages,
-                                                             const int* __restrict__ entry_n, const int* __restrict__ entry_ctx, const int* __restrict__ path, int path_ld,
-                                                             const int* __restrict__ kept, int pieces) {
+__global__ void __launch_bounds__(kThreads) keep_rows_kernel(const PgKeepRows a, int pieces) {
   pg::griddep_begin();
-  const int e = blockIdx.x / pieces, c0 = blockIdx.x % pieces * (kCols * kParts);
-  const PgPageOperand op = ops[blockIdx.y];
+  const int e = blockIdx.x / pieces, c0 = blockIdx.x % pieces * (kCols * kParts), page = a.page, max_pages = a.max_pages;
+  const PgPageOperand op = a.operands[blockIdx.y];
   if (c0 >= (op.heads > 0 ? op.heads : op.row_bytes / op.unit)) return;
-  const int n = entry_n[e], ctx = entry_ctx[e], count = min(min(kept[e], path_ld), n);
+  const int n = a.n[e], ctx = a.ctx[e], count = min(min(a.kept[e], a.path_ld), n);
   if (count <= 0 || ctx < 0) return;
-  const int* p = path + static_cast<long long>(e) * path_ld;
-  const int* table = page_table + static_cast<long long>(e) * max_pages;
+  const int* p = a.path + static_cast<long long>(e) * a.path_ld;
+  const int* table = a.page_table + static_cast<long long>(e) * max_pages;
   switch (op.heads > 0 ? 1 : op.unit) {
     case 16: keep_columns<uint4>(op, table, max_pages, p, count, ctx, n, page, c0); break;
     case 4: keep_columns<uint32_t>(op, table, max_pages, p, count, ctx, n, page, c0); break;
@@ -153,15 +151,16 @@ extern "C" int pg_copy_pages(const PgPageOperand* operands, int count, int page,
   return PG_OK;
 }
 
-extern "C" int pg_keep_rows(const PgPageOperand* operands, int count, int page, int most_columns, const int* page_table, int max_pages, const int* entry_n, const int* entry_ctx,
-                            const int* path, int path_ld, const int* kept, int entries, void* stream) {
-  if (operands == nullptr || count <= 0 || count > 65535 || page <= 0 || most_columns <= 0 || page_table == nullptr || max_pages <= 0 || entry_n == nullptr || entry_ctx == nullptr ||
-      path == nullptr || path_ld <= 0 || kept == nullptr || entries <= 0)
+extern "C" int pg_keep_rows(const PgKeepRows* args, void* stream) {
+  if (args == nullptr) return PG_ERR_ARG;
+  const PgKeepRows& a = *args;
+  if (a.operands == nullptr || a.count <= 0 || a.count > 65535 || a.page <= 0 || a.most_columns <= 0 || a.page_table == nullptr || a.max_pages <= 0 || a.n == nullptr ||
+      a.ctx == nullptr || a.path == nullptr || a.path_ld <= 0 || a.kept == nullptr || a.entries <= 0)
     return PG_ERR_ARG;
-  const long long pieces = (most_columns + kCols * kParts - 1) / (kCols * kParts);
-  if (pieces * entries > 0x7fffffff) return PG_ERR_ARG;
-  return pg::launch_kernel(keep_rows_kernel, dim3(static_cast<unsigned>(entries * pieces), count), dim3(kThreads), 0, static_cast<cudaStream_t>(stream), operands, page, page_table,
-                           max_pages, entry_n, entry_ctx, path, path_ld, kept, static_cast<int>(pieces)) == cudaSuccess
+  const long long pieces = (a.most_columns + kCols * kParts - 1) / (kCols * kParts);
+  if (pieces * a.entries > 0x7fffffff) return PG_ERR_ARG;
+  return pg::launch_kernel(keep_rows_kernel, dim3(static_cast<unsigned>(a.entries * pieces), a.count), dim3(kThreads), 0, static_cast<cudaStream_t>(stream), a,
+                           static_cast<int>(pieces)) == cudaSuccess
              ? PG_OK
              : PG_ERR_CUDA;
 }

@@ -736,8 +736,8 @@ def copy_pages(cache: CachePages, moves):
     if not apart:
         raise ValueError("a page that is copied to is no other move's source or destination")
     _on_current_device(cache.table)
-    moves = np.ascontiguousarray(moves, dtype=np.int32)
-    _lib.check(_lib.lib().pg_copy_pages(cache.table.data_ptr(), cache.count, cache.page, cache.most_page_bytes, moves.ctypes.data, n, _lib.stream()), "pg_copy_pages")
+    moves = moves.astype(np.int32)
+    _lib.check(_lib.lib().pg_copy_pages(cache.table.data_ptr(), cache.count, cache.page, cache.most_page_bytes, moves.tobytes(), n, _lib.stream()), "pg_copy_pages")
 
 
 def keep_rows(cache: CachePages, b: StepBatch, path: torch.Tensor, kept: torch.Tensor):
@@ -751,8 +751,9 @@ def keep_rows(cache: CachePages, b: StepBatch, path: torch.Tensor, kept: torch.T
     if path.device != cache.device or kept.device != cache.device or b.page_table.device != cache.device:
         raise ValueError(f"paths, counts and page table lie on the cache's device, {cache.device}")
     _on_current_device(cache.table)
-    _lib.check(_lib.lib().pg_keep_rows(cache.table.data_ptr(), cache.count, cache.page, cache.most_columns, b.page_table.data_ptr(), b.max_pages, b.n.data_ptr(), b.ctx.data_ptr(),
-                                       path.data_ptr(), path.shape[1], kept.data_ptr(), b.E, _lib.stream()), "pg_keep_rows")
+    a = _lib.KEEP_ROWS.pack(cache.table.data_ptr(), b.page_table.data_ptr(), b.n.data_ptr(), b.ctx.data_ptr(), path.data_ptr(), kept.data_ptr(), cache.count, cache.page,
+                            cache.most_columns, b.max_pages, path.shape[1], b.E)
+    _lib.check(_lib.lib().pg_keep_rows(a, _lib.stream()), "pg_keep_rows")
 
 
 # ---- low-rank adapters of the step's requests -----------------------------------------------------------------------
