@@ -1,22 +1,24 @@
 // Low-rank adapters of many requests beside a shared projection: out[t] = y[t] + gain scale[s] B_s (A_s x[t]) for the rows t of adapter s.
 //
 // A tile is up to 16 or 128 rows of one adapter, gathered by number, so decoded tokens of requests that share an adapter and the rows of a prompt are one thing.  A
-// cluster of CTAs takes a tile in one launch: each CTA multiplies a share of K (v = A x, rank columns), the shares are added through distributed shared memory in
-// a fixed order, and each CTA then makes a share of the columns (B v) and adds it to y.  v stays in shared memory.
+// cluster of CTAs takes a tile in one launch: each CTA multiplies a share of K (v = A x, rank columns), the shares are added in a fixed order, and each CTA then makes a share of the
+// columns (B v) and adds it to y.  v stays in shared memory.  The shares of 16 rows meet through distributed shared memory; those of 128 through L2, see there.
 //
 // Matrix instructions take 16-bit operands; v is fp32 and is handed on as two bf16 terms where the output is bf16 (error 2^-17 of v, the output's rounding is
-// 2^-9) and as three where it is fp32.  fp32 operands are three terms each, six products.  The instruction cuts off what it adds to a long sum: sums of 64
-// products are added up in fp32.
+// 2^-9) and as three where it is fp32.  fp32 operands are three terms each, six products.  The instruction cuts off what it adds to a long sum: in tiles of 16 rows sums of 32
+// products are added up in fp32; in tiles of 128 K / 16 additions are cut off (numbers of one sign, K of 2048 in one share: 5e-6 of the sum; 2e-7 the other way).
 // Fragments are 16-byte pieces of the operands' rows: the k index is permuted alike in both factors, and four column tiles are interleaved so that a thread
 // holds eight neighbouring outputs.
 //
-// What bounds it: the bytes of y in and out and of x for prompts; the adapters' bytes and a chain of trips to memory for decoded tokens.
+// What bounds it: for decoded tokens a chain of trips to memory (one row beside 2048 x 2560 columns 8 us, 64 requests of 20 adapters 10); for prompts how long a CTA takes from one block
+// of columns to the next (6516 rows of 7 adapters beside 2048 x 2560 columns, rank 3 x 64: 45 us, 27 of them in ten blocks, 7 in the share of K, 6 in the join; 35 without y and out, 93 MB
+// in all: 2.1 TB/s).
 #include "common.cuh"
 #include "paligemma_b200.h"
 
 namespace {
 
-constexpr int kThreads = 256, kWarps = 8, kMostRanks = 8, kMostShared = 220 * 1024;
+constexpr int kThreads = 256, kWarps = 8, kMostRanks = 8, kMostShared = 220 * 1024, kTwoShared = 110 * 1024;  // (a CTA's; of two on an SM)
 
 PG_DEVINL uint4 zero4() { return make_uint4(0u, 0u, 0u, 0u); }
 
@@ -165,19 +167,19 @@ PG_DEVINL void copy_rows(const PgAdapter& a, const int* row_of, int count, int r
   else copy_pieces<uint16_t>(a, row_of, count, rank, ranks, a.F * kOut, kOut);
 }
 
-// Eight numbers of v, the CTAs' shares added in their order, two asked for at once
+// Eight numbers of v, the CTAs' shares added in their order, four asked for at once
 PG_DEVINL void joined8(const float* from, int ranks, float (&f)[8]) {
   const int own = pg::cluster_ctarank();
 #pragma unroll
   for (int i = 0; i < 8; ++i) f[i] = 0.0f;
-  for (int p = 0; p < ranks; p += 2) {
-    float4 v[2][2];
+  for (int p = 0; p < ranks; p += 4) {
+    float4 v[4][2];
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int k = 0; k < 4; ++k)
 #pragma unroll
       for (int h = 0; h < 2; ++h) v[k][h] = get_f4(from + 4 * h, min(p + k, ranks - 1), own);
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int k = 0; k < 4; ++k)
       if (p + k < ranks)
 #pragma unroll
         for (int h = 0; h < 2; ++h) f[4 * h] += v[k][h].x, f[4 * h + 1] += v[k][h].y, f[4 * h + 2] += v[k][h].z, f[4 * h + 3] += v[k][h].w;
@@ -755,32 +757,55 @@ __global__ void __launch_bounds__(kTensorThreads, 1) adapter_tensor_kernel(const
   }
 }
 
-template <typename Kern, typename... Args>
-int launch(Kern kern, bool (&configured)[pg::kMaxDevices], long long items, int ranks, int threads, size_t smem, cudaStream_t st, Args... args) {
+template <typename Kern>
+bool allow_shared(Kern kern, bool (&configured)[pg::kMaxDevices]) {
   bool& done = configured[pg::current_device()];
   if (!done) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared) != cudaSuccess) {
       cudaGetLastError();
-      return PG_ERR_CUDA;
+      return false;
     }
     done = true;
   }
-  if (smem > kMostShared || items * ranks > 0x7fffffff) return PG_ERR_ARG;
+  return true;
+}
+struct Config {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(items * ranks));
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ranks;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pg_pdl_enabled() ? 2 : 1;
+  Config(long long ctas, int ranks, int threads, size_t smem, cudaStream_t st) {
+    cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ranks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pg_pdl_enabled() ? 2 : 1;
+  }
+};
+template <typename Kern, typename... Args>
+int launch(Kern kern, long long items, int ranks, int threads, size_t smem, cudaStream_t st, Args... args) {
+  if (smem > kMostShared || items * ranks > 0x7fffffff) return PG_ERR_ARG;
+  const Config c(items * ranks, ranks, threads, smem, st);
   pg_count_launch(1);
-  return cudaLaunchKernelEx(&cfg, kern, args...) == cudaSuccess ? PG_OK : PG_ERR_CUDA;
+  return cudaLaunchKernelEx(&c.cfg, kern, args...) == cudaSuccess ? PG_OK : PG_ERR_CUDA;
+}
+// How many clusters of `ranks` CTAs run at once: fewer than SMs / ranks, since a cluster lies in one part of the device (asked once; `known` is the kernel's)
+template <typename Kern>
+int at_once(Kern kern, int (&known)[pg::kMaxDevices][kMostRanks + 1], int ranks, int threads, size_t smem) {
+  int& n = known[pg::current_device()][ranks];
+  if (n == 0) {
+    Config c(ranks, ranks, threads, smem, nullptr);
+    c.cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kern, &c.cfg) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = 1;
+    }
+  }
+  return n;
 }
 
 Layout layout_of(const PgAdapter& a) {
@@ -807,10 +832,14 @@ void plan_of(const PgAdapter& a, const Layout& lay, Plan& plan) {
   plan.smem = (stages > behind ? stages : behind) + 1024;
   if (a.tile_rows != kRows || a.in_f32 || plan.R16 > 256 || plan.smem > kMostShared) plan.stages = 0;
 }
-int shares_of(const PgAdapter& a) {  // of K and of the columns, a CTA each: all CTAs at once
-  int ranks = pg::num_sms() / a.tile_count;
-  ranks = ranks < 1 ? 1 : ranks > kMostRanks ? kMostRanks : ranks;
-  while (ranks > 1 && a.K / ranks < 128) --ranks;
+// Shares of K and of the columns, a CTA each: as many as leave all clusters of the launch room at once.  (16 tiles of 2048 x 2560 with as many as fit and with 8: 24 and 43 us.)
+template <bool OUT32>
+int shares_of(const PgAdapter& a) {
+  static bool configured[pg::kMaxDevices] = {};
+  static int known[pg::kMaxDevices][kMostRanks + 1] = {};
+  if (!allow_shared(adapter_tensor_kernel<OUT32>, configured)) return 0;
+  int ranks = kMostRanks;
+  while (ranks > 1 && (a.K / ranks < 128 || at_once(adapter_tensor_kernel<OUT32>, known, ranks, kTensorThreads, kMostShared) < a.tile_count)) --ranks;
   return ranks;
 }
 
@@ -822,20 +851,27 @@ int pick(const PgAdapter& a, cudaStream_t st, int x_vec, int y_vec) {
     Plan plan;
     plan_of<VT>(a, lay, plan);
     if (plan.stages > 0 && x_vec && a.K % 8 == 0) {
-      const int ranks = shares_of(a);
+      const int ranks = shares_of<OUT32>(a);
+      if (ranks < 1) return PG_ERR_CUDA;
       if (ranks > 1 && a.shares == nullptr) return PG_ERR_ARG;
-      static bool configured[pg::kMaxDevices] = {};
-      return launch(adapter_tensor_kernel<OUT32>, configured, a.tile_count, ranks, kTensorThreads, plan.smem, st, a, lay, plan, y_vec);
+      return launch(adapter_tensor_kernel<OUT32>, a.tile_count, ranks, kTensorThreads, plan.smem, st, a, lay, plan, y_vec);
     }
   }
+  auto kern = adapter_rows_kernel<NW, IN32, OUT32>;
+  static bool configured[pg::kMaxDevices] = {};
+  static int known[2][pg::kMaxDevices][kMostRanks + 1] = {};  // two CTAs an SM, one
+  if (!allow_shared(kern, configured)) return PG_ERR_CUDA;
   const int subs = a.tile_rows / 16;
   const long long items = static_cast<long long>(a.tile_count) * subs;
   int ranks = 1, wn = 1;
-  while (ranks < kMostRanks && items * ranks * 2 <= 2 * pg::num_sms() && a.K / (ranks * 2) >= 128) ranks *= 2;
   while (wn < kWarps && wn * NW < lay.R / 8) wn *= 2;
   const size_t smem = sizeof(float) * (kWarps / wn) * 16 * lay.partial_ld + sizeof(uint16_t) * VT * 16 * lay.v_ld;
-  static bool configured[pg::kMaxDevices] = {};
-  return launch(adapter_rows_kernel<NW, IN32, OUT32>, configured, items, ranks, kThreads, smem, st, a, lay, subs, x_vec, y_vec);
+  const bool two = smem <= kTwoShared;
+  // A share is read by all CTAs of its cluster: eight for few tiles alone.  (2048 x 2560, us with 2, 4, 8: rank 3 x 64, 8 tiles 21, 14, 13, 16 tiles 22, 16, 26; rank 3 x 16, 8 tiles 12,
+  // 8.8, 7.9, 32 tiles 13, 10, 13.)
+  const int most = items <= pg::num_sms() / 16 ? kMostRanks : kMostRanks / 2;
+  while (ranks < most && a.K / (ranks * 2) >= 128 && at_once(kern, known[!two], ranks * 2, kThreads, two ? kTwoShared : kMostShared) >= items) ranks *= 2;
+  return launch(kern, items, ranks, kThreads, smem, st, a, lay, subs, x_vec, y_vec);
 }
 
 }  // namespace
@@ -845,7 +881,7 @@ extern "C" long long pg_adapter_scratch(const PgAdapter* args) {
   Plan plan;
   if (args->out_f32) plan_of<3>(*args, layout_of(*args), plan);
   else plan_of<2>(*args, layout_of(*args), plan);
-  const int ranks = plan.stages > 0 ? shares_of(*args) : 1;
+  const int ranks = plan.stages == 0 ? 1 : args->out_f32 ? shares_of<true>(*args) : shares_of<false>(*args);
   return ranks > 1 ? static_cast<long long>(sizeof(float)) * args->tile_count * ranks * kRows * args->parts * args->rank : 0;
 }
 

@@ -834,10 +834,13 @@ class AdapterBank:
 
 class AdapterPlan:
     """Which rows of a step go through which adapter: entries of ns[e] rows, one behind the other, with adapters[e] (-1: none).  Rows of one adapter stand together in
-    tiles, whichever entries they belong to.  tiles: a fixed number of them (a plan that is `fill`ed again, for a step that is captured)."""
+    tiles, whichever entries they belong to.  tiles: a fixed number of them (a plan that is `fill`ed again, for a step that is captured).  tile_rows: how many rows a tile
+    has at most, 16 or 128 (None: by the rows)."""
 
-    def __init__(self, ns: Sequence[int], adapters: Sequence[int], device="cuda", tiles: Optional[int] = None):
-        self.T, self.fixed, self._copied, self.host = 0, tiles, None, None
+    def __init__(self, ns: Sequence[int], adapters: Sequence[int], device="cuda", tiles: Optional[int] = None, tile_rows: Optional[int] = None):
+        if tile_rows not in (None, 16, 128):
+            raise ValueError(f"tiles of 16 or 128 rows: got {tile_rows}")
+        self.T, self.fixed, self._copied, self.host, self.tile_rows = 0, tiles, None, None, tile_rows
         self._make(ns, adapters, device)
 
     def _order(self, ns, adapters):
@@ -853,8 +856,9 @@ class AdapterPlan:
 
     def _make(self, ns, adapters, device):
         order, ids, first, count = self._order(ns, adapters)
-        # by the rows of an adapter on average: tiles of 128 go over the tensor memory, tiles of 16 are more CTAs (decoded tokens)
-        size = 128 if self.fixed is None and len(order) >= 64 * len(ids) else 16
+        # Tiles of 128 rows go over the tensor memory, and their way is long: they pay once tiles of 16 are more than the SMs, where adapters fill half of one on average.  (K 2048, 2560
+        # columns, us with 16 and 128: 7 adapters of 320 rows, rank 3 x 16 16 and 22, 3 x 64 30 and 25; of 384 rows 24 and 22, 47 and 24; 48 of 64 rows 25 and 32, 60 and 38.)
+        size = self.tile_rows or (128 if self.fixed is None and len(order) > max(16 * 148, 64 * len(ids) - 1) else 16)
         tiles = [(a, f + o, min(size, c - o)) for a, f, c in zip(ids.tolist(), first.tolist(), count.tolist()) for o in range(0, c, size)]
         n = len(tiles) if self.fixed is None else self.fixed
         if len(tiles) > n:
@@ -898,7 +902,8 @@ def _rows_overlap(a, a_pitch, a_bytes, b, b_pitch, b_bytes, rows):
 
 def adapter_add(x: torch.Tensor, y: torch.Tensor, bank: AdapterBank, plan: AdapterPlan, out: Optional[torch.Tensor] = None, gain: float = 1.0):
     """out[t] = y[t] + gain * scale[s] * b[s] (a[s] x[t]) for the rows of adapter s, y[t] for those without (out None: y, in place).  x [rows, K] of the bank's type, y and
-    out [rows, columns] bf16 or fp32 (fp32 beside fp32 adapters), unit last strides, any row pitch.  The sum over K and over the rank is fp32; y is added to it and rounded once.  A row of x that is not
+    out [rows, columns] bf16 or fp32 (fp32 beside fp32 adapters), unit last strides, any row pitch.  The sum over K and over the rank is fp32 (tiles of
+    128 rows: the tensor cores' own, K / 16 additions that are cut off); y is added to it and rounded once.  A row of x that is not
     finite makes its own row of out NaN."""
     out = y if out is None else out
     T, K, F, dtype, index = plan.T, bank.K, bank.F, bank.dtype, bank.index

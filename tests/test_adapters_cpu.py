@@ -101,3 +101,13 @@ def test_outputs_that_lie_in_their_inputs_are_refused():
 
     assert not overlap(both[:3, :24], both[:3, 24:48]) and not overlap(both[:2], both[2:])
     assert overlap(both[:3, 76:], both[:3, :25]) is False and overlap(both[:3, :25], both[:3, 24:48])
+
+
+@pytest.mark.parametrize("ns,who,rows", [([1] * 40, [0, 1] * 20, 16), ([2368], [0], 16), ([2369], [0], 128), ([1024, 1, 1344], [0, 1, -1], 128), ([64] * 40, list(range(40)), 128), ([63] * 40, list(range(40)), 16)])
+def test_tiles_by_the_rows(ns, who, rows):
+    plan = seq_ops.AdapterPlan(ns, who, device="cpu")
+    assert plan.tile_rows == rows and seq_ops.AdapterPlan(ns, who, device="cpu", tile_rows=144 - rows).tile_rows == 144 - rows
+    tiles = plan.tiles.view(-1, 3).tolist()
+    assert sum(n for _, _, n in tiles) == sum(ns) and all(0 < n <= rows for _, _, n in tiles)
+    with pytest.raises(ValueError):
+        seq_ops.AdapterPlan(ns, who, device="cpu", tile_rows=64)

@@ -56,12 +56,13 @@ STEPS = [([1], [0], 1), ([1] * 64, [i * 7 % 20 - (i % 9 == 0) for i in range(64)
          ([400, 1, 1, 1], [1, 1, 0, -1], 2)]
 
 
+@pytest.mark.parametrize("tile_rows", [16, 128])
 @pytest.mark.parametrize("dtype,out", FORMS)
 @pytest.mark.parametrize("ns,who,slots", STEPS)
 @pytest.mark.parametrize("K,parts,rank", [(256, [128], 16), (1000, [96, 40, 8], 8), (77, [33, 5], 3), (2048, [512, 64, 64], 64)])
-def test_adapters(dtype, out, ns, who, slots, K, parts, rank):
+def test_adapters(dtype, out, ns, who, slots, K, parts, rank, tile_rows):
     x, y, a, b, scale = make(ns, who, K, parts, rank, slots, dtype, out)
-    bank, plan = seq_ops.AdapterBank(a.cuda(), b.cuda(), scale.cuda(), parts), seq_ops.AdapterPlan(ns, who)
+    bank, plan = seq_ops.AdapterBank(a.cuda(), b.cuda(), scale.cuda(), parts), seq_ops.AdapterPlan(ns, who, tile_rows=tile_rows)
     value, bound = expected(x, y, a, b, scale, ns, who, parts, rank)
     apart = seq_ops.adapter_add(x.cuda(), y.cuda(), bank, plan, out=torch.full_like(y, float("nan"), device="cuda"))
     compare(apart, value, bound)
@@ -69,25 +70,27 @@ def test_adapters(dtype, out, ns, who, slots, K, parts, rank):
     assert seq_ops.adapter_add(x.cuda(), z, bank, plan) is z and torch.equal(z, apart)
 
 
+@pytest.mark.parametrize("tile_rows", [16, 128])
 @pytest.mark.parametrize("rank,parts", [(128, [64] * 8), (100, [320, 200]), (1, [8]), (40, [24, 24, 24, 24, 24])])
 @pytest.mark.parametrize("dtype,out", FORMS)
-def test_ranks_and_runs(rank, parts, dtype, out):
+def test_ranks_and_runs(rank, parts, dtype, out, tile_rows):
     ns, who = [90, 1, 30], [1, 0, 1]
     x, y, a, b, scale = make(ns, who, 136, parts, rank, 2, dtype, out, seed=rank)
-    bank, plan = seq_ops.AdapterBank(a.cuda(), b.cuda(), scale.cuda(), parts), seq_ops.AdapterPlan(ns, who)
+    bank, plan = seq_ops.AdapterBank(a.cuda(), b.cuda(), scale.cuda(), parts), seq_ops.AdapterPlan(ns, who, tile_rows=tile_rows)
     value, bound = expected(x, y, a, b, scale, ns, who, parts, rank, gain=-1.5)
     compare(seq_ops.adapter_add(x.cuda(), y.cuda(), bank, plan, gain=-1.5), value, bound)
 
 
+@pytest.mark.parametrize("tile_rows", [16, 128])
 @pytest.mark.parametrize("dtype,out", FORMS)
 @pytest.mark.parametrize("pitch,off", [(264, 8), (261, 3), (272, 1)])
-def test_rows_at_any_pitch_and_columns_beside(dtype, out, pitch, off):
+def test_rows_at_any_pitch_and_columns_beside(dtype, out, pitch, off, tile_rows):
     ns, who, parts, K, rank = [40, 1, 1, 30], [0, 1, -1, 1], [100, 28], 200, 16
     x, y, a, b, scale = make(ns, who, K, parts, rank, 2, dtype, out)
     X, Y = torch.full((72, pitch), float("nan"), dtype=dtype, device="cuda"), torch.full((72, pitch), float("nan"), dtype=out, device="cuda")
     X[:, off:off + K], Y[:, off:off + 128] = x.cuda(), y.cuda()
     before = Y.clone()
-    bank, plan = seq_ops.AdapterBank(a.cuda(), b.cuda(), scale.cuda(), parts), seq_ops.AdapterPlan(ns, who)
+    bank, plan = seq_ops.AdapterBank(a.cuda(), b.cuda(), scale.cuda(), parts), seq_ops.AdapterPlan(ns, who, tile_rows=tile_rows)
     seq_ops.adapter_add(X[:, off:off + K], Y[:, off:off + 128], bank, plan)
     value, bound = expected(x, y, a, b, scale, ns, who, parts, rank)
     compare(Y[:, off:off + 128], value, bound)
@@ -95,11 +98,12 @@ def test_rows_at_any_pitch_and_columns_beside(dtype, out, pitch, off):
     assert torch.equal(Y.view(torch.uint8), before.view(torch.uint8))
 
 
-def test_what_is_not_finite_stays_in_its_row():
+@pytest.mark.parametrize("tile_rows", [16, 128])
+def test_what_is_not_finite_stays_in_its_row(tile_rows):
     ns, who = [20, 3], [0, -1]
     x, y, a, b, scale = make(ns, who, 64, [32], 8, 1, torch.bfloat16, torch.float32)
     x[5, 3], x[21, 0], y[22, 1] = float("nan"), float("inf"), float("-inf")
-    bank, plan = seq_ops.AdapterBank(a.cuda(), b.cuda(), scale.cuda(), [32]), seq_ops.AdapterPlan(ns, who)
+    bank, plan = seq_ops.AdapterBank(a.cuda(), b.cuda(), scale.cuda(), [32]), seq_ops.AdapterPlan(ns, who, tile_rows=tile_rows)
     got = seq_ops.adapter_add(x.cuda(), y.cuda(), bank, plan, out=torch.empty(23, 32, device="cuda")).cpu()
     assert got[5].isnan().all() and torch.equal(got[20:], y[20:])
     x[5] = 0
@@ -150,8 +154,7 @@ def test_tiles_of_many_rows(rank, parts, dtype, out, ns, who, slots):
     """Blocks of 64 ranks and 128 columns that are not full, several parts, shares of K that differ, rows without an adapter beside."""
     K = 1096
     x, y, a, b, scale = make(ns, who, K, parts, rank, slots, dtype, out, seed=rank)
-    bank, plan = seq_ops.AdapterBank(a.cuda(), b.cuda(), scale.cuda(), parts), seq_ops.AdapterPlan(ns, who)
-    assert plan.tile_rows == 128
+    bank, plan = seq_ops.AdapterBank(a.cuda(), b.cuda(), scale.cuda(), parts), seq_ops.AdapterPlan(ns, who, tile_rows=128)
     value, bound = expected(x, y, a, b, scale, ns, who, parts, rank)
     z = y.cuda()
     apart = seq_ops.adapter_add(x.cuda(), z, bank, plan, out=torch.full_like(z, float("nan")))
@@ -165,7 +168,7 @@ def test_tiles_of_many_rows(rank, parts, dtype, out, ns, who, slots):
 def test_more_tiles_than_processors(dtype, out, K):
     ns, who, parts, rank = [20100, 300], [0, 1], [40, 136], 24
     x, y, a, b, scale = make(ns, who, K, parts, rank, 2, dtype, out)
-    bank, plan = seq_ops.AdapterBank(a.cuda(), b.cuda(), scale.cuda(), parts), seq_ops.AdapterPlan(ns, who)
+    bank, plan = seq_ops.AdapterBank(a.cuda(), b.cuda(), scale.cuda(), parts), seq_ops.AdapterPlan(ns, who, tile_rows=128)
     value, bound = expected(x, y, a, b, scale, ns, who, parts, rank)
     compare(seq_ops.adapter_add(x.cuda(), y.cuda(), bank, plan), value, bound)
 
@@ -177,7 +180,7 @@ def test_tiles_of_many_rows_at_any_pitch(pitch, off):
     X, Y = torch.full((270, pitch), float("nan"), dtype=torch.bfloat16, device="cuda"), torch.full((270, pitch), float("nan"), dtype=torch.bfloat16, device="cuda")
     X[:, off:off + K], Y[:, off:off + 1020] = x.cuda(), y.cuda()
     before = Y.clone()
-    bank, plan = seq_ops.AdapterBank(a.cuda(), b.cuda(), scale.cuda(), parts), seq_ops.AdapterPlan(ns, who)
+    bank, plan = seq_ops.AdapterBank(a.cuda(), b.cuda(), scale.cuda(), parts), seq_ops.AdapterPlan(ns, who, tile_rows=128)
     seq_ops.adapter_add(X[:, off:off + K], Y[:, off:off + 1020], bank, plan)
     value, bound = expected(x, y, a, b, scale, ns, who, parts, rank)
     compare(Y[:, off:off + 1020], value, bound)
@@ -189,7 +192,7 @@ def test_two_streams_and_a_captured_call():
     """Calls that run at the same time have scratch of their own."""
     ns, who, parts, K, rank = [700], [0], [512, 256], 1024, 64
     x, y, a, b, scale = make(ns, who, K, parts, rank, 1, torch.bfloat16, torch.float32)
-    bank, plan = seq_ops.AdapterBank(a.cuda(), b.cuda(), scale.cuda(), parts), seq_ops.AdapterPlan(ns, who)
+    bank, plan = seq_ops.AdapterBank(a.cuda(), b.cuda(), scale.cuda(), parts), seq_ops.AdapterPlan(ns, who, tile_rows=128)
     X, Y = x.cuda(), y.cuda()
     want = seq_ops.adapter_add(X, Y, bank, plan, out=torch.empty_like(Y))
     value, bound = expected(x, y, a, b, scale, ns, who, parts, rank)
