@@ -205,7 +205,7 @@ PG_DEVINL void join_shares(const PgAdapter& a, const Layout& lay, const float* p
   }
 }
 
-// Eight neighbouring outputs: y, then y + factor v
+// Eight neighbouring outputs: y, then y + factor v.  What is not 16-byte pieces is read when it is needed: registers that a load and a branch both write are waited for where they merge.
 template <bool OUT32>
 struct Eight {
   uint4 y[OUT32 ? 2 : 1];
@@ -214,41 +214,36 @@ struct Eight {
     const bool whole = there && vec && n >= 8;
     y[0] = ld16(p, whole);
     if constexpr (OUT32) y[1] = ld16(p + 16, whole);
-    if (there && !whole) {
-      uint32_t w[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) w[k] = k >= n ? 0u : OUT32 ? reinterpret_cast<const uint32_t*>(p)[k] : reinterpret_cast<const uint16_t*>(p)[k];
-      if constexpr (OUT32) y[0] = make_uint4(w[0], w[1], w[2], w[3]), y[1] = make_uint4(w[4], w[5], w[6], w[7]);
-      else y[0] = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
-    }
   }
-  PG_DEVINL void store(void* base, long long at, int n, bool vec, float factor, const float (&v)[8]) const {
+  PG_DEVINL void store(const void* from, long long from_at, void* to, long long to_at, int n, bool vec, float factor, const float (&v)[8]) const {
     if constexpr (OUT32) {
-      float* p = static_cast<float*>(base) + at;
-      float o[8];
-      const uint32_t w[8] = {y[0].x, y[0].y, y[0].z, y[0].w, y[1].x, y[1].y, y[1].z, y[1].w};
-#pragma unroll
-      for (int k = 0; k < 8; ++k) o[k] = fmaf(factor, v[k], __uint_as_float(w[k]));
+      float* p = static_cast<float*>(to) + to_at;
       if (vec && n >= 8) {
+        const uint32_t w[8] = {y[0].x, y[0].y, y[0].z, y[0].w, y[1].x, y[1].y, y[1].z, y[1].w};
+        float o[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[k] = fmaf(factor, v[k], __uint_as_float(w[k]));
         reinterpret_cast<float4*>(p)[0] = make_float4(o[0], o[1], o[2], o[3]), reinterpret_cast<float4*>(p)[1] = make_float4(o[4], o[5], o[6], o[7]);
       } else {
+        const float* q = static_cast<const float*>(from) + from_at;
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          if (k < n) p[k] = o[k];
+          if (k < n) p[k] = fmaf(factor, v[k], q[k]);
       }
     } else {
-      uint16_t* p = static_cast<uint16_t*>(base) + at;
-      const uint32_t w[4] = {y[0].x, y[0].y, y[0].z, y[0].w};
-      uint32_t o[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        o[k] = pg::pack_bf16(fmaf(factor, v[2 * k], __uint_as_float(w[k] << 16)), fmaf(factor, v[2 * k + 1], __uint_as_float(w[k] & 0xffff0000u)));
+      uint16_t* p = static_cast<uint16_t*>(to) + to_at;
       if (vec && n >= 8) {
+        const uint32_t w[4] = {y[0].x, y[0].y, y[0].z, y[0].w};
+        uint32_t o[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          o[k] = pg::pack_bf16(fmaf(factor, v[2 * k], __uint_as_float(w[k] << 16)), fmaf(factor, v[2 * k + 1], __uint_as_float(w[k] & 0xffff0000u)));
         *reinterpret_cast<uint4*>(p) = make_uint4(o[0], o[1], o[2], o[3]);
       } else {
+        const uint16_t* q = static_cast<const uint16_t*>(from) + from_at;
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          if (k < n) p[k] = static_cast<uint16_t>(o[k / 2] >> 16 * (k % 2));
+          if (k < n) p[k] = static_cast<uint16_t>(pg::pack_bf16(fmaf(factor, v[k], __uint_as_float(static_cast<uint32_t>(q[k]) << 16)), 0.0f));
       }
     }
   }
@@ -335,7 +330,7 @@ struct Columns {
         float v[8];
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[2 * j] = acc[j][2 * h], v[2 * j + 1] = acc[j][2 * h + 1];
-        y[h].store(a.out, t * a.ldo + f0 + 8 * q, wide - 8 * q, vec, factor, v);
+        y[h].store(a.y, t * a.ldy + f0 + 8 * q, a.out, t * a.ldo + f0 + 8 * q, wide - 8 * q, vec, factor, v);
       }
     }
   }
@@ -726,13 +721,14 @@ __global__ void __launch_bounds__(kTensorThreads, 1) adapter_tensor_kernel(const
         __syncwarp();
         pg::tc_fence_after();
         ask_b(b[turn], turn);
+        {
+          uint32_t v[kCols / 16][16];
 #pragma unroll
-        for (int i = 0; i < kCols / 16; ++i) {
-          uint32_t v[16];
-          pg::tmem_ld16(lanes + 256 + kBlock * turn + kCols * group + 16 * i, v);
+          for (int i = 0; i < kCols / 16; ++i) pg::tmem_ld16(lanes + 256 + kBlock * turn + kCols * group + 16 * i, v[i]);
           pg::tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(stage + lane * kStageLd + 16 * i + 4 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          for (int j = 0; j < kCols / 4; ++j)
+            *reinterpret_cast<uint4*>(stage + lane * kStageLd + 4 * j) = make_uint4(v[j / 4][4 * (j % 4)], v[j / 4][4 * (j % 4) + 1], v[j / 4][4 * (j % 4) + 2], v[j / 4][4 * (j % 4) + 3]);
         }
         pg::tc_fence_before();
         arrive(kLeft + turn);
@@ -741,7 +737,7 @@ __global__ void __launch_bounds__(kTensorThreads, 1) adapter_tensor_kernel(const
           const float* from = stage + (8 * i + lane / 4) * kStageLd + lane % 4 * 8;
           const float4 lo = *reinterpret_cast<const float4*>(from), hi = *reinterpret_cast<const float4*>(from + 4);
           const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-          if (row[i] >= 0 && c < now.wide) y[turn][i].store(a.out, row[i] * a.ldo + now.f0 + c, now.wide - c, y_vec, factor, v);
+          if (row[i] >= 0 && c < now.wide) y[turn][i].store(a.y, row[i] * a.ldy + now.f0 + c, a.out, row[i] * a.ldo + now.f0 + c, now.wide - c, y_vec, factor, v);
         }
         pg::cp_async_wait<0>();
         pg::fence_proxy_async_smem();
