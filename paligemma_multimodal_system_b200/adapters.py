@@ -6,8 +6,8 @@
     engine.step([("a", prompt, [])], adapters={"a": "french"})
 
 `tensors` holds A [r, K] and B [columns, r] as "<weight>.A" and "<weight>.B" beside the names that the checkpoint gives the weights: "l3.mix.q.A" stands beside "l3.mix.q".
-Which weights can be adapted is the sub-layers' to say (`adapter_sites`): the attention layers' query, key, value, gate and output projections, the linear attention's, the
-down projections of dense feed-forwards.  Adapters of a lower rank than the set's are padded with zeros.
+Which weights can be adapted is the sub-layers' to say (`adapter_sites`): the attention layers' query, key, value, gate and output projections (latent attention:
+the output), the linear attention's, the down projections of dense feed-forwards and the polynomial-of-norms one's up projection.  Adapters of a lower rank than the set's are padded with zeros.
 """
 from typing import Dict, List, Optional, Sequence
 

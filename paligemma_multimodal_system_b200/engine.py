@@ -264,12 +264,13 @@ class SequenceEngine:
                 self._decode_graphs = {k: v for k, v in self._decode_graphs.items() if len(k) == 2 or k[2] == version}
             slot = self._decode_graphs[key] = dict(static=StaticDecodeBatch(E, pages_cap, ctx_cap), graph=None, logits=None, seen=0)
             if adapters is not None:
-                slot["plan"] = seq_ops.AdapterPlan([1] * E, adapters, tiles=E)
+                slot["plan"], slot["who"] = seq_ops.AdapterPlan([1] * E, adapters, tiles=E), list(adapters)
                 slot["static"].batch = seq_ops.with_adapters(slot["static"].batch, StepAdapters(dict(self.adapters.banks), slot["plan"]))
         st = slot["static"]
         st.fill(batch)
-        if adapters is not None:
+        if adapters is not None and slot["who"] != adapters:
             slot["plan"].fill([1] * E, adapters)
+            slot["who"] = list(adapters)
         slot["seen"] += 1
         if slot["graph"] is None and slot["seen"] >= 2:
             side = torch.cuda.Stream()

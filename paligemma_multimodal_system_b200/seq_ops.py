@@ -851,8 +851,9 @@ class AdapterPlan:
             raise IndexError("adapters are 0 .. slots - 1, -1 for none")
         rows = np.repeat(who, ns)
         order = np.argsort(rows, kind="stable")
-        ids, first, count = np.unique(rows[order], return_index=True, return_counts=True)
-        return order, ids, first, count
+        rows = rows[order]
+        first = np.concatenate([[0], np.flatnonzero(rows[1:] != rows[:-1]) + 1])
+        return order, rows[first], first, np.diff(first, append=len(rows))
 
     def _make(self, ns, adapters, device):
         order, ids, first, count = self._order(ns, adapters)
