@@ -340,3 +340,33 @@ def test_forks_beside_drafts_that_wait_and_of_latent_rows():
     eng.fork("a", ["b"], length=77)
     for rid, full in (("a", prompt), ("b", prompt[:77])):
         assert rel_err(run_cut_live(eng, rid, later, [1, 5]), run_cut(ref, "x", full + later, [len(full), 1, 5])[len(full):]) < TOL[torch.float32]
+
+
+@pytest.mark.parametrize("family,seed", [("fadosun", 2), ("padulorn", 3), ("zigivik", 2), ("pukerax", 3)])
+def test_adapters_and_forks_of_every_family(family, seed):
+    """Beside the weights is as good as merged into them, whatever a family's sub-layers do with their projections; a fork has copies of what its layers keep."""
+    import importlib
+    from paligemma_multimodal_system_b200.adapters import AdapterSet
+    from paligemma_multimodal_system_b200.engine import SequenceEngine
+    t = importlib.import_module(f"test_{family}_gpu")
+    cfg, g = t.BASE_CFG, torch.Generator().manual_seed(seed)
+    weights = t.steady_weights(cfg, seed=2) if family == "padulorn" else t.O.random_weights(cfg, seed=seed)
+    weights = {k: v.to(torch.bfloat16).float() for k, v in weights.items()}  # (as `build` loads them; merged ones are loaded as they are)
+    model = t.build(cfg, weights, torch.float32)
+    sets = AdapterSet(model, 2, 8)
+    own = adapter(sets, shapes(sets), g, 8, sorted(shapes(sets)), size=0.2)
+    assert shapes(sets) and all(w in weights for w in shapes(sets)) and (family == "fadosun" or any(w.endswith("mix.o") for w in shapes(sets)))  # (its mixers take none)
+    sets.load("one", own)
+    V = model.vocab_size
+    eng, ref = SequenceEngine(model, 1024, 3, adapters=sets), SequenceEngine(type(model)(model.config, torch.float32).load_weights(merged(weights, own, 1.0)), 1024, 3)
+    full, other = toks(52, V, 3), toks(30, V, 4)
+    got = eng.step([("a", full[:40], range(40)), ("b", other, [29])], adapters={"a": "one"})
+    want = run_cut(ref, "a", full, [40, 8, 1, 1, 1, 1])
+    assert rel_err(got[:40], want[:40]) < TOL[torch.float32]
+    plain = SequenceEngine(model, 1024, 3)
+    assert rel_err(got[40:], run_cut(plain, "b", other, [30])[29:]) < TOL[torch.float32]
+    eng.fork("a", ["c"])
+    rest = [eng.step([("a", full[40:48], range(8)), ("c", full[40:48], range(8))])] + [eng.step([("c", [x], [0]), ("a", [x], [0])]) for x in full[48:]]
+    a = torch.cat([rest[0][:8]] + [r[1:] for r in rest[1:]])
+    c = torch.cat([rest[0][8:]] + [r[:1] for r in rest[1:]])
+    assert rel_err(a, want[40:]) < TOL[torch.float32] and rel_err(c, want[40:]) < TOL[torch.float32]
