@@ -333,31 +333,43 @@ class SequenceEngine:
         sched = StepScheduler(len(self.store.free_slots), len(self.store.pool.free), self.store.page, step_tokens, eos_token_id)
         for i, pr in enumerate(prompts):
             sched.submit(TokenRequest(("gen", i), [int(t) for t in pr], int(max_new_tokens)))
-        while not sched.idle():
-            plan = sched.plan()
-            if not plan:
-                raise RuntimeError("scheduler made no progress")
-            if draft is not None and all(req.fed == len(req.prompt) for req, _, _ in plan):
-                guessed = self._guesses(plan, draft)
-                if any(len(toks) > 1 for _, toks, _ in guessed):
-                    self._drafted_turn(plan, guessed, sched, do_sample, temperature, top_p, rng, logprobs, records)
-                    continue
-            entries = [(req.rid, toks, [len(toks) - 1] if sample else []) for req, toks, sample in plan]
-            logits = self.step(entries, adapters={rid: named.get(rid) for rid, _, _ in entries} if named else None)
-            picked, said = [], None
-            if logits is not None:
-                out = self._sample(logits, do_sample, temperature, top_p, seed)
-                if logprobs is not None:
-                    said = _records(seq_ops.token_logprobs(logits, out, top=logprobs, temperature=temperature if do_sample else 1.0))
-                picked = out.tolist()
-            it, told = iter(picked), iter(said or ())
-            for req, toks, sample in plan:
-                if sample and said is not None:
-                    records.setdefault(req.rid, []).append(next(told))
-                if sched.advance(req, len(toks), next(it) if sample else None):
-                    self.release(req.rid)
+        with self._released_on_errors([("gen", i) for i in range(len(prompts))]):
+            while not sched.idle():
+                plan = sched.plan()
+                if not plan:
+                    raise RuntimeError("scheduler made no progress")
+                if draft is not None and all(req.fed == len(req.prompt) for req, _, _ in plan):
+                    guessed = self._guesses(plan, draft)
+                    if any(len(toks) > 1 for _, toks, _ in guessed):
+                        self._drafted_turn(plan, guessed, sched, do_sample, temperature, top_p, rng, logprobs, records)
+                        continue
+                entries = [(req.rid, toks, [len(toks) - 1] if sample else []) for req, toks, sample in plan]
+                logits = self.step(entries, adapters={rid: named.get(rid) for rid, _, _ in entries} if named else None)
+                picked, said = [], None
+                if logits is not None:
+                    out = self._sample(logits, do_sample, temperature, top_p, seed)
+                    if logprobs is not None:
+                        said = _records(seq_ops.token_logprobs(logits, out, top=logprobs, temperature=temperature if do_sample else 1.0))
+                    picked = out.tolist()
+                it, told = iter(picked), iter(said or ())
+                for req, toks, sample in plan:
+                    if sample and said is not None:
+                        records.setdefault(req.rid, []).append(next(told))
+                    if sched.advance(req, len(toks), next(it) if sample else None):
+                        self.release(req.rid)
         tokens = [sched.finished[("gen", i)] for i in range(len(prompts))]
         return tokens if logprobs is None else (tokens, [records.get(("gen", i), []) for i in range(len(prompts))])
+
+    @contextlib.contextmanager
+    def _released_on_errors(self, rids):
+        """What raises in between (a `draft` that the caller gave, rows that are no distribution) leaves none of these requests behind."""
+        try:
+            yield
+        except BaseException:
+            for rid in rids:
+                if rid in self.store.live:
+                    self.release(rid)
+            raise
 
     def _guesses(self, plan, draft):
         """Entries of a drafted step: every decoding request's newest token and what is guessed behind it."""

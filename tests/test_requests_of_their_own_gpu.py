@@ -370,3 +370,19 @@ def test_adapters_and_forks_of_every_family(family, seed):
     a = torch.cat([rest[0][:8]] + [r[1:] for r in rest[1:]])
     c = torch.cat([rest[0][8:]] + [r[:1] for r in rest[1:]])
     assert rel_err(a, want[40:]) < TOL[torch.float32] and rel_err(c, want[40:]) < TOL[torch.float32]
+
+
+def test_guesses_that_are_wrong_leave_no_request_behind():
+    eng, prompts = engine(ATTENTION, torch.float32), [toks(20, 80, 1), toks(33, 80, 2)]
+    want = eng.generate(prompts, 12)
+
+    def raises(history):
+        raise OSError("no guess")
+
+    for draft, error in ((raises, OSError), (lambda h: ([5, 6], [-1]), ValueError), (lambda h: ([5], [3]), ValueError), (lambda h: ([80], [-1]), IndexError), (lambda h: ([-1], [-1]), IndexError)):
+        with pytest.raises(error):
+            eng.generate(prompts, 12, draft=draft)
+        assert not eng.store.live and len(eng.store.free_slots) == eng.store.num_slots and len(eng.store.pool.free) == eng.store.pool.num_pages
+    assert eng.generate(prompts, 12, draft=lambda h: ([5, 6, 7], [-1, -1, 0])) == want
+    assert eng.generate(prompts, 12, draft=lambda h: ([5] * 40, range(-1, 39))) == want  # more than there is room for
+    assert eng.generate(prompts, 12, draft=lambda h: ([], [])) == want
