@@ -258,3 +258,35 @@ def test_a_long_chain():
             stop = n if wrong is None else wrong
             assert got[1].tolist() == [stop] * copies and got[0][-1].tolist() == list(range(stop)) + [-1] * (n - stop)
             assert got[2].tolist() == [int(logits[stop - 1].argmax())] * copies
+
+
+@pytest.mark.parametrize("step", ["bfloat16", 0.125, 0.002])
+@pytest.mark.parametrize("V,spread,top_p", [(257216, 3.0, 0.9), (32000, 2.0, 0.7), (32000, 0.3, 0.5), (5000, 4.0, 0.95)])
+def test_logits_of_few_values(step, V, spread, top_p):
+    """Many entries equal the border's, in shares of several CTAs; runs of bit patterns that are divided until they are one."""
+    ns = [3, 4, 2]
+    logits, draft, parents, tokens, u = make(ns, V, 2, 13, spread=spread, temperature=0.8, top_p=top_p)
+    coarse = (lambda t: t.bfloat16().float()) if step == "bfloat16" else (lambda t: (t / step).round() * step)
+    logits, draft = coarse(logits), coarse(draft)
+    for d in (None, draft):
+        got = seq_ops.verify_drafts(logits.cuda(), batch(ns, parents, tokens), u.cuda(), None if d is None else d.cuda(), 0.8, top_p)
+        check(got, ns, logits, parents, tokens, u, d, 0.8, top_p)
+
+
+@pytest.mark.parametrize("greedy,entries,n", [(True, 230, 9), (True, 300, 10), (False, 1900, 9)])
+def test_more_rows_than_the_walk_keeps_in_shared_memory(greedy, entries, n):
+    V, ns = 24, [n] * entries
+    logits, draft, parents, tokens, u = make(ns, V, 2, 17, agree=0.2)
+    u = None if greedy else u
+    got = seq_ops.verify_drafts(logits.cuda(), batch(ns, parents, tokens), None if greedy else u.cuda(), None if greedy else draft.cuda())
+    check(got, ns, logits, parents, tokens, u, None if greedy else draft, 1.0, 1.0)
+
+
+def test_one_row_behind_another_that_is_not_drafted():
+    """A step in which some entries bring prompts: their rows are a chain, their tokens are judged like guesses."""
+    V, ns, g = 700, [1, 70, 5, 1], torch.Generator().manual_seed(23)
+    logits = torch.randn(sum(ns), V, generator=g) * 3
+    parents = [i - 1 for n in ns for i in range(n)]
+    tokens = [int(t) for t in torch.randint(0, V, (sum(ns),), generator=g)]
+    got = seq_ops.verify_drafts(logits.cuda(), batch(ns, parents, tokens))
+    check(got, ns, logits, parents, tokens, None, None, 1.0, 1.0)
