@@ -834,7 +834,7 @@ int pg_keep_rows(const PgKeepRows* a, void* stream);
  *   draft (row v: the distribution q that v's children were drawn from): c = 0, S = 1; children in order: x stays if uniforms[child, 0] q(x) S < max(p(x) - c q(x), 0),
  *     else c += S, S = sum max(p - c q, 0).  Where none stays the walk ends with a draw from max(p - c q, 0), from p where that is nothing
  * path[e, 0 .. kept[e]) = the rows of the walk (-1 behind), next[e] = the token behind it.  A row without a distribution (a NaN, a +inf, nothing but -inf; of the
- * draft's only those with children count) ends the walk with -1.  outcome: rows + 1 words of scratch. */
+ * draft's only those with children count) ends the walk with -1.  outcome: 2 rows + 1 words of scratch on an 8-byte boundary. */
 typedef struct {
   const float *logits, *draft, *uniforms;
   const int *tokens, *parents, *row0, *n;

@@ -19,13 +19,14 @@
 // counted runs, for the run that holds the border and the mass above it; the one that holds the drawn token finishes alone.
 //
 // What bounds it: few rows, that chain (5 rows 29 us, of which 5 are passes; 35 with seven meetings); many rows, how fast an SM takes them from L2 (6.7 TB/s over all while their
-// passes coincide) and the chains between: 256 rows of 257216 beside a draft 257 us, 1.2 TB/s of DRAM, 46 % of the issue slots.  Greedy rows are one pass: 128 of them, some 76 judged, 32 us.
+// passes coincide) and the chains between: 256 rows of 257216 beside a draft 257 us, 1.2 TB/s of DRAM, 46 % of the issue slots.  Greedy walks have a kernel of their own, one pass: 104 rows
+// 27 us, 17 of which their bytes take (with a cluster a row as well 32, some rows left out).
 #include "common.cuh"
 #include "paligemma_b200.h"
 
 namespace {
 
-constexpr int kThreads = 512, kPerSm = 2, kPerSmGreedy = 4, kWarps = kThreads / 32, kRanks = 16, kBins = 1024, kCoarse = kBins / 32, kTable = 256, kList = 32;
+constexpr int kThreads = 512, kPerSm = 2, kWarps = kThreads / 32, kRanks = 16, kBins = 1024, kCoarse = kBins / 32, kTable = 256, kList = 32;
 constexpr int kRun = 128, kRuns = 4;  // entries that a warp takes at once, a float4 a lane; runs under way
 constexpr int kHeld = 512;            // entries of a row that a warp can hold as candidates of the nucleus
 constexpr int kDead = -2147483647 - 1;
@@ -65,13 +66,13 @@ struct __align__(16) Shared {
   double warp[kWarps];
   double all[2][kRanks], part[2][kRanks];  // doubles of every CTA, by turns
   double warp_part[kWarps];
-  unsigned long long key[2][kRanks];
+  unsigned long long top[2][kRanks];       // a CTA's largest entry and what the threads' largest ones sum up to
   unsigned long long hist[kBins];          // mass of runs of bit patterns
   unsigned long long coarse[kRanks][kCoarse], fine[kRanks][32];
   Entry own[kList], list[kRanks][kList];   // entries of the run that holds the border
   int held_count[kWarps], listed[kRanks], over[2][kRanks];
   unsigned long long found_base;
-  float largest[kWarps], whole[2][kRanks]; // what the threads' largest entries sum up to, relative to the CTA's
+  float largest[kWarps];
   int found, pick, state, last, own_listed;
   uint32_t least, top_key;
   int V, bits;
@@ -210,76 +211,47 @@ PG_DEVINL float ex2(float x) {
   return y;
 }
 
-// (largest entry, lowest place) of the row as one number, known to all CTAs.  PLACE false: the entry alone, and in `whole` the sum of the largest entries' weights of all threads,
-// scale being log2(e) / T: less than the row's.
-template <bool PLACE>
-PG_DEVINL unsigned long long row_top(Shared& sh, const Part& p, const Source& s, int& turn, const double& scale, float& whole) {
-  float best = -INFINITY;  // this thread's largest
-  int run = 0;
-  each4(p, s, [&](int i, float4 x) {
-    if (PLACE) {
-      const float four = max_nan(max_nan(x.x, x.y), x.z, x.w);
-      if (four > best) run = i;
-      best = max_nan(best, four);  // (where that is a NaN the place does not matter)
-    } else {
-      best = max_nan(max_nan(best, x.x, x.y), x.z, x.w);
-    }
-  });
-  int at = 0;
-  if (PLACE && run < p.n) {  // the first of the four that were the first to hold it
-    const float4 x = s.four(run, p.n);
-    at = p.lo + run + (x.x == best ? 0 : x.y == best ? 1 : x.z == best ? 2 : 3);
-  }
-  unsigned long long key = static_cast<unsigned long long>(ordered(best)) << 32 | static_cast<uint32_t>(~at);
+PG_DEVINL unsigned long long warp_max(unsigned long long key) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, o);
     key = other > key ? other : key;
   }
-  unsigned long long* mine = reinterpret_cast<unsigned long long*>(sh.warp);
+  return key;
+}
+
+// The row's largest entry as an ordered pattern (a NaN above all), known to all CTAs, and in `whole` the sum of the largest entries' weights of all threads, scale being log2(e) / T:
+// less than the row's.
+PG_DEVINL uint32_t row_top(Shared& sh, const Part& p, const Source& s, int& turn, const double& scale, float& whole) {
+  float best = -INFINITY;  // this thread's largest
+  each4(p, s, [&](int, float4 x) { best = max_nan(max_nan(best, x.x, x.y), x.z, x.w); });
+  const uint32_t key = __reduce_max_sync(0xffffffffu, ordered(best));
+  uint32_t* mine = reinterpret_cast<uint32_t*>(sh.warp);
   __syncthreads();  // (the sums before have been read)
   if (threadIdx.x % 32 == 0) mine[threadIdx.x / 32] = key;
   __syncthreads();
-  if (threadIdx.x < 32) {
-    key = threadIdx.x < kWarps ? mine[threadIdx.x] : 0ull;
+  const float a = static_cast<float>(scale);  // (behind a barrier: the first row's may have been written just now)
+  const uint32_t here = __reduce_max_sync(0xffffffffu, mine[threadIdx.x % kWarps]);
+  float some = ex2((best - unordered(here)) * a);
 #pragma unroll
-    for (int o = kWarps / 2; o > 0; o >>= 1) {
-      const unsigned long long other = __shfl_xor_sync(0xffffffffu, key, o);
-      key = other > key ? other : key;
-    }
-    key = __shfl_sync(0xffffffffu, key, 0);
-    if (static_cast<int>(threadIdx.x) < p.ranks) put64(&sh.key[turn][p.rank], threadIdx.x, key);
-  }
-  const float a = PLACE ? 0.0f : static_cast<float>(scale);  // (behind a barrier: the first row's may have been written just now)
-  if (!PLACE) {
-    unsigned long long here = 0;
-    for (int w = 0; w < kWarps; ++w) here = mine[w] > here ? mine[w] : here;
-    float some = ex2((best - unordered(static_cast<uint32_t>(here >> 32))) * a);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) some += __shfl_xor_sync(0xffffffffu, some, o);
-    if (threadIdx.x % 32 == 0) sh.largest[threadIdx.x / 32] = some;
-    __syncthreads();
-    if (static_cast<int>(threadIdx.x) < p.ranks) {
-      some = 0.0f;
-      for (int w = 0; w < kWarps; ++w) some += sh.largest[w];
-      put32(&sh.whole[turn][p.rank], threadIdx.x, __float_as_int(some));
-    }
+  for (int o = 16; o > 0; o >>= 1) some += __shfl_xor_sync(0xffffffffu, some, o);
+  if (threadIdx.x % 32 == 0) sh.largest[threadIdx.x / 32] = some;
+  __syncthreads();
+  if (static_cast<int>(threadIdx.x) < p.ranks) {
+    some = 0.0f;
+    for (int w = 0; w < kWarps; ++w) some += sh.largest[w];
+    put64(&sh.top[turn][p.rank], threadIdx.x, static_cast<unsigned long long>(here) << 32 | __float_as_uint(some));
   }
   pg::cluster_sync_all();
-  unsigned long long top = 0;
-  for (int r = 0; r < p.ranks; ++r) top = sh.key[turn][r] > top ? sh.key[turn][r] : top;
-  if (!PLACE) {
-    whole = 0.0f;
-    const float m = unordered(static_cast<uint32_t>(top >> 32));
-    for (int r = 0; r < p.ranks; ++r) whole += sh.whole[turn][r] * ex2((unordered(static_cast<uint32_t>(sh.key[turn][r] >> 32)) - m) * a);
-  }
+  uint32_t top = 0;
+  for (int r = 0; r < p.ranks; ++r) top = max(top, static_cast<uint32_t>(sh.top[turn][r] >> 32));
+  whole = 0.0f;
+  const float m = unordered(top);
+  for (int r = 0; r < p.ranks; ++r) whole += __uint_as_float(static_cast<uint32_t>(sh.top[turn][r])) * ex2((unordered(static_cast<uint32_t>(sh.top[turn][r] >> 32)) - m) * a);
   turn ^= 1;
   return top;
 }
-PG_DEVINL bool is_distribution(unsigned long long top) {
-  const uint32_t k = static_cast<uint32_t>(top >> 32);
-  return k > ordered(-INFINITY) && k < ordered(INFINITY);
-}
+PG_DEVINL bool is_distribution(uint32_t top) { return top > ordered(-INFINITY) && top < ordered(INFINITY); }
 
 // What the warps have summed: theirs in sh.warp, the CTAs' in sh.all[turn] (until the next but one), the whole as the result.  The order of additions is fixed.  `over` of any
 // thread becomes all CTAs'; `part`: a second sum.  counted: the runs of sh.hist go along, 32 at a time.
@@ -630,16 +602,16 @@ __device__ __noinline__ Nucleus row_nucleus(Shared& sh, const Part p, const Sour
 PG_DEVINL int distribution(Shared& sh, const Part p, const Source s, const int which, int turn) {
   count_begin(sh);
   float some;
-  const unsigned long long top = row_top<false>(sh, p, s, turn, sh.how[which].a, some);
+  const uint32_t top = row_top(sh, p, s, turn, sh.how[which].a, some);
   if (!is_distribution(top)) {
     if (threadIdx.x == 0) sh.row[which].good = false;
     __syncthreads();
     return turn;
   }
   const double temperature = sh.how[which].temperature;
-  if (threadIdx.x == 0) sh.top_key = static_cast<uint32_t>(top >> 32);
+  if (threadIdx.x == 0) sh.top_key = top;
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const float m = unordered(static_cast<uint32_t>(top >> 32));
+  const float m = unordered(top);
   Scale sc = scale_of(m, sh.how[which].a, temperature);
   const bool in_fp32 = sc.fine > -INFINITY;
   const double whole = logf(fmaxf(1.0f, 0.99f * some));  // small is what is below 2^-16 of e^whole
@@ -770,9 +742,7 @@ PG_DEVINL bool may_be_reached(const int* parents, const int* outcome, int v) {
   }
 }
 
-// GREEDY: no random numbers.  `room`: rows whose outcomes have room in shared memory.
-template <bool GREEDY>
-__global__ void __launch_bounds__(kThreads, GREEDY ? kPerSmGreedy : kPerSm) verify_kernel(const PgVerify a, int share, int bits, int room) {
+__global__ void __launch_bounds__(kThreads, kPerSm) verify_kernel(const PgVerify a, int share, int bits) {
   extern __shared__ __align__(16) char raw[];
   Shared& sh = *reinterpret_cast<Shared*>(raw);
   uint32_t ranks;
@@ -807,104 +777,94 @@ __global__ void __launch_bounds__(kThreads, GREEDY ? kPerSmGreedy : kPerSm) veri
     const float *logits = a.logits + row * a.ld, *draft = a.draft + row * a.draft_ld;
     const Source target(logits, p.lo);
     fam.look();
-    if (!GREEDY) {
-      if (tid >= kTable && tid < kTable + 2) {
-        const bool draft = tid == kTable;
-        const double temperature = draft ? a.draft_temperature : a.temperature, top_p = draft ? a.draft_top_p : a.top_p;
-        if (!draft || a.draft != nullptr) sh.how[tid - kTable] = How{temperature, top_p, kLog2e / temperature, top_p < 1.0 ? log(16.0 * (1.0 - top_p) / a.V) : 0.0};
-        sh.V = a.V, sh.bits = bits;
-      }
-      if (tid < kTable) sh.table[tid] = exp2(static_cast<double>(tid) / kTable);
-    }  // (read behind the first barriers of row_top)
-    if constexpr (GREEDY) {
-      float whole;
-      const unsigned long long top = row_top<true>(sh, p, target, turn, 0.0, whole);
-      const int token = is_distribution(top) ? static_cast<int>(~static_cast<uint32_t>(top)) : -1;
-      const int next = token >= 0 ? fam.with(token) : n;
-      to = next < n ? next : -2 - token;
-    } else {
-      const float u = unit_number(a.uniforms[2 * row + 1]);
-      const Source other(draft, p.lo);
-      int child = a.draft != nullptr ? fam.child(v + 1, x) : n;
-      bool good = true;
+    if (tid >= kTable && tid < kTable + 2) {
+      const bool draft = tid == kTable;
+      const double temperature = draft ? a.draft_temperature : a.temperature, top_p = draft ? a.draft_top_p : a.top_p;
+      if (!draft || a.draft != nullptr) sh.how[tid - kTable] = How{temperature, top_p, kLog2e / temperature, top_p < 1.0 ? log(16.0 * (1.0 - top_p) / a.V) : 0.0};
+      sh.V = a.V, sh.bits = bits;
+    }
+    if (tid < kTable) sh.table[tid] = exp2(static_cast<double>(tid) / kTable);  // (read behind the first barriers of row_top)
+    const float u = unit_number(a.uniforms[2 * row + 1]);
+    const Source other(draft, p.lo);
+    int child = a.draft != nullptr ? fam.child(v + 1, x) : n;
+    bool good = true;
 #pragma unroll 1
-      for (int which = child < n ? 0 : 1; which < 2 && good; ++which) {
-        turn = distribution(sh, p, which == 0 ? other : target, which, turn);
-        good = sh.row[which].good;
-      }
-      if (!good) {
-        to = -1;
-      } else {
-        const Row &t = sh.row[1], &q = sh.row[child < n ? 0 : 1];
-        const Scale ts = t.s, qs = q.s;
-        double mass = t.mass, c = 0.0, left = 1.0, pf = 0.0, qf = 0.0;
-        // max(p - c q, 0); both products rounded alike, so that equal ones leave nothing
-        auto rest_of = [&](double wt, double wq) { return fmax(__dsub_rn(__dmul_rn(pf, wt), __dmul_rn(qf, wq)), 0.0); };
-        auto rest4 = [&](int i, float4 y, double (&w)[4]) {
-          const float4 z = other.four(i, p.n);
-          w[0] = rest_of(weight(sh.table, ts, y.x), weight(sh.table, qs, z.x)), w[1] = rest_of(weight(sh.table, ts, y.y), weight(sh.table, qs, z.y));
-          w[2] = rest_of(weight(sh.table, ts, y.z), weight(sh.table, qs, z.z)), w[3] = rest_of(weight(sh.table, ts, y.w), weight(sh.table, qs, z.w));
-        };
-        const float bound = t.bound;
-        const bool quick = child < n && t.listed && qs.fine > -INFINITY;
-        const Pairs small_t(ts), small_q(qs);
-        float pf0 = 0.0f, pf1 = 0.0f, qf0 = 0.0f, qf1 = 0.0f;  // the factors in two parts
-        auto rest_sum = [&](int i, float4 y) {
-          if (!quick) {
-            double w[4];
-            rest4(i, y, w);
-            return (w[0] + w[1]) + (w[2] + w[3]);
-          }
-          const float4 z = other.four(i, p.n);  // (what is not small is added from the candidates; what p has not is not there, whatever q has)
-          const float2 t0 = small_t(y.x, y.y), t1 = small_t(y.z, y.w), q0 = small_q(z.x, z.y), q1 = small_q(z.z, z.w);
-          const float ys[4] = {y.x, y.y, y.z, y.w}, zs[4] = {z.x, z.y, z.z, z.w}, wt[4] = {t0.x, t0.y, t1.x, t1.y}, wq[4] = {q0.x, q0.y, q1.x, q1.y};
-          float w = 0.0f;
+    for (int which = child < n ? 0 : 1; which < 2 && good; ++which) {
+      turn = distribution(sh, p, which == 0 ? other : target, which, turn);
+      good = sh.row[which].good;
+    }
+    if (!good) {
+      to = -1;
+    } else {
+      const Row &t = sh.row[1], &q = sh.row[child < n ? 0 : 1];
+      const Scale ts = t.s, qs = q.s;
+      double mass = t.mass, c = 0.0, left = 1.0, pf = 0.0, qf = 0.0;
+      // max(p - c q, 0); both products rounded alike, so that equal ones leave nothing
+      auto rest_of = [&](double wt, double wq) { return fmax(__dsub_rn(__dmul_rn(pf, wt), __dmul_rn(qf, wq)), 0.0); };
+      auto rest4 = [&](int i, float4 y, double (&w)[4]) {
+        const float4 z = other.four(i, p.n);
+        w[0] = rest_of(weight(sh.table, ts, y.x), weight(sh.table, qs, z.x)), w[1] = rest_of(weight(sh.table, ts, y.y), weight(sh.table, qs, z.y));
+        w[2] = rest_of(weight(sh.table, ts, y.z), weight(sh.table, qs, z.z)), w[3] = rest_of(weight(sh.table, ts, y.w), weight(sh.table, qs, z.w));
+      };
+      const float bound = t.bound;
+      const bool quick = child < n && t.listed && qs.fine > -INFINITY;
+      const Pairs small_t(ts), small_q(qs);
+      float pf0 = 0.0f, pf1 = 0.0f, qf0 = 0.0f, qf1 = 0.0f;  // the factors in two parts
+      auto rest_sum = [&](int i, float4 y) {
+        if (!quick) {
+          double w[4];
+          rest4(i, y, w);
+          return (w[0] + w[1]) + (w[2] + w[3]);
+        }
+        const float4 z = other.four(i, p.n);  // (what is not small is added from the candidates; what p has not is not there, whatever q has)
+        const float2 t0 = small_t(y.x, y.y), t1 = small_t(y.z, y.w), q0 = small_q(z.x, z.y), q1 = small_q(z.z, z.w);
+        const float ys[4] = {y.x, y.y, y.z, y.w}, zs[4] = {z.x, z.y, z.z, z.w}, wt[4] = {t0.x, t0.y, t1.x, t1.y}, wq[4] = {q0.x, q0.y, q1.x, q1.y};
+        float w = 0.0f;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float b = zs[k] >= qs.cut ? wq[k] : 0.0f;
-            const float left_over = __fsub_rn(fmaf(wt[k], pf0, __fmul_rn(wt[k], pf1)), fmaf(b, qf0, __fmul_rn(b, qf1)));
-            w += ys[k] < bound && ys[k] >= ts.cut ? fmaxf(left_over, 0.0f) : 0.0f;
-          }
-          return static_cast<double>(w);
-        };
-        auto rest1 = [&](const Candidate& k) { return k.x >= ts.cut ? rest_of(weight(sh.table, ts, k.x), weight(sh.table, qs, other.x[k.at])) : 0.0; };
-        auto rest_mass = [&]() {
-          double sum = 0.0;
-          each4(p, target, [&](int i, float4 y) { sum += rest_sum(i, y); });
-          if (quick)
-            for (int i = tid % 32; i < sh.held_count[tid / 32]; i += 32) sum += rest1(sh.held[tid / 32][i]);
-          return share_sums(sh, p, turn, sum);
-        };
-        while (child < n) {
-          if (x >= 0 && x < a.V) {  // (what is no token was drawn from nothing: it takes nothing away)
-            const double pt = weight(sh.table, ts, logits[x]) / mass, qt = weight(sh.table, qs, draft[x]) / q.mass;
-            const bool stays = static_cast<double>(unit_number(a.uniforms[2 * (row0 + child)])) * qt * left < __dsub_rn(pt, __dmul_rn(c, qt));
-            if (stays) break;
-            c += left;
-            pf = 1.0 / mass, qf = c / q.mass;
-            pf0 = static_cast<float>(pf), pf1 = static_cast<float>(pf - pf0), qf0 = static_cast<float>(qf), qf1 = static_cast<float>(qf - qf0);
-            left = t.held ? held_mass(sh, p, turn, rest1) : rest_mass();
-            if (!(left > 0.0)) break;
-          }
-          child = fam.child(child + 1, x);
+        for (int k = 0; k < 4; ++k) {
+          const float b = zs[k] >= qs.cut ? wq[k] : 0.0f;
+          const float left_over = __fsub_rn(fmaf(wt[k], pf0, __fmul_rn(wt[k], pf1)), fmaf(b, qf0, __fmul_rn(b, qf1)));
+          w += ys[k] < bound && ys[k] >= ts.cut ? fmaxf(left_over, 0.0f) : 0.0f;
         }
-        if (child < n && left > 0.0) {
-          to = child;
+        return static_cast<double>(w);
+      };
+      auto rest1 = [&](const Candidate& k) { return k.x >= ts.cut ? rest_of(weight(sh.table, ts, k.x), weight(sh.table, qs, other.x[k.at])) : 0.0; };
+      auto rest_mass = [&]() {
+        double sum = 0.0;
+        each4(p, target, [&](int i, float4 y) { sum += rest_sum(i, y); });
+        if (quick)
+          for (int i = tid % 32; i < sh.held_count[tid / 32]; i += 32) sum += rest1(sh.held[tid / 32][i]);
+        return share_sums(sh, p, turn, sum);
+      };
+      while (child < n) {
+        if (x >= 0 && x < a.V) {  // (what is no token was drawn from nothing: it takes nothing away)
+          const double pt = weight(sh.table, ts, logits[x]) / mass, qt = weight(sh.table, qs, draft[x]) / q.mass;
+          const bool stays = static_cast<double>(unit_number(a.uniforms[2 * (row0 + child)])) * qt * left < __dsub_rn(pt, __dmul_rn(c, qt));
+          if (stays) break;
+          c += left;
+          pf = 1.0 / mass, qf = c / q.mass;
+          pf0 = static_cast<float>(pf), pf1 = static_cast<float>(pf - pf0), qf0 = static_cast<float>(qf), qf1 = static_cast<float>(qf - qf0);
+          left = t.held ? held_mass(sh, p, turn, rest1) : rest_mass();
+          if (!(left > 0.0)) break;
+        }
+        child = fam.child(child + 1, x);
+      }
+      if (child < n && left > 0.0) {
+        to = child;
+      } else {
+        int token;
+        if (c > 0.0 && left > 0.0) {
+          token = t.held ? held_draw(sh, p, turn, left, u, finisher, rest1) : row_draw(sh, p, target, turn, left, u, finisher, rest4);
         } else {
-          int token;
-          if (c > 0.0 && left > 0.0) {
-            token = t.held ? held_draw(sh, p, turn, left, u, finisher, rest1) : row_draw(sh, p, target, turn, left, u, finisher, rest4);
-          } else {
-            auto one = [&](const Candidate& k) { return weight(sh.table, ts, k.x); };
-            auto four = [&](int, float4 y, double (&w)[4]) {
-              w[0] = weight(sh.table, ts, y.x), w[1] = weight(sh.table, ts, y.y), w[2] = weight(sh.table, ts, y.z), w[3] = weight(sh.table, ts, y.w);
-            };
-            if (c > 0.0) mass = t.held ? held_mass(sh, p, turn, one) : row_mass(sh, p, target, turn, [&](int, float4 y) { return weights_sum(sh.table, ts, small_t, y); });
-            token = t.held ? held_draw(sh, p, turn, mass, u, finisher, one) : row_draw(sh, p, target, turn, mass, u, finisher, four);
-          }
-          const int next = a.draft == nullptr && rank == finisher ? fam.with(token) : n;
-          to = next < n ? next : -2 - token;
+          auto one = [&](const Candidate& k) { return weight(sh.table, ts, k.x); };
+          auto four = [&](int, float4 y, double (&w)[4]) {
+            w[0] = weight(sh.table, ts, y.x), w[1] = weight(sh.table, ts, y.y), w[2] = weight(sh.table, ts, y.z), w[3] = weight(sh.table, ts, y.w);
+          };
+          if (c > 0.0) mass = t.held ? held_mass(sh, p, turn, one) : row_mass(sh, p, target, turn, [&](int, float4 y) { return weights_sum(sh.table, ts, small_t, y); });
+          token = t.held ? held_draw(sh, p, turn, mass, u, finisher, one) : row_draw(sh, p, target, turn, mass, u, finisher, four);
         }
+        const int next = a.draft == nullptr && rank == finisher ? fam.with(token) : n;
+        to = next < n ? next : -2 - token;
       }
     }
     if (rank == finisher && tid == 0) outcome[v] = to;
@@ -918,7 +878,7 @@ __global__ void __launch_bounds__(kThreads, GREEDY ? kPerSmGreedy : kPerSm) veri
     }
     __syncthreads();
     if (sh.last) {
-      const bool fits = a.rows <= room;  // (the candidates are not needed any more)
+      const bool fits = a.rows <= static_cast<int>(sizeof(sh.held) / sizeof(int));  // (the candidates are not needed any more)
       int* held = reinterpret_cast<int*>(sh.held);
       if (fits)
         for (int i = tid; i < a.rows; i += kThreads) held[i] = load_relaxed(a.outcome + i);
@@ -947,32 +907,89 @@ __global__ void __launch_bounds__(kThreads, GREEDY ? kPerSmGreedy : kPerSm) veri
   // (what the CTAs hand one another lies in front of a barrier that all have passed)
 }
 
-template <bool GREEDY>
-int launch(const PgVerify& a, long long items, int ranks, int share, int bits, cudaStream_t st) {
-  constexpr int kRoom = GREEDY ? 2048 : static_cast<int>(sizeof(Shared::held) / sizeof(int));  // (a greedy row has no candidates)
-  constexpr int kSmem = GREEDY ? static_cast<int>(offsetof(Shared, held) + kRoom * sizeof(int)) : static_cast<int>(sizeof(Shared));
-  static bool configured[pg::kMaxDevices] = {};
-  bool& done = configured[pg::current_device()];
-  if (!done) {
-    if (cudaFuncSetAttribute(verify_kernel<GREEDY>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess ||
-        cudaFuncSetAttribute(verify_kernel<GREEDY>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
-      cudaGetLastError();
-      return PG_ERR_CUDA;
+// Greedy walks: one pass over all rows of the step, cut into pieces that the CTAs share evenly; (largest entry, lowest place) of a row meet in one word each.  The CTA that is through
+// last walks, a warp an entry: 32 rows of it in the lanes.
+constexpr int kPiece = 4 * kThreads;  // (two CTAs an SM, four loads a thread: 27 us; three or four, eight loads: 27, 29, 29)
+__global__ void __launch_bounds__(kThreads, kPerSm) greedy_kernel(const PgVerify a, int pieces, long long all) {
+  __shared__ int last;
+  unsigned long long* keys = reinterpret_cast<unsigned long long*>(a.outcome);
+  const int tid = threadIdx.x, lane = tid % 32;
+  const long long end = all * (blockIdx.x + 1) / gridDim.x;
+  for (long long u = all * blockIdx.x / gridDim.x; u < end;) {
+    const long long row = u / pieces;
+    const int p0 = static_cast<int>(u % pieces), p1 = static_cast<int>(min(static_cast<long long>(pieces), p0 + (end - u)));
+    const int hi = static_cast<int>(min(static_cast<long long>(a.V), static_cast<long long>(p1) * kPiece));
+    const Source s(a.logits + row * a.ld, 0);
+    float best = -INFINITY;
+    int i = p0 * kPiece + 4 * tid, run = i;  // run: the first four that hold it
+    auto take = [&](int at, float4 x) {
+      const float four = max_nan(max_nan(x.x, x.y), x.z, x.w);
+      if (four > best) run = at;
+      best = max_nan(best, four);  // (where that is a NaN the place does not matter)
+    };
+    if (s.aligned)
+      for (; i + 3LL * kPiece + 4 <= hi; i += 4 * kPiece) {
+        float4 x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = __ldg(reinterpret_cast<const float4*>(s.x + i + k * kPiece));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) take(i + k * kPiece, x[k]);
+      }
+    for (; i < hi; i += kPiece) take(i, s.four(i, hi));
+    unsigned long long key = 0;
+    if (run < hi) {
+      const float4 x = s.four(run, hi);
+      const int at = run + (x.x == best ? 0 : x.y == best ? 1 : x.z == best ? 2 : 3);
+      key = static_cast<unsigned long long>(ordered(best)) << 32 | static_cast<uint32_t>(~at);
     }
-    done = true;
+    key = warp_max(key);
+    if (lane == 0) atomicMax(keys + row, key);
+    u += p1 - p0;
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(items * ranks));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kSmem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ranks;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, verify_kernel<GREEDY>, a, share, bits, kRoom) == cudaSuccess ? PG_OK : PG_ERR_CUDA;
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) {
+    last = atomicAdd(a.outcome + 2 * static_cast<long long>(a.rows), 1) == static_cast<int>(gridDim.x) - 1;
+    __threadfence();
+  }
+  __syncthreads();
+  if (!last) return;
+  for (int e = tid / 32; e < a.entries; e += kWarps) {
+    const int m = a.n[e], row0 = a.row0[e];
+    int* path = a.path + e * a.path_ld;
+    int kept = 0, next = -1;
+    if (m > 0 && m <= a.path_ld && row0 >= 0 && row0 + static_cast<long long>(m) <= a.rows) {
+      int base = 0, up = 0, token = 0, said = -1;  // rows base .. base + 31: what they follow, carry and say
+      auto look = [&](int b) {
+        base = b;
+        const int j = b + lane;
+        if (j >= m) return;
+        const unsigned long long key = __ldcg(keys + row0 + j);
+        up = a.parents[row0 + j], token = a.tokens[row0 + j];
+        said = is_distribution(static_cast<uint32_t>(key >> 32)) ? static_cast<int>(~static_cast<uint32_t>(key)) : -1;
+      };
+      look(0);
+      for (int at = 0;;) {
+        if (lane == 0) path[kept] = at;
+        ++kept;
+        const int t = __shfl_sync(0xffffffffu, said, at - base);
+        uint32_t is = 0;
+        if (t >= 0)
+          for (int b = (at + 1) / 32 * 32; b < m && is == 0; b += 32) {
+            if (b != base) look(b);
+            const int j = b + lane;
+            is = __ballot_sync(0xffffffffu, j > at && j < m && up == at && token == t);
+          }
+        if (is == 0) {
+          next = t;
+          break;
+        }
+        at = base + __ffs(is) - 1;
+      }
+    }
+    if (lane == 0) a.kept[e] = kept, a.next[e] = next;
+    for (long long i = kept + lane; i < a.path_ld; i += 32) path[i] = -1;
+  }
 }
 
 }  // namespace
@@ -982,22 +999,49 @@ extern "C" int pg_verify_drafts(const PgVerify* args, void* stream) {
   const PgVerify& a = *args;
   auto sound = [](double temperature, double top_p) { return temperature > 0.0 && temperature < INFINITY && kLog2e / temperature < 1e30 && top_p >= 0.0 && top_p <= 1.0; };
   if (a.logits == nullptr || a.tokens == nullptr || a.parents == nullptr || a.row0 == nullptr || a.n == nullptr || a.path == nullptr || a.kept == nullptr || a.next == nullptr ||
-      a.outcome == nullptr || a.entries <= 0 || a.rows <= 0 || a.max_n <= 0 || a.V <= 0 || a.ld < a.V || a.path_ld < a.max_n || (a.draft != nullptr && (a.draft_ld < a.V || a.uniforms == nullptr)) ||
+      a.outcome == nullptr || (reinterpret_cast<uintptr_t>(a.outcome) & 7) || a.entries <= 0 || a.rows <= 0 || a.max_n <= 0 || a.V <= 0 || a.ld < a.V || a.path_ld < a.max_n || (a.draft != nullptr && (a.draft_ld < a.V || a.uniforms == nullptr)) ||
       !sound(a.temperature, a.top_p) || (a.draft != nullptr && !sound(a.draft_temperature, a.draft_top_p)) || a.V > 0x7fffff00 / 2)
     return PG_ERR_ARG;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  pg_count_launch(1);
+  if (a.uniforms == nullptr) {
+    const int pieces = (a.V + kPiece - 1) / kPiece;
+    const long long all = static_cast<long long>(a.rows) * pieces, most = static_cast<long long>(kPerSm) * pg::num_sms();
+    if (cudaMemsetAsync(a.outcome, 0, sizeof(int) * (2 * static_cast<size_t>(a.rows) + 1), st) != cudaSuccess) return PG_ERR_CUDA;
+    greedy_kernel<<<static_cast<unsigned>(all < most ? all : most), kThreads, 0, st>>>(a, pieces, all);
+    return cudaGetLastError() == cudaSuccess ? PG_OK : PG_ERR_CUDA;
+  }
   const long long items = static_cast<long long>(a.entries) * a.max_n;
-  // CTAs that share a row: so many that a warp's candidates have room, and more while all of them stay within nine an SM, five of greedy rows.  (us with fewer, as taken, more: 5 rows of
-  // 257216 with 4, 8, 16 CTAs 42, 32, 29; 256 beside a draft with 4, 8 257, 308; 624 of 32000 with 1, 2, 4 132, 111, 131; 128 greedy rows of 257216 with 4, 8 32, 35.)
+  // CTAs that share a row: so many that a warp's candidates have room, and more while all of them stay within nine an SM.  (us with fewer, as taken, more: 5 rows of 257216 with 4, 8, 16
+  // CTAs 42, 32, 29; 256 beside a draft with 4, 8 257, 308; 624 of 32000 with 1, 2, 4 132, 111, 131.)
   int ranks = 1;
   while (ranks < kRanks && a.V / ranks > 65536) ranks *= 2;
-  const long long most = a.uniforms == nullptr ? 5 : 9;
-  while (ranks < kRanks && items * ranks * 2 <= most * pg::num_sms() && a.V / (ranks * 2) >= 4 * kThreads) ranks *= 2;
+  while (ranks < kRanks && items * ranks * 2 <= 9LL * pg::num_sms() && a.V / (ranks * 2) >= 4 * kThreads) ranks *= 2;
   if (items * ranks > 0x7fffffff) return PG_ERR_ARG;
   const int share = ((a.V + ranks - 1) / ranks + 3) / 4 * 4;
   int bits = 62;
   while ((1ll << (62 - bits)) < a.V) --bits;  // V weights of at most 1 stay below 2^62
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  static bool configured[pg::kMaxDevices] = {};
+  bool& done = configured[pg::current_device()];
+  if (!done) {
+    if (cudaFuncSetAttribute(verify_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared)) != cudaSuccess ||
+        cudaFuncSetAttribute(verify_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
+      cudaGetLastError();
+      return PG_ERR_CUDA;
+    }
+    done = true;
+  }
   if (cudaMemsetAsync(a.outcome, 0, sizeof(int) * (static_cast<size_t>(a.rows) + 1), st) != cudaSuccess) return PG_ERR_CUDA;
-  pg_count_launch(1);
-  return a.uniforms == nullptr ? launch<true>(a, items, ranks, share, bits, st) : launch<false>(a, items, ranks, share, bits, st);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(items * ranks));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = sizeof(Shared);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ranks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, verify_kernel, a, share, bits) == cudaSuccess ? PG_OK : PG_ERR_CUDA;
 }

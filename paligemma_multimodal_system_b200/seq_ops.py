@@ -993,7 +993,7 @@ def verify_drafts(logits: torch.Tensor, b: StepBatch, uniforms: Optional[torch.T
             raise ValueError(f"logits, random numbers and the step lie on one device: got {t.device} and {logits.device}")
     _on_current_device(logits)
     i32 = dict(dtype=torch.int32, device=logits.device)
-    path, ends, outcome = torch.empty(b.E, b.max_n, **i32), torch.empty(2, b.E, **i32), torch.empty(b.T + 1, **i32)
+    path, ends, outcome = torch.empty(b.E, b.max_n, **i32), torch.empty(2, b.E, **i32), torch.empty(2 * b.T + 1, **i32)
     pitch = V if b.T == 1 else logits.stride(0)
     dpitch = 0 if draft_logits is None else V if b.T == 1 else draft_logits.stride(0)
     a = _lib.VERIFY.pack(logits.data_ptr(), _lib.ptr(draft_logits), _lib.ptr(uniforms), b.tokens.data_ptr(), b.parents.data_ptr(), b.row0.data_ptr(), b.n.data_ptr(), path.data_ptr(),
