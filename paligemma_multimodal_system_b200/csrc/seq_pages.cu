@@ -11,15 +11,13 @@
 
 namespace {
 
-constexpr int kThreads = 256, kLoads = 4, kPiece = kThreads * kLoads * 16, kMoves = 256, kFewMoves = 16, kCols = 64, kRowLanes = kThreads / kCols, kParts = 4;
+constexpr int kThreads = 256, kLoads = 4, kPiece = kThreads * kLoads * 16, kMoves = 256, kCols = 64, kRowLanes = kThreads / kCols, kParts = 4;
 
-// The moves travel as a kernel's argument: one fork is a call of 9 us on the host with room for 16 moves, of 13 with room for 256.
-template <int N>
 struct Moves {
   int n;
-  int at[N][3];  // source page, destination page, rows
+  int at[kMoves][3];  // source page, destination page, rows
 };
-static_assert(sizeof(Moves<kMoves>) < 4000, "an argument");
+static_assert(sizeof(Moves) < 4000, "the moves travel as a kernel's argument");
 
 template <typename U>
 __device__ __forceinline__ void copy_run(const char* src, char* dst, long long lo, long long hi) {
@@ -37,8 +35,7 @@ __device__ __forceinline__ void copy_run(const char* src, char* dst, long long l
   }
 }
 
-template <int N>
-__global__ void __launch_bounds__(kThreads) copy_pages_kernel(const PgPageOperand* __restrict__ ops, const __grid_constant__ Moves<N> mv, int page, int pieces) {
+__global__ void __launch_bounds__(kThreads) copy_pages_kernel(const PgPageOperand* __restrict__ ops, const __grid_constant__ Moves mv, int page, int pieces) {
   pg::griddep_begin();
   const int m = blockIdx.x / pieces;
   const long long lo = static_cast<long long>(blockIdx.x % pieces) * kPiece;
@@ -127,16 +124,6 @@ __global__ void __launch_bounds__(kThreads) keep_rows_kernel(const PgKeepRows a,
   }
 }
 
-template <int N>
-cudaError_t copy_some(const PgPageOperand* operands, int count, int page, long long pieces, const int* moves_host, int n, void* stream) {
-  Moves<N> mv;
-  mv.n = n;
-  for (int i = 0; i < n; ++i)
-    for (int k = 0; k < 3; ++k) mv.at[i][k] = moves_host[3 * i + k];
-  return pg::launch_kernel(copy_pages_kernel<N>, dim3(static_cast<unsigned>(n * pieces), count), dim3(kThreads), 0, static_cast<cudaStream_t>(stream), operands, mv, page,
-                           static_cast<int>(pieces));
-}
-
 }  // namespace
 
 extern "C" int pg_copy_pages(const PgPageOperand* operands, int count, int page, long long most_page_bytes, const int* moves_host, int moves, void* stream) {
@@ -144,10 +131,13 @@ extern "C" int pg_copy_pages(const PgPageOperand* operands, int count, int page,
   const long long pieces = (most_page_bytes + kPiece - 1) / kPiece;
   if (pieces * kMoves > 0x7fffffff) return PG_ERR_ARG;
   for (int at = 0; at < moves; at += kMoves) {
-    const int n = moves - at < kMoves ? moves - at : kMoves;
-    const cudaError_t err = n <= kFewMoves ? copy_some<kFewMoves>(operands, count, page, pieces, moves_host + 3LL * at, n, stream)
-                                           : copy_some<kMoves>(operands, count, page, pieces, moves_host + 3LL * at, n, stream);
-    if (err != cudaSuccess) return PG_ERR_CUDA;
+    Moves mv;
+    mv.n = moves - at < kMoves ? moves - at : kMoves;
+    for (int i = 0; i < mv.n; ++i)
+      for (int k = 0; k < 3; ++k) mv.at[i][k] = moves_host[(at + i) * 3LL + k];
+    if (pg::launch_kernel(copy_pages_kernel, dim3(static_cast<unsigned>(mv.n * pieces), count), dim3(kThreads), 0, static_cast<cudaStream_t>(stream), operands, mv, page,
+                          static_cast<int>(pieces)) != cudaSuccess)
+      return PG_ERR_CUDA;
   }
   return PG_OK;
 }

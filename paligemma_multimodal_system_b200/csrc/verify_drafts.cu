@@ -8,7 +8,7 @@
 // two numbers and a rejection is one pass over the row, whatever came before it.
 //
 // The results are whole numbers that hang on running sums: a draw is wrong once a sum is off by the distance of u from a token's border.  Weights e^((x - m) / T) from
-// 2^-16 on are therefore made in double, 2^(j / 256) from a table times a polynomial of degree 3 (error below 1e-13); smaller ones in fp32, where a run of 128 holds no other.
+// 2^-16 on are therefore made in double, 2^(j / 256) from a table times a polynomial of degree 3 (error below 2e-13); smaller ones in fp32, where a run of 128 holds no other.
 //
 // The nucleus is a threshold on the logit: the entries above which at most top_p Z lies.  Entries below (1 - top_p) Z / V cannot belong to it.  The others are
 // counted by mass into 1024 runs of the ordered bit patterns, in fixed point (sums do not hang on their order).  The entries of the run that holds the border go to

@@ -721,16 +721,16 @@ def copy_pages(cache: CachePages, moves):
     if moves.ndim != 2 or moves.shape[1] != 3 or moves.dtype.kind not in "iu":
         raise ValueError("moves are (source page, destination page, rows)")
     n = len(moves)
-    if n <= 16:  # (a few numbers are looked over faster one by one)
+    if n <= 32:  # (a few numbers are looked over faster one by one)
         rows = moves.tolist()
         inside = all(0 <= a < cache.pages and 0 <= b < cache.pages and 0 <= r <= cache.page for a, b, r in rows)
         to = {b for _, b, _ in rows}
         apart = len(to) == n and not any(a in to for a, _, _ in rows)
     else:
-        most = moves.max(0)
+        most = moves.max(0).tolist()
         inside = moves.min() >= 0 and most[0] < cache.pages and most[1] < cache.pages and most[2] <= cache.page
-        count = np.bincount(moves[:, 1], minlength=cache.pages) if inside else None
-        apart = inside and count.max() == 1 and not count[moves[:, 0]].any()
+        to = set(moves[:, 1].tolist())
+        apart = len(to) == n and to.isdisjoint(moves[:, 0].tolist())
     if not inside:
         raise IndexError(f"moves go between pages 0 .. {cache.pages - 1} and take up to {cache.page} rows")
     if not apart:
