@@ -2,7 +2,7 @@
 //
 // A row decides by itself where the walk goes on from it (the header has the rules), so rows are judged at once, a cluster of CTAs a row, and the walks are
 // pointer chases at the end, made by the last cluster.  Rows lie depth first in their entries and clusters are started in the order of the rows' places in their
-// entries: one that finds that some row above it goes on elsewhere has nothing to do (256 rows beside a draft 281 -> 257 us, 48 trees 149 -> 111).
+// entries: one that finds that some row above it goes on elsewhere has nothing to do (256 rows beside a draft 281 -> 257 us, 48 trees 149 -> 111 when it came).
 //
 // After rejections the rest is r_j = (p - c_j q)+ / S_j: from r_j q is taken again, (p - c_j q)+ - S_j q = p - (c_j + S_j) q where that is positive, so c and S are
 // two numbers and a rejection is one pass over the row, whatever came before it.
@@ -19,7 +19,7 @@
 // counted runs, for the run that holds the border and the mass above it; the one that holds the drawn token finishes alone.
 //
 // What bounds it: few rows, that chain (5 rows 29 us, of which 5 are passes; 35 with seven meetings); many rows, how fast an SM takes them from L2 (6.7 TB/s over all while their
-// passes coincide) and the chains between: 256 rows of 257216 beside a draft 257 us, 1.2 TB/s of DRAM, 46 % of the issue slots.  Greedy walks have a kernel of their own, one pass: 104 rows
+// passes coincide) and the chains between: 256 rows of 257216 beside a draft 253 us, 1.2 TB/s of DRAM, 37 % of the issue slots.  Greedy walks have a kernel of their own, one pass: 104 rows
 // 27 us, 17 of which their bytes take (with a cluster a row as well 32, some rows left out).
 #include "common.cuh"
 #include "paligemma_b200.h"
@@ -28,7 +28,9 @@ namespace {
 
 constexpr int kThreads = 512, kPerSm = 2, kWarps = kThreads / 32, kRanks = 16, kBins = 1024, kCoarse = kBins / 32, kTable = 256, kList = 32;
 constexpr int kRun = 128, kRuns = 4;  // entries that a warp takes at once, a float4 a lane; runs under way
-constexpr int kHeld = 512;            // entries of a row that a warp can hold as candidates of the nucleus
+// entries of a row that a warp can hold as candidates of the nucleus: what shared memory leaves is L1, where the registers' overflow lies (256 rows of 257216 beside a draft, us with
+// 256, 384, 512: 279 -- some rows need more --, 253, 261; 624 of 32000 104, 106, 109)
+constexpr int kHeld = 384;
 constexpr int kDead = -2147483647 - 1;
 constexpr double kLog2e = 1.4426950408889634, kLn2 = 0.6931471805599453;
 
