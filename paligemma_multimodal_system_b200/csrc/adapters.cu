@@ -422,8 +422,8 @@ __global__ void __launch_bounds__(kThreads, 2) adapter_rows_kernel(const PgAdapt
 
 // Tiles of 128 bf16 rows, both products on the tensor cores with their sums in tensor memory.
 //   v = x A^T        x and A come in stages of 64 k's by asynchronous copies, 128-byte rows whose 16-byte pieces are exchanged by the row's last bits; N = ranks of all parts, up to 256
-//   shares of K      added over the cluster by way of L2 (through distributed shared memory a CTA read 6 bytes a clock: 18,000 clocks for 192 columns of v, 11,000 this way, half of them until all shares are written), as bf16 terms
-//                    into shared memory (operand layout, 64 ranks a block of 16 KB)
+//   shares of K      added over the cluster by way of L2 (through distributed shared memory a CTA read 6 bytes a clock: 18,000 clocks for 192 columns of v, 11,000 this way, half of
+//                    them until all shares are written), as bf16 terms into shared memory (operand layout, 64 ranks a block of 16 KB)
 //   B v              blocks of 128 columns: every term times the same rows of B, a block ahead of the one whose sums leave; y is asked for a block ahead as well; sums leave through
 //                    shared memory so that lanes read and write neighbouring pieces of y and out
 // 256 columns of tensor memory for v, two times 128 for the blocks: one CTA an SM.
