@@ -325,7 +325,7 @@ PG_DEVINL double held_mass(Shared& sh, const Part& p, int& turn, F f) {
 }
 
 // Where u times the whole lies among n sums (n <= 32, one a lane): the first whose running sum is above `rest`, else the last with any mass; `run` becomes what lies in
-// front of it.  Whole warps; every lane has the result.
+// front of it.  -1 where none has any.  Whole warps; every lane has the result.
 PG_DEVINL int place_among(double mine, int n, double rest, double& run) {
   const int lane = threadIdx.x % 32;
   double incl = lane < n ? mine : 0.0;
@@ -341,22 +341,25 @@ PG_DEVINL int place_among(double mine, int n, double rest, double& run) {
 }
 
 // The token at u times the whole, whose sums are in sh.warp and sh.all (`turn` behind them): the first place whose running sum is above that.  Known to the CTA that holds it,
-// `owner`, alone.  (Where rounding leaves no border behind u: the last place with any mass.)  find(warp, rest, run) gives the place in the share, within that warp's part.
+// `owner`, alone.  (Where rounding leaves no border behind u: the last place with any mass.)  find(warp, rest, run) gives the place from the share's first entry on, within that warp's
+// part where that has any mass.  Where no sum is above zero the token is -1.
 template <typename F>
 PG_DEVINL int share_draw(Shared& sh, const Part& p, int turn, double total, float u, int& owner, F find) {
   const int lane = threadIdx.x % 32;
   double rest = static_cast<double>(u) * total, run = 0.0;
-  owner = place_among(lane < p.ranks ? sh.all[turn ^ 1][lane] : 0.0, p.ranks, rest, run);
+  owner = max(place_among(lane < p.ranks ? sh.all[turn ^ 1][lane] : 0.0, p.ranks, rest, run), 0);
   if (owner != p.rank) return -1;
   const int mine = place_among(lane < kWarps ? sh.warp[lane] : 0.0, kWarps, rest, run);
+  if (mine < 0) return -1;  // (the same in the whole CTA)
   __syncthreads();  // (the warps' sums have been read)
   const int place = find(mine, rest, run);
   if (static_cast<int>(threadIdx.x) / 32 == mine && lane == 0) sh.pick = p.lo + place;
   __syncthreads();
   return sh.pick;
 }
-template <typename F>
-PG_DEVINL int row_draw(Shared& sh, const Part& p, const Source& s, int turn, double total, float u, int& owner, F f) {
+// (next: see next_with_mass.)
+template <typename F, typename N>
+PG_DEVINL int row_draw(Shared& sh, const Part& p, const Source& s, int turn, double total, float u, int& owner, F f, N next) {
   return share_draw(sh, p, turn, total, u, owner, [&](int mine, double rest, double run) {
     // all warps sum pieces of that warp's part, which then looks for the piece, the lane and the entry
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, begin = mine * p.seg, end = min(begin + p.seg, p.n);
@@ -374,6 +377,7 @@ PG_DEVINL int row_draw(Shared& sh, const Part& p, const Source& s, int turn, dou
     int place = -1, last = 0;
     if (warp == mine) {
       const int at = place_among(lane < kWarps ? sh.warp[lane] : 0.0, kWarps, rest, run);
+      if (at < 0) return next(p.lo + end) - p.lo;
       const int begin2 = min(begin + at * piece, end), end2 = min(begin2 + piece, end);
       for (int i = begin2; i < end2 && place < 0; i += kRun) {
         double w[4];
@@ -694,6 +698,27 @@ PG_DEVINL int distribution(Shared& sh, const Part p, const Source s, const int w
   return turn;
 }
 
+// A part's sum may come from entries that weigh nothing in double: masked ones count as 2^-100 in fp32, and what the draft leaves is rounded otherwise there.  Then the token is this: the
+// first from `from` on, around the row's end, with any mass in p or, beside a draft's row, in max(pf wp - qf wq, 0).  -1: there is none.  A warp; out of line, since it is hardly ever needed.
+__device__ __noinline__ int next_with_mass(const Shared& sh, const float* logits, const float* draft, const double pf, const double qf, const int V, const int from) {
+  const int lane = threadIdx.x % 32;
+  const Source target(logits, 0), other(draft != nullptr ? draft : logits, 0);
+  auto mass = [&](float y, float z) {
+    const double w = weight(sh.table, sh.row[1].s, y);
+    return draft == nullptr ? w : __dsub_rn(__dmul_rn(pf, w), __dmul_rn(qf, weight(sh.table, sh.row[0].s, z)));
+  };
+#pragma unroll 1
+  for (int round = 0; round < 2; ++round)
+#pragma unroll 1
+    for (int i = round == 0 ? from : 0, to = round == 0 ? V : from; i < to; i += kRun) {
+      const float4 y = target.four(i + 4 * lane, to), z = other.four(i + 4 * lane, to);
+      const int is = (mass(y.x, z.x) > 0.0 ? 1 : 0) | (mass(y.y, z.y) > 0.0 ? 2 : 0) | (mass(y.z, z.z) > 0.0 ? 4 : 0) | (mass(y.w, z.w) > 0.0 ? 8 : 0);
+      const uint32_t some = __ballot_sync(0xffffffffu, is != 0);
+      if (some) return __shfl_sync(0xffffffffu, i + 4 * lane + __ffs(is) - 1, __ffs(some) - 1);
+    }
+  return -1;
+}
+
 PG_DEVINL float unit_number(float u) { return fminf(fmaxf(u, 0.0f), 1.0f - 0x1p-24f); }  // (a NaN is 0)
 
 struct Family {  // parents and tokens of an entry; those of the 32 rows behind v lie in the lanes
@@ -855,15 +880,16 @@ __global__ void __launch_bounds__(kThreads, kPerSm) verify_kernel(const PgVerify
         to = child;
       } else {
         int token;
+        auto behind = [&](int from) { return next_with_mass(sh, logits, c > 0.0 && left > 0.0 ? draft : nullptr, pf, qf, a.V, from); };
         if (c > 0.0 && left > 0.0) {
-          token = t.held ? held_draw(sh, p, turn, left, u, finisher, rest1) : row_draw(sh, p, target, turn, left, u, finisher, rest4);
+          token = t.held ? held_draw(sh, p, turn, left, u, finisher, rest1) : row_draw(sh, p, target, turn, left, u, finisher, rest4, behind);
         } else {
           auto one = [&](const Candidate& k) { return weight(sh.table, ts, k.x); };
           auto four = [&](int, float4 y, double (&w)[4]) {
             w[0] = weight(sh.table, ts, y.x), w[1] = weight(sh.table, ts, y.y), w[2] = weight(sh.table, ts, y.z), w[3] = weight(sh.table, ts, y.w);
           };
           if (c > 0.0) mass = t.held ? held_mass(sh, p, turn, one) : row_mass(sh, p, target, turn, [&](int, float4 y) { return weights_sum(sh.table, ts, small_t, y); });
-          token = t.held ? held_draw(sh, p, turn, mass, u, finisher, one) : row_draw(sh, p, target, turn, mass, u, finisher, four);
+          token = t.held ? held_draw(sh, p, turn, mass, u, finisher, one) : row_draw(sh, p, target, turn, mass, u, finisher, four, behind);
         }
         const int next = a.draft == nullptr && rank == finisher ? fam.with(token) : n;
         to = next < n ? next : -2 - token;
