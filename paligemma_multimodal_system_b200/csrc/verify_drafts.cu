@@ -121,13 +121,14 @@ PG_DEVINL Scale scale_of(float m, double a, double temperature) {
   s.a = a;
   s.shift = -static_cast<double>(m) * s.a;
   s.cut = nextafterf(__double2float_rd(static_cast<double>(m) - 1000.0 * kLn2 * temperature), INFINITY);
-  if (!(fabs(s.shift) < 0x1p40)) s.a = s.shift = 0.0, s.cut = m;  // the float in front of m weighs less than 2^-1000 here: what equals m shares the mass
+  const bool equals = !(fabs(s.shift) < 0x1p40);  // the float in front of m weighs less than 2^-1000 here: what equals m shares the mass
+  if (equals) s.a = s.shift = 0.0, s.cut = m;
   s.a0 = static_cast<float>(s.a);
   s.a1 = static_cast<float>(s.a - s.a0);
   s.s0 = static_cast<float>(rint(s.shift * 256.0) / 256.0);
   s.s1 = static_cast<float>(s.shift - s.s0);
   s.low = static_cast<float>((-100.0 - s.shift) * kLn2 * temperature);
-  s.fine = fabs(s.shift) < 0x1p15 ? static_cast<float>(static_cast<double>(m) - 16.0 * kLn2 * temperature) : -INFINITY;
+  s.fine = fabs(s.shift) < 0x1p15 && !equals ? static_cast<float>(static_cast<double>(m) - 16.0 * kLn2 * temperature) : -INFINITY;
   return s;
 }
 PG_DEVINL double weight(const double* table, const Scale& s, float x) {

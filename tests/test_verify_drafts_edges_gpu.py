@@ -1,4 +1,5 @@
-"""Verified drafts at the ends of their ranges, against 64 bits: random numbers of 0, entries that are masked in front of the first one with any mass."""
+"""Verified drafts at the ends of their ranges, against 64 bits: temperatures that leave nothing but the largest entries, random numbers of 0, entries that are masked in front of the first one
+with any mass."""
 import pytest
 import torch
 
@@ -6,6 +7,21 @@ from paligemma_multimodal_system_b200 import seq_ops
 from test_verify_drafts_gpu import batch, check, make
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("V,most", [(70001, 69000), (70001, 31), (5000, 4321)])
+@pytest.mark.parametrize("temperature", [1e-12, 1e-20, 1e-29])
+@pytest.mark.parametrize("top_p", [1.0, 0.9])
+def test_temperatures_that_leave_the_largest_entries(V, most, temperature, top_p):
+    """The largest entry, at any share of a row, has all of the mass: guesses of it stay, a draft's other token does not."""
+    ns = [3, 2, 3]
+    logits, draft, parents, tokens, u = make(ns, V, 1, 5, agree=0.0)
+    logits[:, most], draft[:, (most + V // 2) % V] = 40.0, 40.0
+    logits[7, most] = logits[7, most // 2] = 41.0  # two largest ones share it
+    tokens[1:3], tokens[4], tokens[6:8] = [most, most], (most + V // 2) % V, [(most + V // 2) % V, most]
+    for d in (None, draft, logits.clone()):
+        got = seq_ops.verify_drafts(logits.cuda(), batch(ns, parents, tokens), u.cuda(), None if d is None else d.cuda(), temperature, top_p)
+        check(got, ns, logits, parents, tokens, u, d, temperature, top_p)
 
 
 @pytest.mark.parametrize("V,masked", [(3001, 1200), (70001, 30000), (257216, 257000), (257216, 129)])
