@@ -48,7 +48,8 @@ struct Candidate {
 struct Scale {
   double a, shift;
   float cut;
-  // for fp32: a and shift in two parts, shift's first a multiple of 2^-8; runs with an entry of `fine` or more are weighed in double
+  // for fp32: a and shift in two parts, shift's first a multiple of 2^-8; runs with an entry of `fine` or more are weighed in double (all where it is -inf: what equals m has the mass, or
+  // `low` is past fp32's end)
   float a0, a1, s0, s1, fine, low;
 };
 struct Row {  // a row's distribution: weights / mass
@@ -128,7 +129,7 @@ PG_DEVINL Scale scale_of(float m, double a, double temperature) {
   s.s0 = static_cast<float>(rint(s.shift * 256.0) / 256.0);
   s.s1 = static_cast<float>(s.shift - s.s0);
   s.low = static_cast<float>((-100.0 - s.shift) * kLn2 * temperature);
-  s.fine = fabs(s.shift) < 0x1p15 && !equals ? static_cast<float>(static_cast<double>(m) - 16.0 * kLn2 * temperature) : -INFINITY;
+  s.fine = fabs(s.shift) < 0x1p15 && !equals && s.low > -INFINITY ? static_cast<float>(static_cast<double>(m) - 16.0 * kLn2 * temperature) : -INFINITY;
   return s;
 }
 PG_DEVINL double weight(const double* table, const Scale& s, float x) {

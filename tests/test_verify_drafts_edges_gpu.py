@@ -1,5 +1,5 @@
-"""Verified drafts at the ends of their ranges, against 64 bits: temperatures that leave nothing but the largest entries, random numbers of 0, entries that are masked in front of the first one
-with any mass."""
+"""Verified drafts at the ends of their ranges, against 64 bits: temperatures that leave nothing but the largest entries or make all of them alike, random numbers of 0, entries that are masked
+in front of the first one with any mass."""
 import pytest
 import torch
 
@@ -20,6 +20,19 @@ def test_temperatures_that_leave_the_largest_entries(V, most, temperature, top_p
     logits[7, most] = logits[7, most // 2] = 41.0  # two largest ones share it
     tokens[1:3], tokens[4], tokens[6:8] = [most, most], (most + V // 2) % V, [(most + V // 2) % V, most]
     for d in (None, draft, logits.clone()):
+        got = seq_ops.verify_drafts(logits.cuda(), batch(ns, parents, tokens), u.cuda(), None if d is None else d.cuda(), temperature, top_p)
+        check(got, ns, logits, parents, tokens, u, d, temperature, top_p)
+
+
+@pytest.mark.parametrize("V", [5001, 70001])
+@pytest.mark.parametrize("temperature", [4e36, 5e36, 1e37, 3e37, 4e37])
+@pytest.mark.parametrize("top_p", [1.0, 0.5])
+def test_temperatures_that_make_all_alike(V, temperature, top_p):
+    """Logits over a temperature near the end of fp32, masked entries among them."""
+    ns = [2, 3, 1]
+    logits, draft, parents, tokens, u = make(ns, V, 2, 5, spread=1e36, temperature=temperature, top_p=top_p)
+    logits[:, V // 3:V // 2], draft[:, V // 2:V // 2 + 40] = float("-inf"), float("-inf")
+    for d in (None, draft):
         got = seq_ops.verify_drafts(logits.cuda(), batch(ns, parents, tokens), u.cuda(), None if d is None else d.cuda(), temperature, top_p)
         check(got, ns, logits, parents, tokens, u, d, temperature, top_p)
 
