@@ -238,9 +238,9 @@ class SequenceEngine:
     def fork(self, rid, new: Sequence[object], length: Optional[int] = None):
         """New requests, admitted under the names `new`, that go on where the first `length` stored tokens (None: all) of `rid` end, with its adapter.  Full pages are
         shared; what each owns is a copy of the last, partly filled page and of the states.  Models with states fork behind the last token only."""
-        self.store.fork(rid, new, length)
+        made = self.store.fork(rid, new, length)
         if rid in self._adapter_of:
-            self._adapter_of.update((n, self._adapter_of[rid]) for n in new)
+            self._adapter_of.update((r.rid, self._adapter_of[rid]) for r in made)
 
     def remove_adapter(self, name: str):
         users = [rid for rid, n in self._adapter_of.items() if n == name]

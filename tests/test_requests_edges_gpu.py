@@ -1,0 +1,32 @@
+"""Requests of the ragged-step engine beside one another: names, slots, adapters and rows of a step that other requests have or had."""
+import pytest
+import torch
+
+from oracle import mapedra_oracle as O
+from test_engine_operators_gpu import ATTENTION, TOL, engine, rel_err
+from test_mapedra_gpu import run_cut, toks
+from test_requests_of_their_own_gpu import adapter, build, merged, run_cut_live, shapes
+
+pytestmark = pytest.mark.gpu
+
+
+def adapted(slots=4):
+    """(engine with one adapter loaded, engine of the model that it makes, engine of the plain one)"""
+    from paligemma_multimodal_system_b200.adapters import AdapterSet
+    from paligemma_multimodal_system_b200.engine import SequenceEngine
+    weights, g = O.random_weights(ATTENTION, seed=3), torch.Generator().manual_seed(4)
+    model = build(ATTENTION, weights, torch.float32)
+    sets = AdapterSet(model, 2, 8)
+    own = adapter(sets, shapes(sets), g, 8, sorted(shapes(sets)))
+    sets.load("one", own)
+    return SequenceEngine(model, 2048, slots, adapters=sets), SequenceEngine(build(ATTENTION, merged(weights, own, 1.0), torch.float32), 2048, slots), SequenceEngine(model, 2048, slots)
+
+
+def test_forks_named_by_an_iterator_keep_the_adapter():
+    eng, ref, _ = adapted()
+    prompt, later = toks(70, 80, 1), toks(5, 80, 2)
+    eng.step([("a", prompt, [])], adapters={"a": "one"})
+    eng.fork("a", (n for n in ("b", "c")))
+    want = run_cut(ref, "x", prompt + later, [70, 4, 1])[70:]
+    for rid in "abc":
+        assert rel_err(run_cut_live(eng, rid, later, [4, 1]), want) < TOL[torch.float32], rid
