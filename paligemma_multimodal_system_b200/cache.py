@@ -77,10 +77,10 @@ class PagePool:
 
 
 class SequenceRecord:
-    __slots__ = ("rid", "slot", "pages", "length")
+    __slots__ = ("rid", "slot", "pages", "length", "adapter")
 
     def __init__(self, rid, slot):
-        self.rid, self.slot, self.pages, self.length = rid, slot, [], 0
+        self.rid, self.slot, self.pages, self.length, self.adapter = rid, slot, [], 0, None  # (adapter: its name, None for the shared weights alone)
 
 
 class SequenceStore:
@@ -175,7 +175,7 @@ class SequenceStore:
         mine = self.pool.take(len(new)) if rest else []
         made = [self.admit(n) for n in new]
         for i, r in enumerate(made):
-            r.pages, r.length = rec.pages[:full] + mine[i:i + 1], length
+            r.pages, r.length, r.adapter = rec.pages[:full] + mine[i:i + 1], length, rec.adapter
             self.pool.share(rec.pages[:full])
         pages, states = self.operands()
         try:

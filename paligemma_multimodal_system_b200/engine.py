@@ -71,7 +71,6 @@ class SequenceEngine:
         _lib.require_device()
         self.model = model
         self.adapters = adapters
-        self._adapter_of: Dict[object, str] = {}
         self.store = SequenceStore(model.cache_layout(), max_tokens, num_slots, model.prec.dtype, kv_format=kv_format)
         self._drafted: Dict[object, List[int]] = {}  # request -> parents of the drafted tokens whose rows stand behind its own
         self._step_no = torch.zeros(1, device="cuda", dtype=torch.int32)
@@ -90,7 +89,7 @@ class SequenceEngine:
         for rid, name in (adapters or {}).items():
             if name is not None and (self.adapters is None or name not in self.adapters.names):
                 raise KeyError(f"request {rid!r}: no adapter {name!r} is loaded")
-            if rid in store.live and self._adapter_of.get(rid) != name:
+            if rid in store.live and store.live[rid].adapter != name:
                 raise ValueError(f"request {rid!r} is live: it keeps the adapter that it was admitted with")
         seen = set()
         for rid, toks, w in entries:
@@ -99,9 +98,7 @@ class SequenceEngine:
             seen.add(rid)
             toks = self._checked(rid, toks)
             if rid not in store.live:
-                store.admit(rid)
-                if adapters and adapters.get(rid) is not None:
-                    self._adapter_of[rid] = adapters[rid]
+                store.admit(rid).adapter = (adapters or {}).get(rid)
             rec = store.reserve(rid, len(toks))
             batch.append(dict(tokens=toks, ctx=rec.length, slot=rec.slot, pages=rec.pages))
             for k in w:
@@ -151,7 +148,7 @@ class SequenceEngine:
 
     def _slots_of(self, rids):
         """Adapters of requests by their places, None where no request has one."""
-        names = [self._adapter_of.get(rid) for rid in rids]
+        names = [self.store.live[rid].adapter for rid in rids]
         return self.adapters.slots_of(names) if any(n is not None for n in names) else None
 
     def _adapted(self, b, rids, ns):
@@ -238,12 +235,10 @@ class SequenceEngine:
     def fork(self, rid, new: Sequence[object], length: Optional[int] = None):
         """New requests, admitted under the names `new`, that go on where the first `length` stored tokens (None: all) of `rid` end, with its adapter.  Full pages are
         shared; what each owns is a copy of the last, partly filled page and of the states.  Models with states fork behind the last token only."""
-        made = self.store.fork(rid, new, length)
-        if rid in self._adapter_of:
-            self._adapter_of.update((r.rid, self._adapter_of[rid]) for r in made)
+        self.store.fork(rid, new, length)
 
     def remove_adapter(self, name: str):
-        users = [rid for rid, n in self._adapter_of.items() if n == name]
+        users = [rid for rid, rec in self.store.live.items() if rec.adapter == name]
         if users:
             raise ValueError(f"adapter {name!r} is in use by {users[:4]}")
         self.adapters.remove(name)
@@ -293,7 +288,6 @@ class SequenceEngine:
 
     def release(self, rid):
         self._drafted.pop(rid, None)
-        self._adapter_of.pop(rid, None)
         self.store.release(rid)
 
     # -- generation ------------------------------------------------------------------------------------------------

@@ -30,3 +30,13 @@ def test_forks_named_by_an_iterator_keep_the_adapter():
     want = run_cut(ref, "x", prompt + later, [70, 4, 1])[70:]
     for rid in "abc":
         assert rel_err(run_cut_live(eng, rid, later, [4, 1]), want) < TOL[torch.float32], rid
+
+
+def test_a_name_that_is_taken_again_has_no_adapter_of_before():
+    eng, _, plain = adapted()
+    prompt = toks(30, 80, 1)
+    eng.step([("a", toks(9, 80, 3), [])], adapters={"a": "one"})
+    eng.store.release("a")
+    eng.remove_adapter("one")  # nobody has it
+    got = eng.step([("a", prompt, range(30))])
+    assert rel_err(got, run_cut(plain, "a", prompt, [30])) < TOL[torch.float32]
