@@ -322,6 +322,11 @@ class SequenceEngine:
         rng = torch.Generator(device="cuda").manual_seed(int(seed)) if draft is not None and do_sample else None
         if logprobs is not None and not 0 <= logprobs <= min(32, self.model.vocab_size):
             raise ValueError(f"logprobs is 0 .. 32 and at most the vocabulary: got {logprobs}")
+        if len(prompts) == 0:
+            return [] if logprobs is None else ([], [])
+        for left, what in ((self.store.free_slots, "sequence slots"), (self.store.pool.free, "cache pages")):
+            if not left:
+                raise MemoryError(f"live requests hold all {what}: release some before others are generated")
         records = {}
         # (what live requests hold stays theirs)
         sched = StepScheduler(len(self.store.free_slots), len(self.store.pool.free), self.store.page, step_tokens, eos_token_id)

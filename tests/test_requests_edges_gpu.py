@@ -40,3 +40,18 @@ def test_a_name_that_is_taken_again_has_no_adapter_of_before():
     eng.remove_adapter("one")  # nobody has it
     got = eng.step([("a", prompt, range(30))])
     assert rel_err(got, run_cut(plain, "a", prompt, [30])) < TOL[torch.float32]
+
+
+def test_generation_where_nothing_is_free():
+    eng = engine(ATTENTION, torch.float32, slots=2)
+    eng.step([("a", toks(9, 80, 1), []), ("b", toks(9, 80, 2), [])])
+    assert eng.generate([], 4) == [] and eng.generate([], 4, logprobs=1) == ([], [])
+    with pytest.raises(MemoryError, match="slots"):
+        eng.generate([[1, 2]], 4)
+    eng.release("a")
+    assert len(eng.generate([[1, 2]], 4)[0]) == 4
+    eng = engine(ATTENTION, torch.float32, max_tokens=128)
+    eng.step([("a", toks(100, 80, 1), [])])
+    with pytest.raises(MemoryError, match="pages"):
+        eng.generate([[1, 2]], 4)
+    assert list(eng.store.live) == ["a"]
