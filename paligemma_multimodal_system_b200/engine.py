@@ -17,6 +17,7 @@ that has some -- whole prompts, portions of prompts and single decoded tokens si
 The model supplies `cache_layout()`, `step(batch, store, want_rows)`, `prec` and `vocab_size` (modeling_mapedra.py).
 """
 import contextlib
+import itertools
 from typing import Callable, Dict, List, Optional, Sequence, Tuple
 
 import torch
@@ -318,7 +319,6 @@ class SequenceEngine:
             raise ValueError("drafted trees need a model whose layers keep nothing but keys and values: a state has no branches")
         if adapters is not None and len(adapters) != len(prompts):
             raise ValueError("one adapter (or None) for every prompt")
-        named = {("gen", i): n for i, n in enumerate(adapters or ())}
         rng = torch.Generator(device="cuda").manual_seed(int(seed)) if draft is not None and do_sample else None
         if logprobs is not None and not 0 <= logprobs <= min(32, self.model.vocab_size):
             raise ValueError(f"logprobs is 0 .. 32 and at most the vocabulary: got {logprobs}")
@@ -327,12 +327,16 @@ class SequenceEngine:
         for left, what in ((self.store.free_slots, "sequence slots"), (self.store.pool.free, "cache pages")):
             if not left:
                 raise MemoryError(f"live requests hold all {what}: release some before others are generated")
+        # (names that no live request has: not the caller's, nor those of a generation whose `draft` asks for another)
+        free = (("gen", i) for i in itertools.count())
+        names = list(itertools.islice((rid for rid in free if rid not in self.store.live), len(prompts)))
+        named = dict(zip(names, adapters or ()))
         records = {}
         # (what live requests hold stays theirs)
         sched = StepScheduler(len(self.store.free_slots), len(self.store.pool.free), self.store.page, step_tokens, eos_token_id)
-        for i, pr in enumerate(prompts):
-            sched.submit(TokenRequest(("gen", i), [int(t) for t in pr], int(max_new_tokens)))
-        with self._released_on_errors([("gen", i) for i in range(len(prompts))]):
+        for rid, pr in zip(names, prompts):
+            sched.submit(TokenRequest(rid, [int(t) for t in pr], int(max_new_tokens)))
+        with self._released_on_errors(names):
             while not sched.idle():
                 plan = sched.plan()
                 if not plan:
@@ -356,8 +360,8 @@ class SequenceEngine:
                         records.setdefault(req.rid, []).append(next(told))
                     if sched.advance(req, len(toks), next(it) if sample else None):
                         self.release(req.rid)
-        tokens = [sched.finished[("gen", i)] for i in range(len(prompts))]
-        return tokens if logprobs is None else (tokens, [records.get(("gen", i), []) for i in range(len(prompts))])
+        tokens = [sched.finished[rid] for rid in names]
+        return tokens if logprobs is None else (tokens, [records.get(rid, []) for rid in names])
 
     @contextlib.contextmanager
     def _released_on_errors(self, rids):

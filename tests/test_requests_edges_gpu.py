@@ -42,6 +42,29 @@ def test_a_name_that_is_taken_again_has_no_adapter_of_before():
     assert rel_err(got, run_cut(plain, "a", prompt, [30])) < TOL[torch.float32]
 
 
+def test_generation_leaves_requests_of_any_name_alone():
+    eng, ref = engine(ATTENTION, torch.float32), engine(ATTENTION, torch.float32)
+    prompt, mine, later = toks(20, 80, 1), toks(33, 80, 2), toks(4, 80, 3)
+    want = ref.generate([prompt, prompt[:7]], 6)
+    eng.step([(("gen", 0), mine, [])])
+    assert eng.generate([prompt, prompt[:7]], 6) == want
+    with pytest.raises(OSError):
+        eng.generate([prompt], 6, draft=_fails)
+    assert list(eng.store.live) == [("gen", 0)]
+    assert rel_err(run_cut_live(eng, ("gen", 0), later, [3, 1]), run_cut(ref, "x", mine + later, [33, 3, 1])[33:]) < TOL[torch.float32]
+    inner = []
+
+    def asks(history):  # a draft that is made by the same engine
+        inner.append(eng.generate([history], 2)[0])
+        return inner[-1], [-1, 0]
+
+    assert eng.generate([prompt, prompt[:7]], 6, draft=asks) == want and inner
+
+
+def _fails(history):
+    raise OSError("no guess")
+
+
 def test_generation_where_nothing_is_free():
     eng = engine(ATTENTION, torch.float32, slots=2)
     eng.step([("a", toks(9, 80, 1), []), ("b", toks(9, 80, 2), [])])
