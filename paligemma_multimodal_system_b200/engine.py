@@ -313,8 +313,9 @@ class SequenceEngine:
         logprobs = k (0 .. 32): (tokens, records), records per prompt and token a dict with its logprob, rank and entropy and the k most likely (id, logprob)
         pairs in `top`, under softmax(logits / temperature) where tokens are sampled and softmax(logits) else.
         draft: guesses how a request goes on -- its tokens so far -> (drafted tokens, parents), parents[i] the drafted token that token i follows or -1 the newest one
-        (LookupDrafter) -- and steps of decoded tokens run the guesses along and keep those that the model says as well: the tokens of a greedy run are the same, those of a
-        sampled one have the same distribution.  adapters: one name or None for every prompt."""
+        (LookupDrafter) -- and steps of decoded tokens run the guesses along, `step_tokens` rows a step at most, and keep those that the model says as well: the tokens of a greedy
+        run are the same where its logits are (a drafted step's kernels add in another order: near ties may fall otherwise, in bf16 above all), those of a sampled one have the same
+        distribution.  adapters: one name or None for every prompt."""
         if draft is not None and any(spec is not None and spec[0] != "kv" for spec in self.store.layout):
             raise ValueError("drafted trees need a model whose layers keep nothing but keys and values: a state has no branches")
         if adapters is not None and len(adapters) != len(prompts):
@@ -342,7 +343,7 @@ class SequenceEngine:
                 if not plan:
                     raise RuntimeError("scheduler made no progress")
                 if draft is not None and all(req.fed == len(req.prompt) for req, _, _ in plan):
-                    guessed = self._guesses(plan, draft)
+                    guessed = self._guesses(plan, draft, step_tokens)
                     if any(len(toks) > 1 for _, toks, _ in guessed):
                         self._drafted_turn(plan, guessed, sched, do_sample, temperature, top_p, rng, logprobs, records)
                         continue
@@ -374,13 +375,15 @@ class SequenceEngine:
                     self.release(rid)
             raise
 
-    def _guesses(self, plan, draft):
-        """Entries of a drafted step: every decoding request's newest token and what is guessed behind it."""
-        entries = []
-        for req, toks, _ in plan:
+    def _guesses(self, plan, draft, step_tokens):
+        """Entries of a drafted step: every decoding request's newest token and what is guessed behind it, `step_tokens` rows at most (each has its logits)."""
+        entries, left = [], step_tokens - len(plan)
+        for i, (req, toks, _) in enumerate(plan):
             tokens, parents = draft(req.prompt + req.tokens)
-            room = req.max_new_tokens - len(req.tokens) - 1  # (rows that the request's pages have room for beside the newest token's)
+            # rows that the request's pages have room for beside the newest token's, and its share of the step's
+            room = min(req.max_new_tokens - len(req.tokens) - 1, left // (len(plan) - i))
             tokens, parents = list(tokens)[:room], list(parents)[:room]
+            left -= len(tokens)
             entries.append((req.rid, toks + tokens, [-1] + [int(p) + 1 for p in parents]))
         return entries
 

@@ -78,3 +78,18 @@ def test_generation_where_nothing_is_free():
     with pytest.raises(MemoryError, match="pages"):
         eng.generate([[1, 2]], 4)
     assert list(eng.store.live) == ["a"]
+
+
+@pytest.mark.parametrize("step_tokens,most", [(512, 4 * 9), (16, 16), (7, 7), (4, 4)])
+def test_steps_of_drafts_have_no_more_rows_than_other_steps(step_tokens, most, monkeypatch):
+    eng = engine(ATTENTION, torch.float32)
+    prompts = [toks(n, 80, n) for n in (3, 4, 2, 1)]
+    want, rows, run = eng.generate(prompts, 12), [], type(eng)._draft_step
+
+    def counted(self, entries):
+        rows.append(sum(len(t) for _, t, _ in entries))
+        return run(self, entries)
+
+    monkeypatch.setattr(type(eng), "_draft_step", counted)
+    assert eng.generate(prompts, 12, step_tokens=step_tokens, draft=lambda h: ([h[-1]] * 8, range(-1, 7))) == want
+    assert (not rows or max(rows) <= most) and (step_tokens < 5 or max(rows) > 4)
