@@ -4,7 +4,9 @@ There is no CPU fallback: `lib()` raises if the shared library is missing, and e
 non-zero return code.  Tensors are passed as raw device pointers (`tensor.data_ptr()`); torch only owns the memory and
 the stream.
 """
+import contextlib
 import ctypes as C
+import gc
 import os
 import struct
 
@@ -275,6 +277,19 @@ def stream():
     if not torch.cuda.is_initialized():
         torch.cuda.init()
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+@contextlib.contextmanager
+def captured(graph, stream):
+    """torch.cuda.graph while Python's collector rests: a graph that it found to be garbage would be destroyed inside the capture, which ends that with an error."""
+    on = gc.isenabled()
+    gc.disable()
+    try:
+        with torch.cuda.graph(graph, stream=stream):
+            yield
+    finally:
+        if on:
+            gc.enable()
 
 
 def ptr(t):

@@ -273,7 +273,7 @@ class SequenceEngine:
             side.wait_stream(torch.cuda.current_stream())
             with torch.cuda.stream(side):
                 g = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(g, stream=side), _weights_follow():
+                with _lib.captured(g, side), _weights_follow():
                     slot["logits"] = self.model.step(st.batch, self.store, st.rows)
             torch.cuda.current_stream().wait_stream(side)
             slot["graph"] = g

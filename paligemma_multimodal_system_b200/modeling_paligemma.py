@@ -300,7 +300,7 @@ class PaliGemmaForConditionalGeneration(nn.Module):
                 side.wait_stream(torch.cuda.current_stream())
                 with torch.cuda.stream(side):
                     g = torch.cuda.CUDAGraph()
-                    with torch.cuda.graph(g, stream=side):
+                    with _lib.captured(g, side):
                         pf["logits"], pf["err"] = run(pf["ids"], pf["mask"], pf["px"])
                 torch.cuda.current_stream().wait_stream(side)
                 pf["graph"] = g
@@ -406,7 +406,7 @@ class PaliGemmaForConditionalGeneration(nn.Module):
             side.wait_stream(torch.cuda.current_stream())
             with torch.cuda.stream(side):
                 g = torch.cuda.CUDAGraph()
-                with torch.cuda.graph(g, stream=side):
+                with _lib.captured(g, side):
                     for _ in range(n_steps):
                         decode_step()
             torch.cuda.current_stream().wait_stream(side)

@@ -380,7 +380,7 @@ class ContinuousBatcher:
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
             g = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(g, stream=side):
+            with _lib.captured(g, side):
                 for _ in range(self.GK):
                     self._step()
         torch.cuda.current_stream().wait_stream(side)
