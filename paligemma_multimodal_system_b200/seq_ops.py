@@ -763,8 +763,9 @@ ADAPTER_MOST_RANK, ADAPTER_MOST_PARTS = 128, 8
 class AdapterBank:
     """The low-rank adapters that stand beside one shared projection [columns, K]: adapter s adds scale[s] * b[s] (a[s] x).  The projection's columns are `parts` runs
     (a joint query, key and value projection has three); each run has `rank` rows of a[s] for itself: a [slots, len(parts) * rank, K], b [slots, sum(parts), rank], both
-    bf16 or fp32 on the device, scale fp32 [slots].  They are laid out anew, once; `put` replaces one."""
+    bf16 or fp32 on the device, scale fp32 [slots].  They are laid out anew, once; `put` replaces one.  (Parameters are taken as numbers: nothing here has gradients.)"""
 
+    @torch.no_grad()
     def __init__(self, a: torch.Tensor, b: torch.Tensor, scale: torch.Tensor, parts: Sequence[int]):
         parts = [int(n) for n in parts]
         if not 1 <= len(parts) <= ADAPTER_MOST_PARTS or min(parts) < 1:
@@ -811,6 +812,7 @@ class AdapterBank:
         return cls(torch.zeros(slots, len(parts) * rank, K, device=device, dtype=dtype), torch.zeros(slots, sum(parts), rank, device=device, dtype=dtype),
                    torch.zeros(slots, device=device), parts)
 
+    @torch.no_grad()
     def put(self, slot: int, part: int, a: torch.Tensor, b: torch.Tensor):
         """One run's matrices of one adapter: a [r, K], b [columns of the run, r], r up to the bank's rank (the rest becomes zero)."""
         r = a.shape[0]
