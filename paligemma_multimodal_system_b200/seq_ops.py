@@ -834,6 +834,14 @@ class AdapterBank:
         self.scale[slot] = 0
 
 
+def _adapter_tile_rows(rows: int, adapters: int, processors: int) -> int:
+    """Tiles of 128 rows go over the tensor memory, and their way is long: they pay once tiles of 16 are more than the processors, where adapters fill half of one on average.  A plan serves
+    every projection of a step and does not know their ranks, by which the border moves both ways (K 2048, 2560 columns, us with 16 and 128: 7 adapters of 320 rows, rank 3 x 16 16 and 22,
+    3 x 64 30 and 25; of 384 rows 24 and 22, 47 and 24; 48 of 64 rows 25 and 32, 60 and 38).  Projections that the tensor memory does not take (more runs or higher ranks than its operands have
+    room for) run a tile of 128 as eight of 16, as long as those: four runs of rank 64 over 7 x 384 rows 94."""
+    return 128 if rows > max(16 * processors, 64 * adapters - 1) else 16
+
+
 class AdapterPlan:
     """Which rows of a step go through which adapter: entries of ns[e] rows, one behind the other, with adapters[e] (-1: none).  Rows of one adapter stand together in
     tiles, whichever entries they belong to.  tiles: a fixed number of them (a plan that is `fill`ed again, for a step that is captured).  tile_rows: how many rows a tile
@@ -859,9 +867,7 @@ class AdapterPlan:
 
     def _make(self, ns, adapters, device):
         order, ids, first, count = self._order(ns, adapters)
-        # Tiles of 128 rows go over the tensor memory, and their way is long: they pay once tiles of 16 are more than the SMs, where adapters fill half of one on average.  (K 2048, 2560
-        # columns, us with 16 and 128: 7 adapters of 320 rows, rank 3 x 16 16 and 22, 3 x 64 30 and 25; of 384 rows 24 and 22, 47 and 24; 48 of 64 rows 25 and 32, 60 and 38.)
-        size = self.tile_rows or (128 if self.fixed is None and len(order) > max(16 * 148, 64 * len(ids) - 1) else 16)
+        size = self.tile_rows or (16 if self.fixed is not None else _adapter_tile_rows(len(order), len(ids), _lib.num_sms() if torch.device(device).type == "cuda" else 148))
         tiles = [(a, f + o, min(size, c - o)) for a, f, c in zip(ids.tolist(), first.tolist(), count.tolist()) for o in range(0, c, size)]
         n = len(tiles) if self.fixed is None else self.fixed
         if len(tiles) > n:
@@ -880,7 +886,7 @@ class AdapterPlan:
         h[:T] = order
         h[T:] = 0
         h[T:T + 3 * len(tiles)] = np.asarray(tiles).reshape(-1)
-        self.most, self.used = int(ids[-1]), sum(int(a) >= 0 for a in ids)
+        self.most = int(ids[-1])
         self.dev.copy_(self.host, non_blocking=True)
         if self.fixed is not None and self.dev.is_cuda:
             self._copied = torch.cuda.Event()
