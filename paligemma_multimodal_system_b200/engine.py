@@ -88,8 +88,7 @@ class SequenceEngine:
         store = self.store
         batch, want, row = [], [], 0
         for rid, name in (adapters or {}).items():
-            if name is not None and (self.adapters is None or name not in self.adapters.names):
-                raise KeyError(f"request {rid!r}: no adapter {name!r} is loaded")
+            self._check_adapter(name, f"request {rid!r}")
             if rid in store.live and store.live[rid].adapter != name:
                 raise ValueError(f"request {rid!r} is live: it keeps the adapter that it was admitted with")
         seen = set()
@@ -125,6 +124,10 @@ class SequenceEngine:
             if rid in store.live:
                 self.release(rid)
         return logits
+
+    def _check_adapter(self, name, whose):
+        if name is not None and (self.adapters is None or name not in self.adapters.names):
+            raise KeyError(f"{whose}: no adapter {name!r} is loaded")
 
     def _checked(self, rid, toks):
         toks = [int(t) for t in toks]
@@ -320,6 +323,8 @@ class SequenceEngine:
             raise ValueError("drafted trees need a model whose layers keep nothing but keys and values: a state has no branches")
         if adapters is not None and len(adapters) != len(prompts):
             raise ValueError("one adapter (or None) for every prompt")
+        for i, name in enumerate(adapters or ()):
+            self._check_adapter(name, f"prompt {i}")
         rng = torch.Generator(device="cuda").manual_seed(int(seed)) if draft is not None and do_sample else None
         if logprobs is not None and not 0 <= logprobs <= min(32, self.model.vocab_size):
             raise ValueError(f"logprobs is 0 .. 32 and at most the vocabulary: got {logprobs}")

@@ -93,3 +93,12 @@ def test_steps_of_drafts_have_no_more_rows_than_other_steps(step_tokens, most, m
     monkeypatch.setattr(type(eng), "_draft_step", counted)
     assert eng.generate(prompts, 12, step_tokens=step_tokens, draft=lambda h: ([h[-1]] * 8, range(-1, 7))) == want
     assert (not rows or max(rows) <= most) and (step_tokens < 5 or max(rows) > 4)
+
+
+def test_an_adapter_that_nobody_loaded_is_refused_before_anything_runs(monkeypatch):
+    eng, _, _ = adapted(slots=1)
+    monkeypatch.setattr(eng.model, "step", lambda *a, **k: pytest.fail("a step ran"))
+    with pytest.raises(KeyError, match="prompt 1"):
+        eng.generate([[1, 2], [3]], 4, adapters=["one", "two"])
+    with pytest.raises(KeyError, match="prompt 0"):
+        engine(ATTENTION, torch.float32).generate([[1, 2]], 4, adapters=["one"])
