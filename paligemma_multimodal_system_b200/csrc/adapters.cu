@@ -11,7 +11,7 @@
 // holds eight neighbouring outputs.
 //
 // What bounds it: for decoded tokens a chain of trips to memory (one row beside 2048 x 2560 columns 8 us, 64 requests of 20 adapters 10); for prompts how long a CTA takes from one block
-// of columns to the next (6516 rows of 7 adapters beside 2048 x 2560 columns, rank 3 x 64: 45 us, 27 of them in ten blocks, 7 in the share of K, 6 in the join; 35 without y and out, 93 MB
+// of columns to the next (6516 rows of 7 adapters beside 2048 x 2560 columns, rank 3 x 64: 44 us, 42 in a row of launches, 27 of them in ten blocks, 7 in the share of K, 6 in the join; 35 without y and out, 93 MB
 // in all: 2.1 TB/s).
 #include "common.cuh"
 #include "paligemma_b200.h"
@@ -813,7 +813,8 @@ Layout layout_of(const PgAdapter& a) {
   lay.v_ld += (lay.v_ld % 64 == 32) ? 0 : 32;  // eight lanes' 16-byte pieces of two rows lie in different banks
   return lay;
 }
-// Shared memory of a tile of 128 rows; no stages: it does not go over the tensor memory (few rows of an adapter, more than 256 columns of v, no room for its terms)
+// Shared memory of a tile of 128 rows; no stages: it does not go over the tensor memory (few rows of an adapter, more than 256 columns of v, no room for its terms: every run takes blocks of 64
+// ranks, so that four runs do not fit at any rank.  6432 rows of 7 adapters, K 2048, rank 64: three runs of 2560 columns 44 us, four of 4608 in tiles of 16 180)
 template <int VT>
 void plan_of(const PgAdapter& a, const Layout& lay, Plan& plan) {
   plan.R16 = (lay.R + 15) / 16 * 16;

@@ -19,7 +19,7 @@
 // counted runs, for the run that holds the border and the mass above it; the one that holds the drawn token finishes alone.
 //
 // What bounds it: few rows, that chain (5 rows 29 us, of which 5 are passes; 35 with seven meetings); many rows, how fast an SM takes them from L2 (6.7 TB/s over all while their
-// passes coincide) and the chains between: 256 rows of 257216 beside a draft 253 us, 1.2 TB/s of DRAM, 37 % of the issue slots.  Greedy walks have a kernel of their own, one pass: 104 rows
+// passes coincide) and the chains between: 256 rows of 257216 beside a draft 251 us, 1.2 TB/s of DRAM, 36 % of the issue slots.  Greedy walks have a kernel of their own, one pass: 104 rows
 // 27 us, 17 of which their bytes take (with a cluster a row as well 32, some rows left out).
 #include "common.cuh"
 #include "paligemma_b200.h"
