@@ -618,6 +618,7 @@ PG_DEVINL int distribution(Shared& sh, const Part p, const Source s, const int w
   }
   const double temperature = sh.how[which].temperature;
   if (threadIdx.x == 0) sh.top_key = top;
+  __syncthreads();  // (a warp without entries reads it at once)
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const float m = unordered(top);
   Scale sc = scale_of(m, sh.how[which].a, temperature);

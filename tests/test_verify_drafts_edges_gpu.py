@@ -50,3 +50,21 @@ def test_a_random_number_of_zero_draws_the_first_token_with_any_mass(V, masked, 
         got = seq_ops.verify_drafts(logits.cuda(), batch(ns, parents, tokens), u.cuda(), None if d is None else d.cuda(), 1.0, top_p)
         assert all(int(t) >= masked for t in got[2])
         check(got, ns, logits, parents, tokens, u, d, 1.0, top_p)
+
+
+@pytest.mark.parametrize("V", [1, 40, 129, 700, 2049])
+def test_rows_that_leave_most_of_a_cta_without_entries(V):
+    """Warps without entries are through with a row at once; what they go by next is their own, whenever the others come.  The same answer every time, on three streams at once."""
+    ns = [3, 2, 4, 1] * 40
+    logits, draft, parents, tokens, u = make(ns, V, 2, 5, temperature=0.8, top_p=0.7)
+    dev = (logits.cuda(), batch(ns, parents, tokens), u.cuda(), draft.cuda(), 0.8, 0.7)
+    first = seq_ops.verify_drafts(*dev)
+    check(first, ns, logits, parents, tokens, u, draft, 0.8, 0.7)
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(3)], []
+    for s in streams * 40:
+        with torch.cuda.stream(s):
+            outs.append(seq_ops.verify_drafts(*dev))
+    torch.cuda.synchronize()
+    for o in outs:
+        assert all(torch.equal(a, b) for a, b in zip(o, first))
