@@ -348,7 +348,7 @@ class SequenceEngine:
                 if not plan:
                     raise RuntimeError("scheduler made no progress")
                 if draft is not None and all(req.fed == len(req.prompt) for req, _, _ in plan):
-                    guessed = self._guesses(plan, draft, step_tokens)
+                    guessed = self._guesses(plan, draft, sched.step_tokens)
                     if any(len(toks) > 1 for _, toks, _ in guessed):
                         self._drafted_turn(plan, guessed, sched, do_sample, temperature, top_p, rng, logprobs, records)
                         continue
